@@ -1,0 +1,250 @@
+/*
+ * api_paged.cpp — the paged-cache operators of hearth_gpu.h: host-side checks, then one or two
+ * launches on the caller's stream. Every field that a kernel uses as a bound or an index is
+ * checked here; what lies in device memory (page ids, lengths) is checked in the kernels.
+ */
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+
+#include "hx_host.h"
+#include "hx_paged.h"
+
+using namespace hx;
+using namespace hxp;
+
+namespace {
+
+constexpr int64_t MAX_STRIDE = (int64_t)1 << 46;   /* elements: products with 31-bit indices stay within 64 bits */
+
+bool pow2(int x) { return x > 0 && (x & (x - 1)) == 0; }
+
+bool rows_ok(const hearth_gpu_rows &r, const hearth_gpu_cache &c) {
+    const bool mx = c.dtype == HEARTH_GPU_MX8;
+    const int es = mx ? 1 : 2;
+    const int64_t block = (int64_t)c.page * c.width;
+    if (!r.data || (uintptr_t)r.data % 16) return false;
+    if (r.head_stride < (c.n_heads > 1 ? block : 0) || r.page_stride < (c.n_pages > 1 ? block : 0)) return false;
+    if (r.head_stride > MAX_STRIDE || r.page_stride > MAX_STRIDE) return false;
+    if (r.head_stride * es % 16 || r.page_stride * es % 16) return false;
+    if (!mx) return true;
+    if (!r.scales || r.scale_head_stride < (c.n_heads > 1 ? block / MX_BLOCK : 0) || r.scale_head_stride > MAX_STRIDE) return false;
+    return r.scale_page_stride >= (c.n_pages > 1 ? block / MX_BLOCK : 0) && r.scale_page_stride <= MAX_STRIDE;
+}
+
+bool cache_ok(const hearth_gpu_cache *c) {
+    if (!c || (c->dtype != HEARTH_F16 && c->dtype != HEARTH_BF16 && c->dtype != HEARTH_GPU_MX8)) return false;
+    if (c->n_pages < 1 || c->n_heads < 1 || c->n_heads > 4096 || !pow2(c->page) || c->page < 16 || c->page > 4096) return false;
+    if (c->width < 32 || c->width > 1024 || c->width % 32) return false;
+    return rows_ok(c->k, *c) && (!c->v.data || rows_ok(c->v, *c));
+}
+
+bool batch_ok(const hearth_gpu_batch *b) {
+    if (!b || b->n_seqs < 0 || b->n_seqs > 65535 || b->n_tokens < 0 || b->max_q < 0 || b->max_kv < 0 || b->pages_per_seq < 0) return false;
+    if (b->n_seqs && (!b->kv_len || !b->q_start || (b->pages_per_seq && !b->pages))) return false;
+    if (b->ld_pages < b->pages_per_seq && b->n_seqs > 1) return false;
+    if (b->ld_pages < 0 || b->ld_pages > MAX_STRIDE) return false;
+    return !b->mask || (b->mask_words >= 1 && (int64_t)b->mask_words * 64 >= b->max_q);
+}
+
+int elem(int dtype) { return dtype == HEARTH_F32 ? 4 : dtype == HEARTH_F16 || dtype == HEARTH_BF16 ? 2 : 0; }
+
+bool array_ok(const hearth_gpu_array *x) {
+    if (!x || !x->data || !elem(x->dtype) || x->n_heads < 1 || x->n_heads > 65536 || x->width < 1 || x->width > 65536) return false;
+    if ((uintptr_t)x->data % elem(x->dtype)) return false;
+    return std::llabs(x->token_stride) <= MAX_STRIDE && std::llabs(x->head_stride) <= MAX_STRIDE;
+}
+
+/* pointer and strides on 16 bytes */
+bool on16(const hearth_gpu_array &x) {
+    const int64_t es = elem(x.dtype);
+    return (uintptr_t)x.data % 16 == 0 && x.token_stride * es % 16 == 0 && x.head_stride * es % 16 == 0;
+}
+
+Rows rows_of(const hearth_gpu_rows &r, int dtype) {
+    const int64_t es = dtype == HEARTH_GPU_MX8 ? 1 : 2;
+    return {(uint8_t *)r.data, r.scales, r.page_stride * es, r.head_stride * es, r.scale_page_stride, r.scale_head_stride};
+}
+
+Batch batch_of(const hearth_gpu_batch &b, const hearth_gpu_cache &c) {
+    Batch o{};
+    o.pages = b.pages; o.kv_len = b.kv_len; o.q_start = b.q_start;
+    o.mask = (const unsigned long long *)b.mask;
+    o.ld_pages = b.ld_pages; o.n_seqs = b.n_seqs; o.n_tokens = b.n_tokens;
+    o.max_q = std::min(b.max_q, b.n_tokens); o.mask_words = b.mask_words;
+    o.kv_cap = (int)std::min<int64_t>(b.max_kv, std::min<int64_t>((int64_t)b.pages_per_seq * c.page, 0x7fffff00));
+    o.n_pages = c.n_pages;
+    o.page_shift = __builtin_ctz((unsigned)c.page);
+    return o;
+}
+
+/* OK when the calling thread holds no unread HIP error and `dev` can be made current */
+int launch_on(int dev, const DeviceGuard &g) {
+    (void)dev;
+    return g.ok ? OK : E_IO;
+}
+
+int finish() { return hipGetLastError() == hipSuccess ? OK : E_IO; }   /* this call's launches only */
+
+int copy_call(bool write, const hearth_gpu_cache *c, const hearth_gpu_batch *b, const hearth_gpu_array *k,
+              const hearth_gpu_array *v, int dev, void *stream) {
+    if (!cache_ok(c) || !batch_ok(b) || dev < 0) return E_ARG;
+    const bool latent = !c->v.data;
+    if (v && !v->data) v = nullptr;
+    if (!array_ok(k) || (v && !array_ok(v)) || (!latent && !v)) return E_ARG;
+    if (v && v->dtype != k->dtype) return E_ARG;
+    CopyArgs a{};
+    a.b = batch_of(*b, *c);
+    a.n_pieces = v ? 2 : 1;
+    int col = 0;
+    bool wide = true;
+    for (int i = 0; i < a.n_pieces; i++) {
+        const hearth_gpu_array &x = i ? *v : *k;
+        if (x.n_heads != c->n_heads || x.width % 32) return E_ARG;
+        Piece &p = a.p[i];
+        const int es = elem(x.dtype);
+        p.arr = (uint8_t *)x.data; p.at = x.token_stride * es; p.ah = x.head_stride * es;
+        p.rows = rows_of(i && !latent ? c->v : c->k, c->dtype);
+        p.col = latent ? col : 0; p.width = x.width; p.row_width = c->width; p.heads = x.n_heads;
+        col += x.width;
+        if (!latent && x.width != c->width) return E_ARG;
+        a.octs += p.heads * (p.width / 8);
+        wide = wide && on16(x);
+    }
+    if (latent && (col != c->width || (v && c->n_heads != 1))) return E_ARG;
+    if (!a.b.n_seqs || !a.b.max_q) return OK;
+    if (hipPeekAtLastError() != hipSuccess) return E_IO;
+    DeviceGuard g(dev);
+    if (launch_on(dev, g) != OK) return E_IO;
+    if (write) kv_append(a, k->dtype, c->dtype, wide, (hipStream_t)stream);
+    else kv_read(a, k->dtype, c->dtype, wide, (hipStream_t)stream);
+    return finish();
+}
+
+/* arguments that both attentions share; value_width: 0 for grouped heads, C for latent rows */
+bool attend_shape_ok(const hearth_gpu_cache *c, const hearth_gpu_batch *b, int heads) {
+    if (!cache_ok(c) || !batch_ok(b)) return false;
+    if (heads < 1 || heads % c->n_heads) return false;
+    if ((int64_t)std::min(b->max_q, b->n_tokens) * heads > (1 << 26)) return false;
+    if (c->v.data) return c->width == 64 || c->width == 128 || c->width == 256;
+    return c->width == 576 && c->n_heads == 1;
+}
+
+int64_t part_bytes(const hearth_gpu_cache &c, const hearth_gpu_batch &b, int heads, Split &s) {
+    const Batch o = batch_of(b, c);
+    if (!o.n_seqs || !o.max_q) { s = {0x40000000, 1}; return 0; }
+    s = attend_split(o.n_seqs, o.max_q, o.kv_cap, heads, c.n_heads, !c.v.data);
+    const int64_t dv = c.v.data ? c.width : 512;
+    return s.n == 1 ? 0 : (int64_t)o.n_tokens * heads * s.n * (dv + 2) * (int64_t)sizeof(float);
+}
+
+int attend_call(const hearth_gpu_cache *c, const hearth_gpu_batch *b, const hearth_gpu_array *q, const hearth_gpu_array *q_pe,
+                const hearth_gpu_array *out, float *lse, float scale, void *work, size_t work_bytes, int dev, void *stream) {
+    if (!array_ok(q) || !array_ok(out) || !attend_shape_ok(c, b, q->n_heads) || dev < 0 || !std::isfinite(scale)) return E_ARG;
+    const bool latent = q_pe != nullptr;
+    if (latent != !c->v.data) return E_ARG;
+    if ((q->dtype != HEARTH_F16 && q->dtype != HEARTH_BF16) || out->dtype != q->dtype) return E_ARG;
+    if (c->dtype != HEARTH_GPU_MX8 && c->dtype != q->dtype) return E_ARG;
+    const int width = latent ? 512 : c->width;
+    if (q->width != width || out->width != width || out->n_heads != q->n_heads) return E_ARG;
+    if (latent && (!array_ok(q_pe) || q_pe->dtype != q->dtype || q_pe->n_heads != q->n_heads || q_pe->width != 64)) return E_ARG;
+    Split s;
+    const int64_t need = part_bytes(*c, *b, q->n_heads, s);
+    if (need && ((uintptr_t)work % 16 || !work)) return E_ARG;
+    if ((uint64_t)need > work_bytes) return E_CAPACITY;
+    AttendArgs a{};
+    a.b = batch_of(*b, *c);
+    if (!a.b.n_seqs || !a.b.max_q) return OK;
+    a.k = rows_of(c->k, c->dtype);
+    if (!latent) a.v = rows_of(c->v, c->dtype);
+    a.q = (const uint8_t *)q->data; a.qt = 2 * q->token_stride; a.qh = 2 * q->head_stride;
+    a.out = (uint8_t *)out->data; a.ot = 2 * out->token_stride; a.oh = 2 * out->head_stride;
+    a.aligned = on16(*q) && on16(*out);
+    if (latent) {
+        a.q_pe = (const uint8_t *)q_pe->data; a.pt = 2 * q_pe->token_stride; a.ph = 2 * q_pe->head_stride;
+        a.aligned = a.aligned && on16(*q_pe);
+    }
+    a.lse = lse;
+    a.heads = q->n_heads; a.kv_heads = c->n_heads; a.group = a.heads / a.kv_heads;
+    a.scale2 = scale * 1.44269504088896340736f;
+    a.chunk = s.chunk; a.n_splits = s.n;
+    a.part = (float *)work;
+    if (hipPeekAtLastError() != hipSuccess) return E_IO;
+    DeviceGuard g(dev);
+    if (launch_on(dev, g) != OK) return E_IO;
+    if (latent) attend_latent(a, q->dtype, c->dtype, (hipStream_t)stream);
+    else attend(a, q->dtype, c->dtype, c->width, (hipStream_t)stream);
+    return finish();
+}
+
+} // namespace
+
+extern "C" {
+
+HEARTH_API int hearth_gpu_rope(const hearth_gpu_array *x, const hearth_gpu_array *out, const hearth_gpu_array *k,
+                               const hearth_gpu_array *k_out, int n_tokens, const void *pos, int pos64,
+                               const double *freqs, int n_freqs, int offset, int interleaved, int inverse,
+                               double factor, int dev, void *stream) {
+    if (k && !k->data) k = nullptr;
+    if (k_out && !k_out->data) k_out = nullptr;
+    if (!array_ok(x) || !array_ok(out) || !k != !k_out || n_tokens < 0 || !pos || !freqs || dev < 0) return E_ARG;
+    if (n_freqs < 1 || n_freqs > 512 || offset < 0 || (int64_t)offset + 2 * n_freqs > x->width) return E_ARG;
+    if (!std::isfinite(factor) || (uintptr_t)pos % (pos64 ? 8 : 4) || (uintptr_t)freqs % 8) return E_ARG;
+    RopeArgs a{};
+    a.in_place = true;
+    a.n_pairs = k ? 2 : 1;
+    for (int i = 0; i < a.n_pairs; i++) {
+        const hearth_gpu_array *s = i ? k : x, *d = i ? k_out : out;
+        if (!array_ok(s) || !array_ok(d) || s->dtype != x->dtype || d->dtype != x->dtype || s->width != x->width ||
+            d->width != x->width || s->n_heads != d->n_heads) return E_ARG;
+        const int64_t es = elem(s->dtype);
+        a.p[i] = {(const uint8_t *)s->data, (uint8_t *)d->data, s->token_stride * es, s->head_stride * es,
+                  d->token_stride * es, d->head_stride * es, s->n_heads};
+        const bool same = s->data == d->data;
+        if (same && (s->token_stride != d->token_stride || s->head_stride != d->head_stride)) return E_ARG;
+        a.in_place = a.in_place && same;
+    }
+    a.pos = pos; a.pos64 = pos64 != 0; a.freqs = freqs;
+    a.n_tokens = n_tokens; a.width = x->width; a.n_freqs = n_freqs; a.offset = offset; a.interleaved = interleaved != 0;
+    a.factor = (float)factor; a.sign = inverse ? -1.0f : 1.0f;
+    if (!n_tokens) return OK;
+    if (hipPeekAtLastError() != hipSuccess) return E_IO;
+    DeviceGuard g(dev);
+    if (launch_on(dev, g) != OK) return E_IO;
+    rope(a, x->dtype, (hipStream_t)stream);
+    return finish();
+}
+
+HEARTH_API int hearth_gpu_kv_append(const hearth_gpu_cache *c, const hearth_gpu_batch *b, const hearth_gpu_array *k,
+                                    const hearth_gpu_array *v, int dev, void *stream) {
+    return copy_call(true, c, b, k, v, dev, stream);
+}
+
+HEARTH_API int hearth_gpu_kv_read(const hearth_gpu_cache *c, const hearth_gpu_batch *b, const hearth_gpu_array *k,
+                                  const hearth_gpu_array *v, int dev, void *stream) {
+    return copy_call(false, c, b, k, v, dev, stream);
+}
+
+HEARTH_API int64_t hearth_gpu_attend_workspace(const hearth_gpu_cache *c, const hearth_gpu_batch *b, int n_heads) {
+    if (!attend_shape_ok(c, b, n_heads)) return E_ARG;
+    Split s;
+    return part_bytes(*c, *b, n_heads, s);
+}
+
+HEARTH_API int hearth_gpu_attend(const hearth_gpu_cache *c, const hearth_gpu_batch *b, const hearth_gpu_array *q,
+                                 const hearth_gpu_array *out, float *lse, float scale, void *work, size_t work_bytes,
+                                 int dev, void *stream) {
+    return attend_call(c, b, q, nullptr, out, lse, scale, work, work_bytes, dev, stream);
+}
+
+HEARTH_API int hearth_gpu_attend_latent(const hearth_gpu_cache *c, const hearth_gpu_batch *b,
+                                        const hearth_gpu_array *q, const hearth_gpu_array *q_pe,
+                                        const hearth_gpu_array *out, float *lse, float scale, void *work,
+                                        size_t work_bytes, int dev, void *stream) {
+    if (!q_pe) return E_ARG;
+    return attend_call(c, b, q, q_pe, out, lse, scale, work, work_bytes, dev, stream);
+}
+
+} // extern "C"

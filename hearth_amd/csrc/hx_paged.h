@@ -1,0 +1,185 @@
+/*
+ * hx_paged.h — argument blocks, device helpers and launchers of the paged-cache operators
+ * (rotary positions, cache writes and reads, attention over pages). api_paged.cpp checks
+ * every host-side field before a launch; lengths and page ids live in device memory and are
+ * cut or checked in the kernels (seq_of, page_ok).
+ */
+#pragma once
+
+#include "hx_host.h"
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+namespace hxp {
+
+enum { DT_F32 = HEARTH_F32, DT_F16 = HEARTH_F16, DT_BF16 = HEARTH_BF16, DT_MX8 = HEARTH_GPU_MX8 };
+constexpr int MX_BLOCK = 32;
+
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+typedef float f2 __attribute__((ext_vector_type(2)));
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef float f16v __attribute__((ext_vector_type(16)));
+typedef unsigned u2 __attribute__((ext_vector_type(2)));
+typedef unsigned u4 __attribute__((ext_vector_type(4)));
+
+/* hearth_gpu_batch with the bounds of every sequence's rows folded in */
+struct Batch {
+    const int *pages, *kv_len, *q_start;
+    const unsigned long long *mask;
+    int64_t ld_pages;
+    int n_seqs, n_tokens, max_q, mask_words;
+    int kv_cap;       /* min(max_kv, pages_per_seq * page): rows past it do not exist for the call */
+    int n_pages, page_shift;
+};
+
+struct Rows {
+    uint8_t *data;    /* bytes */
+    uint8_t *scales;
+    int64_t page_stride, head_stride;               /* bytes */
+    int64_t scale_page_stride, scale_head_stride;   /* bytes */
+};
+
+/* ---- rotary positions ---- */
+struct RopeArgs {
+    struct Pair { const uint8_t *x; uint8_t *y; int64_t xt, xh, yt, yh; int heads; } p[2];   /* strides in bytes */
+    const void *pos;
+    const double *freqs;
+    int n_tokens, width, n_freqs, offset, pos64, interleaved, n_pairs;
+    float factor, sign;
+    bool in_place;    /* the elements outside the rotated part are where they belong */
+};
+
+/* ---- cache writes and reads: up to two pieces of a row (k and v, or latent and rotated part) ---- */
+struct Piece {
+    uint8_t *arr;             /* the caller's rows */
+    int64_t at, ah;           /* its strides, bytes */
+    Rows rows;
+    int col, width, row_width, heads;   /* elements [col, col + width) of cache rows of row_width */
+};
+struct CopyArgs {
+    Batch b;
+    Piece p[2];
+    int n_pieces, octs;       /* groups of 8 elements of a token over all pieces and heads */
+};
+
+/* ---- attention ---- */
+struct AttendArgs {
+    Batch b;
+    Rows k, v;
+    const uint8_t *q, *q_pe;
+    uint8_t *out;
+    float *lse;
+    int64_t qt, qh, pt, ph, ot, oh;   /* strides of q, q_pe, out; bytes */
+    int heads, kv_heads, group;       /* group: query heads per kv head */
+    float scale2;                     /* scale * log2(e): probabilities are powers of two */
+    int chunk, n_splits;              /* rows of a split (a multiple of the kernels' row step); splits of the longest */
+    bool aligned;                     /* q, q_pe and out start and step on 16 bytes */
+    float *part;                      /* [n_tokens][heads][n_splits][DV] sums, then [..][2] maximum and sum */
+};
+
+/* device of a call made current while the object lives */
+struct DeviceGuard {
+    int old = -1;
+    bool ok = false;
+    explicit DeviceGuard(int dev) {
+        if (hipGetDevice(&old) != hipSuccess) return;
+        ok = old == dev || hipSetDevice(dev) == hipSuccess;
+        if (old == dev) old = -1;
+    }
+    ~DeviceGuard() { if (ok && old >= 0) (void)hipSetDevice(old); }
+};
+
+void rope(const RopeArgs &a, int dtype, hipStream_t st);
+void kv_append(const CopyArgs &a, int src_dtype, int cache_dtype, bool aligned, hipStream_t st);
+void kv_read(const CopyArgs &a, int dst_dtype, int cache_dtype, bool aligned, hipStream_t st);
+
+/* Split of the rows axis: rows per split and splits of the longest sequence. Depends on the
+ * host-side fields only. latent: the kernels of attend_latent. */
+struct Split { int chunk, n; };
+Split attend_split(int n_seqs, int max_q, int kv_cap, int heads, int kv_heads, bool latent);
+void attend(const AttendArgs &a, int q_dtype, int cache_dtype, int width, hipStream_t st);
+void attend_latent(const AttendArgs &a, int q_dtype, int cache_dtype, hipStream_t st);
+
+/* ------------------------------------------------------------------ device helpers */
+
+struct Seq {
+    int q0, n;       /* first token of the call, tokens */
+    int kv;          /* rows that exist */
+    int base;        /* position of its first token of the call (negative: more tokens than rows) */
+};
+
+__device__ __forceinline__ Seq seq_of(const Batch &b, int s) {
+    Seq r;
+    const int lo = min(max(b.q_start[s], 0), b.n_tokens);
+    const int hi = min(max(b.q_start[s + 1], lo), b.n_tokens);
+    const int len = max(b.kv_len[s], 0);
+    r.q0 = lo;
+    r.n = hi - lo;
+    r.kv = min(len, b.kv_cap);
+    r.base = len - r.n;
+    return r;
+}
+
+__device__ __forceinline__ bool page_ok(const Batch &b, int id) { return (unsigned)id < (unsigned)b.n_pages; }
+
+/* 16-bit types: the matrix instructions and conversions of one type */
+struct Bf16 {
+    using v8 = b8;
+    using v2 = b2;
+    using e = __bf16;
+    static constexpr int dt = DT_BF16;
+    static __device__ __forceinline__ f4 mfma16(v8 a, v8 b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+    static __device__ __forceinline__ f16v mfma32(v8 a, v8 b, f16v c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+    /* codes (two bytes of x, the upper two with HI) times a power of two; exact but for underflow */
+    template <bool HI> static __device__ __forceinline__ unsigned from_mx8(unsigned x, float s) {
+        return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, s, HI));
+    }
+    /* round to nearest even, both halves */
+    static __device__ __forceinline__ unsigned pack(float a, float b) { return __builtin_bit_cast(unsigned, __builtin_convertvector((f2){a, b}, b2)); }
+    /* true where a half of x is infinite or NaN */
+    static __device__ __forceinline__ bool odd(unsigned x) { return (x & 0x7f80u) == 0x7f80u || (x & 0x7f800000u) == 0x7f800000u; }
+};
+struct F16 {
+    using v8 = h8;
+    using v2 = h2;
+    using e = _Float16;
+    static constexpr int dt = DT_F16;
+    static __device__ __forceinline__ f4 mfma16(v8 a, v8 b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+    static __device__ __forceinline__ f16v mfma32(v8 a, v8 b, f16v c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+    template <bool HI> static __device__ __forceinline__ unsigned from_mx8(unsigned x, float s) {
+        return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, s, HI));
+    }
+    static __device__ __forceinline__ unsigned pack(float a, float b) { return __builtin_bit_cast(unsigned, __builtin_convertvector((f2){a, b}, h2)); }
+    static __device__ __forceinline__ bool odd(unsigned x) { return (x & 0x7c00u) == 0x7c00u || (x & 0x7c000000u) == 0x7c000000u; }
+};
+
+/* the scale of a block from its byte (1 .. 254) */
+__device__ __forceinline__ float mx_scale(unsigned byte) { return __uint_as_float((byte & 255u) << 23); }
+
+/* maximum / sum of a value over the lanes l, l ^ 32 */
+__device__ __forceinline__ float max32(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float sum32(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+/* ... over the lanes l, l ^ 16 */
+__device__ __forceinline__ float max16(float x) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float sum16(float x) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+__device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
+
+} // namespace hxp

@@ -1,0 +1,437 @@
+/*
+ * k_paged_attn.hip — attention over a paged cache: few query rows a kv head (single tokens,
+ * chains), split over the cache's length and joined.
+ *
+ * The products run transposed: S^T = K Q^T (rows: cache rows, columns: query rows, one column
+ * a (token, head) pair of the kv head's group) and O^T = V^T P^T. In the 16 x 16 result of the
+ * first a lane holds four cache rows of one column, which is, two tiles together, the operand
+ * that the second product takes for the same column: the probabilities never leave the
+ * registers. V comes in by rows (8 elements of 8 cache rows a lane) and is transposed there,
+ * a byte permutation a pair of elements.
+ */
+#include "hx_paged.h"
+
+#include <algorithm>
+
+namespace hxp {
+
+namespace {
+
+constexpr int FEW_WAVES = 4, FEW_STEP = 32;   /* a wave takes 32 cache rows at a time, the workgroup 128 */
+
+__device__ __forceinline__ unsigned lo16(unsigned a, unsigned b) { return __builtin_amdgcn_perm(b, a, 0x05040100u); }
+__device__ __forceinline__ unsigned hi16(unsigned a, unsigned b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
+
+template <class T, bool MX, int DK, int DV, int NT, bool LATENT>
+struct Few {
+    using v8 = typename T::v8;
+    static constexpr int KS = DK / 32;                    /* matrix steps of the score */
+    static constexpr int BD = DV < 128 ? DV : 128;        /* elements of a V block: 16 lanes x PL */
+    static constexpr int NB = DV / BD, PL = BD / 16;      /* blocks; elements of a row a lane takes */
+    static constexpr int ES = MX ? 1 : 2;                 /* bytes of a stored element */
+
+    /* scores of 16 cache rows: row pointer of this lane's row */
+    static __device__ __forceinline__ void scores(const uint8_t *row, const uint8_t *sc, int g, const v8 (&q)[NT][KS], f4 (&s)[NT]) {
+        if constexpr (MX) {
+            u4 raw[DK / 64];
+            unsigned sb[DK / 64];
+#pragma unroll
+            for (int i = 0; i < DK / 64; i++) {
+                raw[i] = *(const u4 *)(row + 64 * i + 16 * g);
+                sb[i] = sc[2 * i + (g >> 1)];
+            }
+#pragma unroll
+            for (int i = 0; i < DK / 64; i++) {
+                const float f = mx_scale(sb[i]);
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const unsigned a = raw[i][2 * h], b = raw[i][2 * h + 1];
+                    const u4 w = {T::template from_mx8<false>(a, f), T::template from_mx8<true>(a, f),
+                                  T::template from_mx8<false>(b, f), T::template from_mx8<true>(b, f)};
+#pragma unroll
+                    for (int n = 0; n < NT; n++) s[n] = T::mfma16(__builtin_bit_cast(v8, w), q[n][2 * i + h], s[n]);
+                }
+            }
+        } else {
+            u4 raw[KS];
+#pragma unroll
+            for (int i = 0; i < KS; i++) raw[i] = *(const u4 *)(row + 64 * i + 16 * g);
+#pragma unroll
+            for (int i = 0; i < KS; i++)
+#pragma unroll
+                for (int n = 0; n < NT; n++) s[n] = T::mfma16(__builtin_bit_cast(v8, raw[i]), q[n][i], s[n]);
+        }
+    }
+
+    /* PL elements of one cache row as 16-bit pairs */
+    static __device__ __forceinline__ void v_row(const uint8_t *row, const uint8_t *sc, int d, unsigned (&w)[PL / 2]) {
+        if constexpr (MX) {
+            const float f = mx_scale(sc[d / MX_BLOCK]);
+#pragma unroll
+            for (int i = 0; i < PL / 4; i++) {
+                const unsigned c = ((const unsigned *)(row + d))[i];
+                w[2 * i] = T::template from_mx8<false>(c, f);
+                w[2 * i + 1] = T::template from_mx8<true>(c, f);
+            }
+        } else if constexpr (PL == 8) {
+            const u4 x = *(const u4 *)(row + 2 * d);
+#pragma unroll
+            for (int i = 0; i < 4; i++) w[i] = x[i];
+        } else {
+            const u2 x = *(const u2 *)(row + 2 * d);
+            w[0] = x[0]; w[1] = x[1];
+        }
+    }
+};
+
+template <class T, bool MX, int DK, int DV, int NT, bool LATENT>
+__global__ __launch_bounds__(64 * FEW_WAVES) void k_attend_few(AttendArgs a) {
+    using F = Few<T, MX, DK, DV, NT, LATENT>;
+    using v8 = typename T::v8;
+    constexpr int PL = F::PL, NB = F::NB, BD = F::BD, ES = F::ES, CT = 16 * NT;
+    __shared__ float lds_o[FEW_WAVES][16][BD + 4];
+    __shared__ float lds_m[FEW_WAVES][CT], lds_l[FEW_WAVES][CT];
+
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int g = lane >> 4, lc = lane & 15;
+    int bx = blockIdx.x;
+    const int sp = bx % a.n_splits;
+    bx /= a.n_splits;
+    const int kvh = bx % a.kv_heads, tile = bx / a.kv_heads;
+    const int seq = blockIdx.z;
+    const Seq q = seq_of(a.b, seq);
+    const int cols = min(q.n, a.b.max_q) * a.group;
+    if (tile * CT >= cols) return;
+    const int n_sp = max(1, (q.kv + a.chunk - 1) / a.chunk);
+    if (sp >= n_sp) return;
+
+    /* this lane's columns */
+    int tok[NT], head[NT], lim[NT];   /* lim: rows it attends without a mask (causal), or rows before the call's */
+    v8 qf[NT][F::KS];
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+        const int c = tile * CT + 16 * n + lc;
+        const bool on = c < cols;
+        tok[n] = on ? c / a.group : 0;
+        head[n] = kvh * a.group + (on ? c % a.group : 0);
+        lim[n] = !on ? 0 : a.b.mask ? min(q.base, q.kv) : min(q.base + tok[n] + 1, q.kv);
+        const uint8_t *qp = a.q + (int64_t)(q.q0 + tok[n]) * a.qt + (int64_t)head[n] * a.qh;
+        const uint8_t *pp = LATENT ? a.q_pe + (int64_t)(q.q0 + tok[n]) * a.pt + (int64_t)head[n] * a.ph : nullptr;
+#pragma unroll
+        for (int i = 0; i < F::KS; i++) {
+            const int d = MX ? 64 * (i / 2) + 16 * g + 8 * (i % 2) : 32 * i + 8 * g;
+            const unsigned short *p = (const unsigned short *)(LATENT && d >= DV ? pp : qp) + (LATENT && d >= DV ? d - DV : d);
+            u4 w = {0, 0, 0, 0};
+            if (on) {
+                if (a.aligned) w = *(const u4 *)p;
+                else
+#pragma unroll
+                    for (int k = 0; k < 4; k++) w[k] = p[2 * k] | (unsigned)p[2 * k + 1] << 16;
+            }
+            qf[n][i] = __builtin_bit_cast(v8, w);
+        }
+    }
+    /* rows [lo, hi) of this split that some column of the tile may attend; below `full` every
+     * valid column attends every row */
+    const int t_first = tile * CT / a.group, t_last = min(cols - 1, tile * CT + CT - 1) / a.group;
+    const int hi = min(min(q.kv, a.b.mask ? q.kv : q.base + t_last + 1), (sp + 1) * a.chunk);
+    const int full = a.b.mask ? q.base : q.base + t_first + 1;
+
+    f4 acc[NT][NB * PL];
+    float m[NT], l[NT];
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+        m[n] = -__builtin_huge_valf();
+        l[n] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NB * PL; i++) acc[n][i] = (f4){0, 0, 0, 0};
+    }
+    const int *pages = a.b.pages + (int64_t)seq * a.b.ld_pages;
+    const int page_rows = 1 << a.b.page_shift;
+    const uint8_t *kbase = a.k.data + (int64_t)kvh * a.k.head_stride, *vbase = LATENT ? kbase : a.v.data + (int64_t)kvh * a.v.head_stride;
+    const uint8_t *ksb = MX ? a.k.scales + (int64_t)kvh * a.k.scale_head_stride : nullptr;
+    const uint8_t *vsb = MX ? (LATENT ? ksb : a.v.scales + (int64_t)kvh * a.v.scale_head_stride) : nullptr;
+    const Rows &kr = a.k, &vr = LATENT ? a.k : a.v;
+
+    for (int t0 = sp * a.chunk + FEW_STEP * wave; t0 < hi; t0 += FEW_STEP * FEW_WAVES) {
+        /* pages of the two tiles of 16 rows; a tile past hi or without a page is not read */
+        int pid[2];
+        bool ok[2];
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            const int t = t0 + 16 * u;
+            pid[u] = t < hi ? pages[t >> a.b.page_shift] : -1;
+            ok[u] = page_ok(a.b, pid[u]);
+        }
+        f4 s[2][NT];
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+#pragma unroll
+            for (int n = 0; n < NT; n++) s[u][n] = (f4){0, 0, 0, 0};
+            if (ok[u]) {
+                const int r = ((t0 + 16 * u) & (page_rows - 1)) + lc;
+                const uint8_t *row = kbase + (int64_t)pid[u] * kr.page_stride + (int64_t)r * (DK * ES);
+                const uint8_t *sc = MX ? ksb + (int64_t)pid[u] * kr.scale_page_stride + (int64_t)r * (DK / MX_BLOCK) : nullptr;
+                F::scores(row, sc, g, qf, s[u]);
+            }
+        }
+        const bool whole = t0 + FEW_STEP <= full && t0 + FEW_STEP <= hi && ok[0] && ok[1];
+        /* bit j of vis[n]: column n attends this lane's j-th row */
+        unsigned vis[NT];
+        v8 pf[NT];
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            float x[8];
+            vis[n] = 255u;
+#pragma unroll
+            for (int j = 0; j < 8; j++) x[j] = s[j >> 2][n][j & 3] * a.scale2;
+            if (!whole) {
+                vis[n] = 0;
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const int t = t0 + 16 * (j >> 2) + 4 * g + (j & 3);
+                    bool v = t < lim[n];
+                    if (a.b.mask && !v && tile * CT + 16 * n + lc < cols && t >= q.base && t < q.kv) {
+                        const int nt = t - q.base;
+                        v = (nt >> 6) < a.b.mask_words &&
+                            (a.b.mask[(int64_t)(q.q0 + tok[n]) * a.b.mask_words + (nt >> 6)] >> (nt & 63) & 1);
+                    }
+                    v = v && t < hi && ok[j >> 2];
+                    vis[n] |= (unsigned)v << j;
+                    x[j] = v ? x[j] : -__builtin_huge_valf();
+                }
+            }
+            float mx = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+            mx = fmaxf(m[n], max16(max32(mx)));
+            const float ms = mx == -__builtin_huge_valf() ? 0.0f : mx;
+            if (__any(mx > m[n])) {
+                const float al = exp2_hw(m[n] - ms);
+                l[n] *= al;
+#pragma unroll
+                for (int i = 0; i < NB * PL; i++) acc[n][i] *= al;
+                m[n] = mx;
+            }
+            float p[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                p[j] = exp2_hw(x[j] - ms);
+                l[n] += p[j];
+            }
+            const u4 w = {T::pack(p[0], p[1]), T::pack(p[2], p[3]), T::pack(p[4], p[5]), T::pack(p[6], p[7])};
+            pf[n] = __builtin_bit_cast(v8, w);
+        }
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
+            unsigned w[8][PL / 2];
+            const int d = b * BD + lc * PL;
+            bool odd = false;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const int u = j >> 2, t = t0 + 16 * u + 4 * g + (j & 3), r = t & (page_rows - 1);
+                if (ok[u]) {
+                    F::v_row(vbase + (int64_t)pid[u] * vr.page_stride + (int64_t)r * (DK * ES),
+                             MX ? vsb + (int64_t)pid[u] * vr.scale_page_stride + (int64_t)r * (DK / MX_BLOCK) : nullptr, d, w[j]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < PL / 2; i++) w[j][i] = 0;
+                }
+                if (!whole) {
+#pragma unroll
+                    for (int i = 0; i < PL / 2; i++) {
+                        w[j][i] = t < hi ? w[j][i] : 0u;
+                        odd = odd || T::odd(w[j][i]);
+                    }
+                }
+            }
+            if (whole || !__any(odd)) {
+#pragma unroll
+                for (int i = 0; i < PL / 2; i++) {
+                    const u4 e = {lo16(w[0][i], w[1][i]), lo16(w[2][i], w[3][i]), lo16(w[4][i], w[5][i]), lo16(w[6][i], w[7][i])};
+                    const u4 o = {hi16(w[0][i], w[1][i]), hi16(w[2][i], w[3][i]), hi16(w[4][i], w[5][i]), hi16(w[6][i], w[7][i])};
+#pragma unroll
+                    for (int n = 0; n < NT; n++) {
+                        acc[n][b * PL + 2 * i] = T::mfma16(__builtin_bit_cast(v8, e), pf[n], acc[n][b * PL + 2 * i]);
+                        acc[n][b * PL + 2 * i + 1] = T::mfma16(__builtin_bit_cast(v8, o), pf[n], acc[n][b * PL + 2 * i + 1]);
+                    }
+                }
+            } else {
+                /* an infinity or NaN among rows that some columns do not attend (0 * inf would
+                 * reach them): one row at a time, added only where it is attended */
+#pragma unroll 1
+                for (int t = 0; t < 32; t++) {
+                    const int gg = (t >> 2) & 3, jj = (t >> 4) * 4 + (t & 3);
+                    const unsigned half = jj & 1 ? 0xffff0000u : 0x0000ffffu;
+                    bool on[NT];
+#pragma unroll
+                    for (int n = 0; n < NT; n++) on[n] = __shfl((int)(vis[n] >> jj & 1u), lc + 16 * gg) != 0;
+#pragma unroll
+                    for (int i = 0; i < PL / 2; i++) {
+                        u4 e = {lo16(w[0][i], w[1][i]), lo16(w[2][i], w[3][i]), lo16(w[4][i], w[5][i]), lo16(w[6][i], w[7][i])};
+                        u4 o = {hi16(w[0][i], w[1][i]), hi16(w[2][i], w[3][i]), hi16(w[4][i], w[5][i]), hi16(w[6][i], w[7][i])};
+#pragma unroll
+                        for (int k = 0; k < 4; k++) {
+                            const unsigned keep = g == gg && k == jj >> 1 ? half : 0u;
+                            e[k] &= keep;
+                            o[k] &= keep;
+                        }
+#pragma unroll
+                        for (int n = 0; n < NT; n++) {
+                            const f4 z = {0, 0, 0, 0};
+                            const f4 re = T::mfma16(__builtin_bit_cast(v8, e), pf[n], z), ro = T::mfma16(__builtin_bit_cast(v8, o), pf[n], z);
+#pragma unroll
+                            for (int k = 0; k < 4; k++) {
+                                acc[n][b * PL + 2 * i][k] += on[n] ? re[k] : 0.0f;
+                                acc[n][b * PL + 2 * i + 1][k] += on[n] ? ro[k] : 0.0f;
+                            }
+                        }
+                    }
+                }
+            }
+        }
+    }
+
+    /* the four waves' columns together: a lane's sums cover its own rows of each step only */
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+        l[n] = sum16(sum32(l[n]));
+        if (g == 0) { lds_m[wave][16 * n + lc] = m[n]; lds_l[wave][16 * n + lc] = l[n]; }
+    }
+    __syncthreads();
+    const bool direct = n_sp == 1;
+    const int oc = threadIdx.x >> 4, od = (threadIdx.x & 15) * PL;   /* output column and element of this thread */
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+        float M = lds_m[0][16 * n + lc];
+#pragma unroll
+        for (int w = 1; w < FEW_WAVES; w++) M = fmaxf(M, lds_m[w][16 * n + lc]);
+        const float f = m[n] == -__builtin_huge_valf() ? (l[n] == 0.0f ? 0.0f : 1.0f) : exp2_hw(m[n] - M);
+        /* the output thread's column */
+        float Mo = lds_m[0][16 * n + oc], Lo = 0.0f;
+#pragma unroll
+        for (int w = 1; w < FEW_WAVES; w++) Mo = fmaxf(Mo, lds_m[w][16 * n + oc]);
+#pragma unroll
+        for (int w = 0; w < FEW_WAVES; w++) {
+            const float mw = lds_m[w][16 * n + oc], lw = lds_l[w][16 * n + oc];
+            Lo += mw == -__builtin_huge_valf() ? lw : lw * exp2_hw(mw - Mo);
+        }
+        const int c = tile * CT + 16 * n + oc;
+        const bool on = c < cols;
+        const int ot = on ? c / a.group : 0, oh = kvh * a.group + (on ? c % a.group : 0);
+        const int64_t row = (int64_t)(q.q0 + ot) * a.heads + oh;
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
+            if (n + b) __syncthreads();
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int j = 0; j < PL; j += 4)
+                    *(f4 *)&lds_o[wave][lc][(4 * g + i) * PL + j] =
+                        (f4){acc[n][b * PL + j][i] * f, acc[n][b * PL + j + 1][i] * f, acc[n][b * PL + j + 2][i] * f, acc[n][b * PL + j + 3][i] * f};
+            __syncthreads();
+            if (!on) continue;
+            float o[PL];
+#pragma unroll
+            for (int j = 0; j < PL; j++) {
+                o[j] = 0.0f;
+#pragma unroll
+                for (int w = 0; w < FEW_WAVES; w++) o[j] += lds_o[w][oc][od + j];
+            }
+            if (direct) {
+                const float inv = Lo == 0.0f ? 0.0f : 1.0f / Lo;
+                uint8_t *out = a.out + (int64_t)(q.q0 + ot) * a.ot + (int64_t)oh * a.oh + 2 * (b * BD + od);
+                if (a.aligned) {
+#pragma unroll
+                    for (int j = 0; j < PL; j += 4)
+                        *(u2 *)(out + 2 * j) = (u2){T::pack(o[j] * inv, o[j + 1] * inv), T::pack(o[j + 2] * inv, o[j + 3] * inv)};
+                } else {
+#pragma unroll
+                    for (int j = 0; j < PL; j++) ((typename T::e *)out)[j] = (typename T::e)(o[j] * inv);
+                }
+            } else if (!(Lo == 0.0f)) {
+                float *po = a.part + (row * a.n_splits + sp) * DV + b * BD + od;
+#pragma unroll
+                for (int j = 0; j < PL; j += 4) *(f4 *)(po + j) = (f4){o[j], o[j + 1], o[j + 2], o[j + 3]};
+            }
+        }
+        if (on && (threadIdx.x & 15) == 0) {
+            if (!direct) {
+                float *ml = a.part + (int64_t)a.b.n_tokens * a.heads * a.n_splits * DV + (row * a.n_splits + sp) * 2;
+                ml[0] = Mo;
+                ml[1] = Lo;
+            } else if (a.lse) a.lse[row] = Lo == 0.0f ? -__builtin_huge_valf() : (Mo + __log2f(Lo)) * 0.69314718055994531f;
+        }
+    }
+}
+
+/* The splits of a query row joined: out = sum_i o_i 2^(m_i - M) / sum_i l_i 2^(m_i - M). One wave
+ * a (token, head); a split whose sum is 0 attended nothing and holds no sums. */
+template <class T, int DV>
+__global__ __launch_bounds__(64) void k_attend_join(AttendArgs a) {
+    constexpr int PL = DV / 64;
+    const int seq = blockIdx.z, lane = threadIdx.x;
+    const Seq q = seq_of(a.b, seq);
+    const int t = blockIdx.x / a.heads, h = blockIdx.x % a.heads;
+    if (t >= min(q.n, a.b.max_q)) return;
+    const int n_sp = max(1, (q.kv + a.chunk - 1) / a.chunk);
+    if (n_sp == 1) return;
+    const int64_t row = (int64_t)(q.q0 + t) * a.heads + h;
+    const float *po = a.part + row * a.n_splits * DV + lane * PL;
+    const float *ml = a.part + (int64_t)a.b.n_tokens * a.heads * a.n_splits * DV + row * a.n_splits * 2;
+    float M = -__builtin_huge_valf();
+    for (int i = lane; i < n_sp; i += 64) M = fmaxf(M, ml[2 * i]);
+#pragma unroll
+    for (int d = 32; d; d >>= 1) M = fmaxf(M, __shfl_xor(M, d));
+    float L = 0.0f, o[PL] = {};
+    for (int i = 0; i < n_sp; i++) {
+        const float mi = ml[2 * i], li = ml[2 * i + 1];
+        if (li == 0.0f) continue;
+        const float f = mi == -__builtin_huge_valf() ? 1.0f : exp2_hw(mi - M);
+        L += li * f;
+#pragma unroll
+        for (int j = 0; j < PL; j++) o[j] = __builtin_fmaf(po[(int64_t)i * DV + j], f, o[j]);
+    }
+    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+    typename T::e *out = (typename T::e *)(a.out + (int64_t)(q.q0 + t) * a.ot + (int64_t)h * a.oh) + lane * PL;
+#pragma unroll
+    for (int j = 0; j < PL; j++) out[j] = (typename T::e)(o[j] * inv);
+    if (a.lse && lane == 0) a.lse[row] = L == 0.0f ? -__builtin_huge_valf() : (M + __log2f(L)) * 0.69314718055994531f;
+}
+
+template <class T, bool MX, int DK, int DV, bool LATENT>
+void attend_t(const AttendArgs &a, hipStream_t st) {
+    const int cols = a.b.max_q * a.group;
+    const int tiles = (cols + 15) / 16;
+    const dim3 grid((unsigned)a.n_splits * a.kv_heads * tiles, 1, a.b.n_seqs);
+    hipLaunchKernelGGL((k_attend_few<T, MX, DK, DV, 1, LATENT>), grid, dim3(64 * FEW_WAVES), 0, st, a);
+    if (a.n_splits > 1)
+        hipLaunchKernelGGL((k_attend_join<T, DV>), dim3((unsigned)a.b.max_q * a.heads, 1, a.b.n_seqs), dim3(64), 0, st, a);
+}
+
+} // namespace
+
+/* Rows a split takes: enough workgroups for the 256 units, at least one step of every wave. */
+Split attend_split(int n_seqs, int max_q, int kv_cap, int heads, int kv_heads, bool latent) {
+    const int64_t wgs = (int64_t)n_seqs * kv_heads * (((int64_t)max_q * (heads / kv_heads) + 15) / 16);
+    const int64_t want = std::max<int64_t>(1, 1024 / std::max<int64_t>(wgs, 1));
+    const int step = FEW_STEP * FEW_WAVES;
+    int64_t chunk = (kv_cap + want - 1) / want;
+    chunk = std::max<int64_t>((chunk + step - 1) / step * step, step);
+    (void)latent;
+    return {(int)std::min<int64_t>(chunk, 0x40000000), std::max(1, (int)((kv_cap + chunk - 1) / chunk))};
+}
+
+void attend(const AttendArgs &a, int q_dtype, int cache_dtype, int width, hipStream_t st) {
+    const bool mx = cache_dtype == DT_MX8;
+#define HXP_ATTEND(T, D) (mx ? attend_t<T, true, D, D, false>(a, st) : attend_t<T, false, D, D, false>(a, st))
+    if (q_dtype == DT_BF16) width == 64 ? HXP_ATTEND(Bf16, 64) : width == 128 ? HXP_ATTEND(Bf16, 128) : HXP_ATTEND(Bf16, 256);
+    else width == 64 ? HXP_ATTEND(F16, 64) : width == 128 ? HXP_ATTEND(F16, 128) : HXP_ATTEND(F16, 256);
+#undef HXP_ATTEND
+}
+
+void attend_latent(const AttendArgs &a, int q_dtype, int cache_dtype, hipStream_t st) {
+    const bool mx = cache_dtype == DT_MX8;
+    if (q_dtype == DT_BF16) mx ? attend_t<Bf16, true, 576, 512, true>(a, st) : attend_t<Bf16, false, 576, 512, true>(a, st);
+    else mx ? attend_t<F16, true, 576, 512, true>(a, st) : attend_t<F16, false, 576, 512, true>(a, st);
+}
+
+} // namespace hxp

@@ -276,6 +276,123 @@ HEARTH_API int hearth_gpu_get_store_info(hearth_engine *e, hearth_gpu_store_info
 /* Device the library runs on (HEARTH_DEVICE, default 0) and its name. */
 HEARTH_API int hearth_gpu_device(char *name, size_t n);
 
+/* ---- paged key-value caches (device buffers, any stream) --------------------------
+ *
+ * Operators for programs that keep the rows of many conversations in pages on the GPU:
+ * rotary positions, writing new tokens' rows, reading rows back, and the attention over
+ * the pages. No counterpart in the reference (its engine keeps one conversation's rows in
+ * float32). They are separate from an engine: every pointer is the caller's DEVICE memory
+ * on device `dev` (a HIP device index; the calling thread's current device is left as it
+ * was), the work is enqueued on `stream` (a hipStream_t of that device, NULL: the null
+ * stream) and not waited for, and nothing is allocated, so the calls may be captured into a
+ * graph. Returns 0, -1 for bad arguments, -3 for a workspace that is too small, -4 for a
+ * device error of the call's launches, or -4 without launching when the calling thread holds
+ * a HIP error it has not read yet (that error is left for the caller).
+ *
+ * What lies in device memory (page ids, lengths) cannot be checked by the host; the kernels
+ * check it: a page id outside [0, n_pages) is neither read nor written (its rows count as
+ * masked, read as zeros and are not stored), lengths are cut to what the page table and the
+ * buffers hold. */
+#define HEARTH_GPU_MX8 16   /* cache rows of e4m3 codes (OCP FP8, finite) with one E8M0 scale byte per 32 elements */
+
+/* One tensor of a cache: rows [n_pages][n_heads][page][width], the last two dimensions
+ * dense. Strides in elements; data and strides are multiples of 16 bytes. MX8: scales
+ * [n_pages][n_heads][page][width / 32], the last two dimensions dense: element = code *
+ * 2^(scale - 127). */
+typedef struct hearth_gpu_rows {
+    void *data;
+    uint8_t *scales;
+    int64_t page_stride, head_stride;
+    int64_t scale_page_stride, scale_head_stride;
+} hearth_gpu_rows;
+
+/* A cache: k and v of the same shape, or k alone (v.data NULL: latent rows, which hold a
+ * token's latent vector and then its rotated part). page: a power of two from 16 to 4096;
+ * width: a multiple of 32 up to 1024; dtype: HEARTH_F16, HEARTH_BF16 or HEARTH_GPU_MX8. */
+typedef struct hearth_gpu_cache {
+    hearth_gpu_rows k, v;
+    int32_t dtype, n_pages, n_heads, page, width;
+} hearth_gpu_cache;
+
+/* The sequences of a call. Sequence s holds kv_len[s] rows, row p in page
+ * pages[s * ld_pages + p / page], and its last q_start[s + 1] - q_start[s] rows belong to
+ * the call's tokens q_start[s] .. q_start[s + 1) (of n_tokens in all; tokens behind the last
+ * sequence's are padding and left alone). max_q and max_kv bound every sequence's token
+ * count and length: what lies beyond them is not computed. mask: NULL (each token attends
+ * the rows up to its own) or [n_tokens][mask_words] 64-bit words: a token attends its
+ * sequence's rows before the call's tokens, and the call's token j of its sequence where
+ * bit j is set (a draft tree). */
+typedef struct hearth_gpu_batch {
+    const int32_t *pages, *kv_len, *q_start;
+    const uint64_t *mask;
+    int64_t ld_pages;
+    int32_t n_seqs, pages_per_seq, n_tokens, max_q, max_kv, mask_words;
+} hearth_gpu_batch;
+
+/* A caller's array [n_tokens][n_heads][width] of dtype HEARTH_F32, HEARTH_F16 or
+ * HEARTH_BF16, the last dimension dense, strides in elements. */
+typedef struct hearth_gpu_array {
+    void *data;
+    int64_t token_stride, head_stride;
+    int32_t dtype, n_heads, width;
+} hearth_gpu_array;
+
+/* Rotary positions: for every token t and head, with a = pos[t] * freqs[j] (radians, in
+ * float64), the pair (x[o + j], x[o + j + n_freqs]) (interleaved 0) or (x[o + 2j],
+ * x[o + 2j + 1]) (interleaved 1), o = offset, becomes factor * (u cos a - v sin a,
+ * v cos a + u sin a); inverse 1 rotates by -a (the gradient's direction). Elements outside
+ * [o, o + 2 n_freqs) are copied. out may be x (in place) or share no element with it. x, out
+ * and, when k_out.data is not NULL, k, k_out (a second pair, rotated in the same launch) have
+ * one dtype and width; positions int32, or int64 when pos64 is 1. */
+HEARTH_API int hearth_gpu_rope(const hearth_gpu_array *x, const hearth_gpu_array *out, const hearth_gpu_array *k,
+                               const hearth_gpu_array *k_out, int n_tokens, const void *pos, int pos64,
+                               const double *freqs, int n_freqs, int offset, int interleaved, int inverse,
+                               double factor, int dev, void *stream);
+
+/* Writes the call's tokens' rows into the cache, converted (16-bit) or quantised (MX8). With
+ * k and v in the cache, the arrays have its heads and width; a latent cache takes the latent
+ * as k and the rotated part as v (NULL: none), one head each, widths multiples of 32 that add
+ * up to the cache's. MX8: a block's scale is the least power of two with max |x| / scale <=
+ * 448 over the block's finite values (scale byte 1 at least), codes round to nearest even; a
+ * NaN or infinity is stored as NaN; a value whose rounding would leave the range of x's type
+ * is stored as the largest code within it. Tokens at negative positions (more tokens than
+ * rows) and rows past the bounds are not stored; two sequences that share a page in which
+ * they write the same row leave one or a mixture of the two. */
+HEARTH_API int hearth_gpu_kv_append(const hearth_gpu_cache *c, const hearth_gpu_batch *b, const hearth_gpu_array *k,
+                                    const hearth_gpu_array *v, int dev, void *stream);
+
+/* The inverse: the call's tokens' rows read back into the arrays (q_start = running sum of
+ * kv_len reads whole sequences). Rows that are not in the cache read as zeros. */
+HEARTH_API int hearth_gpu_kv_read(const hearth_gpu_cache *c, const hearth_gpu_batch *b, const hearth_gpu_array *k,
+                                  const hearth_gpu_array *v, int dev, void *stream);
+
+/* Attention of the call's tokens over the cache: q [n_tokens][H][width], out alike, of dtype
+ * HEARTH_F16 or HEARTH_BF16; H a multiple of the cache's heads, head h reads kv head
+ * h / (H / n_heads); width 64, 128 or 256. out = softmax(scale * q . k) v over the rows a
+ * token attends; a token that attends nothing gets zeros. 16-bit caches have q's dtype; MX8
+ * rows are taken as their values in q's dtype. Scores, softmax statistics and sums are
+ * float32; the probabilities are rounded to q's dtype for the product with v. lse: NULL or
+ * [n_tokens][H] float32, the natural logarithm of the sum of exponentials (-infinity where
+ * nothing is attended). work: device memory of hearth_gpu_attend_workspace bytes, 16-byte
+ * aligned; calls that may run at the same time must not share it. */
+HEARTH_API int hearth_gpu_attend(const hearth_gpu_cache *c, const hearth_gpu_batch *b, const hearth_gpu_array *q,
+                                 const hearth_gpu_array *out, float *lse, float scale, void *work, size_t work_bytes,
+                                 int dev, void *stream);
+
+/* The absorbed form of latent attention: q [n_tokens][H][C] (each head's query taken through
+ * its key projection) and q_pe [n_tokens][H][R] (its rotated part) against the latent rows'
+ * first C and last R elements, out [n_tokens][H][C] = softmax(scale * (q . c + q_pe . pe)) c.
+ * C = 512, R = 64, cache width 576, one cache head; everything else as hearth_gpu_attend. */
+HEARTH_API int hearth_gpu_attend_latent(const hearth_gpu_cache *c, const hearth_gpu_batch *b,
+                                        const hearth_gpu_array *q, const hearth_gpu_array *q_pe,
+                                        const hearth_gpu_array *out, float *lse, float scale, void *work,
+                                        size_t work_bytes, int dev, void *stream);
+
+/* Workspace of either attention for n_heads query heads: bytes (0: none needed), or -1 for
+ * arguments the attention would refuse. It depends on the host-side fields only, and not on
+ * anything in device memory. */
+HEARTH_API int64_t hearth_gpu_attend_workspace(const hearth_gpu_cache *c, const hearth_gpu_batch *b, int n_heads);
+
 #ifdef __cplusplus
 }
 #endif
