@@ -134,8 +134,8 @@ bool attend_shape_ok(const hearth_gpu_cache *c, const hearth_gpu_batch *b, int h
 
 int64_t part_bytes(const hearth_gpu_cache &c, const hearth_gpu_batch &b, int heads, Split &s) {
     const Batch o = batch_of(b, c);
-    if (!o.n_seqs || !o.max_q) { s = {0x40000000, 1}; return 0; }
-    s = attend_split(o.n_seqs, o.max_q, o.kv_cap, heads, c.n_heads, !c.v.data);
+    if (!o.n_seqs || !o.max_q) { s = {0x40000000, 1, false}; return 0; }
+    s = attend_split(o.n_seqs, b.max_q, o.kv_cap, heads, c.n_heads, !c.v.data);
     const int64_t dv = c.v.data ? c.width : 512;
     return s.n == 1 ? 0 : (int64_t)o.n_tokens * heads * s.n * (dv + 2) * (int64_t)sizeof(float);
 }
@@ -175,7 +175,7 @@ int attend_call(const hearth_gpu_cache *c, const hearth_gpu_batch *b, const hear
     DeviceGuard g(dev);
     if (launch_on(dev, g) != OK) return E_IO;
     if (latent) attend_latent(a, q->dtype, c->dtype, (hipStream_t)stream);
-    else attend(a, q->dtype, c->dtype, c->width, (hipStream_t)stream);
+    else attend(a, q->dtype, c->dtype, c->width, s.many, (hipStream_t)stream);
     return finish();
 }
 

@@ -98,11 +98,13 @@ void rope(const RopeArgs &a, int dtype, hipStream_t st);
 void kv_append(const CopyArgs &a, int src_dtype, int cache_dtype, bool aligned, hipStream_t st);
 void kv_read(const CopyArgs &a, int dst_dtype, int cache_dtype, bool aligned, hipStream_t st);
 
-/* Split of the rows axis: rows per split and splits of the longest sequence. Depends on the
- * host-side fields only. latent: the kernels of attend_latent. */
-struct Split { int chunk, n; };
+/* Split of the rows axis: rows per split and splits of the longest sequence, and whether the
+ * kernel of many query rows takes the call. Depends on the host-side fields only, and not on the
+ * call's token count. latent: the kernels of attend_latent. */
+struct Split { int chunk, n; bool many; };
 Split attend_split(int n_seqs, int max_q, int kv_cap, int heads, int kv_heads, bool latent);
-void attend(const AttendArgs &a, int q_dtype, int cache_dtype, int width, hipStream_t st);
+void attend(const AttendArgs &a, int q_dtype, int cache_dtype, int width, bool many, hipStream_t st);
+void attend_many(const AttendArgs &a, int q_dtype, int cache_dtype, int width, hipStream_t st);   /* k_paged_many.hip */
 void attend_latent(const AttendArgs &a, int q_dtype, int cache_dtype, hipStream_t st);
 
 /* ------------------------------------------------------------------ device helpers */
@@ -141,6 +143,11 @@ struct Bf16 {
     }
     /* round to nearest even, both halves */
     static __device__ __forceinline__ unsigned pack(float a, float b) { return __builtin_bit_cast(unsigned, __builtin_convertvector((f2){a, b}, b2)); }
+    static __device__ __forceinline__ float wide(unsigned x) { return __uint_as_float(x << 16); }   /* of the lower half */
+    /* x with infinite and NaN halves as zeros */
+    static __device__ __forceinline__ unsigned clean(unsigned x) {
+        return ((x & 0x7f80u) == 0x7f80u ? 0u : x & 0xffffu) | ((x & 0x7f800000u) == 0x7f800000u ? 0u : x & 0xffff0000u);
+    }
     /* true where a half of x is infinite or NaN */
     static __device__ __forceinline__ bool odd(unsigned x) { return (x & 0x7f80u) == 0x7f80u || (x & 0x7f800000u) == 0x7f800000u; }
 };
@@ -155,8 +162,21 @@ struct F16 {
         return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, s, HI));
     }
     static __device__ __forceinline__ unsigned pack(float a, float b) { return __builtin_bit_cast(unsigned, __builtin_convertvector((f2){a, b}, h2)); }
+    static __device__ __forceinline__ float wide(unsigned x) { return (float)__builtin_bit_cast(_Float16, (unsigned short)x); }
+    static __device__ __forceinline__ unsigned clean(unsigned x) {
+        return ((x & 0x7c00u) == 0x7c00u ? 0u : x & 0xffffu) | ((x & 0x7c000000u) == 0x7c000000u ? 0u : x & 0xffff0000u);
+    }
     static __device__ __forceinline__ bool odd(unsigned x) { return (x & 0x7c00u) == 0x7c00u || (x & 0x7c000000u) == 0x7c000000u; }
 };
+
+/* Element d of a stored row (row: its first byte, sc: its first scale byte) in T's format */
+template <class T, bool MX>
+__device__ __forceinline__ unsigned row_elem(const uint8_t *row, const uint8_t *sc, int d) {
+    if constexpr (MX)
+        return T::template from_mx8<false>((unsigned)row[d], __uint_as_float((unsigned)sc[d / MX_BLOCK] << 23)) & 0xffffu;
+    else
+        return ((const unsigned short *)row)[d];
+}
 
 /* the scale of a block from its byte (1 .. 254) */
 __device__ __forceinline__ float mx_scale(unsigned byte) { return __uint_as_float((byte & 255u) << 23); }

@@ -137,8 +137,20 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_attend_few(AttendArgs a) {
     const int hi = min(min(q.kv, a.b.mask ? q.kv : q.base + t_last + 1), (sp + 1) * a.chunk);
     const int full = a.b.mask ? q.base : q.base + t_first + 1;
 
+    /* whether column n of this lane attends row t of the sequence (if its page exists) */
+    auto attended = [&](int n, int t) {
+        bool v = t < lim[n];
+        if (a.b.mask && !v && tile * CT + 16 * n + lc < cols && t >= q.base && t < q.kv) {
+            const int nt = t - q.base;
+            v = (nt >> 6) < a.b.mask_words &&
+                (a.b.mask[(int64_t)(q.q0 + tok[n]) * a.b.mask_words + (nt >> 6)] >> (nt & 63) & 1);
+        }
+        return v && t < hi;
+    };
+
     f4 acc[NT][NB * PL];
     float m[NT], l[NT];
+    bool odd = false;   /* V held an infinity or NaN in a row that some column does not attend */
 #pragma unroll
     for (int n = 0; n < NT; n++) {
         m[n] = -__builtin_huge_valf();
@@ -176,28 +188,17 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_attend_few(AttendArgs a) {
             }
         }
         const bool whole = t0 + FEW_STEP <= full && t0 + FEW_STEP <= hi && ok[0] && ok[1];
-        /* bit j of vis[n]: column n attends this lane's j-th row */
-        unsigned vis[NT];
         v8 pf[NT];
 #pragma unroll
         for (int n = 0; n < NT; n++) {
             float x[8];
-            vis[n] = 255u;
 #pragma unroll
             for (int j = 0; j < 8; j++) x[j] = s[j >> 2][n][j & 3] * a.scale2;
             if (!whole) {
-                vis[n] = 0;
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
                     const int t = t0 + 16 * (j >> 2) + 4 * g + (j & 3);
-                    bool v = t < lim[n];
-                    if (a.b.mask && !v && tile * CT + 16 * n + lc < cols && t >= q.base && t < q.kv) {
-                        const int nt = t - q.base;
-                        v = (nt >> 6) < a.b.mask_words &&
-                            (a.b.mask[(int64_t)(q.q0 + tok[n]) * a.b.mask_words + (nt >> 6)] >> (nt & 63) & 1);
-                    }
-                    v = v && t < hi && ok[j >> 2];
-                    vis[n] |= (unsigned)v << j;
+                    const bool v = attended(n, t) && ok[j >> 2];
                     x[j] = v ? x[j] : -__builtin_huge_valf();
                 }
             }
@@ -224,7 +225,6 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_attend_few(AttendArgs a) {
         for (int b = 0; b < NB; b++) {
             unsigned w[8][PL / 2];
             const int d = b * BD + lc * PL;
-            bool odd = false;
 #pragma unroll
             for (int j = 0; j < 8; j++) {
                 const int u = j >> 2, t = t0 + 16 * u + 4 * g + (j & 3), r = t & (page_rows - 1);
@@ -240,52 +240,45 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_attend_few(AttendArgs a) {
                     for (int i = 0; i < PL / 2; i++) {
                         w[j][i] = t < hi ? w[j][i] : 0u;
                         odd = odd || T::odd(w[j][i]);
+                        w[j][i] = T::clean(w[j][i]);
                     }
                 }
             }
-            if (whole || !__any(odd)) {
 #pragma unroll
-                for (int i = 0; i < PL / 2; i++) {
-                    const u4 e = {lo16(w[0][i], w[1][i]), lo16(w[2][i], w[3][i]), lo16(w[4][i], w[5][i]), lo16(w[6][i], w[7][i])};
-                    const u4 o = {hi16(w[0][i], w[1][i]), hi16(w[2][i], w[3][i]), hi16(w[4][i], w[5][i]), hi16(w[6][i], w[7][i])};
+            for (int i = 0; i < PL / 2; i++) {
+                const u4 e = {lo16(w[0][i], w[1][i]), lo16(w[2][i], w[3][i]), lo16(w[4][i], w[5][i]), lo16(w[6][i], w[7][i])};
+                const u4 o = {hi16(w[0][i], w[1][i]), hi16(w[2][i], w[3][i]), hi16(w[4][i], w[5][i]), hi16(w[6][i], w[7][i])};
 #pragma unroll
-                    for (int n = 0; n < NT; n++) {
-                        acc[n][b * PL + 2 * i] = T::mfma16(__builtin_bit_cast(v8, e), pf[n], acc[n][b * PL + 2 * i]);
-                        acc[n][b * PL + 2 * i + 1] = T::mfma16(__builtin_bit_cast(v8, o), pf[n], acc[n][b * PL + 2 * i + 1]);
-                    }
+                for (int n = 0; n < NT; n++) {
+                    acc[n][b * PL + 2 * i] = T::mfma16(__builtin_bit_cast(v8, e), pf[n], acc[n][b * PL + 2 * i]);
+                    acc[n][b * PL + 2 * i + 1] = T::mfma16(__builtin_bit_cast(v8, o), pf[n], acc[n][b * PL + 2 * i + 1]);
                 }
-            } else {
-                /* an infinity or NaN among rows that some columns do not attend (0 * inf would
-                 * reach them): one row at a time, added only where it is attended */
+            }
+        }
+    }
+    /* an infinity or NaN among rows that some columns do not attend would reach them as 0 * inf:
+     * left out above, added here to the columns that do attend it */
+    if (__any(odd)) {
+        for (int t0 = sp * a.chunk + FEW_STEP * wave; t0 < hi; t0 += FEW_STEP * FEW_WAVES) {
 #pragma unroll 1
-                for (int t = 0; t < 32; t++) {
-                    const int gg = (t >> 2) & 3, jj = (t >> 4) * 4 + (t & 3);
-                    const unsigned half = jj & 1 ? 0xffff0000u : 0x0000ffffu;
-                    bool on[NT];
+            for (int t = t0; t < min(t0 + FEW_STEP, hi); t++) {
+                const int id = pages[t >> a.b.page_shift];
+                if (t0 + FEW_STEP <= full && t0 + FEW_STEP <= hi && page_ok(a.b, pages[t0 >> a.b.page_shift]) &&
+                    page_ok(a.b, pages[(t0 + 16) >> a.b.page_shift])) break;   /* a step taken as it is */
+                if (!page_ok(a.b, id)) continue;
+                const uint8_t *row = vbase + (int64_t)id * vr.page_stride + (int64_t)(t & (page_rows - 1)) * (DK * ES);
+                const uint8_t *sc = MX ? vsb + (int64_t)id * vr.scale_page_stride + (t & (page_rows - 1)) * (DK / MX_BLOCK) : nullptr;
 #pragma unroll
-                    for (int n = 0; n < NT; n++) on[n] = __shfl((int)(vis[n] >> jj & 1u), lc + 16 * gg) != 0;
+                for (int b = 0; b < NB; b++)
 #pragma unroll
-                    for (int i = 0; i < PL / 2; i++) {
-                        u4 e = {lo16(w[0][i], w[1][i]), lo16(w[2][i], w[3][i]), lo16(w[4][i], w[5][i]), lo16(w[6][i], w[7][i])};
-                        u4 o = {hi16(w[0][i], w[1][i]), hi16(w[2][i], w[3][i]), hi16(w[4][i], w[5][i]), hi16(w[6][i], w[7][i])};
+                    for (int j = 0; j < PL; j++)
 #pragma unroll
-                        for (int k = 0; k < 4; k++) {
-                            const unsigned keep = g == gg && k == jj >> 1 ? half : 0u;
-                            e[k] &= keep;
-                            o[k] &= keep;
+                        for (int i = 0; i < 4; i++) {
+                            const unsigned x = row_elem<T, MX>(row, sc, b * BD + (4 * g + i) * PL + j);
+#pragma unroll
+                            for (int n = 0; n < NT; n++)
+                                acc[n][b * PL + j][i] += T::odd(x) && attended(n, t) ? T::wide(x) : 0.0f;
                         }
-#pragma unroll
-                        for (int n = 0; n < NT; n++) {
-                            const f4 z = {0, 0, 0, 0};
-                            const f4 re = T::mfma16(__builtin_bit_cast(v8, e), pf[n], z), ro = T::mfma16(__builtin_bit_cast(v8, o), pf[n], z);
-#pragma unroll
-                            for (int k = 0; k < 4; k++) {
-                                acc[n][b * PL + 2 * i][k] += on[n] ? re[k] : 0.0f;
-                                acc[n][b * PL + 2 * i + 1][k] += on[n] ? ro[k] : 0.0f;
-                            }
-                        }
-                    }
-                }
             }
         }
     }
@@ -398,40 +391,59 @@ __global__ __launch_bounds__(64) void k_attend_join(AttendArgs a) {
 }
 
 template <class T, bool MX, int DK, int DV, bool LATENT>
-void attend_t(const AttendArgs &a, hipStream_t st) {
-    const int cols = a.b.max_q * a.group;
-    const int tiles = (cols + 15) / 16;
+void few_t(const AttendArgs &a, hipStream_t st) {
+    const int tiles = (a.b.max_q * a.group + 15) / 16;
     const dim3 grid((unsigned)a.n_splits * a.kv_heads * tiles, 1, a.b.n_seqs);
     hipLaunchKernelGGL((k_attend_few<T, MX, DK, DV, 1, LATENT>), grid, dim3(64 * FEW_WAVES), 0, st, a);
-    if (a.n_splits > 1)
-        hipLaunchKernelGGL((k_attend_join<T, DV>), dim3((unsigned)a.b.max_q * a.heads, 1, a.b.n_seqs), dim3(64), 0, st, a);
+}
+
+template <class T, int DV>
+void join_t(const AttendArgs &a, hipStream_t st) {
+    hipLaunchKernelGGL((k_attend_join<T, DV>), dim3((unsigned)a.b.max_q * a.heads, 1, a.b.n_seqs), dim3(64), 0, st, a);
 }
 
 } // namespace
 
+/* Columns (query rows of a kv head) from which the kernel of many rows is taken. */
+static bool takes_many(int64_t cols, bool latent) { return !latent && cols > 32; }
+
 /* Rows a split takes: enough workgroups for the 256 units, at least one step of every wave. */
 Split attend_split(int n_seqs, int max_q, int kv_cap, int heads, int kv_heads, bool latent) {
-    const int64_t wgs = (int64_t)n_seqs * kv_heads * (((int64_t)max_q * (heads / kv_heads) + 15) / 16);
-    const int64_t want = std::max<int64_t>(1, 1024 / std::max<int64_t>(wgs, 1));
+    const int64_t cols = (int64_t)max_q * (heads / kv_heads);
+    const bool many = takes_many(cols, latent);
+    const int64_t wgs = (int64_t)n_seqs * kv_heads * (many ? (cols + 127) / 128 : (cols + 15) / 16);
+    const int64_t want = std::max<int64_t>(1, (many ? 512 : 1024) / std::max<int64_t>(wgs, 1));
     const int step = FEW_STEP * FEW_WAVES;
     int64_t chunk = (kv_cap + want - 1) / want;
     chunk = std::max<int64_t>((chunk + step - 1) / step * step, step);
-    (void)latent;
-    return {(int)std::min<int64_t>(chunk, 0x40000000), std::max(1, (int)((kv_cap + chunk - 1) / chunk))};
+    return {(int)std::min<int64_t>(chunk, 0x40000000), std::max(1, (int)((kv_cap + chunk - 1) / chunk)), many};
 }
 
-void attend(const AttendArgs &a, int q_dtype, int cache_dtype, int width, hipStream_t st) {
+void attend(const AttendArgs &a, int q_dtype, int cache_dtype, int width, bool many, hipStream_t st) {
     const bool mx = cache_dtype == DT_MX8;
-#define HXP_ATTEND(T, D) (mx ? attend_t<T, true, D, D, false>(a, st) : attend_t<T, false, D, D, false>(a, st))
-    if (q_dtype == DT_BF16) width == 64 ? HXP_ATTEND(Bf16, 64) : width == 128 ? HXP_ATTEND(Bf16, 128) : HXP_ATTEND(Bf16, 256);
-    else width == 64 ? HXP_ATTEND(F16, 64) : width == 128 ? HXP_ATTEND(F16, 128) : HXP_ATTEND(F16, 256);
-#undef HXP_ATTEND
+#define HXP_BY(F, T) (width == 64 ? F(T, 64) : width == 128 ? F(T, 128) : F(T, 256))
+#define HXP_FEW(T, D) (mx ? few_t<T, true, D, D, false>(a, st) : few_t<T, false, D, D, false>(a, st))
+#define HXP_JOIN(T, D) join_t<T, D>(a, st)
+    if (many) attend_many(a, q_dtype, cache_dtype, width, st);
+    else if (q_dtype == DT_BF16) HXP_BY(HXP_FEW, Bf16);
+    else HXP_BY(HXP_FEW, F16);
+    if (a.n_splits == 1) return;
+    if (q_dtype == DT_BF16) HXP_BY(HXP_JOIN, Bf16);
+    else HXP_BY(HXP_JOIN, F16);
+#undef HXP_JOIN
+#undef HXP_FEW
+#undef HXP_BY
 }
 
 void attend_latent(const AttendArgs &a, int q_dtype, int cache_dtype, hipStream_t st) {
     const bool mx = cache_dtype == DT_MX8;
-    if (q_dtype == DT_BF16) mx ? attend_t<Bf16, true, 576, 512, true>(a, st) : attend_t<Bf16, false, 576, 512, true>(a, st);
-    else mx ? attend_t<F16, true, 576, 512, true>(a, st) : attend_t<F16, false, 576, 512, true>(a, st);
+#define HXP_FEW(T) (mx ? few_t<T, true, 576, 512, true>(a, st) : few_t<T, false, 576, 512, true>(a, st))
+    if (q_dtype == DT_BF16) HXP_FEW(Bf16);
+    else HXP_FEW(F16);
+#undef HXP_FEW
+    if (a.n_splits == 1) return;
+    if (q_dtype == DT_BF16) join_t<Bf16, 512>(a, st);
+    else join_t<F16, 512>(a, st);
 }
 
 } // namespace hxp

@@ -1,0 +1,396 @@
+/*
+ * k_paged_many.hip — attention over a paged cache for many query rows a kv head: prompts and
+ * draft trees.
+ *
+ * As in k_paged_attn.hip the products run transposed, S^T = K Q^T and O^T = V^T P^T, here with
+ * the 32 x 32 x 16 matrix instruction: a wave owns 32 columns ((token, head) pairs of the kv
+ * head's group), a lane half of one column's scores, so the softmax needs one exchange between
+ * lanes l and l ^ 32, and the scores' registers, packed, are the second product's operand.
+ * Four waves (128 columns) share 64 cache rows (32 of width 256) at a time through LDS: K by rows, V transposed on
+ * the way in (8 rows x 8 elements a thread, byte permutations) with the rows of each group of 16
+ * in the order in which a lane's scores hold them (0-3 8-11 | 4-7 12-15), both padded by 16 bytes
+ * a row against bank conflicts, double-buffered; the next step's loads are in flight while
+ * this one is worked on. 8-bit rows become 16-bit ones on the way into LDS, once for the four waves.
+ */
+#include "hx_paged.h"
+
+#include <algorithm>
+
+namespace hxp {
+
+namespace {
+
+constexpr int MANY_WAVES = 4, MANY_COLS = 32 * MANY_WAVES;
+
+__device__ __forceinline__ unsigned lo16(unsigned a, unsigned b) { return __builtin_amdgcn_perm(b, a, 0x05040100u); }
+__device__ __forceinline__ unsigned hi16(unsigned a, unsigned b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
+
+template <class T, bool MX, int D>
+struct Many {
+    static constexpr int ROWS = D <= 128 ? 64 : 32;               /* cache rows of a step */
+    static constexpr int KLD = D + 8, VLD = ROWS + 8;             /* LDS rows, elements */
+    static constexpr int KB = ROWS * KLD * 2, VB = D * VLD * 2;   /* bytes of a buffer */
+    static constexpr int LDS = 2 * (KB + VB);
+    static constexpr int VI = D * ROWS / 64;                      /* threads that bring in V; as many bring in K */
+    static constexpr int GROUPS = ROWS / 16, TILES = ROWS / 32;
+    static_assert(2 * VI <= 64 * MANY_WAVES, "a thread takes one item");
+
+    struct Stage {
+        u4 w[8];     /* MX: codes in the first two words */
+        unsigned s[8];
+    };
+
+    /* row of the tile that piece j of item `it` reads (V: rows of one operand chunk) */
+    static __device__ __forceinline__ int row_of(bool v, int it, int j) {
+        if (v) {
+            const int c = it % (ROWS / 8);             /* chunk: group of 16, half */
+            return (c >> 1) * 16 + (c & 1) * 4 + (j & 3) + (j >> 2) * 8;
+        }
+        return it / (D / 8) + ROWS / 8 * j;
+    }
+    static __device__ __forceinline__ int elem_of(bool v, int it) { return v ? it / (ROWS / 8) * 8 : it % (D / 8) * 8; }
+};
+
+template <class T, bool MX, int D>
+__global__ __launch_bounds__(64 * MANY_WAVES, D <= 128 ? 2 : 1) void k_attend_many(AttendArgs a) {
+    using M = Many<T, MX, D>;
+    using v8 = typename T::v8;
+    constexpr int KS = D / 16, DT = D / 32;
+    constexpr float NINF = -__builtin_huge_valf();
+    __shared__ __align__(16) uint8_t lds[M::LDS];
+    __shared__ int odd_flag;
+
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int half = lane >> 5, lc = lane & 31;
+    int bx = blockIdx.x;
+    const int kvh = bx % a.kv_heads;
+    bx /= a.kv_heads;
+    const int sp = bx % a.n_splits;
+    const int tiles = gridDim.x / (a.kv_heads * a.n_splits), tile = tiles - 1 - bx / a.n_splits;   /* the longest first */
+    const int seq = blockIdx.z;
+    const Seq q = seq_of(a.b, seq);
+    const int cols = min(q.n, a.b.max_q) * a.group;
+    if (tile * MANY_COLS >= cols) return;
+    const int n_sp = max(1, (q.kv + a.chunk - 1) / a.chunk);
+    if (sp >= n_sp) return;
+
+    const int c = tile * MANY_COLS + 32 * wave + lc;
+    const bool on = c < cols;
+    const int tok = on ? c / a.group : 0, head = kvh * a.group + (on ? c % a.group : 0);
+    const int lim = !on ? 0 : a.b.mask ? min(q.base, q.kv) : min(q.base + tok + 1, q.kv);
+    const unsigned flip = a.scale2 < 0.0f ? 0x80008000u : 0u;   /* a negative scale turns q's signs */
+    const float scale2 = __builtin_fabsf(a.scale2);
+    v8 qf[KS];
+    {
+        const uint8_t *qp = a.q + (int64_t)(q.q0 + tok) * a.qt + (int64_t)head * a.qh;
+#pragma unroll
+        for (int i = 0; i < KS; i++) {
+            const unsigned short *p = (const unsigned short *)qp + 16 * i + 8 * half;
+            u4 w = {0, 0, 0, 0};
+            if (on) {
+                if (a.aligned) w = *(const u4 *)p;
+                else
+#pragma unroll
+                    for (int k = 0; k < 4; k++) w[k] = p[2 * k] | (unsigned)p[2 * k + 1] << 16;
+            }
+            qf[i] = __builtin_bit_cast(v8, w ^ flip);
+        }
+    }
+    const int t_last = min(cols - 1, tile * MANY_COLS + MANY_COLS - 1) / a.group;
+    const int hi = min(min(q.kv, a.b.mask ? q.kv : q.base + t_last + 1), (sp + 1) * a.chunk);
+    const int full = a.b.mask ? q.base : q.base + tile * MANY_COLS / a.group + 1;
+    const int lo = sp * a.chunk;
+
+    /* whether this lane's column attends row t of the sequence (if its page exists) */
+    auto attended = [&](int t) {
+        bool v = t < lim;
+        if (a.b.mask && !v && on && t >= q.base && t < q.kv) {
+            const int nt = t - q.base;
+            v = (nt >> 6) < a.b.mask_words &&
+                (a.b.mask[(int64_t)(q.q0 + tok) * a.b.mask_words + (nt >> 6)] >> (nt & 63) & 1);
+        }
+        return v && t < hi;
+    };
+
+    f16v acc[DT];
+#pragma unroll
+    for (int i = 0; i < DT; i++)
+#pragma unroll
+        for (int j = 0; j < 16; j++) acc[i][j] = 0.0f;
+    float m = NINF, l = 0.0f;
+
+    const int *pages = a.b.pages + (int64_t)seq * a.b.ld_pages;
+    const int rmask = (1 << a.b.page_shift) - 1;
+    const uint8_t *kbase = a.k.data + (int64_t)kvh * a.k.head_stride, *vbase = a.v.data + (int64_t)kvh * a.v.head_stride;
+    const uint8_t *ksb = MX ? a.k.scales + (int64_t)kvh * a.k.scale_head_stride : nullptr;
+    const uint8_t *vsb = MX ? a.v.scales + (int64_t)kvh * a.v.scale_head_stride : nullptr;
+
+    int pid[M::GROUPS];              /* pages of the groups of 16 rows, -1: none */
+    auto load_pages = [&](int t0) {
+#pragma unroll
+        for (int u = 0; u < M::GROUPS; u++) {
+            const int t = t0 + 16 * u;
+            const int id = t < hi ? pages[t >> a.b.page_shift] : -1;
+            pid[u] = page_ok(a.b, id) ? id : -1;
+        }
+    };
+    auto page_of = [&](int r) {
+        int id = pid[0];
+#pragma unroll
+        for (int u = 1; u < M::GROUPS; u++) id = r >> 4 == u ? pid[u] : id;
+        return id;
+    };
+    const bool st_v = (int)threadIdx.x < M::VI, st_on = (int)threadIdx.x < 2 * M::VI;
+    const int st_it = st_v ? threadIdx.x : threadIdx.x - M::VI, st_e = M::elem_of(st_v, st_it);
+    const uint8_t *st_base = st_v ? vbase : kbase, *st_sb = st_v ? vsb : ksb;
+    const int64_t st_ps = st_v ? a.v.page_stride : a.k.page_stride, st_ss = st_v ? a.v.scale_page_stride : a.k.scale_page_stride;
+    typename M::Stage st;
+    auto load = [&](int t0) {
+        if (!st_on) return;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const int r = M::row_of(st_v, st_it, j), id = page_of(r);
+            st.w[j] = (u4){0, 0, 0, 0};
+            st.s[j] = 127;
+            if (id >= 0 && t0 + r < hi) {
+                const int el = ((t0 + r) & rmask) * D + st_e;
+                const uint8_t *base = st_base + (int64_t)id * st_ps;
+                if constexpr (MX) {
+                    const u2 x = *(const u2 *)(base + el);
+                    st.w[j] = (u4){x[0], x[1], 0, 0};
+                    st.s[j] = (st_sb + (int64_t)id * st_ss)[el / MX_BLOCK];
+                } else {
+                    st.w[j] = *(const u4 *)(base + 2 * (int64_t)el);
+                }
+            }
+        }
+    };
+    /* The loaded rows into LDS. `some`: rows that some columns do not attend; an infinity or NaN
+     * of V there would reach them as 0 * inf, so it is left out and added at the end. */
+    auto store = [&](int buf, bool some) {
+        if (!st_on) return;
+        uint8_t *kb = lds + buf * M::KB, *vb = lds + 2 * M::KB + buf * M::VB;
+        u4 w[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            if constexpr (MX) {
+                const float f = mx_scale(st.s[j]);
+                const unsigned x = st.w[j][0], y = st.w[j][1];
+                w[j] = (u4){T::template from_mx8<false>(x, f), T::template from_mx8<true>(x, f),
+                            T::template from_mx8<false>(y, f), T::template from_mx8<true>(y, f)};
+            } else {
+                w[j] = st.w[j];
+            }
+        }
+        if (st_v) {
+            if (some) {
+                bool odd = false;
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        odd = odd || T::odd(w[j][k]);
+                        w[j][k] = T::clean(w[j][k]);
+                    }
+                if (odd) odd_flag = 1;
+            }
+            uint8_t *p = vb + (st_e * M::VLD + st_it % (M::ROWS / 8) * 8) * 2;
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                *(u4 *)(p + 4 * k * M::VLD) =
+                    (u4){lo16(w[0][k], w[1][k]), lo16(w[2][k], w[3][k]), lo16(w[4][k], w[5][k]), lo16(w[6][k], w[7][k])};
+                *(u4 *)(p + (4 * k + 2) * M::VLD) =
+                    (u4){hi16(w[0][k], w[1][k]), hi16(w[2][k], w[3][k]), hi16(w[4][k], w[5][k]), hi16(w[6][k], w[7][k])};
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; j++) *(u4 *)(kb + (M::row_of(false, st_it, j) * M::KLD + st_e) * 2) = w[j];
+        }
+    };
+    /* whether some column of the workgroup may not attend every row of the step at t0 (pages: bit
+     * u where group u has one) */
+    auto edge_at = [&](int t0, unsigned have) {
+        return !(t0 + M::ROWS <= full && t0 + M::ROWS <= hi && have == (1u << M::GROUPS) - 1);
+    };
+
+    if (threadIdx.x == 0) odd_flag = 0;
+    unsigned have_now = 0, have_next = 0;   /* bit u: group u has a page */
+    auto have = [&] {
+        unsigned b = 0;
+#pragma unroll
+        for (int u = 0; u < M::GROUPS; u++) b |= pid[u] >= 0 ? 1u << u : 0u;
+        return b;
+    };
+    __syncthreads();
+    if (lo < hi) {
+        load_pages(lo);
+        have_next = have();
+        load(lo);
+        store(0, lo + M::ROWS > full);
+        if (lo + M::ROWS < hi) load_pages(lo + M::ROWS);
+    }
+    __syncthreads();
+
+    int buf = 0;
+    for (int t0 = lo; t0 < hi; t0 += M::ROWS, buf ^= 1) {
+        const bool more = t0 + M::ROWS < hi;
+        have_now = have_next;
+        if (more) {
+            have_next = have();
+            load(t0 + M::ROWS);
+            if (t0 + 2 * M::ROWS < hi) load_pages(t0 + 2 * M::ROWS);
+        }
+        const uint8_t *kb = lds + buf * M::KB, *vb = lds + 2 * M::KB + buf * M::VB;
+        f16v s[M::TILES];
+#pragma unroll
+        for (int u = 0; u < M::TILES; u++)
+#pragma unroll
+            for (int j = 0; j < 16; j++) s[u][j] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < KS; i++)
+#pragma unroll
+            for (int u = 0; u < M::TILES; u++)
+                s[u] = T::mfma32(*(const v8 *)(kb + ((32 * u + lc) * M::KLD + 16 * i + 8 * half) * 2), qf[i], s[u]);
+
+        const bool edge = edge_at(t0, have_now);
+        v8 pf[M::GROUPS];
+        float mx;
+        if (!edge) {
+            mx = s[0][0];
+#pragma unroll
+            for (int u = 0; u < M::TILES; u++)
+#pragma unroll
+                for (int j = 0; j < 16; j++) mx = fmaxf(mx, s[u][j]);
+            mx = max32(mx) * scale2;
+        } else {
+            mx = NINF;
+#pragma unroll
+            for (int u = 0; u < M::TILES; u++)
+#pragma unroll
+                for (int j = 0; j < 16; j++) {
+                    const int r = 32 * u + 8 * (j >> 2) + 4 * half + (j & 3), t = t0 + r;
+                    const bool v = attended(t) && (have_now >> (r >> 4) & 1);
+                    s[u][j] = v ? s[u][j] * scale2 : NINF;
+                    mx = fmaxf(mx, s[u][j]);
+                }
+            mx = max32(mx);
+        }
+        mx = fmaxf(mx, m);
+        const float ms = mx == NINF ? 0.0f : mx;
+        if (__any(mx > m)) {
+            const float al = exp2_hw(m - ms);
+            l *= al;
+#pragma unroll
+            for (int i = 0; i < DT; i++) acc[i] *= al;
+            m = mx;
+        }
+        const float sc = edge ? 1.0f : scale2;
+        float ls = 0.0f;
+#pragma unroll
+        for (int u = 0; u < M::TILES; u++)
+#pragma unroll
+            for (int j = 0; j < 16; j++) {
+                s[u][j] = exp2_hw(__builtin_fmaf(s[u][j], sc, -ms));
+                ls += s[u][j];
+            }
+        l += ls;
+#pragma unroll
+        for (int g = 0; g < M::GROUPS; g++) {
+            const f16v &x = s[g >> 1];
+            const int o = 8 * (g & 1);
+            const u4 w = {T::pack(x[o], x[o + 1]), T::pack(x[o + 2], x[o + 3]), T::pack(x[o + 4], x[o + 5]), T::pack(x[o + 6], x[o + 7])};
+            pf[g] = __builtin_bit_cast(v8, w);
+        }
+#pragma unroll
+        for (int g = 0; g < M::GROUPS; g++)
+#pragma unroll
+            for (int i = 0; i < DT; i++)
+                acc[i] = T::mfma32(*(const v8 *)(vb + ((32 * i + lc) * M::VLD + 16 * g + 8 * half) * 2), pf[g], acc[i]);
+        if (more) store(buf ^ 1, t0 + 2 * M::ROWS > full);
+        __syncthreads();
+    }
+
+    if (odd_flag) {
+#pragma unroll 1
+        for (int t = max(lo, full / M::ROWS * M::ROWS); t < hi; t++) {
+            const int id = pages[t >> a.b.page_shift];
+            if (!page_ok(a.b, id)) continue;
+            const bool add = attended(t);
+            const uint8_t *row = vbase + (int64_t)id * a.v.page_stride + (int64_t)(t & rmask) * (D * (MX ? 1 : 2));
+            const uint8_t *sc = MX ? vsb + (int64_t)id * a.v.scale_page_stride + (t & rmask) * (D / MX_BLOCK) : nullptr;
+#pragma unroll
+            for (int i = 0; i < DT; i++)
+#pragma unroll
+                for (int j = 0; j < 16; j++) {
+                    const unsigned x = row_elem<T, MX>(row, sc, 32 * i + 8 * (j >> 2) + 4 * half + (j & 3));
+                    acc[i][j] += add && T::odd(x) ? T::wide(x) : 0.0f;
+                }
+        }
+    }
+
+    l = sum32(l);
+    if (!on) return;
+    const int64_t row = (int64_t)(q.q0 + tok) * a.heads + head;
+    if (n_sp == 1) {
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        uint8_t *out = a.out + (int64_t)(q.q0 + tok) * a.ot + (int64_t)head * a.oh;
+#pragma unroll
+        for (int i = 0; i < DT; i++)
+#pragma unroll
+            for (int b = 0; b < 4; b += 2) {
+                /* lanes l and l ^ 32 hold elements 0-3 8-11 and 4-7 12-15 of these 16: after the
+                 * exchange each has 8 consecutive ones */
+                unsigned x[2][2];
+#pragma unroll
+                for (int k = 0; k < 2; k++)
+#pragma unroll
+                    for (int w = 0; w < 2; w++)
+                        x[k][w] = T::pack(acc[i][4 * (b + k) + 2 * w] * inv, acc[i][4 * (b + k) + 2 * w + 1] * inv);
+                u4 o;
+#pragma unroll
+                for (int w = 0; w < 2; w++) {
+                    const auto r = __builtin_amdgcn_permlane32_swap(x[0][w], x[1][w], false, false);
+                    o[w] = r[0];
+                    o[2 + w] = r[1];
+                }
+                uint8_t *p = out + 2 * (32 * i + 8 * b + 8 * half);
+                if (a.aligned) *(u4 *)p = o;
+                else
+#pragma unroll
+                    for (int k = 0; k < 8; k++) ((unsigned short *)p)[k] = (unsigned short)(o[k >> 1] >> (16 * (k & 1)));
+            }
+        if (a.lse && half == 0) a.lse[row] = l == 0.0f ? NINF : (m + __log2f(l)) * 0.69314718055994531f;
+    } else {
+        float *po = a.part + (row * a.n_splits + sp) * D;
+        if (!(l == 0.0f))
+#pragma unroll
+            for (int i = 0; i < DT; i++)
+#pragma unroll
+                for (int b = 0; b < 4; b++)
+                    *(f4 *)(po + 32 * i + 8 * b + 4 * half) = (f4){acc[i][4 * b], acc[i][4 * b + 1], acc[i][4 * b + 2], acc[i][4 * b + 3]};
+        if (half == 0) {
+            float *ml = a.part + (int64_t)a.b.n_tokens * a.heads * a.n_splits * D + (row * a.n_splits + sp) * 2;
+            ml[0] = m;
+            ml[1] = l;
+        }
+    }
+}
+
+template <class T, bool MX, int D>
+void many_t(const AttendArgs &a, hipStream_t st) {
+    const int64_t tiles = ((int64_t)a.b.max_q * a.group + MANY_COLS - 1) / MANY_COLS;
+    const dim3 grid((unsigned)(tiles * a.n_splits * a.kv_heads), 1, a.b.n_seqs);
+    hipLaunchKernelGGL((k_attend_many<T, MX, D>), grid, dim3(64 * MANY_WAVES), 0, st, a);
+}
+
+} // namespace
+
+void attend_many(const AttendArgs &a, int q_dtype, int cache_dtype, int width, hipStream_t st) {
+    const bool mx = cache_dtype == DT_MX8;
+#define HXP_MANY(T, D) (mx ? many_t<T, true, D>(a, st) : many_t<T, false, D>(a, st))
+    if (q_dtype == DT_BF16) width == 64 ? HXP_MANY(Bf16, 64) : width == 128 ? HXP_MANY(Bf16, 128) : HXP_MANY(Bf16, 256);
+    else width == 64 ? HXP_MANY(F16, 64) : width == 128 ? HXP_MANY(F16, 128) : HXP_MANY(F16, 256);
+#undef HXP_MANY
+}
+
+} // namespace hxp
