@@ -105,6 +105,7 @@ struct Split { int chunk, n; bool many; };
 Split attend_split(int n_seqs, int max_q, int kv_cap, int heads, int kv_heads, bool latent);
 void attend(const AttendArgs &a, int q_dtype, int cache_dtype, int width, bool many, hipStream_t st);
 void attend_many(const AttendArgs &a, int q_dtype, int cache_dtype, int width, hipStream_t st);   /* k_paged_many.hip */
+void latent_rows(const AttendArgs &a, int q_dtype, bool mx, hipStream_t st);                         /* k_paged_latent.hip */
 void attend_latent(const AttendArgs &a, int q_dtype, int cache_dtype, hipStream_t st);
 
 /* ------------------------------------------------------------------ device helpers */

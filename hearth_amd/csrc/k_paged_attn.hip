@@ -22,26 +22,26 @@ constexpr int FEW_WAVES = 4, FEW_STEP = 32;   /* a wave takes 32 cache rows at a
 __device__ __forceinline__ unsigned lo16(unsigned a, unsigned b) { return __builtin_amdgcn_perm(b, a, 0x05040100u); }
 __device__ __forceinline__ unsigned hi16(unsigned a, unsigned b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
 
-template <class T, bool MX, int DK, int DV, int NT, bool LATENT>
+template <class T, bool MX, int D, int NT>
 struct Few {
     using v8 = typename T::v8;
-    static constexpr int KS = DK / 32;                    /* matrix steps of the score */
-    static constexpr int BD = DV < 128 ? DV : 128;        /* elements of a V block: 16 lanes x PL */
-    static constexpr int NB = DV / BD, PL = BD / 16;      /* blocks; elements of a row a lane takes */
+    static constexpr int KS = D / 32;                    /* matrix steps of the score */
+    static constexpr int BD = D < 128 ? D : 128;        /* elements of a V block: 16 lanes x PL */
+    static constexpr int NB = D / BD, PL = BD / 16;      /* blocks; elements of a row a lane takes */
     static constexpr int ES = MX ? 1 : 2;                 /* bytes of a stored element */
 
     /* scores of 16 cache rows: row pointer of this lane's row */
     static __device__ __forceinline__ void scores(const uint8_t *row, const uint8_t *sc, int g, const v8 (&q)[NT][KS], f4 (&s)[NT]) {
         if constexpr (MX) {
-            u4 raw[DK / 64];
-            unsigned sb[DK / 64];
+            u4 raw[D / 64];
+            unsigned sb[D / 64];
 #pragma unroll
-            for (int i = 0; i < DK / 64; i++) {
+            for (int i = 0; i < D / 64; i++) {
                 raw[i] = *(const u4 *)(row + 64 * i + 16 * g);
                 sb[i] = sc[2 * i + (g >> 1)];
             }
 #pragma unroll
-            for (int i = 0; i < DK / 64; i++) {
+            for (int i = 0; i < D / 64; i++) {
                 const float f = mx_scale(sb[i]);
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
@@ -84,9 +84,9 @@ struct Few {
     }
 };
 
-template <class T, bool MX, int DK, int DV, int NT, bool LATENT>
+template <class T, bool MX, int D, int NT>
 __global__ __launch_bounds__(64 * FEW_WAVES) void k_attend_few(AttendArgs a) {
-    using F = Few<T, MX, DK, DV, NT, LATENT>;
+    using F = Few<T, MX, D, NT>;
     using v8 = typename T::v8;
     constexpr int PL = F::PL, NB = F::NB, BD = F::BD, ES = F::ES, CT = 16 * NT;
     __shared__ float lds_o[FEW_WAVES][16][BD + 4];
@@ -116,11 +116,10 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_attend_few(AttendArgs a) {
         head[n] = kvh * a.group + (on ? c % a.group : 0);
         lim[n] = !on ? 0 : a.b.mask ? min(q.base, q.kv) : min(q.base + tok[n] + 1, q.kv);
         const uint8_t *qp = a.q + (int64_t)(q.q0 + tok[n]) * a.qt + (int64_t)head[n] * a.qh;
-        const uint8_t *pp = LATENT ? a.q_pe + (int64_t)(q.q0 + tok[n]) * a.pt + (int64_t)head[n] * a.ph : nullptr;
 #pragma unroll
         for (int i = 0; i < F::KS; i++) {
             const int d = MX ? 64 * (i / 2) + 16 * g + 8 * (i % 2) : 32 * i + 8 * g;
-            const unsigned short *p = (const unsigned short *)(LATENT && d >= DV ? pp : qp) + (LATENT && d >= DV ? d - DV : d);
+            const unsigned short *p = (const unsigned short *)qp + d;
             u4 w = {0, 0, 0, 0};
             if (on) {
                 if (a.aligned) w = *(const u4 *)p;
@@ -160,10 +159,10 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_attend_few(AttendArgs a) {
     }
     const int *pages = a.b.pages + (int64_t)seq * a.b.ld_pages;
     const int page_rows = 1 << a.b.page_shift;
-    const uint8_t *kbase = a.k.data + (int64_t)kvh * a.k.head_stride, *vbase = LATENT ? kbase : a.v.data + (int64_t)kvh * a.v.head_stride;
+    const uint8_t *kbase = a.k.data + (int64_t)kvh * a.k.head_stride, *vbase = a.v.data + (int64_t)kvh * a.v.head_stride;
     const uint8_t *ksb = MX ? a.k.scales + (int64_t)kvh * a.k.scale_head_stride : nullptr;
-    const uint8_t *vsb = MX ? (LATENT ? ksb : a.v.scales + (int64_t)kvh * a.v.scale_head_stride) : nullptr;
-    const Rows &kr = a.k, &vr = LATENT ? a.k : a.v;
+    const uint8_t *vsb = MX ? a.v.scales + (int64_t)kvh * a.v.scale_head_stride : nullptr;
+    const Rows &kr = a.k, &vr = a.v;
 
     for (int t0 = sp * a.chunk + FEW_STEP * wave; t0 < hi; t0 += FEW_STEP * FEW_WAVES) {
         /* pages of the two tiles of 16 rows; a tile past hi or without a page is not read */
@@ -182,8 +181,8 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_attend_few(AttendArgs a) {
             for (int n = 0; n < NT; n++) s[u][n] = (f4){0, 0, 0, 0};
             if (ok[u]) {
                 const int r = ((t0 + 16 * u) & (page_rows - 1)) + lc;
-                const uint8_t *row = kbase + (int64_t)pid[u] * kr.page_stride + (int64_t)r * (DK * ES);
-                const uint8_t *sc = MX ? ksb + (int64_t)pid[u] * kr.scale_page_stride + (int64_t)r * (DK / MX_BLOCK) : nullptr;
+                const uint8_t *row = kbase + (int64_t)pid[u] * kr.page_stride + (int64_t)r * (D * ES);
+                const uint8_t *sc = MX ? ksb + (int64_t)pid[u] * kr.scale_page_stride + (int64_t)r * (D / MX_BLOCK) : nullptr;
                 F::scores(row, sc, g, qf, s[u]);
             }
         }
@@ -229,8 +228,8 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_attend_few(AttendArgs a) {
             for (int j = 0; j < 8; j++) {
                 const int u = j >> 2, t = t0 + 16 * u + 4 * g + (j & 3), r = t & (page_rows - 1);
                 if (ok[u]) {
-                    F::v_row(vbase + (int64_t)pid[u] * vr.page_stride + (int64_t)r * (DK * ES),
-                             MX ? vsb + (int64_t)pid[u] * vr.scale_page_stride + (int64_t)r * (DK / MX_BLOCK) : nullptr, d, w[j]);
+                    F::v_row(vbase + (int64_t)pid[u] * vr.page_stride + (int64_t)r * (D * ES),
+                             MX ? vsb + (int64_t)pid[u] * vr.scale_page_stride + (int64_t)r * (D / MX_BLOCK) : nullptr, d, w[j]);
                 } else {
 #pragma unroll
                     for (int i = 0; i < PL / 2; i++) w[j][i] = 0;
@@ -266,8 +265,8 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_attend_few(AttendArgs a) {
                 if (t0 + FEW_STEP <= full && t0 + FEW_STEP <= hi && page_ok(a.b, pages[t0 >> a.b.page_shift]) &&
                     page_ok(a.b, pages[(t0 + 16) >> a.b.page_shift])) break;   /* a step taken as it is */
                 if (!page_ok(a.b, id)) continue;
-                const uint8_t *row = vbase + (int64_t)id * vr.page_stride + (int64_t)(t & (page_rows - 1)) * (DK * ES);
-                const uint8_t *sc = MX ? vsb + (int64_t)id * vr.scale_page_stride + (t & (page_rows - 1)) * (DK / MX_BLOCK) : nullptr;
+                const uint8_t *row = vbase + (int64_t)id * vr.page_stride + (int64_t)(t & (page_rows - 1)) * (D * ES);
+                const uint8_t *sc = MX ? vsb + (int64_t)id * vr.scale_page_stride + (t & (page_rows - 1)) * (D / MX_BLOCK) : nullptr;
 #pragma unroll
                 for (int b = 0; b < NB; b++)
 #pragma unroll
@@ -341,14 +340,14 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_attend_few(AttendArgs a) {
                     for (int j = 0; j < PL; j++) ((typename T::e *)out)[j] = (typename T::e)(o[j] * inv);
                 }
             } else if (!(Lo == 0.0f)) {
-                float *po = a.part + (row * a.n_splits + sp) * DV + b * BD + od;
+                float *po = a.part + (row * a.n_splits + sp) * D + b * BD + od;
 #pragma unroll
                 for (int j = 0; j < PL; j += 4) *(f4 *)(po + j) = (f4){o[j], o[j + 1], o[j + 2], o[j + 3]};
             }
         }
         if (on && (threadIdx.x & 15) == 0) {
             if (!direct) {
-                float *ml = a.part + (int64_t)a.b.n_tokens * a.heads * a.n_splits * DV + (row * a.n_splits + sp) * 2;
+                float *ml = a.part + (int64_t)a.b.n_tokens * a.heads * a.n_splits * D + (row * a.n_splits + sp) * 2;
                 ml[0] = Mo;
                 ml[1] = Lo;
             } else if (a.lse) a.lse[row] = Lo == 0.0f ? -__builtin_huge_valf() : (Mo + __log2f(Lo)) * 0.69314718055994531f;
@@ -390,11 +389,11 @@ __global__ __launch_bounds__(64) void k_attend_join(AttendArgs a) {
     if (a.lse && lane == 0) a.lse[row] = L == 0.0f ? -__builtin_huge_valf() : (M + __log2f(L)) * 0.69314718055994531f;
 }
 
-template <class T, bool MX, int DK, int DV, bool LATENT>
+template <class T, bool MX, int D>
 void few_t(const AttendArgs &a, hipStream_t st) {
     const int tiles = (a.b.max_q * a.group + 15) / 16;
     const dim3 grid((unsigned)a.n_splits * a.kv_heads * tiles, 1, a.b.n_seqs);
-    hipLaunchKernelGGL((k_attend_few<T, MX, DK, DV, 1, LATENT>), grid, dim3(64 * FEW_WAVES), 0, st, a);
+    hipLaunchKernelGGL((k_attend_few<T, MX, D, 1>), grid, dim3(64 * FEW_WAVES), 0, st, a);
 }
 
 template <class T, int DV>
@@ -405,15 +404,16 @@ void join_t(const AttendArgs &a, hipStream_t st) {
 } // namespace
 
 /* Columns (query rows of a kv head) from which the kernel of many rows is taken. */
-static bool takes_many(int64_t cols, bool latent) { return !latent && cols > 32; }
+static bool takes_many(int64_t cols) { return cols > 32; }
 
-/* Rows a split takes: enough workgroups for the 256 units, at least one step of every wave. */
+/* Rows a split takes: enough workgroups for the 256 units (as many as run at once), at least one
+ * step of every wave. */
 Split attend_split(int n_seqs, int max_q, int kv_cap, int heads, int kv_heads, bool latent) {
     const int64_t cols = (int64_t)max_q * (heads / kv_heads);
-    const bool many = takes_many(cols, latent);
-    const int64_t wgs = (int64_t)n_seqs * kv_heads * (many ? (cols + 127) / 128 : (cols + 15) / 16);
-    const int64_t want = std::max<int64_t>(1, (many ? 512 : 1024) / std::max<int64_t>(wgs, 1));
-    const int step = FEW_STEP * FEW_WAVES;
+    const bool many = !latent && takes_many(cols);
+    const int tile = latent ? 64 : many ? 128 : 16, step = latent ? 64 : FEW_STEP * FEW_WAVES, at_once = latent ? 256 : many ? 512 : 1024;
+    const int64_t wgs = std::max<int64_t>((int64_t)n_seqs * kv_heads * ((cols + tile - 1) / tile), 1);
+    const int64_t want = std::max<int64_t>(1, at_once / wgs);
     int64_t chunk = (kv_cap + want - 1) / want;
     chunk = std::max<int64_t>((chunk + step - 1) / step * step, step);
     return {(int)std::min<int64_t>(chunk, 0x40000000), std::max(1, (int)((kv_cap + chunk - 1) / chunk)), many};
@@ -422,7 +422,7 @@ Split attend_split(int n_seqs, int max_q, int kv_cap, int heads, int kv_heads, b
 void attend(const AttendArgs &a, int q_dtype, int cache_dtype, int width, bool many, hipStream_t st) {
     const bool mx = cache_dtype == DT_MX8;
 #define HXP_BY(F, T) (width == 64 ? F(T, 64) : width == 128 ? F(T, 128) : F(T, 256))
-#define HXP_FEW(T, D) (mx ? few_t<T, true, D, D, false>(a, st) : few_t<T, false, D, D, false>(a, st))
+#define HXP_FEW(T, D) (mx ? few_t<T, true, D>(a, st) : few_t<T, false, D>(a, st))
 #define HXP_JOIN(T, D) join_t<T, D>(a, st)
     if (many) attend_many(a, q_dtype, cache_dtype, width, st);
     else if (q_dtype == DT_BF16) HXP_BY(HXP_FEW, Bf16);
@@ -436,11 +436,7 @@ void attend(const AttendArgs &a, int q_dtype, int cache_dtype, int width, bool m
 }
 
 void attend_latent(const AttendArgs &a, int q_dtype, int cache_dtype, hipStream_t st) {
-    const bool mx = cache_dtype == DT_MX8;
-#define HXP_FEW(T) (mx ? few_t<T, true, 576, 512, true>(a, st) : few_t<T, false, 576, 512, true>(a, st))
-    if (q_dtype == DT_BF16) HXP_FEW(Bf16);
-    else HXP_FEW(F16);
-#undef HXP_FEW
+    latent_rows(a, q_dtype, cache_dtype == DT_MX8, st);
     if (a.n_splits == 1) return;
     if (q_dtype == DT_BF16) join_t<Bf16, 512>(a, st);
     else join_t<F16, 512>(a, st);
