@@ -130,6 +130,31 @@ __device__ __forceinline__ Seq seq_of(const Batch &b, int s) {
 
 __device__ __forceinline__ bool page_ok(const Batch &b, int id) { return (unsigned)id < (unsigned)b.n_pages; }
 
+/* Which of the 64 rows from t0 on a column attends: those below lim and, in a tree, the call's
+ * tokens of its mask row `words` (token j is row base + j); none from hi on. Two words are read a
+ * step: a load a score cost a tree's last steps 30 us. */
+__device__ __forceinline__ unsigned long long step_mask(int t0, int lim, int hi, int base, const unsigned long long *words, int n_words) {
+    const int n = lim - t0, h = hi - t0;
+    unsigned long long x = n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1;
+    if (words) {
+        const int64_t off = (int64_t)t0 - base;
+        if (off > -64 && off < 64 * (int64_t)n_words) {
+            const int k = (int)(off >> 6), sh = (int)(off & 63);   /* floor: k = -1 where the call's tokens begin inside the step */
+            const unsigned long long a = k >= 0 ? words[k] : 0, b = k + 1 < n_words ? words[k + 1] : 0;
+            x |= sh ? a >> sh | b << (64 - sh) : a;
+        }
+    }
+    return h >= 64 ? x : h <= 0 ? 0ull : x & ((1ull << h) - 1);
+}
+
+/* bits of 16 rows a page group each, from bits of groups */
+__device__ __forceinline__ unsigned long long group_rows(unsigned have) {
+    unsigned long long x = 0;
+#pragma unroll
+    for (int u = 0; u < 4; u++) x |= have >> u & 1 ? 0xffffull << (16 * u) : 0;
+    return x;
+}
+
 /* 16-bit types: the matrix instructions and conversions of one type */
 struct Bf16 {
     using v8 = b8;

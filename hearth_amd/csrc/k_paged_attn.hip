@@ -136,15 +136,11 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_attend_few(AttendArgs a) {
     const int hi = min(min(q.kv, a.b.mask ? q.kv : q.base + t_last + 1), (sp + 1) * a.chunk);
     const int full = a.b.mask ? q.base : q.base + t_first + 1;
 
-    /* whether column n of this lane attends row t of the sequence (if its page exists) */
-    auto attended = [&](int n, int t) {
-        bool v = t < lim[n];
-        if (a.b.mask && !v && tile * CT + 16 * n + lc < cols && t >= q.base && t < q.kv) {
-            const int nt = t - q.base;
-            v = (nt >> 6) < a.b.mask_words &&
-                (a.b.mask[(int64_t)(q.q0 + tok[n]) * a.b.mask_words + (nt >> 6)] >> (nt & 63) & 1);
-        }
-        return v && t < hi;
+    /* which of the 64 rows from t0 on column n of this lane attends (where their pages exist) */
+    auto attended = [&](int n, int t0) {
+        return step_mask(t0, lim[n], hi, q.base,
+                         a.b.mask && tile * CT + 16 * n + lc < cols ? a.b.mask + (int64_t)(q.q0 + tok[n]) * a.b.mask_words : nullptr,
+                         a.b.mask_words);
     };
 
     f4 acc[NT][NB * PL];
@@ -194,12 +190,9 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_attend_few(AttendArgs a) {
 #pragma unroll
             for (int j = 0; j < 8; j++) x[j] = s[j >> 2][n][j & 3] * a.scale2;
             if (!whole) {
+                const unsigned long long vis = (attended(n, t0) & group_rows((ok[0] ? 1u : 0u) | (ok[1] ? 2u : 0u))) >> (4 * g);
 #pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    const int t = t0 + 16 * (j >> 2) + 4 * g + (j & 3);
-                    const bool v = attended(n, t) && ok[j >> 2];
-                    x[j] = v ? x[j] : -__builtin_huge_valf();
-                }
+                for (int j = 0; j < 8; j++) x[j] = vis >> (16 * (j >> 2) + (j & 3)) & 1 ? x[j] : -__builtin_huge_valf();
             }
             float mx = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
             mx = fmaxf(m[n], max16(max32(mx)));
@@ -276,7 +269,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_attend_few(AttendArgs a) {
                             const unsigned x = row_elem<T, MX>(row, sc, b * BD + (4 * g + i) * PL + j);
 #pragma unroll
                             for (int n = 0; n < NT; n++)
-                                acc[n][b * PL + j][i] += T::odd(x) && attended(n, t) ? T::wide(x) : 0.0f;
+                                acc[n][b * PL + j][i] += T::odd(x) && (attended(n, t) & 1) ? T::wide(x) : 0.0f;
                         }
             }
         }

@@ -89,15 +89,9 @@ __global__ __launch_bounds__(L_THREADS, 2) void k_attend_latent(AttendArgs a) {
     const int hi = min(min(q.kv, a.b.mask ? q.kv : q.base + t_last + 1), (sp + 1) * a.chunk);
     const int full = a.b.mask ? q.base : q.base + tile * L_COLS / a.heads + 1;
     const int lo = sp * a.chunk;
-    auto attended = [&](int t) {
-        bool v = t < lim;
-        if (a.b.mask && !v && on && t >= q.base && t < q.kv) {
-            const int nt = t - q.base;
-            v = (nt >> 6) < a.b.mask_words &&
-                (a.b.mask[(int64_t)(q.q0 + tok) * a.b.mask_words + (nt >> 6)] >> (nt & 63) & 1);
-        }
-        return v && t < hi;
-    };
+    /* which of the 64 rows from t0 on this lane's column attends (where their pages exist) */
+    const unsigned long long *words = a.b.mask && on ? a.b.mask + (int64_t)(q.q0 + tok) * a.b.mask_words : nullptr;
+    auto attended = [&](int t0) { return step_mask(t0, lim, hi, q.base, words, a.b.mask_words); };
 
     f4 acc[DT];
 #pragma unroll
@@ -193,7 +187,7 @@ __global__ __launch_bounds__(L_THREADS, 2) void k_attend_latent(AttendArgs a) {
                     }
                 }
         }
-        return odd;
+        return odd && t0 + L_ROWS > full;
     };
 
     unsigned have_now = 0, have_next = 0;
@@ -236,11 +230,9 @@ __global__ __launch_bounds__(L_THREADS, 2) void k_attend_latent(AttendArgs a) {
 #pragma unroll
         for (int j = 0; j < 8; j++) x[j] = s[j >> 2][j & 3] * a.scale2;
         if (edge) {
+            const unsigned long long vis = (attended(t0) & group_rows(have_now)) >> (r0 + 4 * g);
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const int r = r0 + 16 * (j >> 2) + 4 * g + (j & 3);
-                x[j] = attended(t0 + r) && (have_now >> (r >> 4) & 1) ? x[j] : NINF;
-            }
+            for (int j = 0; j < 8; j++) x[j] = vis >> (16 * (j >> 2) + (j & 3)) & 1 ? x[j] : NINF;
             if (__syncthreads_or(odd_now)) {
                 /* an infinity or NaN among rows that some columns do not attend would reach them as
                  * 0 * inf: the scores are done with the rows, so it is taken out of LDS and added
@@ -298,7 +290,7 @@ __global__ __launch_bounds__(L_THREADS, 2) void k_attend_latent(AttendArgs a) {
 #pragma unroll 1
         for (int t = max(lo, full / L_ROWS * L_ROWS); t < hi; t++) {
             const int id = pages[t >> a.b.page_shift];
-            if (!page_ok(a.b, id) || !attended(t)) continue;
+            if (!page_ok(a.b, id) || !(attended(t) & 1)) continue;
             const uint8_t *row = a.k.data + (int64_t)id * a.k.page_stride + (int64_t)(t & rmask) * (LW * (MX ? 1 : 2));
             const uint8_t *sc = MX ? a.k.scales + (int64_t)id * a.k.scale_page_stride + (t & rmask) * (LW / MX_BLOCK) : nullptr;
 #pragma unroll 1

@@ -101,16 +101,9 @@ __global__ __launch_bounds__(64 * MANY_WAVES, D <= 128 ? 2 : 1) void k_attend_ma
     const int full = a.b.mask ? q.base : q.base + tile * MANY_COLS / a.group + 1;
     const int lo = sp * a.chunk;
 
-    /* whether this lane's column attends row t of the sequence (if its page exists) */
-    auto attended = [&](int t) {
-        bool v = t < lim;
-        if (a.b.mask && !v && on && t >= q.base && t < q.kv) {
-            const int nt = t - q.base;
-            v = (nt >> 6) < a.b.mask_words &&
-                (a.b.mask[(int64_t)(q.q0 + tok) * a.b.mask_words + (nt >> 6)] >> (nt & 63) & 1);
-        }
-        return v && t < hi;
-    };
+    /* which of the 64 rows from t0 on this lane's column attends (where their pages exist) */
+    const unsigned long long *words = a.b.mask && on ? a.b.mask + (int64_t)(q.q0 + tok) * a.b.mask_words : nullptr;
+    auto attended = [&](int t0) { return step_mask(t0, lim, hi, q.base, words, a.b.mask_words); };
 
     f16v acc[DT];
 #pragma unroll
@@ -140,34 +133,54 @@ __global__ __launch_bounds__(64 * MANY_WAVES, D <= 128 ? 2 : 1) void k_attend_ma
         for (int u = 1; u < M::GROUPS; u++) id = r >> 4 == u ? pid[u] : id;
         return id;
     };
-    const bool st_v = (int)threadIdx.x < M::VI, st_on = (int)threadIdx.x < 2 * M::VI;
-    const int st_it = st_v ? threadIdx.x : threadIdx.x - M::VI, st_e = M::elem_of(st_v, st_it);
+    /* what this thread brings in (whole waves bring in V, whole waves K) */
+    const bool st_v = 64 * wave < M::VI, st_on = 64 * wave < 2 * M::VI;
+    const int st_it = st_v ? threadIdx.x : threadIdx.x - M::VI, st_e = M::elem_of(st_v, st_it), st_r = M::row_of(st_v, st_it, 0);
     const uint8_t *st_base = st_v ? vbase : kbase, *st_sb = st_v ? vsb : ksb;
     const int64_t st_ps = st_v ? a.v.page_stride : a.k.page_stride, st_ss = st_v ? a.v.scale_page_stride : a.k.scale_page_stride;
+    constexpr int ES = MX ? 1 : 2;
+    const bool one_page = rmask >= M::ROWS - 1;   /* a step lies in one page */
     typename M::Stage st;
+    auto fetch = [&](int j, const uint8_t *p, const uint8_t *sp) {
+        if constexpr (MX) {
+            const u2 x = *(const u2 *)p;
+            st.w[j] = (u4){x[0], x[1], 0, 0};
+            st.s[j] = *sp;
+        } else {
+            st.w[j] = *(const u4 *)p;
+        }
+    };
+    /* Every load goes to a row of the cache: rows past hi lie in the same page, those of a page that
+     * is not there are taken from page 0; store clears both. */
     auto load = [&](int t0) {
         if (!st_on) return;
+        if (one_page) {
+            const int id = max(pid[0], 0), row = t0 & rmask;
+            const uint8_t *p = st_base + (int64_t)id * st_ps + row * (D * ES);
+            const uint8_t *sp = MX ? st_sb + (int64_t)id * st_ss + row * (D / MX_BLOCK) : nullptr;
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const int r = M::row_of(st_v, st_it, j), id = page_of(r);
-            st.w[j] = (u4){0, 0, 0, 0};
-            st.s[j] = 127;
-            if (id >= 0 && t0 + r < hi) {
-                const int el = ((t0 + r) & rmask) * D + st_e;
-                const uint8_t *base = st_base + (int64_t)id * st_ps;
-                if constexpr (MX) {
-                    const u2 x = *(const u2 *)(base + el);
-                    st.w[j] = (u4){x[0], x[1], 0, 0};
-                    st.s[j] = (st_sb + (int64_t)id * st_ss)[el / MX_BLOCK];
-                } else {
-                    st.w[j] = *(const u4 *)(base + 2 * (int64_t)el);
-                }
+            for (int j = 0; j < 8; j++) {
+                const int dr = st_v ? (j & 3) + 8 * (j >> 2) : M::ROWS / 8 * j;
+                fetch(j, p + (st_r + dr) * (D * ES) + st_e * ES, sp + (st_r + dr) * (D / MX_BLOCK) + st_e / MX_BLOCK);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const int r = M::row_of(st_v, st_it, j), id = max(page_of(r), 0), row = (t0 + r) & rmask;
+                fetch(j, st_base + (int64_t)id * st_ps + row * (D * ES) + st_e * ES,
+                      MX ? st_sb + (int64_t)id * st_ss + row * (D / MX_BLOCK) + st_e / MX_BLOCK : nullptr);
             }
         }
     };
-    /* The loaded rows into LDS. `some`: rows that some columns do not attend; an infinity or NaN
-     * of V there would reach them as 0 * inf, so it is left out and added at the end. */
-    auto store = [&](int buf, bool some) {
+    /* whether some column of the workgroup may not attend every row of the step at t0 (pages: bit
+     * u where group u has one) */
+    auto edge_at = [&](int t0, unsigned have) {
+        return !(t0 + M::ROWS <= full && t0 + M::ROWS <= hi && have == (1u << M::GROUPS) - 1);
+    };
+    /* The loaded rows of the step at t0 into LDS. Past `full` (rows that some columns do not attend)
+     * an infinity or NaN of V would reach those columns as 0 * inf, so it is left out and added at
+     * the end; rows that do not exist are cleared. */
+    auto store = [&](int buf, int t0, unsigned have) {
         if (!st_on) return;
         uint8_t *kb = lds + buf * M::KB, *vb = lds + 2 * M::KB + buf * M::VB;
         u4 w[8];
@@ -183,15 +196,19 @@ __global__ __launch_bounds__(64 * MANY_WAVES, D <= 128 ? 2 : 1) void k_attend_ma
             }
         }
         if (st_v) {
-            if (some) {
+            if (edge_at(t0, have)) {
+                const bool some = t0 + M::ROWS > full;
                 bool odd = false;
 #pragma unroll
-                for (int j = 0; j < 8; j++)
+                for (int j = 0; j < 8; j++) {
+                    const int r = M::row_of(true, st_it, j);
+                    const bool ok = t0 + r < hi && (have >> (r >> 4) & 1);
 #pragma unroll
                     for (int k = 0; k < 4; k++) {
-                        odd = odd || T::odd(w[j][k]);
-                        w[j][k] = T::clean(w[j][k]);
+                        odd = odd || (ok && some && T::odd(w[j][k]));
+                        w[j][k] = ok ? some ? T::clean(w[j][k]) : w[j][k] : 0u;
                     }
+                }
                 if (odd) odd_flag = 1;
             }
             uint8_t *p = vb + (st_e * M::VLD + st_it % (M::ROWS / 8) * 8) * 2;
@@ -207,12 +224,6 @@ __global__ __launch_bounds__(64 * MANY_WAVES, D <= 128 ? 2 : 1) void k_attend_ma
             for (int j = 0; j < 8; j++) *(u4 *)(kb + (M::row_of(false, st_it, j) * M::KLD + st_e) * 2) = w[j];
         }
     };
-    /* whether some column of the workgroup may not attend every row of the step at t0 (pages: bit
-     * u where group u has one) */
-    auto edge_at = [&](int t0, unsigned have) {
-        return !(t0 + M::ROWS <= full && t0 + M::ROWS <= hi && have == (1u << M::GROUPS) - 1);
-    };
-
     if (threadIdx.x == 0) odd_flag = 0;
     unsigned have_now = 0, have_next = 0;   /* bit u: group u has a page */
     auto have = [&] {
@@ -226,7 +237,7 @@ __global__ __launch_bounds__(64 * MANY_WAVES, D <= 128 ? 2 : 1) void k_attend_ma
         load_pages(lo);
         have_next = have();
         load(lo);
-        store(0, lo + M::ROWS > full);
+        store(0, lo, have_next);
         if (lo + M::ROWS < hi) load_pages(lo + M::ROWS);
     }
     __syncthreads();
@@ -264,13 +275,12 @@ __global__ __launch_bounds__(64 * MANY_WAVES, D <= 128 ? 2 : 1) void k_attend_ma
             mx = max32(mx) * scale2;
         } else {
             mx = NINF;
+            const unsigned long long vis = (attended(t0) & group_rows(have_now)) >> (4 * half);
 #pragma unroll
             for (int u = 0; u < M::TILES; u++)
 #pragma unroll
                 for (int j = 0; j < 16; j++) {
-                    const int r = 32 * u + 8 * (j >> 2) + 4 * half + (j & 3), t = t0 + r;
-                    const bool v = attended(t) && (have_now >> (r >> 4) & 1);
-                    s[u][j] = v ? s[u][j] * scale2 : NINF;
+                    s[u][j] = vis >> (32 * u + 8 * (j >> 2) + (j & 3)) & 1 ? s[u][j] * scale2 : NINF;
                     mx = fmaxf(mx, s[u][j]);
                 }
             mx = max32(mx);
@@ -306,7 +316,7 @@ __global__ __launch_bounds__(64 * MANY_WAVES, D <= 128 ? 2 : 1) void k_attend_ma
 #pragma unroll
             for (int i = 0; i < DT; i++)
                 acc[i] = T::mfma32(*(const v8 *)(vb + ((32 * i + lc) * M::VLD + 16 * g + 8 * half) * 2), pf[g], acc[i]);
-        if (more) store(buf ^ 1, t0 + 2 * M::ROWS > full);
+        if (more) store(buf ^ 1, t0 + M::ROWS, have_next);
         __syncthreads();
     }
 
@@ -315,7 +325,7 @@ __global__ __launch_bounds__(64 * MANY_WAVES, D <= 128 ? 2 : 1) void k_attend_ma
         for (int t = max(lo, full / M::ROWS * M::ROWS); t < hi; t++) {
             const int id = pages[t >> a.b.page_shift];
             if (!page_ok(a.b, id)) continue;
-            const bool add = attended(t);
+            const bool add = attended(t) & 1;
             const uint8_t *row = vbase + (int64_t)id * a.v.page_stride + (int64_t)(t & rmask) * (D * (MX ? 1 : 2));
             const uint8_t *sc = MX ? vsb + (int64_t)id * a.v.scale_page_stride + (t & rmask) * (D / MX_BLOCK) : nullptr;
 #pragma unroll

@@ -371,6 +371,18 @@ def test_nan_and_infinity_in_rows_not_attended(latent, store, long):
 
 
 @pytest.mark.parametrize("latent", [False, True])
+@pytest.mark.parametrize("heads", [4, 64])
+def test_infinity_beside_a_missing_page(latent, heads):
+    """A step that lacks a page and whose other rows everyone attends keeps their infinities."""
+    pages = torch.tensor([[0, 77, 2, 3, 4, 5, 1, 6]], dtype=torch.int32)
+
+    def edit(c, pages):
+        c["k" if latent else "v"][2, :, 3, 7] = math.inf
+
+    run_attend(_gen(14), BF, "bf16", heads, 1, 64, [128], [2], 16, pages=pages, n_pages=7, latent=latent, edit=edit)
+
+
+@pytest.mark.parametrize("latent", [False, True])
 def test_bad_pages_count_as_masked(latent):
     g = _gen(4)
     pages = torch.tensor([[0, 77, 2, 3], [1, 4, -1, 5], [88, 88, 88, 88]], dtype=torch.int32)
