@@ -6,11 +6,12 @@
  * the 32 x 32 x 16 matrix instruction: a wave owns 32 columns ((token, head) pairs of the kv
  * head's group), a lane half of one column's scores, so the softmax needs one exchange between
  * lanes l and l ^ 32, and the scores' registers, packed, are the second product's operand.
- * Four waves (128 columns) share 64 cache rows (32 of width 256) at a time through LDS: K by rows, V transposed on
- * the way in (8 rows x 8 elements a thread, byte permutations) with the rows of each group of 16
- * in the order in which a lane's scores hold them (0-3 8-11 | 4-7 12-15), both padded by 16 bytes
- * a row against bank conflicts, double-buffered; the next step's loads are in flight while
- * this one is worked on. 8-bit rows become 16-bit ones on the way into LDS, once for the four waves.
+ * Four waves (128 columns) share 64 cache rows (32 of width 256) at a time through LDS, K and V as
+ * they lie in memory: the scores read K along its rows, the sums read V through the transposing
+ * LDS load. The 16-byte pieces of a row are exchanged by row (piece p of row r at p ^ swz(r)), so
+ * that neither read meets a bank conflict. 16-bit rows go from memory to LDS directly, 8-bit rows
+ * through registers, where they become 16-bit ones once for the four waves; the next step's are
+ * in flight while this one is worked on (two buffers).
  */
 #include "hx_paged.h"
 
@@ -22,42 +23,39 @@ namespace {
 
 constexpr int MANY_WAVES = 4, MANY_COLS = 32 * MANY_WAVES;
 
-__device__ __forceinline__ unsigned lo16(unsigned a, unsigned b) { return __builtin_amdgcn_perm(b, a, 0x05040100u); }
-__device__ __forceinline__ unsigned hi16(unsigned a, unsigned b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
-
-template <class T, bool MX, int D>
+template <int D>
 struct Many {
-    static constexpr int ROWS = D <= 128 ? 64 : 32;               /* cache rows of a step */
-    static constexpr int KLD = D + 8, VLD = ROWS + 8;             /* LDS rows, elements */
-    static constexpr int KB = ROWS * KLD * 2, VB = D * VLD * 2;   /* bytes of a buffer */
-    static constexpr int LDS = 2 * (KB + VB);
-    static constexpr int VI = D * ROWS / 64;                      /* threads that bring in V; as many bring in K */
+    static constexpr int ROWS = D <= 128 ? 64 : 32;        /* cache rows of a step */
+    static constexpr int PIECES = D / 8;                   /* 16-byte pieces of a row in LDS */
+    static constexpr int TILE = ROWS * D * 2;              /* bytes of K or V of a step */
     static constexpr int GROUPS = ROWS / 16, TILES = ROWS / 32;
-    static_assert(2 * VI <= 64 * MANY_WAVES, "a thread takes one item");
 
-    struct Stage {
-        u4 w[8];     /* MX: codes in the first two words */
-        unsigned s[8];
-    };
-
-    /* row of the tile that piece j of item `it` reads (V: rows of one operand chunk) */
-    static __device__ __forceinline__ int row_of(bool v, int it, int j) {
-        if (v) {
-            const int c = it % (ROWS / 8);             /* chunk: group of 16, half */
-            return (c >> 1) * 16 + (c & 1) * 4 + (j & 3) + (j >> 2) * 8;
-        }
-        return it / (D / 8) + ROWS / 8 * j;
+    /* Exchange of a row's pieces. Scores: 16 lanes read the same piece of 16 rows, which must fall
+     * into 16 different 16-byte columns of the 256 bytes of banks. Sums: 32 lanes read 4 pieces
+     * (aligned) of 4 rows, whose groups of 4 must differ. Rows of 128 bytes alternate between the
+     * halves of the banks by themselves. */
+    static __device__ __forceinline__ int swz(int r) {
+        if constexpr (D == 64) { const int k = r >> 1 & 7; return (k & 1) << 2 | k >> 1; }
+        else return (r & 3) << 2 | (r >> 2 & 3);
     }
-    static __device__ __forceinline__ int elem_of(bool v, int it) { return v ? it / (ROWS / 8) * 8 : it % (D / 8) * 8; }
+    static __device__ __forceinline__ int at(int r, int p) { return (r * PIECES + (p ^ swz(r))) * 16; }
 };
+
+typedef short s4v __attribute__((ext_vector_type(4)));
+
+/* transposing LDS load: lane i of 16 gives the address of 4 elements of row i / 4 and gets element
+ * i of the four rows */
+__device__ __forceinline__ u2 read_tr(const uint8_t *p) {
+    return __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4v *)p));
+}
 
 template <class T, bool MX, int D>
 __global__ __launch_bounds__(64 * MANY_WAVES, D <= 128 ? 2 : 1) void k_attend_many(AttendArgs a) {
-    using M = Many<T, MX, D>;
+    using M = Many<D>;
     using v8 = typename T::v8;
     constexpr int KS = D / 16, DT = D / 32;
     constexpr float NINF = -__builtin_huge_valf();
-    __shared__ __align__(16) uint8_t lds[M::LDS];
+    __shared__ __align__(16) uint8_t lds[2][2][M::TILE];   /* buffer, K or V */
     __shared__ int odd_flag;
 
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -118,57 +116,48 @@ __global__ __launch_bounds__(64 * MANY_WAVES, D <= 128 ? 2 : 1) void k_attend_ma
     const uint8_t *ksb = MX ? a.k.scales + (int64_t)kvh * a.k.scale_head_stride : nullptr;
     const uint8_t *vsb = MX ? a.v.scales + (int64_t)kvh * a.v.scale_head_stride : nullptr;
 
-    int pid[M::GROUPS];              /* pages of the groups of 16 rows, -1: none */
+    int pid[4];                      /* pages of the groups of 16 rows, -1: none */
     auto load_pages = [&](int t0) {
 #pragma unroll
-        for (int u = 0; u < M::GROUPS; u++) {
+        for (int u = 0; u < 4; u++) {
             const int t = t0 + 16 * u;
-            const int id = t < hi ? pages[t >> a.b.page_shift] : -1;
+            const int id = u < M::GROUPS && t < hi ? pages[t >> a.b.page_shift] : -1;
             pid[u] = page_ok(a.b, id) ? id : -1;
         }
     };
     auto page_of = [&](int r) {
-        int id = pid[0];
-#pragma unroll
-        for (int u = 1; u < M::GROUPS; u++) id = r >> 4 == u ? pid[u] : id;
-        return id;
+        const int u = r >> 4;
+        return u == 0 ? pid[0] : u == 1 ? pid[1] : u == 2 ? pid[2] : pid[3];
     };
-    /* what this thread brings in (whole waves bring in V, whole waves K) */
-    const bool st_v = 64 * wave < M::VI, st_on = 64 * wave < 2 * M::VI;
-    const int st_it = st_v ? threadIdx.x : threadIdx.x - M::VI, st_e = M::elem_of(st_v, st_it), st_r = M::row_of(st_v, st_it, 0);
-    const uint8_t *st_base = st_v ? vbase : kbase, *st_sb = st_v ? vsb : ksb;
-    const int64_t st_ps = st_v ? a.v.page_stride : a.k.page_stride, st_ss = st_v ? a.v.scale_page_stride : a.k.scale_page_stride;
-    constexpr int ES = MX ? 1 : 2;
+    /* Pieces that a thread brings in: half of K, half of V. 16-bit: a 16-byte piece of LDS each,
+     * in lane order; 8-bit: 16 codes, two pieces. */
+    constexpr int PER = MX ? 2 : 1, N = 2 * M::ROWS * M::PIECES / PER / 256, RP = M::PIECES / PER;   /* RP: of a row */
+    static_assert(N % 2 == 0 && N >= 2, "K and V alike");
     const bool one_page = rmask >= M::ROWS - 1;   /* a step lies in one page */
-    typename M::Stage st;
-    auto fetch = [&](int j, const uint8_t *p, const uint8_t *sp) {
-        if constexpr (MX) {
-            const u2 x = *(const u2 *)p;
-            st.w[j] = (u4){x[0], x[1], 0, 0};
-            st.s[j] = *sp;
-        } else {
-            st.w[j] = *(const u4 *)p;
-        }
+    u4 sw[MX ? N : 1];
+    unsigned ss[MX ? N : 1];
+    auto place = [&](int z, int &r, int &p) {
+        const int idx = (wave * (N / 2) + z % (N / 2)) * 64 + lane;
+        r = idx / RP;
+        p = idx % RP;
     };
     /* Every load goes to a row of the cache: rows past hi lie in the same page, those of a page that
-     * is not there are taken from page 0; store clears both. */
-    auto load = [&](int t0) {
-        if (!st_on) return;
-        if (one_page) {
-            const int id = max(pid[0], 0), row = t0 & rmask;
-            const uint8_t *p = st_base + (int64_t)id * st_ps + row * (D * ES);
-            const uint8_t *sp = MX ? st_sb + (int64_t)id * st_ss + row * (D / MX_BLOCK) : nullptr;
+     * is not there are taken from page 0; settle clears both. */
+    auto load = [&](int t0, int buf) {
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const int dr = st_v ? (j & 3) + 8 * (j >> 2) : M::ROWS / 8 * j;
-                fetch(j, p + (st_r + dr) * (D * ES) + st_e * ES, sp + (st_r + dr) * (D / MX_BLOCK) + st_e / MX_BLOCK);
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const int r = M::row_of(st_v, st_it, j), id = max(page_of(r), 0), row = (t0 + r) & rmask;
-                fetch(j, st_base + (int64_t)id * st_ps + row * (D * ES) + st_e * ES,
-                      MX ? st_sb + (int64_t)id * st_ss + row * (D / MX_BLOCK) + st_e / MX_BLOCK : nullptr);
+        for (int z = 0; z < N; z++) {
+            const bool v = z >= N / 2;
+            int r, p;
+            place(z, r, p);
+            const int id = max(one_page ? pid[0] : page_of(r), 0), row = one_page ? (t0 & rmask) + r : (t0 + r) & rmask;
+            const uint8_t *base = (v ? vbase : kbase) + (int64_t)id * (v ? a.v.page_stride : a.k.page_stride);
+            if constexpr (MX) {
+                sw[z] = *(const u4 *)(base + row * D + 16 * p);
+                ss[z] = ((v ? vsb : ksb) + (int64_t)id * (v ? a.v.scale_page_stride : a.k.scale_page_stride))[row * (D / MX_BLOCK) + (p >> 1)];
+            } else {
+                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(base + (row * D + 8 * (p ^ M::swz(r))) * 2),
+                                                 (__attribute__((address_space(3))) void *)(lds[buf][v] + (wave * (N / 2) + z % (N / 2)) * 1024),
+                                                 16, 0, 0);
             }
         }
     };
@@ -177,81 +166,74 @@ __global__ __launch_bounds__(64 * MANY_WAVES, D <= 128 ? 2 : 1) void k_attend_ma
     auto edge_at = [&](int t0, unsigned have) {
         return !(t0 + M::ROWS <= full && t0 + M::ROWS <= hi && have == (1u << M::GROUPS) - 1);
     };
-    /* The loaded rows of the step at t0 into LDS. Past `full` (rows that some columns do not attend)
-     * an infinity or NaN of V would reach those columns as 0 * inf, so it is left out and added at
-     * the end; rows that do not exist are cleared. */
-    auto store = [&](int buf, int t0, unsigned have) {
-        if (!st_on) return;
-        uint8_t *kb = lds + buf * M::KB, *vb = lds + 2 * M::KB + buf * M::VB;
-        u4 w[8];
+    /* The loaded step made ready in LDS. Past `full` (rows that some columns do not attend) an
+     * infinity or NaN of V would reach those columns as 0 * inf, so it is left out and added at the
+     * end; rows that do not exist are cleared. */
+    auto settle = [&](int buf, int t0, unsigned have) {
+        const bool edge = edge_at(t0, have), some = t0 + M::ROWS > full;
+        bool odd = false;
+        auto clear = [&](int r, const u4 x) {
+            const bool ok = t0 + r < hi && (have >> (r >> 4) & 1);
+            odd = odd || (ok && some && (T::odd(x[0]) || T::odd(x[1]) || T::odd(x[2]) || T::odd(x[3])));
+            const u4 y = some ? (u4){T::clean(x[0]), T::clean(x[1]), T::clean(x[2]), T::clean(x[3])} : x;
+            return ok ? y : (u4){0, 0, 0, 0};
+        };
+        if constexpr (MX) {
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            if constexpr (MX) {
-                const float f = mx_scale(st.s[j]);
-                const unsigned x = st.w[j][0], y = st.w[j][1];
-                w[j] = (u4){T::template from_mx8<false>(x, f), T::template from_mx8<true>(x, f),
+            for (int z = 0; z < N; z++) {
+                int r, p;
+                place(z, r, p);
+                const float f = mx_scale(ss[z]);
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const unsigned x = sw[z][2 * h], y = sw[z][2 * h + 1];
+                    u4 w = {T::template from_mx8<false>(x, f), T::template from_mx8<true>(x, f),
                             T::template from_mx8<false>(y, f), T::template from_mx8<true>(y, f)};
-            } else {
-                w[j] = st.w[j];
-            }
-        }
-        if (st_v) {
-            if (edge_at(t0, have)) {
-                const bool some = t0 + M::ROWS > full;
-                bool odd = false;
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    const int r = M::row_of(true, st_it, j);
-                    const bool ok = t0 + r < hi && (have >> (r >> 4) & 1);
-#pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        odd = odd || (ok && some && T::odd(w[j][k]));
-                        w[j][k] = ok ? some ? T::clean(w[j][k]) : w[j][k] : 0u;
-                    }
+                    if (z >= N / 2 && edge) w = clear(r, w);
+                    *(u4 *)(lds[buf][z >= N / 2] + M::at(r, 2 * p + h)) = w;
                 }
-                if (odd) odd_flag = 1;
-            }
-            uint8_t *p = vb + (st_e * M::VLD + st_it % (M::ROWS / 8) * 8) * 2;
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                *(u4 *)(p + 4 * k * M::VLD) =
-                    (u4){lo16(w[0][k], w[1][k]), lo16(w[2][k], w[3][k]), lo16(w[4][k], w[5][k]), lo16(w[6][k], w[7][k])};
-                *(u4 *)(p + (4 * k + 2) * M::VLD) =
-                    (u4){hi16(w[0][k], w[1][k]), hi16(w[2][k], w[3][k]), hi16(w[4][k], w[5][k]), hi16(w[6][k], w[7][k])};
             }
         } else {
-#pragma unroll
-            for (int j = 0; j < 8; j++) *(u4 *)(kb + (M::row_of(false, st_it, j) * M::KLD + st_e) * 2) = w[j];
+            __builtin_amdgcn_s_waitcnt(0x0f70);   /* vmcnt(0): this thread's pieces have arrived */
+            if (edge)
+#pragma unroll 1
+                for (int z = 0; z < N / 2; z++) {
+                    int r, p;
+                    place(z, r, p);
+                    u4 *x = (u4 *)(lds[buf][1] + ((wave * (N / 2) + z) * 64 + lane) * 16);
+                    *x = clear(r, *x);
+                }
         }
+        if (odd) odd_flag = 1;
     };
     if (threadIdx.x == 0) odd_flag = 0;
     unsigned have_now = 0, have_next = 0;   /* bit u: group u has a page */
-    auto have = [&] {
-        unsigned b = 0;
-#pragma unroll
-        for (int u = 0; u < M::GROUPS; u++) b |= pid[u] >= 0 ? 1u << u : 0u;
-        return b;
-    };
+    auto have = [&] { return (pid[0] >= 0 ? 1u : 0u) | (pid[1] >= 0 ? 2u : 0u) | (pid[2] >= 0 ? 4u : 0u) | (pid[3] >= 0 ? 8u : 0u); };
     __syncthreads();
     if (lo < hi) {
         load_pages(lo);
         have_next = have();
-        load(lo);
-        store(0, lo, have_next);
+        load(lo, 0);
+        settle(0, lo, have_next);
         if (lo + M::ROWS < hi) load_pages(lo + M::ROWS);
     }
     __syncthreads();
 
+    /* Byte addresses in K and V of a step: scores read row 32 u + lc, pieces 2 i + half (an exclusive
+     * or with 32 i); sums read rows 16 g + 4 half .. + 3 and 8 further, elements 32 i .. 32 i + 31
+     * (with 64 i) */
+    const int vr = 4 * half + ((lane & 15) >> 2), vp = 2 * (lane >> 4 & 1) + (lane >> 1 & 1);
+    const int k_at = M::at(lc, half), v_at[2] = {M::at(vr, vp) + 8 * (lane & 1), M::at(vr + 8, vp) + 8 * (lane & 1)};
     int buf = 0;
     for (int t0 = lo; t0 < hi; t0 += M::ROWS, buf ^= 1) {
         const bool more = t0 + M::ROWS < hi;
         have_now = have_next;
         if (more) {
             have_next = have();
-            load(t0 + M::ROWS);
+            load(t0 + M::ROWS, buf ^ 1);
             if (t0 + 2 * M::ROWS < hi) load_pages(t0 + 2 * M::ROWS);
         }
-        const uint8_t *kb = lds + buf * M::KB, *vb = lds + 2 * M::KB + buf * M::VB;
+        const uint8_t *kb = lds[buf][0], *vb = lds[buf][1];
         f16v s[M::TILES];
 #pragma unroll
         for (int u = 0; u < M::TILES; u++)
@@ -261,7 +243,7 @@ __global__ __launch_bounds__(64 * MANY_WAVES, D <= 128 ? 2 : 1) void k_attend_ma
         for (int i = 0; i < KS; i++)
 #pragma unroll
             for (int u = 0; u < M::TILES; u++)
-                s[u] = T::mfma32(*(const v8 *)(kb + ((32 * u + lc) * M::KLD + 16 * i + 8 * half) * 2), qf[i], s[u]);
+                s[u] = T::mfma32(*(const v8 *)(kb + (k_at ^ 32 * i) + 32 * u * (2 * D)), qf[i], s[u]);
 
         const bool edge = edge_at(t0, have_now);
         v8 pf[M::GROUPS];
@@ -314,9 +296,11 @@ __global__ __launch_bounds__(64 * MANY_WAVES, D <= 128 ? 2 : 1) void k_attend_ma
 #pragma unroll
         for (int g = 0; g < M::GROUPS; g++)
 #pragma unroll
-            for (int i = 0; i < DT; i++)
-                acc[i] = T::mfma32(*(const v8 *)(vb + ((32 * i + lc) * M::VLD + 16 * g + 8 * half) * 2), pf[g], acc[i]);
-        if (more) store(buf ^ 1, t0 + M::ROWS, have_next);
+            for (int i = 0; i < DT; i++) {
+                const u2 x = read_tr(vb + (v_at[0] ^ 64 * i) + 16 * g * (2 * D)), y = read_tr(vb + (v_at[1] ^ 64 * i) + 16 * g * (2 * D));
+                acc[i] = T::mfma32(__builtin_bit_cast(v8, (u4){x[0], x[1], y[0], y[1]}), pf[g], acc[i]);
+            }
+        if (more) settle(buf ^ 1, t0 + M::ROWS, have_next);
         __syncthreads();
     }
 
