@@ -110,6 +110,10 @@ void attend_latent(const AttendArgs &a, int q_dtype, int cache_dtype, hipStream_
 
 /* ------------------------------------------------------------------ device helpers */
 
+/* A word that the whole workgroup reads and no kernel of the call writes, through the scalar cache:
+ * a vector load's wait would wait for every row load issued before it as well. */
+__device__ __forceinline__ int word_of(const int *p, int64_t i) { return ((const __attribute__((address_space(4))) int *)p)[i]; }
+
 struct Seq {
     int q0, n;       /* first token of the call, tokens */
     int kv;          /* rows that exist */
@@ -118,9 +122,9 @@ struct Seq {
 
 __device__ __forceinline__ Seq seq_of(const Batch &b, int s) {
     Seq r;
-    const int lo = min(max(b.q_start[s], 0), b.n_tokens);
-    const int hi = min(max(b.q_start[s + 1], lo), b.n_tokens);
-    const int len = max(b.kv_len[s], 0);
+    const int lo = min(max(word_of(b.q_start, s), 0), b.n_tokens);
+    const int hi = min(max(word_of(b.q_start, s + 1), lo), b.n_tokens);
+    const int len = max(word_of(b.kv_len, s), 0);
     r.q0 = lo;
     r.n = hi - lo;
     r.kv = min(len, b.kv_cap);

@@ -167,7 +167,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_attend_few(AttendArgs a) {
 #pragma unroll
         for (int u = 0; u < 2; u++) {
             const int t = t0 + 16 * u;
-            pid[u] = t < hi ? pages[t >> a.b.page_shift] : -1;
+            pid[u] = t < hi ? word_of(pages, t >> a.b.page_shift) : -1;
             ok[u] = page_ok(a.b, pid[u]);
         }
         f4 s[2][NT];
@@ -254,9 +254,9 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_attend_few(AttendArgs a) {
         for (int t0 = sp * a.chunk + FEW_STEP * wave; t0 < hi; t0 += FEW_STEP * FEW_WAVES) {
 #pragma unroll 1
             for (int t = t0; t < min(t0 + FEW_STEP, hi); t++) {
-                const int id = pages[t >> a.b.page_shift];
-                if (t0 + FEW_STEP <= full && t0 + FEW_STEP <= hi && page_ok(a.b, pages[t0 >> a.b.page_shift]) &&
-                    page_ok(a.b, pages[(t0 + 16) >> a.b.page_shift])) break;   /* a step taken as it is */
+                const int id = word_of(pages, t >> a.b.page_shift);
+                if (t0 + FEW_STEP <= full && t0 + FEW_STEP <= hi && page_ok(a.b, word_of(pages, t0 >> a.b.page_shift)) &&
+                    page_ok(a.b, word_of(pages, (t0 + 16) >> a.b.page_shift))) break;   /* a step taken as it is */
                 if (!page_ok(a.b, id)) continue;
                 const uint8_t *row = vbase + (int64_t)id * vr.page_stride + (int64_t)(t & (page_rows - 1)) * (D * ES);
                 const uint8_t *sc = MX ? vsb + (int64_t)id * vr.scale_page_stride + (t & (page_rows - 1)) * (D / MX_BLOCK) : nullptr;

@@ -105,7 +105,7 @@ __global__ __launch_bounds__(L_THREADS, 2) void k_attend_latent(AttendArgs a) {
 #pragma unroll
         for (int u = 0; u < 4; u++) {
             const int t = t0 + 16 * u;
-            const int id = t < hi ? pages[t >> a.b.page_shift] : -1;
+            const int id = t < hi ? word_of(pages, t >> a.b.page_shift) : -1;
             pid[u] = page_ok(a.b, id) ? id : -1;
         }
     };
@@ -289,7 +289,7 @@ __global__ __launch_bounds__(L_THREADS, 2) void k_attend_latent(AttendArgs a) {
     if (odd_any) {   /* what was taken out of LDS above */
 #pragma unroll 1
         for (int t = max(lo, full / L_ROWS * L_ROWS); t < hi; t++) {
-            const int id = pages[t >> a.b.page_shift];
+            const int id = word_of(pages, t >> a.b.page_shift);
             if (!page_ok(a.b, id) || !(attended(t) & 1)) continue;
             const uint8_t *row = a.k.data + (int64_t)id * a.k.page_stride + (int64_t)(t & rmask) * (LW * (MX ? 1 : 2));
             const uint8_t *sc = MX ? a.k.scales + (int64_t)id * a.k.scale_page_stride + (t & rmask) * (LW / MX_BLOCK) : nullptr;

@@ -121,7 +121,7 @@ __global__ __launch_bounds__(64 * MANY_WAVES, D <= 128 ? 2 : 1) void k_attend_ma
 #pragma unroll
         for (int u = 0; u < 4; u++) {
             const int t = t0 + 16 * u;
-            const int id = u < M::GROUPS && t < hi ? pages[t >> a.b.page_shift] : -1;
+            const int id = u < M::GROUPS && t < hi ? word_of(pages, t >> a.b.page_shift) : -1;
             pid[u] = page_ok(a.b, id) ? id : -1;
         }
     };
@@ -143,21 +143,32 @@ __global__ __launch_bounds__(64 * MANY_WAVES, D <= 128 ? 2 : 1) void k_attend_ma
     };
     /* Every load goes to a row of the cache: rows past hi lie in the same page, those of a page that
      * is not there are taken from page 0; settle clears both. */
+    auto load_from = [&](int z, int id, int row, int r, int p, int buf) {
+        const bool v = z >= N / 2;
+        const uint8_t *base = (v ? vbase : kbase) + (int64_t)id * (v ? a.v.page_stride : a.k.page_stride);
+        if constexpr (MX) {
+            sw[z] = *(const u4 *)(base + row * D + 16 * p);
+            ss[z] = ((v ? vsb : ksb) + (int64_t)id * (v ? a.v.scale_page_stride : a.k.scale_page_stride))[row * (D / MX_BLOCK) + (p >> 1)];
+        } else {
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(base + (row * D + 8 * (p ^ M::swz(r))) * 2),
+                                             (__attribute__((address_space(3))) void *)(lds[buf][v] + (wave * (N / 2) + z % (N / 2)) * 1024),
+                                             16, 0, 0);
+        }
+    };
     auto load = [&](int t0, int buf) {
+        int r, p;
+        if (one_page) {
+            const int id = max(pid[0], 0), row = t0 & rmask;
 #pragma unroll
-        for (int z = 0; z < N; z++) {
-            const bool v = z >= N / 2;
-            int r, p;
-            place(z, r, p);
-            const int id = max(one_page ? pid[0] : page_of(r), 0), row = one_page ? (t0 & rmask) + r : (t0 + r) & rmask;
-            const uint8_t *base = (v ? vbase : kbase) + (int64_t)id * (v ? a.v.page_stride : a.k.page_stride);
-            if constexpr (MX) {
-                sw[z] = *(const u4 *)(base + row * D + 16 * p);
-                ss[z] = ((v ? vsb : ksb) + (int64_t)id * (v ? a.v.scale_page_stride : a.k.scale_page_stride))[row * (D / MX_BLOCK) + (p >> 1)];
-            } else {
-                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(base + (row * D + 8 * (p ^ M::swz(r))) * 2),
-                                                 (__attribute__((address_space(3))) void *)(lds[buf][v] + (wave * (N / 2) + z % (N / 2)) * 1024),
-                                                 16, 0, 0);
+            for (int z = 0; z < N; z++) {
+                place(z, r, p);
+                load_from(z, id, row + r, r, p, buf);
+            }
+        } else {
+#pragma unroll
+            for (int z = 0; z < N; z++) {
+                place(z, r, p);
+                load_from(z, max(page_of(r), 0), (t0 + r) & rmask, r, p, buf);
             }
         }
     };
@@ -307,7 +318,7 @@ __global__ __launch_bounds__(64 * MANY_WAVES, D <= 128 ? 2 : 1) void k_attend_ma
     if (odd_flag) {
 #pragma unroll 1
         for (int t = max(lo, full / M::ROWS * M::ROWS); t < hi; t++) {
-            const int id = pages[t >> a.b.page_shift];
+            const int id = word_of(pages, t >> a.b.page_shift);
             if (!page_ok(a.b, id)) continue;
             const bool add = attended(t) & 1;
             const uint8_t *row = vbase + (int64_t)id * a.v.page_stride + (int64_t)(t & rmask) * (D * (MX ? 1 : 2));

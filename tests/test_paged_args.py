@@ -274,8 +274,8 @@ def test_sequence_bounds():
     """seq_of of hx_paged.h, restated and enumerated over wild lengths and starts: tokens stay in
     [0, n_tokens), rows in [0, kv_cap), table entries in [0, pages_per_seq)."""
     text = (Path(paged.__file__).parent / "csrc" / "hx_paged.h").read_text()
-    for line in ("const int lo = min(max(b.q_start[s], 0), b.n_tokens);", "const int hi = min(max(b.q_start[s + 1], lo), b.n_tokens);",
-                 "const int len = max(b.kv_len[s], 0);", "r.kv = min(len, b.kv_cap);", "r.base = len - r.n;"):
+    for line in ("const int lo = min(max(word_of(b.q_start, s), 0), b.n_tokens);", "const int hi = min(max(word_of(b.q_start, s + 1), lo), b.n_tokens);",
+                 "const int len = max(word_of(b.kv_len, s), 0);", "r.kv = min(len, b.kv_cap);", "r.base = len - r.n;"):
         assert line in re.sub(r"[ ]+", " ", text), "the restatement below is of other code"
     wild = [-2 ** 31, -7, 0, 1, 5, 16, 40, 64, 100, 2 ** 31 - 1]
     n_tokens, per, page = 40, 4, 16
