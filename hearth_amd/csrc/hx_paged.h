@@ -11,6 +11,7 @@
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 namespace hxp {
 
@@ -229,6 +230,42 @@ __device__ __forceinline__ float sum16(float x) {
     const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
+
+/* 16 bytes a lane from memory straight to LDS: lane l's, at base + off + OFS, to dst + 16 l (base and
+ * dst: the same for the wave). Written out because the compiler, which cannot tell the buffers of a
+ * double buffer apart, lets every later LDS read wait for the builtin's loads. No register is
+ * written; the loads have arrived after vm_wait(), and are there for the other waves after a barrier
+ * behind it. */
+template <int OFS>
+__device__ __forceinline__ void to_lds(const uint8_t *base, int off, uint8_t *dst) {
+    const unsigned at = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)dst) - OFS;   /* the instruction adds OFS here too */
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 offset:%3" ::"s"(at), "v"(off), "s"(base), "n"(OFS)
+                 : "memory");
+}
+/* the same address for the whole wave, in scalar registers */
+__device__ __forceinline__ const uint8_t *same(const uint8_t *p) {
+    const uint64_t x = (uint64_t)p;
+    return (const uint8_t *)((uint64_t)(unsigned)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32 |
+                             (unsigned)__builtin_amdgcn_readfirstlane((int)x));
+}
+template <int N, class F> __device__ __forceinline__ void each(F f) {   /* f(constant 0) .. f(constant N - 1) */
+    if constexpr (N > 0) {
+        each<N - 1>(f);
+        f(std::integral_constant<int, N - 1>{});
+    }
+}
+__device__ __forceinline__ void vm_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+/* Every load has arrived and the compiler knows it: without this the first use inside a loop of a
+ * value loaded before it waits, in every round, for all loads under way. */
+__device__ __forceinline__ void arrived() {
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt(0x0f70);   /* vmcnt(0) */
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+/* keeps what stands before it in the source before what stands behind it */
+__device__ __forceinline__ void in_order() { __builtin_amdgcn_sched_barrier(0); }
 
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 

@@ -4,14 +4,19 @@
  *
  * With 2 x 1088 flops a (column, row) against 1152 bytes a row it is bound by the matrix units
  * from about 150 columns a sequence on, and by the rows' bytes below. The products run transposed
- * as in k_paged_attn.hip (S^T = K Q^T, O^T = C^T P^T, 16 x 16 x 32): a wave keeps 16 columns'
- * queries (72 registers) and sums (128) and takes 32 rows of a step of 64; four waves side by
- * side cover 64 columns, the other four the step's other 32 rows (joined at the end through LDS).
+ * as in k_paged_many.hip (S^T = K Q^T, O^T = C^T P^T, 32 x 32 x 16). A workgroup of four waves, one
+ * a SIMD, takes 64 columns and 64 rows a step; for the scores a wave has 32 columns (their queries
+ * in 144 registers) and 32 rows, for the sums its 32 columns, all 64 rows and half of the latent
+ * (128 registers): the two waves of a column pair exchange probabilities through LDS (2 KiB each,
+ * in the operand's layout). Eight waves of 16 columns and 256 registers had none left to read LDS
+ * ahead and took 14400 cycles a step where the products take 2200; all 512 latent elements in one
+ * wave (256 registers of sums) spilled.
  * The rows of a step lie in LDS once, row-major, for both products: the score reads them along
- * the row, the sum through the transposing LDS load. Of the 16-byte pieces of a row, the eight of
- * each 128 bytes are exchanged by row (piece p of row r at p ^ swz(r)), so that neither read meets
- * a bank conflict although a row is 1152 bytes. 16-bit rows go from memory to LDS directly, 8-bit
- * rows through registers, where they become 16-bit ones; the next step's are in flight meanwhile.
+ * the row, the sum through the transposing LDS load. The eight 16-byte pieces of each 128 bytes are
+ * exchanged by row (piece p of row r at p ^ swz(r)), so that neither read meets a bank conflict.
+ * 16-bit rows go from memory to LDS directly, 8-bit rows through registers, where they become
+ * 16-bit ones; the next step's are in flight meanwhile. A wave brings in 16 rows, which lie in one
+ * page whatever its size.
  */
 #include "hx_paged.h"
 
@@ -22,15 +27,20 @@ namespace hxp {
 namespace {
 
 constexpr int LW = 576, LC = 512;                   /* row width (latent, rotated part), latent */
-constexpr int L_WAVES = 8, L_THREADS = 64 * L_WAVES, L_COLS = 64, L_ROWS = 64;
-constexpr int L_PIECES = LW / 8;                    /* 16-byte pieces of a 16-bit row */
+constexpr int L_WAVES = 4, L_THREADS = 64 * L_WAVES, L_COLS = 64, L_ROWS = 64;
 constexpr int L_TILE = L_ROWS * LW * 2;             /* bytes of a step in LDS */
+constexpr int L_CHUNKS = LW / 64;                   /* 128-byte chunks of a 16-bit row: 8 pieces of 16 bytes */
 
 __device__ __forceinline__ int swz(int r) {
     const int k = r >> 1 & 7;
-    return (k & 3) << 1 | k >> 2;
+    return (k & 1) << 2 | k >> 1;
 }
-__device__ __forceinline__ int piece_at(int r, int p) { return (r * L_PIECES + (p ^ swz(r))) * 16; }
+/* A step in LDS: blocks of 8 rows x one chunk (1 KiB), the chunks of 8 rows side by side, so that one
+ * load instruction's 64 pieces of 16 bytes are a block and its addresses one lane constant plus the
+ * block's */
+__device__ __forceinline__ int piece_at(int r, int p) {
+    return ((r >> 3) * L_CHUNKS + (p >> 3)) * 1024 + (r & 7) * 128 + ((p & 7) ^ swz(r)) * 16;
+}
 
 typedef short s4v __attribute__((ext_vector_type(4)));
 
@@ -41,21 +51,23 @@ __device__ __forceinline__ u2 read_tr(const uint8_t *p) {
 }
 
 template <class T, bool MX>
-__global__ __launch_bounds__(L_THREADS, 2) void k_attend_latent(AttendArgs a) {
+__global__ __launch_bounds__(L_THREADS, 1) void k_attend_latent(AttendArgs a) {
     using v8 = typename T::v8;
-    constexpr int KS = LW / 32, DT = LC / 16;
+    constexpr int KS = LW / 16, DT = LC / 64;   /* score steps; tiles of 32 latent elements of a wave */
     constexpr float NINF = -__builtin_huge_valf();
-    constexpr int N = MX ? (L_ROWS * LW / 16 + L_THREADS - 1) / L_THREADS : L_ROWS * L_PIECES / L_THREADS;   /* pieces a thread brings in */
     __shared__ __align__(16) uint8_t lds[2][L_TILE];
-    __shared__ float lds_m[2][L_COLS], lds_l[2][L_COLS];
+    __shared__ float lds_m[2][L_COLS];
+    __shared__ __align__(16) u4 lds_p[2][2][2][64];   /* column pair, half of the rows, group of 16 */
+    __shared__ int lds_grow;
 
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const int g = lane >> 4, lc = lane & 15, wc = wave & 3, wt = wave >> 2;
-    /* the column tiles of one (sequence, split) follow each other on one XCD (workgroup i runs on
-     * XCD i % 8), whose L2 then holds their rows */
+    const int half = lane >> 5, lc = lane & 31, wc = wave & 1, wt = wave >> 1;
+    /* workgroup i runs on XCD i % 8: each XCD takes an eighth of the (sequence, split, column tile)
+     * list, in which the column tiles of the same rows follow each other and share its L2 */
     const int tiles = (int)(((int64_t)a.b.max_q * a.heads + L_COLS - 1) / L_COLS);
-    const int pair = (int)(blockIdx.x / (8 * tiles)) * 8 + (int)(blockIdx.x & 7), tile = (int)(blockIdx.x >> 3) % tiles;
-    if (pair >= a.b.n_seqs * a.n_splits) return;
+    const int64_t total = (int64_t)a.b.n_seqs * a.n_splits * tiles, w = (blockIdx.x & 7) * ((total + 7) / 8) + (blockIdx.x >> 3);
+    if ((int64_t)(blockIdx.x >> 3) >= (total + 7) / 8 || w >= total) return;
+    const int pair = (int)(w / tiles), tile = (int)(w % tiles);
     const int seq = pair / a.n_splits, sp = pair % a.n_splits;
     const Seq q = seq_of(a.b, seq);
     const int cols = min(q.n, a.b.max_q) * a.heads;
@@ -63,7 +75,7 @@ __global__ __launch_bounds__(L_THREADS, 2) void k_attend_latent(AttendArgs a) {
     const int n_sp = max(1, (q.kv + a.chunk - 1) / a.chunk);
     if (sp >= n_sp) return;
 
-    const int c = tile * L_COLS + 16 * wc + lc;
+    const int c = tile * L_COLS + 32 * wc + lc;
     const bool on = c < cols;
     const int tok = on ? c / a.heads : 0, head = on ? c % a.heads : 0;
     const int lim = !on ? 0 : a.b.mask ? min(q.base, q.kv) : min(q.base + tok + 1, q.kv);
@@ -73,7 +85,7 @@ __global__ __launch_bounds__(L_THREADS, 2) void k_attend_latent(AttendArgs a) {
         const uint8_t *pp = a.q_pe + (int64_t)(q.q0 + tok) * a.pt + (int64_t)head * a.ph;
 #pragma unroll
         for (int i = 0; i < KS; i++) {
-            const int d = 32 * i + 8 * g;
+            const int d = 16 * i + 8 * half;
             const unsigned short *p = d < LC ? (const unsigned short *)qp + d : (const unsigned short *)pp + (d - LC);
             u4 w = {0, 0, 0, 0};
             if (on) {
@@ -85,6 +97,7 @@ __global__ __launch_bounds__(L_THREADS, 2) void k_attend_latent(AttendArgs a) {
             qf[i] = __builtin_bit_cast(v8, w);
         }
     }
+    arrived();
     const int t_last = min(cols - 1, tile * L_COLS + L_COLS - 1) / a.heads;
     const int hi = min(min(q.kv, a.b.mask ? q.kv : q.base + t_last + 1), (sp + 1) * a.chunk);
     const int full = a.b.mask ? q.base : q.base + tile * L_COLS / a.heads + 1;
@@ -93,9 +106,11 @@ __global__ __launch_bounds__(L_THREADS, 2) void k_attend_latent(AttendArgs a) {
     const unsigned long long *words = a.b.mask && on ? a.b.mask + (int64_t)(q.q0 + tok) * a.b.mask_words : nullptr;
     auto attended = [&](int t0) { return step_mask(t0, lim, hi, q.base, words, a.b.mask_words); };
 
-    f4 acc[DT];
+    f16v acc[DT];
 #pragma unroll
-    for (int i = 0; i < DT; i++) acc[i] = (f4){0, 0, 0, 0};
+    for (int i = 0; i < DT; i++)
+#pragma unroll
+        for (int j = 0; j < 16; j++) acc[i][j] = 0.0f;
     float m = NINF, l = 0.0f;
 
     const int *pages = a.b.pages + (int64_t)seq * a.b.ld_pages;
@@ -109,78 +124,69 @@ __global__ __launch_bounds__(L_THREADS, 2) void k_attend_latent(AttendArgs a) {
             pid[u] = page_ok(a.b, id) ? id : -1;
         }
     };
-    auto page_of = [&](int r) {
-        const int u = r >> 4;
-        return u == 0 ? pid[0] : u == 1 ? pid[1] : u == 2 ? pid[2] : pid[3];
-    };
     auto have = [&] { return (pid[0] >= 0 ? 1u : 0u) | (pid[1] >= 0 ? 2u : 0u) | (pid[2] >= 0 ? 4u : 0u) | (pid[3] >= 0 ? 8u : 0u); };
     auto edge_at = [&](int t0, unsigned h) { return !(t0 + L_ROWS <= full && t0 + L_ROWS <= hi && h == 15u); };
 
-    u4 sw[MX ? N : 1];
-    unsigned ss[MX ? N : 1];
-    /* the loads of the step at t0: to LDS (16-bit; rows that are not there take the cache's first
-     * row and are cleared in settle) or to registers (8-bit) */
-    auto load = [&](int t0, int buf) {
-        int tid = threadIdx.x;
-        asm volatile("" : "+v"(tid));   /* the pieces' places are worked out anew: held, they cost registers */
+    /* 8-bit: 16 codes of row 16 wave + lane / 4, four lanes a chunk */
+    u4 sw[MX ? L_CHUNKS : 1];
+    unsigned ss[MX ? L_CHUNKS : 1];
+    const int mr = 16 * wave + (lane >> 2), mc = lane & 3;
+    /* The loads of the step at t0, to LDS (16-bit) or to registers (8-bit). Every load goes to a row
+     * of the cache: rows past hi lie in the same page, those of a page that is not there are taken
+     * from page 0; settle clears both. */
+    auto load = [&](int t0, uint8_t *dst) {
+        const int64_t id = max(wave == 0 ? pid[0] : wave == 1 ? pid[1] : wave == 2 ? pid[2] : pid[3], 0);
+        const int row = (t0 + 16 * wave) & rmask;
         if constexpr (MX) {
+            const uint8_t *p = a.k.data + id * a.k.page_stride + (row + (lane >> 2)) * LW + 16 * mc;
+            const uint8_t *sp = a.k.scales + id * a.k.scale_page_stride + (row + (lane >> 2)) * (LW / MX_BLOCK) + (mc >> 1);
 #pragma unroll
-            for (int i = 0; i < N; i++) {
-                const int idx = tid + L_THREADS * i, r = idx / (LW / 16), p = idx % (LW / 16);
-                sw[i] = (u4){0, 0, 0, 0};
-                ss[i] = 127;
-                const int id = page_of(r);
-                if (idx < L_ROWS * (LW / 16) && id >= 0 && t0 + r < hi) {
-                    const int row = (t0 + r) & rmask;
-                    sw[i] = *(const u4 *)(a.k.data + (int64_t)id * a.k.page_stride + row * LW + 16 * p);
-                    ss[i] = a.k.scales[(int64_t)id * a.k.scale_page_stride + row * (LW / MX_BLOCK) + (p >> 1)];
-                }
+            for (int i = 0; i < L_CHUNKS; i++) {
+                sw[i] = *(const u4 *)(p + 64 * i);
+                ss[i] = sp[2 * i];
             }
         } else {
+            const uint8_t *base = same(a.k.data + id * a.k.page_stride + (int64_t)row * (2 * LW));
 #pragma unroll
-            for (int i = 0; i < N; i++) {
-                const int at = (wave * N + i) * 64, idx = at + (tid & 63), r = idx / L_PIECES, p = idx % L_PIECES;
-                const int id = page_of(r);
-                const bool ok = id >= 0 && t0 + r < hi;
-                const uint8_t *src = a.k.data + (ok ? (int64_t)id * a.k.page_stride + (int64_t)(((t0 + r) & rmask) * LW + 8 * (p ^ swz(r))) * 2 : 0);
-                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)src,
-                                                 (__attribute__((address_space(3))) void *)(lds[buf] + at * 16), 16, 0, 0);
+            for (int h = 0; h < 2; h++) {   /* eight rows */
+                const int off = (lane >> 3) * (2 * LW) + ((lane & 7) ^ swz(8 * h + (lane >> 3))) * 16;
+                each<L_CHUNKS>([&](auto i) { to_lds<128 * i.value>(base + h * 8 * (2 * LW), off, dst + ((2 * wave + h) * L_CHUNKS + i.value) * 1024); });
             }
         }
     };
     /* The loaded step made ready in LDS; in edge steps true where a latent element that some
      * column does not attend is infinite or NaN. */
-    auto settle = [&](int t0, int buf, unsigned h, bool edge) {
+    auto settle = [&](int t0, uint8_t *dst, unsigned h, bool edge) {
         bool odd = false;
         if constexpr (MX) {
-            int tid = threadIdx.x;
-            asm volatile("" : "+v"(tid));
+            const bool ok = !edge || (t0 + mr < hi && (h >> wave & 1));
+            const int at0 = piece_at(mr, 2 * mc), at1 = piece_at(mr, 2 * mc + 1);
 #pragma unroll
-            for (int i = 0; i < N; i++) {
-                const int idx = tid + L_THREADS * i, r = idx / (LW / 16), p = idx % (LW / 16);
-                if (idx < L_ROWS * (LW / 16)) {
-                    const float f = mx_scale(ss[i]);
-                    u4 w[2];
+            for (int i = 0; i < L_CHUNKS; i++) {
+                const float f = mx_scale(ss[i]);
+                u4 w[2];
 #pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        w[k >> 1][2 * (k & 1)] = T::template from_mx8<false>(sw[i][k], f);
-                        w[k >> 1][2 * (k & 1) + 1] = T::template from_mx8<true>(sw[i][k], f);
-                    }
-#pragma unroll
-                    for (int k = 0; k < 2; k++) *(u4 *)(lds[buf] + piece_at(r, 2 * p + k)) = w[k];
-                    if (edge)
-#pragma unroll
-                        for (int k = 0; k < 8; k++) odd = odd || T::odd(w[k >> 2][k & 3]);
+                for (int k = 0; k < 4; k++) {
+                    w[k >> 1][2 * (k & 1)] = T::template from_mx8<false>(sw[i][k], f);
+                    w[k >> 1][2 * (k & 1) + 1] = T::template from_mx8<true>(sw[i][k], f);
                 }
+                if (edge)
+#pragma unroll
+                    for (int k = 0; k < 2; k++) {
+                        w[k] = ok ? w[k] : (u4){0, 0, 0, 0};
+                        odd = odd || T::odd(w[k][0]) || T::odd(w[k][1]) || T::odd(w[k][2]) || T::odd(w[k][3]);
+                    }
+                *(u4 *)(dst + at0 + 1024 * i) = w[0];
+                *(u4 *)(dst + at1 + 1024 * i) = w[1];
             }
         } else {
-            __builtin_amdgcn_s_waitcnt(0x0f70);   /* vmcnt(0): this thread's pieces have arrived */
+            vm_wait();   /* this thread's pieces have arrived */
             if (edge)
 #pragma unroll 1
-                for (int i = 0; i < N; i++) {
-                    const int idx = (wave * N + i) * 64 + lane, r = idx / L_PIECES;
-                    u4 *p = (u4 *)(lds[buf] + idx * 16);
-                    if (!(h >> (r >> 4) & 1) || t0 + r >= hi) *p = (u4){0, 0, 0, 0};
+                for (int i = 0; i < 2 * L_CHUNKS; i++) {
+                    const int r = 16 * wave + (i >= L_CHUNKS ? 8 : 0) + (lane >> 3);
+                    u4 *p = (u4 *)(dst + (2 * wave * L_CHUNKS + i) * 1024 + lane * 16);
+                    if (!(h >> wave & 1) || t0 + r >= hi) *p = (u4){0, 0, 0, 0};
                     else {
                         const u4 w = *p;
                         odd = odd || T::odd(w[0]) || T::odd(w[1]) || T::odd(w[2]) || T::odd(w[3]);
@@ -192,149 +198,246 @@ __global__ __launch_bounds__(L_THREADS, 2) void k_attend_latent(AttendArgs a) {
 
     unsigned have_now = 0, have_next = 0;
     bool odd_now = false, odd_next = false, odd_any = false;
+    if (threadIdx.x == 0) lds_grow = 0;
+
+    /* Byte addresses in a step: scores read row 32 wt + lc, pieces 2 i + half; sums read rows 16 g +
+     * 4 half .. + 3 and 8 further, elements 256 wt + 32 i .. + 31; the exchange of pieces is an
+     * exclusive or with a constant */
+    const int r0 = 32 * wt, vr = 4 * half + ((lane & 15) >> 2), vp = 2 * (lane >> 4 & 1) + (lane >> 1 & 1);
+    const int k_at = piece_at(r0 + lc, half);
+    const int v_at[2] = {piece_at(vr, vp + 32 * wt) + 8 * (lane & 1), piece_at(vr + 8, vp + 32 * wt) + 8 * (lane & 1)};
+    /* The maximum that probabilities are taken against is the first step's, common to the two waves of
+     * a column; they may exceed 1 by 2^14, which costs no accuracy in either 16-bit type. Where a
+     * later score exceeds it by more, the rows are gone through for the maxima alone and then once
+     * more: the sums are never rescaled. (The compiler keeps them in registers that only the matrix
+     * unit can work on; scaling them inside the loop took 128 more, and the loop spilled.) */
+    constexpr float ROOM = 14.0f;
+    bool maxima = false, again = false;
+    for (int pass = 0; pass < 3; pass++) {   /* sums; where there was no room: maxima; sums */
+    again = false;
     if (lo < hi) {
         load_pages(lo);
         have_next = have();
-        load(lo, 0);
-        odd_next = settle(lo, 0, have_next, edge_at(lo, have_next));
+        load(lo, lds[0]);
+        odd_next = settle(lo, lds[0], have_next, edge_at(lo, have_next));
         if (lo + L_ROWS < hi) load_pages(lo + L_ROWS);
     }
     __syncthreads();
-
-    /* Byte addresses in a step's tile. A row is nine times 128 bytes, so the exchange of pieces is
-     * an exclusive or with a constant: scores read row 16 u + lc, pieces 4 i + g; sums read rows
-     * 4 g .. 4 g + 3 of either tile of 16, elements 16 i .. 16 i + 15 */
-    const int r0 = 32 * wt, ra = r0 + 4 * g + (lc >> 2);
-    const int k_at[2] = {piece_at(r0 + lc, g), piece_at(r0 + 16 + lc, g)};
-    const int v_at[2] = {piece_at(ra, lc >> 1 & 1) + 8 * (lc & 1), piece_at(ra + 16, lc >> 1 & 1) + 8 * (lc & 1)};
     int buf = 0;
     for (int t0 = lo; t0 < hi; t0 += L_ROWS, buf ^= 1) {
+        uint8_t *tl = lds[buf], *nx = lds[buf ^ 1];
         const bool more = t0 + L_ROWS < hi;
         have_now = have_next;
         odd_now = odd_next;
         if (more) {
             have_next = have();
-            load(t0 + L_ROWS, buf ^ 1);
+            load(t0 + L_ROWS, nx);
             if (t0 + 2 * L_ROWS < hi) load_pages(t0 + 2 * L_ROWS);
         }
-        f4 s[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
-        const uint8_t *tl = lds[buf];
+        f16v s, s1;   /* two sums: an instruction that adds to the one before it waits for it */
 #pragma unroll
-        for (int i = 0; i < KS; i++)
+        for (int j = 0; j < 16; j++) s[j] = s1[j] = 0.0f;
+        /* Six instructions' reads ahead of their use, in this order: left to itself the compiler puts
+         * each read right before its instruction and waits for it. */
+        constexpr int KB = 6;
+        v8 kr[2][KB];
+        auto read_k = [&](int i) { return *(const v8 *)(tl + (k_at ^ 32 * (i & 3)) + 1024 * (i >> 2)); };
 #pragma unroll
-            for (int u = 0; u < 2; u++)
-                s[u] = T::mfma16(*(const v8 *)(tl + (k_at[u] ^ 64 * (i & 1)) + 128 * (i >> 1)), qf[i], s[u]);
+        for (int i = 0; i < KB; i++) kr[0][i] = read_k(i);
+        in_order();
+#pragma unroll
+        for (int n = 0; n < KS / KB; n++) {
+#pragma unroll
+            for (int i = 0; i < KB; i++)
+                if (n + 1 < KS / KB) kr[(n + 1) & 1][i] = read_k((n + 1) * KB + i);
+            in_order();
+#pragma unroll
+            for (int i = 0; i < KB; i += 2) {
+                s = T::mfma32(kr[n & 1][i], qf[n * KB + i], s);
+                s1 = T::mfma32(kr[n & 1][i + 1], qf[n * KB + i + 1], s1);
+            }
+            in_order();
+        }
+        s += s1;
 
         const bool edge = edge_at(t0, have_now);
-        float x[8], mx = NINF;
-#pragma unroll
-        for (int j = 0; j < 8; j++) x[j] = s[j >> 2][j & 3] * a.scale2;
+        float mx = NINF;
+        s *= a.scale2;
         if (edge) {
-            const unsigned long long vis = (attended(t0) & group_rows(have_now)) >> (r0 + 4 * g);
+            const unsigned long long vis = (attended(t0) & group_rows(have_now)) >> (r0 + 4 * half);
 #pragma unroll
-            for (int j = 0; j < 8; j++) x[j] = vis >> (16 * (j >> 2) + (j & 3)) & 1 ? x[j] : NINF;
-            if (__syncthreads_or(odd_now)) {
+            for (int j = 0; j < 16; j++) s[j] = vis >> (8 * (j >> 2) + (j & 3)) & 1 ? s[j] : NINF;
+            if (!maxima && __syncthreads_or(odd_now)) {
                 /* an infinity or NaN among rows that some columns do not attend would reach them as
                  * 0 * inf: the scores are done with the rows, so it is taken out of LDS and added
                  * at the end to the columns that attend it */
                 odd_any = true;
                 for (int i = threadIdx.x; i < L_TILE / 4; i += L_THREADS) {
-                    unsigned *p = (unsigned *)lds[buf] + i;
+                    unsigned *p = (unsigned *)tl + i;
                     *p = T::clean(*p);
                 }
                 __syncthreads();
             }
         }
 #pragma unroll
-        for (int j = 0; j < 8; j++) mx = fmaxf(mx, x[j]);
-        mx = fmaxf(m, max16(max32(mx)));
-        const float ms = mx == NINF ? 0.0f : mx;
-        if (__any(mx > m)) {
-            const float al = exp2_hw(m - ms);
-            l *= al;
-#pragma unroll
-            for (int i = 0; i < DT; i++) acc[i] *= al;
-            m = mx;
+        for (int j = 0; j < 16; j++) mx = fmaxf(mx, s[j]);
+        mx = max32(mx);
+        if (maxima) {
+            m = fmaxf(m, mx);
+            if (more) odd_next = settle(t0 + L_ROWS, nx, have_next, edge_at(t0 + L_ROWS, have_next));
+            __syncthreads();
+            continue;
         }
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-            x[j] = exp2_hw(x[j] - ms);
-            l += x[j];
+        float ms = m == NINF ? 0.0f : m;
+        if (half == 0) lds_m[wt][32 * wc + lc] = mx;
+        if (__any(mx > m + ROOM)) {   /* 1: a column without a maximum yet has one; 2: no room above a maximum */
+            const int grow = __any(mx > m + ROOM && m != NINF) ? 3 : 1;
+            if (lane == 0) atomicOr(&lds_grow, grow);
         }
-        const u4 pw = {T::pack(x[0], x[1]), T::pack(x[2], x[3]), T::pack(x[4], x[5]), T::pack(x[6], x[7])};
-        const v8 pf = __builtin_bit_cast(v8, pw);
+        v8 pf[2][2];
+        auto weigh = [&] {
+            float x[16], sum = 0.0f;
 #pragma unroll
-        for (int i = 0; i < DT; i++) {
-            const u2 va = read_tr(tl + (v_at[0] ^ 32 * (i & 3)) + 128 * (i >> 2));
-            const u2 vb = read_tr(tl + (v_at[1] ^ 32 * (i & 3)) + 128 * (i >> 2));
-            acc[i] = T::mfma16(__builtin_bit_cast(v8, (u4){va[0], va[1], vb[0], vb[1]}), pf, acc[i]);
+            for (int j = 0; j < 16; j++) {
+                x[j] = exp2_hw(s[j] - ms);
+                sum += x[j];
+            }
+#pragma unroll
+            for (int g = 0; g < 2; g++) {
+                const u4 w = {T::pack(x[8 * g], x[8 * g + 1]), T::pack(x[8 * g + 2], x[8 * g + 3]),
+                              T::pack(x[8 * g + 4], x[8 * g + 5]), T::pack(x[8 * g + 6], x[8 * g + 7])};
+                lds_p[wc][wt][g][lane] = w;
+            }
+            return sum;
+        };
+        float sum = weigh();
+        __syncthreads();
+        const int grow = lds_grow;
+        if (grow) {
+            if ((grow & 2) && pass == 0) {
+                again = true;
+                break;
+            }
+            if (m == NINF) m = fmaxf(lds_m[0][32 * wc + lc], lds_m[1][32 * wc + lc]);
+            ms = m == NINF ? 0.0f : m;
+            sum = weigh();
+            __syncthreads();
+            if (threadIdx.x == 0) lds_grow = 0;
         }
-        if (more) odd_next = settle(t0 + L_ROWS, buf ^ 1, have_next, edge_at(t0 + L_ROWS, have_next));
+        l += sum;
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int g = 0; g < 2; g++) pf[h][g] = __builtin_bit_cast(v8, lds_p[wc][h][g][lane]);
+        v8 vr8[2][4];
+        auto read_v = [&](int i, int g) {
+            const u2 x = read_tr(tl + (v_at[0] ^ 64 * (i & 1)) + 1024 * (i >> 1) + g * (2048 * L_CHUNKS));
+            const u2 y = read_tr(tl + (v_at[1] ^ 64 * (i & 1)) + 1024 * (i >> 1) + g * (2048 * L_CHUNKS));
+            return __builtin_bit_cast(v8, (u4){x[0], x[1], y[0], y[1]});
+        };
+#pragma unroll
+        for (int i = 0; i < 4; i++) vr8[0][i] = read_v(i, 0);
+        in_order();
+#pragma unroll
+        for (int n = 0; n < DT; n++) {   /* four tiles of the latent at a time, the rows' groups outside */
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (n + 1 < DT) vr8[(n + 1) & 1][i] = read_v(((n + 1) & 1) * 4 + i, (n + 1) >> 1);
+            in_order();
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                acc[(n & 1) * 4 + i] = T::mfma32(vr8[n & 1][i], pf[n >> 2][n >> 1 & 1], acc[(n & 1) * 4 + i]);
+            in_order();
+        }
+        if (more) odd_next = settle(t0 + L_ROWS, nx, have_next, edge_at(t0 + L_ROWS, have_next));
         __syncthreads();
     }
-    /* the two halves of the rows together, through the steps' LDS */
-    l = sum16(sum32(l));
-    if (g == 0) { lds_m[wt][16 * wc + lc] = m; lds_l[wt][16 * wc + lc] = l; }
+    if (!again && !maxima) break;
+    vm_wait();
     __syncthreads();
-    const float m0 = lds_m[0][16 * wc + lc], m1 = lds_m[1][16 * wc + lc];
-    const float M = fmaxf(m0, m1);
-    const float f0 = m0 == NINF ? 1.0f : exp2_hw(m0 - M), f1 = m1 == NINF ? 1.0f : exp2_hw(m1 - M);
-    const float L = lds_l[0][16 * wc + lc] * f0 + lds_l[1][16 * wc + lc] * f1;
-    f4 *half = (f4 *)lds[0] + wc * (DT * 64);     /* 4 x 32 KiB of the 144 KiB */
-    if (wt == 1) {
-#pragma unroll
-        for (int i = 0; i < DT; i++) half[i * 64 + lane] = acc[i] * f1;
+    if (maxima) {   /* the pair's common maxima are known */
+        if (half == 0) lds_m[wt][32 * wc + lc] = m;
+        __syncthreads();
+        m = fmaxf(lds_m[0][32 * wc + lc], lds_m[1][32 * wc + lc]);
     }
+    if (threadIdx.x == 0) lds_grow = 0;
+    maxima = again;
+    l = 0.0f;
+    odd_any = false;
+#pragma unroll
+    for (int i = 0; i < DT; i++)
+#pragma unroll
+        for (int j = 0; j < 16; j++) acc[i][j] = 0.0f;
+    }
+
+    /* the pair's sums of probabilities; each wave has its half of the latent whole */
+    l = sum32(l);
+    if (half == 0) lds_m[wt][32 * wc + lc] = l;
     __syncthreads();
-    if (odd_any) {   /* what was taken out of LDS above */
+    const float L = lds_m[0][32 * wc + lc] + lds_m[1][32 * wc + lc];
+    const int64_t row = (int64_t)(q.q0 + tok) * a.heads + head;
+    const bool direct = n_sp == 1;
+    const float inv = direct ? L == 0.0f ? 0.0f : 1.0f / L : 1.0f;
+    uint8_t *out = a.out + (int64_t)(q.q0 + tok) * a.ot + (int64_t)head * a.oh;
+    float *po = a.part + (row * a.n_splits + sp) * LC;
+    auto emit = [&](int d, f4 o) {
+        o *= inv;
+        if (!direct) {
+            if (!(L == 0.0f)) *(f4 *)(po + d) = o;
+        } else if (a.aligned) {
+            *(u2 *)(out + 2 * d) = (u2){T::pack(o[0], o[1]), T::pack(o[2], o[3])};
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++) ((typename T::e *)out)[d + j] = (typename T::e)o[j];
+        }
+    };
+    if (!odd_any) {
+        if (on)
+#pragma unroll
+            for (int i = 0; i < DT * 4; i++) {
+                const f16v &x = acc[i >> 2];
+                const int k = 4 * (i & 3);
+                emit(256 * wt + 8 * i + 4 * half, (f4){x[k], x[k + 1], x[k + 2], x[k + 3]});
+            }
+    } else {   /* with what was taken out of LDS above; the sums go through the steps' LDS, where a loop can index them */
+        f4 *own = (f4 *)lds[0] + wave * (DT * 4 * 64);     /* 4 x 32 KiB of the 144 KiB */
+#pragma unroll
+        for (int i = 0; i < DT * 4; i++) {
+            const f16v &x = acc[i >> 2];
+            const int k = 4 * (i & 3);
+            own[i * 64 + lane] = (f4){x[k], x[k + 1], x[k + 2], x[k + 3]};
+        }
 #pragma unroll 1
         for (int t = max(lo, full / L_ROWS * L_ROWS); t < hi; t++) {
             const int id = word_of(pages, t >> a.b.page_shift);
             if (!page_ok(a.b, id) || !(attended(t) & 1)) continue;
-            const uint8_t *row = a.k.data + (int64_t)id * a.k.page_stride + (int64_t)(t & rmask) * (LW * (MX ? 1 : 2));
+            const uint8_t *rp = a.k.data + (int64_t)id * a.k.page_stride + (int64_t)(t & rmask) * (LW * (MX ? 1 : 2));
             const uint8_t *sc = MX ? a.k.scales + (int64_t)id * a.k.scale_page_stride + (t & rmask) * (LW / MX_BLOCK) : nullptr;
 #pragma unroll 1
-            for (int e = 0; e < DT / 2 * 4; e++) {
-                const int i = wt * (DT / 2) + (e >> 2), j = e & 3;
-                const unsigned v = row_elem<T, MX>(row, sc, 16 * i + 4 * g + j);
-                if (T::odd(v)) ((float *)&half[i * 64 + lane])[j] += T::wide(v);
+            for (int e = 0; e < DT * 16; e++) {
+                const unsigned v = row_elem<T, MX>(rp, sc, 256 * wt + 8 * (e >> 2) + 4 * half + (e & 3));
+                if (T::odd(v)) ((float *)&own[(e >> 2) * 64 + lane])[e & 3] += T::wide(v);
             }
         }
-        __syncthreads();
+        if (on)
+#pragma unroll 1
+            for (int i = 0; i < DT * 4; i++) emit(256 * wt + 8 * i + 4 * half, own[i * 64 + lane]);
     }
-    if (wt == 1 || !on) return;
-    const int64_t row = (int64_t)(q.q0 + tok) * a.heads + head;
-    if (n_sp == 1) {
-        const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-        uint8_t *out = a.out + (int64_t)(q.q0 + tok) * a.ot + (int64_t)head * a.oh;
-#pragma unroll
-        for (int i = 0; i < DT; i++) {
-            const f4 o = (acc[i] * f0 + half[i * 64 + lane]) * inv;
-            uint8_t *p = out + 2 * (16 * i + 4 * g);
-            if (a.aligned) *(u2 *)p = (u2){T::pack(o[0], o[1]), T::pack(o[2], o[3])};
-            else
-#pragma unroll
-                for (int j = 0; j < 4; j++) ((typename T::e *)p)[j] = (typename T::e)o[j];
-        }
-        if (a.lse && g == 0) a.lse[row] = L == 0.0f ? NINF : (M + __log2f(L)) * 0.69314718055994531f;
+    if (half || wt || !on) return;
+    if (direct) {
+        if (a.lse) a.lse[row] = L == 0.0f ? NINF : (m + __log2f(L)) * 0.69314718055994531f;
     } else {
-        float *po = a.part + (row * a.n_splits + sp) * LC;
-        if (!(L == 0.0f))
-#pragma unroll
-            for (int i = 0; i < DT; i++) *(f4 *)(po + 16 * i + 4 * g) = acc[i] * f0 + half[i * 64 + lane];
-        if (g == 0) {
-            float *ml = a.part + (int64_t)a.b.n_tokens * a.heads * a.n_splits * LC + (row * a.n_splits + sp) * 2;
-            ml[0] = M;
-            ml[1] = L;
-        }
+        float *ml = a.part + (int64_t)a.b.n_tokens * a.heads * a.n_splits * LC + (row * a.n_splits + sp) * 2;
+        ml[0] = m;
+        ml[1] = L;
     }
 }
 
 template <class T, bool MX>
 void latent_t(const AttendArgs &a, hipStream_t st) {
     const int64_t tiles = ((int64_t)a.b.max_q * a.heads + L_COLS - 1) / L_COLS;
-    const int64_t pairs = ((int64_t)a.b.n_seqs * a.n_splits + 7) / 8 * 8;
-    hipLaunchKernelGGL((k_attend_latent<T, MX>), dim3((unsigned)(pairs * tiles)), dim3(L_THREADS), 0, st, a);
+    const int64_t total = (int64_t)a.b.n_seqs * a.n_splits * tiles;
+    hipLaunchKernelGGL((k_attend_latent<T, MX>), dim3((unsigned)((total + 7) / 8 * 8)), dim3(L_THREADS), 0, st, a);
 }
 
 } // namespace

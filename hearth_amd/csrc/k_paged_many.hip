@@ -94,6 +94,7 @@ __global__ __launch_bounds__(64 * MANY_WAVES, D <= 128 ? 2 : 1) void k_attend_ma
             qf[i] = __builtin_bit_cast(v8, w ^ flip);
         }
     }
+    arrived();
     const int t_last = min(cols - 1, tile * MANY_COLS + MANY_COLS - 1) / a.group;
     const int hi = min(min(q.kv, a.b.mask ? q.kv : q.base + t_last + 1), (sp + 1) * a.chunk);
     const int full = a.b.mask ? q.base : q.base + tile * MANY_COLS / a.group + 1;
@@ -125,50 +126,34 @@ __global__ __launch_bounds__(64 * MANY_WAVES, D <= 128 ? 2 : 1) void k_attend_ma
             pid[u] = page_ok(a.b, id) ? id : -1;
         }
     };
-    auto page_of = [&](int r) {
-        const int u = r >> 4;
-        return u == 0 ? pid[0] : u == 1 ? pid[1] : u == 2 ? pid[2] : pid[3];
-    };
-    /* Pieces that a thread brings in: half of K, half of V. 16-bit: a 16-byte piece of LDS each,
-     * in lane order; 8-bit: 16 codes, two pieces. */
-    constexpr int PER = MX ? 2 : 1, N = 2 * M::ROWS * M::PIECES / PER / 256, RP = M::PIECES / PER;   /* RP: of a row */
-    static_assert(N % 2 == 0 && N >= 2, "K and V alike");
-    const bool one_page = rmask >= M::ROWS - 1;   /* a step lies in one page */
-    u4 sw[MX ? N : 1];
-    unsigned ss[MX ? N : 1];
-    auto place = [&](int z, int &r, int &p) {
-        const int idx = (wave * (N / 2) + z % (N / 2)) * 64 + lane;
-        r = idx / RP;
-        p = idx % RP;
-    };
+    /* A wave brings in a quarter of the step's rows of K and of V; they lie in one page. 16-bit: 1 KiB
+     * of LDS an instruction, 16 bytes a lane; 8-bit: 16 codes a lane, two pieces. */
+    constexpr int RW = M::ROWS / 4, LANES = MX ? M::PIECES / 2 : M::PIECES, RI = 64 / LANES, N = RW / RI;   /* lanes of a row, rows an instruction, instructions */
+    const int my = wave * RW, lr = lane / LANES, lp = lane % LANES;
+    u4 sw[MX ? 2 * N : 1];
+    unsigned ss[MX ? 2 * N : 1];
     /* Every load goes to a row of the cache: rows past hi lie in the same page, those of a page that
      * is not there are taken from page 0; settle clears both. */
-    auto load_from = [&](int z, int id, int row, int r, int p, int buf) {
-        const bool v = z >= N / 2;
-        const uint8_t *base = (v ? vbase : kbase) + (int64_t)id * (v ? a.v.page_stride : a.k.page_stride);
-        if constexpr (MX) {
-            sw[z] = *(const u4 *)(base + row * D + 16 * p);
-            ss[z] = ((v ? vsb : ksb) + (int64_t)id * (v ? a.v.scale_page_stride : a.k.scale_page_stride))[row * (D / MX_BLOCK) + (p >> 1)];
-        } else {
-            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(base + (row * D + 8 * (p ^ M::swz(r))) * 2),
-                                             (__attribute__((address_space(3))) void *)(lds[buf][v] + (wave * (N / 2) + z % (N / 2)) * 1024),
-                                             16, 0, 0);
-        }
-    };
     auto load = [&](int t0, int buf) {
-        int r, p;
-        if (one_page) {
-            const int id = max(pid[0], 0), row = t0 & rmask;
+        const int u = my >> 4;
+        const int64_t id = max(u == 0 ? pid[0] : u == 1 ? pid[1] : u == 2 ? pid[2] : pid[3], 0);
+        const int row = (t0 + my) & rmask;
+        if constexpr (MX) {
+            const uint8_t *kp = kbase + id * a.k.page_stride + row * D, *vp = vbase + id * a.v.page_stride + row * D;
+            const uint8_t *kq = ksb + id * a.k.scale_page_stride + row * (D / MX_BLOCK), *vq = vsb + id * a.v.scale_page_stride + row * (D / MX_BLOCK);
 #pragma unroll
-            for (int z = 0; z < N; z++) {
-                place(z, r, p);
-                load_from(z, id, row + r, r, p, buf);
+            for (int z = 0; z < 2 * N; z++) {
+                const int r = z % N * RI + lr;
+                sw[z] = *(const u4 *)((z < N ? kp : vp) + r * D + 16 * lp);
+                ss[z] = (z < N ? kq : vq)[r * (D / MX_BLOCK) + (lp >> 1)];
             }
         } else {
+            const uint8_t *kp = same(kbase + id * a.k.page_stride + (int64_t)row * (2 * D)), *vp = same(vbase + id * a.v.page_stride + (int64_t)row * (2 * D));
 #pragma unroll
             for (int z = 0; z < N; z++) {
-                place(z, r, p);
-                load_from(z, max(page_of(r), 0), (t0 + r) & rmask, r, p, buf);
+                const int off = (z * RI + lr) * (2 * D) + (lp ^ M::swz(my + z * RI + lr)) * 16;
+                to_lds<0>(kp, off, lds[buf][0] + (my + z * RI) * (2 * D));
+                to_lds<0>(vp, off, lds[buf][1] + (my + z * RI) * (2 * D));
             }
         }
     };
@@ -191,28 +176,25 @@ __global__ __launch_bounds__(64 * MANY_WAVES, D <= 128 ? 2 : 1) void k_attend_ma
         };
         if constexpr (MX) {
 #pragma unroll
-            for (int z = 0; z < N; z++) {
-                int r, p;
-                place(z, r, p);
+            for (int z = 0; z < 2 * N; z++) {
+                const int r = my + z % N * RI + lr;
                 const float f = mx_scale(ss[z]);
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
                     const unsigned x = sw[z][2 * h], y = sw[z][2 * h + 1];
                     u4 w = {T::template from_mx8<false>(x, f), T::template from_mx8<true>(x, f),
                             T::template from_mx8<false>(y, f), T::template from_mx8<true>(y, f)};
-                    if (z >= N / 2 && edge) w = clear(r, w);
-                    *(u4 *)(lds[buf][z >= N / 2] + M::at(r, 2 * p + h)) = w;
+                    if (z >= N && edge) w = clear(r, w);
+                    *(u4 *)(lds[buf][z >= N] + M::at(r, 2 * lp + h)) = w;
                 }
             }
         } else {
-            __builtin_amdgcn_s_waitcnt(0x0f70);   /* vmcnt(0): this thread's pieces have arrived */
+            vm_wait();   /* this thread's pieces have arrived */
             if (edge)
 #pragma unroll 1
-                for (int z = 0; z < N / 2; z++) {
-                    int r, p;
-                    place(z, r, p);
-                    u4 *x = (u4 *)(lds[buf][1] + ((wave * (N / 2) + z) * 64 + lane) * 16);
-                    *x = clear(r, *x);
+                for (int z = 0; z < N; z++) {
+                    u4 *x = (u4 *)(lds[buf][1] + (my + z * RI) * (2 * D) + lane * 16);
+                    *x = clear(my + z * RI + lr, *x);
                 }
         }
         if (odd) odd_flag = 1;
