@@ -104,19 +104,15 @@ __global__ __launch_bounds__(L_THREADS, 1) void k_attend_latent(AttendArgs a) {
     const int lo = sp * a.chunk;
     /* which of the 64 rows from t0 on this lane's column attends (where their pages exist) */
     const unsigned long long *words = a.b.mask && on ? a.b.mask + (int64_t)(q.q0 + tok) * a.b.mask_words : nullptr;
-    auto attended = [&](int t0) { return step_mask(t0, lim, hi, q.base, words, a.b.mask_words); };
+    auto attended = [&](int t0) __attribute__((always_inline)) { return step_mask(t0, lim, hi, q.base, words, a.b.mask_words); };
 
     f16v acc[DT];
-#pragma unroll
-    for (int i = 0; i < DT; i++)
-#pragma unroll
-        for (int j = 0; j < 16; j++) acc[i][j] = 0.0f;
     float m = NINF, l = 0.0f;
 
     const int *pages = a.b.pages + (int64_t)seq * a.b.ld_pages;
     const int rmask = (1 << a.b.page_shift) - 1;
     int pid[4];
-    auto load_pages = [&](int t0) {
+    auto load_pages = [&](int t0) __attribute__((always_inline)) {
 #pragma unroll
         for (int u = 0; u < 4; u++) {
             const int t = t0 + 16 * u;
@@ -124,8 +120,8 @@ __global__ __launch_bounds__(L_THREADS, 1) void k_attend_latent(AttendArgs a) {
             pid[u] = page_ok(a.b, id) ? id : -1;
         }
     };
-    auto have = [&] { return (pid[0] >= 0 ? 1u : 0u) | (pid[1] >= 0 ? 2u : 0u) | (pid[2] >= 0 ? 4u : 0u) | (pid[3] >= 0 ? 8u : 0u); };
-    auto edge_at = [&](int t0, unsigned h) { return !(t0 + L_ROWS <= full && t0 + L_ROWS <= hi && h == 15u); };
+    auto have = [&]() __attribute__((always_inline)) { return (pid[0] >= 0 ? 1u : 0u) | (pid[1] >= 0 ? 2u : 0u) | (pid[2] >= 0 ? 4u : 0u) | (pid[3] >= 0 ? 8u : 0u); };
+    auto edge_at = [&](int t0, unsigned h) __attribute__((always_inline)) { return !(t0 + L_ROWS <= full && t0 + L_ROWS <= hi && h == 15u); };
 
     /* 8-bit: 16 codes of row 16 wave + lane / 4, four lanes a chunk */
     u4 sw[MX ? L_CHUNKS : 1];
@@ -134,7 +130,7 @@ __global__ __launch_bounds__(L_THREADS, 1) void k_attend_latent(AttendArgs a) {
     /* The loads of the step at t0, to LDS (16-bit) or to registers (8-bit). Every load goes to a row
      * of the cache: rows past hi lie in the same page, those of a page that is not there are taken
      * from page 0; settle clears both. */
-    auto load = [&](int t0, uint8_t *dst) {
+    auto load = [&](int t0, uint8_t *dst) __attribute__((always_inline)) {
         const int64_t id = max(wave == 0 ? pid[0] : wave == 1 ? pid[1] : wave == 2 ? pid[2] : pid[3], 0);
         const int row = (t0 + 16 * wave) & rmask;
         if constexpr (MX) {
@@ -156,7 +152,7 @@ __global__ __launch_bounds__(L_THREADS, 1) void k_attend_latent(AttendArgs a) {
     };
     /* The loaded step made ready in LDS; in edge steps true where a latent element that some
      * column does not attend is infinite or NaN. */
-    auto settle = [&](int t0, uint8_t *dst, unsigned h, bool edge) {
+    auto settle = [&](int t0, uint8_t *dst, unsigned h, bool edge) __attribute__((always_inline)) {
         bool odd = false;
         if constexpr (MX) {
             const bool ok = !edge || (t0 + mr < hi && (h >> wave & 1));
@@ -206,34 +202,32 @@ __global__ __launch_bounds__(L_THREADS, 1) void k_attend_latent(AttendArgs a) {
     const int r0 = 32 * wt, vr = 4 * half + ((lane & 15) >> 2), vp = 2 * (lane >> 4 & 1) + (lane >> 1 & 1);
     const int k_at = piece_at(r0 + lc, half);
     const int v_at[2] = {piece_at(vr, vp + 32 * wt) + 8 * (lane & 1), piece_at(vr + 8, vp + 32 * wt) + 8 * (lane & 1)};
-    /* The maximum that probabilities are taken against is the first step's, common to the two waves of
-     * a column; they may exceed 1 by 2^14, which costs no accuracy in either 16-bit type. Where a
-     * later score exceeds it by more, the rows are gone through for the maxima alone and then once
-     * more: the sums are never rescaled. (The compiler keeps them in registers that only the matrix
-     * unit can work on; scaling them inside the loop took 128 more, and the loop spilled.) */
-    constexpr float ROOM = 14.0f;
-    bool maxima = false, again = false;
-    for (int pass = 0; pass < 3; pass++) {   /* sums; where there was no room: maxima; sums */
-    again = false;
-    if (lo < hi) {
-        load_pages(lo);
-        have_next = have();
-        load(lo, lds[0]);
-        odd_next = settle(lo, lds[0], have_next, edge_at(lo, have_next));
-        if (lo + L_ROWS < hi) load_pages(lo + L_ROWS);
-    }
-    __syncthreads();
-    int buf = 0;
-    for (int t0 = lo; t0 < hi; t0 += L_ROWS, buf ^= 1) {
-        uint8_t *tl = lds[buf], *nx = lds[buf ^ 1];
-        const bool more = t0 + L_ROWS < hi;
+    /* the first step's rows; then, a step: the next one's under way */
+    auto begin = [&]() __attribute__((always_inline)) {
+        if (lo < hi) {
+            load_pages(lo);
+            have_next = have();
+            load(lo, lds[0]);
+            odd_next = settle(lo, lds[0], have_next, edge_at(lo, have_next));
+            if (lo + L_ROWS < hi) load_pages(lo + L_ROWS);
+        }
+        __syncthreads();
+    };
+    auto ahead = [&](int t0, uint8_t *nx) __attribute__((always_inline)) {
         have_now = have_next;
         odd_now = odd_next;
-        if (more) {
+        if (t0 + L_ROWS < hi) {
             have_next = have();
             load(t0 + L_ROWS, nx);
             if (t0 + 2 * L_ROWS < hi) load_pages(t0 + 2 * L_ROWS);
         }
+    };
+    auto finish = [&](int t0, uint8_t *nx) __attribute__((always_inline)) {
+        if (t0 + L_ROWS < hi) odd_next = settle(t0 + L_ROWS, nx, have_next, edge_at(t0 + L_ROWS, have_next));
+        __syncthreads();
+    };
+    /* scores of this wave's rows, scaled; rows that are not attended -infinity */
+    auto scores = [&](int t0, const uint8_t *tl) __attribute__((always_inline)) {
         f16v s, s1;   /* two sums: an instruction that adds to the one before it waits for it */
 #pragma unroll
         for (int j = 0; j < 16; j++) s[j] = s1[j] = 0.0f;
@@ -241,7 +235,7 @@ __global__ __launch_bounds__(L_THREADS, 1) void k_attend_latent(AttendArgs a) {
          * each read right before its instruction and waits for it. */
         constexpr int KB = 6;
         v8 kr[2][KB];
-        auto read_k = [&](int i) { return *(const v8 *)(tl + (k_at ^ 32 * (i & 3)) + 1024 * (i >> 2)); };
+        auto read_k = [&](int i) __attribute__((always_inline)) { return *(const v8 *)(tl + (k_at ^ 32 * (i & 3)) + 1024 * (i >> 2)); };
 #pragma unroll
         for (int i = 0; i < KB; i++) kr[0][i] = read_k(i);
         in_order();
@@ -258,19 +252,38 @@ __global__ __launch_bounds__(L_THREADS, 1) void k_attend_latent(AttendArgs a) {
             }
             in_order();
         }
-        s += s1;
-
-        const bool edge = edge_at(t0, have_now);
-        float mx = NINF;
-        s *= a.scale2;
-        if (edge) {
+        s = (s + s1) * a.scale2;
+        if (edge_at(t0, have_now)) {
             const unsigned long long vis = (attended(t0) & group_rows(have_now)) >> (r0 + 4 * half);
 #pragma unroll
             for (int j = 0; j < 16; j++) s[j] = vis >> (8 * (j >> 2) + (j & 3)) & 1 ? s[j] : NINF;
-            if (!maxima && __syncthreads_or(odd_now)) {
+        }
+        return s;
+    };
+    auto largest = [&](const f16v &s) __attribute__((always_inline)) {
+        float x = s[0];
+#pragma unroll
+        for (int j = 1; j < 16; j++) x = fmaxf(x, s[j]);
+        return max32(x);
+    };
+    /* The maximum that probabilities are taken against is the first step's, common to the two waves of
+     * a column; they may exceed 1 by 2^14, which costs no accuracy in either 16-bit type. Where a
+     * later score exceeds it by more, the rows are gone through for the maxima alone and then once
+     * more: the sums are never rescaled. (The compiler keeps them in registers that only the matrix
+     * unit can work on; scaling them inside the loop took 128 more, and the loop spilled.) Returns
+     * whether that happened. */
+    constexpr float ROOM = 14.0f;
+    auto attend = [&]() __attribute__((always_inline)) {
+        bool again = false;
+        begin();
+        for (int t0 = lo, buf = 0; t0 < hi; t0 += L_ROWS, buf ^= 1) {
+            uint8_t *tl = lds[buf], *nx = lds[buf ^ 1];
+            ahead(t0, nx);
+            const f16v s = scores(t0, tl);
+            if (edge_at(t0, have_now) && __syncthreads_or(odd_now)) {
                 /* an infinity or NaN among rows that some columns do not attend would reach them as
-                 * 0 * inf: the scores are done with the rows, so it is taken out of LDS and added
-                 * at the end to the columns that attend it */
+                 * 0 * inf: the scores are done with the rows, so it is taken out of LDS and added at
+                 * the end to the columns that attend it */
                 odd_any = true;
                 for (int i = threadIdx.x; i < L_TILE / 4; i += L_THREADS) {
                     unsigned *p = (unsigned *)tl + i;
@@ -278,96 +291,91 @@ __global__ __launch_bounds__(L_THREADS, 1) void k_attend_latent(AttendArgs a) {
                 }
                 __syncthreads();
             }
-        }
+            const float mx = largest(s);
+            float ms = m == NINF ? 0.0f : m;
+            if (half == 0) lds_m[wt][32 * wc + lc] = mx;
+            if (__any(mx > m + ROOM)) {   /* 1: a column without a maximum yet has one; 2: no room above a maximum */
+                const int grow = __any(mx > m + ROOM && m != NINF) ? 3 : 1;
+                if (lane == 0) atomicOr(&lds_grow, grow);
+            }
+            v8 pf[2][2];
+            auto weigh = [&]() __attribute__((always_inline)) {
+                float x[16], sum = 0.0f;
 #pragma unroll
-        for (int j = 0; j < 16; j++) mx = fmaxf(mx, s[j]);
-        mx = max32(mx);
-        if (maxima) {
-            m = fmaxf(m, mx);
-            if (more) odd_next = settle(t0 + L_ROWS, nx, have_next, edge_at(t0 + L_ROWS, have_next));
+                for (int j = 0; j < 16; j++) {
+                    x[j] = exp2_hw(s[j] - ms);
+                    sum += x[j];
+                }
+#pragma unroll
+                for (int g = 0; g < 2; g++) {
+                    const u4 w = {T::pack(x[8 * g], x[8 * g + 1]), T::pack(x[8 * g + 2], x[8 * g + 3]),
+                                  T::pack(x[8 * g + 4], x[8 * g + 5]), T::pack(x[8 * g + 6], x[8 * g + 7])};
+                    lds_p[wc][wt][g][lane] = w;
+                }
+                return sum;
+            };
+            float sum = weigh();
             __syncthreads();
-            continue;
-        }
-        float ms = m == NINF ? 0.0f : m;
-        if (half == 0) lds_m[wt][32 * wc + lc] = mx;
-        if (__any(mx > m + ROOM)) {   /* 1: a column without a maximum yet has one; 2: no room above a maximum */
-            const int grow = __any(mx > m + ROOM && m != NINF) ? 3 : 1;
-            if (lane == 0) atomicOr(&lds_grow, grow);
-        }
-        v8 pf[2][2];
-        auto weigh = [&] {
-            float x[16], sum = 0.0f;
-#pragma unroll
-            for (int j = 0; j < 16; j++) {
-                x[j] = exp2_hw(s[j] - ms);
-                sum += x[j];
+            const int grow = lds_grow;
+            if (grow) {
+                again = again || (grow & 2);   /* and on: leaving the loop here costs 256 register moves a step */
+                if (m == NINF) m = fmaxf(lds_m[0][32 * wc + lc], lds_m[1][32 * wc + lc]);
+                ms = m == NINF ? 0.0f : m;
+                sum = weigh();
+                __syncthreads();
+                if (threadIdx.x == 0) lds_grow = 0;
             }
+            l += sum;
 #pragma unroll
-            for (int g = 0; g < 2; g++) {
-                const u4 w = {T::pack(x[8 * g], x[8 * g + 1]), T::pack(x[8 * g + 2], x[8 * g + 3]),
-                              T::pack(x[8 * g + 4], x[8 * g + 5]), T::pack(x[8 * g + 6], x[8 * g + 7])};
-                lds_p[wc][wt][g][lane] = w;
-            }
-            return sum;
-        };
-        float sum = weigh();
-        __syncthreads();
-        const int grow = lds_grow;
-        if (grow) {
-            if ((grow & 2) && pass == 0) {
-                again = true;
-                break;
-            }
-            if (m == NINF) m = fmaxf(lds_m[0][32 * wc + lc], lds_m[1][32 * wc + lc]);
-            ms = m == NINF ? 0.0f : m;
-            sum = weigh();
-            __syncthreads();
-            if (threadIdx.x == 0) lds_grow = 0;
-        }
-        l += sum;
+            for (int h = 0; h < 2; h++)
 #pragma unroll
-        for (int h = 0; h < 2; h++)
+                for (int g = 0; g < 2; g++) pf[h][g] = __builtin_bit_cast(v8, lds_p[wc][h][g][lane]);
+            v8 vr8[2][4];
+            auto read_v = [&](int i, int g) __attribute__((always_inline)) {
+                const u2 x = read_tr(tl + (v_at[0] ^ 64 * (i & 1)) + 1024 * (i >> 1) + g * (2048 * L_CHUNKS));
+                const u2 y = read_tr(tl + (v_at[1] ^ 64 * (i & 1)) + 1024 * (i >> 1) + g * (2048 * L_CHUNKS));
+                return __builtin_bit_cast(v8, (u4){x[0], x[1], y[0], y[1]});
+            };
 #pragma unroll
-            for (int g = 0; g < 2; g++) pf[h][g] = __builtin_bit_cast(v8, lds_p[wc][h][g][lane]);
-        v8 vr8[2][4];
-        auto read_v = [&](int i, int g) {
-            const u2 x = read_tr(tl + (v_at[0] ^ 64 * (i & 1)) + 1024 * (i >> 1) + g * (2048 * L_CHUNKS));
-            const u2 y = read_tr(tl + (v_at[1] ^ 64 * (i & 1)) + 1024 * (i >> 1) + g * (2048 * L_CHUNKS));
-            return __builtin_bit_cast(v8, (u4){x[0], x[1], y[0], y[1]});
-        };
-#pragma unroll
-        for (int i = 0; i < 4; i++) vr8[0][i] = read_v(i, 0);
-        in_order();
-#pragma unroll
-        for (int n = 0; n < DT; n++) {   /* four tiles of the latent at a time, the rows' groups outside */
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-                if (n + 1 < DT) vr8[(n + 1) & 1][i] = read_v(((n + 1) & 1) * 4 + i, (n + 1) >> 1);
+            for (int i = 0; i < 4; i++) vr8[0][i] = read_v(i, 0);
             in_order();
 #pragma unroll
-            for (int i = 0; i < 4; i++)
-                acc[(n & 1) * 4 + i] = T::mfma32(vr8[n & 1][i], pf[n >> 2][n >> 1 & 1], acc[(n & 1) * 4 + i]);
-            in_order();
+            for (int n = 0; n < DT; n++) {   /* four tiles of the latent at a time, the rows' groups outside */
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    if (n + 1 < DT) vr8[(n + 1) & 1][i] = read_v(((n + 1) & 1) * 4 + i, (n + 1) >> 1);
+                in_order();
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    acc[(n & 1) * 4 + i] = T::mfma32(vr8[n & 1][i], pf[n >> 2][n >> 1 & 1], acc[(n & 1) * 4 + i]);
+                in_order();
+            }
+            finish(t0, nx);
         }
-        if (more) odd_next = settle(t0 + L_ROWS, nx, have_next, edge_at(t0 + L_ROWS, have_next));
-        __syncthreads();
-    }
-    if (!again && !maxima) break;
-    vm_wait();
-    __syncthreads();
-    if (maxima) {   /* the pair's common maxima are known */
+        return again;
+    };
+    auto clear = [&]() __attribute__((always_inline)) {
+        l = 0.0f;
+        odd_any = false;
+#pragma unroll
+        for (int i = 0; i < DT; i++)
+#pragma unroll
+            for (int j = 0; j < 16; j++) acc[i][j] = 0.0f;
+    };
+    clear();
+    if (attend()) {
+        begin();
+        for (int t0 = lo, buf = 0; t0 < hi; t0 += L_ROWS, buf ^= 1) {
+            ahead(t0, lds[buf ^ 1]);
+            m = fmaxf(m, largest(scores(t0, lds[buf])));
+            finish(t0, lds[buf ^ 1]);
+        }
         if (half == 0) lds_m[wt][32 * wc + lc] = m;
         __syncthreads();
         m = fmaxf(lds_m[0][32 * wc + lc], lds_m[1][32 * wc + lc]);
-    }
-    if (threadIdx.x == 0) lds_grow = 0;
-    maxima = again;
-    l = 0.0f;
-    odd_any = false;
-#pragma unroll
-    for (int i = 0; i < DT; i++)
-#pragma unroll
-        for (int j = 0; j < 16; j++) acc[i][j] = 0.0f;
+        __syncthreads();
+        clear();
+        attend();
     }
 
     /* the pair's sums of probabilities; each wave has its half of the latent whole */
@@ -380,7 +388,7 @@ __global__ __launch_bounds__(L_THREADS, 1) void k_attend_latent(AttendArgs a) {
     const float inv = direct ? L == 0.0f ? 0.0f : 1.0f / L : 1.0f;
     uint8_t *out = a.out + (int64_t)(q.q0 + tok) * a.ot + (int64_t)head * a.oh;
     float *po = a.part + (row * a.n_splits + sp) * LC;
-    auto emit = [&](int d, f4 o) {
+    auto emit = [&](int d, f4 o) __attribute__((always_inline)) {
         o *= inv;
         if (!direct) {
             if (!(L == 0.0f)) *(f4 *)(po + d) = o;

@@ -236,7 +236,7 @@ def test_strided_cache_and_arrays(store):
 # ---------------------------------------------------------------- attention
 
 def run_attend(g, kind, store, heads, kv_heads, width, lens, news, page, trees=None, latent=False, pages=None,
-               n_pages=None, edit=None, pad=2, scale=None, max_kv=None):
+               n_pages=None, edit=None, pad=2, scale=None, max_kv=None, queries=None):
     """One call against the oracle; returns (out, lse) on the CPU"""
     if pages is None:
         pages, n_pages = deal(g, lens, page)
@@ -249,6 +249,8 @@ def run_attend(g, kind, store, heads, kv_heads, width, lens, news, page, trees=N
     q = torch.randn(T + pad, heads, W, generator=g).to(kind)
     if latent:
         q[..., :512] *= 0.35
+    if queries:
+        queries(q)
     scale = (192 ** -0.5 if latent else width ** -0.5) if scale is None else scale
     mask = O.words(trees, max(news)) if trees else None
     if mask is not None:
@@ -402,10 +404,39 @@ def test_latent_tree_and_split(kind, store):
     run_attend(_gen(6), kind, store, 16, 1, 0, [2000, 85], [5, 85], 64, [O.tree(5, 2), O.tree(85)], latent=True)
 
 
+@pytest.mark.parametrize("latent", [False, True])
+@pytest.mark.parametrize("heads", [8, 64])
 @pytest.mark.parametrize("scale", [-0.3, 0.0, 40.0])
-def test_attend_scales(scale):
+def test_attend_scales(scale, heads, latent):
     """A negative scale, none, and one that leaves a single row."""
-    run_attend(_gen(8), BF, "bf16", 8, 2, 64, [50, 200], [3, 1], 16, scale=scale)
+    run_attend(_gen(8), BF, "bf16", heads, 1, 64, [50, 200], [3, 1], 16, scale=scale, latent=latent)
+
+
+@pytest.mark.parametrize("kind,store", STORES)
+@pytest.mark.parametrize("heads,latent", [(8, False), (64, False), (64, True)])
+def test_scores_that_grow_along_the_rows(kind, store, heads, latent):
+    """Each row's scores far above those of the rows before it, and far below: maxima that grow in
+    every step, and a first maximum that stays."""
+    def edit(c, pages):
+        for s, up in ((0, True), (1, False)):
+            for t in range(300):
+                at = (pages[s, t // 16].item(), slice(None), t % 16)
+                row = torch.zeros(c["k"].shape[1], c["k"].shape[-1])
+                row[:, 64 if latent else 0] = (t if up else 300 - t) * 0.25
+                row[:, 70 if latent else 5] = math.sin(t)
+                row = row.to(kind)
+                if store == "mx8":
+                    codes, sc = O.mx8(row)
+                    c["k"].view(torch.uint8)[at], c["ks"][at] = codes.view(torch.uint8), sc
+                else:
+                    c["k"][at] = row
+
+    def queries(q):
+        q.zero_()
+        q[..., 64 if latent else 0] = 3.0
+        q[..., 70 if latent else 5] = 1.0
+
+    run_attend(_gen(61), kind, store, heads, 1, 64, [300, 300], [1, 2], 16, latent=latent, edit=edit, scale=1.0, queries=queries)
 
 
 def test_attend_strided_unaligned():
