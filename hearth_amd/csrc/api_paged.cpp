@@ -161,10 +161,8 @@ int attend_call(const hearth_gpu_cache *c, const hearth_gpu_batch *b, const hear
     if (!latent) a.v = rows_of(c->v, c->dtype);
     a.q = (const uint8_t *)q->data; a.qt = 2 * q->token_stride; a.qh = 2 * q->head_stride;
     a.out = (uint8_t *)out->data; a.ot = 2 * out->token_stride; a.oh = 2 * out->head_stride;
-    a.aligned = on16(*q) && on16(*out);
     if (latent) {
         a.q_pe = (const uint8_t *)q_pe->data; a.pt = 2 * q_pe->token_stride; a.ph = 2 * q_pe->head_stride;
-        a.aligned = a.aligned && on16(*q_pe);
     }
     a.lse = lse;
     a.heads = q->n_heads; a.kv_heads = c->n_heads; a.group = a.heads / a.kv_heads;

@@ -79,7 +79,6 @@ struct AttendArgs {
     int heads, kv_heads, group;       /* group: query heads per kv head */
     float scale2;                     /* scale * log2(e): probabilities are powers of two */
     int chunk, n_splits;              /* rows of a split (a multiple of the kernels' row step); splits of the longest */
-    bool aligned;                     /* q, q_pe and out start and step on 16 bytes */
     float *part;                      /* [n_tokens][heads][n_splits][DV] sums, then [..][2] maximum and sum */
 };
 
@@ -208,6 +207,10 @@ __device__ __forceinline__ unsigned row_elem(const uint8_t *row, const uint8_t *
     else
         return ((const unsigned short *)row)[d];
 }
+
+/* 16 and 8 bytes at any even address (the memory system takes them as one access) */
+typedef u4 u4_any __attribute__((aligned(2)));
+typedef u2 u2_any __attribute__((aligned(2)));
 
 /* the scale of a block from its byte (1 .. 254) */
 __device__ __forceinline__ float mx_scale(unsigned byte) { return __uint_as_float((byte & 255u) << 23); }

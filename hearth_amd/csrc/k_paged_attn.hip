@@ -122,10 +122,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_attend_few(AttendArgs a) {
             const unsigned short *p = (const unsigned short *)qp + d;
             u4 w = {0, 0, 0, 0};
             if (on) {
-                if (a.aligned) w = *(const u4 *)p;
-                else
-#pragma unroll
-                    for (int k = 0; k < 4; k++) w[k] = p[2 * k] | (unsigned)p[2 * k + 1] << 16;
+                w = *(const u4_any *)p;
             }
             qf[n][i] = __builtin_bit_cast(v8, w);
         }
@@ -324,14 +321,9 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_attend_few(AttendArgs a) {
             if (direct) {
                 const float inv = Lo == 0.0f ? 0.0f : 1.0f / Lo;
                 uint8_t *out = a.out + (int64_t)(q.q0 + ot) * a.ot + (int64_t)oh * a.oh + 2 * (b * BD + od);
-                if (a.aligned) {
 #pragma unroll
-                    for (int j = 0; j < PL; j += 4)
-                        *(u2 *)(out + 2 * j) = (u2){T::pack(o[j] * inv, o[j + 1] * inv), T::pack(o[j + 2] * inv, o[j + 3] * inv)};
-                } else {
-#pragma unroll
-                    for (int j = 0; j < PL; j++) ((typename T::e *)out)[j] = (typename T::e)(o[j] * inv);
-                }
+                for (int j = 0; j < PL; j += 4)
+                    *(u2_any *)(out + 2 * j) = (u2){T::pack(o[j] * inv, o[j + 1] * inv), T::pack(o[j + 2] * inv, o[j + 3] * inv)};
             } else if (!(Lo == 0.0f)) {
                 float *po = a.part + (row * a.n_splits + sp) * D + b * BD + od;
 #pragma unroll
@@ -409,10 +401,7 @@ __global__ __launch_bounds__(JOIN_THREADS) void k_attend_join(AttendArgs a) {
     }
     const float inv = L == 0.0f ? 0.0f : 1.0f / L;
     uint8_t *out = a.out + (int64_t)(q.q0 + t) * a.ot + (int64_t)h * a.oh + 2 * e;
-    if (a.aligned) *(u2 *)out = (u2){T::pack(o[0] * inv, o[1] * inv), T::pack(o[2] * inv, o[3] * inv)};
-    else
-#pragma unroll
-        for (int j = 0; j < 4; j++) ((typename T::e *)out)[j] = (typename T::e)(o[j] * inv);
+    *(u2_any *)out = (u2){T::pack(o[0] * inv, o[1] * inv), T::pack(o[2] * inv, o[3] * inv)};
     if (a.lse && e == 0) a.lse[row] = L == 0.0f ? NINF : (M + __log2f(L)) * 0.69314718055994531f;
 }
 

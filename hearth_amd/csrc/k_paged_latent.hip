@@ -79,25 +79,6 @@ __global__ __launch_bounds__(L_THREADS, 1) void k_attend_latent(AttendArgs a) {
     const bool on = c < cols;
     const int tok = on ? c / a.heads : 0, head = on ? c % a.heads : 0;
     const int lim = !on ? 0 : a.b.mask ? min(q.base, q.kv) : min(q.base + tok + 1, q.kv);
-    v8 qf[KS];
-    {
-        const uint8_t *qp = a.q + (int64_t)(q.q0 + tok) * a.qt + (int64_t)head * a.qh;
-        const uint8_t *pp = a.q_pe + (int64_t)(q.q0 + tok) * a.pt + (int64_t)head * a.ph;
-#pragma unroll
-        for (int i = 0; i < KS; i++) {
-            const int d = 16 * i + 8 * half;
-            const unsigned short *p = d < LC ? (const unsigned short *)qp + d : (const unsigned short *)pp + (d - LC);
-            u4 w = {0, 0, 0, 0};
-            if (on) {
-                if (a.aligned) w = *(const u4 *)p;
-                else
-#pragma unroll
-                    for (int k = 0; k < 4; k++) w[k] = p[2 * k] | (unsigned)p[2 * k + 1] << 16;
-            }
-            qf[i] = __builtin_bit_cast(v8, w);
-        }
-    }
-    arrived();
     const int t_last = min(cols - 1, tile * L_COLS + L_COLS - 1) / a.heads;
     const int hi = min(min(q.kv, a.b.mask ? q.kv : q.base + t_last + 1), (sp + 1) * a.chunk);
     const int full = a.b.mask ? q.base : q.base + tile * L_COLS / a.heads + 1;
@@ -178,7 +159,7 @@ __global__ __launch_bounds__(L_THREADS, 1) void k_attend_latent(AttendArgs a) {
         } else {
             vm_wait();   /* this thread's pieces have arrived */
             if (edge)
-#pragma unroll 1
+#pragma unroll 6
                 for (int i = 0; i < 2 * L_CHUNKS; i++) {
                     const int r = 16 * wave + (i >= L_CHUNKS ? 8 : 0) + (lane >> 3);
                     u4 *p = (u4 *)(dst + (2 * wave * L_CHUNKS + i) * 1024 + lane * 16);
@@ -195,6 +176,31 @@ __global__ __launch_bounds__(L_THREADS, 1) void k_attend_latent(AttendArgs a) {
     unsigned have_now = 0, have_next = 0;
     bool odd_now = false, odd_next = false, odd_any = false;
     if (threadIdx.x == 0) lds_grow = 0;
+    /* the first step's loads go out before the queries', which arrive with them */
+    auto start = [&]() __attribute__((always_inline)) {
+        if (lo < hi) {
+            load_pages(lo);
+            have_next = have();
+            load(lo, lds[0]);
+        }
+    };
+    start();
+    v8 qf[KS];
+    {
+        const uint8_t *qp = a.q + (int64_t)(q.q0 + tok) * a.qt + (int64_t)head * a.qh;
+        const uint8_t *pp = a.q_pe + (int64_t)(q.q0 + tok) * a.pt + (int64_t)head * a.ph;
+#pragma unroll
+        for (int i = 0; i < KS; i++) {
+            const int d = 16 * i + 8 * half;
+            const unsigned short *p = d < LC ? (const unsigned short *)qp + d : (const unsigned short *)pp + (d - LC);
+            u4 w = {0, 0, 0, 0};
+            if (on) {
+                w = *(const u4_any *)p;
+            }
+            qf[i] = __builtin_bit_cast(v8, w);
+        }
+    }
+    arrived();
 
     /* Byte addresses in a step: scores read row 32 wt + lc, pieces 2 i + half; sums read rows 16 g +
      * 4 half .. + 3 and 8 further, elements 256 wt + 32 i .. + 31; the exchange of pieces is an
@@ -205,9 +211,6 @@ __global__ __launch_bounds__(L_THREADS, 1) void k_attend_latent(AttendArgs a) {
     /* the first step's rows; then, a step: the next one's under way */
     auto begin = [&]() __attribute__((always_inline)) {
         if (lo < hi) {
-            load_pages(lo);
-            have_next = have();
-            load(lo, lds[0]);
             odd_next = settle(lo, lds[0], have_next, edge_at(lo, have_next));
             if (lo + L_ROWS < hi) load_pages(lo + L_ROWS);
         }
@@ -354,16 +357,15 @@ __global__ __launch_bounds__(L_THREADS, 1) void k_attend_latent(AttendArgs a) {
         }
         return again;
     };
-    auto clear = [&]() __attribute__((always_inline)) {
+    for (int pass = 0; pass < 2; pass++) {
         l = 0.0f;
         odd_any = false;
 #pragma unroll
         for (int i = 0; i < DT; i++)
 #pragma unroll
             for (int j = 0; j < 16; j++) acc[i][j] = 0.0f;
-    };
-    clear();
-    if (attend()) {
+        if (!attend() || pass) break;
+        start();
         begin();
         for (int t0 = lo, buf = 0; t0 < hi; t0 += L_ROWS, buf ^= 1) {
             ahead(t0, lds[buf ^ 1]);
@@ -374,8 +376,7 @@ __global__ __launch_bounds__(L_THREADS, 1) void k_attend_latent(AttendArgs a) {
         __syncthreads();
         m = fmaxf(lds_m[0][32 * wc + lc], lds_m[1][32 * wc + lc]);
         __syncthreads();
-        clear();
-        attend();
+        start();
     }
 
     /* the pair's sums of probabilities; each wave has its half of the latent whole */
@@ -388,25 +389,22 @@ __global__ __launch_bounds__(L_THREADS, 1) void k_attend_latent(AttendArgs a) {
     const float inv = direct ? L == 0.0f ? 0.0f : 1.0f / L : 1.0f;
     uint8_t *out = a.out + (int64_t)(q.q0 + tok) * a.ot + (int64_t)head * a.oh;
     float *po = a.part + (row * a.n_splits + sp) * LC;
-    auto emit = [&](int d, f4 o) __attribute__((always_inline)) {
+    auto emit = [&](int d, f4 o, bool whole) __attribute__((always_inline)) {
         o *= inv;
-        if (!direct) {
-            if (!(L == 0.0f)) *(f4 *)(po + d) = o;
-        } else if (a.aligned) {
-            *(u2 *)(out + 2 * d) = (u2){T::pack(o[0], o[1]), T::pack(o[2], o[3])};
-        } else {
+        if (whole) *(u2_any *)(out + 2 * d) = (u2){T::pack(o[0], o[1]), T::pack(o[2], o[3])};
+        else *(f4 *)(po + d) = o;
+    };
+    auto emit_all = [&](bool whole) __attribute__((always_inline)) {
 #pragma unroll
-            for (int j = 0; j < 4; j++) ((typename T::e *)out)[d + j] = (typename T::e)o[j];
+        for (int i = 0; i < DT * 4; i++) {
+            const f16v &x = acc[i >> 2];
+            const int k = 4 * (i & 3);
+            emit(256 * wt + 8 * i + 4 * half, (f4){x[k], x[k + 1], x[k + 2], x[k + 3]}, whole);
         }
     };
     if (!odd_any) {
-        if (on)
-#pragma unroll
-            for (int i = 0; i < DT * 4; i++) {
-                const f16v &x = acc[i >> 2];
-                const int k = 4 * (i & 3);
-                emit(256 * wt + 8 * i + 4 * half, (f4){x[k], x[k + 1], x[k + 2], x[k + 3]});
-            }
+        if (on && direct) emit_all(true);
+        else if (on && !(L == 0.0f)) emit_all(false);
     } else {   /* with what was taken out of LDS above; the sums go through the steps' LDS, where a loop can index them */
         f4 *own = (f4 *)lds[0] + wave * (DT * 4 * 64);     /* 4 x 32 KiB of the 144 KiB */
 #pragma unroll
@@ -429,7 +427,7 @@ __global__ __launch_bounds__(L_THREADS, 1) void k_attend_latent(AttendArgs a) {
         }
         if (on)
 #pragma unroll 1
-            for (int i = 0; i < DT * 4; i++) emit(256 * wt + 8 * i + 4 * half, own[i * 64 + lane]);
+            for (int i = 0; i < DT * 4; i++) emit(256 * wt + 8 * i + 4 * half, own[i * 64 + lane], direct);
     }
     if (half || wt || !on) return;
     if (direct) {

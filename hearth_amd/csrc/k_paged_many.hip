@@ -86,10 +86,7 @@ __global__ __launch_bounds__(64 * MANY_WAVES, D <= 128 ? 2 : 1) void k_attend_ma
             const unsigned short *p = (const unsigned short *)qp + 16 * i + 8 * half;
             u4 w = {0, 0, 0, 0};
             if (on) {
-                if (a.aligned) w = *(const u4 *)p;
-                else
-#pragma unroll
-                    for (int k = 0; k < 4; k++) w[k] = p[2 * k] | (unsigned)p[2 * k + 1] << 16;
+                w = *(const u4_any *)p;
             }
             qf[i] = __builtin_bit_cast(v8, w ^ flip);
         }
@@ -341,10 +338,7 @@ __global__ __launch_bounds__(64 * MANY_WAVES, D <= 128 ? 2 : 1) void k_attend_ma
                     o[2 + w] = r[1];
                 }
                 uint8_t *p = out + 2 * (32 * i + 8 * b + 8 * half);
-                if (a.aligned) *(u4 *)p = o;
-                else
-#pragma unroll
-                    for (int k = 0; k < 8; k++) ((unsigned short *)p)[k] = (unsigned short)(o[k >> 1] >> (16 * (k & 1)));
+                *(u4_any *)p = o;
             }
         if (a.lse && half == 0) a.lse[row] = l == 0.0f ? NINF : (m + __log2f(l)) * 0.69314718055994531f;
     } else {
