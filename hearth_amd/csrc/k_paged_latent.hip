@@ -102,6 +102,9 @@ __global__ __launch_bounds__(L_THREADS, 1) void k_attend_latent(AttendArgs a) {
         }
     };
     auto have = [&]() __attribute__((always_inline)) { return (pid[0] >= 0 ? 1u : 0u) | (pid[1] >= 0 ? 2u : 0u) | (pid[2] >= 0 ? 4u : 0u) | (pid[3] >= 0 ? 8u : 0u); };
+    /* whether the step has rows that only some columns attend; that some column may not attend each
+     * of its 64 rows (pages: bit u where group u of 16 has one) */
+    auto some_at = [&](int t0) __attribute__((always_inline)) { return full < min(hi, t0 + L_ROWS); };
     auto edge_at = [&](int t0, unsigned h) __attribute__((always_inline)) { return !(t0 + L_ROWS <= full && t0 + L_ROWS <= hi && h == 15u); };
 
     /* 8-bit: 16 codes of row 16 wave + lane / 4, four lanes a chunk */
@@ -131,12 +134,12 @@ __global__ __launch_bounds__(L_THREADS, 1) void k_attend_latent(AttendArgs a) {
             }
         }
     };
-    /* The loaded step made ready in LDS; in edge steps true where a latent element that some
-     * column does not attend is infinite or NaN. */
+    /* The loaded step made ready in LDS; true where it has rows that only some columns attend and an
+     * element of it is infinite or NaN. */
     auto settle = [&](int t0, uint8_t *dst, unsigned h, bool edge) __attribute__((always_inline)) {
         bool odd = false;
         if constexpr (MX) {
-            const bool ok = !edge || (t0 + mr < hi && (h >> wave & 1));
+            const bool ok = !edge || (t0 + mr < hi && (h >> wave & 1)), some = some_at(t0);
             const int at0 = piece_at(mr, 2 * mc), at1 = piece_at(mr, 2 * mc + 1);
 #pragma unroll
             for (int i = 0; i < L_CHUNKS; i++) {
@@ -151,26 +154,25 @@ __global__ __launch_bounds__(L_THREADS, 1) void k_attend_latent(AttendArgs a) {
 #pragma unroll
                     for (int k = 0; k < 2; k++) {
                         w[k] = ok ? w[k] : (u4){0, 0, 0, 0};
-                        odd = odd || T::odd(w[k][0]) || T::odd(w[k][1]) || T::odd(w[k][2]) || T::odd(w[k][3]);
+                        odd = odd || (some && (T::odd(w[k][0]) || T::odd(w[k][1]) || T::odd(w[k][2]) || T::odd(w[k][3])));
                     }
                 *(u4 *)(dst + at0 + 1024 * i) = w[0];
                 *(u4 *)(dst + at1 + 1024 * i) = w[1];
             }
         } else {
             vm_wait();   /* this thread's pieces have arrived */
-            if (edge)
+            if (!(h >> wave & 1) || t0 + 16 * wave + 16 > hi)
+                for (int i = 0; i < 2 * L_CHUNKS; i++)
+                    if (!(h >> wave & 1) || t0 + 16 * wave + (i >= L_CHUNKS ? 8 : 0) + (lane >> 3) >= hi)
+                        *(u4 *)(dst + (2 * wave * L_CHUNKS + i) * 1024 + lane * 16) = (u4){0, 0, 0, 0};
+            if (some_at(t0))
 #pragma unroll 6
                 for (int i = 0; i < 2 * L_CHUNKS; i++) {
-                    const int r = 16 * wave + (i >= L_CHUNKS ? 8 : 0) + (lane >> 3);
-                    u4 *p = (u4 *)(dst + (2 * wave * L_CHUNKS + i) * 1024 + lane * 16);
-                    if (!(h >> wave & 1) || t0 + r >= hi) *p = (u4){0, 0, 0, 0};
-                    else {
-                        const u4 w = *p;
-                        odd = odd || T::odd(w[0]) || T::odd(w[1]) || T::odd(w[2]) || T::odd(w[3]);
-                    }
+                    const u4 w = *(const u4 *)(dst + (2 * wave * L_CHUNKS + i) * 1024 + lane * 16);
+                    odd = odd || T::odd(w[0]) || T::odd(w[1]) || T::odd(w[2]) || T::odd(w[3]);
                 }
         }
-        return odd && t0 + L_ROWS > full;
+        return odd;
     };
 
     unsigned have_now = 0, have_next = 0;
@@ -185,20 +187,31 @@ __global__ __launch_bounds__(L_THREADS, 1) void k_attend_latent(AttendArgs a) {
         }
     };
     start();
+    /* The queries come in by rows, eight lanes 128 bytes, and go to the waves' operands through the
+     * second buffer: read as operands, 32 rows of 32 bytes an instruction, they took 10000 cycles. */
     v8 qf[KS];
     {
-        const uint8_t *qp = a.q + (int64_t)(q.q0 + tok) * a.qt + (int64_t)head * a.qh;
-        const uint8_t *pp = a.q_pe + (int64_t)(q.q0 + tok) * a.pt + (int64_t)head * a.ph;
+        u4 w[2 * L_CHUNKS];
 #pragma unroll
-        for (int i = 0; i < KS; i++) {
-            const int d = 16 * i + 8 * half;
-            const unsigned short *p = d < LC ? (const unsigned short *)qp + d : (const unsigned short *)pp + (d - LC);
-            u4 w = {0, 0, 0, 0};
-            if (on) {
-                w = *(const u4_any *)p;
+        for (int h = 0; h < 2; h++) {
+            const int r = 8 * (2 * wave + h) + (lane >> 3), qc = tile * L_COLS + r;
+            const int qt = qc < cols ? qc / a.heads : 0, qh = qc < cols ? qc % a.heads : 0;
+            const uint8_t *qp = a.q + (int64_t)(q.q0 + qt) * a.qt + (int64_t)qh * a.qh + 16 * (lane & 7);
+            const uint8_t *pp = a.q_pe + (int64_t)(q.q0 + qt) * a.pt + (int64_t)qh * a.ph + 16 * (lane & 7);
+#pragma unroll
+            for (int i = 0; i < L_CHUNKS; i++) {
+                w[L_CHUNKS * h + i] = *(const u4_any *)(i < LC / 64 ? qp + 128 * i : pp);
+                if (qc >= cols) w[L_CHUNKS * h + i] = (u4){0, 0, 0, 0};
             }
-            qf[i] = __builtin_bit_cast(v8, w);
         }
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int i = 0; i < L_CHUNKS; i++)
+                *(u4 *)(lds[1] + piece_at(8 * (2 * wave + h) + (lane >> 3), 8 * i + (lane & 7))) = w[L_CHUNKS * h + i];
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < KS; i++) qf[i] = *(const v8 *)(lds[1] + piece_at(32 * wc + lc, 2 * i + half));
     }
     arrived();
 
@@ -283,7 +296,7 @@ __global__ __launch_bounds__(L_THREADS, 1) void k_attend_latent(AttendArgs a) {
             uint8_t *tl = lds[buf], *nx = lds[buf ^ 1];
             ahead(t0, nx);
             const f16v s = scores(t0, tl);
-            if (edge_at(t0, have_now) && __syncthreads_or(odd_now)) {
+            if (some_at(t0) && __syncthreads_or(odd_now)) {
                 /* an infinity or NaN among rows that some columns do not attend would reach them as
                  * 0 * inf: the scores are done with the rows, so it is taken out of LDS and added at
                  * the end to the columns that attend it */
@@ -386,33 +399,17 @@ __global__ __launch_bounds__(L_THREADS, 1) void k_attend_latent(AttendArgs a) {
     const float L = lds_m[0][32 * wc + lc] + lds_m[1][32 * wc + lc];
     const int64_t row = (int64_t)(q.q0 + tok) * a.heads + head;
     const bool direct = n_sp == 1;
-    const float inv = direct ? L == 0.0f ? 0.0f : 1.0f / L : 1.0f;
-    uint8_t *out = a.out + (int64_t)(q.q0 + tok) * a.ot + (int64_t)head * a.oh;
-    float *po = a.part + (row * a.n_splits + sp) * LC;
-    auto emit = [&](int d, f4 o, bool whole) __attribute__((always_inline)) {
-        o *= inv;
-        if (whole) *(u2_any *)(out + 2 * d) = (u2){T::pack(o[0], o[1]), T::pack(o[2], o[3])};
-        else *(f4 *)(po + d) = o;
-    };
-    auto emit_all = [&](bool whole) __attribute__((always_inline)) {
+    /* The sums go out by rows, through the steps' LDS (column c's 16-byte unit u at u ^ c mod 32, so that
+     * neither the columns' writes nor the rows' reads meet a bank conflict): 16 bytes a lane and row
+     * straight from the registers took 8000 cycles. */
+    auto unit = [&](int c, int u) __attribute__((always_inline)) { return (f4 *)lds[0] + c * (LC / 4) + (u ^ (c & 31)); };
 #pragma unroll
-        for (int i = 0; i < DT * 4; i++) {
-            const f16v &x = acc[i >> 2];
-            const int k = 4 * (i & 3);
-            emit(256 * wt + 8 * i + 4 * half, (f4){x[k], x[k + 1], x[k + 2], x[k + 3]}, whole);
-        }
-    };
-    if (!odd_any) {
-        if (on && direct) emit_all(true);
-        else if (on && !(L == 0.0f)) emit_all(false);
-    } else {   /* with what was taken out of LDS above; the sums go through the steps' LDS, where a loop can index them */
-        f4 *own = (f4 *)lds[0] + wave * (DT * 4 * 64);     /* 4 x 32 KiB of the 144 KiB */
-#pragma unroll
-        for (int i = 0; i < DT * 4; i++) {
-            const f16v &x = acc[i >> 2];
-            const int k = 4 * (i & 3);
-            own[i * 64 + lane] = (f4){x[k], x[k + 1], x[k + 2], x[k + 3]};
-        }
+    for (int i = 0; i < DT * 4; i++) {
+        const f16v &x = acc[i >> 2];
+        const int k = 4 * (i & 3);
+        *unit(32 * wc + lc, 64 * wt + 2 * i + half) = (f4){x[k], x[k + 1], x[k + 2], x[k + 3]};
+    }
+    if (odd_any) {   /* what was taken out of LDS above, added to this wave's half of its columns' latents */
 #pragma unroll 1
         for (int t = max(lo, full / L_ROWS * L_ROWS); t < hi; t++) {
             const int id = word_of(pages, t >> a.b.page_shift);
@@ -420,14 +417,31 @@ __global__ __launch_bounds__(L_THREADS, 1) void k_attend_latent(AttendArgs a) {
             const uint8_t *rp = a.k.data + (int64_t)id * a.k.page_stride + (int64_t)(t & rmask) * (LW * (MX ? 1 : 2));
             const uint8_t *sc = MX ? a.k.scales + (int64_t)id * a.k.scale_page_stride + (t & rmask) * (LW / MX_BLOCK) : nullptr;
 #pragma unroll 1
-            for (int e = 0; e < DT * 16; e++) {
-                const unsigned v = row_elem<T, MX>(rp, sc, 256 * wt + 8 * (e >> 2) + 4 * half + (e & 3));
-                if (T::odd(v)) ((float *)&own[(e >> 2) * 64 + lane])[e & 3] += T::wide(v);
+            for (int e = 0; e < 128; e++) {
+                const int u = 64 * wt + 2 * (e >> 2) + half;
+                const unsigned v = row_elem<T, MX>(rp, sc, 4 * u + (e & 3));
+                if (T::odd(v)) ((float *)unit(32 * wc + lc, u))[e & 3] += T::wide(v);
             }
         }
-        if (on)
-#pragma unroll 1
-            for (int i = 0; i < DT * 4; i++) emit(256 * wt + 8 * i + 4 * half, own[i * 64 + lane], direct);
+    }
+    float *lds_l = (float *)lds_p;
+    if (wt == 0 && half == 0) lds_l[32 * wc + lc] = L;
+    __syncthreads();
+    for (int r = wave; r < L_COLS; r += L_WAVES) {   /* a row a wave at a time */
+        const int rc = tile * L_COLS + r;
+        if (rc >= cols) break;
+        const int rt = rc / a.heads, rh = rc % a.heads;
+        const float Lr = lds_l[r];
+        if (direct) {
+            const float f = Lr == 0.0f ? 0.0f : 1.0f / Lr;
+            const f4 x = *unit(r, 2 * lane) * f, y = *unit(r, 2 * lane + 1) * f;
+            *(u4_any *)(a.out + (int64_t)(q.q0 + rt) * a.ot + (int64_t)rh * a.oh + 16 * lane) =
+                (u4){T::pack(x[0], x[1]), T::pack(x[2], x[3]), T::pack(y[0], y[1]), T::pack(y[2], y[3])};
+        } else if (!(Lr == 0.0f)) {
+            f4 *po = (f4 *)(a.part + (((int64_t)(q.q0 + rt) * a.heads + rh) * a.n_splits + sp) * LC);
+            po[lane] = *unit(r, lane);
+            po[64 + lane] = *unit(r, 64 + lane);
+        }
     }
     if (half || wt || !on) return;
     if (direct) {
