@@ -114,24 +114,26 @@ __global__ __launch_bounds__(L_THREADS, 1) void k_attend_latent(AttendArgs a) {
     /* The loads of the step at t0, to LDS (16-bit) or to registers (8-bit). Every load goes to a row
      * of the cache: rows past hi lie in the same page, those of a page that is not there are taken
      * from page 0; settle clears both. */
-    auto load = [&](int t0, uint8_t *dst) __attribute__((always_inline)) {
+    const uint8_t *from = nullptr, *from_s = nullptr;   /* where this wave's 16 rows of the next step lie; 8-bit: this lane's codes and scales */
+    auto aim = [&](int t0) __attribute__((always_inline)) {
         const int64_t id = max(wave == 0 ? pid[0] : wave == 1 ? pid[1] : wave == 2 ? pid[2] : pid[3], 0);
         const int row = (t0 + 16 * wave) & rmask;
         if constexpr (MX) {
-            const uint8_t *p = a.k.data + id * a.k.page_stride + (row + (lane >> 2)) * LW + 16 * mc;
-            const uint8_t *sp = a.k.scales + id * a.k.scale_page_stride + (row + (lane >> 2)) * (LW / MX_BLOCK) + (mc >> 1);
-#pragma unroll
-            for (int i = 0; i < L_CHUNKS; i++) {
-                sw[i] = *(const u4 *)(p + 64 * i);
-                ss[i] = sp[2 * i];
-            }
+            from = a.k.data + id * a.k.page_stride + (row + (lane >> 2)) * LW + 16 * mc;
+            from_s = a.k.scales + id * a.k.scale_page_stride + (row + (lane >> 2)) * (LW / MX_BLOCK) + (mc >> 1);
         } else {
-            const uint8_t *base = same(a.k.data + id * a.k.page_stride + (int64_t)row * (2 * LW));
-#pragma unroll
-            for (int h = 0; h < 2; h++) {   /* eight rows */
-                const int off = (lane >> 3) * (2 * LW) + ((lane & 7) ^ swz(8 * h + (lane >> 3))) * 16;
-                each<L_CHUNKS>([&](auto i) { to_lds<128 * i.value>(base + h * 8 * (2 * LW), off, dst + ((2 * wave + h) * L_CHUNKS + i.value) * 1024); });
-            }
+            from = same(a.k.data + id * a.k.page_stride + (int64_t)row * (2 * LW));
+        }
+    };
+    constexpr int LOADS = MX ? L_CHUNKS : 2 * L_CHUNKS;
+    const int off8[2] = {(lane >> 3) * (2 * LW) + ((lane & 7) ^ swz(lane >> 3)) * 16, (lane >> 3) * (2 * LW) + ((lane & 7) ^ swz(8 + (lane >> 3))) * 16};
+    auto load = [&](auto j, uint8_t *dst) __attribute__((always_inline)) {   /* the j-th load of a step, j a constant */
+        constexpr int h = j.value / L_CHUNKS, i = j.value % L_CHUNKS;
+        if constexpr (MX) {
+            sw[i] = *(const u4 *)(from + 64 * i);
+            ss[i] = from_s[2 * i];
+        } else {
+            to_lds<128 * i>(from + h * 8 * (2 * LW), off8[h], dst + ((2 * wave + h) * L_CHUNKS + i) * 1024);
         }
     };
     /* The loaded step made ready in LDS; true where it has rows that only some columns attend and an
@@ -183,7 +185,8 @@ __global__ __launch_bounds__(L_THREADS, 1) void k_attend_latent(AttendArgs a) {
         if (lo < hi) {
             load_pages(lo);
             have_next = have();
-            load(lo, lds[0]);
+            aim(lo);
+            each<LOADS>([&](auto j) { load(j, lds[0]); });
         }
     };
     start();
@@ -229,12 +232,12 @@ __global__ __launch_bounds__(L_THREADS, 1) void k_attend_latent(AttendArgs a) {
         }
         __syncthreads();
     };
-    auto ahead = [&](int t0, uint8_t *nx) __attribute__((always_inline)) {
+    auto ahead = [&](int t0) __attribute__((always_inline)) {
         have_now = have_next;
         odd_now = odd_next;
         if (t0 + L_ROWS < hi) {
             have_next = have();
-            load(t0 + L_ROWS, nx);
+            aim(t0 + L_ROWS);
             if (t0 + 2 * L_ROWS < hi) load_pages(t0 + 2 * L_ROWS);
         }
     };
@@ -242,32 +245,39 @@ __global__ __launch_bounds__(L_THREADS, 1) void k_attend_latent(AttendArgs a) {
         if (t0 + L_ROWS < hi) odd_next = settle(t0 + L_ROWS, nx, have_next, edge_at(t0 + L_ROWS, have_next));
         __syncthreads();
     };
-    /* scores of this wave's rows, scaled; rows that are not attended -infinity */
-    auto scores = [&](int t0, const uint8_t *tl) __attribute__((always_inline)) {
+    /* Scores of this wave's rows, scaled; rows that are not attended -infinity. The next step's loads go
+     * out among the products: 18 in a row take 1800 cycles to issue, since the address units take 64
+     * bytes a cycle of the four waves' together. */
+    auto scores = [&](int t0, const uint8_t *tl, uint8_t *nx) __attribute__((always_inline)) {
+        const bool more = t0 + L_ROWS < hi;
         f16v s, s1;   /* two sums: an instruction that adds to the one before it waits for it */
 #pragma unroll
         for (int j = 0; j < 16; j++) s[j] = s1[j] = 0.0f;
         /* Six instructions' reads ahead of their use, in this order: left to itself the compiler puts
          * each read right before its instruction and waits for it. */
-        constexpr int KB = 6;
+        constexpr int KB = 6, BATCHES = KS / KB;
         v8 kr[2][KB];
         auto read_k = [&](int i) __attribute__((always_inline)) { return *(const v8 *)(tl + (k_at ^ 32 * (i & 3)) + 1024 * (i >> 2)); };
 #pragma unroll
         for (int i = 0; i < KB; i++) kr[0][i] = read_k(i);
         in_order();
-#pragma unroll
-        for (int n = 0; n < KS / KB; n++) {
+        each<BATCHES>([&](auto n_) {
+            constexpr int n = n_.value, from_j = LOADS * n / BATCHES, to_j = LOADS * (n + 1) / BATCHES;
 #pragma unroll
             for (int i = 0; i < KB; i++)
-                if (n + 1 < KS / KB) kr[(n + 1) & 1][i] = read_k((n + 1) * KB + i);
+                if (n + 1 < BATCHES) kr[(n + 1) & 1][i] = read_k((n + 1) * KB + i);
             in_order();
-#pragma unroll
-            for (int i = 0; i < KB; i += 2) {
+            each<KB / 2>([&](auto i_) {
+                constexpr int i = 2 * i_.value;
                 s = T::mfma32(kr[n & 1][i], qf[n * KB + i], s);
                 s1 = T::mfma32(kr[n & 1][i + 1], qf[n * KB + i + 1], s1);
-            }
-            in_order();
-        }
+                in_order();
+                if constexpr (from_j + i_.value < to_j) {
+                    if (more) load(std::integral_constant<int, from_j + i_.value>{}, nx);
+                    in_order();
+                }
+            });
+        });
         s = (s + s1) * a.scale2;
         if (edge_at(t0, have_now)) {
             const unsigned long long vis = (attended(t0) & group_rows(have_now)) >> (r0 + 4 * half);
@@ -294,8 +304,8 @@ __global__ __launch_bounds__(L_THREADS, 1) void k_attend_latent(AttendArgs a) {
         begin();
         for (int t0 = lo, buf = 0; t0 < hi; t0 += L_ROWS, buf ^= 1) {
             uint8_t *tl = lds[buf], *nx = lds[buf ^ 1];
-            ahead(t0, nx);
-            const f16v s = scores(t0, tl);
+            ahead(t0);
+            const f16v s = scores(t0, tl, nx);
             if (some_at(t0) && __syncthreads_or(odd_now)) {
                 /* an infinity or NaN among rows that some columns do not attend would reach them as
                  * 0 * inf: the scores are done with the rows, so it is taken out of LDS and added at
@@ -381,8 +391,8 @@ __global__ __launch_bounds__(L_THREADS, 1) void k_attend_latent(AttendArgs a) {
         start();
         begin();
         for (int t0 = lo, buf = 0; t0 < hi; t0 += L_ROWS, buf ^= 1) {
-            ahead(t0, lds[buf ^ 1]);
-            m = fmaxf(m, largest(scores(t0, lds[buf])));
+            ahead(t0);
+            m = fmaxf(m, largest(scores(t0, lds[buf], lds[buf ^ 1])));
             finish(t0, lds[buf ^ 1]);
         }
         if (half == 0) lds_m[wt][32 * wc + lc] = m;
