@@ -30,56 +30,94 @@ struct Few {
     static constexpr int NB = D / BD, PL = BD / 16;      /* blocks; elements of a row a lane takes */
     static constexpr int ES = MX ? 1 : 2;                 /* bytes of a stored element */
 
-    /* scores of 16 cache rows: row pointer of this lane's row */
-    static __device__ __forceinline__ void scores(const uint8_t *row, const uint8_t *sc, int g, const v8 (&q)[NT][KS], f4 (&s)[NT]) {
+    static constexpr int KL = MX ? D / 64 : KS;           /* 16-byte loads of a row for the score */
+    static constexpr int VW = MX ? PL / 4 : PL / 2;       /* words of a row and block for the sum */
+    static constexpr int SW = D / 32 < 4 ? 1 : D / 128;   /* words that hold a row's scales */
+
+    struct K { u4 w[2][KL]; unsigned s[2][SW]; };         /* a lane's row of either tile of 16 */
+    struct V { unsigned w[NB][8][VW]; unsigned s[2][D / 32]; };   /* eight rows; scales of the four rows of either tile */
+
+    /* row: first of the tile in its page (a multiple of 16) */
+    static __device__ __forceinline__ void load_k(K &k, int u, const uint8_t *page, const uint8_t *sc, int row, int g, int lc) {
+        const uint8_t *p = page + (row + lc) * (D * ES) + 16 * g;
+#pragma unroll
+        for (int i = 0; i < KL; i++) k.w[u][i] = *(const u4 *)(p + 64 * i);
         if constexpr (MX) {
-            u4 raw[D / 64];
-            unsigned sb[D / 64];
+            const uint8_t *q = sc + (row + lc) * (D / MX_BLOCK);
+            if constexpr (D == 64) k.s[u][0] = *(const unsigned short *)q;
+            else
 #pragma unroll
-            for (int i = 0; i < D / 64; i++) {
-                raw[i] = *(const u4 *)(row + 64 * i + 16 * g);
-                sb[i] = sc[2 * i + (g >> 1)];
+                for (int i = 0; i < SW; i++) k.s[u][i] = ((const unsigned_any *)q)[i];
+        }
+    }
+    static __device__ __forceinline__ void load_v(V &v, int u, const uint8_t *page, const uint8_t *sc, int row, int g, int lc) {
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const uint8_t *p = page + (row + 4 * g + j) * (D * ES) + (b * BD + lc * PL) * ES;
+                if constexpr (VW == 4) {
+                    const u4 x = *(const u4 *)p;
+#pragma unroll
+                    for (int i = 0; i < 4; i++) v.w[b][4 * u + j][i] = x[i];
+                } else if constexpr (VW == 2) {
+                    const u2 x = *(const u2 *)p;
+                    v.w[b][4 * u + j][0] = x[0]; v.w[b][4 * u + j][1] = x[1];
+                } else {
+                    v.w[b][4 * u + j][0] = *(const unsigned *)p;
+                }
             }
+        if constexpr (MX) {   /* four rows' scales lie side by side */
+            const uint8_t *q = sc + (row + 4 * g) * (D / MX_BLOCK);
 #pragma unroll
-            for (int i = 0; i < D / 64; i++) {
-                const float f = mx_scale(sb[i]);
+            for (int i = 0; i < D / 32; i += D / 32 >= 4 ? 4 : 2)
+                if constexpr (D / 32 >= 4) {
+                    const u4 x = *(const u4_any *)(q + 4 * i);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) v.s[u][i + j] = x[j];
+                } else {
+                    const u2 x = *(const u2_any *)(q + 4 * i);
+                    v.s[u][i] = x[0]; v.s[u][i + 1] = x[1];
+                }
+        }
+    }
+    /* scores of the 16 rows of tile u */
+    static __device__ __forceinline__ void scores(const K &k, int u, int g, const v8 (&q)[NT][KS], f4 (&s)[NT]) {
+#pragma unroll
+        for (int i = 0; i < KL; i++) {
+            if constexpr (MX) {
+                /* block 2 i + g / 2 */
+                const float f = mx_scale(k.s[u][i >> 1] >> (16 * (i & 1) + 8 * (g >> 1)));
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
-                    const unsigned a = raw[i][2 * h], b = raw[i][2 * h + 1];
+                    const unsigned a = k.w[u][i][2 * h], b = k.w[u][i][2 * h + 1];
                     const u4 w = {T::template from_mx8<false>(a, f), T::template from_mx8<true>(a, f),
                                   T::template from_mx8<false>(b, f), T::template from_mx8<true>(b, f)};
 #pragma unroll
                     for (int n = 0; n < NT; n++) s[n] = T::mfma16(__builtin_bit_cast(v8, w), q[n][2 * i + h], s[n]);
                 }
+            } else {
+#pragma unroll
+                for (int n = 0; n < NT; n++) s[n] = T::mfma16(__builtin_bit_cast(v8, k.w[u][i]), q[n][i], s[n]);
             }
-        } else {
-            u4 raw[KS];
-#pragma unroll
-            for (int i = 0; i < KS; i++) raw[i] = *(const u4 *)(row + 64 * i + 16 * g);
-#pragma unroll
-            for (int i = 0; i < KS; i++)
-#pragma unroll
-                for (int n = 0; n < NT; n++) s[n] = T::mfma16(__builtin_bit_cast(v8, raw[i]), q[n][i], s[n]);
         }
     }
-
-    /* PL elements of one cache row as 16-bit pairs */
-    static __device__ __forceinline__ void v_row(const uint8_t *row, const uint8_t *sc, int d, unsigned (&w)[PL / 2]) {
+    /* PL elements of row j, block b, as 16-bit pairs */
+    static __device__ __forceinline__ void v_row(const V &v, int b, int j, int lc, unsigned (&w)[PL / 2]) {
         if constexpr (MX) {
-            const float f = mx_scale(sc[d / MX_BLOCK]);
+            const int jj = j & 3;
+            unsigned x;
+            if constexpr (D == 64) x = v.s[j >> 2][jj >> 1] >> (16 * (jj & 1) + 8 * (lc >> 3));
+            else x = v.s[j >> 2][jj * (D / 128) + b] >> (8 * (lc >> 2));
+            const float f = mx_scale(x);
 #pragma unroll
-            for (int i = 0; i < PL / 4; i++) {
-                const unsigned c = ((const unsigned *)(row + d))[i];
-                w[2 * i] = T::template from_mx8<false>(c, f);
-                w[2 * i + 1] = T::template from_mx8<true>(c, f);
+            for (int i = 0; i < VW; i++) {
+                w[2 * i] = T::template from_mx8<false>(v.w[b][j][i], f);
+                w[2 * i + 1] = T::template from_mx8<true>(v.w[b][j][i], f);
             }
-        } else if constexpr (PL == 8) {
-            const u4 x = *(const u4 *)(row + 2 * d);
-#pragma unroll
-            for (int i = 0; i < 4; i++) w[i] = x[i];
         } else {
-            const u2 x = *(const u2 *)(row + 2 * d);
-            w[0] = x[0]; w[1] = x[1];
+#pragma unroll
+            for (int i = 0; i < VW; i++) w[i] = v.w[b][j][i];
         }
     }
 };
@@ -155,30 +193,55 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_attend_few(AttendArgs a) {
     const uint8_t *kbase = a.k.data + (int64_t)kvh * a.k.head_stride, *vbase = a.v.data + (int64_t)kvh * a.v.head_stride;
     const uint8_t *ksb = MX ? a.k.scales + (int64_t)kvh * a.k.scale_head_stride : nullptr;
     const uint8_t *vsb = MX ? a.v.scales + (int64_t)kvh * a.v.scale_head_stride : nullptr;
-    const Rows &kr = a.k, &vr = a.v;
 
-    for (int t0 = sp * a.chunk + FEW_STEP * wave; t0 < hi; t0 += FEW_STEP * FEW_WAVES) {
-        /* pages of the two tiles of 16 rows; a tile past hi or without a page is not read */
-        int pid[2];
+    /* Pages of the two tiles of 16 rows (-1: none). Every load goes to a row of the cache: rows past hi
+     * lie in the same page, those of a page that is not there are taken from page 0; both are
+     * masked, and cleared in V. */
+    auto page_at = [&](int t) __attribute__((always_inline)) {
+        const int id = t < hi ? word_of(pages, t >> a.b.page_shift) : -1;
+        return page_ok(a.b, id) ? id : -1;
+    };
+    typename F::K kr;
+    typename F::V vw;
+    auto load_k = [&](int t0, const int (&id)[2]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            const int64_t i = max(id[u], 0);
+            F::load_k(kr, u, kbase + i * a.k.page_stride, MX ? ksb + i * a.k.scale_page_stride : nullptr, (t0 + 16 * u) & (page_rows - 1), g, lc);
+        }
+    };
+    auto load_v = [&](int t0, const int (&id)[2]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            const int64_t i = max(id[u], 0);
+            F::load_v(vw, u, vbase + i * a.v.page_stride, MX ? vsb + i * a.v.scale_page_stride : nullptr, (t0 + 16 * u) & (page_rows - 1), g, lc);
+        }
+    };
+    const int first = sp * a.chunk + FEW_STEP * wave;
+    int pid[2] = {-1, -1}, next[2] = {page_at(first), page_at(first + 16)};
+    arrived();
+    if (first < hi) load_k(first, next);
+    /* a step: V on its way before the scores, the next step's K as soon as these have taken K */
+    for (int t0 = first; t0 < hi; t0 += FEW_STEP * FEW_WAVES) {
         bool ok[2];
 #pragma unroll
         for (int u = 0; u < 2; u++) {
-            const int t = t0 + 16 * u;
-            pid[u] = t < hi ? word_of(pages, t >> a.b.page_shift) : -1;
-            ok[u] = page_ok(a.b, pid[u]);
+            pid[u] = next[u];
+            ok[u] = pid[u] >= 0;
+            next[u] = page_at(t0 + FEW_STEP * FEW_WAVES + 16 * u);
         }
+        load_v(t0, pid);
+        in_order();
         f4 s[2][NT];
 #pragma unroll
         for (int u = 0; u < 2; u++) {
 #pragma unroll
             for (int n = 0; n < NT; n++) s[u][n] = (f4){0, 0, 0, 0};
-            if (ok[u]) {
-                const int r = ((t0 + 16 * u) & (page_rows - 1)) + lc;
-                const uint8_t *row = kbase + (int64_t)pid[u] * kr.page_stride + (int64_t)r * (D * ES);
-                const uint8_t *sc = MX ? ksb + (int64_t)pid[u] * kr.scale_page_stride + (int64_t)r * (D / MX_BLOCK) : nullptr;
-                F::scores(row, sc, g, qf, s[u]);
-            }
+            F::scores(kr, u, g, qf, s[u]);
         }
+        in_order();
+        if (t0 + FEW_STEP * FEW_WAVES < hi) load_k(t0 + FEW_STEP * FEW_WAVES, next);
+        in_order();
         const bool whole = t0 + FEW_STEP <= full && t0 + FEW_STEP <= hi && ok[0] && ok[1];
         v8 pf[NT];
 #pragma unroll
@@ -213,21 +276,14 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_attend_few(AttendArgs a) {
 #pragma unroll
         for (int b = 0; b < NB; b++) {
             unsigned w[8][PL / 2];
-            const int d = b * BD + lc * PL;
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-                const int u = j >> 2, t = t0 + 16 * u + 4 * g + (j & 3), r = t & (page_rows - 1);
-                if (ok[u]) {
-                    F::v_row(vbase + (int64_t)pid[u] * vr.page_stride + (int64_t)r * (D * ES),
-                             MX ? vsb + (int64_t)pid[u] * vr.scale_page_stride + (int64_t)r * (D / MX_BLOCK) : nullptr, d, w[j]);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < PL / 2; i++) w[j][i] = 0;
-                }
+                const int u = j >> 2, t = t0 + 16 * u + 4 * g + (j & 3);
+                F::v_row(vw, b, j, lc, w[j]);
                 if (!whole) {
 #pragma unroll
                     for (int i = 0; i < PL / 2; i++) {
-                        w[j][i] = t < hi ? w[j][i] : 0u;
+                        w[j][i] = t < hi && ok[u] ? w[j][i] : 0u;
                         odd = odd || T::odd(w[j][i]);
                         w[j][i] = T::clean(w[j][i]);
                     }
@@ -255,8 +311,8 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_attend_few(AttendArgs a) {
                 if (t0 + FEW_STEP <= full && t0 + FEW_STEP <= hi && page_ok(a.b, word_of(pages, t0 >> a.b.page_shift)) &&
                     page_ok(a.b, word_of(pages, (t0 + 16) >> a.b.page_shift))) break;   /* a step taken as it is */
                 if (!page_ok(a.b, id)) continue;
-                const uint8_t *row = vbase + (int64_t)id * vr.page_stride + (int64_t)(t & (page_rows - 1)) * (D * ES);
-                const uint8_t *sc = MX ? vsb + (int64_t)id * vr.scale_page_stride + (t & (page_rows - 1)) * (D / MX_BLOCK) : nullptr;
+                const uint8_t *row = vbase + (int64_t)id * a.v.page_stride + (int64_t)(t & (page_rows - 1)) * (D * ES);
+                const uint8_t *sc = MX ? vsb + (int64_t)id * a.v.scale_page_stride + (t & (page_rows - 1)) * (D / MX_BLOCK) : nullptr;
 #pragma unroll
                 for (int b = 0; b < NB; b++)
 #pragma unroll
