@@ -8,8 +8,8 @@ For programs that keep many conversations' rows in pages next to (or without) an
     attend(cache, batch, q, out)     grouped-head attention: tokens, chains, draft trees, prompts
     attend_latent(...)               absorbed latent attention over one row a token
 
-Arrays are device tensors: anything with data_ptr(), shape, stride(), dtype, device and
-element_size() as torch tensors have them (torch itself is not imported). Work is enqueued
+Arrays are device tensors: anything with data_ptr(), shape, stride(), dtype, get_device(),
+element_size() and is_contiguous() as torch tensors have them (torch itself is not imported). Work is enqueued
 on `stream` (a HIP stream handle such as torch.cuda.current_stream().cuda_stream; 0 is the
 null stream) of the tensors' device and not waited for; nothing is allocated, so a call may
 be captured into a graph. ValueError for arguments that do not fit together, HearthError for
@@ -111,35 +111,46 @@ def _dtype(t) -> int:
 
 
 def _device(t, what, want=None) -> int:
-    d = t.device
-    if d.type != "cuda":
-        raise ValueError(f"{what} is on {d}, not on a GPU")
-    i = d.index or 0
+    i = t.get_device()
+    if i < 0:
+        raise ValueError(f"{what} is not on a GPU")
     if want is not None and i != want:
-        raise ValueError(f"{what} is on device {i}, the cache on device {want}")
+        raise ValueError(f"{what} is on device {i}, not on device {want}")
     return i
 
 
 def _array(t, what, dev) -> _Array:
     """[tokens, heads, width] with a dense last dimension."""
-    if len(t.shape) != 3:
-        raise ValueError(f"{what}: shape {tuple(t.shape)} is not [tokens, heads, width]")
-    st = t.stride()
-    if t.shape[2] > 1 and st[2] != 1:
-        raise ValueError(f"{what}: the last dimension is not dense (stride {st[2]})")
-    _device(t, what, dev)
-    dt = _dtype(t)
+    shape = t.shape
+    if len(shape) != 3:
+        raise ValueError(f"{what}: shape {tuple(shape)} is not [tokens, heads, width]")
+    _, heads, width = shape
+    st, sh, sw = t.stride()
+    if sw != 1 and width > 1:
+        raise ValueError(f"{what}: the last dimension is not dense (stride {sw})")
+    if t.get_device() != dev:
+        _device(t, what, dev)
+    dt = _seen_dtypes.get(t.dtype)
+    if dt is None:
+        dt = _dtype(t)
     if dt == MX8:
         raise ValueError(f"{what}: {t.dtype} rows live in a cache only")
-    return _Array(t.data_ptr(), st[0], st[1], dt, t.shape[1], t.shape[2])
+    return _Array(t.data_ptr(), st, sh, dt, heads, width)
+
+
+_seen_ints: dict = {}
 
 
 def _ints(t, what, dev, ndim, names=("torch.int32", "int32")):
-    if str(t.dtype) not in names or len(t.shape) != ndim:
-        raise ValueError(f"{what}: {t.dtype}{tuple(t.shape)}, wanted {names[-1]} with {ndim} dimension(s)")
-    if ndim and t.shape[-1] > 1 and t.stride()[-1] != 1:
+    shape, name = t.shape, _seen_ints.get(t.dtype)
+    if name is None:
+        name = _seen_ints[t.dtype] = str(t.dtype)
+    if name not in names or len(shape) != ndim:
+        raise ValueError(f"{what}: {t.dtype}{tuple(shape)}, wanted {names[-1]} with {ndim} dimension(s)")
+    if shape[-1] > 1 and t.stride()[-1] != 1:
         raise ValueError(f"{what}: the last dimension is not dense")
-    _device(t, what, dev)
+    if t.get_device() != dev:
+        _device(t, what, dev)
     return t.data_ptr()
 
 
@@ -260,7 +271,8 @@ def _pair(cache, batch, k, v, what):
         b = _array(v, "v", cache.device)
         if v.shape[0] != k.shape[0] or b.dtype != a.dtype:
             raise ValueError(f"{what}: k is {k.dtype}{tuple(k.shape)}, v {v.dtype}{tuple(v.shape)}")
-    heads, width, latent = cache._s.n_heads, cache._s.width, cache.v is None
+    c = cache._s
+    heads, width, latent = c.n_heads, c.width, cache.v is None
     if not latent and v is None:
         raise ValueError(f"{what}: the cache holds keys and values, v is missing")
     total = a.width + b.width if latent and b is not None else a.width
@@ -275,8 +287,9 @@ def append(cache: Cache, batch: Batch, k, v=None, *, stream=0) -> None:
     """Writes the call's tokens' rows k, v [tokens, heads, width] (float32, float16 or bfloat16)
     into the cache; a latent cache takes the latents as k and their rotated parts as v."""
     a, b, bs = _pair(cache, batch, k, v, "append")
-    _check(_fn("hearth_gpu_kv_append")(cache._ref, bs, byref(a), byref(b) if b is not None else None,
-                                       cache.device, stream), "append")
+    rc = _fn("hearth_gpu_kv_append")(cache._ref, bs, byref(a), byref(b) if b is not None else None, cache.device, stream)
+    if rc:
+        _check(rc, "append")
 
 
 def read(cache: Cache, batch: Batch, k, v=None, *, stream=0) -> None:
@@ -284,8 +297,9 @@ def read(cache: Cache, batch: Batch, k, v=None, *, stream=0) -> None:
     (zeros for rows that are not in the cache). q_start = running sum of kv_len reads whole
     sequences."""
     a, b, bs = _pair(cache, batch, k, v, "read")
-    _check(_fn("hearth_gpu_kv_read")(cache._ref, bs, byref(a), byref(b) if b is not None else None,
-                                     cache.device, stream), "read")
+    rc = _fn("hearth_gpu_kv_read")(cache._ref, bs, byref(a), byref(b) if b is not None else None, cache.device, stream)
+    if rc:
+        _check(rc, "read")
 
 
 def workspace_bytes(cache: Cache, batch: Batch, heads: int, tokens: int | None = None) -> int:
@@ -304,16 +318,11 @@ def _attend(name, cache, batch, q, q_pe, out, lse, scale, workspace, stream):
     dev = cache.device
     if batch.device != dev:
         raise ValueError(f"{name}: the batch is on device {batch.device}, the cache on device {dev}")
-    a, o = _array(q, "q", dev), _array(out, "out", dev)
-    if tuple(out.shape) != tuple(q.shape) or a.dtype != o.dtype:
+    a, o, tokens = _array(q, "q", dev), _array(out, "out", dev), q.shape[0]
+    if out.shape[0] != tokens or o.n_heads != a.n_heads or o.width != a.width or a.dtype != o.dtype:
         raise ValueError(f"{name}: out is {out.dtype}{tuple(out.shape)}, q {q.dtype}{tuple(q.shape)}")
     if a.dtype == F32 or cache._s.dtype not in (MX8, a.dtype):
         raise ValueError(f"{name}: q is {q.dtype} over a cache of {cache.k.dtype}")
-    pe = None
-    if q_pe is not None:
-        pe = _array(q_pe, "q_pe", dev)
-        if tuple(q_pe.shape[:2]) != tuple(q.shape[:2]) or pe.dtype != a.dtype:
-            raise ValueError(f"{name}: q_pe is {q_pe.dtype}{tuple(q_pe.shape)}, q {q.dtype}{tuple(q.shape)}")
     lp = None
     if lse is not None:
         if tuple(lse.shape) != tuple(q.shape[:2]) or str(lse.dtype) != "torch.float32" or not lse.is_contiguous():
@@ -323,17 +332,21 @@ def _attend(name, cache, batch, q, q_pe, out, lse, scale, workspace, stream):
     wp, wb = None, 0
     if workspace is not None:
         _device(workspace, "workspace", dev)
+        if not workspace.is_contiguous():
+            raise ValueError("workspace: not dense")
         wp, wb = workspace.data_ptr(), workspace.numel() * workspace.element_size()
-    bs = batch._of(q.shape[0])
-    if pe is None:
-        rc = _fn("hearth_gpu_attend")(cache._ref, bs, byref(a), byref(o), lp, scale, wp, wb, dev, stream)
+    bs = batch._of(tokens)
+    if q_pe is None:
+        rc = _fn("hearth_gpu_attend")(cache._ref, bs, byref(a), byref(o), lp, float(scale), wp, wb, dev, stream)
     else:
-        rc = _fn("hearth_gpu_attend_latent")(cache._ref, bs, byref(a), byref(pe), byref(o), lp, scale, wp, wb,
-                                             dev, stream)
-    if rc == -1 and (wp is None or wp % 16) and workspace_bytes(cache, batch, a.n_heads, q.shape[0]):
-        raise ValueError(f"{name}: a workspace of {workspace_bytes(cache, batch, a.n_heads, q.shape[0])} bytes on "
-                         f"16 is needed")
-    _check(rc, name)
+        pe = _array(q_pe, "q_pe", dev)
+        if q_pe.shape[0] != tokens or pe.n_heads != a.n_heads or pe.dtype != a.dtype:
+            raise ValueError(f"{name}: q_pe is {q_pe.dtype}{tuple(q_pe.shape)}, q {q.dtype}{tuple(q.shape)}")
+        rc = _fn("hearth_gpu_attend_latent")(cache._ref, bs, byref(a), byref(pe), byref(o), lp, float(scale), wp, wb, dev, stream)
+    if rc == -1 and (wp is None or wp % 16) and (need := workspace_bytes(cache, batch, a.n_heads, tokens)):
+        raise ValueError(f"{name}: a workspace of {need} bytes on 16 is needed")
+    if rc:
+        _check(rc, name)
 
 
 def attend(cache: Cache, batch: Batch, q, out, *, scale: float, lse=None, workspace=None, stream=0) -> None:
@@ -367,29 +380,31 @@ def rope(x, pos, freqs, *, factor=1.0, layout="half", offset=0, out=None, k=None
     dev = _device(x, "x")
     out = x if out is None else out
     ax, ao = _array(x, "x", dev), _array(out, "out", dev)
-    if tuple(out.shape) != tuple(x.shape) or ao.dtype != ax.dtype:
+    tokens = x.shape[0]
+    if out.shape[0] != tokens or ao.n_heads != ax.n_heads or ao.width != ax.width or ao.dtype != ax.dtype:
         raise ValueError(f"out is {out.dtype}{tuple(out.shape)}, x {x.dtype}{tuple(x.shape)}")
     ak = ako = None
     if k is not None:
         k_out = k if k_out is None else k_out
         ak, ako = _array(k, "k", dev), _array(k_out, "k_out", dev)
-        if k.shape[0] != x.shape[0] or ak.width != ax.width or ak.dtype != ax.dtype:
+        if k.shape[0] != tokens or ak.width != ax.width or ak.dtype != ax.dtype:
             raise ValueError(f"k is {k.dtype}{tuple(k.shape)}, x {x.dtype}{tuple(x.shape)}")
-        if tuple(k_out.shape) != tuple(k.shape) or ako.dtype != ak.dtype:
+        if k_out.shape[0] != tokens or ako.n_heads != ak.n_heads or ako.width != ak.width or ako.dtype != ak.dtype:
             raise ValueError(f"k_out is {k_out.dtype}{tuple(k_out.shape)}, k {k.dtype}{tuple(k.shape)}")
     elif k_out is not None:
         raise ValueError("k_out without k")
     p = _ints(pos, "pos", dev, 1, ("torch.int32", "torch.int64", "int32 or int64"))
     f = _ints(freqs, "freqs", dev, 1, ("torch.float64", "float64"))
     n = freqs.shape[0]
-    if pos.shape[0] != x.shape[0]:
-        raise ValueError(f"{pos.shape[0]} positions for {x.shape[0]} tokens")
+    if pos.shape[0] != tokens:
+        raise ValueError(f"{pos.shape[0]} positions for {tokens} tokens")
     if not 1 <= n <= 512 or offset < 0 or offset + 2 * n > ax.width:
         raise ValueError(f"{n} pairs at {offset} do not fit a width of {ax.width}")
-    _check(_fn("hearth_gpu_rope")(byref(ax), byref(ao), byref(ak) if ak is not None else None,
-                                  byref(ako) if ako is not None else None, x.shape[0], p, int("int64" in str(pos.dtype)),
-                                  f, n, offset, int(layout == "interleaved"), int(bool(inverse)), float(factor), dev,
-                                  stream), "rope")
+    rc = _fn("hearth_gpu_rope")(byref(ax), byref(ao), byref(ak) if ak is not None else None,
+                                byref(ako) if ako is not None else None, tokens, p, _seen_ints[pos.dtype] == "torch.int64",
+                                f, n, offset, layout == "interleaved", bool(inverse), float(factor), dev, stream)
+    if rc:
+        _check(rc, "rope")
 
 
 def rope_frequencies(rot: int, base: float = 10000.0, scaling: str | None = None, *, factor: float = 1.0,

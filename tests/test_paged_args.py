@@ -44,6 +44,9 @@ class Fake:
     def stride(self):
         return self._s
 
+    def get_device(self):
+        return self.device.index if self.device.type == "cuda" else -1
+
     def data_ptr(self):
         return self._p
 
