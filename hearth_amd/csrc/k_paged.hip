@@ -157,18 +157,34 @@ __global__ __launch_bounds__(ROPE_THREADS) void k_rope(RopeArgs a, int tok) {
  * above 1.9375) the code is cut to 240, which is within half a step (2^-4) of the value. */
 __device__ __forceinline__ bool fin(float x) { return __builtin_fabsf(x) < __builtin_huge_valf(); }
 
+/* The eight elements that a thread of either kernel takes of each of its tokens: octs threads a
+ * token (grid.z of them where that is more than a workgroup), several tokens a workgroup where it is
+ * less; where they lie is worked out once for COPY_TOKENS tokens. */
+constexpr int COPY_TOKENS = 4;
+struct Place {
+    const Piece *p;
+    int h, d;          /* head; element in the piece's row */
+    int tok, step;     /* first token, tokens a round; tok < 0: none */
+};
+__device__ __forceinline__ Place place_of(const CopyArgs &a) {
+    Place r;
+    const int per = min(a.octs, 256), tpb = 256 / per;   /* threads of a token, tokens a round of the workgroup */
+    int o = threadIdx.x % per + blockIdx.z * 256;
+    const int tl = threadIdx.x / per, o0 = a.p[0].heads * (a.p[0].width / 8);
+    const bool second = o >= o0;
+    r.p = &a.p[second ? 1 : 0];
+    if (second) o -= o0;
+    r.h = o / (r.p->width / 8);
+    r.d = o % (r.p->width / 8) * 8;
+    r.tok = tl < tpb && o + (second ? o0 : 0) < a.octs ? (int)blockIdx.x * tpb * COPY_TOKENS + tl : -1;
+    r.step = tpb;
+    return r;
+}
+
 /* lanes of one block of 32 come here together: octs and every piece's width / 8 are multiples of 4 */
 template <int SRC, int DST, bool WIDE>
-__device__ __forceinline__ void append_item(const CopyArgs &a, const Seq &q, int64_t i) {
+__device__ __forceinline__ void append_item(const CopyArgs &a, const Seq &q, const Piece &p, int tok, int h, int d) {
     using E = Elem<SRC>;
-    const int tok = (int)(i / a.octs);
-    int o = (int)(i % a.octs);
-    const Piece &p0 = a.p[0];
-    const int o0 = p0.heads * (p0.width / 8);
-    const bool second = o >= o0;
-    const Piece &p = a.p[second ? 1 : 0];
-    if (second) o -= o0;
-    const int per = p.width / 8, h = o / per, d = o % per * 8;
     const int pos = q.base + tok;
     if (pos < 0 || pos >= q.kv) return;
     const int page = a.b.pages[(int64_t)blockIdx.y * a.b.ld_pages + (pos >> a.b.page_shift)];
@@ -221,23 +237,20 @@ __device__ __forceinline__ void append_item(const CopyArgs &a, const Seq &q, int
 template <int SRC, int DST, bool WIDE>
 __global__ __launch_bounds__(256) void k_kv_append(CopyArgs a) {
     const Seq q = seq_of(a.b, blockIdx.y);
-    const int64_t items = (int64_t)min(q.n, a.b.max_q) * a.octs;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < items; i += (int64_t)gridDim.x * 256)
-        append_item<SRC, DST, WIDE>(a, q, i);
+    const int n = min(q.n, a.b.max_q);
+    const Place r = place_of(a);
+    if (r.tok < 0) return;
+#pragma unroll
+    for (int i = 0; i < COPY_TOKENS; i++) {
+        const int tok = r.tok + i * r.step;
+        if (tok < n) append_item<SRC, DST, WIDE>(a, q, *r.p, tok, r.h, r.d);
+    }
 }
 
 /* ---------------------------------------------------------------- cache reads */
 template <int DST, int SRC, bool WIDE>
-__device__ __forceinline__ void read_item(const CopyArgs &a, const Seq &q, int64_t i) {
+__device__ __forceinline__ void read_item(const CopyArgs &a, const Seq &q, const Piece &p, int tok, int h, int d) {
     using E = Elem<DST>;
-    const int tok = (int)(i / a.octs);
-    int o = (int)(i % a.octs);
-    const Piece &p0 = a.p[0];
-    const int o0 = p0.heads * (p0.width / 8);
-    const bool second = o >= o0;
-    const Piece &p = a.p[second ? 1 : 0];
-    if (second) o -= o0;
-    const int per = p.width / 8, h = o / per, d = o % per * 8;
     const int pos = q.base + tok;
     int page = -1;
     if (pos >= 0 && pos < q.kv) page = a.b.pages[(int64_t)blockIdx.y * a.b.ld_pages + (pos >> a.b.page_shift)];
@@ -275,15 +288,23 @@ __device__ __forceinline__ void read_item(const CopyArgs &a, const Seq &q, int64
 template <int DST, int SRC, bool WIDE>
 __global__ __launch_bounds__(256) void k_kv_read(CopyArgs a) {
     const Seq q = seq_of(a.b, blockIdx.y);
-    const int64_t items = (int64_t)min(q.n, a.b.max_q) * a.octs;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < items; i += (int64_t)gridDim.x * 256)
-        read_item<DST, SRC, WIDE>(a, q, i);
+    const int n = min(q.n, a.b.max_q);
+    const Place r = place_of(a);
+    if (r.tok < 0) return;
+#pragma unroll
+    for (int i = 0; i < COPY_TOKENS; i++) {
+        const int tok = r.tok + i * r.step;
+        if (tok < n) read_item<DST, SRC, WIDE>(a, q, *r.p, tok, r.h, r.d);
+    }
 }
 
 } // namespace
 
-/* grid of a 1-d loop over `items` in workgroups of 256: the kernels stride over what is left */
-static unsigned grid_for(int64_t items) { return (unsigned)std::min<int64_t>(std::max<int64_t>((items + 255) / 256, 1), 1 << 18); }
+/* grid of place_of */
+static dim3 copy_grid(const CopyArgs &a) {
+    const int tokens = 256 / std::min(a.octs, 256) * COPY_TOKENS;
+    return dim3((a.b.max_q + tokens - 1) / tokens, a.b.n_seqs, (a.octs + 255) / 256);
+}
 
 template <int DT, bool HALF>
 static void rope_t(const RopeArgs &a, bool wide, int tok, hipStream_t st) {
@@ -323,7 +344,7 @@ static void by_types(int arr, int rows, F f) {
 }
 
 void kv_append(const CopyArgs &a, int src_dtype, int cache_dtype, bool aligned, hipStream_t st) {
-    const dim3 grid(grid_for((int64_t)a.b.max_q * a.octs), a.b.n_seqs), block(256);
+    const dim3 grid = copy_grid(a), block(256);
     by_types(src_dtype, cache_dtype, [&](auto s, auto c) {
         if (aligned) hipLaunchKernelGGL((k_kv_append<s.value, c.value, true>), grid, block, 0, st, a);
         else hipLaunchKernelGGL((k_kv_append<s.value, c.value, false>), grid, block, 0, st, a);
@@ -331,7 +352,7 @@ void kv_append(const CopyArgs &a, int src_dtype, int cache_dtype, bool aligned, 
 }
 
 void kv_read(const CopyArgs &a, int dst_dtype, int cache_dtype, bool aligned, hipStream_t st) {
-    const dim3 grid(grid_for((int64_t)a.b.max_q * a.octs), a.b.n_seqs), block(256);
+    const dim3 grid = copy_grid(a), block(256);
     by_types(dst_dtype, cache_dtype, [&](auto d, auto c) {
         if (aligned) hipLaunchKernelGGL((k_kv_read<d.value, c.value, true>), grid, block, 0, st, a);
         else hipLaunchKernelGGL((k_kv_read<d.value, c.value, false>), grid, block, 0, st, a);
