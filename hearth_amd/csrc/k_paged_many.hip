@@ -229,11 +229,29 @@ __global__ __launch_bounds__(64 * MANY_WAVES, D <= 128 ? 2 : 1) void k_attend_ma
         for (int u = 0; u < M::TILES; u++)
 #pragma unroll
             for (int j = 0; j < 16; j++) s[u][j] = 0.0f;
+        /* four instructions' reads ahead of their use, in this order: left to itself the compiler puts
+         * each read right before its instruction */
+        constexpr int KN = KS * M::TILES, AHEAD = 4;
+        v8 kr[2][AHEAD];
+        auto read_k = [&](int n) __attribute__((always_inline)) {
+            return *(const v8 *)(kb + (k_at ^ 32 * (n / M::TILES)) + 32 * (n % M::TILES) * (2 * D));
+        };
 #pragma unroll
-        for (int i = 0; i < KS; i++)
+        for (int n = 0; n < AHEAD; n++) kr[0][n] = read_k(n);
+        in_order();
 #pragma unroll
-            for (int u = 0; u < M::TILES; u++)
-                s[u] = T::mfma32(*(const v8 *)(kb + (k_at ^ 32 * i) + 32 * u * (2 * D)), qf[i], s[u]);
+        for (int b = 0; b < KN / AHEAD; b++) {
+#pragma unroll
+            for (int n = 0; n < AHEAD; n++)
+                if (b + 1 < KN / AHEAD) kr[(b + 1) & 1][n] = read_k((b + 1) * AHEAD + n);
+            in_order();
+#pragma unroll
+            for (int n = 0; n < AHEAD; n++) {
+                const int z = b * AHEAD + n;
+                s[z % M::TILES] = T::mfma32(kr[b & 1][n], qf[z / M::TILES], s[z % M::TILES]);
+            }
+            in_order();
+        }
 
         const bool edge = edge_at(t0, have_now);
         v8 pf[M::GROUPS];
@@ -257,15 +275,17 @@ __global__ __launch_bounds__(64 * MANY_WAVES, D <= 128 ? 2 : 1) void k_attend_ma
                 }
             mx = max32(mx);
         }
-        mx = fmaxf(mx, m);
-        const float ms = mx == NINF ? 0.0f : mx;
-        if (__any(mx > m)) {
-            const float al = exp2_hw(m - ms);
+        /* the sums are rescaled only where a maximum has grown by more than 2^8: until then the
+         * probabilities stay below 2^8, which costs no accuracy in either 16-bit type */
+        if (__any(mx > m + 8.0f)) {
+            mx = fmaxf(mx, m);
+            const float al = mx == NINF ? 0.0f : exp2_hw(m - mx);
             l *= al;
 #pragma unroll
             for (int i = 0; i < DT; i++) acc[i] *= al;
             m = mx;
         }
+        const float ms = m == NINF ? 0.0f : m;
         const float sc = edge ? 1.0f : scale2;
         float ls = 0.0f;
 #pragma unroll
@@ -283,13 +303,29 @@ __global__ __launch_bounds__(64 * MANY_WAVES, D <= 128 ? 2 : 1) void k_attend_ma
             const u4 w = {T::pack(x[o], x[o + 1]), T::pack(x[o + 2], x[o + 3]), T::pack(x[o + 4], x[o + 5]), T::pack(x[o + 6], x[o + 7])};
             pf[g] = __builtin_bit_cast(v8, w);
         }
+        constexpr int VN = M::GROUPS * DT, VAHEAD = VN < 8 ? 2 : 4;
+        v8 vr8[2][VAHEAD];
+        auto read_v = [&](int n) __attribute__((always_inline)) {
+            const int g = n / DT, i = n % DT;
+            const u2 x = read_tr(vb + (v_at[0] ^ 64 * i) + 16 * g * (2 * D)), y = read_tr(vb + (v_at[1] ^ 64 * i) + 16 * g * (2 * D));
+            return __builtin_bit_cast(v8, (u4){x[0], x[1], y[0], y[1]});
+        };
 #pragma unroll
-        for (int g = 0; g < M::GROUPS; g++)
+        for (int n = 0; n < VAHEAD; n++) vr8[0][n] = read_v(n);
+        in_order();
 #pragma unroll
-            for (int i = 0; i < DT; i++) {
-                const u2 x = read_tr(vb + (v_at[0] ^ 64 * i) + 16 * g * (2 * D)), y = read_tr(vb + (v_at[1] ^ 64 * i) + 16 * g * (2 * D));
-                acc[i] = T::mfma32(__builtin_bit_cast(v8, (u4){x[0], x[1], y[0], y[1]}), pf[g], acc[i]);
+        for (int b = 0; b < VN / VAHEAD; b++) {
+#pragma unroll
+            for (int n = 0; n < VAHEAD; n++)
+                if (b + 1 < VN / VAHEAD) vr8[(b + 1) & 1][n] = read_v((b + 1) * VAHEAD + n);
+            in_order();
+#pragma unroll
+            for (int n = 0; n < VAHEAD; n++) {
+                const int z = b * VAHEAD + n;
+                acc[z % DT] = T::mfma32(vr8[b & 1][n], pf[z / DT], acc[z % DT]);
             }
+            in_order();
+        }
         if (more) settle(buf ^ 1, t0 + M::ROWS, have_next);
         __syncthreads();
     }
