@@ -484,8 +484,9 @@ static bool takes_many(int64_t cols) { return cols > 32; }
 
 /* Rows a split takes: enough workgroups for the 256 units (as many as run at once). Few query rows
  * are not split below 512 rows: one launch of 500 rows takes 13.4 us where a split one and its join
- * take 16, at 1000 rows they are level. The others' splits begin at 128 rows (9 tokens over 2000
- * rows: 17 us, with splits from 512 rows on 23). */
+ * take 16, at 1000 rows they are level. Many are split down to 192 rows (85 tokens over 2132 rows:
+ * 26 us, at 128 rows 31; 64 over 500: 17 us, at 256 rows 20), the latent form down to 128 (1 token
+ * over 500 rows: 21 us, at 256 rows 26; 1 over 8192: 30 us, at 64 rows 35). */
 Split attend_split(int n_seqs, int max_q, int kv_cap, int heads, int kv_heads, bool latent) {
     const int64_t cols = (int64_t)max_q * (heads / kv_heads);
     const bool many = !latent && takes_many(cols);
@@ -493,7 +494,7 @@ Split attend_split(int n_seqs, int max_q, int kv_cap, int heads, int kv_heads, b
     const int64_t wgs = std::max<int64_t>((int64_t)n_seqs * kv_heads * ((cols + tile - 1) / tile), 1);
     const int64_t want = std::max<int64_t>(1, at_once / wgs);
     int64_t chunk = (kv_cap + want - 1) / want;
-    chunk = std::max<int64_t>((chunk + step - 1) / step * step, latent || many ? 128 : 512);
+    chunk = std::max<int64_t>((chunk + step - 1) / step * step, latent ? 128 : many ? 192 : 512);
     return {(int)std::min<int64_t>(chunk, 0x40000000), std::max(1, (int)((kv_cap + chunk - 1) / chunk)), many};
 }
 
