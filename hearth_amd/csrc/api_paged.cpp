@@ -17,7 +17,10 @@ using namespace hxp;
 
 namespace {
 
-constexpr int64_t MAX_STRIDE = (int64_t)1 << 46;   /* elements: products with 31-bit indices stay within 64 bits */
+constexpr int64_t MAX_STRIDE = (int64_t)1 << 46;   /* elements: past any memory, and far from 64 bits in bytes */
+constexpr int MAX_ROWS = 0x3fff0000;                /* rows of a sequence that an attention takes: split ends stay within 31 bits */
+constexpr int64_t MAX_LATENT_TILES = 0xfffff0;      /* workgroups of 256 threads in one dimension of a grid (below 2^32 threads) */
+constexpr int64_t MAX_ROPE_ROW = 1 << 24;           /* elements of a token: four of them count within 31 bits */
 
 bool pow2(int x) { return x > 0 && (x & (x - 1)) == 0; }
 
@@ -46,13 +49,15 @@ bool batch_ok(const hearth_gpu_batch *b) {
     if (b->n_seqs && (!b->kv_len || !b->q_start || (b->pages_per_seq && !b->pages))) return false;
     if (b->ld_pages < b->pages_per_seq && b->n_seqs > 1) return false;
     if (b->ld_pages < 0 || b->ld_pages > MAX_STRIDE) return false;
+    if (((uintptr_t)b->pages | (uintptr_t)b->kv_len | (uintptr_t)b->q_start) % 4 || (uintptr_t)b->mask % 8) return false;
     return !b->mask || (b->mask_words >= 1 && (int64_t)b->mask_words * 64 >= b->max_q);
 }
 
 int elem(int dtype) { return dtype == HEARTH_F32 ? 4 : dtype == HEARTH_F16 || dtype == HEARTH_BF16 ? 2 : 0; }
 
-bool array_ok(const hearth_gpu_array *x) {
-    if (!x || !x->data || !elem(x->dtype) || x->n_heads < 1 || x->n_heads > 65536 || x->width < 1 || x->width > 65536) return false;
+/* n: tokens; without any, data may be NULL */
+bool array_ok(const hearth_gpu_array *x, int n) {
+    if (!x || (n && !x->data) || !elem(x->dtype) || x->n_heads < 1 || x->n_heads > 65536 || x->width < 1 || x->width > 65536) return false;
     if ((uintptr_t)x->data % elem(x->dtype)) return false;
     return std::llabs(x->token_stride) <= MAX_STRIDE && std::llabs(x->head_stride) <= MAX_STRIDE;
 }
@@ -80,20 +85,15 @@ Batch batch_of(const hearth_gpu_batch &b, const hearth_gpu_cache &c) {
     return o;
 }
 
-/* OK when the calling thread holds no unread HIP error and `dev` can be made current */
-int launch_on(int dev, const DeviceGuard &g) {
-    (void)dev;
-    return g.ok ? OK : E_IO;
-}
-
 int finish() { return hipGetLastError() == hipSuccess ? OK : E_IO; }   /* this call's launches only */
 
 int copy_call(bool write, const hearth_gpu_cache *c, const hearth_gpu_batch *b, const hearth_gpu_array *k,
               const hearth_gpu_array *v, int dev, void *stream) {
     if (!cache_ok(c) || !batch_ok(b) || dev < 0) return E_ARG;
     const bool latent = !c->v.data;
-    if (v && !v->data) v = nullptr;
-    if (!array_ok(k) || (v && !array_ok(v)) || (!latent && !v)) return E_ARG;
+    const int n = b->n_tokens;
+    if (v && !v->data && n) v = nullptr;
+    if (!array_ok(k, n) || (v && !array_ok(v, n)) || (!latent && !v)) return E_ARG;
     if (v && v->dtype != k->dtype) return E_ARG;
     CopyArgs a{};
     a.b = batch_of(*b, *c);
@@ -117,17 +117,19 @@ int copy_call(bool write, const hearth_gpu_cache *c, const hearth_gpu_batch *b, 
     if (!a.b.n_seqs || !a.b.max_q) return OK;
     if (hipPeekAtLastError() != hipSuccess) return E_IO;
     DeviceGuard g(dev);
-    if (launch_on(dev, g) != OK) return E_IO;
+    if (!g.ok) return E_IO;
     if (write) kv_append(a, k->dtype, c->dtype, wide, (hipStream_t)stream);
     else kv_read(a, k->dtype, c->dtype, wide, (hipStream_t)stream);
     return finish();
 }
 
-/* arguments that both attentions share; value_width: 0 for grouped heads, C for latent rows */
+/* arguments that both attentions share */
 bool attend_shape_ok(const hearth_gpu_cache *c, const hearth_gpu_batch *b, int heads) {
     if (!cache_ok(c) || !batch_ok(b)) return false;
     if (heads < 1 || heads % c->n_heads) return false;
-    if ((int64_t)std::min(b->max_q, b->n_tokens) * heads > (1 << 26)) return false;
+    const Batch o = batch_of(*b, *c);
+    if ((int64_t)o.max_q * heads > (1 << 26) || o.kv_cap > MAX_ROWS) return false;
+    if (!c->v.data && ((int64_t)o.max_q * heads + 63) / 64 * o.n_seqs > MAX_LATENT_TILES) return false;
     if (c->v.data) return c->width == 64 || c->width == 128 || c->width == 256;
     return c->width == 576 && c->n_heads == 1;
 }
@@ -142,14 +144,14 @@ int64_t part_bytes(const hearth_gpu_cache &c, const hearth_gpu_batch &b, int hea
 
 int attend_call(const hearth_gpu_cache *c, const hearth_gpu_batch *b, const hearth_gpu_array *q, const hearth_gpu_array *q_pe,
                 const hearth_gpu_array *out, float *lse, float scale, void *work, size_t work_bytes, int dev, void *stream) {
-    if (!array_ok(q) || !array_ok(out) || !attend_shape_ok(c, b, q->n_heads) || dev < 0 || !std::isfinite(scale)) return E_ARG;
+    if (!q || !attend_shape_ok(c, b, q->n_heads) || !array_ok(q, b->n_tokens) || !array_ok(out, b->n_tokens) || dev < 0) return E_ARG;
     const bool latent = q_pe != nullptr;
-    if (latent != !c->v.data) return E_ARG;
+    if (latent != !c->v.data || (uintptr_t)lse % 4 || !std::isfinite(scale * 1.44269504088896340736f)) return E_ARG;
     if ((q->dtype != HEARTH_F16 && q->dtype != HEARTH_BF16) || out->dtype != q->dtype) return E_ARG;
     if (c->dtype != HEARTH_GPU_MX8 && c->dtype != q->dtype) return E_ARG;
     const int width = latent ? 512 : c->width;
     if (q->width != width || out->width != width || out->n_heads != q->n_heads) return E_ARG;
-    if (latent && (!array_ok(q_pe) || q_pe->dtype != q->dtype || q_pe->n_heads != q->n_heads || q_pe->width != 64)) return E_ARG;
+    if (latent && (!array_ok(q_pe, b->n_tokens) || q_pe->dtype != q->dtype || q_pe->n_heads != q->n_heads || q_pe->width != 64)) return E_ARG;
     Split s;
     const int64_t need = part_bytes(*c, *b, q->n_heads, s);
     if (need && ((uintptr_t)work % 16 || !work)) return E_ARG;
@@ -171,7 +173,7 @@ int attend_call(const hearth_gpu_cache *c, const hearth_gpu_batch *b, const hear
     a.part = (float *)work;
     if (hipPeekAtLastError() != hipSuccess) return E_IO;
     DeviceGuard g(dev);
-    if (launch_on(dev, g) != OK) return E_IO;
+    if (!g.ok) return E_IO;
     if (latent) attend_latent(a, q->dtype, c->dtype, (hipStream_t)stream);
     else attend(a, q->dtype, c->dtype, c->width, s.many, (hipStream_t)stream);
     return finish();
@@ -185,17 +187,19 @@ HEARTH_API int hearth_gpu_rope(const hearth_gpu_array *x, const hearth_gpu_array
                                const hearth_gpu_array *k_out, int n_tokens, const void *pos, int pos64,
                                const double *freqs, int n_freqs, int offset, int interleaved, int inverse,
                                double factor, int dev, void *stream) {
-    if (k && !k->data) k = nullptr;
-    if (k_out && !k_out->data) k_out = nullptr;
-    if (!array_ok(x) || !array_ok(out) || !k != !k_out || n_tokens < 0 || !pos || !freqs || dev < 0) return E_ARG;
+    if (k && !k->data && n_tokens) k = nullptr;
+    if (k_out && !k_out->data && n_tokens) k_out = nullptr;
+    if (!array_ok(x, n_tokens) || !array_ok(out, n_tokens) || !k != !k_out || n_tokens < 0 || (n_tokens && !pos) || !freqs || dev < 0) return E_ARG;
     if (n_freqs < 1 || n_freqs > 512 || offset < 0 || (int64_t)offset + 2 * n_freqs > x->width) return E_ARG;
+    if ((int64_t)x->n_heads * x->width > MAX_ROPE_ROW || (k && (int64_t)k->n_heads * x->width > MAX_ROPE_ROW)) return E_ARG;
+    if (k && n_tokens && (k->data == x->data || k_out->data == out->data)) return E_ARG;
     if (!std::isfinite(factor) || (uintptr_t)pos % (pos64 ? 8 : 4) || (uintptr_t)freqs % 8) return E_ARG;
     RopeArgs a{};
     a.in_place = true;
     a.n_pairs = k ? 2 : 1;
     for (int i = 0; i < a.n_pairs; i++) {
         const hearth_gpu_array *s = i ? k : x, *d = i ? k_out : out;
-        if (!array_ok(s) || !array_ok(d) || s->dtype != x->dtype || d->dtype != x->dtype || s->width != x->width ||
+        if (!array_ok(s, n_tokens) || !array_ok(d, n_tokens) || s->dtype != x->dtype || d->dtype != x->dtype || s->width != x->width ||
             d->width != x->width || s->n_heads != d->n_heads) return E_ARG;
         const int64_t es = elem(s->dtype);
         a.p[i] = {(const uint8_t *)s->data, (uint8_t *)d->data, s->token_stride * es, s->head_stride * es,
@@ -210,7 +214,7 @@ HEARTH_API int hearth_gpu_rope(const hearth_gpu_array *x, const hearth_gpu_array
     if (!n_tokens) return OK;
     if (hipPeekAtLastError() != hipSuccess) return E_IO;
     DeviceGuard g(dev);
-    if (launch_on(dev, g) != OK) return E_IO;
+    if (!g.ok) return E_IO;
     rope(a, x->dtype, (hipStream_t)stream);
     return finish();
 }

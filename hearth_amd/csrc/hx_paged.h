@@ -213,7 +213,7 @@ typedef u4 u4_any __attribute__((aligned(1)));
 typedef u2 u2_any __attribute__((aligned(1)));
 typedef unsigned unsigned_any __attribute__((aligned(1)));
 
-/* the scale of a block from its byte (1 .. 254) */
+/* the scale of a block from its byte (1 to 254) */
 __device__ __forceinline__ float mx_scale(unsigned byte) { return __uint_as_float((byte & 255u) << 23); }
 
 /* maximum / sum of a value over the lanes l, l ^ 32 */

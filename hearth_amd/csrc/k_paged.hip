@@ -73,77 +73,81 @@ template <> struct Elem<DT_BF16> : Elem16<Bf16> {};
  * float32. One workgroup takes `TOK` tokens: cosines and sines once into LDS (n_freqs a
  * token), then all heads of both tensors, eight elements of each half a thread. */
 constexpr int ROPE_THREADS = 256;
-constexpr int ROPE_MAX_FREQS = 512;
+constexpr int ROPE_GROUPS = 1 << 20;   /* at most; longer calls go round */
 
 template <int DT, bool HALF, bool WIDE>
 __global__ __launch_bounds__(ROPE_THREADS) void k_rope(RopeArgs a, int tok) {
     extern __shared__ f2 cs[];   /* [tok][n_freqs] */
     using E = Elem<DT>;
     constexpr int S = E::size;
-    const int t0 = blockIdx.x * tok, nt = min(tok, a.n_tokens - t0);
-    for (int i = threadIdx.x; i < nt * a.n_freqs; i += ROPE_THREADS) {
-        const int t = t0 + i / a.n_freqs, j = i % a.n_freqs;
-        const double pos = a.pos64 ? (double)((const int64_t *)a.pos)[t] : (double)((const int *)a.pos)[t];
-        const double turns = pos * (a.freqs[j] * 0.15915494309189533577);
-        const float r = 2.0f * (float)(turns - rint(turns));
-        float s, c;
-        sincospif(r, &s, &c);
-        cs[i] = (f2){c * a.factor, s * a.factor * a.sign};
-    }
-    __syncthreads();
-    /* an item is 8 elements of each half (HALF), 16 consecutive ones (interleaved), or, WIDE
-     * false, one pair; then the elements outside the rotated part, one at a time */
-    constexpr int PER = WIDE ? 8 : 1;
-    const int items = a.n_freqs / PER;
-    for (int z = 0; z < a.n_pairs; z++) {
-        const auto &p = a.p[z];
-        const int per_tok = p.heads * items;
-        for (int i = threadIdx.x; i < nt * per_tok; i += ROPE_THREADS) {
-            const int tl = i / per_tok, rem = i % per_tok, h = rem / items, j = rem % items * PER;
-            const uint8_t *x = p.x + (int64_t)(t0 + tl) * p.xt + (int64_t)h * p.xh + a.offset * S;
-            uint8_t *y = p.y + (int64_t)(t0 + tl) * p.yt + (int64_t)h * p.yh + a.offset * S;
-            const f2 *w = cs + tl * a.n_freqs + j;
-            if constexpr (WIDE) {
-                const int o0 = HALF ? j * S : 2 * j * S, o1 = HALF ? (j + a.n_freqs) * S : (2 * j + 8) * S;
-                float u[8], v[8], ru[8], rv[8];
-                E::load8(x + o0, true, u);
-                E::load8(x + o1, true, v);
-                if constexpr (HALF) {
+    for (int64_t t0 = (int64_t)blockIdx.x * tok; t0 < a.n_tokens; t0 += (int64_t)gridDim.x * tok) {
+        const int nt = (int)min((int64_t)tok, a.n_tokens - t0);
+        for (int i = threadIdx.x; i < nt * a.n_freqs; i += ROPE_THREADS) {
+            const int64_t t = t0 + i / a.n_freqs;
+            const int j = i % a.n_freqs;
+            const double pos = a.pos64 ? (double)((const int64_t *)a.pos)[t] : (double)((const int *)a.pos)[t];
+            const double turns = pos * (a.freqs[j] * 0.15915494309189533577);
+            const float r = 2.0f * (float)(turns - rint(turns));
+            float s, c;
+            sincospif(r, &s, &c);
+            cs[i] = (f2){c * a.factor, s * a.factor * a.sign};
+        }
+        __syncthreads();
+        /* an item is 8 elements of each half (HALF), 16 consecutive ones (interleaved), or, WIDE
+         * false, one pair; then the elements outside the rotated part, one at a time */
+        constexpr int PER = WIDE ? 8 : 1;
+        const int items = a.n_freqs / PER;
+        for (int z = 0; z < a.n_pairs; z++) {
+            const auto &p = a.p[z];
+            const int per_tok = p.heads * items;
+            for (int i = threadIdx.x; i < nt * per_tok; i += ROPE_THREADS) {
+                const int tl = i / per_tok, rem = i % per_tok, h = rem / items, j = rem % items * PER;
+                const uint8_t *x = p.x + (t0 + tl) * p.xt + (int64_t)h * p.xh + a.offset * S;
+                uint8_t *y = p.y + (t0 + tl) * p.yt + (int64_t)h * p.yh + a.offset * S;
+                const f2 *w = cs + tl * a.n_freqs + j;
+                if constexpr (WIDE) {
+                    const int o0 = HALF ? j * S : 2 * j * S, o1 = HALF ? (j + a.n_freqs) * S : (2 * j + 8) * S;
+                    float u[8], v[8], ru[8], rv[8];
+                    E::load8(x + o0, true, u);
+                    E::load8(x + o1, true, v);
+                    if constexpr (HALF) {
 #pragma unroll
-                    for (int i8 = 0; i8 < 8; i8++) {
-                        ru[i8] = __builtin_fmaf(u[i8], w[i8][0], -(v[i8] * w[i8][1]));
-                        rv[i8] = __builtin_fmaf(v[i8], w[i8][0], u[i8] * w[i8][1]);
+                        for (int i8 = 0; i8 < 8; i8++) {
+                            ru[i8] = __builtin_fmaf(u[i8], w[i8][0], -(v[i8] * w[i8][1]));
+                            rv[i8] = __builtin_fmaf(v[i8], w[i8][0], u[i8] * w[i8][1]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int i4 = 0; i4 < 4; i4++) {
+                            ru[2 * i4] = __builtin_fmaf(u[2 * i4], w[i4][0], -(u[2 * i4 + 1] * w[i4][1]));
+                            ru[2 * i4 + 1] = __builtin_fmaf(u[2 * i4 + 1], w[i4][0], u[2 * i4] * w[i4][1]);
+                            rv[2 * i4] = __builtin_fmaf(v[2 * i4], w[4 + i4][0], -(v[2 * i4 + 1] * w[4 + i4][1]));
+                            rv[2 * i4 + 1] = __builtin_fmaf(v[2 * i4 + 1], w[4 + i4][0], v[2 * i4] * w[4 + i4][1]);
+                        }
                     }
+                    E::store8(y + o0, true, ru);
+                    E::store8(y + o1, true, rv);
                 } else {
-#pragma unroll
-                    for (int i4 = 0; i4 < 4; i4++) {
-                        ru[2 * i4] = __builtin_fmaf(u[2 * i4], w[i4][0], -(u[2 * i4 + 1] * w[i4][1]));
-                        ru[2 * i4 + 1] = __builtin_fmaf(u[2 * i4 + 1], w[i4][0], u[2 * i4] * w[i4][1]);
-                        rv[2 * i4] = __builtin_fmaf(v[2 * i4], w[4 + i4][0], -(v[2 * i4 + 1] * w[4 + i4][1]));
-                        rv[2 * i4 + 1] = __builtin_fmaf(v[2 * i4 + 1], w[4 + i4][0], v[2 * i4] * w[4 + i4][1]);
-                    }
+                    const int o0 = HALF ? j * S : 2 * j * S, o1 = HALF ? (j + a.n_freqs) * S : (2 * j + 1) * S;
+                    const float u = E::load(x + o0), v = E::load(x + o1);
+                    E::store(y + o0, __builtin_fmaf(u, w[0][0], -(v * w[0][1])));
+                    E::store(y + o1, __builtin_fmaf(v, w[0][0], u * w[0][1]));
                 }
-                E::store8(y + o0, true, ru);
-                E::store8(y + o1, true, rv);
-            } else {
-                const int o0 = HALF ? j * S : 2 * j * S, o1 = HALF ? (j + a.n_freqs) * S : (2 * j + 1) * S;
-                const float u = E::load(x + o0), v = E::load(x + o1);
-                E::store(y + o0, __builtin_fmaf(u, w[0][0], -(v * w[0][1])));
-                E::store(y + o1, __builtin_fmaf(v, w[0][0], u * w[0][1]));
+            }
+            if (!a.in_place) {
+                const int rest = a.width - 2 * a.n_freqs;
+                for (int i = threadIdx.x; i < nt * p.heads * rest; i += ROPE_THREADS) {
+                    const int tl = i / (p.heads * rest), rem = i % (p.heads * rest), h = rem / rest;
+                    int d = rem % rest;
+                    if (d >= a.offset) d += 2 * a.n_freqs;
+                    const uint8_t *x = p.x + (t0 + tl) * p.xt + (int64_t)h * p.xh + (int64_t)d * S;
+                    uint8_t *y = p.y + (t0 + tl) * p.yt + (int64_t)h * p.yh + (int64_t)d * S;
+                    if constexpr (S == 4) *(unsigned *)y = *(const unsigned *)x;
+                    else *(unsigned short *)y = *(const unsigned short *)x;
+                }
             }
         }
-        if (!a.in_place) {
-            const int rest = a.width - 2 * a.n_freqs;
-            for (int i = threadIdx.x; i < nt * p.heads * rest; i += ROPE_THREADS) {
-                const int tl = i / (p.heads * rest), rem = i % (p.heads * rest), h = rem / rest;
-                int d = rem % rest;
-                if (d >= a.offset) d += 2 * a.n_freqs;
-                const uint8_t *x = p.x + (int64_t)(t0 + tl) * p.xt + (int64_t)h * p.xh + (int64_t)d * S;
-                uint8_t *y = p.y + (int64_t)(t0 + tl) * p.yt + (int64_t)h * p.yh + (int64_t)d * S;
-                if constexpr (S == 4) *(unsigned *)y = *(const unsigned *)x;
-                else *(unsigned short *)y = *(const unsigned short *)x;
-            }
-        }
+        __syncthreads();   /* the next tokens' cosines go where these lie */
     }
 }
 
@@ -308,7 +312,7 @@ static dim3 copy_grid(const CopyArgs &a) {
 
 template <int DT, bool HALF>
 static void rope_t(const RopeArgs &a, bool wide, int tok, hipStream_t st) {
-    const dim3 grid((a.n_tokens + tok - 1) / tok), block(ROPE_THREADS);
+    const dim3 grid(std::min((a.n_tokens - 1) / tok + 1, ROPE_GROUPS)), block(ROPE_THREADS);
     const size_t lds = sizeof(f2) * (size_t)tok * a.n_freqs;
     if (wide) hipLaunchKernelGGL((k_rope<DT, HALF, true>), grid, block, lds, st, a, tok);
     else hipLaunchKernelGGL((k_rope<DT, HALF, false>), grid, block, lds, st, a, tok);

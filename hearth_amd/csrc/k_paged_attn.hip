@@ -495,7 +495,7 @@ Split attend_split(int n_seqs, int max_q, int kv_cap, int heads, int kv_heads, b
     const int64_t want = std::max<int64_t>(1, at_once / wgs);
     int64_t chunk = (kv_cap + want - 1) / want;
     chunk = std::max<int64_t>((chunk + step - 1) / step * step, latent ? 128 : many ? 192 : 512);
-    return {(int)std::min<int64_t>(chunk, 0x40000000), std::max(1, (int)((kv_cap + chunk - 1) / chunk)), many};
+    return {(int)chunk, std::max(1, (int)((kv_cap + chunk - 1) / chunk)), many};
 }
 
 void attend(const AttendArgs &a, int q_dtype, int cache_dtype, int width, bool many, hipStream_t st) {

@@ -11,8 +11,8 @@ For programs that keep many conversations' rows in pages next to (or without) an
 Arrays are device tensors: anything with data_ptr(), shape, stride(), dtype, get_device(),
 element_size() and is_contiguous() as torch tensors have them (torch itself is not imported). Work is enqueued
 on `stream` (a HIP stream handle such as torch.cuda.current_stream().cuda_stream; 0 is the
-null stream) of the tensors' device and not waited for; nothing is allocated, so a call may
-be captured into a graph. ValueError for arguments that do not fit together, HearthError for
+null stream) of the tensors' device and not waited for, so the tensors must live until it has
+run; nothing is allocated, so a call may be captured into a graph. ValueError for arguments that do not fit together, HearthError for
 a device error.
 
 No counterpart in the reference, whose engine keeps one conversation in float32 on the host.
@@ -255,6 +255,8 @@ class Batch:
 
     def _of(self, n):
         """The struct of a call of n tokens: a copy, so that threads may share a Batch."""
+        if n > 0x7fffffff:
+            raise ValueError(f"{n} tokens (at most 2147483647)")
         if self.mask is not None and self.mask.shape[0] < n:
             raise ValueError(f"mask: {self.mask.shape[0]} rows for {n} tokens")
         s = _BatchS.from_buffer_copy(self._s)
@@ -374,7 +376,8 @@ def rope(x, pos, freqs, *, factor=1.0, layout="half", offset=0, out=None, k=None
     multiplied by factor. freqs: float64 [n] on the device (rope_frequencies). layout "half":
     pairs (j, j + n); "interleaved": (2j, 2j + 1). In place, or into out, which then gets the
     other elements too (out is x or shares nothing with it). k, k_out: a second array of the
-    same width, rotated in the same launch. inverse: by the negative angle."""
+    same width that shares nothing with the first, rotated in the same launch. inverse: by the
+    negative angle."""
     if layout not in ("half", "interleaved"):
         raise ValueError(f"layout {layout!r} is neither 'half' nor 'interleaved'")
     dev = _device(x, "x")
@@ -396,8 +399,12 @@ def rope(x, pos, freqs, *, factor=1.0, layout="half", offset=0, out=None, k=None
     p = _ints(pos, "pos", dev, 1, ("torch.int32", "torch.int64", "int32 or int64"))
     f = _ints(freqs, "freqs", dev, 1, ("torch.float64", "float64"))
     n = freqs.shape[0]
-    if pos.shape[0] != tokens:
+    if pos.shape[0] != tokens or tokens > 0x7fffffff:
         raise ValueError(f"{pos.shape[0]} positions for {tokens} tokens")
+    if max(ax.n_heads, ak.n_heads if ak is not None else 0) * ax.width > 1 << 24:
+        raise ValueError("more than 2^24 elements a token")
+    if ak is not None and tokens and (ak.data == ax.data or ako.data == ao.data):
+        raise ValueError("k shares x's elements")
     if not 1 <= n <= 512 or offset < 0 or offset + 2 * n > ax.width:
         raise ValueError(f"{n} pairs at {offset} do not fit a width of {ax.width}")
     rc = _fn("hearth_gpu_rope")(byref(ax), byref(ao), byref(ak) if ak is not None else None,

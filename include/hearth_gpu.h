@@ -298,7 +298,7 @@ HEARTH_API int hearth_gpu_device(char *name, size_t n);
 /* One tensor of a cache: rows [n_pages][n_heads][page][width], the last two dimensions
  * dense. Strides in elements; data and strides are multiples of 16 bytes. MX8: scales
  * [n_pages][n_heads][page][width / 32], the last two dimensions dense: element = code *
- * 2^(scale - 127). */
+ * 2^(scale - 127), scale bytes 1 to 254 (those that hearth_gpu_kv_append writes). */
 typedef struct hearth_gpu_rows {
     void *data;
     uint8_t *scales;
@@ -342,8 +342,9 @@ typedef struct hearth_gpu_array {
  * x[o + 2j + 1]) (interleaved 1), o = offset, becomes factor * (u cos a - v sin a,
  * v cos a + u sin a); inverse 1 rotates by -a (the gradient's direction). Elements outside
  * [o, o + 2 n_freqs) are copied. out may be x (in place) or share no element with it. x, out
- * and, when k_out.data is not NULL, k, k_out (a second pair, rotated in the same launch) have
- * one dtype and width; positions int32, or int64 when pos64 is 1. */
+ * and, when k_out.data is not NULL, k, k_out (a second pair, rotated in the same launch, which
+ * shares no element with the first) have one dtype and width; positions int32, or int64 when
+ * pos64 is 1. n_freqs up to 512, n_heads * width up to 2^24. */
 HEARTH_API int hearth_gpu_rope(const hearth_gpu_array *x, const hearth_gpu_array *out, const hearth_gpu_array *k,
                                const hearth_gpu_array *k_out, int n_tokens, const void *pos, int pos64,
                                const double *freqs, int n_freqs, int offset, int interleaved, int inverse,
@@ -370,7 +371,8 @@ HEARTH_API int hearth_gpu_kv_read(const hearth_gpu_cache *c, const hearth_gpu_ba
  * HEARTH_F16 or HEARTH_BF16; H a multiple of the cache's heads, head h reads kv head
  * h / (H / n_heads); width 64, 128 or 256. out = softmax(scale * q . k) v over the rows a
  * token attends; a token that attends nothing gets zeros. 16-bit caches have q's dtype; MX8
- * rows are taken as their values in q's dtype. Scores, softmax statistics and sums are
+ * rows are taken as their values in q's dtype, in whose range they must lie. min(max_q,
+ * n_tokens) * H up to 2^26; min(max_kv, pages_per_seq * page) below 2^30 - 65536. Scores, softmax statistics and sums are
  * float32; the probabilities are rounded to q's dtype for the product with v. lse: NULL or
  * [n_tokens][H] float32, the natural logarithm of the sum of exponentials (-infinity where
  * nothing is attended). work: device memory of hearth_gpu_attend_workspace bytes, 16-byte
@@ -382,7 +384,8 @@ HEARTH_API int hearth_gpu_attend(const hearth_gpu_cache *c, const hearth_gpu_bat
 /* The absorbed form of latent attention: q [n_tokens][H][C] (each head's query taken through
  * its key projection) and q_pe [n_tokens][H][R] (its rotated part) against the latent rows'
  * first C and last R elements, out [n_tokens][H][C] = softmax(scale * (q . c + q_pe . pe)) c.
- * C = 512, R = 64, cache width 576, one cache head; everything else as hearth_gpu_attend. */
+ * C = 512, R = 64, cache width 576, one cache head, n_seqs * max_q * H up to 2^29; everything
+ * else as hearth_gpu_attend. */
 HEARTH_API int hearth_gpu_attend_latent(const hearth_gpu_cache *c, const hearth_gpu_batch *b,
                                         const hearth_gpu_array *q, const hearth_gpu_array *q_pe,
                                         const hearth_gpu_array *out, float *lse, float scale, void *work,

@@ -543,3 +543,83 @@ def test_decode_loop_together_eager_and_captured(store):
         assert torch.equal(out, eager[i]), i
         _ = (qs[i].float() @ qs[i].float().transpose(-1, -2)).sum().item()
     assert torch.equal(d1["k"].cpu().view(torch.uint8), d2["k"].cpu().view(torch.uint8))
+
+
+def test_calls_without_tokens():
+    """Empty arrays (whose data may be no address at all) and batches without sequences."""
+    g = _gen(41)
+    d, cache = on_gpu(make_cache(g, 3, 2, 16, 64, BF, "bf16"))
+    _, lat = on_gpu(make_cache(g, 3, 1, 16, 576, BF, "bf16", latent=True))
+    before = d["k"].clone()
+    e = lambda h, w: torch.empty(0, h, w, dtype=BF, device="cuda")
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    freqs = torch.from_numpy(paged.rope_frequencies(64)[0]).cuda()
+    for b in (paged.Batch(torch.zeros(2, 1, dtype=torch.int32, device="cuda"), i32(5, 0), i32(0, 0, 0), max_q=4, max_kv=16),
+              paged.Batch(torch.zeros(0, 1, dtype=torch.int32, device="cuda"), i32(), i32(0), max_q=0, max_kv=0)):
+        paged.rope(e(4, 64), i32(), freqs, k=e(2, 64), stream=_stream())
+        paged.append(cache, b, e(2, 64), e(2, 64), stream=_stream())
+        paged.read(cache, b, e(2, 64), e(2, 64), stream=_stream())
+        paged.attend(cache, b, e(4, 64), e(4, 64), scale=0.1, stream=_stream())
+        paged.append(lat, b, e(1, 512), e(1, 64), stream=_stream())
+        paged.attend_latent(lat, b, e(4, 512), e(4, 64), e(4, 512), scale=0.1, stream=_stream())
+    torch.cuda.synchronize()
+    assert torch.equal(d["k"], before)
+
+
+def test_rope_of_more_tokens_than_one_round():
+    """2^22 + 5 tokens: the workgroups of one launch go round. One pair a token; bf16 results lie
+    within half a step (2^-8) of the exact ones, plus 2^-21 of |u| + |v| for float32 sines, cosines and sums."""
+    T = (1 << 22) + 5
+    x = torch.randn(T, 1, 2, generator=_gen(43)).to(BF)
+    pos = torch.arange(T, dtype=torch.int32)
+    freqs = torch.tensor([0.37], dtype=torch.float64)
+    got = x.cuda()
+    paged.rope(got, pos.cuda(), freqs.cuda(), stream=_stream())
+    want, size = O.rope(x.double(), pos, freqs, 1.0, "half", 0)
+    assert ((got.cpu().double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -21 * size).all()
+
+
+@pytest.mark.parametrize("store", ["bf16", "mx8"])
+@pytest.mark.parametrize("heads,news,latent", [(8, 1, False), (64, 9, False), (16, 2, True)])
+def test_split_calls_captured_and_replayed(store, heads, news, latent):
+    """A split attention and its join (every kernel of rows), and a read of the cache, in one
+    graph whose queries and lengths change between the replays; eager calls of the same
+    workspace's size run between them. Each replay gives the eager call's bits."""
+    g = _gen(heads + news)
+    page, L = 64, 5000
+    W, DV, kv_heads = (576, 512, 1) if latent else (128, 128, 4)
+    pages, n_pages = deal(g, [L], page)
+    _, cache = on_gpu(make_cache(g, n_pages, kv_heads, page, W, BF, store, latent))
+    kv_len, q_start = torch.tensor([L], dtype=torch.int32).cuda(), torch.tensor([0, news], dtype=torch.int32).cuda()
+    b = paged.Batch(pages.cuda(), kv_len, q_start, max_q=news, max_kv=L)
+    need = paged.workspace_bytes(cache, b, heads, news)
+    assert need > 0
+
+    def call(q, out, lse, rows, work):
+        kw = dict(scale=W ** -0.5, lse=lse, workspace=work, stream=_stream())
+        if latent:
+            paged.attend_latent(cache, b, q[..., :512], q[..., 512:], out, **kw)
+            paged.read(cache, b, rows, stream=_stream())
+        else:
+            paged.attend(cache, b, q, out, **kw)
+            paged.read(cache, b, rows, torch.empty_like(rows), stream=_stream())
+
+    def buffers():
+        return (torch.zeros(news, heads, DV, dtype=BF, device="cuda"), torch.zeros(news, heads, device="cuda"),
+                torch.zeros(news, kv_heads, W, dtype=BF, device="cuda"), torch.zeros(need, dtype=torch.uint8, device="cuda"))
+
+    q = torch.zeros(news, heads, W, dtype=BF, device="cuda")
+    mine, other = buffers(), buffers()
+    call(q, *other)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call(q, *mine)
+    for i in range(4):
+        q.copy_(torch.randn(news, heads, W, generator=g).to(BF))
+        kv_len.fill_(L - 700 * i)
+        graph.replay()
+        call(q, *other)
+        torch.cuda.synchronize()
+        for x, y in zip(mine[:3], other[:3]):
+            assert torch.equal(x, y), i

@@ -178,6 +178,62 @@ def test_rope_refusals():
             paged.rope(*args, **kw)
 
 
+def test_sizes_past_the_index_types_are_refused():
+    """Token counts that a 32-bit field would cut, and elements a token that a product would."""
+    c, b = cache(), batch()
+    many = Fake((1 << 31, 2, 64), strides=(0, 64, 1))
+    with pytest.raises(ValueError):
+        paged.append(c, b, many, many)
+    x = Fake((1 << 31, 4, 64), strides=(0, 64, 1))
+    with pytest.raises(ValueError):
+        paged.rope(x, Fake((1 << 31,), "int32"), Fake((32,), "float64"))
+    with pytest.raises(ValueError):
+        paged.rope(Fake((1, 4097, 4096)), Fake((1,), "int32"), Fake((32,), "float64"))
+    x = Fake((5, 4, 64))
+    with pytest.raises(ValueError):      # rotated twice, by whichever thread comes first
+        paged.rope(x, Fake((5,), "int32"), Fake((32,), "float64"), k=x)
+
+
+def test_c_entries_refuse_sizes_and_addresses():
+    """Rows past 2^30, grids past 2^32 threads, addresses off their type's size, a scale that
+    overflows with log2 e: -1 before any device call; no tokens need no arrays."""
+    L = _native.lib()
+    for n, (res, args) in paged._PROTOS.items():
+        getattr(L, n).restype, getattr(L, n).argtypes = res, args
+    E = -1
+    c, b = cache()._s, batch()._of(5)._obj
+    q, r = paged._array(Fake((5, 4, 64)), "q", 0), paged._array(Fake((5, 2, 64)), "k", 0)
+    lat = cache(heads=1, width=576, latent=True)._s
+
+    def but(s, **kw):
+        t = type(s)()
+        ctypes.memmove(byref(t), byref(s), ctypes.sizeof(s))
+        for name, value in kw.items():
+            setattr(t, name, value)
+        return t
+
+    def attend(bb, lse=None, scale=0.1):
+        return L.hearth_gpu_attend(byref(c), byref(bb), byref(q), byref(q), lse, scale, None, 0, 0, None)
+
+    far = but(b, max_kv=0x7fffffff, pages_per_seq=1 << 28, ld_pages=1 << 28)
+    assert attend(far) == E and L.hearth_gpu_attend_workspace(byref(c), byref(far), 4) == E
+    wide = but(b, n_seqs=65535, max_q=1 << 15, n_tokens=1 << 15)
+    assert L.hearth_gpu_attend_workspace(byref(lat), byref(wide), 128) == E
+    assert L.hearth_gpu_attend_workspace(byref(lat), byref(but(wide, max_q=1)), 128) >= 0
+    for field, by in (("pages", 2), ("kv_len", 1), ("q_start", 3), ("mask", 4)):
+        extra = {"mask_words": 1} if field == "mask" else {}
+        bad = but(b, **{field: (1 << 40) + by}, **extra)
+        assert attend(bad) == E, field
+        assert L.hearth_gpu_kv_append(byref(c), byref(bad), byref(r), byref(r), 0, None) == E, field
+    assert attend(b, lse=(1 << 40) + 2) == E
+    assert attend(b, scale=3e38) == E
+    none, no = but(b, n_tokens=0), lambda a: but(a, data=None)
+    assert attend(none) == 0
+    assert L.hearth_gpu_kv_append(byref(c), byref(none), byref(no(r)), byref(no(r)), 0, None) == 0
+    assert L.hearth_gpu_attend(byref(c), byref(none), byref(no(q)), byref(no(q)), None, 0.1, None, 0, 0, None) == 0
+    assert L.hearth_gpu_rope(byref(no(q)), byref(no(q)), byref(no(r)), byref(no(r)), 0, None, 0, 1 << 40, 32, 0, 0, 0, 1.0, 0, None) == 0
+
+
 def test_c_entries_refuse():
     """NULL structs, shapes and strides that the kernels' indexing does not allow: -1, no device call."""
     L = _native.lib()
