@@ -479,10 +479,15 @@ void join_t(const AttendArgs &a, hipStream_t st) {
 
 } // namespace
 
-/* Columns (query rows of a kv head) from which the kernel of many rows is taken. */
+/* Columns (query rows of a kv head) up to which the kernel of few rows is taken, 16 of them a
+ * workgroup: past 32 its further passes over the cache cost more than the other's idle columns. 32
+ * sequences of 4096 rows, width 128, few against many: 8-bit rows 42 and 51 us at 32 columns, 82
+ * and 51 at 40; 16-bit ones 47 and 44 at 32, 111 and 46 at 48; of width 256 108 and 132 at 24. */
 static bool takes_many(int64_t cols) { return cols > 32; }
 
-/* Rows a split takes: enough workgroups for the 256 units (as many as run at once). Few query rows
+/* Rows a split takes: enough workgroups for the 256 units, two each (one of the latent form, which
+ * fills a unit; with four of few rows a unit 32 tokens over 4096 8-bit rows each took 51 us, not 45,
+ * and one over 131071 16-bit rows 59, not 55: more partial sums to write and join). Few query rows
  * are not split below 512 rows: one launch of 500 rows takes 13.4 us where a split one and its join
  * take 16, at 1000 rows they are level. Many are split down to 192 rows (85 tokens over 2132 rows:
  * 26 us, at 128 rows 31; 64 over 500: 17 us, at 256 rows 20), the latent form down to 128 (1 token
@@ -490,7 +495,7 @@ static bool takes_many(int64_t cols) { return cols > 32; }
 Split attend_split(int n_seqs, int max_q, int kv_cap, int heads, int kv_heads, bool latent) {
     const int64_t cols = (int64_t)max_q * (heads / kv_heads);
     const bool many = !latent && takes_many(cols);
-    const int tile = latent ? 64 : many ? 128 : 16, step = latent ? 64 : FEW_STEP * FEW_WAVES, at_once = latent ? 256 : many ? 512 : 1024;
+    const int tile = latent ? 64 : many ? 128 : 16, step = latent ? 64 : FEW_STEP * FEW_WAVES, at_once = latent ? 256 : 512;
     const int64_t wgs = std::max<int64_t>((int64_t)n_seqs * kv_heads * ((cols + tile - 1) / tile), 1);
     const int64_t want = std::max<int64_t>(1, at_once / wgs);
     int64_t chunk = (kv_cap + want - 1) / want;
