@@ -258,7 +258,8 @@ template <int N, class F> __device__ __forceinline__ void each(F f) {   /* f(con
         f(std::integral_constant<int, N - 1>{});
     }
 }
-__device__ __forceinline__ void vm_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+/* all but the wave's last N loads have arrived */
+template <int N = 0> __device__ __forceinline__ void vm_wait() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 
 /* Every load has arrived and the compiler knows it: without this the first use inside a loop of a
  * value loaded before it waits, in every round, for all loads under way. */
