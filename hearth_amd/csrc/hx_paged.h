@@ -246,6 +246,20 @@ __device__ __forceinline__ void to_lds(const uint8_t *base, int off, uint8_t *ds
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 offset:%3" ::"s"(at), "v"(off), "s"(base), "n"(OFS)
                  : "memory");
 }
+/* N instructions of the same kind, the z-th 1 KiB further in memory (from off[z]) and in LDS */
+template <int N>
+__device__ __forceinline__ void to_lds_rows(const uint8_t *base, const int (&off)[N], uint8_t *dst) {
+    static_assert(N == 2 || N == 4);
+    const unsigned at = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)dst);
+    if constexpr (N == 2)
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %3\n\t"
+                     "global_load_lds_dwordx4 %2, %3 offset:1024" ::"s"(at), "v"(off[0]), "v"(off[1]), "s"(base) : "memory");
+    else
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %5\n\t"
+                     "global_load_lds_dwordx4 %2, %5 offset:1024\n\tglobal_load_lds_dwordx4 %3, %5 offset:2048\n\t"
+                     "global_load_lds_dwordx4 %4, %5 offset:3072"
+                     ::"s"(at), "v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3]), "s"(base) : "memory");
+}
 /* the same address for the whole wave, in scalar registers */
 __device__ __forceinline__ const uint8_t *same(const uint8_t *p) {
     const uint64_t x = (uint64_t)p;

@@ -119,26 +119,35 @@ __global__ __launch_bounds__(64 * MANY_WAVES, D <= 128 ? 2 : 1) void k_attend_ma
     const uint8_t *ksb = MX ? a.k.scales + (int64_t)kvh * a.k.scale_head_stride : nullptr;
     const uint8_t *vsb = MX ? a.v.scales + (int64_t)kvh * a.v.scale_head_stride : nullptr;
 
-    int pid[4];                      /* pages of the groups of 16 rows, -1: none */
-    auto load_pages = [&](int t0) {
-#pragma unroll
-        for (int u = 0; u < 4; u++) {
-            const int t = t0 + 16 * u;
-            const int id = u < M::GROUPS && t < hi ? word_of(pages, t >> a.b.page_shift) : -1;
-            pid[u] = page_ok(a.b, id) ? id : -1;
-        }
+    /* Page ids of a step's groups of 16 rows, one a lane (its number in the group of 16 lanes past
+     * GROUPS: none). They are loaded a step before their use, when every load has been waited for;
+     * by scalar instructions, checks included, they took a third of a wave's instructions. */
+    int pv = -1;
+    auto load_pages = [&](int t0) __attribute__((always_inline)) {
+        const int t = t0 + 16 * lane;
+        pv = lane < M::GROUPS && t < hi ? pages[t >> a.b.page_shift] : -1;
+    };
+    unsigned have_now = 0, have_next = 0;   /* bit u: group u has a page */
+    int id_next = 0;                        /* the page of this wave's rows, 0 where there is none */
+    auto look = [&]() __attribute__((always_inline)) {
+        const bool ok = page_ok(a.b, pv);
+        have_next = (unsigned)__ballot(ok);
+        id_next = __builtin_amdgcn_readlane(ok ? pv : 0, wave * (M::ROWS / 4) / 16);
     };
     /* A wave brings in a quarter of the step's rows of K and of V; they lie in one page. 16-bit: 1 KiB
      * of LDS an instruction, 16 bytes a lane; 8-bit: 16 codes a lane, two pieces. */
     constexpr int RW = M::ROWS / 4, LANES = MX ? M::PIECES / 2 : M::PIECES, RI = 64 / LANES, N = RW / RI;   /* lanes of a row, rows an instruction, instructions */
     const int my = wave * RW, lr = lane / LANES, lp = lane % LANES;
+    /* 16-bit: byte of a lane's pieces in memory (the z-th instruction's 1 KiB further, there and in LDS) */
+    int off[N];
+#pragma unroll
+    for (int z = 0; z < N; z++) off[z] = lr * (2 * D) + (lp ^ M::swz(my + z * RI + lr)) * 16;
     u4 sw[MX ? 2 * N : 1];
     unsigned ss[MX ? 2 * N : 1];
     /* Every load goes to a row of the cache: rows past hi lie in the same page, those of a page that
      * is not there are taken from page 0; settle clears both. */
     auto load = [&](int t0, int buf) {
-        const int u = my >> 4;
-        const int64_t id = max(u == 0 ? pid[0] : u == 1 ? pid[1] : u == 2 ? pid[2] : pid[3], 0);
+        const int64_t id = id_next;
         const int row = (t0 + my) & rmask;
         if constexpr (MX) {
             const uint8_t *kp = kbase + id * a.k.page_stride + row * D, *vp = vbase + id * a.v.page_stride + row * D;
@@ -151,12 +160,8 @@ __global__ __launch_bounds__(64 * MANY_WAVES, D <= 128 ? 2 : 1) void k_attend_ma
             }
         } else {
             const uint8_t *kp = same(kbase + id * a.k.page_stride + (int64_t)row * (2 * D)), *vp = same(vbase + id * a.v.page_stride + (int64_t)row * (2 * D));
-#pragma unroll
-            for (int z = 0; z < N; z++) {
-                const int off = (z * RI + lr) * (2 * D) + (lp ^ M::swz(my + z * RI + lr)) * 16;
-                to_lds<0>(kp, off, lds[buf][0] + (my + z * RI) * (2 * D));
-                to_lds<0>(vp, off, lds[buf][1] + (my + z * RI) * (2 * D));
-            }
+            to_lds_rows<N>(kp, off, lds[buf][0] + my * (2 * D));
+            to_lds_rows<N>(vp, off, lds[buf][1] + my * (2 * D));
         }
     };
     /* whether some column of the workgroup may not attend every row of the step at t0 (pages: bit
@@ -202,15 +207,13 @@ __global__ __launch_bounds__(64 * MANY_WAVES, D <= 128 ? 2 : 1) void k_attend_ma
         if (odd) odd_flag = 1;
     };
     if (threadIdx.x == 0) odd_flag = 0;
-    unsigned have_now = 0, have_next = 0;   /* bit u: group u has a page */
-    auto have = [&] { return (pid[0] >= 0 ? 1u : 0u) | (pid[1] >= 0 ? 2u : 0u) | (pid[2] >= 0 ? 4u : 0u) | (pid[3] >= 0 ? 8u : 0u); };
     __syncthreads();
     if (lo < hi) {
         load_pages(lo);
-        have_next = have();
+        look();
         load(lo, 0);
         settle(0, lo, have_next);
-        if (lo + M::ROWS < hi) load_pages(lo + M::ROWS);
+        load_pages(lo + M::ROWS);
     }
     __syncthreads();
 
@@ -224,9 +227,9 @@ __global__ __launch_bounds__(64 * MANY_WAVES, D <= 128 ? 2 : 1) void k_attend_ma
         const bool more = t0 + M::ROWS < hi;
         have_now = have_next;
         if (more) {
-            have_next = have();
+            look();
             load(t0 + M::ROWS, buf ^ 1);
-            if (t0 + 2 * M::ROWS < hi) load_pages(t0 + 2 * M::ROWS);
+            load_pages(t0 + 2 * M::ROWS);
         }
         const uint8_t *kb = lds[buf][0], *vb = lds[buf][1];
         f16v s[M::TILES];
