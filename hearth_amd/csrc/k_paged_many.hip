@@ -226,11 +226,6 @@ __global__ __launch_bounds__(64 * MANY_WAVES, D <= 128 ? 2 : 1) void k_attend_ma
     for (int t0 = lo; t0 < hi; t0 += M::ROWS, buf ^= 1) {
         const bool more = t0 + M::ROWS < hi;
         have_now = have_next;
-        if (more) {
-            look();
-            load(t0 + M::ROWS, buf ^ 1);
-            load_pages(t0 + 2 * M::ROWS);
-        }
         const uint8_t *kb = lds[buf][0], *vb = lds[buf][1];
         f16v s[M::TILES];
 #pragma unroll
@@ -246,6 +241,12 @@ __global__ __launch_bounds__(64 * MANY_WAVES, D <= 128 ? 2 : 1) void k_attend_ma
         };
 #pragma unroll
         for (int n = 0; n < AHEAD; n++) kr[0][n] = read_k(n);
+        in_order();
+        if (more) {   /* the next step's rows are sent for while the first reads are on their way */
+            look();
+            load(t0 + M::ROWS, buf ^ 1);
+            load_pages(t0 + 2 * M::ROWS);
+        }
         in_order();
 #pragma unroll
         for (int b = 0; b < KN / AHEAD; b++) {

@@ -623,3 +623,38 @@ def test_split_calls_captured_and_replayed(store, heads, news, latent):
         torch.cuda.synchronize()
         for x, y in zip(mine[:3], other[:3]):
             assert torch.equal(x, y), i
+
+
+@pytest.mark.parametrize("latent", [False, True])
+def test_two_calls_at_once(latent):
+    """Two split calls on two streams over one cache, each with its workspace, again and again:
+    the bits of the calls one after the other."""
+    g = _gen(47)
+    lens, page = [3000, 1700], 32
+    W, DV, heads, kv_heads = (576, 512, 16, 1) if latent else (128, 128, 16, 4)
+    pages, n_pages = deal(g, lens, page)
+    _, cache = on_gpu(make_cache(g, n_pages, kv_heads, page, W, BF, "mx8", latent))
+    b, _ = batch_of(pages, lens, [1, 1])
+    need = paged.workspace_bytes(cache, b, heads, 2)
+    assert need > 0
+    q = [torch.randn(2, heads, W, generator=g).to(BF).cuda() for _ in range(2)]
+    out, ref = ([torch.zeros(2, heads, DV, dtype=BF, device="cuda") for _ in range(2)] for _ in range(2))
+    work = [torch.empty(need, dtype=torch.uint8, device="cuda") for _ in range(2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+
+    def call(i, o, s):
+        kw = dict(scale=W ** -0.5, workspace=work[i], stream=s)
+        if latent:
+            paged.attend_latent(cache, b, q[i][..., :512], q[i][..., 512:], o, **kw)
+        else:
+            paged.attend(cache, b, q[i], o, **kw)
+
+    for i in range(2):
+        call(i, ref[i], _stream())
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for i in range(2):
+            call(i, out[i], streams[i].cuda_stream)
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert torch.equal(out[i], ref[i])
