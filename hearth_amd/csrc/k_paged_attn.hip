@@ -26,7 +26,7 @@ constexpr int FEW_WAVES = 4, FEW_STEP = 32;   /* a wave takes 32 cache rows at a
 __device__ __forceinline__ unsigned lo16(unsigned a, unsigned b) { return __builtin_amdgcn_perm(b, a, 0x05040100u); }
 __device__ __forceinline__ unsigned hi16(unsigned a, unsigned b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
 
-template <class T, bool MX, int D, int NT>
+template <class T, bool MX, int D>
 struct Few {
     using v8 = typename T::v8;
     static constexpr int KS = D / 32;                    /* matrix steps of the score */
@@ -86,7 +86,7 @@ struct Few {
         }
     }
     /* scores of the 16 rows of tile u */
-    static __device__ __forceinline__ void scores(const K &k, int u, int g, const v8 (&q)[NT][KS], f4 (&s)[NT]) {
+    static __device__ __forceinline__ void scores(const K &k, int u, int g, const v8 (&q)[KS], f4 &s) {
 #pragma unroll
         for (int i = 0; i < KL; i++) {
             if constexpr (MX) {
@@ -97,12 +97,10 @@ struct Few {
                     const unsigned a = k.w[u][i][2 * h], b = k.w[u][i][2 * h + 1];
                     const u4 w = {T::template from_mx8<false>(a, f), T::template from_mx8<true>(a, f),
                                   T::template from_mx8<false>(b, f), T::template from_mx8<true>(b, f)};
-#pragma unroll
-                    for (int n = 0; n < NT; n++) s[n] = T::mfma16(__builtin_bit_cast(v8, w), q[n][2 * i + h], s[n]);
+                    s = T::mfma16(__builtin_bit_cast(v8, w), q[2 * i + h], s);
                 }
             } else {
-#pragma unroll
-                for (int n = 0; n < NT; n++) s[n] = T::mfma16(__builtin_bit_cast(v8, k.w[u][i]), q[n][i], s[n]);
+                s = T::mfma16(__builtin_bit_cast(v8, k.w[u][i]), q[i], s);
             }
         }
     }
@@ -126,11 +124,11 @@ struct Few {
     }
 };
 
-template <class T, bool MX, int D, int NT>
+template <class T, bool MX, int D>
 __global__ __launch_bounds__(64 * FEW_WAVES) void k_attend_few(AttendArgs a) {
-    using F = Few<T, MX, D, NT>;
+    using F = Few<T, MX, D>;
     using v8 = typename T::v8;
-    constexpr int PL = F::PL, NB = F::NB, BD = F::BD, ES = F::ES, CT = 16 * NT;
+    constexpr int PL = F::PL, NB = F::NB, BD = F::BD, ES = F::ES, CT = 16;
     __shared__ float lds_o[FEW_WAVES][16][BD + 4];
     __shared__ float lds_m[FEW_WAVES][CT], lds_l[FEW_WAVES][CT];
 
@@ -147,27 +145,21 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_attend_few(AttendArgs a) {
     const int n_sp = max(1, (q.kv + a.chunk - 1) / a.chunk);
     if (sp >= n_sp) return;
 
-    /* this lane's columns */
-    int tok[NT], head[NT], lim[NT];   /* lim: rows it attends without a mask (causal), or rows before the call's */
-    v8 qf[NT][F::KS];
+    /* this lane's column */
+    v8 qf[F::KS];
+    const int c = tile * CT + lc;
+    const bool on = c < cols;
+    const int tok = on ? c / a.group : 0, head = kvh * a.group + (on ? c % a.group : 0);
+    /* rows it attends without a mask (causal), or rows before the call's */
+    const int lim = !on ? 0 : a.b.mask ? min(q.base, q.kv) : min(q.base + tok + 1, q.kv);
+    const uint8_t *qp = a.q + (int64_t)(q.q0 + tok) * a.qt + (int64_t)head * a.qh;
 #pragma unroll
-    for (int n = 0; n < NT; n++) {
-        const int c = tile * CT + 16 * n + lc;
-        const bool on = c < cols;
-        tok[n] = on ? c / a.group : 0;
-        head[n] = kvh * a.group + (on ? c % a.group : 0);
-        lim[n] = !on ? 0 : a.b.mask ? min(q.base, q.kv) : min(q.base + tok[n] + 1, q.kv);
-        const uint8_t *qp = a.q + (int64_t)(q.q0 + tok[n]) * a.qt + (int64_t)head[n] * a.qh;
-#pragma unroll
-        for (int i = 0; i < F::KS; i++) {
-            const int d = MX ? 64 * (i / 2) + 16 * g + 8 * (i % 2) : 32 * i + 8 * g;
-            const unsigned short *p = (const unsigned short *)qp + d;
-            u4 w = {0, 0, 0, 0};
-            if (on) {
-                w = *(const u4_any *)p;
-            }
-            qf[n][i] = __builtin_bit_cast(v8, w);
-        }
+    for (int i = 0; i < F::KS; i++) {
+        const int d = MX ? 64 * (i / 2) + 16 * g + 8 * (i % 2) : 32 * i + 8 * g;
+        const unsigned short *p = (const unsigned short *)qp + d;
+        u4 w = {0, 0, 0, 0};
+        if (on) w = *(const u4_any *)p;
+        qf[i] = __builtin_bit_cast(v8, w);
     }
     /* rows [lo, hi) of this split that some column of the tile may attend; below `full` every
      * valid column attends every row */
@@ -175,23 +167,18 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_attend_few(AttendArgs a) {
     const int hi = min(min(q.kv, a.b.mask ? q.kv : q.base + t_last + 1), (sp + 1) * a.chunk);
     const int full = a.b.mask ? q.base : q.base + t_first + 1;
 
-    /* which of the 64 rows from t0 on column n of this lane attends (where their pages exist) */
-    auto attended = [&](int n, int t0) {
-        return step_mask(t0, lim[n], hi, q.base,
-                         a.b.mask && tile * CT + 16 * n + lc < cols ? a.b.mask + (int64_t)(q.q0 + tok[n]) * a.b.mask_words : nullptr,
+    /* which of the 64 rows from t0 on this lane's column attends (where their pages exist) */
+    auto attended = [&](int t0) {
+        return step_mask(t0, lim, hi, q.base,
+                         a.b.mask && on ? a.b.mask + (int64_t)(q.q0 + tok) * a.b.mask_words : nullptr,
                          a.b.mask_words);
     };
 
-    f4 acc[NT][NB * PL];
-    float m[NT], l[NT];
+    f4 acc[NB * PL];
+    float m = -__builtin_huge_valf(), l = 0.0f;
     bool odd = false;   /* V held an infinity or NaN in a row that some column does not attend */
 #pragma unroll
-    for (int n = 0; n < NT; n++) {
-        m[n] = -__builtin_huge_valf();
-        l[n] = 0.0f;
-#pragma unroll
-        for (int i = 0; i < NB * PL; i++) acc[n][i] = (f4){0, 0, 0, 0};
-    }
+    for (int i = 0; i < NB * PL; i++) acc[i] = (f4){0, 0, 0, 0};
     const int *pages = a.b.pages + (int64_t)seq * a.b.ld_pages;
     const int page_rows = 1 << a.b.page_shift;
     const uint8_t *kbase = a.k.data + (int64_t)kvh * a.k.head_stride, *vbase = a.v.data + (int64_t)kvh * a.v.head_stride;
@@ -236,47 +223,43 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_attend_few(AttendArgs a) {
         }
         load_v(t0, pid);
         in_order();
-        f4 s[2][NT];
+        f4 s[2];
 #pragma unroll
         for (int u = 0; u < 2; u++) {
-#pragma unroll
-            for (int n = 0; n < NT; n++) s[u][n] = (f4){0, 0, 0, 0};
+            s[u] = (f4){0, 0, 0, 0};
             F::scores(kr, u, g, qf, s[u]);
         }
         in_order();
         if (t0 + FEW_STEP * FEW_WAVES < hi) load_k(t0 + FEW_STEP * FEW_WAVES, next);
         in_order();
         const bool whole = t0 + FEW_STEP <= full && t0 + FEW_STEP <= hi && ok[0] && ok[1];
-        v8 pf[NT];
+        v8 pf;
+        float x[8];
 #pragma unroll
-        for (int n = 0; n < NT; n++) {
-            float x[8];
+        for (int j = 0; j < 8; j++) x[j] = s[j >> 2][j & 3] * a.scale2;
+        if (!whole) {
+            const unsigned long long vis = (attended(t0) & group_rows((ok[0] ? 1u : 0u) | (ok[1] ? 2u : 0u))) >> (4 * g);
 #pragma unroll
-            for (int j = 0; j < 8; j++) x[j] = s[j >> 2][n][j & 3] * a.scale2;
-            if (!whole) {
-                const unsigned long long vis = (attended(n, t0) & group_rows((ok[0] ? 1u : 0u) | (ok[1] ? 2u : 0u))) >> (4 * g);
-#pragma unroll
-                for (int j = 0; j < 8; j++) x[j] = vis >> (16 * (j >> 2) + (j & 3)) & 1 ? x[j] : -__builtin_huge_valf();
-            }
-            float mx = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
-            mx = fmaxf(m[n], max16(max32(mx)));
-            const float ms = mx == -__builtin_huge_valf() ? 0.0f : mx;
-            if (__any(mx > m[n])) {
-                const float al = exp2_hw(m[n] - ms);
-                l[n] *= al;
-#pragma unroll
-                for (int i = 0; i < NB * PL; i++) acc[n][i] *= al;
-                m[n] = mx;
-            }
-            float p[8];
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                p[j] = exp2_hw(x[j] - ms);
-                l[n] += p[j];
-            }
-            const u4 w = {T::pack(p[0], p[1]), T::pack(p[2], p[3]), T::pack(p[4], p[5]), T::pack(p[6], p[7])};
-            pf[n] = __builtin_bit_cast(v8, w);
+            for (int j = 0; j < 8; j++) x[j] = vis >> (16 * (j >> 2) + (j & 3)) & 1 ? x[j] : -__builtin_huge_valf();
         }
+        float mx = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+        mx = fmaxf(m, max16(max32(mx)));
+        const float ms = mx == -__builtin_huge_valf() ? 0.0f : mx;
+        if (__any(mx > m)) {
+            const float al = exp2_hw(m - ms);
+            l *= al;
+#pragma unroll
+            for (int i = 0; i < NB * PL; i++) acc[i] *= al;
+            m = mx;
+        }
+        float p[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            p[j] = exp2_hw(x[j] - ms);
+            l += p[j];
+        }
+        const u4 w = {T::pack(p[0], p[1]), T::pack(p[2], p[3]), T::pack(p[4], p[5]), T::pack(p[6], p[7])};
+        pf = __builtin_bit_cast(v8, w);
 #pragma unroll
         for (int b = 0; b < NB; b++) {
             unsigned w[8][PL / 2];
@@ -297,11 +280,8 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_attend_few(AttendArgs a) {
             for (int i = 0; i < PL / 2; i++) {
                 const u4 e = {lo16(w[0][i], w[1][i]), lo16(w[2][i], w[3][i]), lo16(w[4][i], w[5][i]), lo16(w[6][i], w[7][i])};
                 const u4 o = {hi16(w[0][i], w[1][i]), hi16(w[2][i], w[3][i]), hi16(w[4][i], w[5][i]), hi16(w[6][i], w[7][i])};
-#pragma unroll
-                for (int n = 0; n < NT; n++) {
-                    acc[n][b * PL + 2 * i] = T::mfma16(__builtin_bit_cast(v8, e), pf[n], acc[n][b * PL + 2 * i]);
-                    acc[n][b * PL + 2 * i + 1] = T::mfma16(__builtin_bit_cast(v8, o), pf[n], acc[n][b * PL + 2 * i + 1]);
-                }
+                acc[b * PL + 2 * i] = T::mfma16(__builtin_bit_cast(v8, e), pf, acc[b * PL + 2 * i]);
+                acc[b * PL + 2 * i + 1] = T::mfma16(__builtin_bit_cast(v8, o), pf, acc[b * PL + 2 * i + 1]);
             }
         }
     }
@@ -324,79 +304,71 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_attend_few(AttendArgs a) {
 #pragma unroll
                         for (int i = 0; i < 4; i++) {
                             const unsigned x = row_elem<T, MX>(row, sc, b * BD + (4 * g + i) * PL + j);
-#pragma unroll
-                            for (int n = 0; n < NT; n++)
-                                acc[n][b * PL + j][i] += T::odd(x) && (attended(n, t) & 1) ? T::wide(x) : 0.0f;
+                            acc[b * PL + j][i] += T::odd(x) && (attended(t) & 1) ? T::wide(x) : 0.0f;
                         }
             }
         }
     }
 
     /* the four waves' columns together: a lane's sums cover its own rows of each step only */
-#pragma unroll
-    for (int n = 0; n < NT; n++) {
-        l[n] = sum16(sum32(l[n]));
-        if (g == 0) { lds_m[wave][16 * n + lc] = m[n]; lds_l[wave][16 * n + lc] = l[n]; }
-    }
+    l = sum16(sum32(l));
+    if (g == 0) { lds_m[wave][lc] = m; lds_l[wave][lc] = l; }
     __syncthreads();
     const bool direct = n_sp == 1;
     const int oc = threadIdx.x >> 4, od = (threadIdx.x & 15) * PL;   /* output column and element of this thread */
+    float M = lds_m[0][lc];
 #pragma unroll
-    for (int n = 0; n < NT; n++) {
-        float M = lds_m[0][16 * n + lc];
+    for (int w = 1; w < FEW_WAVES; w++) M = fmaxf(M, lds_m[w][lc]);
+    const float f = m == -__builtin_huge_valf() ? (l == 0.0f ? 0.0f : 1.0f) : exp2_hw(m - M);
+    /* the output thread's column */
+    float Mo = lds_m[0][oc], Lo = 0.0f;
 #pragma unroll
-        for (int w = 1; w < FEW_WAVES; w++) M = fmaxf(M, lds_m[w][16 * n + lc]);
-        const float f = m[n] == -__builtin_huge_valf() ? (l[n] == 0.0f ? 0.0f : 1.0f) : exp2_hw(m[n] - M);
-        /* the output thread's column */
-        float Mo = lds_m[0][16 * n + oc], Lo = 0.0f;
+    for (int w = 1; w < FEW_WAVES; w++) Mo = fmaxf(Mo, lds_m[w][oc]);
 #pragma unroll
-        for (int w = 1; w < FEW_WAVES; w++) Mo = fmaxf(Mo, lds_m[w][16 * n + oc]);
+    for (int w = 0; w < FEW_WAVES; w++) {
+        const float mw = lds_m[w][oc], lw = lds_l[w][oc];
+        Lo += mw == -__builtin_huge_valf() ? lw : lw * exp2_hw(mw - Mo);
+    }
+    const int co = tile * CT + oc;
+    const bool here = co < cols;
+    const int ot = here ? co / a.group : 0, oh = kvh * a.group + (here ? co % a.group : 0);
+    const int64_t row = (int64_t)(q.q0 + ot) * a.heads + oh;
 #pragma unroll
-        for (int w = 0; w < FEW_WAVES; w++) {
-            const float mw = lds_m[w][16 * n + oc], lw = lds_l[w][16 * n + oc];
-            Lo += mw == -__builtin_huge_valf() ? lw : lw * exp2_hw(mw - Mo);
+    for (int b = 0; b < NB; b++) {
+        if (b) __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int j = 0; j < PL; j += 4)
+                *(f4 *)&lds_o[wave][lc][(4 * g + i) * PL + j] =
+                    (f4){acc[b * PL + j][i] * f, acc[b * PL + j + 1][i] * f, acc[b * PL + j + 2][i] * f, acc[b * PL + j + 3][i] * f};
+        __syncthreads();
+        if (!here) continue;
+        float o[PL];
+#pragma unroll
+        for (int j = 0; j < PL; j++) {
+            o[j] = 0.0f;
+#pragma unroll
+            for (int w = 0; w < FEW_WAVES; w++) o[j] += lds_o[w][oc][od + j];
         }
-        const int c = tile * CT + 16 * n + oc;
-        const bool on = c < cols;
-        const int ot = on ? c / a.group : 0, oh = kvh * a.group + (on ? c % a.group : 0);
-        const int64_t row = (int64_t)(q.q0 + ot) * a.heads + oh;
+        if (direct) {
+            const float inv = Lo == 0.0f ? 0.0f : 1.0f / Lo;
+            uint8_t *out = a.out + (int64_t)(q.q0 + ot) * a.ot + (int64_t)oh * a.oh + 2 * (b * BD + od);
 #pragma unroll
-        for (int b = 0; b < NB; b++) {
-            if (n + b) __syncthreads();
+            for (int j = 0; j < PL; j += 4)
+                *(u2_any *)(out + 2 * j) = (u2){T::pack(o[j] * inv, o[j + 1] * inv), T::pack(o[j + 2] * inv, o[j + 3] * inv)};
+        } else if (!(Lo == 0.0f)) {
+            float *po = a.part + (row * a.n_splits + sp) * D + b * BD + od;
 #pragma unroll
-            for (int i = 0; i < 4; i++)
-#pragma unroll
-                for (int j = 0; j < PL; j += 4)
-                    *(f4 *)&lds_o[wave][lc][(4 * g + i) * PL + j] =
-                        (f4){acc[n][b * PL + j][i] * f, acc[n][b * PL + j + 1][i] * f, acc[n][b * PL + j + 2][i] * f, acc[n][b * PL + j + 3][i] * f};
-            __syncthreads();
-            if (!on) continue;
-            float o[PL];
-#pragma unroll
-            for (int j = 0; j < PL; j++) {
-                o[j] = 0.0f;
-#pragma unroll
-                for (int w = 0; w < FEW_WAVES; w++) o[j] += lds_o[w][oc][od + j];
-            }
-            if (direct) {
-                const float inv = Lo == 0.0f ? 0.0f : 1.0f / Lo;
-                uint8_t *out = a.out + (int64_t)(q.q0 + ot) * a.ot + (int64_t)oh * a.oh + 2 * (b * BD + od);
-#pragma unroll
-                for (int j = 0; j < PL; j += 4)
-                    *(u2_any *)(out + 2 * j) = (u2){T::pack(o[j] * inv, o[j + 1] * inv), T::pack(o[j + 2] * inv, o[j + 3] * inv)};
-            } else if (!(Lo == 0.0f)) {
-                float *po = a.part + (row * a.n_splits + sp) * D + b * BD + od;
-#pragma unroll
-                for (int j = 0; j < PL; j += 4) *(f4 *)(po + j) = (f4){o[j], o[j + 1], o[j + 2], o[j + 3]};
-            }
+            for (int j = 0; j < PL; j += 4) *(f4 *)(po + j) = (f4){o[j], o[j + 1], o[j + 2], o[j + 3]};
         }
-        if (on && (threadIdx.x & 15) == 0) {
-            if (!direct) {
-                float *ml = a.part + (int64_t)a.b.n_tokens * a.heads * a.n_splits * D + (row * a.n_splits + sp) * 2;
-                ml[0] = Mo;
-                ml[1] = Lo;
-            } else if (a.lse) a.lse[row] = Lo == 0.0f ? -__builtin_huge_valf() : (Mo + __log2f(Lo)) * 0.69314718055994531f;
-        }
+    }
+    if (here && (threadIdx.x & 15) == 0) {
+        if (!direct) {
+            float *ml = a.part + (int64_t)a.b.n_tokens * a.heads * a.n_splits * D + (row * a.n_splits + sp) * 2;
+            ml[0] = Mo;
+            ml[1] = Lo;
+        } else if (a.lse) a.lse[row] = Lo == 0.0f ? -__builtin_huge_valf() : (Mo + __log2f(Lo)) * 0.69314718055994531f;
     }
 }
 
@@ -469,7 +441,7 @@ template <class T, bool MX, int D>
 void few_t(const AttendArgs &a, hipStream_t st) {
     const int tiles = (a.b.max_q * a.group + 15) / 16;
     const dim3 grid((unsigned)a.n_splits * a.kv_heads * tiles, 1, a.b.n_seqs);
-    hipLaunchKernelGGL((k_attend_few<T, MX, D, 1>), grid, dim3(64 * FEW_WAVES), 0, st, a);
+    hipLaunchKernelGGL((k_attend_few<T, MX, D>), grid, dim3(64 * FEW_WAVES), 0, st, a);
 }
 
 template <class T, int DV>

@@ -91,9 +91,7 @@ __global__ __launch_bounds__(64 * MANY_WAVES, D <= 128 ? 2 : 1) void k_attend_ma
         for (int i = 0; i < KS; i++) {
             const unsigned short *p = (const unsigned short *)qp + 16 * i + 8 * half;
             u4 w = {0, 0, 0, 0};
-            if (on) {
-                w = *(const u4_any *)p;
-            }
+            if (on) w = *(const u4_any *)p;
             qf[i] = __builtin_bit_cast(v8, w ^ flip);
         }
     }
