@@ -162,9 +162,7 @@ __device__ __forceinline__ unsigned long long group_rows(unsigned have) {
 /* 16-bit types: the matrix instructions and conversions of one type */
 struct Bf16 {
     using v8 = b8;
-    using v2 = b2;
     using e = __bf16;
-    static constexpr int dt = DT_BF16;
     static __device__ __forceinline__ f4 mfma16(v8 a, v8 b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
     static __device__ __forceinline__ f16v mfma32(v8 a, v8 b, f16v c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
     /* codes (two bytes of x, the upper two with HI) times a power of two; exact but for underflow */
@@ -183,9 +181,7 @@ struct Bf16 {
 };
 struct F16 {
     using v8 = h8;
-    using v2 = h2;
     using e = _Float16;
-    static constexpr int dt = DT_F16;
     static __device__ __forceinline__ f4 mfma16(v8 a, v8 b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
     static __device__ __forceinline__ f16v mfma32(v8 a, v8 b, f16v c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
     template <bool HI> static __device__ __forceinline__ unsigned from_mx8(unsigned x, float s) {
@@ -253,12 +249,13 @@ __device__ __forceinline__ void to_lds_rows(const uint8_t *base, const int (&off
     const unsigned at = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)dst);
     if constexpr (N == 2)
         asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %3\n\t"
-                     "global_load_lds_dwordx4 %2, %3 offset:1024" ::"s"(at), "v"(off[0]), "v"(off[1]), "s"(base) : "memory");
+                     "global_load_lds_dwordx4 %2, %3 offset:%4" ::"s"(at), "v"(off[0]), "v"(off[1]), "s"(base), "n"(1 << 10) : "memory");
     else
         asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %5\n\t"
-                     "global_load_lds_dwordx4 %2, %5 offset:1024\n\tglobal_load_lds_dwordx4 %3, %5 offset:2048\n\t"
-                     "global_load_lds_dwordx4 %4, %5 offset:3072"
-                     ::"s"(at), "v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3]), "s"(base) : "memory");
+                     "global_load_lds_dwordx4 %2, %5 offset:%6\n\tglobal_load_lds_dwordx4 %3, %5 offset:%7\n\t"
+                     "global_load_lds_dwordx4 %4, %5 offset:%8"
+                     ::"s"(at), "v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3]), "s"(base), "n"(1 << 10), "n"(2 << 10), "n"(3 << 10)
+                     : "memory");
 }
 /* the same address for the whole wave, in scalar registers */
 __device__ __forceinline__ const uint8_t *same(const uint8_t *p) {

@@ -1,9 +1,9 @@
 /*
  * k_paged.hip — rotary positions and the writes and reads of a paged cache. All three move
  * each element once and are bound by HBM for prompts and by launch latency for single tokens:
- * rotating 64 of 192 elements of 2001 tokens of 128 heads (66 MB) takes 13.4 us (4.9 TB/s, a large
- * copy's rate), quantising 3 x 4093 rows (31 MB) 13.5 us, reading 8 x 4095 back (71 MB) 18.3 us
- * (3.9 TB/s), the rows of 32 single tokens 3.3 us.
+ * rotating 64 of 192 elements of 2001 tokens of 128 heads (66 MB) takes 13.9 us (4.8 TB/s, near a
+ * large copy's 4.9), quantising 3 x 4093 rows (31 MB) 13.2 us, reading 8 x 4095 back (71 MB) 19 us
+ * (3.7 TB/s), the rows of 32 single tokens 3.5 us.
  */
 #include "hx_paged.h"
 

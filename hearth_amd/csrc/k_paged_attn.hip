@@ -8,8 +8,8 @@
  * that the second product takes for the same column: the probabilities never leave the
  * registers. V comes in by rows (8 elements of 8 cache rows a lane) and is transposed there,
  * a byte permutation a pair of elements.
- * It is bound by the cache's bytes: 268 MB of one token over 131071 rows in 49.5 us (5.4 TB/s), 178
- * MB of 32 tokens over 8-bit rows in 41 us (4.3 TB/s), the joins 5 us each. Nothing of the cache
+ * It is bound by the cache's bytes: 268 MB of one token over 131071 rows in 49.7 us (5.4 TB/s), 178
+ * MB of 32 tokens over 8-bit rows in 44 us (4.1 TB/s), the joins 5 us each. Nothing of the cache
  * goes through LDS (no row is read by two waves), V is under way before the scores and the next K
  * before the sums (32 tokens over 8-bit rows with each load where it is used: 114 us, not 48).
  */
