@@ -20,6 +20,7 @@ namespace {
 constexpr int64_t MAX_STRIDE = (int64_t)1 << 46;   /* elements: past any memory, and far from 64 bits in bytes */
 constexpr int MAX_ROWS = 0x3fff0000;                /* rows of a sequence that an attention takes: split ends stay within 31 bits */
 constexpr int64_t MAX_LATENT_TILES = 0x7ffff0;      /* workgroups of 512 threads in one dimension of a grid (below 2^32 threads) */
+constexpr int64_t MAX_COPY_GROUPS = 0xffffff;       /* workgroups of 256 likewise */
 constexpr int64_t MAX_ROPE_ROW = 1 << 24;           /* elements of a token: four of them count within 31 bits */
 
 bool pow2(int x) { return x > 0 && (x & (x - 1)) == 0; }
@@ -115,6 +116,7 @@ int copy_call(bool write, const hearth_gpu_cache *c, const hearth_gpu_batch *b, 
     }
     if (latent && (col != c->width || (v && c->n_heads != 1))) return E_ARG;
     if (!a.b.n_seqs || !a.b.max_q) return OK;
+    if (copy_groups(a) > MAX_COPY_GROUPS) return E_ARG;
     if (hipPeekAtLastError() != hipSuccess) return E_IO;
     DeviceGuard g(dev);
     if (!g.ok) return E_IO;

@@ -95,6 +95,7 @@ struct DeviceGuard {
 };
 
 void rope(const RopeArgs &a, int dtype, hipStream_t st);
+int64_t copy_groups(const CopyArgs &a);   /* workgroups of a sequence's tokens */
 void kv_append(const CopyArgs &a, int src_dtype, int cache_dtype, bool aligned, hipStream_t st);
 void kv_read(const CopyArgs &a, int dst_dtype, int cache_dtype, bool aligned, hipStream_t st);
 

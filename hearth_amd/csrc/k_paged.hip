@@ -310,10 +310,11 @@ __global__ __launch_bounds__(256) void k_kv_read(CopyArgs a) {
 } // namespace
 
 /* grid of place_of */
-static dim3 copy_grid(const CopyArgs &a) {
+int64_t copy_groups(const CopyArgs &a) {
     const int tokens = 256 / std::min(a.octs, 256) * COPY_TOKENS;
-    return dim3((a.b.max_q + tokens - 1) / tokens, a.b.n_seqs, (a.octs + 255) / 256);
+    return ((int64_t)a.b.max_q + tokens - 1) / tokens;
 }
+static dim3 copy_grid(const CopyArgs &a) { return dim3((unsigned)copy_groups(a), a.b.n_seqs, (a.octs + 255) / 256); }
 
 template <int DT, bool HALF>
 static void rope_t(const RopeArgs &a, bool wide, int tok, hipStream_t st) {

@@ -357,7 +357,8 @@ HEARTH_API int hearth_gpu_rope(const hearth_gpu_array *x, const hearth_gpu_array
  * 448 over the block's finite values (scale byte 1 at least), codes round to nearest even; a
  * NaN or infinity is stored as NaN; a value whose rounding would leave the range of x's type
  * is stored as the largest code within it. Tokens at negative positions (more tokens than
- * rows) and rows past the bounds are not stored; two sequences that share a page in which
+ * rows) and rows past the bounds are not stored; at most 2^26 - 4 tokens a sequence (more where
+ * a token's rows have fewer than 2048 elements); two sequences that share a page in which
  * they write the same row leave one or a mixture of the two. */
 HEARTH_API int hearth_gpu_kv_append(const hearth_gpu_cache *c, const hearth_gpu_batch *b, const hearth_gpu_array *k,
                                     const hearth_gpu_array *v, int dev, void *stream);

@@ -215,6 +215,10 @@ def test_c_entries_refuse_sizes_and_addresses():
     def attend(bb, lse=None, scale=0.1):
         return L.hearth_gpu_attend(byref(c), byref(bb), byref(q), byref(q), lse, scale, None, 0, 0, None)
 
+    long = but(b, n_tokens=0x7fffffff, max_q=0x7fffffff)
+    flat = but(r, token_stride=0)
+    for fn in (L.hearth_gpu_kv_append, L.hearth_gpu_kv_read):
+        assert fn(byref(c), byref(long), byref(flat), byref(flat), 0, None) == E
     far = but(b, max_kv=0x7fffffff, pages_per_seq=1 << 28, ld_pages=1 << 28)
     assert attend(far) == E and L.hearth_gpu_attend_workspace(byref(c), byref(far), 4) == E
     wide = but(b, n_seqs=65535, max_q=1 << 15, n_tokens=1 << 15)
