@@ -381,19 +381,21 @@ def rope(x, pos, freqs, *, factor=1.0, layout="half", offset=0, out=None, k=None
     if layout not in ("half", "interleaved"):
         raise ValueError(f"layout {layout!r} is neither 'half' nor 'interleaved'")
     dev = _device(x, "x")
-    out = x if out is None else out
-    ax, ao = _array(x, "x", dev), _array(out, "out", dev)
+    ao = ax = _array(x, "x", dev)
     tokens = x.shape[0]
-    if out.shape[0] != tokens or ao.n_heads != ax.n_heads or ao.width != ax.width or ao.dtype != ax.dtype:
-        raise ValueError(f"out is {out.dtype}{tuple(out.shape)}, x {x.dtype}{tuple(x.shape)}")
+    if out is not None and out is not x:
+        ao = _array(out, "out", dev)
+        if out.shape[0] != tokens or ao.n_heads != ax.n_heads or ao.width != ax.width or ao.dtype != ax.dtype:
+            raise ValueError(f"out is {out.dtype}{tuple(out.shape)}, x {x.dtype}{tuple(x.shape)}")
     ak = ako = None
     if k is not None:
-        k_out = k if k_out is None else k_out
-        ak, ako = _array(k, "k", dev), _array(k_out, "k_out", dev)
+        ako = ak = _array(k, "k", dev)
         if k.shape[0] != tokens or ak.width != ax.width or ak.dtype != ax.dtype:
             raise ValueError(f"k is {k.dtype}{tuple(k.shape)}, x {x.dtype}{tuple(x.shape)}")
-        if k_out.shape[0] != tokens or ako.n_heads != ak.n_heads or ako.width != ak.width or ako.dtype != ak.dtype:
-            raise ValueError(f"k_out is {k_out.dtype}{tuple(k_out.shape)}, k {k.dtype}{tuple(k.shape)}")
+        if k_out is not None and k_out is not k:
+            ako = _array(k_out, "k_out", dev)
+            if k_out.shape[0] != tokens or ako.n_heads != ak.n_heads or ako.width != ak.width or ako.dtype != ak.dtype:
+                raise ValueError(f"k_out is {k_out.dtype}{tuple(k_out.shape)}, k {k.dtype}{tuple(k.shape)}")
     elif k_out is not None:
         raise ValueError("k_out without k")
     p = _ints(pos, "pos", dev, 1, ("torch.int32", "torch.int64", "int32 or int64"))
