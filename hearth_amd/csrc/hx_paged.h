@@ -234,13 +234,14 @@ __device__ __forceinline__ float sum16(float x) {
 
 /* 16 bytes a lane from memory straight to LDS: lane l's, at base + off + OFS, to dst + 16 l (base and
  * dst: the same for the wave). Written out because the compiler, which cannot tell the buffers of a
- * double buffer apart, lets every later LDS read wait for the builtin's loads. No register is
- * written; the loads have arrived after vm_wait(), and are there for the other waves after a barrier
- * behind it. */
+ * double buffer apart, lets every later LDS read wait for the builtin's loads. The LDS address is
+ * handed over in m0, which the compiler writes, so that it knows of it (it takes m0 for no clobber);
+ * no register is written here. The loads have arrived after vm_wait(), and are there for the other
+ * waves after a barrier behind it. */
 template <int OFS>
 __device__ __forceinline__ void to_lds(const uint8_t *base, int off, uint8_t *dst) {
     const unsigned at = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)dst) - OFS;   /* the instruction adds OFS here too */
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 offset:%3" ::"s"(at), "v"(off), "s"(base), "n"(OFS)
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 offset:%3" ::"{m0}"(at), "v"(off), "s"(base), "n"(OFS)
                  : "memory");
 }
 /* N instructions of the same kind, the z-th 1 KiB further in memory (from off[z]) and in LDS */
@@ -249,13 +250,13 @@ __device__ __forceinline__ void to_lds_rows(const uint8_t *base, const int (&off
     static_assert(N == 2 || N == 4);
     const unsigned at = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)dst);
     if constexpr (N == 2)
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %3\n\t"
-                     "global_load_lds_dwordx4 %2, %3 offset:%4" ::"s"(at), "v"(off[0]), "v"(off[1]), "s"(base), "n"(1 << 10) : "memory");
+        asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, %3\n\t"
+                     "global_load_lds_dwordx4 %2, %3 offset:%4" ::"{m0}"(at), "v"(off[0]), "v"(off[1]), "s"(base), "n"(1 << 10) : "memory");
     else
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %5\n\t"
+        asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, %5\n\t"
                      "global_load_lds_dwordx4 %2, %5 offset:%6\n\tglobal_load_lds_dwordx4 %3, %5 offset:%7\n\t"
                      "global_load_lds_dwordx4 %4, %5 offset:%8"
-                     ::"s"(at), "v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3]), "s"(base), "n"(1 << 10), "n"(2 << 10), "n"(3 << 10)
+                     ::"{m0}"(at), "v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3]), "s"(base), "n"(1 << 10), "n"(2 << 10), "n"(3 << 10)
                      : "memory");
 }
 /* the same address for the whole wave, in scalar registers */
