@@ -205,10 +205,11 @@ __device__ __forceinline__ unsigned row_elem(const uint8_t *row, const uint8_t *
         return ((const unsigned short *)row)[d];
 }
 
-/* 16, 8 and 4 bytes at any address (the memory system takes each as one access) */
+/* 16, 8, 4 and 2 bytes at any address (the memory system takes each as one access) */
 typedef u4 u4_any __attribute__((aligned(1)));
 typedef u2 u2_any __attribute__((aligned(1)));
 typedef unsigned unsigned_any __attribute__((aligned(1)));
+typedef unsigned short ushort_any __attribute__((aligned(1)));
 
 /* the scale of a block from its byte (1 to 254) */
 __device__ __forceinline__ float mx_scale(unsigned byte) { return __uint_as_float((byte & 255u) << 23); }

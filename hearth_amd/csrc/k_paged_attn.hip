@@ -48,7 +48,7 @@ struct Few {
         for (int i = 0; i < KL; i++) k.w[u][i] = *(const u4 *)(p + 64 * i);
         if constexpr (MX) {
             const uint8_t *q = sc + (row + lc) * (D / MX_BLOCK);
-            if constexpr (D == 64) k.s[u][0] = *(const unsigned short *)q;
+            if constexpr (D == 64) k.s[u][0] = *(const ushort_any *)q;
             else
 #pragma unroll
                 for (int i = 0; i < SW; i++) k.s[u][i] = ((const unsigned_any *)q)[i];

@@ -57,3 +57,13 @@ def test_the_check_sees_them():
     assert sum("_lds_" in _template(s) for f, s in ASMS if f == "hx_paged.h") == 3
     assert not _m0('asm volatile("s_mov_b32 m0, %0\\n\\tglobal_load_lds_dwordx4 %1, %2" ::"s"(a), "v"(o), "s"(b) : "memory")')
     assert not _m0('asm volatile("global_load_lds_dwordx4 %1, %2" ::"s"(a), "v"(o), "s"(b) : "memory")')
+
+
+def test_scales_are_read_at_any_address():
+    """A cache's scale bytes may lie at any address: wider reads of them go through types that say so."""
+    text = COMMENT.sub(" ", (build.CSRC / "k_paged_attn.hip").read_text())
+    reads = re.findall(r"\(const (\w+) \*\)\(?q\b", text)
+    assert len(reads) >= 4 and all(t.endswith("_any") for t in reads), reads
+    header = (build.CSRC / "hx_paged.h").read_text()
+    for t in set(reads):
+        assert re.search(rf"typedef [\w ]+ {t} __attribute__\(\(aligned\(1\)\)\);", header), t
