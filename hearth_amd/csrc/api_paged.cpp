@@ -88,6 +88,12 @@ Batch batch_of(const hearth_gpu_batch &b, const hearth_gpu_cache &c) {
 
 int finish() { return hipGetLastError() == hipSuccess ? OK : E_IO; }   /* this call's launches only */
 
+/* The call's own error, read so that the thread's next call does not take it for the caller's. */
+int no_device() {
+    (void)hipGetLastError();
+    return E_IO;
+}
+
 int copy_call(bool write, const hearth_gpu_cache *c, const hearth_gpu_batch *b, const hearth_gpu_array *k,
               const hearth_gpu_array *v, int dev, void *stream) {
     if (!cache_ok(c) || !batch_ok(b) || dev < 0) return E_ARG;
@@ -119,7 +125,7 @@ int copy_call(bool write, const hearth_gpu_cache *c, const hearth_gpu_batch *b, 
     if (copy_groups(a) > MAX_COPY_GROUPS) return E_ARG;
     if (hipPeekAtLastError() != hipSuccess) return E_IO;
     DeviceGuard g(dev);
-    if (!g.ok) return E_IO;
+    if (!g.ok) return no_device();
     if (write) kv_append(a, k->dtype, c->dtype, wide, (hipStream_t)stream);
     else kv_read(a, k->dtype, c->dtype, wide, (hipStream_t)stream);
     return finish();
@@ -175,7 +181,7 @@ int attend_call(const hearth_gpu_cache *c, const hearth_gpu_batch *b, const hear
     a.part = (float *)work;
     if (hipPeekAtLastError() != hipSuccess) return E_IO;
     DeviceGuard g(dev);
-    if (!g.ok) return E_IO;
+    if (!g.ok) return no_device();
     if (latent) attend_latent(a, q->dtype, c->dtype, (hipStream_t)stream);
     else attend(a, q->dtype, c->dtype, c->width, s.many, (hipStream_t)stream);
     return finish();
@@ -216,7 +222,7 @@ HEARTH_API int hearth_gpu_rope(const hearth_gpu_array *x, const hearth_gpu_array
     if (!n_tokens) return OK;
     if (hipPeekAtLastError() != hipSuccess) return E_IO;
     DeviceGuard g(dev);
-    if (!g.ok) return E_IO;
+    if (!g.ok) return no_device();
     rope(a, x->dtype, (hipStream_t)stream);
     return finish();
 }
