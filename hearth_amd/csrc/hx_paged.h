@@ -152,6 +152,10 @@ __device__ __forceinline__ unsigned long long step_mask(int t0, int lim, int hi,
     return h >= 64 ? x : h <= 0 ? 0ull : x & ((1ull << h) - 1);
 }
 
+/* The sum of exponentials is 0 where a column attends nothing, and where it attends rows whose scores
+ * are all -infinity. The first result is 0, the second 0 / 0: NaN, as in the formula. */
+constexpr float UNDEFINED = __builtin_nanf("");
+
 /* bits of 16 rows a page group each, from bits of groups */
 __device__ __forceinline__ unsigned long long group_rows(unsigned have) {
     unsigned long long x = 0;

@@ -131,6 +131,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_attend_few(AttendArgs a) {
     constexpr int PL = F::PL, NB = F::NB, BD = F::BD, ES = F::ES, CT = 16;
     __shared__ float lds_o[FEW_WAVES][16][BD + 4];
     __shared__ float lds_m[FEW_WAVES][CT], lds_l[FEW_WAVES][CT];
+    __shared__ unsigned lds_some[FEW_WAVES];   /* bit c: column c attends a row of the wave's */
 
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int g = lane >> 4, lc = lane & 15;
@@ -176,6 +177,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_attend_few(AttendArgs a) {
 
     f4 acc[NB * PL];
     float m = -__builtin_huge_valf(), l = 0.0f;
+    bool some = false;  /* this lane's column attends a row of the wave's */
     bool odd = false;   /* V held an infinity or NaN in a row that some column does not attend */
 #pragma unroll
     for (int i = 0; i < NB * PL; i++) acc[i] = (f4){0, 0, 0, 0};
@@ -237,8 +239,11 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_attend_few(AttendArgs a) {
         float x[8];
 #pragma unroll
         for (int j = 0; j < 8; j++) x[j] = s[j >> 2][j & 3] * a.scale2;
-        if (!whole) {
-            const unsigned long long vis = (attended(t0) & group_rows((ok[0] ? 1u : 0u) | (ok[1] ? 2u : 0u))) >> (4 * g);
+        if (whole) {
+            some = true;
+        } else {
+            const unsigned long long at = attended(t0) & group_rows((ok[0] ? 1u : 0u) | (ok[1] ? 2u : 0u)), vis = at >> (4 * g);
+            some = some || at;
 #pragma unroll
             for (int j = 0; j < 8; j++) x[j] = vis >> (16 * (j >> 2) + (j & 3)) & 1 ? x[j] : -__builtin_huge_valf();
         }
@@ -313,6 +318,8 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_attend_few(AttendArgs a) {
     /* the four waves' columns together: a lane's sums cover its own rows of each step only */
     l = sum16(sum32(l));
     if (g == 0) { lds_m[wave][lc] = m; lds_l[wave][lc] = l; }
+    const unsigned mine = (unsigned)__ballot(some);
+    if (lane == 0) lds_some[wave] = mine;
     __syncthreads();
     const bool direct = n_sp == 1;
     const int oc = threadIdx.x >> 4, od = (threadIdx.x & 15) * PL;   /* output column and element of this thread */
@@ -329,6 +336,8 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_attend_few(AttendArgs a) {
         const float mw = lds_m[w][oc], lw = lds_l[w][oc];
         Lo += mw == -__builtin_huge_valf() ? lw : lw * exp2_hw(mw - Mo);
     }
+    static_assert(FEW_WAVES == 4);
+    const bool undefined = Lo == 0.0f && ((lds_some[0] | lds_some[1] | lds_some[2] | lds_some[3]) >> oc & 1);
     const int co = tile * CT + oc;
     const bool here = co < cols;
     const int ot = here ? co / a.group : 0, oh = kvh * a.group + (here ? co % a.group : 0);
@@ -352,7 +361,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_attend_few(AttendArgs a) {
             for (int w = 0; w < FEW_WAVES; w++) o[j] += lds_o[w][oc][od + j];
         }
         if (direct) {
-            const float inv = Lo == 0.0f ? 0.0f : 1.0f / Lo;
+            const float inv = undefined ? UNDEFINED : Lo == 0.0f ? 0.0f : 1.0f / Lo;
             uint8_t *out = a.out + (int64_t)(q.q0 + ot) * a.ot + (int64_t)oh * a.oh + 2 * (b * BD + od);
 #pragma unroll
             for (int j = 0; j < PL; j += 4)
@@ -366,7 +375,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_attend_few(AttendArgs a) {
     if (here && (threadIdx.x & 15) == 0) {
         if (!direct) {
             float *ml = a.part + (int64_t)a.b.n_tokens * a.heads * a.n_splits * D + (row * a.n_splits + sp) * 2;
-            ml[0] = Mo;
+            ml[0] = undefined ? UNDEFINED : Mo;
             ml[1] = Lo;
         } else if (a.lse) a.lse[row] = Lo == 0.0f ? -__builtin_huge_valf() : (Mo + __log2f(Lo)) * 0.69314718055994531f;
     }
@@ -376,8 +385,8 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_attend_few(AttendArgs a) {
  * threads take a row, four elements each, so a workgroup holds JOIN_THREADS / (DV / 4) groups of
  * threads: with few splits each group has a row of its own; with many (MANY) they share one row's
  * splits and meet in LDS, since one group's loads of 256 splits, one after the other, took 86 us
- * where the attention over 131071 rows took 59. A split whose sum is 0 attended nothing and holds
- * no sums. */
+ * where the attention over 131071 rows took 59. A split whose sum is 0 holds no sums; its maximum is
+ * -infinity where the row attends nothing of it, NaN where scores were all -infinity. */
 constexpr int JOIN_THREADS = 256, JOIN_MANY = 16;
 
 template <class T, int DV, bool MANY>
@@ -386,6 +395,7 @@ __global__ __launch_bounds__(JOIN_THREADS) void k_attend_join(AttendArgs a) {
     constexpr float NINF = -__builtin_huge_valf();
     __shared__ __align__(16) f4 lds_o[MANY ? JOIN_THREADS : 1];
     __shared__ float lds_l[NG], lds_m[JOIN_THREADS / 64];
+    __shared__ bool lds_some[JOIN_THREADS / 64];
     const int seq = blockIdx.z, grp = threadIdx.x / TPR, e = threadIdx.x % TPR * 4;
     const Seq q = seq_of(a.b, seq);
     const int r = MANY ? blockIdx.x : blockIdx.x * NG + grp;
@@ -398,15 +408,25 @@ __global__ __launch_bounds__(JOIN_THREADS) void k_attend_join(AttendArgs a) {
     const float *po = a.part + row * a.n_splits * DV + e;
     const float *ml = a.part + (int64_t)a.b.n_tokens * a.heads * a.n_splits * DV + row * a.n_splits * 2;
     float M = NINF;
+    bool some = false;   /* a split whose scores were all -infinity */
+    auto take = [&](float m) __attribute__((always_inline)) {
+        some = some || m != m;
+        M = fmaxf(M, m);   /* not the NaN */
+    };
     if constexpr (MANY) {
-        for (int i = threadIdx.x; i < n_sp; i += JOIN_THREADS) M = fmaxf(M, ml[2 * i]);
+        for (int i = threadIdx.x; i < n_sp; i += JOIN_THREADS) take(ml[2 * i]);
 #pragma unroll
         for (int d = 32; d; d >>= 1) M = fmaxf(M, __shfl_xor(M, d));
-        if ((threadIdx.x & 63) == 0) lds_m[threadIdx.x >> 6] = M;
+        some = __any(some);
+        if ((threadIdx.x & 63) == 0) {
+            lds_m[threadIdx.x >> 6] = M;
+            lds_some[threadIdx.x >> 6] = some;
+        }
         __syncthreads();
         M = fmaxf(fmaxf(lds_m[0], lds_m[1]), fmaxf(lds_m[2], lds_m[3]));
+        some = lds_some[0] || lds_some[1] || lds_some[2] || lds_some[3];
     } else {
-        for (int i = 0; i < n_sp; i++) M = fmaxf(M, ml[2 * i]);
+        for (int i = 0; i < n_sp; i++) take(ml[2 * i]);
     }
     float L = 0.0f;
     f4 o = {0, 0, 0, 0};
@@ -431,7 +451,7 @@ __global__ __launch_bounds__(JOIN_THREADS) void k_attend_join(AttendArgs a) {
             L += lds_l[k];
         }
     }
-    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+    const float inv = L == 0.0f ? (some ? UNDEFINED : 0.0f) : 1.0f / L;
     uint8_t *out = a.out + (int64_t)(q.q0 + t) * a.ot + (int64_t)h * a.oh + 2 * e;
     *(u2_any *)out = (u2){T::pack(o[0] * inv, o[1] * inv), T::pack(o[2] * inv, o[3] * inv)};
     if (a.lse && e == 0) a.lse[row] = L == 0.0f ? NINF : (M + __log2f(L)) * 0.69314718055994531f;

@@ -282,6 +282,7 @@ __global__ __launch_bounds__(L_THREADS) void k_attend_latent(AttendArgs a) {
         arrived();
         const int k_at = piece_at(r0 + c, g);
         float m[2] = {NINF, NINF}, l[2];
+        unsigned some = 0;   /* bit n: the column attends a row of the split (as truth values they took scalars, which ran out) */
         /* Scores of step s, scaled; rows that are not attended -infinity. The rows two steps on are
          * sent for among the products: the address units take 64 bytes a cycle of all waves' together. */
         f4 s[2];
@@ -314,10 +315,12 @@ __global__ __launch_bounds__(L_THREADS) void k_attend_latent(AttendArgs a) {
             const int t0 = lo + step * L_ROWS;
 #pragma unroll
             for (int n = 0; n < 2; n++) s[n] = (x[0][n] + x[1][n]) * a.scale2;
-            if (edge_at(t0, h))
+            if (!edge_at(t0, h)) some = 3;
+            else
 #pragma unroll
                 for (int n = 0; n < 2; n++) {
-                    const unsigned long long vis = (attended(col[n], t0) & group_rows(h)) >> (r0 + 4 * g);
+                    const unsigned long long at = attended(col[n], t0) & group_rows(h), vis = at >> (r0 + 4 * g);
+                    some |= at ? 1u << n : 0u;
 #pragma unroll
                     for (int j = 0; j < 4; j++) s[n][j] = vis >> j & 1 ? s[n][j] : NINF;
                 }
@@ -407,7 +410,7 @@ __global__ __launch_bounds__(L_THREADS) void k_attend_latent(AttendArgs a) {
             const float y = sum16(sum32(l[n]));
             if (g == 0) {
                 lds_l[wave >> 1][first + 16 * n + c] = y;
-                if (!(wave >> 1)) lds_m[0][first + 16 * n + c] = m[n];
+                if (!(wave >> 1)) lds_m[0][first + 16 * n + c] = m[n] == NINF && (some >> n & 1) ? UNDEFINED : m[n];
             }
         }
         __syncthreads();   /* (C) */
@@ -530,7 +533,7 @@ __global__ __launch_bounds__(L_THREADS) void k_attend_latent(AttendArgs a) {
         const float L = lds_l[0][r] + lds_l[1][r], m = lds_m[0][r];
         const int64_t row = (int64_t)(q.q0 + col.tok) * a.heads + col.head;
         if (direct) {
-            const float f = L == 0.0f ? 0.0f : 1.0f / L;
+            const float f = L == 0.0f ? (m == m ? 0.0f : UNDEFINED) : 1.0f / L;
             const f4 x = *unit(r, 2 * lane) * f, y = *unit(r, 2 * lane + 1) * f;
             *(u4_any *)(a.out + (int64_t)(q.q0 + col.tok) * a.ot + (int64_t)col.head * a.oh + 16 * lane) =
                 (u4){T::pack(x[0], x[1]), T::pack(x[2], x[3]), T::pack(y[0], y[1]), T::pack(y[2], y[3])};

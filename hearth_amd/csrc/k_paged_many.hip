@@ -111,6 +111,7 @@ __global__ __launch_bounds__(64 * MANY_WAVES, D <= 128 ? 2 : 1) void k_attend_ma
 #pragma unroll
         for (int j = 0; j < 16; j++) acc[i][j] = 0.0f;
     float m = NINF, l = 0.0f;
+    bool some = false;   /* this lane's column attends a row of the split */
 
     const int *pages = a.b.pages + (int64_t)seq * a.b.ld_pages;
     const int rmask = (1 << a.b.page_shift) - 1;
@@ -265,6 +266,7 @@ __global__ __launch_bounds__(64 * MANY_WAVES, D <= 128 ? 2 : 1) void k_attend_ma
         v8 pf[M::GROUPS];
         float mx;
         if (!edge) {
+            some = true;
             mx = s[0][0];
 #pragma unroll
             for (int u = 0; u < M::TILES; u++)
@@ -273,7 +275,8 @@ __global__ __launch_bounds__(64 * MANY_WAVES, D <= 128 ? 2 : 1) void k_attend_ma
             mx = max32(mx) * scale2;
         } else {
             mx = NINF;
-            const unsigned long long vis = (attended(t0) & group_rows(have_now)) >> (4 * half);
+            const unsigned long long at = attended(t0) & group_rows(have_now), vis = at >> (4 * half);
+            some = some || at;
 #pragma unroll
             for (int u = 0; u < M::TILES; u++)
 #pragma unroll
@@ -360,7 +363,7 @@ __global__ __launch_bounds__(64 * MANY_WAVES, D <= 128 ? 2 : 1) void k_attend_ma
     if (!on) return;
     const int64_t row = (int64_t)(q.q0 + tok) * a.heads + head;
     if (n_sp == 1) {
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        const float inv = l == 0.0f ? (some ? UNDEFINED : 0.0f) : 1.0f / l;
         uint8_t *out = a.out + (int64_t)(q.q0 + tok) * a.ot + (int64_t)head * a.oh;
 #pragma unroll
         for (int i = 0; i < DT; i++)
@@ -395,7 +398,7 @@ __global__ __launch_bounds__(64 * MANY_WAVES, D <= 128 ? 2 : 1) void k_attend_ma
                     *(f4 *)(po + 32 * i + 8 * b + 4 * half) = (f4){acc[i][4 * b], acc[i][4 * b + 1], acc[i][4 * b + 2], acc[i][4 * b + 3]};
         if (half == 0) {
             float *ml = a.part + (int64_t)a.b.n_tokens * a.heads * a.n_splits * D + (row * a.n_splits + sp) * 2;
-            ml[0] = m;
+            ml[0] = l == 0.0f && some ? UNDEFINED : m;
             ml[1] = l;
         }
     }

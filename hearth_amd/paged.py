@@ -356,7 +356,7 @@ def attend(cache: Cache, batch: Batch, q, out, *, scale: float, lse=None, worksp
     [tokens, heads, width] of the cache's 16-bit dtype (any over mx8 rows), heads a multiple of
     the cache's. lse: float32 [tokens, heads] or None. workspace: a device tensor of
     workspace_bytes; calls that may run at the same time must not share one. A token that
-    attends nothing gets zeros (lse -inf)."""
+    attends nothing gets zeros, one all of whose scores are -inf gets NaN (lse -inf for both)."""
     _attend("attend", cache, batch, q, None, out, lse, scale, workspace, stream)
 
 

@@ -371,12 +371,13 @@ HEARTH_API int hearth_gpu_kv_read(const hearth_gpu_cache *c, const hearth_gpu_ba
 /* Attention of the call's tokens over the cache: q [n_tokens][H][width], out alike, of dtype
  * HEARTH_F16 or HEARTH_BF16; H a multiple of the cache's heads, head h reads kv head
  * h / (H / n_heads); width 64, 128 or 256. out = softmax(scale * q . k) v over the rows a
- * token attends; a token that attends nothing gets zeros. 16-bit caches have q's dtype; MX8
+ * token attends; a token that attends nothing gets zeros, one all of whose scores are -infinity
+ * NaN (0 / 0). 16-bit caches have q's dtype; MX8
  * rows are taken as their values in q's dtype, in whose range they must lie. min(max_q,
  * n_tokens) * H up to 2^26; min(max_kv, pages_per_seq * page) below 2^30 - 65536. Scores, softmax statistics and sums are
  * float32; the probabilities are rounded to q's dtype for the product with v. lse: NULL or
  * [n_tokens][H] float32, the natural logarithm of the sum of exponentials (-infinity where
- * nothing is attended). work: device memory of hearth_gpu_attend_workspace bytes, 16-byte
+ * that is 0). work: device memory of hearth_gpu_attend_workspace bytes, 16-byte
  * aligned; calls that may run at the same time must not share it. */
 HEARTH_API int hearth_gpu_attend(const hearth_gpu_cache *c, const hearth_gpu_batch *b, const hearth_gpu_array *q,
                                  const hearth_gpu_array *out, float *lse, float scale, void *work, size_t work_bytes,
