@@ -13,7 +13,8 @@ element_size() and is_contiguous() as torch tensors have them (torch itself is n
 on `stream` (a HIP stream handle such as torch.cuda.current_stream().cuda_stream; 0 is the
 null stream) of the tensors' device and not waited for, so the tensors must live until it has
 run; nothing is allocated, so a call may be captured into a graph. ValueError for arguments that do not fit together, HearthError for
-a device error.
+a device error. The operators have no gradients: tensors that require one are refused where
+gradients are recorded (call under torch.no_grad(), or detach them).
 
 No counterpart in the reference, whose engine keeps one conversation in float32 on the host.
 """
@@ -21,6 +22,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import sys
 from ctypes import POINTER, Structure, byref, c_double, c_float, c_int, c_int32, c_int64, c_size_t, c_void_p
 
 import numpy as np
@@ -119,8 +121,17 @@ def _device(t, what, want=None) -> int:
     return i
 
 
+def _refuse_gradient(what):
+    """For a tensor that requires a gradient: autograd would not see what the call reads or writes."""
+    torch = sys.modules.get("torch")
+    if torch is None or torch.is_grad_enabled():
+        raise ValueError(f"{what} requires a gradient, and these operators have none: call under torch.no_grad() or detach it")
+
+
 def _array(t, what, dev) -> _Array:
     """[tokens, heads, width] with a dense last dimension."""
+    if getattr(t, "requires_grad", False):
+        _refuse_gradient(what)
     shape = t.shape
     if len(shape) != 3:
         raise ValueError(f"{what}: shape {tuple(shape)} is not [tokens, heads, width]")
@@ -191,6 +202,10 @@ class Cache:
             raise ValueError(f"width {s.width}: a multiple of 32 up to 1024 is needed")
         self._s = s
         self._ref = byref(s)
+
+    def _no_gradient(self):
+        if getattr(self.k, "requires_grad", False) or getattr(self.v, "requires_grad", False):
+            _refuse_gradient("the cache")
 
     def _rows(self, t, scale, what, like, dt) -> _Rows:
         if tuple(t.shape) != tuple(like.shape) or _dtype(t) != dt:
@@ -267,6 +282,7 @@ class Batch:
 def _pair(cache, batch, k, v, what):
     if batch.device != cache.device:
         raise ValueError(f"{what}: the batch is on device {batch.device}, the cache on device {cache.device}")
+    cache._no_gradient()
     a = _array(k, "k", cache.device)
     b = None
     if v is not None:
@@ -320,6 +336,7 @@ def _attend(name, cache, batch, q, q_pe, out, lse, scale, workspace, stream):
     dev = cache.device
     if batch.device != dev:
         raise ValueError(f"{name}: the batch is on device {batch.device}, the cache on device {dev}")
+    cache._no_gradient()
     a, o, tokens = _array(q, "q", dev), _array(out, "out", dev), q.shape[0]
     if out.shape[0] != tokens or o.n_heads != a.n_heads or o.width != a.width or a.dtype != o.dtype:
         raise ValueError(f"{name}: out is {out.dtype}{tuple(out.shape)}, q {q.dtype}{tuple(q.shape)}")
@@ -330,6 +347,8 @@ def _attend(name, cache, batch, q, q_pe, out, lse, scale, workspace, stream):
         if tuple(lse.shape) != tuple(q.shape[:2]) or str(lse.dtype) != "torch.float32" or not lse.is_contiguous():
             raise ValueError(f"lse: {lse.dtype}{tuple(lse.shape)}, wanted dense float32{tuple(q.shape[:2])}")
         _device(lse, "lse", dev)
+        if getattr(lse, "requires_grad", False):
+            _refuse_gradient("lse")
         lp = lse.data_ptr()
     wp, wb = None, 0
     if workspace is not None:
@@ -400,6 +419,8 @@ def rope(x, pos, freqs, *, factor=1.0, layout="half", offset=0, out=None, k=None
         raise ValueError("k_out without k")
     p = _ints(pos, "pos", dev, 1, ("torch.int32", "torch.int64", "int32 or int64"))
     f = _ints(freqs, "freqs", dev, 1, ("torch.float64", "float64"))
+    if getattr(freqs, "requires_grad", False):
+        _refuse_gradient("freqs")
     n = freqs.shape[0]
     if pos.shape[0] != tokens or tokens > 0x7fffffff:
         raise ValueError(f"{pos.shape[0]} positions for {tokens} tokens")
