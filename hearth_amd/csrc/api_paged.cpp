@@ -63,6 +63,11 @@ bool array_ok(const hearth_gpu_array *x, int n) {
     return std::llabs(x->token_stride) <= MAX_STRIDE && std::llabs(x->head_stride) <= MAX_STRIDE;
 }
 
+/* of an array that is written: neighbouring rows share no element (broadcast ones do) */
+bool apart(const hearth_gpu_array &x, int n) {
+    return (x.n_heads < 2 || std::llabs(x.head_stride) >= x.width) && (n < 2 || std::llabs(x.token_stride) >= x.width);
+}
+
 /* pointer and strides on 16 bytes */
 bool on16(const hearth_gpu_array &x) {
     const int64_t es = elem(x.dtype);
@@ -109,7 +114,7 @@ int copy_call(bool write, const hearth_gpu_cache *c, const hearth_gpu_batch *b, 
     bool wide = true;
     for (int i = 0; i < a.n_pieces; i++) {
         const hearth_gpu_array &x = i ? *v : *k;
-        if (x.n_heads != c->n_heads || x.width % 32) return E_ARG;
+        if (x.n_heads != c->n_heads || x.width % 32 || (!write && !apart(x, n))) return E_ARG;
         Piece &p = a.p[i];
         const int es = elem(x.dtype);
         p.arr = (uint8_t *)x.data; p.at = x.token_stride * es; p.ah = x.head_stride * es;
@@ -155,7 +160,7 @@ int attend_call(const hearth_gpu_cache *c, const hearth_gpu_batch *b, const hear
     if (!q || !attend_shape_ok(c, b, q->n_heads) || !array_ok(q, b->n_tokens) || !array_ok(out, b->n_tokens) || dev < 0) return E_ARG;
     const bool latent = q_pe != nullptr;
     if (latent != !c->v.data || (uintptr_t)lse % 4 || !std::isfinite(scale * 1.44269504088896340736f)) return E_ARG;
-    if ((q->dtype != HEARTH_F16 && q->dtype != HEARTH_BF16) || out->dtype != q->dtype) return E_ARG;
+    if ((q->dtype != HEARTH_F16 && q->dtype != HEARTH_BF16) || out->dtype != q->dtype || !apart(*out, b->n_tokens)) return E_ARG;
     if (c->dtype != HEARTH_GPU_MX8 && c->dtype != q->dtype) return E_ARG;
     const int width = latent ? 512 : c->width;
     if (q->width != width || out->width != width || out->n_heads != q->n_heads) return E_ARG;
@@ -208,7 +213,7 @@ HEARTH_API int hearth_gpu_rope(const hearth_gpu_array *x, const hearth_gpu_array
     for (int i = 0; i < a.n_pairs; i++) {
         const hearth_gpu_array *s = i ? k : x, *d = i ? k_out : out;
         if (!array_ok(s, n_tokens) || !array_ok(d, n_tokens) || s->dtype != x->dtype || d->dtype != x->dtype || s->width != x->width ||
-            d->width != x->width || s->n_heads != d->n_heads) return E_ARG;
+            d->width != x->width || s->n_heads != d->n_heads || !apart(*d, n_tokens)) return E_ARG;
         const int64_t es = elem(s->dtype);
         a.p[i] = {(const uint8_t *)s->data, (uint8_t *)d->data, s->token_stride * es, s->head_stride * es,
                   d->token_stride * es, d->head_stride * es, s->n_heads};

@@ -330,7 +330,8 @@ typedef struct hearth_gpu_batch {
 } hearth_gpu_batch;
 
 /* A caller's array [n_tokens][n_heads][width] of dtype HEARTH_F32, HEARTH_F16 or
- * HEARTH_BF16, the last dimension dense, strides in elements. */
+ * HEARTH_BF16, the last dimension dense, strides in elements. The rows of an array that is
+ * written share no element: strides below the width (a broadcast dimension) are refused there. */
 typedef struct hearth_gpu_array {
     void *data;
     int64_t token_stride, head_stride;
