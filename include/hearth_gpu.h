@@ -358,8 +358,8 @@ HEARTH_API int hearth_gpu_rope(const hearth_gpu_array *x, const hearth_gpu_array
  * 448 over the block's finite values (scale byte 1 at least), codes round to nearest even; a
  * NaN or infinity is stored as NaN; a value whose rounding would leave the range of x's type
  * is stored as the largest code within it. Tokens at negative positions (more tokens than
- * rows) and rows past the bounds are not stored; at most 2^26 - 4 tokens a sequence (more where
- * a token's rows have fewer than 2048 elements); two sequences that share a page in which
+ * rows) and rows past the bounds are not stored; min(max_q, n_tokens) is at most 2^26 - 4 (more
+ * where a token's rows, k and v together, have at most 1024 elements; reads alike); two sequences that share a page in which
  * they write the same row leave one or a mixture of the two. */
 HEARTH_API int hearth_gpu_kv_append(const hearth_gpu_cache *c, const hearth_gpu_batch *b, const hearth_gpu_array *k,
                                     const hearth_gpu_array *v, int dev, void *stream);
@@ -387,8 +387,8 @@ HEARTH_API int hearth_gpu_attend(const hearth_gpu_cache *c, const hearth_gpu_bat
 /* The absorbed form of latent attention: q [n_tokens][H][C] (each head's query taken through
  * its key projection) and q_pe [n_tokens][H][R] (its rotated part) against the latent rows'
  * first C and last R elements, out [n_tokens][H][C] = softmax(scale * (q . c + q_pe . pe)) c.
- * C = 512, R = 64, cache width 576, one cache head, n_seqs * max_q * H up to 2^29; everything
- * else as hearth_gpu_attend. */
+ * C = 512, R = 64, cache width 576, one cache head; n_seqs times min(max_q, n_tokens) * H / 64,
+ * rounded up, at most 8388592 (somewhat below 2^29 / 64); everything else as hearth_gpu_attend. */
 HEARTH_API int hearth_gpu_attend_latent(const hearth_gpu_cache *c, const hearth_gpu_batch *b,
                                         const hearth_gpu_array *q, const hearth_gpu_array *q_pe,
                                         const hearth_gpu_array *out, float *lse, float scale, void *work,
