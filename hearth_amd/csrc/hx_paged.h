@@ -27,6 +27,7 @@ typedef float f4 __attribute__((ext_vector_type(4)));
 typedef float f16v __attribute__((ext_vector_type(16)));
 typedef unsigned u2 __attribute__((ext_vector_type(2)));
 typedef unsigned u4 __attribute__((ext_vector_type(4)));
+typedef short s4v __attribute__((ext_vector_type(4)));
 
 /* hearth_gpu_batch with the bounds of every sequence's rows folded in */
 struct Batch {
@@ -264,6 +265,12 @@ __device__ __forceinline__ void to_lds_rows(const uint8_t *base, const int (&off
                      ::"{m0}"(at), "v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3]), "s"(base), "n"(1 << 10), "n"(2 << 10), "n"(3 << 10)
                      : "memory");
 }
+/* transposing LDS load: lane i of 16 gives the address of 4 elements of row i / 4 and gets element
+ * i of the four rows */
+__device__ __forceinline__ u2 read_tr(const uint8_t *p) {
+    return __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4v *)p));
+}
+
 /* the same address for the whole wave, in scalar registers */
 __device__ __forceinline__ const uint8_t *same(const uint8_t *p) {
     const uint64_t x = (uint64_t)p;

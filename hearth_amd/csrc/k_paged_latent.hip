@@ -50,14 +50,6 @@ __device__ __forceinline__ int piece_at(int r, int p) {
     return ((r >> 3) * L_CHUNKS + (p >> 3)) * 1024 + (r & 7) * 128 + ((p & 7) ^ swz(r)) * 16;
 }
 
-typedef short s4v __attribute__((ext_vector_type(4)));
-
-/* four rows of one element each a lane (transposing LDS load): lane i of 16 gives the address of 4
- * elements of row i / 4 and gets element i of the four rows */
-__device__ __forceinline__ u2 read_tr(const uint8_t *p) {
-    return __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4v *)p));
-}
-
 template <class T, bool MX>
 __global__ __launch_bounds__(L_THREADS) void k_attend_latent(AttendArgs a) {
     using v8 = typename T::v8;

@@ -47,14 +47,6 @@ struct Many {
     static __device__ __forceinline__ int at(int r, int p) { return (r * PIECES + (p ^ swz(r))) * 16; }
 };
 
-typedef short s4v __attribute__((ext_vector_type(4)));
-
-/* transposing LDS load: lane i of 16 gives the address of 4 elements of row i / 4 and gets element
- * i of the four rows */
-__device__ __forceinline__ u2 read_tr(const uint8_t *p) {
-    return __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4v *)p));
-}
-
 template <class T, bool MX, int D>
 __global__ __launch_bounds__(64 * MANY_WAVES, D <= 128 ? 2 : 1) void k_attend_many(AttendArgs a) {
     using M = Many<D>;
