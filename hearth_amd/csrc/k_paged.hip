@@ -167,8 +167,10 @@ __device__ __forceinline__ bool fin(float x) { return __builtin_fabsf(x) < __bui
 
 /* The eight elements that a thread of either kernel takes of each of its tokens: octs threads a
  * token (grid.z of them where that is more than a workgroup), several tokens a workgroup where it is
- * less; where they lie is worked out once for COPY_TOKENS tokens (16 x 4093 rows of 4 heads of 128
- * into 8 bits: 37 us, one by one 44, eight at once 15% more than four on 3 x 4093). */
+ * less; which piece, head and element they are is worked out once for COPY_TOKENS tokens (16 x 4093
+ * rows of 4 heads of 128 into 8 bits: 37 us, one by one 44, eight at once 15% more than four on 3 x
+ * 4093). The piece's addresses and strides are read from the arguments again for each token, so the
+ * four tokens' way from page id to store is walked one after the other: that bounds prompts. */
 constexpr int COPY_TOKENS = 4;
 struct Place {
     const Piece *p;

@@ -12,6 +12,13 @@
  * MB of 32 tokens over 8-bit rows in 44 us (4.1 TB/s), the joins 5 us each. Nothing of the cache
  * goes through LDS (no row is read by two waves), V is under way before the scores and the next K
  * before the sums (32 tokens over 8-bit rows with each load where it is used: 114 us, not 48).
+ *
+ * Scores, maxima, sums of probabilities and of rows are float32. The probabilities alone are rounded
+ * to the 16-bit type, in this kernel and the two for many rows: the matrix units take both factors in
+ * 16 bits, and split into two 16-bit parts they would double the second product. Each rounding is
+ * off by half a step at most, which is as much as the result's own (relative error of 2000 tokens
+ * over 4048 rows against 64 bits: 0.0022 where the result's rounding alone gives 0.0017); float16
+ * takes those below 2^-25 of the maximum they are taken against as 0. Their sum is taken before.
  */
 #include "hx_paged.h"
 
@@ -482,10 +489,10 @@ void join_t(const AttendArgs &a, hipStream_t st) {
 static bool takes_many(int64_t cols) { return cols > 32; }
 
 /* Rows a split takes: enough workgroups for the 256 units, two each (one of the latent form, which
- * fills a unit; with four of few rows a unit 32 tokens over 4096 8-bit rows each took 51 us, not 45,
- * and one over 131071 16-bit rows 59, not 55: more partial sums to write and join). Few query rows
- * are not split below 512 rows: one launch of 500 rows takes 13.4 us where a split one and its join
- * take 16, at 1000 rows they are level. Many are split down to 192 rows (85 tokens over 2132 rows:
+ * fills a unit; with four of few rows a unit 32 tokens over 2048 to 8192 8-bit rows took 51 us, not
+ * 45, and one over 131071 16-bit rows 59, not 55: more partial sums to write and join). Few query
+ * rows are not split below 512 rows: one launch of 500 rows takes 10 us where a split one and its
+ * join take 12.5; at 1000 rows two splits take 16 us and eight 15. Many are split down to 192 rows (85 tokens over 2132 rows:
  * 26 us, at 128 rows 31; 64 over 500: 17 us, at 256 rows 20), the latent form down to 128 (1 token
  * over 500 rows: 21 us, at 256 rows 26; 1 over 8192: 30 us, at 64 rows 35). */
 Split attend_split(int n_seqs, int max_q, int kv_cap, int heads, int kv_heads, bool latent) {

@@ -10,8 +10,9 @@
  * four take the sums of the step before (each a quarter of the latent and all columns, 128
  * registers). So one role's exponentials, reads and waits run under the other's matrix
  * instructions, with one barrier a step and four steps' rows in LDS (one summed, one scored, two
- * arriving). 9 tokens of 128 heads over 131072 16-bit rows take 400 us (820 TFLOP/s) and over 8-bit
- * ones 430 us; four waves that did both in turn, 64 rows a step, took 478 and 504. A step of 32 rows
+ * arriving). 9 tokens of 128 heads over 131072 16-bit rows take 380 us (865 TFLOP/s) and over 8-bit
+ * ones 390 us; four waves that did both in turn, 64 rows a step, took 478 and 504 (where this took
+ * 400 and 430). A step of 32 rows
  * takes 2600 cycles, its products 1088; the rest is the way from a barrier to the first product
  * (page, addresses, LDS: 400) and from the last to the next barrier (exponentials, packing: 700).
  * The rows of a step lie in LDS once, row-major, for both products: the score reads them along
@@ -341,7 +342,8 @@ __global__ __launch_bounds__(L_THREADS) void k_attend_latent(AttendArgs a) {
         /* The maximum that probabilities are taken against is that of the first step in which a column
          * attends something; they may exceed 1 by 2^14, which costs no accuracy in either 16-bit type.
          * Where a later score exceeds it by more, the rows are gone through for the maxima alone and
-         * then once more: the sums are never rescaled. */
+         * then once more: the sums are never rescaled. So a call's time depends on its scores: queries
+         * three times as wide as those of the 380 us above, whose scores do so, take 930 us. */
         constexpr float ROOM = 14.0f;
         auto pass = [&]() __attribute__((always_inline)) {
             l[0] = l[1] = 0.0f;

@@ -13,9 +13,9 @@
  * through registers, where they become 16-bit ones once for the four waves; the next step's are
  * in flight while this one is worked on (two buffers).
  * It is bound by the products and by what a wave does between them: 8000 tokens at the end of 16384
- * rows, 32 heads of 128 over 4 of 16 bits take 1620 us (1000 TFLOP/s; 8-bit rows 1820), 2000 over 4048
- * 113 us (890); 4000 tokens of width 256 (one workgroup a unit) take 2820 us. A step of the two
- * workgroups of a unit takes 4000 cycles of which the matrix units are busy 52%; the exponentials,
+ * rows, 32 heads of 128 over 4 of 16 bits take 1640 us (990 TFLOP/s; 8-bit rows 1820), 2000 over 4048
+ * 113 us (890); 4000 tokens of width 256 (one workgroup a unit) take 2720 us. A step of the two
+ * workgroups of a unit takes 4000 cycles of which the matrix units are busy 54%; the exponentials,
  * maxima and packing of a wave take about as long as its products. Rows through registers into LDS
  * took 166 us for the 2000 tokens, page ids loaded where they are used 30 more.
  */

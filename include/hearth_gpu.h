@@ -388,7 +388,10 @@ HEARTH_API int hearth_gpu_attend(const hearth_gpu_cache *c, const hearth_gpu_bat
  * its key projection) and q_pe [n_tokens][H][R] (its rotated part) against the latent rows'
  * first C and last R elements, out [n_tokens][H][C] = softmax(scale * (q . c + q_pe . pe)) c.
  * C = 512, R = 64, cache width 576, one cache head; n_seqs times min(max_q, n_tokens) * H / 64,
- * rounded up, at most 8388592 (somewhat below 2^29 / 64); everything else as hearth_gpu_attend. */
+ * rounded up, at most 8388592 (somewhat below 2^29 / 64); everything else as hearth_gpu_attend. Its
+ * time depends on the scores: where a head's scores over a share of the rows exceed the largest of
+ * that share's first 32 by more than 14 ln 2 = 9.7, the share is gone through three times (up to 2.7
+ * times the call's time). */
 HEARTH_API int hearth_gpu_attend_latent(const hearth_gpu_cache *c, const hearth_gpu_batch *b,
                                         const hearth_gpu_array *q, const hearth_gpu_array *q_pe,
                                         const hearth_gpu_array *out, float *lse, float scale, void *work,
