@@ -26,20 +26,20 @@ constexpr int64_t MAX_ROPE_ROW = 1 << 24;           /* elements of a token: four
 bool pow2(int x) { return x > 0 && (x & (x - 1)) == 0; }
 
 bool rows_ok(const hearth_gpu_rows &r, const hearth_gpu_cache &c) {
-    const bool mx = c.dtype == HEARTH_GPU_MX8;
-    const int es = mx ? 1 : 2;
-    const int64_t block = (int64_t)c.page * c.width;
+    const int bits = bits_of(c.dtype);
+    const int es = bits == 16 ? 2 : 1;                                              /* bytes of a stride's element */
+    const int64_t els = (int64_t)c.page * c.width, block = bits == 4 ? els / 2 : els;
     if (!r.data || (uintptr_t)r.data % 16) return false;
     if (r.head_stride < (c.n_heads > 1 ? block : 0) || r.page_stride < (c.n_pages > 1 ? block : 0)) return false;
     if (r.head_stride > MAX_STRIDE || r.page_stride > MAX_STRIDE) return false;
     if (r.head_stride * es % 16 || r.page_stride * es % 16) return false;
-    if (!mx) return true;
-    if (!r.scales || r.scale_head_stride < (c.n_heads > 1 ? block / MX_BLOCK : 0) || r.scale_head_stride > MAX_STRIDE) return false;
-    return r.scale_page_stride >= (c.n_pages > 1 ? block / MX_BLOCK : 0) && r.scale_page_stride <= MAX_STRIDE;
+    if (bits == 16) return true;
+    if (!r.scales || r.scale_head_stride < (c.n_heads > 1 ? els / MX_BLOCK : 0) || r.scale_head_stride > MAX_STRIDE) return false;
+    return r.scale_page_stride >= (c.n_pages > 1 ? els / MX_BLOCK : 0) && r.scale_page_stride <= MAX_STRIDE;
 }
 
 bool cache_ok(const hearth_gpu_cache *c) {
-    if (!c || (c->dtype != HEARTH_F16 && c->dtype != HEARTH_BF16 && c->dtype != HEARTH_GPU_MX8)) return false;
+    if (!c || (c->dtype != HEARTH_F16 && c->dtype != HEARTH_BF16 && c->dtype != HEARTH_GPU_MX8 && c->dtype != HEARTH_GPU_MX4)) return false;
     if (c->n_pages < 1 || c->n_heads < 1 || c->n_heads > 4096 || !pow2(c->page) || c->page < 16 || c->page > 4096) return false;
     if (c->width < 32 || c->width > 1024 || c->width % 32) return false;
     return rows_ok(c->k, *c) && (!c->v.data || rows_ok(c->v, *c));
@@ -75,7 +75,7 @@ bool on16(const hearth_gpu_array &x) {
 }
 
 Rows rows_of(const hearth_gpu_rows &r, int dtype) {
-    const int64_t es = dtype == HEARTH_GPU_MX8 ? 1 : 2;
+    const int64_t es = bits_of(dtype) == 16 ? 2 : 1;
     return {(uint8_t *)r.data, r.scales, r.page_stride * es, r.head_stride * es, r.scale_page_stride, r.scale_head_stride};
 }
 
@@ -144,7 +144,7 @@ bool attend_shape_ok(const hearth_gpu_cache *c, const hearth_gpu_batch *b, int h
     if ((int64_t)o.max_q * heads > (1 << 26) || o.kv_cap > MAX_ROWS) return false;
     if (!c->v.data && ((int64_t)o.max_q * heads + 63) / 64 * o.n_seqs > MAX_LATENT_TILES) return false;
     if (c->v.data) return c->width == 64 || c->width == 128 || c->width == 256;
-    return c->width == 576 && c->n_heads == 1;
+    return c->width == 576 && c->n_heads == 1 && c->dtype != HEARTH_GPU_MX4;
 }
 
 int64_t part_bytes(const hearth_gpu_cache &c, const hearth_gpu_batch &b, int heads, Split &s) {
@@ -161,7 +161,7 @@ int attend_call(const hearth_gpu_cache *c, const hearth_gpu_batch *b, const hear
     const bool latent = q_pe != nullptr;
     if (latent != !c->v.data || (uintptr_t)lse % 4 || !std::isfinite(scale * 1.44269504088896340736f)) return E_ARG;
     if ((q->dtype != HEARTH_F16 && q->dtype != HEARTH_BF16) || out->dtype != q->dtype || !apart(*out, b->n_tokens)) return E_ARG;
-    if (c->dtype != HEARTH_GPU_MX8 && c->dtype != q->dtype) return E_ARG;
+    if (bits_of(c->dtype) == 16 && c->dtype != q->dtype) return E_ARG;
     const int width = latent ? 512 : c->width;
     if (q->width != width || out->width != width || out->n_heads != q->n_heads) return E_ARG;
     if (latent && (!array_ok(q_pe, b->n_tokens) || q_pe->dtype != q->dtype || q_pe->n_heads != q->n_heads || q_pe->width != 64)) return E_ARG;

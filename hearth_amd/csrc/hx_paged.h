@@ -15,8 +15,10 @@
 
 namespace hxp {
 
-enum { DT_F32 = HEARTH_F32, DT_F16 = HEARTH_F16, DT_BF16 = HEARTH_BF16, DT_MX8 = HEARTH_GPU_MX8 };
+enum { DT_F32 = HEARTH_F32, DT_F16 = HEARTH_F16, DT_BF16 = HEARTH_BF16, DT_MX8 = HEARTH_GPU_MX8, DT_MX4 = HEARTH_GPU_MX4 };
 constexpr int MX_BLOCK = 32;
+/* bits of a stored element; below 16: codes with a scale byte for each MX_BLOCK */
+constexpr int bits_of(int dtype) { return dtype == DT_MX4 ? 4 : dtype == DT_MX8 ? 8 : 16; }
 
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
@@ -175,6 +177,10 @@ struct Bf16 {
     template <bool HI> static __device__ __forceinline__ unsigned from_mx8(unsigned x, float s) {
         return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, s, HI));
     }
+    /* two 4-bit codes (byte B of x, the lower half first) likewise */
+    template <int B> static __device__ __forceinline__ unsigned from_mx4(unsigned x, float s) {
+        return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x, s, B));
+    }
     /* round to nearest even, both halves */
     static __device__ __forceinline__ unsigned pack(float a, float b) { return __builtin_bit_cast(unsigned, __builtin_convertvector((f2){a, b}, b2)); }
     static __device__ __forceinline__ float wide(unsigned x) { return __uint_as_float(x << 16); }   /* of the lower half */
@@ -193,6 +199,9 @@ struct F16 {
     template <bool HI> static __device__ __forceinline__ unsigned from_mx8(unsigned x, float s) {
         return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, s, HI));
     }
+    template <int B> static __device__ __forceinline__ unsigned from_mx4(unsigned x, float s) {
+        return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(x, s, B));
+    }
     static __device__ __forceinline__ unsigned pack(float a, float b) { return __builtin_bit_cast(unsigned, __builtin_convertvector((f2){a, b}, h2)); }
     static __device__ __forceinline__ float wide(unsigned x) { return (float)__builtin_bit_cast(_Float16, (unsigned short)x); }
     static __device__ __forceinline__ unsigned clean(unsigned x) {
@@ -202,9 +211,11 @@ struct F16 {
 };
 
 /* Element d of a stored row (row: its first byte, sc: its first scale byte) in T's format */
-template <class T, bool MX>
+template <class T, int BITS>
 __device__ __forceinline__ unsigned row_elem(const uint8_t *row, const uint8_t *sc, int d) {
-    if constexpr (MX)
+    if constexpr (BITS == 4)
+        return T::template from_mx4<0>((unsigned)row[d >> 1] >> (4 * (d & 1)), __uint_as_float((unsigned)sc[d / MX_BLOCK] << 23)) & 0xffffu;
+    else if constexpr (BITS == 8)
         return T::template from_mx8<false>((unsigned)row[d], __uint_as_float((unsigned)sc[d / MX_BLOCK] << 23)) & 0xffffu;
     else
         return ((const unsigned short *)row)[d];
@@ -216,7 +227,8 @@ typedef u2 u2_any __attribute__((aligned(1)));
 typedef unsigned unsigned_any __attribute__((aligned(1)));
 typedef unsigned short ushort_any __attribute__((aligned(1)));
 
-/* the scale of a block from its byte (1 to 254) */
+/* the scale of a block from its byte (1 to 254; 255, of a 4-bit block that holds a NaN or an infinity, makes
+ * every conversion of its codes a NaN) */
 __device__ __forceinline__ float mx_scale(unsigned byte) { return __uint_as_float((byte & 255u) << 23); }
 
 /* maximum / sum of a value over the lanes l, l ^ 32 */

@@ -165,6 +165,12 @@ __global__ __launch_bounds__(ROPE_THREADS) void k_rope(RopeArgs a, int tok) {
  * above 1.9375) the code is cut to 240, which is within half a step (2^-4) of the value. */
 __device__ __forceinline__ bool fin(float x) { return __builtin_fabsf(x) < __builtin_huge_valf(); }
 
+/* over four neighbouring lanes */
+__device__ __forceinline__ float max_of4(float m) {
+    m = fmaxf(m, __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(m), 0xB1, 0xF, 0xF, true)));
+    return fmaxf(m, __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(m), 0x4E, 0xF, 0xF, true)));
+}
+
 /* The eight elements that a thread of either kernel takes of each of its tokens: octs threads a
  * token (grid.z of them where that is more than a workgroup), several tokens a workgroup where it is
  * less; which piece, head and element they are is worked out once for COPY_TOKENS tokens (16 x 4093
@@ -204,7 +210,7 @@ __device__ __forceinline__ void append_item(const CopyArgs &a, const Seq &q, con
     const uint8_t *src = p.arr + (int64_t)(q.q0 + tok) * p.at + (int64_t)h * p.ah + (int64_t)d * E::size;
     uint8_t *dst = p.rows.data + (int64_t)page * p.rows.page_stride + (int64_t)h * p.rows.head_stride;
     const int64_t el = (int64_t)row * p.row_width + p.col + d;
-    if constexpr (DST == SRC && DST != DT_MX8) {
+    if constexpr (DST == SRC) {
         if (WIDE) *(u4 *)(dst + el * 2) = *(const u4 *)src;
         else {
             unsigned short w[8];
@@ -216,14 +222,33 @@ __device__ __forceinline__ void append_item(const CopyArgs &a, const Seq &q, con
     } else {
         float v[8];
         E::load8(src, WIDE, v);
-        if constexpr (DST != DT_MX8) {
+        if constexpr (bits_of(DST) == 16) {
             Elem<DST>::store8(dst + el * 2, true, v);
+        } else if constexpr (DST == DT_MX4) {
+            float m = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8; j++) m = fmaxf(m, fin(v[j]) ? __builtin_fabsf(v[j]) : __builtin_huge_valf());
+            m = max_of4(m);
+            /* least exponent with m <= 7 * 2^e = 1.75 * 2^(e + 2); 255 (a block of NaN) where m is infinite */
+            const int bits = (int)__float_as_uint(m);
+            const bool whole = fin(m);
+            const int byte = whole ? max((bits >> 23) - 2 + ((bits & 0x7fffff) > 0x600000), 1) : 255;
+            const float scale = mx_scale(whole ? byte : 127);
+            /* 4 would leave the source type's range: 3, within half a step */
+            const float top = (SRC == DT_F16 ? byte == 127 + 14 : byte == 127 + 126) ? 3.0f * scale : __builtin_huge_valf();
+            unsigned c = 0;
+            each<4>([&](auto j) {
+                const float a = whole ? fminf(fmaxf(v[2 * j], -top), top) : 0.0f, b = whole ? fminf(fmaxf(v[2 * j + 1], -top), top) : 0.0f;
+                c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, a, b, scale, j);   /* rounds to nearest even, above 6 to 6 */
+            });
+            *(unsigned *)(dst + el / 2) = c;
+            if ((d & 31) == 0)
+                p.rows.scales[(int64_t)page * p.rows.scale_page_stride + (int64_t)h * p.rows.scale_head_stride + el / MX_BLOCK] = (uint8_t)byte;
         } else {
             float m = 0.0f;
 #pragma unroll
             for (int j = 0; j < 8; j++) m = fmaxf(m, fin(v[j]) ? __builtin_fabsf(v[j]) : 0.0f);
-            m = fmaxf(m, __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(m), 0xB1, 0xF, 0xF, true)));
-            m = fmaxf(m, __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(m), 0x4E, 0xF, 0xF, true)));
+            m = max_of4(m);
             const int bits = (int)__float_as_uint(m);
             const int byte = max((bits >> 23) - 8 + ((bits & 0x7fffff) > 0x600000), 1);   /* e + 127 */
             const float inv = __uint_as_float((unsigned)(254 - byte) << 23);
@@ -271,7 +296,14 @@ __device__ __forceinline__ void read_item(const CopyArgs &a, const Seq &q, const
     if (page_ok(a.b, page)) {
         const uint8_t *src = p.rows.data + (int64_t)page * p.rows.page_stride + (int64_t)h * p.rows.head_stride;
         const int64_t el = (int64_t)row * p.row_width + p.col + d;
-        if constexpr (SRC == DT_MX8) {
+        if constexpr (SRC == DT_MX4) {
+            const unsigned c = *(const unsigned *)(src + el / 2);
+            const float s = mx_scale(p.rows.scales[(int64_t)page * p.rows.scale_page_stride + (int64_t)h * p.rows.scale_head_stride + el / MX_BLOCK]);
+            each<4>([&](auto j) {
+                const f2 x = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, j);
+                v[2 * j] = x[0]; v[2 * j + 1] = x[1];
+            });
+        } else if constexpr (SRC == DT_MX8) {
             const u2 c = *(const u2 *)(src + el);
             const float s = mx_scale(p.rows.scales[(int64_t)page * p.rows.scale_page_stride +
                                                    (int64_t)h * p.rows.scale_head_stride + el / MX_BLOCK]);
@@ -352,7 +384,8 @@ static void by_types(int arr, int rows, F f) {
     auto with = [&](auto a) {
         if (rows == DT_F16) f(a, std::integral_constant<int, DT_F16>{});
         else if (rows == DT_BF16) f(a, std::integral_constant<int, DT_BF16>{});
-        else f(a, std::integral_constant<int, DT_MX8>{});
+        else if (rows == DT_MX8) f(a, std::integral_constant<int, DT_MX8>{});
+        else f(a, std::integral_constant<int, DT_MX4>{});
     };
     if (arr == DT_F32) with(std::integral_constant<int, DT_F32>{});
     else if (arr == DT_F16) with(std::integral_constant<int, DT_F16>{});

@@ -33,26 +33,44 @@ constexpr int FEW_WAVES = 4, FEW_STEP = 32;   /* a wave takes 32 cache rows at a
 __device__ __forceinline__ unsigned lo16(unsigned a, unsigned b) { return __builtin_amdgcn_perm(b, a, 0x05040100u); }
 __device__ __forceinline__ unsigned hi16(unsigned a, unsigned b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
 
-template <class T, bool MX, int D>
+template <class T, int BITS, int D>
 struct Few {
     using v8 = typename T::v8;
+    static constexpr bool MX = BITS < 16;
     static constexpr int KS = D / 32;                    /* matrix steps of the score */
     static constexpr int BD = D < 128 ? D : 128;        /* elements of a V block: 16 lanes x PL */
     static constexpr int NB = D / BD, PL = BD / 16;      /* blocks; elements of a row a lane takes */
-    static constexpr int ES = MX ? 1 : 2;                 /* bytes of a stored element */
+    static constexpr int RB = D * BITS / 8;               /* bytes of a row */
 
-    static constexpr int KL = MX ? D / 64 : KS;           /* 16-byte loads of a row for the score */
-    static constexpr int VW = MX ? PL / 4 : PL / 2;       /* words of a row and block for the sum */
+    /* Score: the four lanes of a row take LB bytes each a load, LE elements, SL matrix steps */
+    static constexpr int LB = RB / 4 < 16 ? RB / 4 : 16, KL = RB / (4 * LB), LE = LB * 8 / BITS, SL = LE / 8;
+    static constexpr int VB = PL * BITS / 8;              /* bytes of a row and block for the sum */
+    static constexpr int VW = VB < 4 ? 1 : VB / 4;
     static constexpr int SW = D / 32 < 4 ? 1 : D / 128;   /* words that hold a row's scales */
 
-    struct K { u4 w[2][KL]; unsigned s[2][SW]; };         /* a lane's row of either tile of 16 */
+    struct K { unsigned w[2][KL][LB / 4]; unsigned s[2][SW]; };   /* a lane's row of either tile of 16 */
     struct V { unsigned w[NB][8][VW]; unsigned s[2][D / 32]; };   /* eight rows; scales of the four rows of either tile */
 
+    /* first element that a lane multiplies in matrix step i */
+    static __device__ __forceinline__ int at(int i, int g) { return 4 * LE * (i / SL) + LE * g + 8 * (i % SL); }
+
+    /* BYTES at p (a multiple of 16, 8, 4 or 2) */
+    template <int BYTES> static __device__ __forceinline__ void words(const uint8_t *p, unsigned *w) {
+        if constexpr (BYTES == 16) {
+            const u4 x = *(const u4 *)p;
+#pragma unroll
+            for (int i = 0; i < 4; i++) w[i] = x[i];
+        } else if constexpr (BYTES == 8) {
+            const u2 x = *(const u2 *)p;
+            w[0] = x[0]; w[1] = x[1];
+        } else if constexpr (BYTES == 4) w[0] = *(const unsigned *)p;
+        else w[0] = *(const unsigned short *)p;
+    }
     /* row: first of the tile in its page (a multiple of 16) */
     static __device__ __forceinline__ void load_k(K &k, int u, const uint8_t *page, const uint8_t *sc, int row, int g, int lc) {
-        const uint8_t *p = page + (row + lc) * (D * ES) + 16 * g;
+        const uint8_t *p = page + (row + lc) * RB + LB * g;
 #pragma unroll
-        for (int i = 0; i < KL; i++) k.w[u][i] = *(const u4 *)(p + 64 * i);
+        for (int i = 0; i < KL; i++) words<LB>(p + 4 * LB * i, k.w[u][i]);
         if constexpr (MX) {
             const uint8_t *q = sc + (row + lc) * (D / MX_BLOCK);
             if constexpr (D == 64) k.s[u][0] = *(const ushort_any *)q;
@@ -65,19 +83,8 @@ struct Few {
 #pragma unroll
         for (int b = 0; b < NB; b++)
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const uint8_t *p = page + (row + 4 * g + j) * (D * ES) + (b * BD + lc * PL) * ES;
-                if constexpr (VW == 4) {
-                    const u4 x = *(const u4 *)p;
-#pragma unroll
-                    for (int i = 0; i < 4; i++) v.w[b][4 * u + j][i] = x[i];
-                } else if constexpr (VW == 2) {
-                    const u2 x = *(const u2 *)p;
-                    v.w[b][4 * u + j][0] = x[0]; v.w[b][4 * u + j][1] = x[1];
-                } else {
-                    v.w[b][4 * u + j][0] = *(const unsigned *)p;
-                }
-            }
+            for (int j = 0; j < 4; j++)
+                words<VB>(page + (row + 4 * g + j) * RB + (b * BD + lc * PL) * BITS / 8, v.w[b][4 * u + j]);
         if constexpr (MX) {   /* four rows' scales lie side by side */
             const uint8_t *q = sc + (row + 4 * g) * (D / MX_BLOCK);
 #pragma unroll
@@ -96,18 +103,23 @@ struct Few {
     static __device__ __forceinline__ void scores(const K &k, int u, int g, const v8 (&q)[KS], f4 &s) {
 #pragma unroll
         for (int i = 0; i < KL; i++) {
+            const unsigned *x = k.w[u][i];
             if constexpr (MX) {
-                /* block 2 i + g / 2 */
-                const float f = mx_scale(k.s[u][i >> 1] >> (16 * (i & 1) + 8 * (g >> 1)));
+                /* block LE i / 8 + LE g / 32, which does not leave the word */
+                const float f = mx_scale(k.s[u][LE * i / 32] >> (8 * (LE * i / 8 % 4) + 8 * (LE * g / 32)));
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const unsigned a = k.w[u][i][2 * h], b = k.w[u][i][2 * h + 1];
-                    const u4 w = {T::template from_mx8<false>(a, f), T::template from_mx8<true>(a, f),
-                                  T::template from_mx8<false>(b, f), T::template from_mx8<true>(b, f)};
-                    s = T::mfma16(__builtin_bit_cast(v8, w), q[2 * i + h], s);
+                for (int h = 0; h < SL; h++) {
+                    u4 w;
+                    if constexpr (BITS == 4)
+                        w = (u4){T::template from_mx4<0>(x[h], f), T::template from_mx4<1>(x[h], f), T::template from_mx4<2>(x[h], f),
+                                 T::template from_mx4<3>(x[h], f)};
+                    else
+                        w = (u4){T::template from_mx8<false>(x[2 * h], f), T::template from_mx8<true>(x[2 * h], f),
+                                 T::template from_mx8<false>(x[2 * h + 1], f), T::template from_mx8<true>(x[2 * h + 1], f)};
+                    s = T::mfma16(__builtin_bit_cast(v8, w), q[SL * i + h], s);
                 }
             } else {
-                s = T::mfma16(__builtin_bit_cast(v8, k.w[u][i]), q[i], s);
+                s = T::mfma16(__builtin_bit_cast(v8, (u4){x[0], x[1], x[2], x[3]}), q[i], s);
             }
         }
     }
@@ -119,11 +131,14 @@ struct Few {
             if constexpr (D == 64) x = v.s[j >> 2][jj >> 1] >> (16 * (jj & 1) + 8 * (lc >> 3));
             else x = v.s[j >> 2][jj * (D / 128) + b] >> (8 * (lc >> 2));
             const float f = mx_scale(x);
+            if constexpr (BITS == 4)
+                each<PL / 2>([&](auto i) { w[i] = T::template from_mx4<i.value>(v.w[b][j][0], f); });
+            else
 #pragma unroll
-            for (int i = 0; i < VW; i++) {
-                w[2 * i] = T::template from_mx8<false>(v.w[b][j][i], f);
-                w[2 * i + 1] = T::template from_mx8<true>(v.w[b][j][i], f);
-            }
+                for (int i = 0; i < VW; i++) {
+                    w[2 * i] = T::template from_mx8<false>(v.w[b][j][i], f);
+                    w[2 * i + 1] = T::template from_mx8<true>(v.w[b][j][i], f);
+                }
         } else {
 #pragma unroll
             for (int i = 0; i < VW; i++) w[i] = v.w[b][j][i];
@@ -131,11 +146,12 @@ struct Few {
     }
 };
 
-template <class T, bool MX, int D>
+template <class T, int BITS, int D>
 __global__ __launch_bounds__(64 * FEW_WAVES) void k_attend_few(AttendArgs a) {
-    using F = Few<T, MX, D>;
+    using F = Few<T, BITS, D>;
     using v8 = typename T::v8;
-    constexpr int PL = F::PL, NB = F::NB, BD = F::BD, ES = F::ES, CT = 16;
+    constexpr bool MX = F::MX;
+    constexpr int PL = F::PL, NB = F::NB, BD = F::BD, CT = 16;
     __shared__ float lds_o[FEW_WAVES][16][BD + 4];
     __shared__ float lds_m[FEW_WAVES][CT], lds_l[FEW_WAVES][CT];
     __shared__ unsigned lds_some[FEW_WAVES];   /* bit c: column c attends a row of the wave's */
@@ -163,8 +179,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_attend_few(AttendArgs a) {
     const uint8_t *qp = a.q + (int64_t)(q.q0 + tok) * a.qt + (int64_t)head * a.qh;
 #pragma unroll
     for (int i = 0; i < F::KS; i++) {
-        const int d = MX ? 64 * (i / 2) + 16 * g + 8 * (i % 2) : 32 * i + 8 * g;
-        const unsigned short *p = (const unsigned short *)qp + d;
+        const unsigned short *p = (const unsigned short *)qp + F::at(i, g);
         u4 w = {0, 0, 0, 0};
         if (on) w = *(const u4_any *)p;
         qf[i] = __builtin_bit_cast(v8, w);
@@ -307,7 +322,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_attend_few(AttendArgs a) {
                 if (t0 + FEW_STEP <= full && t0 + FEW_STEP <= hi && page_ok(a.b, word_of(pages, t0 >> a.b.page_shift)) &&
                     page_ok(a.b, word_of(pages, (t0 + 16) >> a.b.page_shift))) break;   /* a step taken as it is */
                 if (!page_ok(a.b, id)) continue;
-                const uint8_t *row = vbase + (int64_t)id * a.v.page_stride + (int64_t)(t & (page_rows - 1)) * (D * ES);
+                const uint8_t *row = vbase + (int64_t)id * a.v.page_stride + (int64_t)(t & (page_rows - 1)) * F::RB;
                 const uint8_t *sc = MX ? vsb + (int64_t)id * a.v.scale_page_stride + (t & (page_rows - 1)) * (D / MX_BLOCK) : nullptr;
 #pragma unroll
                 for (int b = 0; b < NB; b++)
@@ -315,7 +330,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_attend_few(AttendArgs a) {
                     for (int j = 0; j < PL; j++)
 #pragma unroll
                         for (int i = 0; i < 4; i++) {
-                            const unsigned x = row_elem<T, MX>(row, sc, b * BD + (4 * g + i) * PL + j);
+                            const unsigned x = row_elem<T, BITS>(row, sc, b * BD + (4 * g + i) * PL + j);
                             acc[b * PL + j][i] += T::odd(x) && (attended(t) & 1) ? T::wide(x) : 0.0f;
                         }
             }
@@ -464,11 +479,11 @@ __global__ __launch_bounds__(JOIN_THREADS) void k_attend_join(AttendArgs a) {
     if (a.lse && e == 0) a.lse[row] = L == 0.0f ? NINF : (M + __log2f(L)) * 0.69314718055994531f;
 }
 
-template <class T, bool MX, int D>
+template <class T, int BITS, int D>
 void few_t(const AttendArgs &a, hipStream_t st) {
     const int tiles = (a.b.max_q * a.group + 15) / 16;
     const dim3 grid((unsigned)a.n_splits * a.kv_heads * tiles, 1, a.b.n_seqs);
-    hipLaunchKernelGGL((k_attend_few<T, MX, D>), grid, dim3(64 * FEW_WAVES), 0, st, a);
+    hipLaunchKernelGGL((k_attend_few<T, BITS, D>), grid, dim3(64 * FEW_WAVES), 0, st, a);
 }
 
 template <class T, int DV>
@@ -507,9 +522,9 @@ Split attend_split(int n_seqs, int max_q, int kv_cap, int heads, int kv_heads, b
 }
 
 void attend(const AttendArgs &a, int q_dtype, int cache_dtype, int width, bool many, hipStream_t st) {
-    const bool mx = cache_dtype == DT_MX8;
+    const int bits = bits_of(cache_dtype);
 #define HXP_BY(F, T) (width == 64 ? F(T, 64) : width == 128 ? F(T, 128) : F(T, 256))
-#define HXP_FEW(T, D) (mx ? few_t<T, true, D>(a, st) : few_t<T, false, D>(a, st))
+#define HXP_FEW(T, D) (bits == 16 ? few_t<T, 16, D>(a, st) : bits == 8 ? few_t<T, 8, D>(a, st) : few_t<T, 4, D>(a, st))
 #define HXP_JOIN(T, D) join_t<T, D>(a, st)
     if (many) attend_many(a, q_dtype, cache_dtype, width, st);
     else if (q_dtype == DT_BF16) HXP_BY(HXP_FEW, Bf16);

@@ -514,7 +514,7 @@ __global__ __launch_bounds__(L_THREADS) void k_attend_latent(AttendArgs a) {
             const uint8_t *sc = MX ? a.k.scales + (int64_t)id * a.k.scale_page_stride + (t & rmask) * (LW / MX_BLOCK) : nullptr;
 #pragma unroll 1
             for (int e = 0; e < 64; e++) {
-                const unsigned v = row_elem<T, MX>(rp, sc, 64 * wave + e);
+                const unsigned v = row_elem<T, MX ? 8 : 16>(rp, sc, 64 * wave + e);
                 if (T::odd(v)) ((float *)unit(lane, 16 * wave + (e >> 2)))[e & 3] += T::wide(v);
             }
         }

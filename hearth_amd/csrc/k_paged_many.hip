@@ -47,10 +47,11 @@ struct Many {
     static __device__ __forceinline__ int at(int r, int p) { return (r * PIECES + (p ^ swz(r))) * 16; }
 };
 
-template <class T, bool MX, int D>
+template <class T, int BITS, int D>
 __global__ __launch_bounds__(64 * MANY_WAVES, D <= 128 ? 2 : 1) void k_attend_many(AttendArgs a) {
     using M = Many<D>;
     using v8 = typename T::v8;
+    constexpr bool MX = BITS < 16;
     constexpr int KS = D / 16, DT = D / 32;
     constexpr float NINF = -__builtin_huge_valf();
     __shared__ __align__(16) uint8_t lds[2][2][M::TILE];   /* buffer, K or V */
@@ -127,14 +128,18 @@ __global__ __launch_bounds__(64 * MANY_WAVES, D <= 128 ? 2 : 1) void k_attend_ma
         id_next = __builtin_amdgcn_readlane(ok ? pv : 0, wave * (M::ROWS / 4) / 16);
     };
     /* A wave brings in a quarter of the step's rows of K and of V; they lie in one page. 16-bit: 1 KiB
-     * of LDS an instruction, 16 bytes a lane; 8-bit: 16 codes a lane, two pieces. */
-    constexpr int RW = M::ROWS / 4, LANES = MX ? M::PIECES / 2 : M::PIECES, RI = 64 / LANES, N = RW / RI;   /* lanes of a row, rows an instruction, instructions */
+     * of LDS an instruction, 16 bytes a lane; 8-bit: 16 codes a lane, two pieces; 4-bit: 32 codes, four
+     * pieces (of width 64 16, two, so that a lane has no more than a row's part of the wave's 16 rows). */
+    constexpr int PL = BITS == 16 ? 1 : BITS == 8 || D == 64 ? 2 : 4, WORDS = PL * BITS / 4;   /* pieces and words a lane */
+    constexpr int RW = M::ROWS / 4, LANES = M::PIECES / PL, RI = 64 / LANES, N = RW / RI;   /* lanes of a row, rows an instruction, instructions */
+    constexpr int RB = D * BITS / 8;                                                          /* bytes of a row */
+    static_assert(N >= 1 && N * RI == RW);
     const int my = wave * RW, lr = lane / LANES, lp = lane % LANES;
     /* 16-bit: byte of a lane's pieces in memory (the z-th instruction's 1 KiB further, there and in LDS) */
     int off[N];
 #pragma unroll
     for (int z = 0; z < N; z++) off[z] = lr * (2 * D) + (lp ^ M::swz(my + z * RI + lr)) * 16;
-    u4 sw[MX ? 2 * N : 1];
+    unsigned sw[MX ? 2 * N : 1][WORDS];
     unsigned ss[MX ? 2 * N : 1];
     /* Every load goes to a row of the cache: rows past hi lie in the same page, those of a page that
      * is not there are taken from page 0; settle clears both. */
@@ -142,13 +147,21 @@ __global__ __launch_bounds__(64 * MANY_WAVES, D <= 128 ? 2 : 1) void k_attend_ma
         const int64_t id = id_next;
         const int row = (t0 + my) & rmask;
         if constexpr (MX) {
-            const uint8_t *kp = kbase + id * a.k.page_stride + row * D, *vp = vbase + id * a.v.page_stride + row * D;
+            const uint8_t *kp = kbase + id * a.k.page_stride + row * RB, *vp = vbase + id * a.v.page_stride + row * RB;
             const uint8_t *kq = ksb + id * a.k.scale_page_stride + row * (D / MX_BLOCK), *vq = vsb + id * a.v.scale_page_stride + row * (D / MX_BLOCK);
 #pragma unroll
             for (int z = 0; z < 2 * N; z++) {
                 const int r = z % N * RI + lr;
-                sw[z] = *(const u4 *)((z < N ? kp : vp) + r * D + 16 * lp);
-                ss[z] = (z < N ? kq : vq)[r * (D / MX_BLOCK) + (lp >> 1)];
+                const uint8_t *p = (z < N ? kp : vp) + r * RB + 4 * WORDS * lp;
+                if constexpr (WORDS == 4) {
+                    const u4 x = *(const u4 *)p;
+#pragma unroll
+                    for (int i = 0; i < 4; i++) sw[z][i] = x[i];
+                } else {
+                    const u2 x = *(const u2 *)p;
+                    sw[z][0] = x[0]; sw[z][1] = x[1];
+                }
+                ss[z] = (z < N ? kq : vq)[r * (D / MX_BLOCK) + lp * PL / 4];
             }
         } else {
             const uint8_t *kp = same(kbase + id * a.k.page_stride + (int64_t)row * (2 * D)), *vp = same(vbase + id * a.v.page_stride + (int64_t)row * (2 * D));
@@ -179,12 +192,18 @@ __global__ __launch_bounds__(64 * MANY_WAVES, D <= 128 ? 2 : 1) void k_attend_ma
                 const int r = my + z % N * RI + lr;
                 const float f = mx_scale(ss[z]);
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const unsigned x = sw[z][2 * h], y = sw[z][2 * h + 1];
-                    u4 w = {T::template from_mx8<false>(x, f), T::template from_mx8<true>(x, f),
-                            T::template from_mx8<false>(y, f), T::template from_mx8<true>(y, f)};
+                for (int h = 0; h < PL; h++) {
+                    u4 w;
+                    if constexpr (BITS == 4) {
+                        const unsigned x = sw[z][h];
+                        w = (u4){T::template from_mx4<0>(x, f), T::template from_mx4<1>(x, f), T::template from_mx4<2>(x, f), T::template from_mx4<3>(x, f)};
+                    } else {
+                        const unsigned x = sw[z][2 * h], y = sw[z][2 * h + 1];
+                        w = (u4){T::template from_mx8<false>(x, f), T::template from_mx8<true>(x, f),
+                                 T::template from_mx8<false>(y, f), T::template from_mx8<true>(y, f)};
+                    }
                     if (z >= N && edge) w = clear(r, w);
-                    *(u4 *)(lds[buf][z >= N] + M::at(r, 2 * lp + h)) = w;
+                    *(u4 *)(lds[buf][z >= N] + M::at(r, PL * lp + h)) = w;
                 }
             }
         } else {
@@ -339,13 +358,13 @@ __global__ __launch_bounds__(64 * MANY_WAVES, D <= 128 ? 2 : 1) void k_attend_ma
             const int id = word_of(pages, t >> a.b.page_shift);
             if (!page_ok(a.b, id)) continue;
             const bool add = attended(t) & 1;
-            const uint8_t *row = vbase + (int64_t)id * a.v.page_stride + (int64_t)(t & rmask) * (D * (MX ? 1 : 2));
+            const uint8_t *row = vbase + (int64_t)id * a.v.page_stride + (int64_t)(t & rmask) * RB;
             const uint8_t *sc = MX ? vsb + (int64_t)id * a.v.scale_page_stride + (t & rmask) * (D / MX_BLOCK) : nullptr;
 #pragma unroll
             for (int i = 0; i < DT; i++)
 #pragma unroll
                 for (int j = 0; j < 16; j++) {
-                    const unsigned x = row_elem<T, MX>(row, sc, 32 * i + 8 * (j >> 2) + 4 * half + (j & 3));
+                    const unsigned x = row_elem<T, BITS>(row, sc, 32 * i + 8 * (j >> 2) + 4 * half + (j & 3));
                     acc[i][j] += add && T::odd(x) ? T::wide(x) : 0.0f;
                 }
         }
@@ -396,18 +415,18 @@ __global__ __launch_bounds__(64 * MANY_WAVES, D <= 128 ? 2 : 1) void k_attend_ma
     }
 }
 
-template <class T, bool MX, int D>
+template <class T, int BITS, int D>
 void many_t(const AttendArgs &a, hipStream_t st) {
     const int64_t tiles = ((int64_t)a.b.max_q * a.group + MANY_COLS - 1) / MANY_COLS;
     const dim3 grid((unsigned)(tiles * a.n_splits * a.kv_heads), 1, a.b.n_seqs);
-    hipLaunchKernelGGL((k_attend_many<T, MX, D>), grid, dim3(64 * MANY_WAVES), 0, st, a);
+    hipLaunchKernelGGL((k_attend_many<T, BITS, D>), grid, dim3(64 * MANY_WAVES), 0, st, a);
 }
 
 } // namespace
 
 void attend_many(const AttendArgs &a, int q_dtype, int cache_dtype, int width, hipStream_t st) {
-    const bool mx = cache_dtype == DT_MX8;
-#define HXP_MANY(T, D) (mx ? many_t<T, true, D>(a, st) : many_t<T, false, D>(a, st))
+    const int bits = bits_of(cache_dtype);
+#define HXP_MANY(T, D) (bits == 16 ? many_t<T, 16, D>(a, st) : bits == 8 ? many_t<T, 8, D>(a, st) : many_t<T, 4, D>(a, st))
     if (q_dtype == DT_BF16) width == 64 ? HXP_MANY(Bf16, 64) : width == 128 ? HXP_MANY(Bf16, 128) : HXP_MANY(Bf16, 256);
     else width == 64 ? HXP_MANY(F16, 64) : width == 128 ? HXP_MANY(F16, 128) : HXP_MANY(F16, 256);
 #undef HXP_MANY

@@ -3,7 +3,7 @@
 For programs that keep many conversations' rows in pages next to (or without) an Engine:
 
     rope(x, pos, freqs)              rotary positions, in place or into `out`
-    append(cache, batch, k, v)       new tokens' rows into the pages, 16-bit or 8-bit ("mx8")
+    append(cache, batch, k, v)       new tokens' rows into the pages, 16-bit, 8-bit ("mx8") or 4-bit ("mx4")
     read(cache, batch, k, v)         rows back out of the pages
     attend(cache, batch, q, out)     grouped-head attention: tokens, chains, draft trees, prompts
     attend_latent(...)               absorbed latent attention over one row a token
@@ -33,8 +33,8 @@ from .engine import HearthError
 __all__ = ["Cache", "Batch", "rope", "rope_frequencies", "append", "read", "attend", "attend_latent",
            "workspace_bytes"]
 
-F32, F16, BF16, MX8 = 0, 1, 2, 16
-_DTYPES = {"float32": F32, "float16": F16, "bfloat16": BF16, "float8_e4m3fn": MX8}
+F32, F16, BF16, MX8, MX4 = 0, 1, 2, 16, 17
+_DTYPES = {"float32": F32, "float16": F16, "bfloat16": BF16, "float8_e4m3fn": MX8, "float4_e2m1fn_x2": MX4}
 
 
 class _Rows(Structure):
@@ -107,7 +107,7 @@ def _dtype(t) -> int:
     if c is None:
         c = _DTYPES.get(str(d).replace("torch.", ""))
         if c is None:
-            raise ValueError(f"dtype {d} is none of float32, float16, bfloat16 (float8_e4m3fn in a cache)")
+            raise ValueError(f"dtype {d} is none of float32, float16, bfloat16 (float8_e4m3fn, float4_e2m1fn_x2 in a cache)")
         _seen_dtypes[d] = c
     return c
 
@@ -144,7 +144,7 @@ def _array(t, what, dev) -> _Array:
     dt = _seen_dtypes.get(t.dtype)
     if dt is None:
         dt = _dtype(t)
-    if dt == MX8:
+    if dt >= MX8:
         raise ValueError(f"{what}: {t.dtype} rows live in a cache only")
     return _Array(t.data_ptr(), st, sh, dt, heads, width)
 
@@ -176,8 +176,9 @@ def _check(rc, what):
 
 
 class Cache:
-    """Rows of all sequences: k and v [pages, heads, rows a page, width], float16, bfloat16 or
-    float8_e4m3fn with scales (uint8 E8M0, [pages, heads, rows a page, width / 32]); v None:
+    """Rows of all sequences: k and v [pages, heads, rows a page, width], float16, bfloat16,
+    float8_e4m3fn or (two elements a byte, [.., width / 2]) float4_e2m1fn_x2, the latter two with
+    scales (uint8 E8M0, [pages, heads, rows a page, width / 32]); v None:
     latent rows (latent vector, then its rotated part). The last two dimensions are dense; the
     tensors are the caller's and stay referenced."""
 
@@ -186,11 +187,12 @@ class Cache:
         self.device = _device(k, "k")
         dt = _dtype(k)
         if dt == F32:
-            raise ValueError("cache rows are float16, bfloat16 or float8_e4m3fn")
+            raise ValueError("cache rows are float16, bfloat16, float8_e4m3fn or float4_e2m1fn_x2")
         s = _CacheS()
         if len(k.shape) != 4:
             raise ValueError(f"k: shape {tuple(k.shape)} is not [pages, heads, rows a page, width]")
         s.dtype, (s.n_pages, s.n_heads, s.page, s.width) = dt, k.shape
+        s.width *= 2 if dt == MX4 else 1
         s.k = self._rows(k, k_scale, "k", k, dt)
         if v is not None:
             s.v = self._rows(v, v_scale, "v", k, dt)
@@ -217,10 +219,10 @@ class Cache:
         if any(b % 16 for b in (t.data_ptr(), st[0] * t.element_size(), st[1] * t.element_size())):
             raise ValueError(f"{what}: data and strides must be multiples of 16 bytes")
         r = _Rows(t.data_ptr(), None, st[0], st[1], 0, 0)
-        if (scale is not None) != (dt == MX8):
-            raise ValueError(f"{what}: scales go with float8_e4m3fn rows, and only with them")
+        if (scale is not None) != (dt >= MX8):
+            raise ValueError(f"{what}: scales go with float8_e4m3fn and float4_e2m1fn_x2 rows, and only with them")
         if scale is not None:
-            want = (*t.shape[:3], t.shape[3] // 32)
+            want = (*t.shape[:3], t.shape[3] // (16 if dt == MX4 else 32))
             if tuple(scale.shape) != want or str(scale.dtype) not in ("torch.uint8", "torch.float8_e8m0fnu"):
                 raise ValueError(f"{what} scales: {scale.dtype}{tuple(scale.shape)}, wanted uint8{want}")
             _device(scale, f"{what} scales", self.device)
@@ -340,7 +342,7 @@ def _attend(name, cache, batch, q, q_pe, out, lse, scale, workspace, stream):
     a, o, tokens = _array(q, "q", dev), _array(out, "out", dev), q.shape[0]
     if out.shape[0] != tokens or o.n_heads != a.n_heads or o.width != a.width or a.dtype != o.dtype:
         raise ValueError(f"{name}: out is {out.dtype}{tuple(out.shape)}, q {q.dtype}{tuple(q.shape)}")
-    if a.dtype == F32 or cache._s.dtype not in (MX8, a.dtype):
+    if a.dtype == F32 or cache._s.dtype not in (MX8, MX4, a.dtype):
         raise ValueError(f"{name}: q is {q.dtype} over a cache of {cache.k.dtype}")
     lp = None
     if lse is not None:
@@ -372,7 +374,7 @@ def _attend(name, cache, batch, q, q_pe, out, lse, scale, workspace, stream):
 
 def attend(cache: Cache, batch: Batch, q, out, *, scale: float, lse=None, workspace=None, stream=0) -> None:
     """out = softmax(scale * q k) v of the call's tokens over the rows each attends; q, out
-    [tokens, heads, width] of the cache's 16-bit dtype (any over mx8 rows), heads a multiple of
+    [tokens, heads, width] of the cache's 16-bit dtype (either over mx8 and mx4 rows), heads a multiple of
     the cache's. lse: float32 [tokens, heads] or None. workspace: a device tensor of
     workspace_bytes; calls that may run at the same time must not share one. A token that
     attends nothing gets zeros, one all of whose scores are -inf gets NaN (lse -inf for both)."""
@@ -382,7 +384,7 @@ def attend(cache: Cache, batch: Batch, q, out, *, scale: float, lse=None, worksp
 def attend_latent(cache: Cache, batch: Batch, q, q_pe, out, *, scale: float, lse=None, workspace=None,
                   stream=0) -> None:
     """Absorbed latent attention: q [tokens, heads, 512] and q_pe [tokens, heads, 64] over a
-    latent cache of width 576, out [tokens, heads, 512]; the rest as attend."""
+    latent cache of width 576 (not mx4), out [tokens, heads, 512]; the rest as attend."""
     if q_pe is None:
         raise ValueError("attend_latent: q_pe is missing")
     _attend("attend_latent", cache, batch, q, q_pe, out, lse, scale, workspace, stream)

@@ -294,11 +294,13 @@ HEARTH_API int hearth_gpu_device(char *name, size_t n);
  * masked, read as zeros and are not stored), lengths are cut to what the page table and the
  * buffers hold. */
 #define HEARTH_GPU_MX8 16   /* cache rows of e4m3 codes (OCP FP8, finite) with one E8M0 scale byte per 32 elements */
+#define HEARTH_GPU_MX4 17   /* cache rows of e2m1 codes (OCP FP4), two a byte, the even element in the low half, with scales alike */
 
 /* One tensor of a cache: rows [n_pages][n_heads][page][width], the last two dimensions
  * dense. Strides in elements; data and strides are multiples of 16 bytes. MX8: scales
  * [n_pages][n_heads][page][width / 32], the last two dimensions dense: element = code *
- * 2^(scale - 127), scale bytes 1 to 254 (those that hearth_gpu_kv_append writes). */
+ * 2^(scale - 127), scale bytes 1 to 254 (those that hearth_gpu_kv_append writes; 255 in MX4: a block
+ * of NaN). MX4: rows [..][width / 2] bytes, data and scale strides in bytes, scales as in MX8. */
 typedef struct hearth_gpu_rows {
     void *data;
     uint8_t *scales;
@@ -308,7 +310,7 @@ typedef struct hearth_gpu_rows {
 
 /* A cache: k and v of the same shape, or k alone (v.data NULL: latent rows, which hold a
  * token's latent vector and then its rotated part). page: a power of two from 16 to 4096;
- * width: a multiple of 32 up to 1024; dtype: HEARTH_F16, HEARTH_BF16 or HEARTH_GPU_MX8. */
+ * width: a multiple of 32 up to 1024; dtype: HEARTH_F16, HEARTH_BF16, HEARTH_GPU_MX8 or HEARTH_GPU_MX4. */
 typedef struct hearth_gpu_cache {
     hearth_gpu_rows k, v;
     int32_t dtype, n_pages, n_heads, page, width;
@@ -351,13 +353,15 @@ HEARTH_API int hearth_gpu_rope(const hearth_gpu_array *x, const hearth_gpu_array
                                const double *freqs, int n_freqs, int offset, int interleaved, int inverse,
                                double factor, int dev, void *stream);
 
-/* Writes the call's tokens' rows into the cache, converted (16-bit) or quantised (MX8). With
+/* Writes the call's tokens' rows into the cache, converted (16-bit) or quantised (MX8, MX4). With
  * k and v in the cache, the arrays have its heads and width; a latent cache takes the latent
  * as k and the rotated part as v (NULL: none), one head each, widths multiples of 32 that add
  * up to the cache's. MX8: a block's scale is the least power of two with max |x| / scale <=
  * 448 over the block's finite values (scale byte 1 at least), codes round to nearest even; a
  * NaN or infinity is stored as NaN; a value whose rounding would leave the range of x's type
- * is stored as the largest code within it. Tokens at negative positions (more tokens than
+ * is stored as the largest code within it. MX4 alike: max |x| / scale <= 7 (6, the largest code, and
+ * half the step above it: no element is off by more than half a step), and a block that holds a NaN or
+ * an infinity gets scale byte 255 and reads as NaN throughout. Tokens at negative positions (more tokens than
  * rows) and rows past the bounds are not stored; min(max_q, n_tokens) is at most 2^26 - 4 (more
  * where a token's rows, k and v together, have at most 1024 elements; reads alike); two sequences that share a page in which
  * they write the same row leave one or a mixture of the two. */
@@ -373,7 +377,7 @@ HEARTH_API int hearth_gpu_kv_read(const hearth_gpu_cache *c, const hearth_gpu_ba
  * HEARTH_F16 or HEARTH_BF16; H a multiple of the cache's heads, head h reads kv head
  * h / (H / n_heads); width 64, 128 or 256. out = softmax(scale * q . k) v over the rows a
  * token attends; a token that attends nothing gets zeros, one all of whose scores are -infinity
- * NaN (0 / 0). 16-bit caches have q's dtype; MX8
+ * NaN (0 / 0). 16-bit caches have q's dtype; MX8 and MX4
  * rows are taken as their values in q's dtype, in whose range they must lie. min(max_q,
  * n_tokens) * H up to 2^26; min(max_kv, pages_per_seq * page) below 2^30 - 65536. Scores, softmax statistics and sums are
  * float32; the probabilities are rounded to q's dtype for the product with v. lse: NULL or
@@ -387,7 +391,7 @@ HEARTH_API int hearth_gpu_attend(const hearth_gpu_cache *c, const hearth_gpu_bat
 /* The absorbed form of latent attention: q [n_tokens][H][C] (each head's query taken through
  * its key projection) and q_pe [n_tokens][H][R] (its rotated part) against the latent rows'
  * first C and last R elements, out [n_tokens][H][C] = softmax(scale * (q . c + q_pe . pe)) c.
- * C = 512, R = 64, cache width 576, one cache head; n_seqs times min(max_q, n_tokens) * H / 64,
+ * C = 512, R = 64, cache width 576, one cache head, not MX4; n_seqs times min(max_q, n_tokens) * H / 64,
  * rounded up, at most 8388592 (somewhat below 2^29 / 64); everything else as hearth_gpu_attend. Its
  * time depends on the scores: where a head's scores over a share of the rows exceed the largest of
  * that share's first 32 by more than 14 ln 2 = 9.7, the share is gone through three times (up to 2.7
