@@ -99,19 +99,20 @@ int no_device() {
     return E_IO;
 }
 
-int copy_call(bool write, const hearth_gpu_cache *c, const hearth_gpu_batch *b, const hearth_gpu_array *k,
-              const hearth_gpu_array *v, int dev, void *stream) {
+/* Checked arguments of a write or read; a.b.max_q 0: nothing to do. wide: every array's pieces of 8 lie on 16 bytes. */
+int copy_args(bool write, const hearth_gpu_cache *c, const hearth_gpu_batch *b, const hearth_gpu_array *k,
+              const hearth_gpu_array *v, int dev, CopyArgs &a, bool &wide) {
     if (!cache_ok(c) || !batch_ok(b) || dev < 0) return E_ARG;
     const bool latent = !c->v.data;
     const int n = b->n_tokens;
     if (v && !v->data && n) v = nullptr;
     if (!array_ok(k, n) || (v && !array_ok(v, n)) || (!latent && !v)) return E_ARG;
     if (v && v->dtype != k->dtype) return E_ARG;
-    CopyArgs a{};
+    a = {};
     a.b = batch_of(*b, *c);
     a.n_pieces = v ? 2 : 1;
     int col = 0;
-    bool wide = true;
+    wide = true;
     for (int i = 0; i < a.n_pieces; i++) {
         const hearth_gpu_array &x = i ? *v : *k;
         if (x.n_heads != c->n_heads || x.width % 32 || (!write && !apart(x, n))) return E_ARG;
@@ -126,7 +127,16 @@ int copy_call(bool write, const hearth_gpu_cache *c, const hearth_gpu_batch *b, 
         wide = wide && on16(x);
     }
     if (latent && (col != c->width || (v && c->n_heads != 1))) return E_ARG;
-    if (!a.b.n_seqs || !a.b.max_q) return OK;
+    if (!a.b.n_seqs) a.b.max_q = 0;
+    return OK;
+}
+
+int copy_call(bool write, const hearth_gpu_cache *c, const hearth_gpu_batch *b, const hearth_gpu_array *k,
+              const hearth_gpu_array *v, int dev, void *stream) {
+    CopyArgs a;
+    bool wide;
+    if (const int rc = copy_args(write, c, b, k, v, dev, a, wide)) return rc;
+    if (!a.b.max_q) return OK;
     if (copy_groups(a) > MAX_COPY_GROUPS) return E_ARG;
     if (hipPeekAtLastError() != hipSuccess) return E_IO;
     DeviceGuard g(dev);
@@ -235,6 +245,44 @@ HEARTH_API int hearth_gpu_rope(const hearth_gpu_array *x, const hearth_gpu_array
 HEARTH_API int hearth_gpu_kv_append(const hearth_gpu_cache *c, const hearth_gpu_batch *b, const hearth_gpu_array *k,
                                     const hearth_gpu_array *v, int dev, void *stream) {
     return copy_call(true, c, b, k, v, dev, stream);
+}
+
+HEARTH_API int hearth_gpu_kv_append_rotated(const hearth_gpu_cache *c, const hearth_gpu_batch *b, const hearth_gpu_array *q,
+                                            const hearth_gpu_array *q_out, const hearth_gpu_array *k, const hearth_gpu_array *v,
+                                            const void *pos, int pos64, const double *freqs, int n_freqs, int offset,
+                                            int interleaved, double factor, int dev, void *stream) {
+    RotatedArgs a{};
+    bool wide;
+    if (const int rc = copy_args(true, c, b, k, v, dev, a.c, wide)) return rc;
+    const int n = b->n_tokens;
+    if (q && !q->data && n) q = nullptr;
+    if (q_out && !q_out->data && n) q_out = nullptr;
+    const bool latent = !c->v.data;
+    if (!q != !q_out || (latent && a.c.n_pieces != 2) || !freqs) return E_ARG;
+    a.rotated = latent ? 1 : 0;
+    a.width = a.c.p[a.rotated].width;
+    if (n_freqs < 1 || n_freqs > 512 || offset < 0 || (int64_t)offset + 2 * n_freqs > a.width) return E_ARG;
+    if (!std::isfinite(factor) || (uintptr_t)pos % (pos64 ? 8 : 4) || (uintptr_t)freqs % 8) return E_ARG;
+    if (q) {
+        if (!array_ok(q, n) || !array_ok(q_out, n) || q->dtype != k->dtype || q_out->dtype != q->dtype || q->width != a.width ||
+            q_out->width != a.width || q_out->n_heads != q->n_heads || !apart(*q_out, n)) return E_ARG;
+        if ((int64_t)q->n_heads * q->width > MAX_ROPE_ROW) return E_ARG;
+        a.in_place = q->data == q_out->data;
+        if (a.in_place && (q->token_stride != q_out->token_stride || q->head_stride != q_out->head_stride)) return E_ARG;
+        if (n && (q_out->data == k->data || (v && q_out->data == v->data))) return E_ARG;   /* read by some threads, written by others */
+        const int64_t es = elem(q->dtype);
+        a.q = {(const uint8_t *)q->data, (uint8_t *)q_out->data, q->token_stride * es, q->head_stride * es,
+               q_out->token_stride * es, q_out->head_stride * es, q->n_heads};
+    }
+    if ((int64_t)c->n_heads * c->width > MAX_ROPE_ROW / 2 || a.c.b.max_q > MAX_COPY_GROUPS) return E_ARG;
+    a.pos = pos; a.pos64 = pos64 != 0; a.freqs = freqs; a.n_freqs = n_freqs; a.offset = offset;
+    a.interleaved = interleaved != 0; a.factor = (float)factor;
+    if (!a.c.b.max_q) return OK;
+    if (hipPeekAtLastError() != hipSuccess) return E_IO;
+    DeviceGuard g(dev);
+    if (!g.ok) return no_device();
+    kv_append_rotated(a, k->dtype, c->dtype, wide, (hipStream_t)stream);
+    return finish();
 }
 
 HEARTH_API int hearth_gpu_kv_read(const hearth_gpu_cache *c, const hearth_gpu_batch *b, const hearth_gpu_array *k,

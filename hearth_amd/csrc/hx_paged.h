@@ -71,6 +71,18 @@ struct CopyArgs {
     int n_pieces, octs;       /* groups of 8 elements of a token over all pieces and heads */
 };
 
+/* ---- writes of rotated rows ---- */
+struct RotatedArgs {
+    CopyArgs c;
+    RopeArgs::Pair q;         /* heads 0: none */
+    const void *pos;          /* NULL: a token's row in its sequence */
+    const double *freqs;
+    int rotated;              /* which piece is: the keys, or a latent row's second part */
+    int width, n_freqs, offset, pos64, interleaved;
+    float factor;
+    bool in_place;
+};
+
 /* ---- attention ---- */
 struct AttendArgs {
     Batch b;
@@ -100,6 +112,7 @@ struct DeviceGuard {
 void rope(const RopeArgs &a, int dtype, hipStream_t st);
 int64_t copy_groups(const CopyArgs &a);   /* workgroups of a sequence's tokens */
 void kv_append(const CopyArgs &a, int src_dtype, int cache_dtype, bool aligned, hipStream_t st);
+void kv_append_rotated(const RotatedArgs &a, int src_dtype, int cache_dtype, bool aligned, hipStream_t st);
 void kv_read(const CopyArgs &a, int dst_dtype, int cache_dtype, bool aligned, hipStream_t st);
 
 /* Split of the rows axis: rows per split and splits of the longest sequence, and whether the

@@ -40,6 +40,7 @@ template <> struct Elem<DT_F32> {
     }
     static __device__ __forceinline__ float load(const uint8_t *p) { return *(const float *)p; }
     static __device__ __forceinline__ void store(uint8_t *p, float v) { *(float *)p = v; }
+    template <bool> static __device__ __forceinline__ float rounded(float v) { return v; }
 };
 template <class T> struct Elem16 {
     static constexpr int size = 2;
@@ -64,6 +65,12 @@ template <class T> struct Elem16 {
     }
     static __device__ __forceinline__ float load(const uint8_t *p) { return (float)*(const e *)p; }
     static __device__ __forceinline__ void store(uint8_t *p, float v) { *(e *)p = (e)v; }
+    /* to float32 and then to e, as the pairs of store8 are; ALONE: as store, where the compiler may round a
+     * float16's product and sum once */
+    template <bool ALONE> static __device__ __forceinline__ float rounded(float v) {
+        if constexpr (!ALONE) asm("" : "+v"(v));
+        return (float)(e)v;
+    }
 };
 template <> struct Elem<DT_F16> : Elem16<F16> {};
 template <> struct Elem<DT_BF16> : Elem16<Bf16> {};
@@ -79,78 +86,86 @@ template <> struct Elem<DT_BF16> : Elem16<Bf16> {};
 constexpr int ROPE_THREADS = 256;
 constexpr int ROPE_GROUPS = 1 << 20;   /* at most; longer calls go round */
 
+/* cosine and sine of pos * freq, times factor */
+__device__ __forceinline__ f2 turn_of(double pos, double freq, float factor, float sign) {
+    const double turns = pos * (freq * 0.15915494309189533577);
+    const float r = 2.0f * (float)(turns - rint(turns));
+    float s, c;
+    sincospif(r, &s, &c);
+    return (f2){c * factor, s * factor * sign};
+}
+
+/* nt tokens from t0 on of one tensor, their cosines and sines in cs */
+template <int DT, bool HALF, bool WIDE>
+__device__ __forceinline__ void rope_rows(const RopeArgs::Pair &p, int64_t t0, int nt, const f2 *cs, int n_freqs, int offset, int width, bool in_place) {
+    using E = Elem<DT>;
+    constexpr int S = E::size;
+    /* an item is 8 elements of each half (HALF), 16 consecutive ones (interleaved), or, WIDE
+     * false, one pair; then the elements outside the rotated part, one at a time */
+    constexpr int PER = WIDE ? 8 : 1;
+    const int items = n_freqs / PER;
+    const int per_tok = p.heads * items;
+    for (int i = threadIdx.x; i < nt * per_tok; i += ROPE_THREADS) {
+        const int tl = i / per_tok, rem = i % per_tok, h = rem / items, j = rem % items * PER;
+        const uint8_t *x = p.x + (t0 + tl) * p.xt + (int64_t)h * p.xh + offset * S;
+        uint8_t *y = p.y + (t0 + tl) * p.yt + (int64_t)h * p.yh + offset * S;
+        const f2 *w = cs + tl * n_freqs + j;
+        if constexpr (WIDE) {
+            const int o0 = HALF ? j * S : 2 * j * S, o1 = HALF ? (j + n_freqs) * S : (2 * j + 8) * S;
+            float u[8], v[8], ru[8], rv[8];
+            E::load8(x + o0, true, u);
+            E::load8(x + o1, true, v);
+            if constexpr (HALF) {
+#pragma unroll
+                for (int i8 = 0; i8 < 8; i8++) {
+                    ru[i8] = __builtin_fmaf(u[i8], w[i8][0], -(v[i8] * w[i8][1]));
+                    rv[i8] = __builtin_fmaf(v[i8], w[i8][0], u[i8] * w[i8][1]);
+                }
+            } else {
+#pragma unroll
+                for (int i4 = 0; i4 < 4; i4++) {
+                    ru[2 * i4] = __builtin_fmaf(u[2 * i4], w[i4][0], -(u[2 * i4 + 1] * w[i4][1]));
+                    ru[2 * i4 + 1] = __builtin_fmaf(u[2 * i4 + 1], w[i4][0], u[2 * i4] * w[i4][1]);
+                    rv[2 * i4] = __builtin_fmaf(v[2 * i4], w[4 + i4][0], -(v[2 * i4 + 1] * w[4 + i4][1]));
+                    rv[2 * i4 + 1] = __builtin_fmaf(v[2 * i4 + 1], w[4 + i4][0], v[2 * i4] * w[4 + i4][1]);
+                }
+            }
+            E::store8(y + o0, true, ru);
+            E::store8(y + o1, true, rv);
+        } else {
+            const int o0 = HALF ? j * S : 2 * j * S, o1 = HALF ? (j + n_freqs) * S : (2 * j + 1) * S;
+            const float u = E::load(x + o0), v = E::load(x + o1);
+            E::store(y + o0, __builtin_fmaf(u, w[0][0], -(v * w[0][1])));
+            E::store(y + o1, __builtin_fmaf(v, w[0][0], u * w[0][1]));
+        }
+    }
+    if (!in_place) {
+        const int rest = width - 2 * n_freqs;
+        for (int i = threadIdx.x; i < nt * p.heads * rest; i += ROPE_THREADS) {
+            const int tl = i / (p.heads * rest), rem = i % (p.heads * rest), h = rem / rest;
+            int d = rem % rest;
+            if (d >= offset) d += 2 * n_freqs;
+            const uint8_t *x = p.x + (t0 + tl) * p.xt + (int64_t)h * p.xh + (int64_t)d * S;
+            uint8_t *y = p.y + (t0 + tl) * p.yt + (int64_t)h * p.yh + (int64_t)d * S;
+            if constexpr (S == 4) *(unsigned *)y = *(const unsigned *)x;
+            else *(unsigned short *)y = *(const unsigned short *)x;
+        }
+    }
+}
+
 template <int DT, bool HALF, bool WIDE>
 __global__ __launch_bounds__(ROPE_THREADS) void k_rope(RopeArgs a, int tok) {
     extern __shared__ f2 cs[];   /* [tok][n_freqs] */
-    using E = Elem<DT>;
-    constexpr int S = E::size;
     for (int64_t t0 = (int64_t)blockIdx.x * tok; t0 < a.n_tokens; t0 += (int64_t)gridDim.x * tok) {
         const int nt = (int)min((int64_t)tok, a.n_tokens - t0);
         for (int i = threadIdx.x; i < nt * a.n_freqs; i += ROPE_THREADS) {
             const int64_t t = t0 + i / a.n_freqs;
-            const int j = i % a.n_freqs;
             const double pos = a.pos64 ? (double)((const int64_t *)a.pos)[t] : (double)((const int *)a.pos)[t];
-            const double turns = pos * (a.freqs[j] * 0.15915494309189533577);
-            const float r = 2.0f * (float)(turns - rint(turns));
-            float s, c;
-            sincospif(r, &s, &c);
-            cs[i] = (f2){c * a.factor, s * a.factor * a.sign};
+            cs[i] = turn_of(pos, a.freqs[i % a.n_freqs], a.factor, a.sign);
         }
         __syncthreads();
-        /* an item is 8 elements of each half (HALF), 16 consecutive ones (interleaved), or, WIDE
-         * false, one pair; then the elements outside the rotated part, one at a time */
-        constexpr int PER = WIDE ? 8 : 1;
-        const int items = a.n_freqs / PER;
-        for (int z = 0; z < a.n_pairs; z++) {
-            const auto &p = a.p[z];
-            const int per_tok = p.heads * items;
-            for (int i = threadIdx.x; i < nt * per_tok; i += ROPE_THREADS) {
-                const int tl = i / per_tok, rem = i % per_tok, h = rem / items, j = rem % items * PER;
-                const uint8_t *x = p.x + (t0 + tl) * p.xt + (int64_t)h * p.xh + a.offset * S;
-                uint8_t *y = p.y + (t0 + tl) * p.yt + (int64_t)h * p.yh + a.offset * S;
-                const f2 *w = cs + tl * a.n_freqs + j;
-                if constexpr (WIDE) {
-                    const int o0 = HALF ? j * S : 2 * j * S, o1 = HALF ? (j + a.n_freqs) * S : (2 * j + 8) * S;
-                    float u[8], v[8], ru[8], rv[8];
-                    E::load8(x + o0, true, u);
-                    E::load8(x + o1, true, v);
-                    if constexpr (HALF) {
-#pragma unroll
-                        for (int i8 = 0; i8 < 8; i8++) {
-                            ru[i8] = __builtin_fmaf(u[i8], w[i8][0], -(v[i8] * w[i8][1]));
-                            rv[i8] = __builtin_fmaf(v[i8], w[i8][0], u[i8] * w[i8][1]);
-                        }
-                    } else {
-#pragma unroll
-                        for (int i4 = 0; i4 < 4; i4++) {
-                            ru[2 * i4] = __builtin_fmaf(u[2 * i4], w[i4][0], -(u[2 * i4 + 1] * w[i4][1]));
-                            ru[2 * i4 + 1] = __builtin_fmaf(u[2 * i4 + 1], w[i4][0], u[2 * i4] * w[i4][1]);
-                            rv[2 * i4] = __builtin_fmaf(v[2 * i4], w[4 + i4][0], -(v[2 * i4 + 1] * w[4 + i4][1]));
-                            rv[2 * i4 + 1] = __builtin_fmaf(v[2 * i4 + 1], w[4 + i4][0], v[2 * i4] * w[4 + i4][1]);
-                        }
-                    }
-                    E::store8(y + o0, true, ru);
-                    E::store8(y + o1, true, rv);
-                } else {
-                    const int o0 = HALF ? j * S : 2 * j * S, o1 = HALF ? (j + a.n_freqs) * S : (2 * j + 1) * S;
-                    const float u = E::load(x + o0), v = E::load(x + o1);
-                    E::store(y + o0, __builtin_fmaf(u, w[0][0], -(v * w[0][1])));
-                    E::store(y + o1, __builtin_fmaf(v, w[0][0], u * w[0][1]));
-                }
-            }
-            if (!a.in_place) {
-                const int rest = a.width - 2 * a.n_freqs;
-                for (int i = threadIdx.x; i < nt * p.heads * rest; i += ROPE_THREADS) {
-                    const int tl = i / (p.heads * rest), rem = i % (p.heads * rest), h = rem / rest;
-                    int d = rem % rest;
-                    if (d >= a.offset) d += 2 * a.n_freqs;
-                    const uint8_t *x = p.x + (t0 + tl) * p.xt + (int64_t)h * p.xh + (int64_t)d * S;
-                    uint8_t *y = p.y + (t0 + tl) * p.yt + (int64_t)h * p.yh + (int64_t)d * S;
-                    if constexpr (S == 4) *(unsigned *)y = *(const unsigned *)x;
-                    else *(unsigned short *)y = *(const unsigned short *)x;
-                }
-            }
-        }
+        for (int z = 0; z < a.n_pairs; z++)
+            rope_rows<DT, HALF, WIDE>(a.p[z], t0, nt, cs, a.n_freqs, a.offset, a.width, a.in_place);
         __syncthreads();   /* the next tokens' cosines go where these lie */
     }
 }
@@ -198,33 +213,26 @@ __device__ __forceinline__ Place place_of(const CopyArgs &a) {
     return r;
 }
 
-/* lanes of one block of 32 come here together: octs and every piece's width / 8 are multiples of 4 */
-template <int SRC, int DST, bool WIDE>
-__device__ __forceinline__ void append_item(const CopyArgs &a, const Seq &q, const Piece &p, int tok, int h, int d) {
-    using E = Elem<SRC>;
+/* where a token's row lies: its head's rows of a page and the row's number in it; page < 0: nowhere */
+struct Spot { int page, row; };
+__device__ __forceinline__ Spot spot_of(const Batch &b, const Seq &q, int tok) {
     const int pos = q.base + tok;
-    if (pos < 0 || pos >= q.kv) return;
-    const int page = a.b.pages[(int64_t)blockIdx.y * a.b.ld_pages + (pos >> a.b.page_shift)];
-    if (!page_ok(a.b, page)) return;
-    const int row = pos & ((1 << a.b.page_shift) - 1);
-    const uint8_t *src = p.arr + (int64_t)(q.q0 + tok) * p.at + (int64_t)h * p.ah + (int64_t)d * E::size;
-    uint8_t *dst = p.rows.data + (int64_t)page * p.rows.page_stride + (int64_t)h * p.rows.head_stride;
-    const int64_t el = (int64_t)row * p.row_width + p.col + d;
-    if constexpr (DST == SRC) {
-        if (WIDE) *(u4 *)(dst + el * 2) = *(const u4 *)src;
-        else {
-            unsigned short w[8];
-#pragma unroll
-            for (int j = 0; j < 8; j++) w[j] = ((const unsigned short *)src)[j];
-            *(u4 *)(dst + el * 2) = (u4){w[0] | (unsigned)w[1] << 16, w[2] | (unsigned)w[3] << 16,
-                                         w[4] | (unsigned)w[5] << 16, w[6] | (unsigned)w[7] << 16};
-        }
+    if (pos < 0 || pos >= q.kv) return {-1, 0};
+    const int page = b.pages[(int64_t)blockIdx.y * b.ld_pages + (pos >> b.page_shift)];
+    return {page_ok(b, page) ? page : -1, pos & ((1 << b.page_shift) - 1)};
+}
+
+/* Eight values, which SRC holds, into a row of the cache. Lanes of one block of 32 come here together:
+ * octs and every piece's width / 8 are multiples of 4. */
+template <int SRC, int DST>
+__device__ __forceinline__ void put8(const Piece &p, const Spot &at, int h, int d, const float (&v)[8]) {
+    uint8_t *dst = p.rows.data + (int64_t)at.page * p.rows.page_stride + (int64_t)h * p.rows.head_stride;
+    const int64_t el = (int64_t)at.row * p.row_width + p.col + d;
+    if constexpr (bits_of(DST) == 16) {
+        Elem<DST>::store8(dst + el * 2, true, v);
     } else {
-        float v[8];
-        E::load8(src, WIDE, v);
-        if constexpr (bits_of(DST) == 16) {
-            Elem<DST>::store8(dst + el * 2, true, v);
-        } else if constexpr (DST == DT_MX4) {
+        int byte;
+        if constexpr (DST == DT_MX4) {
             float m = 0.0f;
 #pragma unroll
             for (int j = 0; j < 8; j++) m = fmaxf(m, fin(v[j]) ? __builtin_fabsf(v[j]) : __builtin_huge_valf());
@@ -232,7 +240,7 @@ __device__ __forceinline__ void append_item(const CopyArgs &a, const Seq &q, con
             /* least exponent with m <= 7 * 2^e = 1.75 * 2^(e + 2); 255 (a block of NaN) where m is infinite */
             const int bits = (int)__float_as_uint(m);
             const bool whole = fin(m);
-            const int byte = whole ? max((bits >> 23) - 2 + ((bits & 0x7fffff) > 0x600000), 1) : 255;
+            byte = whole ? max((bits >> 23) - 2 + ((bits & 0x7fffff) > 0x600000), 1) : 255;
             const float scale = mx_scale(whole ? byte : 127);
             /* 4 would leave the source type's range: 3, within half a step */
             const float top = (SRC == DT_F16 ? byte == 127 + 14 : byte == 127 + 126) ? 3.0f * scale : __builtin_huge_valf();
@@ -242,15 +250,13 @@ __device__ __forceinline__ void append_item(const CopyArgs &a, const Seq &q, con
                 c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, a, b, scale, j);   /* rounds to nearest even, above 6 to 6 */
             });
             *(unsigned *)(dst + el / 2) = c;
-            if ((d & 31) == 0)
-                p.rows.scales[(int64_t)page * p.rows.scale_page_stride + (int64_t)h * p.rows.scale_head_stride + el / MX_BLOCK] = (uint8_t)byte;
         } else {
             float m = 0.0f;
 #pragma unroll
             for (int j = 0; j < 8; j++) m = fmaxf(m, fin(v[j]) ? __builtin_fabsf(v[j]) : 0.0f);
             m = max_of4(m);
             const int bits = (int)__float_as_uint(m);
-            const int byte = max((bits >> 23) - 8 + ((bits & 0x7fffff) > 0x600000), 1);   /* e + 127 */
+            byte = max((bits >> 23) - 8 + ((bits & 0x7fffff) > 0x600000), 1);   /* e + 127 */
             const float inv = __uint_as_float((unsigned)(254 - byte) << 23);
             const float top = (SRC == DT_F16 ? byte == 127 + 8 : byte == 127 + 120) ? 240.0f : 448.0f;
             unsigned c[2] = {0, 0};
@@ -263,10 +269,32 @@ __device__ __forceinline__ void append_item(const CopyArgs &a, const Seq &q, con
                 c[j >> 2] |= code << (8 * (j & 3));
             }
             *(u2 *)(dst + el) = (u2){c[0], c[1]};
-            if ((d & 31) == 0)
-                p.rows.scales[(int64_t)page * p.rows.scale_page_stride + (int64_t)h * p.rows.scale_head_stride +
-                              el / MX_BLOCK] = (uint8_t)byte;
         }
+        if ((d & 31) == 0)
+            p.rows.scales[(int64_t)at.page * p.rows.scale_page_stride + (int64_t)h * p.rows.scale_head_stride + el / MX_BLOCK] = (uint8_t)byte;
+    }
+}
+
+template <int SRC, int DST, bool WIDE>
+__device__ __forceinline__ void append_item(const CopyArgs &a, const Seq &q, const Piece &p, int tok, int h, int d) {
+    using E = Elem<SRC>;
+    const Spot at = spot_of(a.b, q, tok);
+    if (at.page < 0) return;
+    const uint8_t *src = p.arr + (int64_t)(q.q0 + tok) * p.at + (int64_t)h * p.ah + (int64_t)d * E::size;
+    if constexpr (DST == SRC) {
+        uint8_t *dst = p.rows.data + (int64_t)at.page * p.rows.page_stride + (int64_t)h * p.rows.head_stride + ((int64_t)at.row * p.row_width + p.col + d) * 2;
+        if (WIDE) *(u4 *)dst = *(const u4 *)src;
+        else {
+            unsigned short w[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) w[j] = ((const unsigned short *)src)[j];
+            *(u4 *)dst = (u4){w[0] | (unsigned)w[1] << 16, w[2] | (unsigned)w[3] << 16,
+                              w[4] | (unsigned)w[5] << 16, w[6] | (unsigned)w[7] << 16};
+        }
+    } else {
+        float v[8];
+        E::load8(src, WIDE, v);
+        put8<SRC, DST>(p, at, h, d, v);
     }
 }
 
@@ -280,6 +308,91 @@ __global__ __launch_bounds__(256) void k_kv_append(CopyArgs a) {
     for (int i = 0; i < COPY_TOKENS; i++) {
         const int tok = r.tok + i * r.step;
         if (tok < n) append_item<SRC, DST, WIDE>(a, q, *r.p, tok, r.h, r.d);
+    }
+}
+
+/* ---------------------------------------------------------------- writes of rotated rows
+ *
+ * Rope and append in one pass: the queries as k_rope takes them, the keys on their way into the pages,
+ * which saves a launch and the keys' way to memory and back. A rotated key is rounded to its array's
+ * type before it is stored, so that the cache holds the bits that the two calls, one after the other,
+ * leave there. A key's thread takes eight elements of the row that it writes and reads the eight that
+ * they are turned against as well (the second read of a line that its neighbour brings in). */
+template <int SRC, bool HALF, bool EIGHTS>
+__device__ __forceinline__ void rotated8(const uint8_t *row, int d, const f2 *cs, int n_freqs, int offset, float (&v)[8]) {
+    using E = Elem<SRC>;
+    constexpr int S = E::size;
+    if constexpr (EIGHTS) {   /* all within the rotated part's one half, or all outside of it; on 16 bytes */
+        E::load8(row + d * S, true, v);
+        const int j = d - offset;
+        if (j < 0 || j >= 2 * n_freqs) return;
+        if constexpr (HALF) {
+            const bool second = j >= n_freqs;
+            const f2 *w = cs + (second ? j - n_freqs : j);
+            float x[8];
+            E::load8(row + (second ? d - n_freqs : d + n_freqs) * S, true, x);
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const float t = x[i] * w[i][1];
+                v[i] = E::template rounded<false>(__builtin_fmaf(v[i], w[i][0], second ? t : -t));
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const f2 w = cs[j / 2 + i];
+                const float x = v[2 * i], y = v[2 * i + 1];
+                v[2 * i] = E::template rounded<false>(__builtin_fmaf(x, w[0], -(y * w[1])));
+                v[2 * i + 1] = E::template rounded<false>(__builtin_fmaf(y, w[0], x * w[1]));
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const int j = d + i - offset;
+            v[i] = E::load(row + (d + i) * S);
+            if (j < 0 || j >= 2 * n_freqs) continue;
+            const bool second = HALF ? j >= n_freqs : j & 1;
+            const f2 w = cs[HALF ? (second ? j - n_freqs : j) : j / 2];
+            const int o = HALF ? n_freqs : 1;
+            const float t = E::load(row + (second ? d + i - o : d + i + o) * S) * w[1];
+            v[i] = E::template rounded<true>(__builtin_fmaf(v[i], w[0], second ? t : -t));
+        }
+    }
+}
+
+template <int SRC, int DST, bool HALF, bool WIDE>
+__global__ __launch_bounds__(ROPE_THREADS) void k_kv_append_rotated(RotatedArgs a, int tok) {
+    extern __shared__ f2 cs[];   /* [tok][n_freqs] */
+    const Seq q = seq_of(a.c.b, blockIdx.y);
+    const int n = min(q.n, a.c.b.max_q);
+    const int64_t first = (int64_t)blockIdx.x * tok;
+    if (first >= n) return;
+    const int t0 = (int)first, nt = min(tok, n - t0);
+    for (int i = threadIdx.x; i < nt * a.n_freqs; i += ROPE_THREADS) {
+        const int t = t0 + i / a.n_freqs;
+        const int64_t at = q.q0 + t;
+        const double pos = !a.pos ? (double)(q.base + t) : a.pos64 ? (double)((const int64_t *)a.pos)[at] : (double)((const int *)a.pos)[at];
+        cs[i] = turn_of(pos, a.freqs[i % a.n_freqs], a.factor, 1.0f);
+    }
+    __syncthreads();
+    if (a.q.heads) rope_rows<SRC, HALF, WIDE>(a.q, q.q0 + t0, nt, cs, a.n_freqs, a.offset, a.width, a.in_place);
+    const int o0 = a.c.p[0].heads * (a.c.p[0].width / 8);
+    for (int i = threadIdx.x; i < nt * a.c.octs; i += ROPE_THREADS) {
+        const int tl = i / a.c.octs;
+        int o = i % a.c.octs;
+        const int z = o >= o0 ? 1 : 0;
+        if (z) o -= o0;
+        const Piece &p = a.c.p[z];
+        const int h = o / (p.width / 8), d = o % (p.width / 8) * 8;
+        if (z != a.rotated) {
+            append_item<SRC, DST, WIDE>(a.c, q, p, t0 + tl, h, d);
+            continue;
+        }
+        const Spot at = spot_of(a.c.b, q, t0 + tl);
+        if (at.page < 0) continue;
+        float v[8];
+        rotated8<SRC, HALF, WIDE>(p.arr + (int64_t)(q.q0 + t0 + tl) * p.at + (int64_t)h * p.ah, d, cs + tl * a.n_freqs, a.n_freqs, a.offset, v);
+        put8<SRC, DST>(p, at, h, d, v);
     }
 }
 
@@ -397,6 +510,26 @@ void kv_append(const CopyArgs &a, int src_dtype, int cache_dtype, bool aligned, 
     by_types(src_dtype, cache_dtype, [&](auto s, auto c) {
         if (aligned) hipLaunchKernelGGL((k_kv_append<s.value, c.value, true>), grid, block, 0, st, a);
         else hipLaunchKernelGGL((k_kv_append<s.value, c.value, false>), grid, block, 0, st, a);
+    });
+}
+
+/* Tokens a workgroup takes where it does not fill it: as in rope. wide: q's and the keys' pieces of 8
+ * start on 16 bytes, and none crosses a border of the rotated part. */
+void kv_append_rotated(const RotatedArgs &a, int src_dtype, int cache_dtype, bool aligned, hipStream_t st) {
+    bool wide = aligned && a.n_freqs % 8 == 0 && a.offset % 8 == 0;
+    if (a.q.heads) wide = wide && (((uintptr_t)a.q.x | (uintptr_t)a.q.y | (uint64_t)a.q.xt | (uint64_t)a.q.xh | (uint64_t)a.q.yt | (uint64_t)a.q.yh) & 15) == 0;
+    const int64_t items = (int64_t)a.q.heads * (a.n_freqs / (wide ? 8 : 1)) + a.c.octs;
+    const int tok = a.c.b.max_q >= 1024 && items < ROPE_THREADS ? 4 : 1;
+    const dim3 grid((unsigned)((a.c.b.max_q - 1) / tok + 1), a.c.b.n_seqs), block(ROPE_THREADS);
+    const size_t lds = sizeof(f2) * (size_t)tok * a.n_freqs;
+    by_types(src_dtype, cache_dtype, [&](auto s, auto c) {
+        if (a.interleaved) {
+            if (wide) hipLaunchKernelGGL((k_kv_append_rotated<s.value, c.value, false, true>), grid, block, lds, st, a, tok);
+            else hipLaunchKernelGGL((k_kv_append_rotated<s.value, c.value, false, false>), grid, block, lds, st, a, tok);
+        } else {
+            if (wide) hipLaunchKernelGGL((k_kv_append_rotated<s.value, c.value, true, true>), grid, block, lds, st, a, tok);
+            else hipLaunchKernelGGL((k_kv_append_rotated<s.value, c.value, true, false>), grid, block, lds, st, a, tok);
+        }
     });
 }
 

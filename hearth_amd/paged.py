@@ -4,6 +4,7 @@ For programs that keep many conversations' rows in pages next to (or without) an
 
     rope(x, pos, freqs)              rotary positions, in place or into `out`
     append(cache, batch, k, v)       new tokens' rows into the pages, 16-bit, 8-bit ("mx8") or 4-bit ("mx4")
+    append_rotated(cache, batch, q, k, v, freqs)   rope of q and k and append in one launch
     read(cache, batch, k, v)         rows back out of the pages
     attend(cache, batch, q, out)     grouped-head attention: tokens, chains, draft trees, prompts
     attend_latent(...)               absorbed latent attention over one row a token
@@ -30,7 +31,7 @@ import numpy as np
 from . import _native
 from .engine import HearthError
 
-__all__ = ["Cache", "Batch", "rope", "rope_frequencies", "append", "read", "attend", "attend_latent",
+__all__ = ["Cache", "Batch", "rope", "rope_frequencies", "append", "append_rotated", "read", "attend", "attend_latent",
            "workspace_bytes"]
 
 F32, F16, BF16, MX8, MX4 = 0, 1, 2, 16, 17
@@ -63,6 +64,9 @@ _PROTOS = {
                                 c_int, c_void_p, c_int, c_int, c_int, c_int, c_double, c_int, c_void_p]),
     "hearth_gpu_kv_append": (c_int, [POINTER(_CacheS), POINTER(_BatchS), POINTER(_Array), POINTER(_Array), c_int,
                                      c_void_p]),
+    "hearth_gpu_kv_append_rotated": (c_int, [POINTER(_CacheS), POINTER(_BatchS), POINTER(_Array), POINTER(_Array), POINTER(_Array),
+                                             POINTER(_Array), c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_double, c_int,
+                                             c_void_p]),
     "hearth_gpu_kv_read": (c_int, [POINTER(_CacheS), POINTER(_BatchS), POINTER(_Array), POINTER(_Array), c_int,
                                    c_void_p]),
     "hearth_gpu_attend": (c_int, [POINTER(_CacheS), POINTER(_BatchS), POINTER(_Array), POINTER(_Array), c_void_p,
@@ -310,6 +314,52 @@ def append(cache: Cache, batch: Batch, k, v=None, *, stream=0) -> None:
     rc = _fn("hearth_gpu_kv_append")(cache._ref, bs, byref(a), byref(b) if b is not None else None, cache.device, stream)
     if rc:
         _check(rc, "append")
+
+
+def append_rotated(cache: Cache, batch: Batch, q, k, v, freqs, *, pos=None, factor=1.0, layout="half", offset=0, q_out=None,
+                   stream=0) -> None:
+    """rope of q and k and append of the rotated keys and of v in one launch, to the same bits: q
+    [tokens, heads, width] in place or into q_out (None: keys alone), k on its way into the cache (the
+    tensor stays as it is). A latent cache takes the latents as k and rotates v, their second part,
+    whose width q has. pos [tokens] (int32 or int64), None: each token's row number in its sequence.
+    freqs, factor, layout, offset: as in rope; q_out is q or shares nothing with q, k and v."""
+    if layout not in ("half", "interleaved"):
+        raise ValueError(f"layout {layout!r} is neither 'half' nor 'interleaved'")
+    a, b, bs = _pair(cache, batch, k, v, "append_rotated")
+    dev, latent, tokens = cache.device, cache.v is None, k.shape[0]
+    if latent and b is None:
+        raise ValueError("append_rotated: v, the latent rows' rotated part, is missing")
+    width = b.width if latent else a.width
+    aq = ao = None
+    if q is not None:
+        ao = aq = _array(q, "q", dev)
+        if q.shape[0] != tokens or aq.width != width or aq.dtype != a.dtype:
+            raise ValueError(f"append_rotated: q is {q.dtype}{tuple(q.shape)}, the rotated rows {k.dtype} of width {width}")
+        if q_out is not None and q_out is not q:
+            ao = _array(q_out, "q_out", dev)
+            if q_out.shape[0] != tokens or ao.n_heads != aq.n_heads or ao.width != width or ao.dtype != aq.dtype:
+                raise ValueError(f"q_out is {q_out.dtype}{tuple(q_out.shape)}, q {q.dtype}{tuple(q.shape)}")
+        if tokens and (ao.data == a.data or (b is not None and ao.data == b.data)):
+            raise ValueError("q_out shares the elements of k or v")
+    elif q_out is not None:
+        raise ValueError("q_out without q")
+    f = _ints(freqs, "freqs", dev, 1, ("torch.float64", "float64"))
+    if getattr(freqs, "requires_grad", False):
+        _refuse_gradient("freqs")
+    n = freqs.shape[0]
+    if not 1 <= n <= 512 or offset < 0 or offset + 2 * n > width:
+        raise ValueError(f"{n} pairs at {offset} do not fit a width of {width}")
+    p, p64 = None, False
+    if pos is not None:
+        p = _ints(pos, "pos", dev, 1, ("torch.int32", "torch.int64", "int32 or int64"))
+        p64 = _seen_ints[pos.dtype] == "torch.int64"
+        if pos.shape[0] != tokens:
+            raise ValueError(f"{pos.shape[0]} positions for {tokens} tokens")
+    rc = _fn("hearth_gpu_kv_append_rotated")(cache._ref, bs, byref(aq) if aq is not None else None, byref(ao) if ao is not None else None,
+                                             byref(a), byref(b) if b is not None else None, p, p64, f, n, offset,
+                                             layout == "interleaved", float(factor), dev, stream)
+    if rc:
+        _check(rc, "append_rotated")
 
 
 def read(cache: Cache, batch: Batch, k, v=None, *, stream=0) -> None:

@@ -368,6 +368,19 @@ HEARTH_API int hearth_gpu_rope(const hearth_gpu_array *x, const hearth_gpu_array
 HEARTH_API int hearth_gpu_kv_append(const hearth_gpu_cache *c, const hearth_gpu_batch *b, const hearth_gpu_array *k,
                                     const hearth_gpu_array *v, int dev, void *stream);
 
+/* hearth_gpu_rope of queries and keys and hearth_gpu_kv_append of the rotated keys and the values in one
+ * launch, to the same bits (float16 arrays off 16 bytes or rotated parts off 8 elements: to one rounding):
+ * q [n_tokens][H][width] rotated into q_out (q itself, or an array that shares no element with q, k and v;
+ * both NULL: none), k rotated on its way into the cache (its array is left as it is), v as it is. A latent cache takes the latent as k and rotates v, its second part, whose width q has.
+ * pos: a position for each of the n_tokens tokens (int32, or int64 when pos64 is 1), NULL: a token's row
+ * number in its sequence, q_start and kv_len telling. freqs, n_freqs, offset, interleaved, factor: as in
+ * hearth_gpu_rope. All arrays have one dtype; n_heads * width of the cache up to 2^23, min(max_q, n_tokens)
+ * up to 2^24 - 1. Queries of tokens whose rows are not stored are rotated all the same. */
+HEARTH_API int hearth_gpu_kv_append_rotated(const hearth_gpu_cache *c, const hearth_gpu_batch *b, const hearth_gpu_array *q,
+                                            const hearth_gpu_array *q_out, const hearth_gpu_array *k, const hearth_gpu_array *v,
+                                            const void *pos, int pos64, const double *freqs, int n_freqs, int offset,
+                                            int interleaved, double factor, int dev, void *stream);
+
 /* The inverse: the call's tokens' rows read back into the arrays (q_start = running sum of
  * kv_len reads whole sequences). Rows that are not in the cache read as zeros. */
 HEARTH_API int hearth_gpu_kv_read(const hearth_gpu_cache *c, const hearth_gpu_batch *b, const hearth_gpu_array *k,
