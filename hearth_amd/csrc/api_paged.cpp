@@ -21,6 +21,7 @@ constexpr int64_t MAX_STRIDE = (int64_t)1 << 46;   /* elements: past any memory,
 constexpr int MAX_ROWS = 0x3fff0000;                /* rows of a sequence that an attention takes: split ends stay within 31 bits */
 constexpr int64_t MAX_LATENT_TILES = 0x7ffff0;      /* workgroups of 512 threads in one dimension of a grid (below 2^32 threads) */
 constexpr int64_t MAX_COPY_GROUPS = 0xffffff;       /* workgroups of 256 likewise */
+constexpr int64_t MAX_PICKS = 1 << 23;              /* workgroups of 256 that choose blocks, likewise */
 constexpr int64_t MAX_ROPE_ROW = 1 << 24;           /* elements of a token: four of them count within 31 bits */
 
 bool pow2(int x) { return x > 0 && (x & (x - 1)) == 0; }
@@ -89,6 +90,37 @@ Batch batch_of(const hearth_gpu_batch &b, const hearth_gpu_cache &c) {
     o.n_pages = c.n_pages;
     o.page_shift = __builtin_ctz((unsigned)c.page);
     return o;
+}
+
+Batch batch_of(const hearth_gpu_batch &b, int n_pages, int page) {
+    hearth_gpu_cache c{};
+    c.n_pages = n_pages; c.page = page;
+    return batch_of(b, c);
+}
+
+bool bounds_ok(const hearth_gpu_bounds *s) {
+    if (!s || !s->codes || (uintptr_t)s->codes % 16 || !s->scales) return false;
+    if (s->n_pages < 1 || s->n_heads < 1 || s->n_heads > 4096 || !pow2(s->block) || s->block < 16 || !pow2(s->blocks)) return false;
+    if ((int64_t)s->block * s->blocks > 4096 || (s->width != 64 && s->width != 128 && s->width != 256)) return false;
+    const int64_t els = (int64_t)s->blocks * 2 * s->width;
+    if (s->head_stride < (s->n_heads > 1 ? els : 0) || s->page_stride < (s->n_pages > 1 ? els : 0)) return false;
+    if (s->head_stride > MAX_STRIDE || s->page_stride > MAX_STRIDE || s->head_stride % 16 || s->page_stride % 16) return false;
+    if (s->scale_head_stride < (s->n_heads > 1 ? s->blocks : 0) || s->scale_page_stride < (s->n_pages > 1 ? s->blocks : 0)) return false;
+    return s->scale_head_stride <= MAX_STRIDE && s->scale_page_stride <= MAX_STRIDE;
+}
+
+Bounds bounds_of(const hearth_gpu_bounds &s) {
+    return {(uint8_t *)s.codes, s.scales, s.page_stride, s.head_stride, s.scale_page_stride, s.scale_head_stride,
+            __builtin_ctz((unsigned)s.block), s.blocks};
+}
+
+int64_t blocks_of(int rows, int block) { return ((int64_t)rows + block - 1) / block; }
+
+/* of the blocks chosen for n tokens and so many heads; written: rows share no element */
+bool blocks_ok(const hearth_gpu_blocks *x, int n, int heads, bool written) {
+    if (!x || (n && !x->chosen) || (uintptr_t)x->chosen % 4 || x->top < 1 || x->top > (1 << 20) || !pow2(x->block) || x->block < 16 || x->block > 4096) return false;
+    if (std::llabs(x->token_stride) > MAX_STRIDE || std::llabs(x->head_stride) > MAX_STRIDE) return false;
+    return !written || ((heads < 2 || std::llabs(x->head_stride) >= x->top) && (n < 2 || std::llabs(x->token_stride) >= x->top));
 }
 
 int finish() { return hipGetLastError() == hipSuccess ? OK : E_IO; }   /* this call's launches only */
@@ -165,8 +197,20 @@ int64_t part_bytes(const hearth_gpu_cache &c, const hearth_gpu_batch &b, int hea
     return s.n == 1 ? 0 : (int64_t)o.n_tokens * heads * s.n * (dv + 2) * (int64_t)sizeof(float);
 }
 
+/* the split of an attention over chosen blocks, and its bytes; -1 for arguments that it refuses */
+int64_t blocks_part_bytes(const hearth_gpu_cache *c, const hearth_gpu_batch *b, int heads, int top, int block, Split &s) {
+    if (!attend_shape_ok(c, b, heads) || !c->v.data || top < 1 || top > (1 << 20) || !pow2(block) || block < 16 || block > c->page) return E_ARG;
+    const Batch o = batch_of(*b, *c);
+    if ((int64_t)top * block > MAX_ROWS || (int64_t)o.max_q * c->n_heads * ((heads / c->n_heads + 15) / 16) > MAX_COPY_GROUPS) return E_ARG;
+    s = {0x40000000, 1, false};
+    if (!o.n_seqs || !o.max_q) return 0;
+    s = blocks_split(o.n_seqs, b->max_q, top * block, heads, c->n_heads);
+    return s.n == 1 ? 0 : (int64_t)o.n_tokens * heads * s.n * (c->width + 2) * (int64_t)sizeof(float);
+}
+
 int attend_call(const hearth_gpu_cache *c, const hearth_gpu_batch *b, const hearth_gpu_array *q, const hearth_gpu_array *q_pe,
-                const hearth_gpu_array *out, float *lse, float scale, void *work, size_t work_bytes, int dev, void *stream) {
+                const hearth_gpu_blocks *blocks, const hearth_gpu_array *out, float *lse, float scale, void *work, size_t work_bytes,
+                int dev, void *stream) {
     if (!q || !attend_shape_ok(c, b, q->n_heads) || !array_ok(q, b->n_tokens) || !array_ok(out, b->n_tokens) || dev < 0) return E_ARG;
     const bool latent = q_pe != nullptr;
     if (latent != !c->v.data || (uintptr_t)lse % 4 || !std::isfinite(scale * 1.44269504088896340736f)) return E_ARG;
@@ -175,9 +219,10 @@ int attend_call(const hearth_gpu_cache *c, const hearth_gpu_batch *b, const hear
     const int width = latent ? 512 : c->width;
     if (q->width != width || out->width != width || out->n_heads != q->n_heads) return E_ARG;
     if (latent && (!array_ok(q_pe, b->n_tokens) || q_pe->dtype != q->dtype || q_pe->n_heads != q->n_heads || q_pe->width != 64)) return E_ARG;
+    if (blocks && !blocks_ok(blocks, b->n_tokens, c->n_heads, false)) return E_ARG;
     Split s;
-    const int64_t need = part_bytes(*c, *b, q->n_heads, s);
-    if (need && ((uintptr_t)work % 16 || !work)) return E_ARG;
+    const int64_t need = blocks ? blocks_part_bytes(c, b, q->n_heads, blocks->top, blocks->block, s) : part_bytes(*c, *b, q->n_heads, s);
+    if (need < 0 || (need && ((uintptr_t)work % 16 || !work))) return E_ARG;
     if ((uint64_t)need > work_bytes) return E_CAPACITY;
     AttendArgs a{};
     a.b = batch_of(*b, *c);
@@ -194,12 +239,26 @@ int attend_call(const hearth_gpu_cache *c, const hearth_gpu_batch *b, const hear
     a.scale2 = scale * 1.44269504088896340736f;
     a.chunk = s.chunk; a.n_splits = s.n;
     a.part = (float *)work;
+    if (blocks) {
+        a.chosen = blocks->chosen; a.ct = blocks->token_stride; a.ch = blocks->head_stride;
+        a.top = blocks->top; a.block_shift = __builtin_ctz((unsigned)blocks->block);
+    }
     if (hipPeekAtLastError() != hipSuccess) return E_IO;
     DeviceGuard g(dev);
     if (!g.ok) return no_device();
     if (latent) attend_latent(a, q->dtype, c->dtype, (hipStream_t)stream);
+    else if (blocks) attend_blocks(a, q->dtype, c->dtype, c->width, (hipStream_t)stream);
     else attend(a, q->dtype, c->dtype, c->width, s.many, (hipStream_t)stream);
     return finish();
+}
+
+/* bytes of scores, or -1 for arguments that the selection refuses */
+int64_t score_bytes(const hearth_gpu_bounds *s, const hearth_gpu_batch *b) {
+    if (!bounds_ok(s) || !batch_ok(b)) return E_ARG;
+    const Batch o = batch_of(*b, s->n_pages, s->block * s->blocks);
+    if (o.kv_cap > MAX_ROWS || (int64_t)o.max_q * s->n_heads > MAX_PICKS) return E_ARG;
+    if (!o.n_seqs || !o.max_q) return 0;
+    return (int64_t)o.n_tokens * s->n_heads * blocks_of(o.kv_cap, s->block) * (int64_t)sizeof(float);
 }
 
 } // namespace
@@ -299,7 +358,7 @@ HEARTH_API int64_t hearth_gpu_attend_workspace(const hearth_gpu_cache *c, const 
 HEARTH_API int hearth_gpu_attend(const hearth_gpu_cache *c, const hearth_gpu_batch *b, const hearth_gpu_array *q,
                                  const hearth_gpu_array *out, float *lse, float scale, void *work, size_t work_bytes,
                                  int dev, void *stream) {
-    return attend_call(c, b, q, nullptr, out, lse, scale, work, work_bytes, dev, stream);
+    return attend_call(c, b, q, nullptr, nullptr, out, lse, scale, work, work_bytes, dev, stream);
 }
 
 HEARTH_API int hearth_gpu_attend_latent(const hearth_gpu_cache *c, const hearth_gpu_batch *b,
@@ -307,7 +366,70 @@ HEARTH_API int hearth_gpu_attend_latent(const hearth_gpu_cache *c, const hearth_
                                         const hearth_gpu_array *out, float *lse, float scale, void *work,
                                         size_t work_bytes, int dev, void *stream) {
     if (!q_pe) return E_ARG;
-    return attend_call(c, b, q, q_pe, out, lse, scale, work, work_bytes, dev, stream);
+    return attend_call(c, b, q, q_pe, nullptr, out, lse, scale, work, work_bytes, dev, stream);
+}
+
+HEARTH_API int hearth_gpu_key_bounds(const hearth_gpu_cache *c, const hearth_gpu_batch *b, const hearth_gpu_bounds *s, int dev,
+                                     void *stream) {
+    if (!cache_ok(c) || !batch_ok(b) || !bounds_ok(s) || dev < 0) return E_ARG;
+    if (!c->v.data || s->n_pages != c->n_pages || s->n_heads != c->n_heads || s->width != c->width || s->block * s->blocks != c->page) return E_ARG;
+    BoundsArgs a{};
+    a.b = batch_of(*b, *c);
+    if (!a.b.n_seqs || !a.b.max_q) return OK;
+    a.k = rows_of(c->k, c->dtype);
+    a.s = bounds_of(*s);
+    a.heads = c->n_heads;
+    a.per_seq = std::min<int64_t>((int64_t)a.b.max_q / s->block + 2, blocks_of(a.b.kv_cap, s->block));
+    if (a.per_seq * a.heads > MAX_COPY_GROUPS) return E_ARG;
+    if (!a.per_seq) return OK;
+    if (hipPeekAtLastError() != hipSuccess) return E_IO;
+    DeviceGuard g(dev);
+    if (!g.ok) return no_device();
+    key_bounds(a, c->dtype, c->width, (hipStream_t)stream);
+    return finish();
+}
+
+HEARTH_API int64_t hearth_gpu_select_workspace(const hearth_gpu_bounds *s, const hearth_gpu_batch *b) { return score_bytes(s, b); }
+
+HEARTH_API int hearth_gpu_select_blocks(const hearth_gpu_bounds *s, const hearth_gpu_batch *b, const hearth_gpu_array *q,
+                                        const hearth_gpu_blocks *out, int first, int last, void *work, size_t work_bytes, int dev,
+                                        void *stream) {
+    const int64_t need = score_bytes(s, b);
+    if (need < 0 || dev < 0 || !array_ok(q, b->n_tokens) || !blocks_ok(out, b->n_tokens, s->n_heads, true)) return E_ARG;
+    if ((q->dtype != HEARTH_F16 && q->dtype != HEARTH_BF16) || q->width != s->width || q->n_heads % s->n_heads || out->block != s->block) return E_ARG;
+    const int group = q->n_heads / s->n_heads;
+    if (group > select_group_limit() || first < 0 || last < 1 || first > out->top || last > out->top) return E_ARG;
+    SelectArgs a{};
+    a.b = batch_of(*b, s->n_pages, s->block * s->blocks);
+    /* blocks that a tree's node keeps: from the one of the call's first token on */
+    const int64_t tail = b->mask ? std::max<int64_t>(last, a.b.max_q ? blocks_of(a.b.max_q - 1, s->block) + 1 : 0) : last;
+    if (first + tail > out->top) return E_ARG;
+    if (!a.b.n_seqs || !a.b.max_q) return OK;
+    if (need && (!work || (uintptr_t)work % 16)) return E_ARG;
+    if ((uint64_t)need > work_bytes) return E_CAPACITY;
+    a.s = bounds_of(*s);
+    a.q = (const uint8_t *)q->data; a.qt = 2 * q->token_stride; a.qh = 2 * q->head_stride;
+    a.chosen = out->chosen; a.ct = out->token_stride; a.ch = out->head_stride;
+    a.kv_heads = s->n_heads; a.group = group; a.top = out->top; a.first = first; a.last = last;
+    a.score = (float *)work;
+    a.ld_score = blocks_of(a.b.kv_cap, s->block);
+    if (hipPeekAtLastError() != hipSuccess) return E_IO;
+    DeviceGuard g(dev);
+    if (!g.ok) return no_device();
+    select_blocks(a, q->dtype, s->width, (int)a.ld_score, (hipStream_t)stream);
+    return finish();
+}
+
+HEARTH_API int hearth_gpu_attend_blocks(const hearth_gpu_cache *c, const hearth_gpu_batch *b, const hearth_gpu_array *q,
+                                        const hearth_gpu_blocks *blocks, const hearth_gpu_array *out, float *lse, float scale,
+                                        void *work, size_t work_bytes, int dev, void *stream) {
+    if (!blocks) return E_ARG;
+    return attend_call(c, b, q, nullptr, blocks, out, lse, scale, work, work_bytes, dev, stream);
+}
+
+HEARTH_API int64_t hearth_gpu_attend_blocks_workspace(const hearth_gpu_cache *c, const hearth_gpu_batch *b, int n_heads, int top, int block) {
+    Split s;
+    return blocks_part_bytes(c, b, n_heads, top, block, s);
 }
 
 } // extern "C"

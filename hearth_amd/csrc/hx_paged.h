@@ -95,6 +95,36 @@ struct AttendArgs {
     float scale2;                     /* scale * log2(e): probabilities are powers of two */
     int chunk, n_splits;              /* rows of a split (a multiple of the kernels' row step); splits of the longest */
     float *part;                      /* [n_tokens][heads][n_splits][DV] sums, then [..][2] maximum and sum */
+    /* attend_blocks: the rows are those of the chosen blocks, one after the other */
+    const int *chosen;
+    int64_t ct, ch;                   /* elements */
+    int top, block_shift;             /* top 0: every row */
+};
+
+/* ---- blocks of rows, their bounds and their choice ---- */
+struct Bounds {
+    uint8_t *codes, *scales;
+    int64_t page_stride, head_stride, scale_page_stride, scale_head_stride;   /* bytes */
+    int block_shift, blocks;          /* log2 of a block's rows; blocks of a page */
+};
+struct BoundsArgs {
+    Batch b;
+    Rows k;
+    Bounds s;
+    int heads;
+    int64_t per_seq;                  /* blocks that a sequence's tokens may touch */
+};
+struct SelectArgs {
+    Batch b;
+    Bounds s;
+    const uint8_t *q;
+    int64_t qt, qh;                   /* bytes */
+    int *chosen;
+    int64_t ct, ch;                   /* elements */
+    int kv_heads, group, top, first, last;
+    float *score;                     /* [n_tokens][kv_heads][ld_score] */
+    int64_t ld_score;
+    int chunk, n_chunks;              /* blocks a workgroup scores */
 };
 
 /* device of a call made current while the object lives */
@@ -121,9 +151,15 @@ void kv_read(const CopyArgs &a, int dst_dtype, int cache_dtype, bool aligned, hi
 struct Split { int chunk, n; bool many; };
 Split attend_split(int n_seqs, int max_q, int kv_cap, int heads, int kv_heads, bool latent);
 void attend(const AttendArgs &a, int q_dtype, int cache_dtype, int width, bool many, hipStream_t st);
+Split blocks_split(int n_seqs, int max_q, int rows, int heads, int kv_heads);
+void attend_blocks(const AttendArgs &a, int q_dtype, int cache_dtype, int width, hipStream_t st);
 void attend_many(const AttendArgs &a, int q_dtype, int cache_dtype, int width, hipStream_t st);   /* k_paged_many.hip */
 void latent_rows(const AttendArgs &a, int q_dtype, bool mx, hipStream_t st);                         /* k_paged_latent.hip */
 void attend_latent(const AttendArgs &a, int q_dtype, int cache_dtype, hipStream_t st);
+
+void key_bounds(const BoundsArgs &a, int cache_dtype, int width, hipStream_t st);   /* k_paged_select.hip */
+int select_group_limit();   /* query heads of a kv head */
+void select_blocks(SelectArgs a, int q_dtype, int width, int n_blocks, hipStream_t st);
 
 /* ------------------------------------------------------------------ device helpers */
 

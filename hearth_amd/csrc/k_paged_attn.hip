@@ -146,7 +146,9 @@ struct Few {
     }
 };
 
-template <class T, int BITS, int D>
+/* BLOCKS: of the rows of chosen blocks, which stand one after the other in the place of the
+ * sequence's. A workgroup's columns are then heads of one token, since every token has blocks of its own. */
+template <class T, int BITS, int D, bool BLOCKS>
 __global__ __launch_bounds__(64 * FEW_WAVES) void k_attend_few(AttendArgs a) {
     using F = Few<T, BITS, D>;
     using v8 = typename T::v8;
@@ -161,19 +163,24 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_attend_few(AttendArgs a) {
     int bx = blockIdx.x;
     const int sp = bx % a.n_splits;
     bx /= a.n_splits;
-    const int kvh = bx % a.kv_heads, tile = bx / a.kv_heads;
+    const int kvh = bx % a.kv_heads;
+    bx /= a.kv_heads;
     const int seq = blockIdx.z;
     const Seq q = seq_of(a.b, seq);
-    const int cols = min(q.n, a.b.max_q) * a.group;
-    if (tile * CT >= cols) return;
-    const int n_sp = max(1, (q.kv + a.chunk - 1) / a.chunk);
+    const int head_tiles = (a.group + CT - 1) / CT;
+    /* BLOCKS: the token, and its columns from c0 on; otherwise columns are (token, head) pairs */
+    const int only = BLOCKS ? bx / head_tiles : 0, c0 = (BLOCKS ? bx % head_tiles : bx) * CT;
+    if (BLOCKS && only >= min(q.n, a.b.max_q)) return;
+    const int cols = BLOCKS ? a.group : min(q.n, a.b.max_q) * a.group;
+    if (c0 >= cols) return;
+    const int n_sp = BLOCKS ? a.n_splits : max(1, (q.kv + a.chunk - 1) / a.chunk);
     if (sp >= n_sp) return;
 
     /* this lane's column */
     v8 qf[F::KS];
-    const int c = tile * CT + lc;
+    const int c = c0 + lc;
     const bool on = c < cols;
-    const int tok = on ? c / a.group : 0, head = kvh * a.group + (on ? c % a.group : 0);
+    const int tok = BLOCKS ? only : on ? c / a.group : 0, head = kvh * a.group + (!on ? 0 : BLOCKS ? c : c % a.group);
     /* rows it attends without a mask (causal), or rows before the call's */
     const int lim = !on ? 0 : a.b.mask ? min(q.base, q.kv) : min(q.base + tok + 1, q.kv);
     const uint8_t *qp = a.q + (int64_t)(q.q0 + tok) * a.qt + (int64_t)head * a.qh;
@@ -184,11 +191,13 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_attend_few(AttendArgs a) {
         if (on) w = *(const u4_any *)p;
         qf[i] = __builtin_bit_cast(v8, w);
     }
-    /* rows [lo, hi) of this split that some column of the tile may attend; below `full` every
+    /* rows below hi some column of the tile may attend (without BLOCKS: of this split); below `full` every
      * valid column attends every row */
-    const int t_first = tile * CT / a.group, t_last = min(cols - 1, tile * CT + CT - 1) / a.group;
-    const int hi = min(min(q.kv, a.b.mask ? q.kv : q.base + t_last + 1), (sp + 1) * a.chunk);
+    const int t_first = BLOCKS ? only : c0 / a.group, t_last = BLOCKS ? only : min(cols - 1, c0 + CT - 1) / a.group;
+    const int end = a.b.mask ? q.kv : min(q.kv, q.base + t_last + 1);
+    const int hi = BLOCKS ? end : min(end, (sp + 1) * a.chunk);
     const int full = a.b.mask ? q.base : q.base + t_first + 1;
+    const int stop = BLOCKS ? min(a.top << a.block_shift, (sp + 1) * a.chunk) : hi;   /* of the steps */
 
     /* which of the 64 rows from t0 on this lane's column attends (where their pages exist) */
     auto attended = [&](int t0) {
@@ -209,43 +218,57 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_attend_few(AttendArgs a) {
     const uint8_t *ksb = MX ? a.k.scales + (int64_t)kvh * a.k.scale_head_stride : nullptr;
     const uint8_t *vsb = MX ? a.v.scales + (int64_t)kvh * a.v.scale_head_stride : nullptr;
 
-    /* Pages of the two tiles of 16 rows (-1: none). Every load goes to a row of the cache: rows past hi
+    /* Sixteen rows from `row` on in a page (-1: none). Every load goes to a row of the cache: rows past hi
      * lie in the same page, those of a page that is not there are taken from page 0; both are
      * masked, and cleared in V. */
-    auto page_at = [&](int t) __attribute__((always_inline)) {
-        const int id = t < hi ? word_of(pages, t >> a.b.page_shift) : -1;
-        return page_ok(a.b, id) ? id : -1;
+    struct Tile { int row, page; };
+    const int *list = BLOCKS ? a.chosen + (int64_t)(q.q0 + only) * a.ct + (int64_t)kvh * a.ch : nullptr;
+    auto tile_at = [&](int t) __attribute__((always_inline)) {
+        Tile x = {t, -1};
+        if constexpr (BLOCKS) {
+            const int blk = t < stop ? word_of(list, t >> a.block_shift) : -1;
+            const int64_t row = ((int64_t)blk << a.block_shift) + (t & ((1 << a.block_shift) - 1));
+            x.row = blk >= 0 && row < hi ? (int)row : -1;
+        }
+        const int id = BLOCKS ? x.row >= 0 ? word_of(pages, x.row >> a.b.page_shift) : -1 : t < hi ? word_of(pages, t >> a.b.page_shift) : -1;
+        x.page = page_ok(a.b, id) ? id : -1;
+        return x;
+    };
+    /* whether every valid column attends every row of a step */
+    auto whole_at = [&](int t0, const Tile (&x)[2]) __attribute__((always_inline)) {
+        if constexpr (BLOCKS) return x[0].row + 16 <= full && x[0].row + 16 <= hi && x[1].row + 16 <= full && x[1].row + 16 <= hi && x[0].page >= 0 && x[1].page >= 0;
+        else return t0 + FEW_STEP <= full && t0 + FEW_STEP <= hi && x[0].page >= 0 && x[1].page >= 0;
     };
     typename F::K kr;
     typename F::V vw;
-    auto load_k = [&](int t0, const int (&id)[2]) __attribute__((always_inline)) {
+    auto load_k = [&](const Tile (&x)[2]) __attribute__((always_inline)) {
 #pragma unroll
         for (int u = 0; u < 2; u++) {
-            const int64_t i = max(id[u], 0);
-            F::load_k(kr, u, kbase + i * a.k.page_stride, MX ? ksb + i * a.k.scale_page_stride : nullptr, (t0 + 16 * u) & (page_rows - 1), g, lc);
+            const int64_t i = max(x[u].page, 0);
+            F::load_k(kr, u, kbase + i * a.k.page_stride, MX ? ksb + i * a.k.scale_page_stride : nullptr, x[u].row & (page_rows - 16), g, lc);
         }
     };
-    auto load_v = [&](int t0, const int (&id)[2]) __attribute__((always_inline)) {
+    auto load_v = [&](const Tile (&x)[2]) __attribute__((always_inline)) {
 #pragma unroll
         for (int u = 0; u < 2; u++) {
-            const int64_t i = max(id[u], 0);
-            F::load_v(vw, u, vbase + i * a.v.page_stride, MX ? vsb + i * a.v.scale_page_stride : nullptr, (t0 + 16 * u) & (page_rows - 1), g, lc);
+            const int64_t i = max(x[u].page, 0);
+            F::load_v(vw, u, vbase + i * a.v.page_stride, MX ? vsb + i * a.v.scale_page_stride : nullptr, x[u].row & (page_rows - 16), g, lc);
         }
     };
     const int first = sp * a.chunk + FEW_STEP * wave;
-    int pid[2] = {-1, -1}, next[2] = {page_at(first), page_at(first + 16)};
+    Tile now[2], next[2] = {tile_at(first), tile_at(first + 16)};
     arrived();
-    if (first < hi) load_k(first, next);
+    if (first < stop) load_k(next);
     /* a step: V on its way before the scores, the next step's K as soon as these have taken K */
-    for (int t0 = first; t0 < hi; t0 += FEW_STEP * FEW_WAVES) {
+    for (int t0 = first; t0 < stop; t0 += FEW_STEP * FEW_WAVES) {
         bool ok[2];
 #pragma unroll
         for (int u = 0; u < 2; u++) {
-            pid[u] = next[u];
-            ok[u] = pid[u] >= 0;
-            next[u] = page_at(t0 + FEW_STEP * FEW_WAVES + 16 * u);
+            now[u] = next[u];
+            ok[u] = now[u].page >= 0;
+            next[u] = tile_at(t0 + FEW_STEP * FEW_WAVES + 16 * u);
         }
-        load_v(t0, pid);
+        load_v(now);
         in_order();
         f4 s[2];
 #pragma unroll
@@ -254,9 +277,9 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_attend_few(AttendArgs a) {
             F::scores(kr, u, g, qf, s[u]);
         }
         in_order();
-        if (t0 + FEW_STEP * FEW_WAVES < hi) load_k(t0 + FEW_STEP * FEW_WAVES, next);
+        if (t0 + FEW_STEP * FEW_WAVES < stop) load_k(next);
         in_order();
-        const bool whole = t0 + FEW_STEP <= full && t0 + FEW_STEP <= hi && ok[0] && ok[1];
+        const bool whole = whole_at(t0, now);
         v8 pf;
         float x[8];
 #pragma unroll
@@ -264,7 +287,11 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_attend_few(AttendArgs a) {
         if (whole) {
             some = true;
         } else {
-            const unsigned long long at = attended(t0) & group_rows((ok[0] ? 1u : 0u) | (ok[1] ? 2u : 0u)), vis = at >> (4 * g);
+            unsigned long long at;
+            if constexpr (BLOCKS)
+                at = (ok[0] ? attended(now[0].row) & 0xffff : 0) | (ok[1] ? (attended(now[1].row) & 0xffff) << 16 : 0);
+            else at = attended(t0) & group_rows((ok[0] ? 1u : 0u) | (ok[1] ? 2u : 0u));
+            const unsigned long long vis = at >> (4 * g);
             some = some || at;
 #pragma unroll
             for (int j = 0; j < 8; j++) x[j] = vis >> (16 * (j >> 2) + (j & 3)) & 1 ? x[j] : -__builtin_huge_valf();
@@ -292,7 +319,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_attend_few(AttendArgs a) {
             unsigned w[8][PL / 2];
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-                const int u = j >> 2, t = t0 + 16 * u + 4 * g + (j & 3);
+                const int u = j >> 2, t = (BLOCKS ? now[u].row : t0 + 16 * u) + 4 * g + (j & 3);
                 F::v_row(vw, b, j, lc, w[j]);
                 if (!whole) {
 #pragma unroll
@@ -315,13 +342,13 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_attend_few(AttendArgs a) {
     /* an infinity or NaN among rows that some columns do not attend would reach them as 0 * inf:
      * left out above, added here to the columns that do attend it */
     if (__any(odd)) {
-        for (int t0 = sp * a.chunk + FEW_STEP * wave; t0 < hi; t0 += FEW_STEP * FEW_WAVES) {
+        for (int t0 = first; t0 < stop; t0 += FEW_STEP * FEW_WAVES) {
+            const Tile x[2] = {tile_at(t0), tile_at(t0 + 16)};
+            if (whole_at(t0, x)) continue;   /* a step taken as it is */
 #pragma unroll 1
-            for (int t = t0; t < min(t0 + FEW_STEP, hi); t++) {
-                const int id = word_of(pages, t >> a.b.page_shift);
-                if (t0 + FEW_STEP <= full && t0 + FEW_STEP <= hi && page_ok(a.b, word_of(pages, t0 >> a.b.page_shift)) &&
-                    page_ok(a.b, word_of(pages, (t0 + 16) >> a.b.page_shift))) break;   /* a step taken as it is */
-                if (!page_ok(a.b, id)) continue;
+            for (int z = 0; z < 32; z++) {
+                const int id = z < 16 ? x[0].page : x[1].page, t = (z < 16 ? x[0].row : x[1].row) + (z & 15);
+                if (id < 0 || t >= hi) continue;
                 const uint8_t *row = vbase + (int64_t)id * a.v.page_stride + (int64_t)(t & (page_rows - 1)) * F::RB;
                 const uint8_t *sc = MX ? vsb + (int64_t)id * a.v.scale_page_stride + (t & (page_rows - 1)) * (D / MX_BLOCK) : nullptr;
 #pragma unroll
@@ -360,9 +387,9 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_attend_few(AttendArgs a) {
     }
     static_assert(FEW_WAVES == 4);
     const bool undefined = Lo == 0.0f && ((lds_some[0] | lds_some[1] | lds_some[2] | lds_some[3]) >> oc & 1);
-    const int co = tile * CT + oc;
+    const int co = c0 + oc;
     const bool here = co < cols;
-    const int ot = here ? co / a.group : 0, oh = kvh * a.group + (here ? co % a.group : 0);
+    const int ot = BLOCKS ? only : here ? co / a.group : 0, oh = kvh * a.group + (!here ? 0 : BLOCKS ? co : co % a.group);
     const int64_t row = (int64_t)(q.q0 + ot) * a.heads + oh;
 #pragma unroll
     for (int b = 0; b < NB; b++) {
@@ -422,7 +449,7 @@ __global__ __launch_bounds__(JOIN_THREADS) void k_attend_join(AttendArgs a) {
     const Seq q = seq_of(a.b, seq);
     const int r = MANY ? blockIdx.x : blockIdx.x * NG + grp;
     const int t = r / a.heads, h = r % a.heads;
-    const int n_sp = max(1, (q.kv + a.chunk - 1) / a.chunk);
+    const int n_sp = a.top ? a.n_splits : max(1, (q.kv + a.chunk - 1) / a.chunk);
     if (n_sp == 1) return;
     const bool on = t < min(q.n, a.b.max_q);
     if (!on) return;   /* MANY: the whole workgroup */
@@ -479,11 +506,11 @@ __global__ __launch_bounds__(JOIN_THREADS) void k_attend_join(AttendArgs a) {
     if (a.lse && e == 0) a.lse[row] = L == 0.0f ? NINF : (M + __log2f(L)) * 0.69314718055994531f;
 }
 
-template <class T, int BITS, int D>
+template <class T, int BITS, int D, bool BLOCKS>
 void few_t(const AttendArgs &a, hipStream_t st) {
-    const int tiles = (a.b.max_q * a.group + 15) / 16;
+    const int tiles = BLOCKS ? a.b.max_q * ((a.group + 15) / 16) : (a.b.max_q * a.group + 15) / 16;
     const dim3 grid((unsigned)a.n_splits * a.kv_heads * tiles, 1, a.b.n_seqs);
-    hipLaunchKernelGGL((k_attend_few<T, BITS, D>), grid, dim3(64 * FEW_WAVES), 0, st, a);
+    hipLaunchKernelGGL((k_attend_few<T, BITS, D, BLOCKS>), grid, dim3(64 * FEW_WAVES), 0, st, a);
 }
 
 template <class T, int DV>
@@ -521,20 +548,43 @@ Split attend_split(int n_seqs, int max_q, int kv_cap, int heads, int kv_heads, b
     return {(int)chunk, std::max(1, (int)((kv_cap + chunk - 1) / chunk)), many};
 }
 
-void attend(const AttendArgs &a, int q_dtype, int cache_dtype, int width, bool many, hipStream_t st) {
-    const int bits = bits_of(cache_dtype);
+/* As attend_split; a unit is a token and 16 of a kv head's query heads */
+Split blocks_split(int n_seqs, int max_q, int rows, int heads, int kv_heads) {
+    const int64_t wgs = std::max<int64_t>((int64_t)n_seqs * kv_heads * max_q * ((heads / kv_heads + 15) / 16), 1);
+    const int64_t want = std::max<int64_t>(1, 512 / wgs), step = FEW_STEP * FEW_WAVES;
+    int64_t chunk = (rows + want - 1) / want;
+    chunk = std::max<int64_t>((chunk + step - 1) / step * step, 512);
+    return {(int)chunk, (int)((rows + chunk - 1) / chunk), false};
+}
+
 #define HXP_BY(F, T) (width == 64 ? F(T, 64) : width == 128 ? F(T, 128) : F(T, 256))
-#define HXP_FEW(T, D) (bits == 16 ? few_t<T, 16, D>(a, st) : bits == 8 ? few_t<T, 8, D>(a, st) : few_t<T, 4, D>(a, st))
-#define HXP_JOIN(T, D) join_t<T, D>(a, st)
-    if (many) attend_many(a, q_dtype, cache_dtype, width, st);
-    else if (q_dtype == DT_BF16) HXP_BY(HXP_FEW, Bf16);
+template <bool BLOCKS>
+static void few(const AttendArgs &a, int q_dtype, int cache_dtype, int width, hipStream_t st) {
+    const int bits = bits_of(cache_dtype);
+#define HXP_FEW(T, D) (bits == 16 ? few_t<T, 16, D, BLOCKS>(a, st) : bits == 8 ? few_t<T, 8, D, BLOCKS>(a, st) : few_t<T, 4, D, BLOCKS>(a, st))
+    if (q_dtype == DT_BF16) HXP_BY(HXP_FEW, Bf16);
     else HXP_BY(HXP_FEW, F16);
+#undef HXP_FEW
+}
+
+static void join(const AttendArgs &a, int q_dtype, int width, hipStream_t st) {
     if (a.n_splits == 1) return;
+#define HXP_JOIN(T, D) join_t<T, D>(a, st)
     if (q_dtype == DT_BF16) HXP_BY(HXP_JOIN, Bf16);
     else HXP_BY(HXP_JOIN, F16);
 #undef HXP_JOIN
-#undef HXP_FEW
+}
 #undef HXP_BY
+
+void attend(const AttendArgs &a, int q_dtype, int cache_dtype, int width, bool many, hipStream_t st) {
+    if (many) attend_many(a, q_dtype, cache_dtype, width, st);
+    else few<false>(a, q_dtype, cache_dtype, width, st);
+    join(a, q_dtype, width, st);
+}
+
+void attend_blocks(const AttendArgs &a, int q_dtype, int cache_dtype, int width, hipStream_t st) {
+    few<true>(a, q_dtype, cache_dtype, width, st);
+    join(a, q_dtype, width, st);
 }
 
 void attend_latent(const AttendArgs &a, int q_dtype, int cache_dtype, hipStream_t st) {

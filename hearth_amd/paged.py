@@ -9,6 +9,12 @@ For programs that keep many conversations' rows in pages next to (or without) an
     attend(cache, batch, q, out)     grouped-head attention: tokens, chains, draft trees, prompts
     attend_latent(...)               absorbed latent attention over one row a token
 
+and, for long sequences of which each token looks at a few blocks of rows only:
+
+    update_bounds(cache, batch, bounds)        bounds of the keys of each block, after append
+    select(bounds, batch, q, chosen)           the blocks that each token is to look at
+    attend_blocks(cache, batch, q, chosen, out)   attention over their rows
+
 Arrays are device tensors: anything with data_ptr(), shape, stride(), dtype, get_device(),
 element_size() and is_contiguous() as torch tensors have them (torch itself is not imported). Work is enqueued
 on `stream` (a HIP stream handle such as torch.cuda.current_stream().cuda_stream; 0 is the
@@ -32,7 +38,8 @@ from . import _native
 from .engine import HearthError
 
 __all__ = ["Cache", "Batch", "rope", "rope_frequencies", "append", "append_rotated", "read", "attend", "attend_latent",
-           "workspace_bytes"]
+           "workspace_bytes", "Bounds", "update_bounds", "select", "select_workspace_bytes", "attend_blocks",
+           "attend_blocks_workspace_bytes"]
 
 F32, F16, BF16, MX8, MX4 = 0, 1, 2, 16, 17
 _DTYPES = {"float32": F32, "float16": F16, "bfloat16": BF16, "float8_e4m3fn": MX8, "float4_e2m1fn_x2": MX4}
@@ -59,6 +66,16 @@ class _Array(Structure):
                 ("n_heads", c_int32), ("width", c_int32)]
 
 
+class _BoundsS(Structure):
+    _fields_ = [("codes", c_void_p), ("scales", c_void_p), ("page_stride", c_int64), ("head_stride", c_int64),
+                ("scale_page_stride", c_int64), ("scale_head_stride", c_int64), ("n_pages", c_int32), ("n_heads", c_int32),
+                ("block", c_int32), ("blocks", c_int32), ("width", c_int32)]
+
+
+class _BlocksS(Structure):
+    _fields_ = [("chosen", c_void_p), ("token_stride", c_int64), ("head_stride", c_int64), ("top", c_int32), ("block", c_int32)]
+
+
 _PROTOS = {
     "hearth_gpu_rope": (c_int, [POINTER(_Array), POINTER(_Array), POINTER(_Array), POINTER(_Array), c_int, c_void_p,
                                 c_int, c_void_p, c_int, c_int, c_int, c_int, c_double, c_int, c_void_p]),
@@ -73,6 +90,13 @@ _PROTOS = {
                                   c_float, c_void_p, c_size_t, c_int, c_void_p]),
     "hearth_gpu_attend_latent": (c_int, [POINTER(_CacheS), POINTER(_BatchS), POINTER(_Array), POINTER(_Array),
                                          POINTER(_Array), c_void_p, c_float, c_void_p, c_size_t, c_int, c_void_p]),
+    "hearth_gpu_key_bounds": (c_int, [POINTER(_CacheS), POINTER(_BatchS), POINTER(_BoundsS), c_int, c_void_p]),
+    "hearth_gpu_select_blocks": (c_int, [POINTER(_BoundsS), POINTER(_BatchS), POINTER(_Array), POINTER(_BlocksS), c_int, c_int,
+                                         c_void_p, c_size_t, c_int, c_void_p]),
+    "hearth_gpu_attend_blocks": (c_int, [POINTER(_CacheS), POINTER(_BatchS), POINTER(_Array), POINTER(_BlocksS), POINTER(_Array),
+                                         c_void_p, c_float, c_void_p, c_size_t, c_int, c_void_p]),
+    "hearth_gpu_attend_blocks_workspace": (c_int64, [POINTER(_CacheS), POINTER(_BatchS), c_int, c_int, c_int]),
+    "hearth_gpu_select_workspace": (c_int64, [POINTER(_BoundsS), POINTER(_BatchS)]),
     "hearth_gpu_attend_workspace": (c_int64, [POINTER(_CacheS), POINTER(_BatchS), c_int]),
 }
 _fns: dict = {}
@@ -384,7 +408,7 @@ def workspace_bytes(cache: Cache, batch: Batch, heads: int, tokens: int | None =
     return n
 
 
-def _attend(name, cache, batch, q, q_pe, out, lse, scale, workspace, stream):
+def _attend(name, cache, batch, q, q_pe, out, lse, scale, workspace, stream, chosen=None, block=0):
     dev = cache.device
     if batch.device != dev:
         raise ValueError(f"{name}: the batch is on device {batch.device}, the cache on device {dev}")
@@ -409,15 +433,23 @@ def _attend(name, cache, batch, q, q_pe, out, lse, scale, workspace, stream):
             raise ValueError("workspace: not dense")
         wp, wb = workspace.data_ptr(), workspace.numel() * workspace.element_size()
     bs = batch._of(tokens)
-    if q_pe is None:
+    if chosen is not None:
+        x = _blocks(chosen, "chosen", dev, tokens, cache._s.n_heads, block)
+        rc = _fn("hearth_gpu_attend_blocks")(cache._ref, bs, byref(a), byref(x), byref(o), lp, float(scale), wp, wb, dev, stream)
+    elif q_pe is None:
         rc = _fn("hearth_gpu_attend")(cache._ref, bs, byref(a), byref(o), lp, float(scale), wp, wb, dev, stream)
     else:
         pe = _array(q_pe, "q_pe", dev)
         if q_pe.shape[0] != tokens or pe.n_heads != a.n_heads or pe.dtype != a.dtype:
             raise ValueError(f"{name}: q_pe is {q_pe.dtype}{tuple(q_pe.shape)}, q {q.dtype}{tuple(q.shape)}")
         rc = _fn("hearth_gpu_attend_latent")(cache._ref, bs, byref(a), byref(pe), byref(o), lp, float(scale), wp, wb, dev, stream)
-    if rc == -1 and (wp is None or wp % 16) and (need := workspace_bytes(cache, batch, a.n_heads, tokens)):
-        raise ValueError(f"{name}: a workspace of {need} bytes on 16 is needed")
+    if rc == -1 and (wp is None or wp % 16):
+        if chosen is not None:
+            need = attend_blocks_workspace_bytes(cache, batch, a.n_heads, x.top, block, tokens)
+        else:
+            need = workspace_bytes(cache, batch, a.n_heads, tokens)
+        if need:
+            raise ValueError(f"{name}: a workspace of {need} bytes on 16 is needed")
     if rc:
         _check(rc, name)
 
@@ -438,6 +470,128 @@ def attend_latent(cache: Cache, batch: Batch, q, q_pe, out, *, scale: float, lse
     if q_pe is None:
         raise ValueError("attend_latent: q_pe is missing")
     _attend("attend_latent", cache, batch, q, q_pe, out, lse, scale, workspace, stream)
+
+
+class Bounds:
+    """Bounds of the keys of each block of a cache's rows: low_high int8 [pages, heads, blocks a page, 2,
+    width] (least and greatest value of each element in whole steps) and steps uint8 [pages, heads,
+    blocks a page] (the step as exponent + 127). block: rows of a block, a power of two from 16 up to a
+    page. Dense but for the first two dimensions; the tensors are the caller's, filled by update_bounds."""
+
+    def __init__(self, low_high, steps, *, block: int):
+        self.low_high, self.steps, self.block = low_high, steps, block
+        self.device = _device(low_high, "low_high")
+        shape = tuple(low_high.shape)
+        if len(shape) != 5 or shape[3] != 2 or str(low_high.dtype) not in ("torch.int8", "int8"):
+            raise ValueError(f"low_high: {low_high.dtype}{shape}, wanted int8 [pages, heads, blocks a page, 2, width]")
+        if tuple(steps.shape) != shape[:3] or str(steps.dtype) not in ("torch.uint8", "uint8"):
+            raise ValueError(f"steps: {steps.dtype}{tuple(steps.shape)}, wanted uint8{shape[:3]}")
+        _device(steps, "steps", self.device)
+        st, ss = low_high.stride(), steps.stride()
+        if st[4] != 1 or st[3] != shape[4] or (shape[2] > 1 and st[2] != 2 * shape[4]) or (shape[2] > 1 and ss[2] != 1):
+            raise ValueError(f"low_high, steps: strides {st} and {ss}, dense blocks are wanted")
+        s = _BoundsS()
+        s.codes, s.page_stride, s.head_stride = low_high.data_ptr(), st[0], st[1]
+        s.scales, s.scale_page_stride, s.scale_head_stride = steps.data_ptr(), ss[0], ss[1]
+        (s.n_pages, s.n_heads, s.blocks), s.width, s.block = shape[:3], shape[4], block
+        if not 16 <= block <= 4096 or block & (block - 1) or s.blocks < 1 or s.blocks & (s.blocks - 1) or block * s.blocks > 4096:
+            raise ValueError(f"{s.blocks} blocks of {block} rows do not make a page (powers of two, 16 to 4096 rows)")
+        if s.width not in (64, 128, 256):
+            raise ValueError(f"width {s.width} is none of 64, 128, 256")
+        if s.codes % 16 or (s.n_pages > 1 and st[0] % 16) or (s.n_heads > 1 and st[1] % 16):
+            raise ValueError("low_high: data and strides must be multiples of 16 bytes")
+        self._s = s
+        self._ref = byref(s)
+
+
+def _blocks(chosen, what, dev, tokens, heads, block) -> _BlocksS:
+    """int32 [tokens, heads, top]"""
+    p = _ints(chosen, what, dev, 3)
+    shape, st = chosen.shape, chosen.stride()
+    if shape[0] != tokens or shape[1] != heads or shape[2] < 1:
+        raise ValueError(f"{what}: shape {tuple(shape)} is not [{tokens} tokens, {heads} heads, top]")
+    return _BlocksS(p, st[0], st[1], shape[2], block)
+
+
+def update_bounds(cache: Cache, batch: Batch, bounds: Bounds, *, stream=0) -> None:
+    """Brings the bounds of the blocks that hold rows of the call's tokens (those of the batch: q_start,
+    max_q) up to date, over all of their rows that exist. After append, before select."""
+    dev = cache.device
+    if batch.device != dev or bounds.device != dev:
+        raise ValueError(f"update_bounds: cache, batch and bounds are on devices {dev}, {batch.device} and {bounds.device}")
+    cache._no_gradient()
+    c, s = cache._s, bounds._s
+    if cache.v is None:
+        raise ValueError("update_bounds: a latent cache has no keys of its own")
+    if (s.n_pages, s.n_heads, s.block * s.blocks, s.width) != (c.n_pages, c.n_heads, c.page, c.width):
+        raise ValueError(f"update_bounds: bounds of {s.n_pages} pages of {s.blocks} x {s.block} rows, {s.n_heads} heads of {s.width} over "
+                         f"a cache of {c.n_pages} pages of {c.page} rows, {c.n_heads} heads of {c.width}")
+    b = _BatchS.from_buffer_copy(batch._s)
+    b.mask, b.mask_words, b.n_tokens = None, 0, 0x7fffffff     # the starts tell how many
+    rc = _fn("hearth_gpu_key_bounds")(cache._ref, byref(b), bounds._ref, dev, stream)
+    if rc:
+        _check(rc, "update_bounds")
+
+
+def select_workspace_bytes(bounds: Bounds, batch: Batch, tokens: int | None = None) -> int:
+    """Bytes of device workspace that select needs for `tokens` query tokens (None: as many as sequences
+    times max_q)."""
+    s = _BatchS.from_buffer_copy(batch._s)
+    s.n_tokens = min(s.n_seqs * s.max_q, 0x7fffffff) if tokens is None else tokens
+    n = _fn("hearth_gpu_select_workspace")(bounds._ref, byref(s))
+    if n < 0:
+        raise ValueError(f"select: {s.max_q} tokens of {s.max_kv} rows are beyond its limits (see include/hearth_gpu.h)")
+    return n
+
+
+def select(bounds: Bounds, batch: Batch, q, chosen, *, first: int = 1, last: int = 1, workspace=None, stream=0) -> None:
+    """The best blocks of each token for each cache head: chosen int32 [tokens, heads of the bounds, top],
+    ascending, -1 behind the last. q [tokens, heads, width], float16 or bfloat16, heads a multiple of the
+    bounds'. Every token keeps its `first` first blocks and its `last` last ones (its own among them; in a
+    tree all that hold the call's rows); the others come by an upper bound of their rows' scores (include/
+    hearth_gpu.h), the lower block first where two are equal. workspace: a device tensor of
+    select_workspace_bytes; calls that may run at the same time must not share one."""
+    dev, s = bounds.device, bounds._s
+    if batch.device != dev:
+        raise ValueError(f"select: the batch is on device {batch.device}, the bounds on device {dev}")
+    a, tokens = _array(q, "q", dev), q.shape[0]
+    if a.dtype == F32 or a.width != s.width or a.n_heads % s.n_heads:
+        raise ValueError(f"select: q is {q.dtype}{tuple(q.shape)} over bounds of {s.n_heads} heads of width {s.width}")
+    o = _blocks(chosen, "chosen", dev, tokens, s.n_heads, s.block)
+    wp, wb = None, 0
+    if workspace is not None:
+        _device(workspace, "workspace", dev)
+        if not workspace.is_contiguous():
+            raise ValueError("workspace: not dense")
+        wp, wb = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    rc = _fn("hearth_gpu_select_blocks")(bounds._ref, batch._of(tokens), byref(a), byref(o), first, last, wp, wb, dev, stream)
+    if rc == -1 and (wp is None or wp % 16) and (need := select_workspace_bytes(bounds, batch, tokens)):
+        raise ValueError(f"select: arguments that do not fit together, or a workspace of {need} bytes on 16 is needed")
+    if rc:
+        _check(rc, "select")
+
+
+def attend_blocks_workspace_bytes(cache: Cache, batch: Batch, heads: int, top: int, block: int, tokens: int | None = None) -> int:
+    """Bytes of device workspace that attend_blocks needs for `tokens` query tokens (None: as many as
+    sequences times max_q) of `heads` heads and `top` chosen blocks of `block` rows: 0 when none is."""
+    s = _BatchS.from_buffer_copy(batch._s)
+    s.n_tokens = min(s.n_seqs * s.max_q, 0x7fffffff) if tokens is None else tokens
+    n = _fn("hearth_gpu_attend_blocks_workspace")(cache._ref, byref(s), heads, top, block)
+    if n < 0:
+        raise ValueError(f"no attention over {top} blocks of {block} rows of this cache (pages of {cache._s.page} rows, heads {cache._s.n_heads}, "
+                         f"width {cache._s.width}) with {heads} query heads")
+    return n
+
+
+def attend_blocks(cache: Cache, batch: Batch, q, chosen, out, *, block: int, scale: float, lse=None, workspace=None, stream=0) -> None:
+    """attend over the rows of chosen blocks alone: chosen int32 [tokens, cache heads, top], numbers of
+    blocks of `block` rows (a power of two from 16 up to a page) of the token's sequence, negative ones for none,
+    in any order, each once (one that stands twice counts twice). A token attends those of their rows that it would
+    attend without a choice (its own row at most, its mask). The rest as attend; workspace:
+    attend_blocks_workspace_bytes."""
+    if cache.v is None:
+        raise ValueError("attend_blocks: a latent cache has no keys of its own")
+    _attend("attend_blocks", cache, batch, q, None, out, lse, scale, workspace, stream, chosen, block)
 
 
 def rope(x, pos, freqs, *, factor=1.0, layout="half", offset=0, out=None, k=None, k_out=None, inverse=False,

@@ -419,6 +419,71 @@ HEARTH_API int hearth_gpu_attend_latent(const hearth_gpu_cache *c, const hearth_
  * anything in device memory. */
 HEARTH_API int64_t hearth_gpu_attend_workspace(const hearth_gpu_cache *c, const hearth_gpu_batch *b, int n_heads);
 
+/* ---- attention over chosen blocks -------------------------------------------------
+ *
+ * For long sequences: each token looks at a few blocks of rows only, which a cheap score from
+ * bounds of their keys selects. Blocks are `block` consecutive rows of a sequence (block n: rows n *
+ * block ..), a power of two from 16 up to a page's rows, so none crosses a page. */
+
+/* Bounds of the keys of every block: codes int8 [n_pages][n_heads][blocks][2][width], the least and then the
+ * greatest value of each element over the block's rows in whole steps (up to 127), the step of a block
+ * 2^(scale - 127), scales [n_pages][n_heads][blocks]; blocks: of a page (block * blocks rows of it). The last three
+ * dimensions of codes and the last one of scales are dense; strides in elements, those of codes and its address multiples
+ * of 16. width: 64, 128 or 256. */
+typedef struct hearth_gpu_bounds {
+    int8_t *codes;
+    uint8_t *scales;
+    int64_t page_stride, head_stride;
+    int64_t scale_page_stride, scale_head_stride;
+    int32_t n_pages, n_heads, block, blocks, width;
+} hearth_gpu_bounds;
+
+/* Chosen blocks of each token and cache head: [n_tokens][n_heads][top] block numbers, the last dimension
+ * dense, strides in elements; negative numbers stand for none. top up to 2^20. */
+typedef struct hearth_gpu_blocks {
+    int32_t *chosen;
+    int64_t token_stride, head_stride;
+    int32_t top, block;
+} hearth_gpu_blocks;
+
+/* Brings the bounds of the blocks that hold rows of the call's tokens up to date, from all of their rows that exist (kv_len,
+ * max_kv): call it after the rows are written. Not for latent caches. A row's element that is NaN or infinite
+ * counts as 0. The step is the least power of two with which 127 steps reach the block's largest magnitude (scale
+ * 1 at least), codes round to nearest even. Blocks on pages that are not in the cache are left alone. */
+HEARTH_API int hearth_gpu_key_bounds(const hearth_gpu_cache *c, const hearth_gpu_batch *b, const hearth_gpu_bounds *s, int dev,
+                                     void *stream);
+
+/* The `top` best blocks of each of the call's tokens and cache heads, in ascending order, -1 behind the last
+ * where fewer can be taken. q [n_tokens][H][width] of dtype HEARTH_F16 or HEARTH_BF16; H a multiple of the bounds' heads,
+ * up to 128 of them each. A token may take the blocks up to the one of its own row (or of its sequence's last row
+ * within max_kv, whichever comes first) whose pages are in the cache. It keeps the `first` first of them and the
+ * `last` last (at least 1: its own block, whose bounds look at later rows too); with a mask also those from the block
+ * of the call's first token on. The others come by their score, the greatest over the head's queries of
+ * sum_d max(q_d low_d, q_d high_d), with q in whole numbers of up to 127 steps of the least power of two that reaches its
+ * largest magnitude (NaN and infinities count as 0): whole numbers throughout, so the choice does not depend
+ * on any order of sums, and of equal scores the lower block is taken. first + last <= top; with a mask first + the blocks
+ * that max_q rows may touch as well. out's block is the bounds'. work: hearth_gpu_select_workspace bytes, 16-byte
+ * aligned. n_heads * min(max_q, n_tokens) up to 2^23; tokens of no sequence are left alone. */
+HEARTH_API int hearth_gpu_select_blocks(const hearth_gpu_bounds *s, const hearth_gpu_batch *b, const hearth_gpu_array *q,
+                                        const hearth_gpu_blocks *out, int first, int last, void *work, size_t work_bytes, int dev,
+                                        void *stream);
+
+/* Workspace of hearth_gpu_select_blocks in bytes, from the host-side fields only; -1 for arguments it would refuse. */
+HEARTH_API int64_t hearth_gpu_select_workspace(const hearth_gpu_bounds *s, const hearth_gpu_batch *b);
+
+/* hearth_gpu_attend over the rows of each token's chosen blocks alone: of them a token attends those that it
+ * would attend without a choice (up to its own row, or its mask). Blocks may stand in any order; one that stands
+ * twice counts twice; negative numbers and blocks past the sequence count for nothing. A token whose blocks hold no row that it
+ * attends gets zeros. Not for latent caches. block: a power of two from 16 up to a page, top * block below 2^30 -
+ * 65536; n_heads * min(max_q, n_tokens) * (query heads of a cache head / 16, rounded up) up to 2^24 - 1; the rest
+ * as hearth_gpu_attend. work: device memory of hearth_gpu_attend_blocks_workspace bytes, 16-byte aligned. */
+HEARTH_API int hearth_gpu_attend_blocks(const hearth_gpu_cache *c, const hearth_gpu_batch *b, const hearth_gpu_array *q,
+                                        const hearth_gpu_blocks *blocks, const hearth_gpu_array *out, float *lse, float scale,
+                                        void *work, size_t work_bytes, int dev, void *stream);
+
+/* Its workspace in bytes (0: none needed), from the host-side fields only; -1 for arguments it would refuse. */
+HEARTH_API int64_t hearth_gpu_attend_blocks_workspace(const hearth_gpu_cache *c, const hearth_gpu_batch *b, int n_heads, int top, int block);
+
 #ifdef __cplusplus
 }
 #endif
