@@ -280,6 +280,9 @@ typedef unsigned short ushort_any __attribute__((aligned(1)));
  * every conversion of its codes a NaN) */
 __device__ __forceinline__ float mx_scale(unsigned byte) { return __uint_as_float((byte & 255u) << 23); }
 
+/* of the byte at bit `at` of a word */
+__device__ __forceinline__ float mx_scale_at(unsigned word, unsigned at) { return __uint_as_float(__builtin_amdgcn_ubfe(word, at, 8) << 23); }
+
 /* maximum / sum of a value over the lanes l, l ^ 32 */
 __device__ __forceinline__ float max32(float x) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -337,6 +340,10 @@ __device__ __forceinline__ const uint8_t *same(const uint8_t *p) {
     const uint64_t x = (uint64_t)p;
     return (const uint8_t *)((uint64_t)(unsigned)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32 |
                              (unsigned)__builtin_amdgcn_readfirstlane((int)x));
+}
+/* likewise, for loads: an address of device memory to which a lane adds a 32-bit offset of its own */
+__device__ __forceinline__ const uint8_t *same_global(const uint8_t *p) {
+    return (const uint8_t *)(const __attribute__((address_space(1))) uint8_t *)(uint64_t)same(p);
 }
 template <int N, class F> __device__ __forceinline__ void each(F f) {   /* f(constant 0) .. f(constant N - 1) */
     if constexpr (N > 0) {

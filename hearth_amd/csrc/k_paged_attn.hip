@@ -28,7 +28,9 @@ namespace hxp {
 
 namespace {
 
-constexpr int FEW_WAVES = 4, FEW_STEP = 32;   /* a wave takes 32 cache rows at a time, the workgroup 128 */
+constexpr int FEW_WAVES = 4;
+/* Tiles of 16 cache rows that a wave takes at a time. Rows of 4 bits: twice as many, or too few bytes are under way */
+constexpr int few_tiles(int bits) { return bits == 4 ? 4 : 2; }
 
 __device__ __forceinline__ unsigned lo16(unsigned a, unsigned b) { return __builtin_amdgcn_perm(b, a, 0x05040100u); }
 __device__ __forceinline__ unsigned hi16(unsigned a, unsigned b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
@@ -37,6 +39,7 @@ template <class T, int BITS, int D>
 struct Few {
     using v8 = typename T::v8;
     static constexpr bool MX = BITS < 16;
+    static constexpr int NT = few_tiles(BITS), STEP = 16 * NT;
     static constexpr int KS = D / 32;                    /* matrix steps of the score */
     static constexpr int BD = D < 128 ? D : 128;        /* elements of a V block: 16 lanes x PL */
     static constexpr int NB = D / BD, PL = BD / 16;      /* blocks; elements of a row a lane takes */
@@ -48,8 +51,8 @@ struct Few {
     static constexpr int VW = VB < 4 ? 1 : VB / 4;
     static constexpr int SW = D / 32 < 4 ? 1 : D / 128;   /* words that hold a row's scales */
 
-    struct K { unsigned w[2][KL][LB / 4]; unsigned s[2][SW]; };   /* a lane's row of either tile of 16 */
-    struct V { unsigned w[NB][8][VW]; unsigned s[2][D / 32]; };   /* eight rows; scales of the four rows of either tile */
+    struct K { unsigned w[NT][KL][LB / 4]; unsigned s[NT][SW]; };             /* a lane's row of each tile of 16 */
+    struct V { unsigned w[NB][4 * NT][VW]; unsigned s[NT][D / 32]; };   /* four rows of each tile; their scales */
 
     /* first element that a lane multiplies in matrix step i */
     static __device__ __forceinline__ int at(int i, int g) { return 4 * LE * (i / SL) + LE * g + 8 * (i % SL); }
@@ -66,27 +69,28 @@ struct Few {
         } else if constexpr (BYTES == 4) w[0] = *(const unsigned *)p;
         else w[0] = *(const unsigned short *)p;
     }
-    /* row: first of the tile in its page (a multiple of 16) */
-    static __device__ __forceinline__ void load_k(K &k, int u, const uint8_t *page, const uint8_t *sc, int row, int g, int lc) {
-        const uint8_t *p = page + (row + lc) * RB + LB * g;
+    /* rows, sc: a tile's first row and its scales, the same for the wave; a lane's bytes from there on are a 32-bit
+     * offset, so that no load needs an address of its own */
+    static __device__ __forceinline__ void load_k(K &k, int u, const uint8_t *rows, const uint8_t *sc, int g, int lc) {
+        const unsigned at = lc * RB + LB * g;
 #pragma unroll
-        for (int i = 0; i < KL; i++) words<LB>(p + 4 * LB * i, k.w[u][i]);
+        for (int i = 0; i < KL; i++) words<LB>(rows + at + 4 * LB * i, k.w[u][i]);
         if constexpr (MX) {
-            const uint8_t *q = sc + (row + lc) * (D / MX_BLOCK);
+            const uint8_t *q = sc + (unsigned)(lc * (D / MX_BLOCK));
             if constexpr (D == 64) k.s[u][0] = *(const ushort_any *)q;
             else
 #pragma unroll
                 for (int i = 0; i < SW; i++) k.s[u][i] = ((const unsigned_any *)q)[i];
         }
     }
-    static __device__ __forceinline__ void load_v(V &v, int u, const uint8_t *page, const uint8_t *sc, int row, int g, int lc) {
+    static __device__ __forceinline__ void load_v(V &v, int u, const uint8_t *rows, const uint8_t *sc, int g, int lc) {
+        const unsigned at = 4 * g * RB + lc * VB;
 #pragma unroll
         for (int b = 0; b < NB; b++)
 #pragma unroll
-            for (int j = 0; j < 4; j++)
-                words<VB>(page + (row + 4 * g + j) * RB + (b * BD + lc * PL) * BITS / 8, v.w[b][4 * u + j]);
+            for (int j = 0; j < 4; j++) words<VB>(rows + at + (j * RB + b * BD * BITS / 8), v.w[b][4 * u + j]);
         if constexpr (MX) {   /* four rows' scales lie side by side */
-            const uint8_t *q = sc + (row + 4 * g) * (D / MX_BLOCK);
+            const uint8_t *q = sc + (unsigned)(4 * g * (D / MX_BLOCK));
 #pragma unroll
             for (int i = 0; i < D / 32; i += D / 32 >= 4 ? 4 : 2)
                 if constexpr (D / 32 >= 4) {
@@ -99,38 +103,38 @@ struct Few {
                 }
         }
     }
-    /* scores of the 16 rows of tile u */
-    static __device__ __forceinline__ void scores(const K &k, int u, int g, const v8 (&q)[KS], f4 &s) {
+    /* scores of the tiles' rows; the tiles take turns, since an instruction that adds to the one before waits for it */
+    static __device__ __forceinline__ void scores(const K &k, int g, const v8 (&q)[KS], f4 (&s)[NT]) {
 #pragma unroll
-        for (int i = 0; i < KL; i++) {
-            const unsigned *x = k.w[u][i];
-            if constexpr (MX) {
-                /* block LE i / 8 + LE g / 32, which does not leave the word */
-                const float f = mx_scale(k.s[u][LE * i / 32] >> (8 * (LE * i / 8 % 4) + 8 * (LE * g / 32)));
+        for (int u = 0; u < NT; u++) s[u] = (f4){0, 0, 0, 0};
 #pragma unroll
-                for (int h = 0; h < SL; h++) {
+        for (int i = 0; i < KL; i++)
+#pragma unroll
+            for (int h = 0; h < SL; h++)
+#pragma unroll
+                for (int u = 0; u < NT; u++) {
+                    const unsigned *x = k.w[u][i];
                     u4 w;
-                    if constexpr (BITS == 4)
-                        w = (u4){T::template from_mx4<0>(x[h], f), T::template from_mx4<1>(x[h], f), T::template from_mx4<2>(x[h], f),
-                                 T::template from_mx4<3>(x[h], f)};
-                    else
-                        w = (u4){T::template from_mx8<false>(x[2 * h], f), T::template from_mx8<true>(x[2 * h], f),
-                                 T::template from_mx8<false>(x[2 * h + 1], f), T::template from_mx8<true>(x[2 * h + 1], f)};
-                    s = T::mfma16(__builtin_bit_cast(v8, w), q[SL * i + h], s);
+                    if constexpr (MX) {
+                        /* block LE i / 8 + LE g / 32, which does not leave the word */
+                        const float f = mx_scale_at(k.s[u][LE * i / 32], 8 * (LE * i / 8 % 4) + 8 * (LE * g / 32));
+                        if constexpr (BITS == 4)
+                            w = (u4){T::template from_mx4<0>(x[h], f), T::template from_mx4<1>(x[h], f), T::template from_mx4<2>(x[h], f),
+                                     T::template from_mx4<3>(x[h], f)};
+                        else
+                            w = (u4){T::template from_mx8<false>(x[2 * h], f), T::template from_mx8<true>(x[2 * h], f),
+                                     T::template from_mx8<false>(x[2 * h + 1], f), T::template from_mx8<true>(x[2 * h + 1], f)};
+                    } else w = (u4){x[0], x[1], x[2], x[3]};
+                    s[u] = T::mfma16(__builtin_bit_cast(v8, w), q[SL * i + h], s[u]);
                 }
-            } else {
-                s = T::mfma16(__builtin_bit_cast(v8, (u4){x[0], x[1], x[2], x[3]}), q[i], s);
-            }
-        }
     }
     /* PL elements of row j, block b, as 16-bit pairs */
     static __device__ __forceinline__ void v_row(const V &v, int b, int j, int lc, unsigned (&w)[PL / 2]) {
         if constexpr (MX) {
             const int jj = j & 3;
-            unsigned x;
-            if constexpr (D == 64) x = v.s[j >> 2][jj >> 1] >> (16 * (jj & 1) + 8 * (lc >> 3));
-            else x = v.s[j >> 2][jj * (D / 128) + b] >> (8 * (lc >> 2));
-            const float f = mx_scale(x);
+            float f;
+            if constexpr (D == 64) f = mx_scale_at(v.s[j >> 2][jj >> 1], 16 * (jj & 1) + 8 * (lc >> 3));
+            else f = mx_scale_at(v.s[j >> 2][jj * (D / 128) + b], 8 * (lc >> 2));
             if constexpr (BITS == 4)
                 each<PL / 2>([&](auto i) { w[i] = T::template from_mx4<i.value>(v.w[b][j][0], f); });
             else
@@ -148,12 +152,17 @@ struct Few {
 
 /* BLOCKS: of the rows of chosen blocks, which stand one after the other in the place of the
  * sequence's. A workgroup's columns are then heads of one token, since every token has blocks of its own. */
-template <class T, int BITS, int D, bool BLOCKS>
-__global__ __launch_bounds__(64 * FEW_WAVES) void k_attend_few(AttendArgs a) {
+/* ONE: a step's rows lie in one page (and block), which is looked up once. */
+template <class T, int BITS, int D, bool BLOCKS, bool ONE>
+__global__ __launch_bounds__(64 * FEW_WAVES, D <= 128 ? 2 : 1) void k_attend_few(AttendArgs a) {
     using F = Few<T, BITS, D>;
     using v8 = typename T::v8;
     constexpr bool MX = F::MX;
-    constexpr int PL = F::PL, NB = F::NB, BD = F::BD, CT = 16;
+    /* Rows of 4 bits, whose steps have most to do beside the loads: the sums are rescaled only where a maximum has
+     * grown by more than 2^8, below which the probabilities lose no accuracy in either 16-bit type. */
+    constexpr float GROWTH = BITS == 4 ? 8.0f : 0.0f;
+    constexpr int PL = F::PL, NB = F::NB, BD = F::BD, CT = 16, NT = F::NT, STEP = F::STEP;
+    constexpr int PER = ONE ? NT : 1, NL = NT / PER, RUN = 16 * PER;   /* tiles of a look-up, look-ups of a step, their rows */
     __shared__ float lds_o[FEW_WAVES][16][BD + 4];
     __shared__ float lds_m[FEW_WAVES][CT], lds_l[FEW_WAVES][CT];
     __shared__ unsigned lds_some[FEW_WAVES];   /* bit c: column c attends a row of the wave's */
@@ -218,136 +227,180 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_attend_few(AttendArgs a) {
     const uint8_t *ksb = MX ? a.k.scales + (int64_t)kvh * a.k.scale_head_stride : nullptr;
     const uint8_t *vsb = MX ? a.v.scales + (int64_t)kvh * a.v.scale_head_stride : nullptr;
 
-    /* Sixteen rows from `row` on in a page (-1: none). Every load goes to a row of the cache: rows past hi
+    /* RUN rows from `row` on in a page (-1: none). Every load goes to a row of the cache: rows past hi
      * lie in the same page, those of a page that is not there are taken from page 0; both are
      * masked, and cleared in V. */
-    struct Tile { int row, page; };
+    struct Run { int row, page; };
     const int *list = BLOCKS ? a.chosen + (int64_t)(q.q0 + only) * a.ct + (int64_t)kvh * a.ch : nullptr;
-    auto tile_at = [&](int t) __attribute__((always_inline)) {
-        Tile x = {t, -1};
+    /* in two or three steps, each of which waits for the one before: the block at t, its rows with what the page table
+     * says, the page checked */
+    auto block_at = [&](int t) __attribute__((always_inline)) { return BLOCKS && t < stop ? word_of(list, t >> a.block_shift) : -1; };
+    auto look = [&](int t, int blk) __attribute__((always_inline)) {
+        Run x = {t, -1};
         if constexpr (BLOCKS) {
-            const int blk = t < stop ? word_of(list, t >> a.block_shift) : -1;
             const int64_t row = ((int64_t)blk << a.block_shift) + (t & ((1 << a.block_shift) - 1));
             x.row = blk >= 0 && row < hi ? (int)row : -1;
-        }
-        const int id = BLOCKS ? x.row >= 0 ? word_of(pages, x.row >> a.b.page_shift) : -1 : t < hi ? word_of(pages, t >> a.b.page_shift) : -1;
-        x.page = page_ok(a.b, id) ? id : -1;
+            if (x.row >= 0) x.page = word_of(pages, x.row >> a.b.page_shift);
+        } else if (t < hi) x.page = word_of(pages, t >> a.b.page_shift);
+        return x;
+    };
+    auto checked = [&](Run x) __attribute__((always_inline)) {
+        if (!page_ok(a.b, x.page)) x.page = -1;
         return x;
     };
     /* whether every valid column attends every row of a step */
-    auto whole_at = [&](int t0, const Tile (&x)[2]) __attribute__((always_inline)) {
-        if constexpr (BLOCKS) return x[0].row + 16 <= full && x[0].row + 16 <= hi && x[1].row + 16 <= full && x[1].row + 16 <= hi && x[0].page >= 0 && x[1].page >= 0;
-        else return t0 + FEW_STEP <= full && t0 + FEW_STEP <= hi && x[0].page >= 0 && x[1].page >= 0;
+    auto whole_at = [&](const Run (&x)[NL]) __attribute__((always_inline)) {
+        const int below = min(full, hi);
+        bool all = true;
+#pragma unroll
+        for (int z = 0; z < NL; z++) all = all && x[z].page >= 0 && x[z].row + RUN <= below;
+        return all;
     };
     typename F::K kr;
     typename F::V vw;
-    auto load_k = [&](const Tile (&x)[2]) __attribute__((always_inline)) {
+    auto load_k = [&](const Run (&x)[NL]) __attribute__((always_inline)) {
 #pragma unroll
-        for (int u = 0; u < 2; u++) {
-            const int64_t i = max(x[u].page, 0);
-            F::load_k(kr, u, kbase + i * a.k.page_stride, MX ? ksb + i * a.k.scale_page_stride : nullptr, x[u].row & (page_rows - 16), g, lc);
+        for (int z = 0; z < NL; z++) {
+            const int64_t i = max(x[z].page, 0), row = x[z].row & (page_rows - RUN);
+            const uint8_t *rows = same_global(kbase + i * a.k.page_stride + row * F::RB);
+            const uint8_t *sc = MX ? same_global(ksb + i * a.k.scale_page_stride + row * (D / MX_BLOCK)) : nullptr;
+#pragma unroll
+            for (int u = 0; u < PER; u++) F::load_k(kr, z * PER + u, rows + 16 * u * F::RB, MX ? sc + 16 * u * (D / MX_BLOCK) : nullptr, g, lc);
         }
     };
-    auto load_v = [&](const Tile (&x)[2]) __attribute__((always_inline)) {
+    auto load_v = [&](const Run (&x)[NL]) __attribute__((always_inline)) {
 #pragma unroll
-        for (int u = 0; u < 2; u++) {
-            const int64_t i = max(x[u].page, 0);
-            F::load_v(vw, u, vbase + i * a.v.page_stride, MX ? vsb + i * a.v.scale_page_stride : nullptr, x[u].row & (page_rows - 16), g, lc);
+        for (int z = 0; z < NL; z++) {
+            const int64_t i = max(x[z].page, 0), row = x[z].row & (page_rows - RUN);
+            const uint8_t *rows = same_global(vbase + i * a.v.page_stride + row * F::RB);
+            const uint8_t *sc = MX ? same_global(vsb + i * a.v.scale_page_stride + row * (D / MX_BLOCK)) : nullptr;
+#pragma unroll
+            for (int u = 0; u < PER; u++) F::load_v(vw, z * PER + u, rows + 16 * u * F::RB, MX ? sc + 16 * u * (D / MX_BLOCK) : nullptr, g, lc);
         }
     };
-    const int first = sp * a.chunk + FEW_STEP * wave;
-    Tile now[2], next[2] = {tile_at(first), tile_at(first + 16)};
+    constexpr int ROUND = STEP * FEW_WAVES;
+    const int first = sp * a.chunk + STEP * wave;
+    Run now[NL], next[NL];
+    int blk[NL];
+#pragma unroll
+    for (int z = 0; z < NL; z++) blk[z] = block_at(first + RUN * z);
+#pragma unroll
+    for (int z = 0; z < NL; z++) {
+        next[z] = look(first + RUN * z, blk[z]);
+        blk[z] = block_at(first + ROUND + RUN * z);
+    }
     arrived();
+#pragma unroll
+    for (int z = 0; z < NL; z++) next[z] = checked(next[z]);
     if (first < stop) load_k(next);
     /* a step: V on its way before the scores, the next step's K as soon as these have taken K */
-    for (int t0 = first; t0 < stop; t0 += FEW_STEP * FEW_WAVES) {
-        bool ok[2];
+    for (int t0 = first; t0 < stop; t0 += ROUND) {
 #pragma unroll
-        for (int u = 0; u < 2; u++) {
-            now[u] = next[u];
-            ok[u] = now[u].page >= 0;
-            next[u] = tile_at(t0 + FEW_STEP * FEW_WAVES + 16 * u);
-        }
+        for (int z = 0; z < NL; z++) now[z] = next[z];
         load_v(now);
-        in_order();
-        f4 s[2];
 #pragma unroll
-        for (int u = 0; u < 2; u++) {
-            s[u] = (f4){0, 0, 0, 0};
-            F::scores(kr, u, g, qf, s[u]);
+        for (int z = 0; z < NL; z++) {
+            next[z] = look(t0 + ROUND + RUN * z, blk[z]);
+            blk[z] = block_at(t0 + 2 * ROUND + RUN * z);
         }
         in_order();
-        if (t0 + FEW_STEP * FEW_WAVES < stop) load_k(next);
+        f4 s[NT];
+        F::scores(kr, g, qf, s);
         in_order();
-        const bool whole = whole_at(t0, now);
-        v8 pf;
-        float x[8];
 #pragma unroll
-        for (int j = 0; j < 8; j++) x[j] = s[j >> 2][j & 3] * a.scale2;
+        for (int z = 0; z < NL; z++) next[z] = checked(next[z]);
+        if (t0 + ROUND < stop) load_k(next);
+        in_order();
+        const bool whole = whole_at(now);
+        v8 pf[NT / 2];
+        float x[4 * NT];
+#pragma unroll
+        for (int j = 0; j < 4 * NT; j++) x[j] = s[j >> 2][j & 3] * a.scale2;
         if (whole) {
             some = true;
         } else {
-            unsigned long long at;
-            if constexpr (BLOCKS)
-                at = (ok[0] ? attended(now[0].row) & 0xffff : 0) | (ok[1] ? (attended(now[1].row) & 0xffff) << 16 : 0);
-            else at = attended(t0) & group_rows((ok[0] ? 1u : 0u) | (ok[1] ? 2u : 0u));
+            unsigned long long at = 0;
+            if constexpr (BLOCKS && !ONE) {
+#pragma unroll
+                for (int z = 0; z < NL; z++) at |= now[z].page >= 0 ? (attended(now[z].row) & 0xffff) << (16 * z) : 0;
+            } else {
+                unsigned have = 0;
+#pragma unroll
+                for (int u = 0; u < NT; u++) have |= now[u / PER].page >= 0 ? 1u << u : 0u;
+                at = attended(now[0].row) & group_rows(have);
+            }
             const unsigned long long vis = at >> (4 * g);
             some = some || at;
 #pragma unroll
-            for (int j = 0; j < 8; j++) x[j] = vis >> (16 * (j >> 2) + (j & 3)) & 1 ? x[j] : -__builtin_huge_valf();
+            for (int j = 0; j < 4 * NT; j++) x[j] = vis >> (16 * (j >> 2) + (j & 3)) & 1 ? x[j] : -__builtin_huge_valf();
         }
         float mx = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
-        mx = fmaxf(m, max16(max32(mx)));
-        const float ms = mx == -__builtin_huge_valf() ? 0.0f : mx;
-        if (__any(mx > m)) {
-            const float al = exp2_hw(m - ms);
+#pragma unroll
+        for (int j = 8; j < 4 * NT; j += 4) mx = fmaxf(mx, fmaxf(fmaxf(x[j], x[j + 1]), fmaxf(x[j + 2], x[j + 3])));
+        mx = max16(max32(mx));
+        if (__any(mx > m + GROWTH)) {
+            mx = fmaxf(m, mx);
+            const float al = exp2_hw(m - (mx == -__builtin_huge_valf() ? 0.0f : mx));
             l *= al;
 #pragma unroll
             for (int i = 0; i < NB * PL; i++) acc[i] *= al;
             m = mx;
         }
-        float p[8];
+        const float ms = m == -__builtin_huge_valf() ? 0.0f : m;
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            p[j] = exp2_hw(x[j] - ms);
-            l += p[j];
+        for (int j = 0; j < 4 * NT; j++) {
+            x[j] = exp2_hw(x[j] - ms);
+            l += x[j];
         }
-        const u4 w = {T::pack(p[0], p[1]), T::pack(p[2], p[3]), T::pack(p[4], p[5]), T::pack(p[6], p[7])};
-        pf = __builtin_bit_cast(v8, w);
 #pragma unroll
-        for (int b = 0; b < NB; b++) {
-            unsigned w[8][PL / 2];
+        for (int k = 0; k < NT / 2; k++) {
+            const float *p = x + 8 * k;
+            pf[k] = __builtin_bit_cast(v8, (u4){T::pack(p[0], p[1]), T::pack(p[2], p[3]), T::pack(p[4], p[5]), T::pack(p[6], p[7])});
+        }
+        /* two ways, so that the one of most steps has no branches in it */
+        auto sums = [&](auto all) __attribute__((always_inline)) {
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const int u = j >> 2, t = (BLOCKS ? now[u].row : t0 + 16 * u) + 4 * g + (j & 3);
-                F::v_row(vw, b, j, lc, w[j]);
-                if (!whole) {
+            for (int bk = 0; bk < NB * NT / 2; bk++) {
+                const int b = bk / (NT / 2), k = bk % (NT / 2);   /* block of elements, pair of tiles */
+                unsigned w[8][PL / 2];
 #pragma unroll
-                    for (int i = 0; i < PL / 2; i++) {
-                        w[j][i] = t < hi && ok[u] ? w[j][i] : 0u;
-                        odd = odd || T::odd(w[j][i]);
-                        w[j][i] = T::clean(w[j][i]);
+                for (int j = 0; j < 8; j++) {
+                    const int u = 2 * k + (j >> 2), t = now[u / PER].row + 16 * (u % PER) + 4 * g + (j & 3);
+                    F::v_row(vw, b, 8 * k + j, lc, w[j]);
+                    if constexpr (!all.value) {
+#pragma unroll
+                        for (int i = 0; i < PL / 2; i++) {
+                            w[j][i] &= t < hi && now[u / PER].page >= 0 ? ~0u : 0u;
+                            odd = odd || T::odd(w[j][i]);
+                            w[j][i] = T::clean(w[j][i]);
+                        }
                     }
                 }
-            }
 #pragma unroll
-            for (int i = 0; i < PL / 2; i++) {
-                const u4 e = {lo16(w[0][i], w[1][i]), lo16(w[2][i], w[3][i]), lo16(w[4][i], w[5][i]), lo16(w[6][i], w[7][i])};
-                const u4 o = {hi16(w[0][i], w[1][i]), hi16(w[2][i], w[3][i]), hi16(w[4][i], w[5][i]), hi16(w[6][i], w[7][i])};
-                acc[b * PL + 2 * i] = T::mfma16(__builtin_bit_cast(v8, e), pf, acc[b * PL + 2 * i]);
-                acc[b * PL + 2 * i + 1] = T::mfma16(__builtin_bit_cast(v8, o), pf, acc[b * PL + 2 * i + 1]);
+                for (int i = 0; i < PL / 2; i++) {
+                    const u4 e = {lo16(w[0][i], w[1][i]), lo16(w[2][i], w[3][i]), lo16(w[4][i], w[5][i]), lo16(w[6][i], w[7][i])};
+                    const u4 o = {hi16(w[0][i], w[1][i]), hi16(w[2][i], w[3][i]), hi16(w[4][i], w[5][i]), hi16(w[6][i], w[7][i])};
+                    acc[b * PL + 2 * i] = T::mfma16(__builtin_bit_cast(v8, e), pf[k], acc[b * PL + 2 * i]);
+                    acc[b * PL + 2 * i + 1] = T::mfma16(__builtin_bit_cast(v8, o), pf[k], acc[b * PL + 2 * i + 1]);
+                }
             }
-        }
+        };
+        if (whole) sums(std::true_type{});
+        else sums(std::false_type{});
     }
     /* an infinity or NaN among rows that some columns do not attend would reach them as 0 * inf:
      * left out above, added here to the columns that do attend it */
     if (__any(odd)) {
-        for (int t0 = first; t0 < stop; t0 += FEW_STEP * FEW_WAVES) {
-            const Tile x[2] = {tile_at(t0), tile_at(t0 + 16)};
-            if (whole_at(t0, x)) continue;   /* a step taken as it is */
+        auto run_at = [&](int t) { return checked(look(t, block_at(t))); };
+        for (int t0 = first; t0 < stop; t0 += ROUND) {
+            Run x[NL];
+#pragma unroll
+            for (int z = 0; z < NL; z++) x[z] = run_at(t0 + RUN * z);
+            if (whole_at(x)) continue;   /* a step taken as it is */
 #pragma unroll 1
-            for (int z = 0; z < 32; z++) {
-                const int id = z < 16 ? x[0].page : x[1].page, t = (z < 16 ? x[0].row : x[1].row) + (z & 15);
+            for (int z = 0; z < STEP; z++) {
+                const Run y = run_at(t0 + (z & -RUN));
+                const int id = y.page, t = y.row + (z & (RUN - 1));
                 if (id < 0 || t >= hi) continue;
                 const uint8_t *row = vbase + (int64_t)id * a.v.page_stride + (int64_t)(t & (page_rows - 1)) * F::RB;
                 const uint8_t *sc = MX ? vsb + (int64_t)id * a.v.scale_page_stride + (t & (page_rows - 1)) * (D / MX_BLOCK) : nullptr;
@@ -510,7 +563,10 @@ template <class T, int BITS, int D, bool BLOCKS>
 void few_t(const AttendArgs &a, hipStream_t st) {
     const int tiles = BLOCKS ? a.b.max_q * ((a.group + 15) / 16) : (a.b.max_q * a.group + 15) / 16;
     const dim3 grid((unsigned)a.n_splits * a.kv_heads * tiles, 1, a.b.n_seqs);
-    hipLaunchKernelGGL((k_attend_few<T, BITS, D, BLOCKS>), grid, dim3(64 * FEW_WAVES), 0, st, a);
+    constexpr int STEP = Few<T, BITS, D>::STEP;
+    const bool one = 1 << a.b.page_shift >= STEP && (!BLOCKS || 1 << a.block_shift >= STEP);
+    if (one) hipLaunchKernelGGL((k_attend_few<T, BITS, D, BLOCKS, true>), grid, dim3(64 * FEW_WAVES), 0, st, a);
+    else hipLaunchKernelGGL((k_attend_few<T, BITS, D, BLOCKS, false>), grid, dim3(64 * FEW_WAVES), 0, st, a);
 }
 
 template <class T, int DV>
@@ -540,7 +596,7 @@ static bool takes_many(int64_t cols) { return cols > 32; }
 Split attend_split(int n_seqs, int max_q, int kv_cap, int heads, int kv_heads, bool latent) {
     const int64_t cols = (int64_t)max_q * (heads / kv_heads);
     const bool many = !latent && takes_many(cols);
-    const int tile = latent ? 64 : many ? 128 : 16, step = latent ? 64 : FEW_STEP * FEW_WAVES, at_once = latent ? 256 : 512;
+    const int tile = latent ? 64 : many ? 128 : 16, step = latent ? 64 : 128, at_once = latent ? 256 : 512;
     const int64_t wgs = std::max<int64_t>((int64_t)n_seqs * kv_heads * ((cols + tile - 1) / tile), 1);
     const int64_t want = std::max<int64_t>(1, at_once / wgs);
     int64_t chunk = (kv_cap + want - 1) / want;
@@ -551,7 +607,7 @@ Split attend_split(int n_seqs, int max_q, int kv_cap, int heads, int kv_heads, b
 /* As attend_split; a unit is a token and 16 of a kv head's query heads */
 Split blocks_split(int n_seqs, int max_q, int rows, int heads, int kv_heads) {
     const int64_t wgs = std::max<int64_t>((int64_t)n_seqs * kv_heads * max_q * ((heads / kv_heads + 15) / 16), 1);
-    const int64_t want = std::max<int64_t>(1, 512 / wgs), step = FEW_STEP * FEW_WAVES;
+    const int64_t want = std::max<int64_t>(1, 512 / wgs), step = 128;
     int64_t chunk = (rows + want - 1) / want;
     chunk = std::max<int64_t>((chunk + step - 1) / step * step, 512);
     return {(int)chunk, (int)((rows + chunk - 1) / chunk), false};
