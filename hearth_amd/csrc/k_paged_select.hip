@@ -18,6 +18,7 @@ namespace hxp {
 namespace {
 
 typedef int i4 __attribute__((ext_vector_type(4)));
+typedef unsigned short us2 __attribute__((ext_vector_type(2)));
 
 /* The step of whole numbers up to 127 for magnitudes up to m, as exponent + 127: the least with m <= 127 *
  * 2^e = 1.984375 * 2^(e + 6) */
@@ -134,17 +135,22 @@ __global__ __launch_bounds__(BOUND_THREADS) void k_key_bounds(BoundsArgs a) {
 
 /* ---------------------------------------------------------------- scores
  *
- * S = B Q^T: rows are blocks, a matrix instruction takes 16, columns (token, head) pairs of a kv head's group,
- * 16 a workgroup (TPT tokens of up to 16 heads, or one token of more, 16 heads at a time from LDS). A lane
- * ends with four blocks of one column; the maximum over a token's columns goes through LDS. */
+ * S = Q B^T, 16 rows a workgroup: the (token, head) pairs of one kv head, each token's heads padded to a power of two P
+ * (the last once more, which changes no maximum), so 16 / P tokens, or one token of more than 16 heads, 16 at a time from
+ * LDS. Columns are blocks, 16 a matrix instruction: a lane ends with four rows of one block, whose maximum over a
+ * token's heads is taken in its registers and with the lanes 16 and 32 further. A wave's instructions bound
+ * it (rows and columns the other way round, with the maximum between neighbouring lanes, took 21 us for 600 tokens
+ * over 313 blocks). */
 constexpr int SCORE_WAVES = 4, MAX_CHUNKS = 8;
+
+/* heads of a token in a tile of 16 rows */
+__host__ __device__ inline int padded(int group) { return group > 8 ? 16 : group > 4 ? 8 : group > 2 ? 4 : group; }
 
 template <class T, int D, bool ONE>
 __global__ __launch_bounds__(64 * SCORE_WAVES) void k_block_scores(SelectArgs a) {
     constexpr int KS = D / 64;
     constexpr float NINF = -__builtin_huge_valf();
-    struct Cols { i4 up[KS], down[KS]; int byte; };
-    __shared__ __align__(16) float lds_s[SCORE_WAVES][16][20];
+    struct Rows16 { i4 up[KS], down[KS]; int byte; };
     __shared__ __align__(16) i4 lds_q[ONE ? 1 : MAX_CHUNKS][ONE ? 1 : 2 * KS][ONE ? 1 : 64];
     __shared__ int lds_b[ONE ? 1 : MAX_CHUNKS][16];
 
@@ -155,7 +161,7 @@ __global__ __launch_bounds__(64 * SCORE_WAVES) void k_block_scores(SelectArgs a)
     const int h = bx % a.kv_heads, tile = bx / a.kv_heads;
     const int seq = blockIdx.z;
     const Seq q = seq_of(a.b, seq);
-    const int n = min(q.n, a.b.max_q), cols = ONE ? a.group : 16, tpt = ONE ? 16 / a.group : 1, t0 = tile * tpt;
+    const int n = min(q.n, a.b.max_q), pad = ONE ? padded(a.group) : 16, tpt = 16 / pad, t0 = tile * tpt;
     if (t0 >= n) return;
     const int64_t last = min((int64_t)q.base + min(t0 + tpt, n) - 1, (int64_t)q.kv - 1);   /* the last token's last row */
     if (last < 0) return;
@@ -163,206 +169,282 @@ __global__ __launch_bounds__(64 * SCORE_WAVES) void k_block_scores(SelectArgs a)
     const int lo = chunk * a.chunk, hi = min(nb, lo + a.chunk);
     if (lo >= hi) return;
 
-    /* lane's column of heads h0 .. */
-    auto quantise = [&](int tl, int head, bool on) {
-        Cols c;
+    const int *pages = a.b.pages + (int64_t)seq * a.b.ld_pages;
+    const int per_page = a.b.page_shift - a.s.block_shift;
+    constexpr int STEP = 16 * SCORE_WAVES;
+    const int first = lo + 16 * wave;
+    /* page of this lane's block of the sixteen from b0 on (-1: none); its bounds */
+    auto page_of = [&](int b0) __attribute__((always_inline)) { return b0 + lc < hi ? pages[(b0 + lc) >> per_page] : -1; };
+    struct Codes { i4 low[KS], high[KS]; int byte; } next;
+    const uint8_t *codes = a.s.codes + (int64_t)h * a.s.head_stride, *scales = a.s.scales + (int64_t)h * a.s.scale_head_stride;
+    auto load = [&](int b0, int id) __attribute__((always_inline)) {
+        const bool there = page_ok(a.b, id);
+        const int64_t page = there ? id : 0;
+        const int sub = (b0 + lc) & (a.s.blocks - 1);
+        const uint8_t *p = codes + page * a.s.page_stride + sub * (2 * D) + 16 * g;
+#pragma unroll
+        for (int i = 0; i < KS; i++) { next.low[i] = *(const i4 *)(p + 64 * i); next.high[i] = *(const i4 *)(p + D + 64 * i); }
+        const int byte = scales[page * a.s.scale_page_stride + sub];
+        next.byte = there ? byte : -1;
+    };
+    const int id0 = page_of(first), id1 = page_of(first + STEP);
+
+    /* A lane's part of a row, 16 elements of each 64, as whole numbers: v * r + 3 * 2^22 rounds v / step to
+     * nearest even into the low byte of the float's bits (two's complement, |v| * r <= 127.5). */
+    auto quantise = [&](int tl, int head, bool on) __attribute__((always_inline)) {
+        Rows16 c;
         const int tok = on ? t0 + tl : 0;
         const uint8_t *p = a.q + (int64_t)(q.q0 + tok) * a.qt + (int64_t)(h * a.group + head) * a.qh;
-        float v[KS][16];
-        float m = 0.0f;
+        u4 w[KS][2];
 #pragma unroll
         for (int i = 0; i < KS; i++)
 #pragma unroll
             for (int z = 0; z < 2; z++) {
-                u4 w = {0, 0, 0, 0};
-                if (on) w = *(const u4_any *)(p + 2 * (64 * i + 16 * g + 8 * z));
-                const typename T::v8 x = __builtin_bit_cast(typename T::v8, w);
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    v[i][8 * z + j] = finite_or_0((float)x[j]);
-                    m = fmaxf(m, __builtin_fabsf(v[i][8 * z + j]));
-                }
+                w[i][z] = (u4){0, 0, 0, 0};
+                if (on) w[i][z] = *(const u4_any *)(p + 2 * (64 * i + 16 * g + 8 * z));
             }
-        m = max16(max32(m));
+        /* magnitudes of 16-bit floats order like their bits: two at once */
+        us2 top = {0, 0};
+        auto largest = [&] {
+            top = (us2){0, 0};
+#pragma unroll
+            for (int i = 0; i < KS; i++)
+#pragma unroll
+                for (int z = 0; z < 8; z++) top = __builtin_elementwise_max(top, __builtin_bit_cast(us2, w[i][z >> 2][z & 3] & 0x7fff7fffu));
+        };
+        largest();
+        constexpr unsigned short INF = std::is_same_v<T, Bf16> ? 0x7f80 : 0x7c00;
+        if (__any(top[0] >= INF || top[1] >= INF)) {
+#pragma unroll
+            for (int i = 0; i < KS; i++)
+#pragma unroll
+                for (int z = 0; z < 8; z++) w[i][z >> 2][z & 3] = T::clean(w[i][z >> 2][z & 3]);
+            largest();
+        }
+        const float m = max16(max32(T::wide(max(top[0], top[1]))));
         c.byte = step_byte(m);
         const float r = per_step(c.byte);
 #pragma unroll
         for (int i = 0; i < KS; i++)
 #pragma unroll
             for (int z = 0; z < 4; z++) {
-                unsigned up = 0, down = 0;
+                unsigned b[4];
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
-                    const int x = (int)rintf(v[i][4 * z + j] * r);
-                    up |= (unsigned)max(x, 0) << (8 * j);
-                    down |= ((unsigned)min(x, 0) & 255u) << (8 * j);
+                    const unsigned x = w[i][z >> 1][2 * (z & 1) + (j >> 1)];
+                    const float v = T::wide(j & 1 ? x >> 16 : x);
+                    b[j] = __float_as_uint(__builtin_fmaf(v, r, 12582912.0f));
                 }
-                c.up[i][z] = (int)up;
-                c.down[i][z] = (int)down;
+                const unsigned lo = __builtin_amdgcn_perm(b[1], b[0], 0x0c0c0400u), hi = __builtin_amdgcn_perm(b[3], b[2], 0x04000c0cu), x = lo | hi;
+                const unsigned sign = x >> 7 & 0x01010101u, below = (sign << 8) - sign;   /* 255 in the bytes below 0 */
+                c.up[i][z] = (int)(x & ~below);
+                c.down[i][z] = (int)(x & below);
             }
         return c;
     };
-    Cols mine;
+    Rows16 mine;
     const int chunks = (a.group + 15) / 16;
     if constexpr (ONE) {
-        const int tl = lc / cols;
-        mine = quantise(tl, lc % cols, tl < tpt && t0 + tl < n);
+        const int tl = lc / pad;
+        mine = quantise(tl, min(lc % pad, a.group - 1), t0 + tl < n);
     } else {
         for (int c = wave; c < chunks; c += SCORE_WAVES) {
-            const int head = 16 * c + lc;
-            const Cols x = quantise(0, min(head, a.group - 1), true);   /* heads past the group: the last once more */
+            const Rows16 x = quantise(0, min(16 * c + lc, a.group - 1), true);
 #pragma unroll
             for (int i = 0; i < KS; i++) { lds_q[c][i][lane] = x.up[i]; lds_q[c][KS + i][lane] = x.down[i]; }
             if (g == 0) lds_b[c][lc] = x.byte;
         }
         __syncthreads();
     }
-
-    const int *pages = a.b.pages + (int64_t)seq * a.b.ld_pages;
-    const int per_page = a.b.page_shift - a.s.block_shift;
-    for (int b0 = lo + 16 * wave; b0 < hi; b0 += 16 * SCORE_WAVES) {
-        const int blk = b0 + lc;
-        int page = blk < hi ? pages[blk >> per_page] : -1;
-        const bool there = page_ok(a.b, page);
-        page = there ? page : 0;
-        const int sub = blk & (a.s.blocks - 1);
-        const uint8_t *p = a.s.codes + (int64_t)page * a.s.page_stride + (int64_t)h * a.s.head_stride + (int64_t)sub * (2 * D) + 16 * g;
-        i4 low[KS], high[KS];
+    if (first < hi) load(first, id0);
+    int id = id1;
+    /* the lane's four rows: their steps, and where the first one's token's scores go */
+    int eq[4];
 #pragma unroll
-        for (int i = 0; i < KS; i++) { low[i] = *(const i4 *)(p + 64 * i); high[i] = *(const i4 *)(p + D + 64 * i); }
-        const int eb = there ? (int)a.s.scales[(int64_t)page * a.s.scale_page_stride + (int64_t)h * a.s.scale_head_stride + sub] : -1;
-        int e[4];
-#pragma unroll
-        for (int j = 0; j < 4; j++) e[j] = __shfl(eb, 4 * g + j);
-        f4 s = {NINF, NINF, NINF, NINF};
-        auto take = [&](const i4 (&up)[KS], const i4 (&down)[KS], int byte) {
+    for (int j = 0; j < 4; j++) eq[j] = ONE ? __shfl(mine.byte, 4 * g + j) : 0;
+    const int tl = 4 * g / pad, writers = pad <= 4 ? 4 : 16 / pad;   /* of a tile's g, every 4 / writers-th writes */
+    const int64_t ld_tok = (int64_t)a.kv_heads * a.ld_score;
+    float *out = a.score + (int64_t)(q.q0 + t0 + tl) * ld_tok + (int64_t)h * a.ld_score + lc;
+    const bool writes = g % (4 / writers) == 0 && t0 + tl < n;
+    /* a step's bounds are sent for a step ahead, its page ids two */
+    for (int b0 = first; b0 < hi; b0 += STEP) {
+        const Codes now = next;
+        if (b0 + STEP < hi) load(b0 + STEP, id);
+        id = page_of(b0 + 2 * STEP);
+        float s[4] = {NINF, NINF, NINF, NINF};
+        auto take = [&](const i4 (&up)[KS], const i4 (&down)[KS], const int (&step)[4]) __attribute__((always_inline)) {
             i4 acc = {0, 0, 0, 0};
 #pragma unroll
             for (int i = 0; i < KS; i++) {
-                acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(high[i], up[i], acc, 0, 0, 0);
-                acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(low[i], down[i], acc, 0, 0, 0);
+                acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(up[i], now.high[i], acc, 0, 0, 0);
+                acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(down[i], now.low[i], acc, 0, 0, 0);
             }
 #pragma unroll
-            for (int j = 0; j < 4; j++) s[j] = fmaxf(s[j], __builtin_ldexpf((float)acc[j], e[j] + byte - 254));
+            for (int j = 0; j < 4; j++) {
+                const float x = __builtin_ldexpf((float)acc[j], now.byte + step[j] - 254);
+                s[j] = ONE ? x : fmaxf(s[j], x);
+            }
         };
-        if constexpr (ONE) take(mine.up, mine.down, mine.byte);
+        if constexpr (ONE) take(mine.up, mine.down, eq);
         else
             for (int c = 0; c < chunks; c++) {
                 i4 up[KS], down[KS];
+                int step[4];
 #pragma unroll
                 for (int i = 0; i < KS; i++) { up[i] = lds_q[c][i][lane]; down[i] = lds_q[c][KS + i][lane]; }
-                take(up, down, lds_b[c][lc]);
+#pragma unroll
+                for (int j = 0; j < 4; j++) step[j] = lds_b[c][4 * g + j];
+                take(up, down, step);
             }
-        *(f4 *)&lds_s[wave][lc][4 * g] = s;
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        for (int o = lane; o < 16 * tpt; o += 64) {
-            const int tl = o >> 4, b = o & 15;
-            if (t0 + tl >= n || b0 + b >= hi) continue;
-            float m = lds_s[wave][tl * cols][b];
-            for (int c = 1; c < cols; c++) m = fmaxf(m, lds_s[wave][tl * cols + c][b]);
-            /* -infinity tells a block whose page is not there; an overflow stays above it */
-            m = eb < 0 ? NINF : fmaxf(m, -3.4028234e38f);   /* b is lc: this lane's block */
-            a.score[((int64_t)(q.q0 + t0 + tl) * a.kv_heads + h) * a.ld_score + b0 + b] = m;
+        /* -infinity tells a block whose page is not there; an overflow stays above it */
+        auto put = [&](int t, float x) __attribute__((always_inline)) {
+            if (b0 + lc < hi) out[t * ld_tok + b0] = now.byte < 0 ? NINF : fmaxf(x, -3.4028234e38f);
+        };
+        if (pad >= 4) {
+            float m = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
+            if (pad >= 8) m = max16(m);
+            if (pad == 16) m = max32(m);
+            if (writes) put(0, m);
+        } else if (writes) {
+            if (pad == 2) {
+                put(0, fmaxf(s[0], s[1]));
+                if (t0 + tl + 1 < n) put(1, fmaxf(s[2], s[3]));
+            } else
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    if (t0 + tl + j < n) put(j, s[j]);
         }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
 }
 
 /* ---------------------------------------------------------------- the best of a token
  *
- * A workgroup takes one token and kv head. Keys are the scores' bits in an order of unsigned numbers, the
- * greatest for blocks that are kept in any case, 0 for those that cannot be taken. The top-th greatest key is found
- * eight bits at a time by counting; then every wave counts what it takes of its quarter of the blocks
- * (keys above, and of those equal the first ones) and writes it behind the quarters before. */
-constexpr int PICK_THREADS = 256;
+ * A workgroup takes one token and kv head, a wave a quarter of the blocks, in order. Keys are the scores' bits in an
+ * order of unsigned numbers, the greatest for blocks that are kept in any case, 0 for those that cannot be taken.
+ * Keys of one row lie close together, so the top-th greatest is looked for within their range: 256 bins over
+ * it, then over the bin that holds it, until the bin is taken whole or holds one value (two rounds in most rows). Then
+ * every wave counts what it takes (keys above, and of those equal the first ones) and writes it behind
+ * the waves before. R: keys of a lane that stay in registers (0: they are read again each time). */
+constexpr int PICK_THREADS = 256, PICK_WAVES = PICK_THREADS / 64;
 
+template <int R>
 __global__ __launch_bounds__(PICK_THREADS) void k_block_pick(SelectArgs a) {
-    __shared__ unsigned bins[256];
-    __shared__ unsigned found[2];                        /* bin, keys above it */
-    __shared__ int above[4], equal[4];
+    __shared__ unsigned bins[2][256];
+    __shared__ unsigned lds_lo[PICK_WAVES], lds_hi[PICK_WAVES];
+    __shared__ int lds_can[PICK_WAVES], lds_kept[PICK_WAVES], above[PICK_WAVES], equal[PICK_WAVES];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int h = blockIdx.x % a.kv_heads, tok = blockIdx.x / a.kv_heads, seq = blockIdx.z;
     const Seq q = seq_of(a.b, seq);
     if (tok >= min(q.n, a.b.max_q)) return;
     const int64_t row = min((int64_t)q.base + tok, (int64_t)q.kv - 1);
     const int n = row < 0 ? 0 : (int)(row >> a.s.block_shift) + 1;
-    int kept = max(n - a.last, 0);                       /* blocks from here on are kept */
-    if (a.b.mask) kept = min(kept, max(q.base, 0) >> a.s.block_shift);
+    int tail = max(n - a.last, 0);                       /* blocks from here on are kept */
+    if (a.b.mask) tail = min(tail, max(q.base, 0) >> a.s.block_shift);
     const float *score = a.score + ((int64_t)(q.q0 + tok) * a.kv_heads + h) * a.ld_score;
-    auto key = [&](int i) -> unsigned {
-        const float s = score[i];
-        if (s == -__builtin_huge_valf()) return 0u;
-        if (i < a.first || i >= kept) return ~0u;
+    const int per = (n + PICK_WAVES - 1) / PICK_WAVES, from = min(wave * per, n), to = min(from + per, n);
+    auto fetch = [&](int i) __attribute__((always_inline)) -> unsigned {   /* of block from + i of the wave */
+        if (from + i >= to) return 0u;
+        const float s = score[from + i];
         const unsigned u = __float_as_uint(s);
-        return u & 0x80000000u ? ~u : u | 0x80000000u;
+        if (s == -__builtin_huge_valf()) return 0u;
+        return from + i < a.first || from + i >= tail ? ~0u : u & 0x80000000u ? ~u : u | 0x80000000u;
     };
+    unsigned mine[R ? R : 1];
+    if constexpr (R != 0) {
+#pragma unroll
+        for (int i = 0; i < R; i++) mine[i] = fetch(64 * i + lane);
+    }
+    auto keys = [&](auto f) __attribute__((always_inline)) {   /* f(index in the wave's quarter, key), 64 lanes at once */
+        if constexpr (R != 0) {
+#pragma unroll
+            for (int i = 0; i < R; i++) f(64 * i, mine[i]);
+        } else
+            for (int i = 0; from + i < to; i += 64) f(i, fetch(i + lane));
+    };
+    for (int i = threadIdx.x; i < 2 * 256; i += PICK_THREADS) bins[i >> 8][i & 255] = 0;
+    unsigned lo = ~0u, hi = 0;
+    int can = 0, kept = 0;
+    keys([&](int, unsigned k) {
+        can += __popcll(__ballot(k != 0));
+        kept += __popcll(__ballot(k == ~0u));
+        if (k && k != ~0u) { lo = min(lo, k); hi = max(hi, k); }
+    });
+#pragma unroll
+    for (int d = 32; d; d >>= 1) {
+        lo = min(lo, (unsigned)__shfl_xor((int)lo, d));
+        hi = max(hi, (unsigned)__shfl_xor((int)hi, d));
+    }
+    if (lane == 0) { lds_lo[wave] = lo; lds_hi[wave] = hi; lds_can[wave] = can; lds_kept[wave] = kept; }
+    __syncthreads();
+    static_assert(PICK_WAVES == 4);
+    lo = min(min(lds_lo[0], lds_lo[1]), min(lds_lo[2], lds_lo[3]));
+    hi = max(max(lds_hi[0], lds_hi[1]), max(lds_hi[2], lds_hi[3]));
+    can = lds_can[0] + lds_can[1] + lds_can[2] + lds_can[3];
+    kept = lds_kept[0] + lds_kept[1] + lds_kept[2] + lds_kept[3];
     unsigned limit = 0;          /* keys above it are taken, and `ties` of those equal to it */
-    int ties = 0;
-    if (n > a.top) {
-        unsigned prefix = 0, mask = 0;
-        int left = a.top;        /* to be taken of the keys with the prefix */
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            bins[threadIdx.x] = 0;
-            __syncthreads();
-            for (int i = threadIdx.x; i < n; i += PICK_THREADS) {
-                const unsigned k = key(i);
-                if ((k & mask) == prefix) atomicAdd(&bins[k >> shift & 255u], 1u);
-            }
-            __syncthreads();
-            if (threadIdx.x < 64) {   /* four bins a lane, the greatest first */
-                const int l = threadIdx.x;
+    int ties = 0, left = a.top - kept;   /* to be taken within [lo, hi] */
+    if (can > a.top) {
+        if (left <= 0) limit = ~0u - 1;
+        else
+            for (int round = 0;; round ^= 1) {
+                const int shift = max(24 - __builtin_clz(hi - lo | 1u), 0);   /* (hi - lo) >> shift < 256 */
+                keys([&](int, unsigned k) {
+                    if (k >= lo && k <= hi) atomicAdd(&bins[round][(k - lo) >> shift], 1u);
+                });
+                __syncthreads();
+                /* every wave alike: four bins a lane, the greatest first */
                 unsigned c[4], sum = 0;
 #pragma unroll
-                for (int j = 0; j < 4; j++) { c[j] = bins[255 - 4 * l - j]; sum += c[j]; }
+                for (int j = 0; j < 4; j++) { c[j] = bins[round][255 - 4 * lane - j]; sum += c[j]; }
                 unsigned upto = sum;
 #pragma unroll
                 for (int d = 1; d < 64; d <<= 1) {
-                    const unsigned x = __shfl_up(upto, d);
-                    if (l >= d) upto += x;
+                    const unsigned x = (unsigned)__shfl_up((int)upto, d);
+                    if (lane >= d) upto += x;
                 }
-                unsigned before = upto - sum;
+                unsigned before = upto - sum, bin = 0, over = 0, in = 0;
+                bool here = false;
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
-                    if (before < (unsigned)left && before + c[j] >= (unsigned)left) { found[0] = 255 - 4 * l - j; found[1] = before; }
+                    if (before < (unsigned)left && before + c[j] >= (unsigned)left) { here = true; bin = 255 - 4 * lane - j; over = before; in = c[j]; }
                     before += c[j];
                 }
+                const int who = __ffsll((long long)__ballot(here)) - 1;
+                bin = (unsigned)__builtin_amdgcn_readlane((int)bin, who);
+                left -= __builtin_amdgcn_readlane((int)over, who);
+                in = (unsigned)__builtin_amdgcn_readlane((int)in, who);
+                lo += bin << shift;
+                if (in == (unsigned)left) { limit = lo - 1; break; }
+                if (shift == 0) { limit = lo; ties = left; break; }
+                hi = min(hi, lo + (1u << shift) - 1);
+                /* the other set of bins is clear; this one is for the round after the next */
+                __syncthreads();
+                bins[round][threadIdx.x] = 0;
             }
-            __syncthreads();
-            prefix |= found[0] << shift;
-            mask |= 255u << shift;
-            left -= (int)found[1];
-            __syncthreads();
-        }
-        limit = prefix;
-        ties = limit ? left : 0;   /* keys of 0 are not taken */
     }
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const int per = (n + 3) / 4, from = min(wave * per, n), to = min(from + per, n);
     int na = 0, ne = 0;
-    for (int i = from; i < to; i += 64) {
-        const unsigned k = i + lane < to ? key(i + lane) : 0u;
+    keys([&](int, unsigned k) {
         na += __popcll(__ballot(k > limit));
-        ne += __popcll(__ballot(k == limit && k && i + lane < to));
-    }
+        ne += __popcll(__ballot(k == limit && k));
+    });
     if (lane == 0) { above[wave] = na; equal[wave] = ne; }
     __syncthreads();
     int *out = a.chosen + (int64_t)(q.q0 + tok) * a.ct + (int64_t)h * a.ch;
     int at = 0, eq = 0, total = 0;
 #pragma unroll
-    for (int w = 0; w < 4; w++) {
+    for (int w = 0; w < PICK_WAVES; w++) {
         if (w < wave) { at += above[w]; eq += equal[w]; }
         total += above[w];
     }
     total += min(ties, equal[0] + equal[1] + equal[2] + equal[3]);
     const unsigned long long before = (1ull << lane) - 1;
-    for (int i = from; i < to; i += 64) {
-        const unsigned k = i + lane < to ? key(i + lane) : 0u;
-        const unsigned long long ma = __ballot(k > limit), me = __ballot(k == limit && k && i + lane < to);
+    keys([&](int i, unsigned k) {
+        const unsigned long long ma = __ballot(k > limit), me = __ballot(k == limit && k);
         const int e = eq + __popcll(me & before);
-        const bool take = k > limit || ((me >> lane & 1) && e < ties);
-        if (take) out[at + __popcll(ma & before) + min(e, ties)] = i + lane;
+        if (k > limit || (k == limit && k && e < ties)) out[at + __popcll(ma & before) + min(e, ties)] = from + i + lane;
         at += __popcll(ma);
         eq += __popcll(me);
-    }
+    });
     for (int i = total + (int)threadIdx.x; i < a.top; i += PICK_THREADS) out[i] = -1;
 }
 
@@ -376,7 +458,7 @@ void bounds_t(const BoundsArgs &a, int width, hipStream_t st) {
 
 template <class T, int D>
 void scores_t(const SelectArgs &a, hipStream_t st) {
-    const int tiles = a.group <= 16 ? (a.b.max_q + 16 / a.group - 1) / (16 / a.group) : a.b.max_q;
+    const int tpt = a.group <= 16 ? 16 / padded(a.group) : 1, tiles = (a.b.max_q + tpt - 1) / tpt;
     const dim3 grid((unsigned)((int64_t)tiles * a.n_chunks * a.kv_heads), 1, a.b.n_seqs), block(64 * SCORE_WAVES);
     if (a.group <= 16) hipLaunchKernelGGL((k_block_scores<T, D, true>), grid, block, 0, st, a);
     else hipLaunchKernelGGL((k_block_scores<T, D, false>), grid, block, 0, st, a);
@@ -395,14 +477,18 @@ int select_group_limit() { return 16 * MAX_CHUNKS; }
 
 /* Blocks are shared out among workgroups until two are there for each unit, 64 at least each (16 a wave) */
 void select_blocks(SelectArgs a, int q_dtype, int width, int n_blocks, hipStream_t st) {
-    const int tpt = a.group <= 16 ? 16 / a.group : 1;
+    const int tpt = a.group <= 16 ? 16 / padded(a.group) : 1;
     const int64_t wgs = (int64_t)a.b.n_seqs * a.kv_heads * ((a.b.max_q + tpt - 1) / tpt);
     const int64_t want = std::max<int64_t>(1, 512 / wgs);
     a.chunk = (int)(((n_blocks + want - 1) / want + 63) / 64 * 64);
     a.n_chunks = (n_blocks + a.chunk - 1) / a.chunk;
     if (q_dtype == DT_BF16) width == 64 ? scores_t<Bf16, 64>(a, st) : width == 128 ? scores_t<Bf16, 128>(a, st) : scores_t<Bf16, 256>(a, st);
     else width == 64 ? scores_t<F16, 64>(a, st) : width == 128 ? scores_t<F16, 128>(a, st) : scores_t<F16, 256>(a, st);
-    hipLaunchKernelGGL(k_block_pick, dim3((unsigned)((int64_t)a.b.max_q * a.kv_heads), 1, a.b.n_seqs), dim3(PICK_THREADS), 0, st, a);
+    const dim3 rows((unsigned)((int64_t)a.b.max_q * a.kv_heads), 1, a.b.n_seqs), threads(PICK_THREADS);
+    if (n_blocks <= 2 * PICK_THREADS) hipLaunchKernelGGL(k_block_pick<2>, rows, threads, 0, st, a);
+    else if (n_blocks <= 8 * PICK_THREADS) hipLaunchKernelGGL(k_block_pick<8>, rows, threads, 0, st, a);
+    else if (n_blocks <= 32 * PICK_THREADS) hipLaunchKernelGGL(k_block_pick<32>, rows, threads, 0, st, a);
+    else hipLaunchKernelGGL(k_block_pick<0>, rows, threads, 0, st, a);
 }
 
 } // namespace hxp
