@@ -146,11 +146,115 @@ constexpr int SCORE_WAVES = 4, MAX_CHUNKS = 8;
 /* heads of a token in a tile of 16 rows */
 __host__ __device__ inline int padded(int group) { return group > 8 ? 16 : group > 4 ? 8 : group > 2 ? 4 : group; }
 
+/* Sixteen rows of queries as whole numbers: a lane's row lc, 16 elements of each 64 (from 16 g on), positive and negative
+ * parts, and the step */
+template <int KS> struct Rows16 { i4 up[KS], down[KS]; int byte; };
+
+/* p: a lane's row. v * r + 3 * 2^22 rounds v / step to nearest even into the low byte of the float's bits (two's
+ * complement, |v| * r <= 127). */
+template <class T, int KS>
+__device__ __forceinline__ Rows16<KS> quantise(const uint8_t *p, int g, bool on) {
+    Rows16<KS> c;
+    u4 w[KS][2];
+#pragma unroll
+    for (int i = 0; i < KS; i++)
+#pragma unroll
+        for (int z = 0; z < 2; z++) {
+            w[i][z] = (u4){0, 0, 0, 0};
+            if (on) w[i][z] = *(const u4_any *)(p + 2 * (64 * i + 16 * g + 8 * z));
+        }
+    /* magnitudes of 16-bit floats order like their bits: two at once */
+    us2 top = {0, 0};
+    auto largest = [&] {
+        top = (us2){0, 0};
+#pragma unroll
+        for (int i = 0; i < KS; i++)
+#pragma unroll
+            for (int z = 0; z < 8; z++) top = __builtin_elementwise_max(top, __builtin_bit_cast(us2, w[i][z >> 2][z & 3] & 0x7fff7fffu));
+    };
+    largest();
+    constexpr unsigned short INF = std::is_same_v<T, Bf16> ? 0x7f80 : 0x7c00;
+    if (__any(top[0] >= INF || top[1] >= INF)) {
+#pragma unroll
+        for (int i = 0; i < KS; i++)
+#pragma unroll
+            for (int z = 0; z < 8; z++) w[i][z >> 2][z & 3] = T::clean(w[i][z >> 2][z & 3]);
+        largest();
+    }
+    const float m = max16(max32(T::wide(max(top[0], top[1]))));
+    c.byte = step_byte(m);
+    const float r = per_step(c.byte);
+#pragma unroll
+    for (int i = 0; i < KS; i++)
+#pragma unroll
+        for (int z = 0; z < 4; z++) {
+            unsigned b[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const unsigned x = w[i][z >> 1][2 * (z & 1) + (j >> 1)];
+                const float v = T::wide(j & 1 ? x >> 16 : x);
+                b[j] = __float_as_uint(__builtin_fmaf(v, r, 12582912.0f));
+            }
+            const unsigned lo = __builtin_amdgcn_perm(b[1], b[0], 0x0c0c0400u), hi = __builtin_amdgcn_perm(b[3], b[2], 0x04000c0cu), x = lo | hi;
+            const unsigned sign = x >> 7 & 0x01010101u, below = (sign << 8) - sign;   /* 255 in the bytes below 0 */
+            c.up[i][z] = (int)(x & ~below);
+            c.down[i][z] = (int)(x & below);
+        }
+    return c;
+}
+
+/* What becomes of a lane's four rows (rows 4 g .. of tokens of `pad` heads each) of one block: the token's maxima into `out`,
+ * the first token's place of this block. -infinity tells a block whose page is not there; an overflow stays above it. */
+struct Put {
+    float *out;
+    int64_t ld_tok;
+    int pad, left;      /* tokens from the lane's first one on */
+    bool writes;
+    __device__ __forceinline__ Put(const SelectArgs &a, const Seq &q, int h, int pad, int t0, int n, int g) : pad(pad) {
+        const int tl = 4 * g / pad, each_g = pad <= 4 ? 1 : pad / 4;
+        ld_tok = (int64_t)a.kv_heads * a.ld_score;
+        out = a.score + (int64_t)(q.q0 + t0 + tl) * ld_tok + (int64_t)h * a.ld_score;
+        left = n - t0 - tl;
+        writes = g % each_g == 0 && left > 0;
+    }
+    __device__ __forceinline__ void operator()(int blk, bool there, bool inside, const float (&s)[4]) const {
+        auto put = [&](int t, float x) __attribute__((always_inline)) {
+            if (inside) out[t * ld_tok + blk] = there ? fmaxf(x, -3.4028234e38f) : -__builtin_huge_valf();
+        };
+        if (pad >= 4) {
+            float m = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
+            if (pad >= 8) m = max16(m);
+            if (pad == 16) m = max32(m);
+            if (writes) put(0, m);
+        } else if (writes) {
+            if (pad == 2) {
+                put(0, fmaxf(s[0], s[1]));
+                if (left > 1) put(1, fmaxf(s[2], s[3]));
+            } else
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    if (left > j) put(j, s[j]);
+        }
+    }
+};
+
+/* 16 rows against 16 blocks; step: of the lane's four rows, byte: of its block */
+template <int KS>
+__device__ __forceinline__ void score16(const i4 (&up)[KS], const i4 (&down)[KS], const i4 (&high)[KS], const i4 (&low)[KS], const int (&step)[4], int byte,
+                                        float (&s)[4]) {
+    i4 acc = {0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < KS; i++) {
+        acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(up[i], high[i], acc, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(down[i], low[i], acc, 0, 0, 0);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; j++) s[j] = __builtin_ldexpf((float)acc[j], byte + step[j] - 254);
+}
+
 template <class T, int D, bool ONE>
 __global__ __launch_bounds__(64 * SCORE_WAVES) void k_block_scores(SelectArgs a) {
     constexpr int KS = D / 64;
-    constexpr float NINF = -__builtin_huge_valf();
-    struct Rows16 { i4 up[KS], down[KS]; int byte; };
     __shared__ __align__(16) i4 lds_q[ONE ? 1 : MAX_CHUNKS][ONE ? 1 : 2 * KS][ONE ? 1 : 64];
     __shared__ int lds_b[ONE ? 1 : MAX_CHUNKS][16];
 
@@ -189,67 +293,16 @@ __global__ __launch_bounds__(64 * SCORE_WAVES) void k_block_scores(SelectArgs a)
     };
     const int id0 = page_of(first), id1 = page_of(first + STEP);
 
-    /* A lane's part of a row, 16 elements of each 64, as whole numbers: v * r + 3 * 2^22 rounds v / step to
-     * nearest even into the low byte of the float's bits (two's complement, |v| * r <= 127.5). */
-    auto quantise = [&](int tl, int head, bool on) __attribute__((always_inline)) {
-        Rows16 c;
-        const int tok = on ? t0 + tl : 0;
-        const uint8_t *p = a.q + (int64_t)(q.q0 + tok) * a.qt + (int64_t)(h * a.group + head) * a.qh;
-        u4 w[KS][2];
-#pragma unroll
-        for (int i = 0; i < KS; i++)
-#pragma unroll
-            for (int z = 0; z < 2; z++) {
-                w[i][z] = (u4){0, 0, 0, 0};
-                if (on) w[i][z] = *(const u4_any *)(p + 2 * (64 * i + 16 * g + 8 * z));
-            }
-        /* magnitudes of 16-bit floats order like their bits: two at once */
-        us2 top = {0, 0};
-        auto largest = [&] {
-            top = (us2){0, 0};
-#pragma unroll
-            for (int i = 0; i < KS; i++)
-#pragma unroll
-                for (int z = 0; z < 8; z++) top = __builtin_elementwise_max(top, __builtin_bit_cast(us2, w[i][z >> 2][z & 3] & 0x7fff7fffu));
-        };
-        largest();
-        constexpr unsigned short INF = std::is_same_v<T, Bf16> ? 0x7f80 : 0x7c00;
-        if (__any(top[0] >= INF || top[1] >= INF)) {
-#pragma unroll
-            for (int i = 0; i < KS; i++)
-#pragma unroll
-                for (int z = 0; z < 8; z++) w[i][z >> 2][z & 3] = T::clean(w[i][z >> 2][z & 3]);
-            largest();
-        }
-        const float m = max16(max32(T::wide(max(top[0], top[1]))));
-        c.byte = step_byte(m);
-        const float r = per_step(c.byte);
-#pragma unroll
-        for (int i = 0; i < KS; i++)
-#pragma unroll
-            for (int z = 0; z < 4; z++) {
-                unsigned b[4];
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const unsigned x = w[i][z >> 1][2 * (z & 1) + (j >> 1)];
-                    const float v = T::wide(j & 1 ? x >> 16 : x);
-                    b[j] = __float_as_uint(__builtin_fmaf(v, r, 12582912.0f));
-                }
-                const unsigned lo = __builtin_amdgcn_perm(b[1], b[0], 0x0c0c0400u), hi = __builtin_amdgcn_perm(b[3], b[2], 0x04000c0cu), x = lo | hi;
-                const unsigned sign = x >> 7 & 0x01010101u, below = (sign << 8) - sign;   /* 255 in the bytes below 0 */
-                c.up[i][z] = (int)(x & ~below);
-                c.down[i][z] = (int)(x & below);
-            }
-        return c;
-    };
-    Rows16 mine;
+    Rows16<KS> mine;
+    const uint8_t *qp = a.q + (int64_t)(q.q0 + t0) * a.qt + (int64_t)(h * a.group) * a.qh;
     const int chunks = (a.group + 15) / 16;
     if constexpr (ONE) {
         const int tl = lc / pad;
-        mine = quantise(tl, min(lc % pad, a.group - 1), t0 + tl < n);
+        const bool on = t0 + tl < n;
+        mine = quantise<T, KS>(qp + (on ? tl : 0) * a.qt + min(lc % pad, a.group - 1) * a.qh, g, on);
     } else {
         for (int c = wave; c < chunks; c += SCORE_WAVES) {
-            const Rows16 x = quantise(0, min(16 * c + lc, a.group - 1), true);
+            const Rows16<KS> x = quantise<T, KS>(qp + min(16 * c + lc, a.group - 1) * a.qh, g, true);
 #pragma unroll
             for (int i = 0; i < KS; i++) { lds_q[c][i][lane] = x.up[i]; lds_q[c][KS + i][lane] = x.down[i]; }
             if (g == 0) lds_b[c][lc] = x.byte;
@@ -258,62 +311,123 @@ __global__ __launch_bounds__(64 * SCORE_WAVES) void k_block_scores(SelectArgs a)
     }
     if (first < hi) load(first, id0);
     int id = id1;
-    /* the lane's four rows: their steps, and where the first one's token's scores go */
     int eq[4];
 #pragma unroll
     for (int j = 0; j < 4; j++) eq[j] = ONE ? __shfl(mine.byte, 4 * g + j) : 0;
-    const int tl = 4 * g / pad, writers = pad <= 4 ? 4 : 16 / pad;   /* of a tile's g, every 4 / writers-th writes */
-    const int64_t ld_tok = (int64_t)a.kv_heads * a.ld_score;
-    float *out = a.score + (int64_t)(q.q0 + t0 + tl) * ld_tok + (int64_t)h * a.ld_score + lc;
-    const bool writes = g % (4 / writers) == 0 && t0 + tl < n;
+    const Put put(a, q, h, pad, t0, n, g);
     /* a step's bounds are sent for a step ahead, its page ids two */
     for (int b0 = first; b0 < hi; b0 += STEP) {
         const Codes now = next;
         if (b0 + STEP < hi) load(b0 + STEP, id);
         id = page_of(b0 + 2 * STEP);
-        float s[4] = {NINF, NINF, NINF, NINF};
-        auto take = [&](const i4 (&up)[KS], const i4 (&down)[KS], const int (&step)[4]) __attribute__((always_inline)) {
-            i4 acc = {0, 0, 0, 0};
-#pragma unroll
-            for (int i = 0; i < KS; i++) {
-                acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(up[i], now.high[i], acc, 0, 0, 0);
-                acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(down[i], now.low[i], acc, 0, 0, 0);
-            }
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const float x = __builtin_ldexpf((float)acc[j], now.byte + step[j] - 254);
-                s[j] = ONE ? x : fmaxf(s[j], x);
-            }
-        };
-        if constexpr (ONE) take(mine.up, mine.down, eq);
+        float s[4];
+        if constexpr (ONE) score16<KS>(mine.up, mine.down, now.high, now.low, eq, now.byte, s);
         else
             for (int c = 0; c < chunks; c++) {
                 i4 up[KS], down[KS];
                 int step[4];
+                float x[4];
 #pragma unroll
                 for (int i = 0; i < KS; i++) { up[i] = lds_q[c][i][lane]; down[i] = lds_q[c][KS + i][lane]; }
 #pragma unroll
                 for (int j = 0; j < 4; j++) step[j] = lds_b[c][4 * g + j];
-                take(up, down, step);
-            }
-        /* -infinity tells a block whose page is not there; an overflow stays above it */
-        auto put = [&](int t, float x) __attribute__((always_inline)) {
-            if (b0 + lc < hi) out[t * ld_tok + b0] = now.byte < 0 ? NINF : fmaxf(x, -3.4028234e38f);
-        };
-        if (pad >= 4) {
-            float m = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
-            if (pad >= 8) m = max16(m);
-            if (pad == 16) m = max32(m);
-            if (writes) put(0, m);
-        } else if (writes) {
-            if (pad == 2) {
-                put(0, fmaxf(s[0], s[1]));
-                if (t0 + tl + 1 < n) put(1, fmaxf(s[2], s[3]));
-            } else
+                score16<KS>(up, down, now.high, now.low, step, now.byte, x);
 #pragma unroll
-                for (int j = 0; j < 4; j++)
-                    if (t0 + tl + j < n) put(j, s[j]);
+                for (int j = 0; j < 4; j++) s[j] = c ? fmaxf(s[j], x[j]) : x[j];
+            }
+        put(b0 + lc, now.byte >= 0, b0 + lc < hi, s);
+    }
+}
+
+/* Many tokens: four waves with 16 rows each share the bounds of 64 blocks a step, which come in by whole rows of
+ * codes (16 lanes a row of width 128) and through LDS: read by each wave for itself, 16 bytes of a row a lane, they
+ * were bound by the cache lines that a load touches (600 tokens over 313 blocks: 20 us). Pieces of 16 bytes are
+ * exchanged by row, so that 16 lanes that read one piece of 16 rows meet no bank conflict. The next step's
+ * are in flight meanwhile (two buffers). */
+template <class T, int D>
+__global__ __launch_bounds__(64 * SCORE_WAVES) void k_block_scores_many(SelectArgs a) {
+    constexpr int KS = D / 64, PIECES = D / 8, STEP = 16 * SCORE_WAVES, RI = 64 / PIECES, N = 16 / RI;   /* pieces of a row, rows a load instruction, instructions */
+    __shared__ __align__(16) u4 lds[2][STEP * PIECES];
+    __shared__ int lds_b[2][STEP];
+
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, g = lane >> 4, lc = lane & 15;
+    int bx = blockIdx.x;
+    const int chunk = bx % a.n_chunks;
+    bx /= a.n_chunks;
+    const int h = bx % a.kv_heads, tile = bx / a.kv_heads;
+    const int seq = blockIdx.z;
+    const Seq q = seq_of(a.b, seq);
+    const int n = min(q.n, a.b.max_q), pad = padded(a.group), tpt = 16 / pad, first = tile * tpt * SCORE_WAVES, t0 = first + tpt * wave;
+    if (first >= n) return;
+    const int64_t last = min((int64_t)q.base + min(first + tpt * SCORE_WAVES, n) - 1, (int64_t)q.kv - 1);   /* the last token's last row */
+    if (last < 0) return;
+    const int nb = (int)(last >> a.s.block_shift) + 1;
+    const int lo = chunk * a.chunk, hi = min(nb, lo + a.chunk);
+    if (lo >= hi) return;
+
+    const int *pages = a.b.pages + (int64_t)seq * a.b.ld_pages;
+    const int per_page = a.b.page_shift - a.s.block_shift;
+    /* lanes 0 to 15 look up the pages of the wave's 16 blocks of a step; each load takes its row's from them */
+    auto page_of = [&](int b0) __attribute__((always_inline)) {
+        const int blk = b0 + 16 * wave + lc;
+        const int id = blk < hi ? pages[blk >> per_page] : -1;
+        return page_ok(a.b, id) ? id : -1;
+    };
+    const uint8_t *codes = a.s.codes + (int64_t)h * a.s.head_stride, *scales = a.s.scales + (int64_t)h * a.s.scale_head_stride;
+    const int row = lane / PIECES, piece = lane % PIECES;
+    u4 w[N];
+    int byte;
+    auto load = [&](int b0, int id) __attribute__((always_inline)) {
+#pragma unroll
+        for (int z = 0; z < N; z++) {
+            const int r = z * RI + row;
+            const int64_t page = max(__shfl(id, r), 0);
+            const int sub = (b0 + 16 * wave + r) & (a.s.blocks - 1);
+            w[z] = *(const u4 *)(codes + page * a.s.page_stride + sub * (2 * D) + 16 * piece);
         }
+        const int sub = (b0 + 16 * wave + lc) & (a.s.blocks - 1);
+        const int x = scales[(int64_t)max(id, 0) * a.s.scale_page_stride + sub];
+        byte = id >= 0 ? x : -1;
+    };
+    auto at = [](int r, int p) { return r * PIECES + (D == 64 ? p ^ (r >> 1 & 7) : p ^ (r & 15)); };
+    auto settle = [&](int buf) __attribute__((always_inline)) {
+#pragma unroll
+        for (int z = 0; z < N; z++) lds[buf][at(16 * wave + z * RI + row, piece)] = w[z];
+        if (g == 0) lds_b[buf][16 * wave + lc] = byte;
+    };
+    int id = page_of(lo);
+    load(lo, id);
+    id = page_of(lo + STEP);
+    const int tl = lc / pad;
+    const bool on = t0 + tl < n;
+    const Rows16<KS> mine = quantise<T, KS>(a.q + (int64_t)(q.q0 + (on ? t0 + tl : first)) * a.qt + (int64_t)(h * a.group + min(lc % pad, a.group - 1)) * a.qh, g, on);
+    int eq[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) eq[j] = __shfl(mine.byte, 4 * g + j);
+    const Put put(a, q, h, pad, t0, n, g);
+    settle(0);
+    __syncthreads();
+    int buf = 0;
+    for (int b0 = lo; b0 < hi; b0 += STEP, buf ^= 1) {
+        const bool more = b0 + STEP < hi;
+        if (more) load(b0 + STEP, id);
+        id = page_of(b0 + 2 * STEP);
+#pragma unroll
+        for (int u = 0; u < SCORE_WAVES; u++) {
+            const int r = 16 * u + lc;
+            i4 low[KS], high[KS];
+#pragma unroll
+            for (int i = 0; i < KS; i++) {
+                low[i] = __builtin_bit_cast(i4, lds[buf][at(r, 4 * i + g)]);
+                high[i] = __builtin_bit_cast(i4, lds[buf][at(r, PIECES / 2 + 4 * i + g)]);
+            }
+            const int eb = lds_b[buf][r];
+            float s[4];
+            score16<KS>(mine.up, mine.down, high, low, eq, eb, s);
+            put(b0 + r, eb >= 0, b0 + r < hi, s);
+        }
+        if (more) settle(buf ^ 1);
+        __syncthreads();
     }
 }
 
@@ -457,10 +571,10 @@ void bounds_t(const BoundsArgs &a, int width, hipStream_t st) {
 }
 
 template <class T, int D>
-void scores_t(const SelectArgs &a, hipStream_t st) {
-    const int tpt = a.group <= 16 ? 16 / padded(a.group) : 1, tiles = (a.b.max_q + tpt - 1) / tpt;
+void scores_t(const SelectArgs &a, int tiles, bool many, hipStream_t st) {
     const dim3 grid((unsigned)((int64_t)tiles * a.n_chunks * a.kv_heads), 1, a.b.n_seqs), block(64 * SCORE_WAVES);
-    if (a.group <= 16) hipLaunchKernelGGL((k_block_scores<T, D, true>), grid, block, 0, st, a);
+    if (many) hipLaunchKernelGGL((k_block_scores_many<T, D>), grid, block, 0, st, a);
+    else if (a.group <= 16) hipLaunchKernelGGL((k_block_scores<T, D, true>), grid, block, 0, st, a);
     else hipLaunchKernelGGL((k_block_scores<T, D, false>), grid, block, 0, st, a);
 }
 
@@ -475,15 +589,19 @@ void key_bounds(const BoundsArgs &a, int cache_dtype, int width, hipStream_t st)
 
 int select_group_limit() { return 16 * MAX_CHUNKS; }
 
-/* Blocks are shared out among workgroups until two are there for each unit, 64 at least each (16 a wave) */
+/* Blocks are shared out among workgroups until two are there for each unit, 64 at least each (16 a wave).
+ * Tokens that fill the rows of four waves share their blocks' bounds. */
 void select_blocks(SelectArgs a, int q_dtype, int width, int n_blocks, hipStream_t st) {
-    const int tpt = a.group <= 16 ? 16 / padded(a.group) : 1;
-    const int64_t wgs = (int64_t)a.b.n_seqs * a.kv_heads * ((a.b.max_q + tpt - 1) / tpt);
+    int tpt = a.group <= 16 ? 16 / padded(a.group) : 1;
+    const bool many = a.group <= 16 && a.b.max_q >= SCORE_WAVES * tpt;
+    if (many) tpt *= SCORE_WAVES;
+    const int tiles = (a.b.max_q + tpt - 1) / tpt;
+    const int64_t wgs = (int64_t)a.b.n_seqs * a.kv_heads * tiles;
     const int64_t want = std::max<int64_t>(1, 512 / wgs);
     a.chunk = (int)(((n_blocks + want - 1) / want + 63) / 64 * 64);
     a.n_chunks = (n_blocks + a.chunk - 1) / a.chunk;
-    if (q_dtype == DT_BF16) width == 64 ? scores_t<Bf16, 64>(a, st) : width == 128 ? scores_t<Bf16, 128>(a, st) : scores_t<Bf16, 256>(a, st);
-    else width == 64 ? scores_t<F16, 64>(a, st) : width == 128 ? scores_t<F16, 128>(a, st) : scores_t<F16, 256>(a, st);
+    if (q_dtype == DT_BF16) width == 64 ? scores_t<Bf16, 64>(a, tiles, many, st) : width == 128 ? scores_t<Bf16, 128>(a, tiles, many, st) : scores_t<Bf16, 256>(a, tiles, many, st);
+    else width == 64 ? scores_t<F16, 64>(a, tiles, many, st) : width == 128 ? scores_t<F16, 128>(a, tiles, many, st) : scores_t<F16, 256>(a, tiles, many, st);
     const dim3 rows((unsigned)((int64_t)a.b.max_q * a.kv_heads), 1, a.b.n_seqs), threads(PICK_THREADS);
     if (n_blocks <= 2 * PICK_THREADS) hipLaunchKernelGGL(k_block_pick<2>, rows, threads, 0, st, a);
     else if (n_blocks <= 8 * PICK_THREADS) hipLaunchKernelGGL(k_block_pick<8>, rows, threads, 0, st, a);
