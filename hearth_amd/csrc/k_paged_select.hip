@@ -433,29 +433,39 @@ __global__ __launch_bounds__(64 * SCORE_WAVES) void k_block_scores_many(SelectAr
 
 /* ---------------------------------------------------------------- the best of a token
  *
- * A workgroup takes one token and kv head, a wave a quarter of the blocks, in order. Keys are the scores' bits in an
- * order of unsigned numbers, the greatest for blocks that are kept in any case, 0 for those that cannot be taken.
- * Keys of one row lie close together, so the top-th greatest is looked for within their range: 256 bins over
- * it, then over the bin that holds it, until the bin is taken whole or holds one value (two rounds in most rows). Then
- * every wave counts what it takes (keys above, and of those equal the first ones) and writes it behind
+ * W waves take one token and kv head, each its share of the blocks, in order: four waves, or one where the keys of all
+ * blocks fit its registers, which then waits for no other (2400 rows of 313 blocks: four waves 9.4 us). Keys are the
+ * scores' bits in an order of unsigned numbers, the greatest for blocks that are kept in any case, 0 for those that
+ * cannot be taken. Keys of one row lie close together, so the top-th greatest is looked for within their range: 256
+ * bins over it, then over the bin that holds it, until the bin is taken whole or holds one value (two rounds in most rows).
+ * Then every wave counts what it takes (keys above, and of those equal the first ones) and writes it behind
  * the waves before. R: keys of a lane that stay in registers (0: they are read again each time). */
-constexpr int PICK_THREADS = 256, PICK_WAVES = PICK_THREADS / 64;
+constexpr int PICK_THREADS = 256, PICK_ALONE = 8;   /* keys of a lane of one wave */
 
-template <int R>
+template <int R, int W>
 __global__ __launch_bounds__(PICK_THREADS) void k_block_pick(SelectArgs a) {
-    __shared__ unsigned bins[2][256];
-    __shared__ unsigned lds_lo[PICK_WAVES], lds_hi[PICK_WAVES];
-    __shared__ int lds_can[PICK_WAVES], lds_kept[PICK_WAVES], above[PICK_WAVES], equal[PICK_WAVES];
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const int h = blockIdx.x % a.kv_heads, tok = blockIdx.x / a.kv_heads, seq = blockIdx.z;
+    constexpr int ROWS = PICK_THREADS / 64 / W;      /* of a workgroup */
+    static_assert(W == 1 || ROWS == 1);
+    __shared__ unsigned lds_bins[ROWS][2][256];
+    __shared__ unsigned lds_lo[W], lds_hi[W];
+    __shared__ int lds_can[W], lds_kept[W], above[W], equal[W];
+    const int wave = W == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int mine_of = W == 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0, id = W == 1 ? lane : threadIdx.x;
+    auto meet = [] {
+        if constexpr (W == 1) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        else __syncthreads();
+    };
+    unsigned (*bins)[256] = lds_bins[mine_of];
+    const int unit = blockIdx.x * ROWS + mine_of, seq = blockIdx.z;
+    const int h = unit % a.kv_heads, tok = unit / a.kv_heads;
     const Seq q = seq_of(a.b, seq);
-    if (tok >= min(q.n, a.b.max_q)) return;
+    if (tok >= min(q.n, a.b.max_q)) return;          /* the row's waves alike */
     const int64_t row = min((int64_t)q.base + tok, (int64_t)q.kv - 1);
     const int n = row < 0 ? 0 : (int)(row >> a.s.block_shift) + 1;
     int tail = max(n - a.last, 0);                       /* blocks from here on are kept */
     if (a.b.mask) tail = min(tail, max(q.base, 0) >> a.s.block_shift);
     const float *score = a.score + ((int64_t)(q.q0 + tok) * a.kv_heads + h) * a.ld_score;
-    const int per = (n + PICK_WAVES - 1) / PICK_WAVES, from = min(wave * per, n), to = min(from + per, n);
+    const int per = (n + W - 1) / W, from = min(wave * per, n), to = min(from + per, n);
     auto fetch = [&](int i) __attribute__((always_inline)) -> unsigned {   /* of block from + i of the wave */
         if (from + i >= to) return 0u;
         const float s = score[from + i];
@@ -468,14 +478,14 @@ __global__ __launch_bounds__(PICK_THREADS) void k_block_pick(SelectArgs a) {
 #pragma unroll
         for (int i = 0; i < R; i++) mine[i] = fetch(64 * i + lane);
     }
-    auto keys = [&](auto f) __attribute__((always_inline)) {   /* f(index in the wave's quarter, key), 64 lanes at once */
+    auto keys = [&](auto f) __attribute__((always_inline)) {   /* f(index in the wave's share, key), 64 lanes at once */
         if constexpr (R != 0) {
 #pragma unroll
             for (int i = 0; i < R; i++) f(64 * i, mine[i]);
         } else
             for (int i = 0; from + i < to; i += 64) f(i, fetch(i + lane));
     };
-    for (int i = threadIdx.x; i < 2 * 256; i += PICK_THREADS) bins[i >> 8][i & 255] = 0;
+    for (int i = id; i < 2 * 256; i += 64 * W) bins[i >> 8][i & 255] = 0;
     unsigned lo = ~0u, hi = 0;
     int can = 0, kept = 0;
     keys([&](int, unsigned k) {
@@ -488,13 +498,18 @@ __global__ __launch_bounds__(PICK_THREADS) void k_block_pick(SelectArgs a) {
         lo = min(lo, (unsigned)__shfl_xor((int)lo, d));
         hi = max(hi, (unsigned)__shfl_xor((int)hi, d));
     }
-    if (lane == 0) { lds_lo[wave] = lo; lds_hi[wave] = hi; lds_can[wave] = can; lds_kept[wave] = kept; }
-    __syncthreads();
-    static_assert(PICK_WAVES == 4);
-    lo = min(min(lds_lo[0], lds_lo[1]), min(lds_lo[2], lds_lo[3]));
-    hi = max(max(lds_hi[0], lds_hi[1]), max(lds_hi[2], lds_hi[3]));
-    can = lds_can[0] + lds_can[1] + lds_can[2] + lds_can[3];
-    kept = lds_kept[0] + lds_kept[1] + lds_kept[2] + lds_kept[3];
+    if constexpr (W > 1) {
+        if (lane == 0) { lds_lo[wave] = lo; lds_hi[wave] = hi; lds_can[wave] = can; lds_kept[wave] = kept; }
+        can = kept = 0;
+        meet();
+#pragma unroll
+        for (int w = 0; w < W; w++) {
+            lo = min(lo, lds_lo[w]);
+            hi = max(hi, lds_hi[w]);
+            can += lds_can[w];
+            kept += lds_kept[w];
+        }
+    } else meet();
     unsigned limit = 0;          /* keys above it are taken, and `ties` of those equal to it */
     int ties = 0, left = a.top - kept;   /* to be taken within [lo, hi] */
     if (can > a.top) {
@@ -505,7 +520,7 @@ __global__ __launch_bounds__(PICK_THREADS) void k_block_pick(SelectArgs a) {
                 keys([&](int, unsigned k) {
                     if (k >= lo && k <= hi) atomicAdd(&bins[round][(k - lo) >> shift], 1u);
                 });
-                __syncthreads();
+                meet();
                 /* every wave alike: four bins a lane, the greatest first */
                 unsigned c[4], sum = 0;
 #pragma unroll
@@ -532,8 +547,8 @@ __global__ __launch_bounds__(PICK_THREADS) void k_block_pick(SelectArgs a) {
                 if (shift == 0) { limit = lo; ties = left; break; }
                 hi = min(hi, lo + (1u << shift) - 1);
                 /* the other set of bins is clear; this one is for the round after the next */
-                __syncthreads();
-                bins[round][threadIdx.x] = 0;
+                meet();
+                for (int i = id; i < 256; i += 64 * W) bins[round][i] = 0;
             }
     }
     int na = 0, ne = 0;
@@ -541,16 +556,20 @@ __global__ __launch_bounds__(PICK_THREADS) void k_block_pick(SelectArgs a) {
         na += __popcll(__ballot(k > limit));
         ne += __popcll(__ballot(k == limit && k));
     });
-    if (lane == 0) { above[wave] = na; equal[wave] = ne; }
-    __syncthreads();
     int *out = a.chosen + (int64_t)(q.q0 + tok) * a.ct + (int64_t)h * a.ch;
-    int at = 0, eq = 0, total = 0;
+    int at = 0, eq = 0, total = na, same = ne;
+    if constexpr (W > 1) {
+        if (lane == 0) { above[wave] = na; equal[wave] = ne; }
+        meet();
+        total = same = 0;
 #pragma unroll
-    for (int w = 0; w < PICK_WAVES; w++) {
-        if (w < wave) { at += above[w]; eq += equal[w]; }
-        total += above[w];
+        for (int w = 0; w < W; w++) {
+            if (w < wave) { at += above[w]; eq += equal[w]; }
+            total += above[w];
+            same += equal[w];
+        }
     }
-    total += min(ties, equal[0] + equal[1] + equal[2] + equal[3]);
+    total += min(ties, same);
     const unsigned long long before = (1ull << lane) - 1;
     keys([&](int i, unsigned k) {
         const unsigned long long ma = __ballot(k > limit), me = __ballot(k == limit && k);
@@ -559,7 +578,7 @@ __global__ __launch_bounds__(PICK_THREADS) void k_block_pick(SelectArgs a) {
         at += __popcll(ma);
         eq += __popcll(me);
     });
-    for (int i = total + (int)threadIdx.x; i < a.top; i += PICK_THREADS) out[i] = -1;
+    for (int i = total + id; i < a.top; i += 64 * W) out[i] = -1;
 }
 
 template <int DT>
@@ -589,7 +608,8 @@ void key_bounds(const BoundsArgs &a, int cache_dtype, int width, hipStream_t st)
 
 int select_group_limit() { return 16 * MAX_CHUNKS; }
 
-/* Blocks are shared out among workgroups until two are there for each unit, 64 at least each (16 a wave).
+/* Blocks are shared out among workgroups until four are there for each unit, 64 at least each (16 a wave; 600 tokens over
+ * 313 blocks: 13.2 us, with two 15).
  * Tokens that fill the rows of four waves share their blocks' bounds. */
 void select_blocks(SelectArgs a, int q_dtype, int width, int n_blocks, hipStream_t st) {
     int tpt = a.group <= 16 ? 16 / padded(a.group) : 1;
@@ -597,16 +617,18 @@ void select_blocks(SelectArgs a, int q_dtype, int width, int n_blocks, hipStream
     if (many) tpt *= SCORE_WAVES;
     const int tiles = (a.b.max_q + tpt - 1) / tpt;
     const int64_t wgs = (int64_t)a.b.n_seqs * a.kv_heads * tiles;
-    const int64_t want = std::max<int64_t>(1, 512 / wgs);
+    const int64_t want = std::max<int64_t>(1, 1024 / wgs);
     a.chunk = (int)(((n_blocks + want - 1) / want + 63) / 64 * 64);
     a.n_chunks = (n_blocks + a.chunk - 1) / a.chunk;
     if (q_dtype == DT_BF16) width == 64 ? scores_t<Bf16, 64>(a, tiles, many, st) : width == 128 ? scores_t<Bf16, 128>(a, tiles, many, st) : scores_t<Bf16, 256>(a, tiles, many, st);
     else width == 64 ? scores_t<F16, 64>(a, tiles, many, st) : width == 128 ? scores_t<F16, 128>(a, tiles, many, st) : scores_t<F16, 256>(a, tiles, many, st);
-    const dim3 rows((unsigned)((int64_t)a.b.max_q * a.kv_heads), 1, a.b.n_seqs), threads(PICK_THREADS);
-    if (n_blocks <= 2 * PICK_THREADS) hipLaunchKernelGGL(k_block_pick<2>, rows, threads, 0, st, a);
-    else if (n_blocks <= 8 * PICK_THREADS) hipLaunchKernelGGL(k_block_pick<8>, rows, threads, 0, st, a);
-    else if (n_blocks <= 32 * PICK_THREADS) hipLaunchKernelGGL(k_block_pick<32>, rows, threads, 0, st, a);
-    else hipLaunchKernelGGL(k_block_pick<0>, rows, threads, 0, st, a);
+    const int64_t rows = (int64_t)a.b.max_q * a.kv_heads;
+    const bool alone = n_blocks <= 64 * PICK_ALONE;
+    const dim3 grid((unsigned)(alone ? (rows + 3) / 4 : rows), 1, a.b.n_seqs), threads(PICK_THREADS);
+    if (alone) hipLaunchKernelGGL((k_block_pick<PICK_ALONE, 1>), grid, threads, 0, st, a);
+    else if (n_blocks <= 8 * PICK_THREADS) hipLaunchKernelGGL((k_block_pick<8, 4>), grid, threads, 0, st, a);
+    else if (n_blocks <= 32 * PICK_THREADS) hipLaunchKernelGGL((k_block_pick<32, 4>), grid, threads, 0, st, a);
+    else hipLaunchKernelGGL((k_block_pick<0, 4>), grid, threads, 0, st, a);
 }
 
 } // namespace hxp
