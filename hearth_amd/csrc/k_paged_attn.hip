@@ -71,10 +71,12 @@ struct Few {
     }
     /* rows, sc: a tile's first row and its scales, the same for the wave; a lane's bytes from there on are a 32-bit
      * offset, so that no load needs an address of its own */
-    static __device__ __forceinline__ void load_k(K &k, int u, const uint8_t *rows, const uint8_t *sc, int g, int lc) {
+    static __device__ __forceinline__ void load_k(K &k, int u, const uint8_t *rows, int g, int lc) {
         const unsigned at = lc * RB + LB * g;
 #pragma unroll
         for (int i = 0; i < KL; i++) words<LB>(rows + at + 4 * LB * i, k.w[u][i]);
+    }
+    static __device__ __forceinline__ void load_ks(K &k, int u, const uint8_t *sc, int lc) {
         if constexpr (MX) {
             const uint8_t *q = sc + (unsigned)(lc * (D / MX_BLOCK));
             if constexpr (D == 64) k.s[u][0] = *(const ushort_any *)q;
@@ -82,6 +84,26 @@ struct Few {
 #pragma unroll
                 for (int i = 0; i < SW; i++) k.s[u][i] = ((const unsigned_any *)q)[i];
         }
+    }
+    /* K by way of LDS: 64 lanes bring in 1 KiB of whole rows an instruction, where 16 lanes that read 16 bytes of 16 rows
+     * each touch 16 cache lines. The 16-byte pieces of a row are exchanged by row, so that those 16 lanes meet 16 different
+     * columns of the 256 bytes of banks. */
+    static constexpr int P = RB / 16, RI = 1024 / RB, N = STEP * RB / 1024;   /* pieces of a row, rows an instruction, instructions */
+    static __device__ __forceinline__ int swz(int r) { return P >= 16 ? r & 15 : r / (16 / P) & (P - 1); }
+    /* z: instruction; rows: the first of its rows */
+    static __device__ __forceinline__ void send_k(uint8_t *lds, int z, const uint8_t *rows, int lane) {
+        const int r = lane / P;
+        const unsigned at = r * RB + ((lane % P) ^ swz((z * RI + r) & 15)) * 16;
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(rows + at), (__attribute__((address_space(3))) void *)(lds + 1024 * z), 16, 0, 0);
+    }
+    static __device__ __forceinline__ void read_k(K &k, const uint8_t *lds, int g, int lc) {
+#pragma unroll
+        for (int u = 0; u < NT; u++)
+#pragma unroll
+            for (int i = 0; i < KL; i++) {
+                const int byte = 4 * LB * i + LB * g;
+                words<LB>(lds + (16 * u + lc) * RB + ((byte / 16) ^ swz(lc)) * 16 + byte % 16, k.w[u][i]);
+            }
     }
     static __device__ __forceinline__ void load_v(V &v, int u, const uint8_t *rows, const uint8_t *sc, int g, int lc) {
         const unsigned at = 4 * g * RB + lc * VB;
@@ -128,6 +150,76 @@ struct Few {
                     s[u] = T::mfma16(__builtin_bit_cast(v8, w), q[SL * i + h], s[u]);
                 }
     }
+    /* The softmax of a lane's scores x in base 2, against the running maximum m: x become the probabilities, packed into
+     * pf, l their sum; sums and l are rescaled where a maximum has grown by more than GROWTH. */
+    template <int GROWTH>
+    static __device__ __forceinline__ void weights(float (&x)[4 * NT], v8 (&pf)[NT / 2], f4 (&acc)[NB * PL], float &m, float &l) {
+        float mx = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+#pragma unroll
+        for (int j = 8; j < 4 * NT; j += 4) mx = fmaxf(mx, fmaxf(fmaxf(x[j], x[j + 1]), fmaxf(x[j + 2], x[j + 3])));
+        mx = max16(max32(mx));
+        if (__any(mx > m + (float)GROWTH)) {
+            mx = fmaxf(m, mx);
+            const float al = exp2_hw(m - (mx == -__builtin_huge_valf() ? 0.0f : mx));
+            l *= al;
+#pragma unroll
+            for (int i = 0; i < NB * PL; i++) acc[i] *= al;
+            m = mx;
+        }
+        const float ms = m == -__builtin_huge_valf() ? 0.0f : m;
+#pragma unroll
+        for (int j = 0; j < 4 * NT; j++) {
+            x[j] = exp2_hw(x[j] - ms);
+            l += x[j];
+        }
+#pragma unroll
+        for (int k = 0; k < NT / 2; k++) {
+            const float *p = x + 8 * k;
+            pf[k] = __builtin_bit_cast(v8, (u4){T::pack(p[0], p[1]), T::pack(p[2], p[3]), T::pack(p[4], p[5]), T::pack(p[6], p[7])});
+        }
+    }
+    /* acc += V^T P^T. ALL: every row counts as it is; otherwise rows for which there(tile, row of the tile) is false are taken
+     * as zeros, and so are infinities and NaN, which `odd` tells of */
+    template <bool ALL, class THERE>
+    static __device__ __forceinline__ void add(f4 (&acc)[NB * PL], const V &v, const v8 (&pf)[NT / 2], int lc, bool &odd, THERE there) {
+#pragma unroll
+        for (int bk = 0; bk < NB * NT / 2; bk++) {
+            const int b = bk / (NT / 2), k = bk % (NT / 2);   /* block of elements, pair of tiles */
+            unsigned w[8][PL / 2];
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                v_row(v, b, 8 * k + j, lc, w[j]);
+                if constexpr (!ALL) {
+                    const unsigned keep = there(2 * k + (j >> 2), j & 3) ? ~0u : 0u;
+#pragma unroll
+                    for (int i = 0; i < PL / 2; i++) {
+                        w[j][i] &= keep;
+                        odd = odd || T::odd(w[j][i]);
+                        w[j][i] = T::clean(w[j][i]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < PL / 2; i++) {
+                const u4 e = {lo16(w[0][i], w[1][i]), lo16(w[2][i], w[3][i]), lo16(w[4][i], w[5][i]), lo16(w[6][i], w[7][i])};
+                const u4 o = {hi16(w[0][i], w[1][i]), hi16(w[2][i], w[3][i]), hi16(w[4][i], w[5][i]), hi16(w[6][i], w[7][i])};
+                acc[b * PL + 2 * i] = T::mfma16(__builtin_bit_cast(v8, e), pf[k], acc[b * PL + 2 * i]);
+                acc[b * PL + 2 * i + 1] = T::mfma16(__builtin_bit_cast(v8, o), pf[k], acc[b * PL + 2 * i + 1]);
+            }
+        }
+    }
+    /* the infinities and NaN of one row, to the columns that attend it */
+    static __device__ __forceinline__ void add_odd(f4 (&acc)[NB * PL], const uint8_t *row, const uint8_t *sc, int g, bool mine) {
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int j = 0; j < PL; j++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const unsigned x = row_elem<T, BITS>(row, sc, b * BD + (4 * g + i) * PL + j);
+                    acc[b * PL + j][i] += T::odd(x) && mine ? T::wide(x) : 0.0f;
+                }
+    }
     /* PL elements of row j, block b, as 16-bit pairs */
     static __device__ __forceinline__ void v_row(const V &v, int b, int j, int lc, unsigned (&w)[PL / 2]) {
         if constexpr (MX) {
@@ -158,12 +250,13 @@ __global__ __launch_bounds__(64 * FEW_WAVES, D <= 128 ? 2 : 1) void k_attend_few
     using F = Few<T, BITS, D>;
     using v8 = typename T::v8;
     constexpr bool MX = F::MX;
-    /* Rows of 4 bits, whose steps have most to do beside the loads: the sums are rescaled only where a maximum has
-     * grown by more than 2^8, below which the probabilities lose no accuracy in either 16-bit type. */
-    constexpr float GROWTH = BITS == 4 ? 8.0f : 0.0f;
+    /* Rows of 4 bits and few rows in all have most to do beside the loads: the sums are rescaled only where a maximum
+     * has grown by more than 2^8, below which the probabilities lose no accuracy in either 16-bit type. */
+    constexpr int GROWTH = BITS == 4 || BLOCKS ? 8 : 0;
     constexpr int PL = F::PL, NB = F::NB, BD = F::BD, CT = 16, NT = F::NT, STEP = F::STEP;
     constexpr int PER = ONE ? NT : 1, NL = NT / PER, RUN = 16 * PER;   /* tiles of a look-up, look-ups of a step, their rows */
     __shared__ float lds_o[FEW_WAVES][16][BD + 4];
+    __shared__ __align__(16) uint8_t lds_k[BLOCKS && BITS > 4 ? FEW_WAVES : 1][BLOCKS && BITS > 4 ? STEP * F::RB : 16];
     __shared__ float lds_m[FEW_WAVES][CT], lds_l[FEW_WAVES][CT];
     __shared__ unsigned lds_some[FEW_WAVES];   /* bit c: column c attends a row of the wave's */
 
@@ -258,14 +351,33 @@ __global__ __launch_bounds__(64 * FEW_WAVES, D <= 128 ? 2 : 1) void k_attend_few
     };
     typename F::K kr;
     typename F::V vw;
+    /* Blocks that many tokens choose come from the chip's caches, where the lines that K's loads touch bound the kernel
+     * (600 tokens over 16 blocks each, by LDS and straight: 16-bit rows 66 and 95 us, 8-bit 62 and 77, 4-bit, whose
+     * rows are a quarter of a line's, 61 and 57). */
+    constexpr bool BY_LDS = BLOCKS && BITS > 4;
     auto load_k = [&](const Run (&x)[NL]) __attribute__((always_inline)) {
+        const uint8_t *rows[NL];
 #pragma unroll
         for (int z = 0; z < NL; z++) {
             const int64_t i = max(x[z].page, 0), row = x[z].row & (page_rows - RUN);
-            const uint8_t *rows = same_global(kbase + i * a.k.page_stride + row * F::RB);
-            const uint8_t *sc = MX ? same_global(ksb + i * a.k.scale_page_stride + row * (D / MX_BLOCK)) : nullptr;
+            rows[z] = same_global(kbase + i * a.k.page_stride + row * F::RB);
+            if constexpr (MX) {
+                const uint8_t *sc = same_global(ksb + i * a.k.scale_page_stride + row * (D / MX_BLOCK));
 #pragma unroll
-            for (int u = 0; u < PER; u++) F::load_k(kr, z * PER + u, rows + 16 * u * F::RB, MX ? sc + 16 * u * (D / MX_BLOCK) : nullptr, g, lc);
+                for (int u = 0; u < PER; u++) F::load_ks(kr, z * PER + u, sc + 16 * u * (D / MX_BLOCK), lc);
+            }
+        }
+        if constexpr (!BY_LDS) {
+#pragma unroll
+            for (int u = 0; u < NT; u++) F::load_k(kr, u, rows[u / PER] + 16 * (u % PER) * F::RB, g, lc);
+        } else {
+#pragma unroll
+            for (int z = 0; z < F::N; z++) {
+                constexpr int RI = F::RI;
+                const int r = z * RI;                       /* first row of the instruction's */
+                static_assert(RI <= 16);                    /* of one run */
+                F::send_k(lds_k[wave], z, rows[r / RUN] + (r % RUN) * F::RB, lane);
+            }
         }
     };
     auto load_v = [&](const Run (&x)[NL]) __attribute__((always_inline)) {
@@ -305,6 +417,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES, D <= 128 ? 2 : 1) void k_attend_few
         }
         in_order();
         f4 s[NT];
+        if constexpr (BY_LDS) F::read_k(kr, lds_k[wave], g, lc);
         F::scores(kr, g, qf, s);
         in_order();
 #pragma unroll
@@ -334,59 +447,11 @@ __global__ __launch_bounds__(64 * FEW_WAVES, D <= 128 ? 2 : 1) void k_attend_few
 #pragma unroll
             for (int j = 0; j < 4 * NT; j++) x[j] = vis >> (16 * (j >> 2) + (j & 3)) & 1 ? x[j] : -__builtin_huge_valf();
         }
-        float mx = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
-#pragma unroll
-        for (int j = 8; j < 4 * NT; j += 4) mx = fmaxf(mx, fmaxf(fmaxf(x[j], x[j + 1]), fmaxf(x[j + 2], x[j + 3])));
-        mx = max16(max32(mx));
-        if (__any(mx > m + GROWTH)) {
-            mx = fmaxf(m, mx);
-            const float al = exp2_hw(m - (mx == -__builtin_huge_valf() ? 0.0f : mx));
-            l *= al;
-#pragma unroll
-            for (int i = 0; i < NB * PL; i++) acc[i] *= al;
-            m = mx;
-        }
-        const float ms = m == -__builtin_huge_valf() ? 0.0f : m;
-#pragma unroll
-        for (int j = 0; j < 4 * NT; j++) {
-            x[j] = exp2_hw(x[j] - ms);
-            l += x[j];
-        }
-#pragma unroll
-        for (int k = 0; k < NT / 2; k++) {
-            const float *p = x + 8 * k;
-            pf[k] = __builtin_bit_cast(v8, (u4){T::pack(p[0], p[1]), T::pack(p[2], p[3]), T::pack(p[4], p[5]), T::pack(p[6], p[7])});
-        }
+        F::template weights<GROWTH>(x, pf, acc, m, l);
         /* two ways, so that the one of most steps has no branches in it */
-        auto sums = [&](auto all) __attribute__((always_inline)) {
-#pragma unroll
-            for (int bk = 0; bk < NB * NT / 2; bk++) {
-                const int b = bk / (NT / 2), k = bk % (NT / 2);   /* block of elements, pair of tiles */
-                unsigned w[8][PL / 2];
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    const int u = 2 * k + (j >> 2), t = now[u / PER].row + 16 * (u % PER) + 4 * g + (j & 3);
-                    F::v_row(vw, b, 8 * k + j, lc, w[j]);
-                    if constexpr (!all.value) {
-#pragma unroll
-                        for (int i = 0; i < PL / 2; i++) {
-                            w[j][i] &= t < hi && now[u / PER].page >= 0 ? ~0u : 0u;
-                            odd = odd || T::odd(w[j][i]);
-                            w[j][i] = T::clean(w[j][i]);
-                        }
-                    }
-                }
-#pragma unroll
-                for (int i = 0; i < PL / 2; i++) {
-                    const u4 e = {lo16(w[0][i], w[1][i]), lo16(w[2][i], w[3][i]), lo16(w[4][i], w[5][i]), lo16(w[6][i], w[7][i])};
-                    const u4 o = {hi16(w[0][i], w[1][i]), hi16(w[2][i], w[3][i]), hi16(w[4][i], w[5][i]), hi16(w[6][i], w[7][i])};
-                    acc[b * PL + 2 * i] = T::mfma16(__builtin_bit_cast(v8, e), pf[k], acc[b * PL + 2 * i]);
-                    acc[b * PL + 2 * i + 1] = T::mfma16(__builtin_bit_cast(v8, o), pf[k], acc[b * PL + 2 * i + 1]);
-                }
-            }
-        };
-        if (whole) sums(std::true_type{});
-        else sums(std::false_type{});
+        auto there = [&](int u, int r) { return now[u / PER].row + 16 * (u % PER) + 4 * g + r < hi && now[u / PER].page >= 0; };
+        if (whole) F::template add<true>(acc, vw, pf, lc, odd, there);
+        else F::template add<false>(acc, vw, pf, lc, odd, there);
     }
     /* an infinity or NaN among rows that some columns do not attend would reach them as 0 * inf:
      * left out above, added here to the columns that do attend it */
@@ -404,15 +469,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES, D <= 128 ? 2 : 1) void k_attend_few
                 if (id < 0 || t >= hi) continue;
                 const uint8_t *row = vbase + (int64_t)id * a.v.page_stride + (int64_t)(t & (page_rows - 1)) * F::RB;
                 const uint8_t *sc = MX ? vsb + (int64_t)id * a.v.scale_page_stride + (t & (page_rows - 1)) * (D / MX_BLOCK) : nullptr;
-#pragma unroll
-                for (int b = 0; b < NB; b++)
-#pragma unroll
-                    for (int j = 0; j < PL; j++)
-#pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            const unsigned x = row_elem<T, BITS>(row, sc, b * BD + (4 * g + i) * PL + j);
-                            acc[b * PL + j][i] += T::odd(x) && (attended(t) & 1) ? T::wide(x) : 0.0f;
-                        }
+                F::add_odd(acc, row, sc, g, attended(t) & 1);
             }
         }
     }
@@ -563,10 +620,14 @@ template <class T, int BITS, int D, bool BLOCKS>
 void few_t(const AttendArgs &a, hipStream_t st) {
     const int tiles = BLOCKS ? a.b.max_q * ((a.group + 15) / 16) : (a.b.max_q * a.group + 15) / 16;
     const dim3 grid((unsigned)a.n_splits * a.kv_heads * tiles, 1, a.b.n_seqs);
-    constexpr int STEP = Few<T, BITS, D>::STEP;
+    constexpr int STEP = 16 * few_tiles(BITS);
     const bool one = 1 << a.b.page_shift >= STEP && (!BLOCKS || 1 << a.block_shift >= STEP);
-    if (one) hipLaunchKernelGGL((k_attend_few<T, BITS, D, BLOCKS, true>), grid, dim3(64 * FEW_WAVES), 0, st, a);
-    else hipLaunchKernelGGL((k_attend_few<T, BITS, D, BLOCKS, false>), grid, dim3(64 * FEW_WAVES), 0, st, a);
+    if constexpr (BITS == 4 || BLOCKS)   /* of two look-ups a step one makes no difference to the others, which wait for memory */
+        if (one) {
+            hipLaunchKernelGGL((k_attend_few<T, BITS, D, BLOCKS, true>), grid, dim3(64 * FEW_WAVES), 0, st, a);
+            return;
+        }
+    hipLaunchKernelGGL((k_attend_few<T, BITS, D, BLOCKS, false>), grid, dim3(64 * FEW_WAVES), 0, st, a);
 }
 
 template <class T, int DV>
