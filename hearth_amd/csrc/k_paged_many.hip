@@ -9,7 +9,7 @@
  * Four waves (128 columns) share 64 cache rows (32 of width 256) at a time through LDS, K and V as
  * they lie in memory: the scores read K along its rows, the sums read V through the transposing
  * LDS load. The 16-byte pieces of a row are exchanged by row (piece p of row r at p ^ swz(r)), so
- * that neither read meets a bank conflict. 16-bit rows go from memory to LDS directly, 8-bit rows
+ * that neither read meets a bank conflict. 16-bit rows go from memory to LDS directly, 8- and 4-bit rows
  * through registers, where they become 16-bit ones once for the four waves; the next step's are
  * in flight while this one is worked on (two buffers).
  * It is bound by the products and by what a wave does between them: 8000 tokens at the end of 16384
@@ -134,7 +134,9 @@ __global__ __launch_bounds__(64 * MANY_WAVES, D <= 128 ? 2 : 1) void k_attend_ma
     constexpr int RW = M::ROWS / 4, LANES = M::PIECES / PL, RI = 64 / LANES, N = RW / RI;   /* lanes of a row, rows an instruction, instructions */
     constexpr int RB = D * BITS / 8;                                                          /* bytes of a row */
     static_assert(N >= 1 && N * RI == RW);
-    const int my = wave * RW, lr = lane / LANES, lp = lane % LANES;
+    /* 4-bit: 16 lanes write one piece of 16 rows, which lie in different banks; lanes by rows met four to a column (1000
+     * tokens over 5000 rows: 128 us, so 118; 8-bit rows are faster by rows) */
+    const int my = wave * RW, lr = BITS == 4 ? lane % RI : lane / LANES, lp = BITS == 4 ? lane / RI : lane % LANES;
     /* 16-bit: byte of a lane's pieces in memory (the z-th instruction's 1 KiB further, there and in LDS) */
     int off[N];
 #pragma unroll
