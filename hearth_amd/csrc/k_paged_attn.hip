@@ -299,7 +299,18 @@ __global__ __launch_bounds__(64 * FEW_WAVES, D <= 128 ? 2 : 1) void k_attend_few
     const int end = a.b.mask ? q.kv : min(q.kv, q.base + t_last + 1);
     const int hi = BLOCKS ? end : min(end, (sp + 1) * a.chunk);
     const int full = a.b.mask ? q.base : q.base + t_first + 1;
-    const int stop = BLOCKS ? min(a.top << a.block_shift, (sp + 1) * a.chunk) : hi;   /* of the steps */
+    const int *list = BLOCKS ? a.chosen + (int64_t)(q.q0 + only) * a.ct + (int64_t)kvh * a.ch : nullptr;
+    int stop = hi;                                                                     /* of the steps */
+    if constexpr (BLOCKS) {   /* behind the last block that has rows to attend: lists of early tokens end in entries that are none */
+        const int end_entry = min(a.top, (int)(((int64_t)(sp + 1) * a.chunk + (1 << a.block_shift) - 1) >> a.block_shift));
+        int used = 0;
+        for (int e = sp * a.chunk >> a.block_shift; e < end_entry; e += 64) {
+            const int blk = e + lane < end_entry ? list[e + lane] : -1;
+            const unsigned long long has = __ballot(blk >= 0 && ((int64_t)blk << a.block_shift) < hi);
+            if (has) used = e + 64 - __builtin_clzll(has);
+        }
+        stop = min(used << a.block_shift, (sp + 1) * a.chunk);
+    }
 
     /* which of the 64 rows from t0 on this lane's column attends (where their pages exist) */
     auto attended = [&](int t0) {
@@ -324,7 +335,6 @@ __global__ __launch_bounds__(64 * FEW_WAVES, D <= 128 ? 2 : 1) void k_attend_few
      * lie in the same page, those of a page that is not there are taken from page 0; both are
      * masked, and cleared in V. */
     struct Run { int row, page; };
-    const int *list = BLOCKS ? a.chosen + (int64_t)(q.q0 + only) * a.ct + (int64_t)kvh * a.ch : nullptr;
     /* in two or three steps, each of which waits for the one before: the block at t, its rows with what the page table
      * says, the page checked */
     auto block_at = [&](int t) __attribute__((always_inline)) { return BLOCKS && t < stop ? word_of(list, t >> a.block_shift) : -1; };
