@@ -508,8 +508,10 @@ def _blocks(chosen, what, dev, tokens, heads, block) -> _BlocksS:
     """int32 [tokens, heads, top]"""
     p = _ints(chosen, what, dev, 3)
     shape, st = chosen.shape, chosen.stride()
-    if shape[0] != tokens or shape[1] != heads or shape[2] < 1:
+    if shape[0] != tokens or shape[1] != heads or not 1 <= shape[2] <= 1 << 20:
         raise ValueError(f"{what}: shape {tuple(shape)} is not [{tokens} tokens, {heads} heads, top]")
+    if not 16 <= block <= 4096:
+        raise ValueError(f"blocks of {block} rows (a power of two from 16 up to a page is needed)")
     return _BlocksS(p, st[0], st[1], shape[2], block)
 
 
@@ -558,6 +560,8 @@ def select(bounds: Bounds, batch: Batch, q, chosen, *, first: int = 1, last: int
     if a.dtype == F32 or a.width != s.width or a.n_heads % s.n_heads:
         raise ValueError(f"select: q is {q.dtype}{tuple(q.shape)} over bounds of {s.n_heads} heads of width {s.width}")
     o = _blocks(chosen, "chosen", dev, tokens, s.n_heads, s.block)
+    if first < 0 or last < 1 or first + last > o.top:
+        raise ValueError(f"select: the first {first} and last {last} (at least one) of {o.top} blocks")
     wp, wb = None, 0
     if workspace is not None:
         _device(workspace, "workspace", dev)
@@ -576,7 +580,9 @@ def attend_blocks_workspace_bytes(cache: Cache, batch: Batch, heads: int, top: i
     sequences times max_q) of `heads` heads and `top` chosen blocks of `block` rows: 0 when none is."""
     s = _BatchS.from_buffer_copy(batch._s)
     s.n_tokens = min(s.n_seqs * s.max_q, 0x7fffffff) if tokens is None else tokens
-    n = _fn("hearth_gpu_attend_blocks_workspace")(cache._ref, byref(s), heads, top, block)
+    n = -1
+    if 1 <= heads <= 1 << 26 and 1 <= top <= 1 << 20 and 16 <= block <= 4096:
+        n = _fn("hearth_gpu_attend_blocks_workspace")(cache._ref, byref(s), heads, top, block)
     if n < 0:
         raise ValueError(f"no attention over {top} blocks of {block} rows of this cache (pages of {cache._s.page} rows, heads {cache._s.n_heads}, "
                          f"width {cache._s.width}) with {heads} query heads")

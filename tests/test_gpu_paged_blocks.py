@@ -154,6 +154,31 @@ def test_choice_of_long_sequences():
     choice(base._gen(9), BF, "mx4", 8, 2, 128, [20000, 9000], [1, 1], 64, 64, 16)
 
 
+@pytest.mark.parametrize("heads,kv_heads,width", [(2, 2, 256), (4, 2, 64), (3, 1, 256), (7, 1, 256), (10, 1, 128), (16, 1, 256), (2, 2, 64), (4, 2, 128), (17, 1, 256)])
+def test_choice_of_many_tokens(heads, kv_heads, width):
+    """Tokens that fill several waves' rows, whole and in part, at every width and number of heads to a token."""
+    choice(base._gen(heads * width), BF, "mx8", heads, kv_heads, width, [90, 400, 70, 1], [90, 71, 64, 1], 32, 16, 7, 1, 1)
+    choice(base._gen(heads + width), HF, "f16", heads, kv_heads, width, [1300], [67], 64, 16, 9, 0, 3, trees=[O.tree(67)])
+
+
+def test_choice_of_more_blocks_than_registers_hold():
+    choice(base._gen(14), BF, "bf16", 1, 1, 64, [140001], [1], 64, 16, 25, 1, 2)
+
+
+@pytest.mark.parametrize("rows", [600 * 16, 2500 * 16, 9000 * 16])
+def test_ties_across_waves(rows):
+    """Keys that repeat over long sequences: every second or seventh block scores the same; the lowest are taken, whichever wave
+    they lie with."""
+    for every in (2, 7):
+        def edit(k, pages):
+            for i in range(every, k.shape[0]):
+                k[i] = k[i % every]
+
+        n = rows // 16
+        got = choice(base._gen(every), BF, "bf16", 2, 1, 64, [rows], [1], 16, 16, 11, 0, 1, pages=torch.arange(n, dtype=torch.int32)[None], n_pages=n, edit=edit)
+        assert (got[0, 0, :10].diff() == every).all()
+
+
 @pytest.mark.parametrize("tree", [True, False])
 def test_choice_of_trees_and_max_kv(tree):
     news = [40, 7, 1]

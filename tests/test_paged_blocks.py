@@ -110,6 +110,9 @@ def test_select_refusals():
                      ((q, out), dict(workspace=Fake((1 << 20,), "uint8", dev=_Dev(index=1)))), ((Fake((5, 2 * 129, 64)), out), {}), ((leaf(5, 4, 64), out), {})):
         with pytest.raises(ValueError):
             paged.select(s, b, *args, **{"workspace": work, **kw})
+    for kw in (dict(first=1 << 32), dict(last=(1 << 32) + 1)):       # no cut to 32 bits
+        with pytest.raises(ValueError):
+            paged.select(s, b, q, out, workspace=work, **kw)
     # a tree's own blocks, besides the first ones, have to fit: 33 rows touch at most 3 blocks of 16, wherever they begin
     assert max((at + 32) // 16 - at // 16 + 1 for at in range(16)) == 3
     m = paged.Batch(Fake((2, 4), "int32"), Fake((2,), "int32"), Fake((3,), "int32"), max_q=33, max_kv=100, mask=Fake((40, 1), "int64"))
@@ -134,6 +137,11 @@ def test_attend_blocks_refusals():
         paged.attend_blocks(cache(heads=1, width=576, latent=True), b, Fake((5, 4, 576)), Fake((5, 1, 6), "int32"), Fake((5, 4, 576)), block=16, scale=0.1)
     with pytest.raises(ValueError):
         paged.attend_blocks_workspace_bytes(cache(width=96), b, 4, 6, 16)
+    for kw in (dict(block=(1 << 32) + 16), dict(top=(1 << 32) + 6), dict(heads=(1 << 32) + 4), dict(top=0)):       # no cut to 32 bits
+        with pytest.raises(ValueError):
+            paged.attend_blocks_workspace_bytes(c, b, **{"heads": 4, "top": 6, "block": 16, **kw})
+    with pytest.raises(ValueError):
+        paged.attend_blocks(c, b, q, ch, q, block=(1 << 32) + 16, scale=0.1)
     # a workspace is asked for where rows are split
     one = batch(S=1, per=4096, max_q=1, max_kv=65536)
     q1, many = Fake((1, 4, 64)), Fake((1, 2, 200), "int32")
