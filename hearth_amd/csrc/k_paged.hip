@@ -2,8 +2,9 @@
  * k_paged.hip — rotary positions and the writes and reads of a paged cache. All three move
  * each element once and are bound by HBM for prompts and by launch latency for single tokens:
  * rotating 64 of 192 elements of 2001 tokens of 128 heads (66 MB) takes 13.9 us (4.8 TB/s, near a
- * large copy's 4.9), quantising 3 x 4093 rows (31 MB) 13.2 us, reading 8 x 4095 back (71 MB) 19 us
- * (3.7 TB/s), the rows of 32 single tokens 3.5 us.
+ * large copy's 4.9), quantising 3 x 4093 rows into 8 bits (31 MB) 10 us, reading 8 x 4095 back (71 MB) 15 us
+ * (4.7 TB/s), the rows of 32 single tokens 3.2 us, rotating 3 x 4093 tokens of 32 + 4 heads of 128 into
+ * 16-bit pages (205 MB) 40 us (5.1 TB/s).
  */
 #include "hx_paged.h"
 
@@ -177,21 +178,24 @@ __global__ __launch_bounds__(ROPE_THREADS) void k_rope(RopeArgs a, int tok) {
  * with amax * 2^-e <= 448 = 1.75 * 2^8, read off the bits of amax = m * 2^x: x - 8 where
  * m <= 1.75, else x - 7. Dividing by 2^e is exact; the hardware conversion rounds to nearest
  * even. Where rounding up would leave the range of the source type (its largest exponent, m
- * above 1.9375) the code is cut to 240, which is within half a step (2^-4) of the value. */
+ * above 1.9375) the code is cut to 240, which is within half a step (2^-4) of the value. MX4
+ * alike, with amax * 2^-e <= 7 = 1.75 * 2^2: a value between 6, the largest code, and 7 rounds to 6 and
+ * is off by no more than half the step of the codes above 4. e2m1 has no NaN, so a block that holds one, or an
+ * infinity, gets the scale byte 255, which the conversions back turn into NaN. Looking at every element for these took
+ * 12 us for 3 x 4093 rows of 4 heads of 128 into 4 bits, a look at the block's largest bits 9.1 (floor 6.3). */
 __device__ __forceinline__ bool fin(float x) { return __builtin_fabsf(x) < __builtin_huge_valf(); }
 
 /* over four neighbouring lanes */
-__device__ __forceinline__ float max_of4(float m) {
-    m = fmaxf(m, __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(m), 0xB1, 0xF, 0xF, true)));
-    return fmaxf(m, __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(m), 0x4E, 0xF, 0xF, true)));
+__device__ __forceinline__ unsigned max_of4(unsigned m) {
+    m = max(m, (unsigned)__builtin_amdgcn_update_dpp(0, (int)m, 0xB1, 0xF, 0xF, true));
+    return max(m, (unsigned)__builtin_amdgcn_update_dpp(0, (int)m, 0x4E, 0xF, 0xF, true));
 }
 
 /* The eight elements that a thread of either kernel takes of each of its tokens: octs threads a
  * token (grid.z of them where that is more than a workgroup), several tokens a workgroup where it is
  * less; which piece, head and element they are is worked out once for COPY_TOKENS tokens (16 x 4093
  * rows of 4 heads of 128 into 8 bits: 37 us, one by one 44, eight at once 15% more than four on 3 x
- * 4093). The piece's addresses and strides are read from the arguments again for each token, so the
- * four tokens' way from page id to store is walked one after the other: that bounds prompts. */
+ * 4093). The four tokens' page ids, then their rows, are under way together. */
 constexpr int COPY_TOKENS = 4;
 struct Place {
     const Piece *p;
@@ -231,71 +235,91 @@ __device__ __forceinline__ void put8(const Piece &p, const Spot &at, int h, int 
     if constexpr (bits_of(DST) == 16) {
         Elem<DST>::store8(dst + el * 2, true, v);
     } else {
-        int byte;
-        if constexpr (DST == DT_MX4) {
-            float m = 0.0f;
+        /* Both largest magnitudes of a scale of 1 are 1.75 * 2^TOP_E: 448, and 7 = 6 and half the step above it */
+        constexpr int TOP_E = DST == DT_MX4 ? 2 : 8, FULL = (SRC == DT_F16 ? 15 : 127) + 127 + 1 - TOP_E;
+        auto byte_of = [](unsigned m) { return max((int)(m >> 23) - TOP_E + ((m & 0x7fffff) > 0x600000), 1); };
+        /* magnitudes of floats order like their bits, infinities and NaN above all */
+        unsigned m = 0;
 #pragma unroll
-            for (int j = 0; j < 8; j++) m = fmaxf(m, fin(v[j]) ? __builtin_fabsf(v[j]) : __builtin_huge_valf());
-            m = max_of4(m);
-            /* least exponent with m <= 7 * 2^e = 1.75 * 2^(e + 2); 255 (a block of NaN) where m is infinite */
-            const int bits = (int)__float_as_uint(m);
-            const bool whole = fin(m);
-            byte = whole ? max((bits >> 23) - 2 + ((bits & 0x7fffff) > 0x600000), 1) : 255;
-            const float scale = mx_scale(whole ? byte : 127);
-            /* 4 would leave the source type's range: 3, within half a step */
-            const float top = (SRC == DT_F16 ? byte == 127 + 14 : byte == 127 + 126) ? 3.0f * scale : __builtin_huge_valf();
+        for (int j = 0; j < 8; j++) m = max(m, __float_as_uint(v[j]) & 0x7fffffffu);
+        m = max_of4(m);
+        int byte = byte_of(m);
+        float x[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) x[j] = v[j];
+        unsigned odd = 0;            /* elements whose code is NaN */
+        if (__any(m >= 0x7f800000u || byte == FULL)) {   /* rare: checked element by element, otherwise none can leave the codes' range */
+            const bool whole = m < 0x7f800000u;
+            if constexpr (DST == DT_MX4) {
+                if (!whole) byte = 255;                  /* a block of NaN */
+            } else {
+                unsigned f = 0;                          /* the largest of the finite ones */
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    if (!fin(v[j])) odd |= 1u << j;
+                    f = max(f, fin(v[j]) ? __float_as_uint(v[j]) & 0x7fffffffu : 0u);
+                }
+                byte = byte_of(max_of4(f));
+            }
+            /* the code above these would leave the source type's range: they are within half a step of the value */
+            const float top = byte == FULL ? (DST == DT_MX4 ? 3.0f : 240.0f) * mx_scale(byte) : __builtin_huge_valf();
+#pragma unroll
+            for (int j = 0; j < 8; j++) x[j] = (DST == DT_MX4 ? whole : fin(v[j])) ? fminf(fmaxf(v[j], -top), top) : 0.0f;
+        }
+        if constexpr (DST == DT_MX4) {
+            const float scale = mx_scale(byte == 255 ? 127 : byte);
             unsigned c = 0;
-            each<4>([&](auto j) {
-                const float a = whole ? fminf(fmaxf(v[2 * j], -top), top) : 0.0f, b = whole ? fminf(fmaxf(v[2 * j + 1], -top), top) : 0.0f;
-                c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, a, b, scale, j);   /* rounds to nearest even, above 6 to 6 */
-            });
+            each<4>([&](auto j) { c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x[2 * j], x[2 * j + 1], scale, j); });   /* to nearest even, above 6 to 6 */
             *(unsigned *)(dst + el / 2) = c;
         } else {
-            float m = 0.0f;
-#pragma unroll
-            for (int j = 0; j < 8; j++) m = fmaxf(m, fin(v[j]) ? __builtin_fabsf(v[j]) : 0.0f);
-            m = max_of4(m);
-            const int bits = (int)__float_as_uint(m);
-            byte = max((bits >> 23) - 8 + ((bits & 0x7fffff) > 0x600000), 1);   /* e + 127 */
             const float inv = __uint_as_float((unsigned)(254 - byte) << 23);
-            const float top = (SRC == DT_F16 ? byte == 127 + 8 : byte == 127 + 120) ? 240.0f : 448.0f;
-            unsigned c[2] = {0, 0};
+            u2 c;
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const float s = v[j] * inv;
-                const float t = fin(v[j]) ? fminf(fmaxf(s, -top), top) : 0.0f;
-                unsigned code = (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(t, t, 0, false) & 255u;
-                if (!fin(v[j])) code = 0x7f;
-                c[j >> 2] |= code << (8 * (j & 3));
+            for (int j = 0; j < 2; j++) {
+                int w = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * j] * inv, x[4 * j + 1] * inv, 0, false);
+                c[j] = (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(x[4 * j + 2] * inv, x[4 * j + 3] * inv, w, true);
             }
-            *(u2 *)(dst + el) = (u2){c[0], c[1]};
+            if (__any(odd))
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+                    if (odd >> j & 1) c[j >> 2] = (c[j >> 2] & ~(255u << (8 * (j & 3)))) | 0x7fu << (8 * (j & 3));
+            *(u2 *)(dst + el) = c;
         }
         if ((d & 31) == 0)
             p.rows.scales[(int64_t)at.page * p.rows.scale_page_stride + (int64_t)h * p.rows.scale_head_stride + el / MX_BLOCK] = (uint8_t)byte;
     }
 }
 
+/* Eight elements on their way from a caller's row into the cache: as they are where the types are the same */
 template <int SRC, int DST, bool WIDE>
-__device__ __forceinline__ void append_item(const CopyArgs &a, const Seq &q, const Piece &p, int tok, int h, int d) {
+struct Eight {
     using E = Elem<SRC>;
-    const Spot at = spot_of(a.b, q, tok);
-    if (at.page < 0) return;
-    const uint8_t *src = p.arr + (int64_t)(q.q0 + tok) * p.at + (int64_t)h * p.ah + (int64_t)d * E::size;
-    if constexpr (DST == SRC) {
-        uint8_t *dst = p.rows.data + (int64_t)at.page * p.rows.page_stride + (int64_t)h * p.rows.head_stride + ((int64_t)at.row * p.row_width + p.col + d) * 2;
-        if (WIDE) *(u4 *)dst = *(const u4 *)src;
+    u4 raw;
+    float v[8];
+    __device__ __forceinline__ void load(const uint8_t *src) {
+        if constexpr (DST != SRC) E::load8(src, WIDE, v);
+        else if constexpr (WIDE) raw = *(const u4 *)src;
         else {
             unsigned short w[8];
 #pragma unroll
             for (int j = 0; j < 8; j++) w[j] = ((const unsigned short *)src)[j];
-            *(u4 *)dst = (u4){w[0] | (unsigned)w[1] << 16, w[2] | (unsigned)w[3] << 16,
-                              w[4] | (unsigned)w[5] << 16, w[6] | (unsigned)w[7] << 16};
+            raw = (u4){w[0] | (unsigned)w[1] << 16, w[2] | (unsigned)w[3] << 16, w[4] | (unsigned)w[5] << 16, w[6] | (unsigned)w[7] << 16};
         }
-    } else {
-        float v[8];
-        E::load8(src, WIDE, v);
-        put8<SRC, DST>(p, at, h, d, v);
     }
+    __device__ __forceinline__ void store(const Piece &p, const Spot &at, int h, int d) const {
+        if constexpr (DST != SRC) put8<SRC, DST>(p, at, h, d, v);
+        else
+            *(u4 *)(p.rows.data + (int64_t)at.page * p.rows.page_stride + (int64_t)h * p.rows.head_stride + ((int64_t)at.row * p.row_width + p.col + d) * 2) = raw;
+    }
+};
+
+template <int SRC, int DST, bool WIDE>
+__device__ __forceinline__ void append_item(const CopyArgs &a, const Seq &q, const Piece &p, int tok, int h, int d) {
+    const Spot at = spot_of(a.b, q, tok);
+    if (at.page < 0) return;
+    Eight<SRC, DST, WIDE> x;
+    x.load(p.arr + (int64_t)(q.q0 + tok) * p.at + (int64_t)h * p.ah + (int64_t)d * Elem<SRC>::size);
+    x.store(p, at, h, d);
 }
 
 template <int SRC, int DST, bool WIDE>
@@ -304,11 +328,19 @@ __global__ __launch_bounds__(256) void k_kv_append(CopyArgs a) {
     const int n = min(q.n, a.b.max_q);
     const Place r = place_of(a);
     if (r.tok < 0) return;
+    const Piece p = *r.p;
+    const uint8_t *src = p.arr + (int64_t)q.q0 * p.at + (int64_t)r.h * p.ah + (int64_t)r.d * Elem<SRC>::size;
+    Spot at[COPY_TOKENS];
+    Eight<SRC, DST, WIDE> x[COPY_TOKENS];
 #pragma unroll
     for (int i = 0; i < COPY_TOKENS; i++) {
         const int tok = r.tok + i * r.step;
-        if (tok < n) append_item<SRC, DST, WIDE>(a, q, *r.p, tok, r.h, r.d);
+        at[i] = tok < n ? spot_of(a.b, q, tok) : Spot{-1, 0};
+        if (tok < n) x[i].load(src + (int64_t)tok * p.at);
     }
+#pragma unroll
+    for (int i = 0; i < COPY_TOKENS; i++)
+        if (at[i].page >= 0) x[i].store(p, at[i], r.h, r.d);
 }
 
 /* ---------------------------------------------------------------- writes of rotated rows
@@ -398,59 +430,66 @@ __global__ __launch_bounds__(ROPE_THREADS) void k_kv_append_rotated(RotatedArgs 
 
 /* ---------------------------------------------------------------- cache reads */
 template <int DST, int SRC, bool WIDE>
-__device__ __forceinline__ void read_item(const CopyArgs &a, const Seq &q, const Piece &p, int tok, int h, int d) {
-    using E = Elem<DST>;
-    const int pos = q.base + tok;
-    int page = -1;
-    if (pos >= 0 && pos < q.kv) page = a.b.pages[(int64_t)blockIdx.y * a.b.ld_pages + (pos >> a.b.page_shift)];
-    const int row = pos & ((1 << a.b.page_shift) - 1);
-    uint8_t *dst = p.arr + (int64_t)(q.q0 + tok) * p.at + (int64_t)h * p.ah + (int64_t)d * E::size;
-    float v[8] = {};
-    if (page_ok(a.b, page)) {
-        const uint8_t *src = p.rows.data + (int64_t)page * p.rows.page_stride + (int64_t)h * p.rows.head_stride;
-        const int64_t el = (int64_t)row * p.row_width + p.col + d;
-        if constexpr (SRC == DT_MX4) {
-            const unsigned c = *(const unsigned *)(src + el / 2);
-            const float s = mx_scale(p.rows.scales[(int64_t)page * p.rows.scale_page_stride + (int64_t)h * p.rows.scale_head_stride + el / MX_BLOCK]);
-            each<4>([&](auto j) {
-                const f2 x = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, j);
-                v[2 * j] = x[0]; v[2 * j + 1] = x[1];
-            });
-        } else if constexpr (SRC == DT_MX8) {
-            const u2 c = *(const u2 *)(src + el);
-            const float s = mx_scale(p.rows.scales[(int64_t)page * p.rows.scale_page_stride +
-                                                   (int64_t)h * p.rows.scale_head_stride + el / MX_BLOCK]);
-#pragma unroll
-            for (int j = 0; j < 2; j++) {
-                const f2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)c[j], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)c[j], true);
-                v[4 * j] = lo[0] * s; v[4 * j + 1] = lo[1] * s; v[4 * j + 2] = hi[0] * s; v[4 * j + 3] = hi[1] * s;
-            }
-        } else {
-            if constexpr (SRC == DST) {
-                const u4 w = *(const u4 *)(src + el * 2);
-                if (WIDE) *(u4 *)dst = w;
-                else {
-#pragma unroll
-                    for (int j = 0; j < 8; j++) ((unsigned short *)dst)[j] = (unsigned short)(w[j >> 1] >> (16 * (j & 1)));
-                }
-                return;
-            }
-            Elem<SRC>::load8(src + el * 2, true, v);
-        }
-    }
-    E::store8(dst, WIDE, v);
-}
-
-template <int DST, int SRC, bool WIDE>
 __global__ __launch_bounds__(256) void k_kv_read(CopyArgs a) {
+    using E = Elem<DST>;
     const Seq q = seq_of(a.b, blockIdx.y);
     const int n = min(q.n, a.b.max_q);
     const Place r = place_of(a);
     if (r.tok < 0) return;
+    const Piece p = *r.p;
+    uint8_t *dst = p.arr + (int64_t)q.q0 * p.at + (int64_t)r.h * p.ah + (int64_t)r.d * E::size;
+    Spot at[COPY_TOKENS];
+    u4 w[COPY_TOKENS];              /* 8 stored elements: 16, 8 or 4 bytes */
+    unsigned sc[COPY_TOKENS];
 #pragma unroll
     for (int i = 0; i < COPY_TOKENS; i++) {
         const int tok = r.tok + i * r.step;
-        if (tok < n) read_item<DST, SRC, WIDE>(a, q, *r.p, tok, r.h, r.d);
+        at[i] = tok < n ? spot_of(a.b, q, tok) : Spot{-1, 0};
+    }
+#pragma unroll
+    for (int i = 0; i < COPY_TOKENS; i++) {
+        w[i] = (u4){0, 0, 0, 0};    /* zeros for rows that are not there, in every format */
+        sc[i] = 127;
+        if (at[i].page < 0) continue;
+        const uint8_t *src = p.rows.data + (int64_t)at[i].page * p.rows.page_stride + (int64_t)r.h * p.rows.head_stride;
+        const int64_t el = (int64_t)at[i].row * p.row_width + p.col + r.d;
+        if constexpr (bits_of(SRC) == 16) w[i] = *(const u4 *)(src + el * 2);
+        else {
+            if constexpr (SRC == DT_MX4) w[i][0] = *(const unsigned *)(src + el / 2);
+            else {
+                const u2 c = *(const u2 *)(src + el);
+                w[i][0] = c[0]; w[i][1] = c[1];
+            }
+            sc[i] = p.rows.scales[(int64_t)at[i].page * p.rows.scale_page_stride + (int64_t)r.h * p.rows.scale_head_stride + el / MX_BLOCK];
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < COPY_TOKENS; i++) {
+        const int tok = r.tok + i * r.step;
+        if (tok >= n) return;
+        uint8_t *to = dst + (int64_t)tok * p.at;
+        if constexpr (SRC == DST) {
+            if (WIDE) *(u4 *)to = w[i];
+            else
+#pragma unroll
+                for (int j = 0; j < 8; j++) ((unsigned short *)to)[j] = (unsigned short)(w[i][j >> 1] >> (16 * (j & 1)));
+        } else {
+            float v[8];
+            const float s = mx_scale(sc[i]);
+            if constexpr (SRC == DT_MX4)
+                each<4>([&](auto j) {
+                    const f2 x = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[i][0], s, j);
+                    v[2 * j] = x[0]; v[2 * j + 1] = x[1];
+                });
+            else if constexpr (SRC == DT_MX8)
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    const f2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[i][j], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[i][j], true);
+                    v[4 * j] = lo[0] * s; v[4 * j + 1] = lo[1] * s; v[4 * j + 2] = hi[0] * s; v[4 * j + 3] = hi[1] * s;
+                }
+            else Elem<SRC>::load8((const uint8_t *)&w[i], true, v);
+            E::store8(to, WIDE, v);
+        }
     }
 }
 

@@ -431,6 +431,33 @@ __global__ __launch_bounds__(64 * SCORE_WAVES) void k_block_scores_many(SelectAr
     }
 }
 
+/* f over all lanes, in every lane: lanes ^ 1, ^ 2, the halves of 8 and of 16 turned round, lanes ^ 16, ^ 32 */
+template <class F>
+__device__ __forceinline__ unsigned over_wave(unsigned x, F f) {
+    auto with = [&](auto ctrl) __attribute__((always_inline)) { x = f(x, (unsigned)__builtin_amdgcn_update_dpp((int)x, (int)x, ctrl.value, 0xF, 0xF, false)); };
+    with(std::integral_constant<int, 0xB1>{});
+    with(std::integral_constant<int, 0x4E>{});
+    with(std::integral_constant<int, 0x141>{});
+    with(std::integral_constant<int, 0x140>{});
+    const auto a = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    x = f(a[0], a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return f(b[0], b[1]);
+}
+/* the sum of the lanes up to this one: within 16 lanes by shifts of 1, 2, 4, 8, then lane 15's to the row behind it
+ * and lane 31's to the upper half */
+__device__ __forceinline__ unsigned sum_upto(unsigned x) {
+    auto with = [&](auto ctrl, auto rows) __attribute__((always_inline)) { x += (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, ctrl.value, rows.value, 0xF, false); };
+    using std::integral_constant;
+    with(integral_constant<int, 0x111>{}, integral_constant<int, 0xF>{});
+    with(integral_constant<int, 0x112>{}, integral_constant<int, 0xF>{});
+    with(integral_constant<int, 0x114>{}, integral_constant<int, 0xF>{});
+    with(integral_constant<int, 0x118>{}, integral_constant<int, 0xF>{});
+    with(integral_constant<int, 0x142>{}, integral_constant<int, 0xA>{});
+    with(integral_constant<int, 0x143>{}, integral_constant<int, 0xC>{});
+    return x;
+}
+
 /* ---------------------------------------------------------------- the best of a token
  *
  * W waves take one token and kv head, each its share of the blocks, in order: four waves, or one where the keys of all
@@ -493,11 +520,8 @@ __global__ __launch_bounds__(PICK_THREADS) void k_block_pick(SelectArgs a) {
         kept += __popcll(__ballot(k == ~0u));
         if (k && k != ~0u) { lo = min(lo, k); hi = max(hi, k); }
     });
-#pragma unroll
-    for (int d = 32; d; d >>= 1) {
-        lo = min(lo, (unsigned)__shfl_xor((int)lo, d));
-        hi = max(hi, (unsigned)__shfl_xor((int)hi, d));
-    }
+    lo = over_wave(lo, [](unsigned x, unsigned y) { return min(x, y); });
+    hi = over_wave(hi, [](unsigned x, unsigned y) { return max(x, y); });
     if constexpr (W > 1) {
         if (lane == 0) { lds_lo[wave] = lo; lds_hi[wave] = hi; lds_can[wave] = can; lds_kept[wave] = kept; }
         can = kept = 0;
@@ -525,12 +549,7 @@ __global__ __launch_bounds__(PICK_THREADS) void k_block_pick(SelectArgs a) {
                 unsigned c[4], sum = 0;
 #pragma unroll
                 for (int j = 0; j < 4; j++) { c[j] = bins[round][255 - 4 * lane - j]; sum += c[j]; }
-                unsigned upto = sum;
-#pragma unroll
-                for (int d = 1; d < 64; d <<= 1) {
-                    const unsigned x = (unsigned)__shfl_up((int)upto, d);
-                    if (lane >= d) upto += x;
-                }
+                const unsigned upto = sum_upto(sum);
                 unsigned before = upto - sum, bin = 0, over = 0, in = 0;
                 bool here = false;
 #pragma unroll
