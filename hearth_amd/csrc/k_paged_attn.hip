@@ -243,9 +243,15 @@ struct Few {
 };
 
 /* BLOCKS: of the rows of chosen blocks, which stand one after the other in the place of the
- * sequence's. A workgroup's columns are then heads of one token, since every token has blocks of its own. */
-/* ONE: a step's rows lie in one page (and block), which is looked up once. */
-template <class T, int BITS, int D, bool BLOCKS, bool ONE>
+ * sequence's. A workgroup's columns are then heads of one token, since every token has blocks of its own.
+ * ONE: a step's rows lie in one page (and block), which is looked up once.
+ * BY_LDS: K by way of LDS. Blocks that many tokens choose come from the chip's caches, where the
+ * lines that K's loads touch bound the kernel (a row of 16 lanes' loads at a time from as many rows;
+ * by LDS whole rows): 600 tokens over 16 blocks of 64 rows each, by LDS and straight, 16-bit rows 66 and
+ * 95 us, 8-bit 62 and 77; 4-bit, whose rows are a quarter of a line's, 61 and 57. Single tokens'
+ * blocks come from memory, and straight is faster (32 of them over 32 blocks each, 16-bit rows: 29.5 and
+ * 27.7 us). */
+template <class T, int BITS, int D, bool BLOCKS, bool ONE, bool BY_LDS>
 __global__ __launch_bounds__(64 * FEW_WAVES, D <= 128 ? 2 : 1) void k_attend_few(AttendArgs a) {
     using F = Few<T, BITS, D>;
     using v8 = typename T::v8;
@@ -256,7 +262,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES, D <= 128 ? 2 : 1) void k_attend_few
     constexpr int PL = F::PL, NB = F::NB, BD = F::BD, CT = 16, NT = F::NT, STEP = F::STEP;
     constexpr int PER = ONE ? NT : 1, NL = NT / PER, RUN = 16 * PER;   /* tiles of a look-up, look-ups of a step, their rows */
     __shared__ float lds_o[FEW_WAVES][16][BD + 4];
-    __shared__ __align__(16) uint8_t lds_k[BLOCKS && BITS > 4 ? FEW_WAVES : 1][BLOCKS && BITS > 4 ? STEP * F::RB : 16];
+    __shared__ __align__(16) uint8_t lds_k[BY_LDS ? FEW_WAVES : 1][BY_LDS ? STEP * F::RB : 16];
     __shared__ float lds_m[FEW_WAVES][CT], lds_l[FEW_WAVES][CT];
     __shared__ unsigned lds_some[FEW_WAVES];   /* bit c: column c attends a row of the wave's */
 
@@ -300,17 +306,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES, D <= 128 ? 2 : 1) void k_attend_few
     const int hi = BLOCKS ? end : min(end, (sp + 1) * a.chunk);
     const int full = a.b.mask ? q.base : q.base + t_first + 1;
     const int *list = BLOCKS ? a.chosen + (int64_t)(q.q0 + only) * a.ct + (int64_t)kvh * a.ch : nullptr;
-    int stop = hi;                                                                     /* of the steps */
-    if constexpr (BLOCKS) {   /* behind the last block that has rows to attend: lists of early tokens end in entries that are none */
-        const int end_entry = min(a.top, (int)(((int64_t)(sp + 1) * a.chunk + (1 << a.block_shift) - 1) >> a.block_shift));
-        int used = 0;
-        for (int e = sp * a.chunk >> a.block_shift; e < end_entry; e += 64) {
-            const int blk = e + lane < end_entry ? list[e + lane] : -1;
-            const unsigned long long has = __ballot(blk >= 0 && ((int64_t)blk << a.block_shift) < hi);
-            if (has) used = e + 64 - __builtin_clzll(has);
-        }
-        stop = min(used << a.block_shift, (sp + 1) * a.chunk);
-    }
+    const int stop = BLOCKS ? min(a.top << a.block_shift, (sp + 1) * a.chunk) : hi;   /* of the steps */
 
     /* which of the 64 rows from t0 on this lane's column attends (where their pages exist) */
     auto attended = [&](int t0) {
@@ -361,10 +357,6 @@ __global__ __launch_bounds__(64 * FEW_WAVES, D <= 128 ? 2 : 1) void k_attend_few
     };
     typename F::K kr;
     typename F::V vw;
-    /* Blocks that many tokens choose come from the chip's caches, where the lines that K's loads touch bound the kernel
-     * (600 tokens over 16 blocks each, by LDS and straight: 16-bit rows 66 and 95 us, 8-bit 62 and 77, 4-bit, whose
-     * rows are a quarter of a line's, 61 and 57). */
-    constexpr bool BY_LDS = BLOCKS && BITS > 4;
     auto load_k = [&](const Run (&x)[NL]) __attribute__((always_inline)) {
         const uint8_t *rows[NL];
 #pragma unroll
@@ -419,7 +411,11 @@ __global__ __launch_bounds__(64 * FEW_WAVES, D <= 128 ? 2 : 1) void k_attend_few
     for (int t0 = first; t0 < stop; t0 += ROUND) {
 #pragma unroll
         for (int z = 0; z < NL; z++) now[z] = next[z];
-        load_v(now);
+        /* lists of early tokens end in entries that are none */
+        bool none = BLOCKS;
+#pragma unroll
+        for (int z = 0; z < NL; z++) none = none && now[z].page < 0;
+        if (!none) load_v(now);
 #pragma unroll
         for (int z = 0; z < NL; z++) {
             next[z] = look(t0 + ROUND + RUN * z, blk[z]);
@@ -428,11 +424,12 @@ __global__ __launch_bounds__(64 * FEW_WAVES, D <= 128 ? 2 : 1) void k_attend_few
         in_order();
         f4 s[NT];
         if constexpr (BY_LDS) F::read_k(kr, lds_k[wave], g, lc);
-        F::scores(kr, g, qf, s);
+        if (!none) F::scores(kr, g, qf, s);
         in_order();
 #pragma unroll
         for (int z = 0; z < NL; z++) next[z] = checked(next[z]);
         if (t0 + ROUND < stop) load_k(next);
+        if (none) continue;
         in_order();
         const bool whole = whole_at(now);
         v8 pf[NT / 2];
@@ -626,18 +623,26 @@ __global__ __launch_bounds__(JOIN_THREADS) void k_attend_join(AttendArgs a) {
     if (a.lse && e == 0) a.lse[row] = L == 0.0f ? NINF : (M + __log2f(L)) * 0.69314718055994531f;
 }
 
+/* Tokens of a sequence from which on K goes by LDS (see BY_LDS; one sequence, 16 blocks a token, by LDS
+ * and straight: 1 to 8 tokens level, 16 10.3 and 11.4, 128 17.4 and 24.4 us) */
+constexpr int SHARING = 16;
+
 template <class T, int BITS, int D, bool BLOCKS>
 void few_t(const AttendArgs &a, hipStream_t st) {
     const int tiles = BLOCKS ? a.b.max_q * ((a.group + 15) / 16) : (a.b.max_q * a.group + 15) / 16;
     const dim3 grid((unsigned)a.n_splits * a.kv_heads * tiles, 1, a.b.n_seqs);
     constexpr int STEP = 16 * few_tiles(BITS);
     const bool one = 1 << a.b.page_shift >= STEP && (!BLOCKS || 1 << a.block_shift >= STEP);
+    auto launch = [&](auto one, auto lds) {
+        hipLaunchKernelGGL((k_attend_few<T, BITS, D, BLOCKS, one.value, lds.value>), grid, dim3(64 * FEW_WAVES), 0, st, a);
+    };
+    constexpr std::true_type yes;
+    constexpr std::false_type no;
+    if constexpr (BLOCKS && BITS > 4)
+        if (one && a.b.max_q >= SHARING) return launch(yes, yes);
     if constexpr (BITS == 4 || BLOCKS)   /* of two look-ups a step one makes no difference to the others, which wait for memory */
-        if (one) {
-            hipLaunchKernelGGL((k_attend_few<T, BITS, D, BLOCKS, true>), grid, dim3(64 * FEW_WAVES), 0, st, a);
-            return;
-        }
-    hipLaunchKernelGGL((k_attend_few<T, BITS, D, BLOCKS, false>), grid, dim3(64 * FEW_WAVES), 0, st, a);
+        if (one) return launch(yes, no);
+    launch(no, no);
 }
 
 template <class T, int DV>
