@@ -285,6 +285,42 @@ def test_sparse_split(kind, store, width):
     sparse(base._gen(width + 1), kind, store, 4, 1, width, [20000], [1], 64, 64, 200)
 
 
+@pytest.mark.parametrize("kind,store", STORES)
+@pytest.mark.parametrize("heads,kv_heads,width,page,block", [(8, 2, 128, 64, 64), (7, 1, 64, 64, 32), (4, 4, 256, 64, 64), (40, 2, 64, 256, 64), (16, 1, 128, 256, 128)])
+def test_sparse_of_many_tokens(kind, store, heads, kv_heads, width, page, block):
+    """Sequences of 15 tokens at most and of 16; lists with gaps of whole steps, without any block, and trees."""
+    for n in (15, 16):
+        g = base._gen(heads + width + n)
+        lens, news = [1, 70, 700, n], [1, 3, n, n]
+        chosen = random_blocks(g, lens, news, kv_heads, 5, block)
+        chosen[4:8] = -1                                              # the third sequence's first four tokens: none,
+        chosen[5, :, 0] = chosen[6, :, 4] = 0                         # the first entry, the last,
+        chosen[7, :, 1] = chosen[7, :, 3] = torch.arange(kv_heads, dtype=torch.int32) % (700 // block)   # one twice between gaps
+        chosen[7, :, 3] += 1
+        sparse(g, kind, store, heads, kv_heads, width, lens, news, page, block, 5, chosen=chosen)
+    news = [33, 16, 1]
+    sparse(base._gen(width), kind, store, heads, kv_heads, width, [500, 16, 90], news, page, block, 9, trees=[O.tree(n) for n in news])
+
+
+@pytest.mark.parametrize("kind,store", STORES)
+def test_sparse_of_many_tokens_and_bad_rows(kind, store):
+    """An infinity in a later row of the tokens' own block, a NaN there, pages that are not there."""
+    def edit(c, pages):
+        v = c["v"].view(torch.uint8 if store in ("mx8", "mx4") else torch.int16)
+        if store == "mx4":
+            c["vs"][pages[0, 3].item(), :, 15] = 255
+        else:
+            v[pages[0, 3].item(), 0, 14, 3] = {"bf16": 0x7f80, "f16": 0x7c00, "mx8": 0x7f}[store]
+            v[pages[0, 3].item(), 1, 15, 5] = {"bf16": 0x7fc0, "f16": 0x7e00, "mx8": 0xff}[store]
+        v[pages[0, 3].item(), :, 20:] = 0x7fff if v.dtype == torch.int16 else 0x7f
+    g = base._gen(77)
+    pages, n_pages = torch.tensor([[1, 99, 4, 2, 3], [0, 5, -8, 7, 6]], dtype=torch.int32), 8
+    lens, news = [3 * 64 + 17, 300], [17, 20]
+    chosen = torch.arange(5, dtype=torch.int32).expand(37 + 2, 2, 5).contiguous()
+    got = sparse(g, kind, store, 8, 2, 128, lens, news, 64, 64, 5, pages=pages, n_pages=n_pages, edit=edit, chosen=chosen)
+    assert got[:14].isfinite().all() and not got[15:17].isfinite().all()
+
+
 def test_every_block_is_the_attention():
     """All blocks chosen: the bits of attend where the rows fall into the same steps, whatever the group."""
     g = base._gen(31)
