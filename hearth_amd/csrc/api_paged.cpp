@@ -192,7 +192,7 @@ bool attend_shape_ok(const hearth_gpu_cache *c, const hearth_gpu_batch *b, int h
 int64_t part_bytes(const hearth_gpu_cache &c, const hearth_gpu_batch &b, int heads, Split &s) {
     const Batch o = batch_of(b, c);
     if (!o.n_seqs || !o.max_q) { s = {0x40000000, 1, false}; return 0; }
-    s = attend_split(o.n_seqs, b.max_q, o.kv_cap, heads, c.n_heads, !c.v.data);
+    s = attend_split(o.n_seqs, b.max_q, o.kv_cap, heads, c.n_heads, !c.v.data, c.dtype == HEARTH_GPU_MX4);
     const int64_t dv = c.v.data ? c.width : 512;
     return s.n == 1 ? 0 : (int64_t)o.n_tokens * heads * s.n * (dv + 2) * (int64_t)sizeof(float);
 }

@@ -149,7 +149,7 @@ void kv_read(const CopyArgs &a, int dst_dtype, int cache_dtype, bool aligned, hi
  * kernel of many query rows takes the call. Depends on the host-side fields only, and not on the
  * call's token count. latent: the kernels of attend_latent. */
 struct Split { int chunk, n; bool many; };
-Split attend_split(int n_seqs, int max_q, int kv_cap, int heads, int kv_heads, bool latent);
+Split attend_split(int n_seqs, int max_q, int kv_cap, int heads, int kv_heads, bool latent, bool four);
 void attend(const AttendArgs &a, int q_dtype, int cache_dtype, int width, bool many, hipStream_t st);
 Split blocks_split(int n_seqs, int max_q, int rows, int heads, int kv_heads);
 void attend_blocks(const AttendArgs &a, int q_dtype, int cache_dtype, int width, hipStream_t st);

@@ -11,7 +11,13 @@
  * It is bound by the cache's bytes: 268 MB of one token over 131071 rows in 49.7 us (5.4 TB/s), 178
  * MB of 32 tokens over 8-bit rows in 44 us (4.1 TB/s), the joins 5 us each. Nothing of the cache
  * goes through LDS (no row is read by two waves), V is under way before the scores and the next K
- * before the sums (32 tokens over 8-bit rows with each load where it is used: 114 us, not 48).
+ * before the sums (32 tokens over 8-bit rows with each load where it is used: 114 us, not 48). Rows
+ * of 4 bits (32 tokens, 92 MB: 24.7 us, 3.7 TB/s) are bound by their conversions and the exchanges
+ * between lanes as much as by bytes: an instruction converts two codes a lane in 4.5 cycles, 72 for
+ * 16 rows of 128, whose matrix products take 64.
+ * Chosen blocks: 32 tokens over 32 blocks of 64 16-bit rows each 27.7 us (134 MB, 4.8 TB/s), 600
+ * tokens over 16 blocks of 8-bit rows each 66.6 (from the chip's caches, 8 of a
+ * tile's 16 columns in use for 8 heads a kv head; bound by the conversions, 24 M vector instructions).
  *
  * Scores, maxima, sums of probabilities and of rows are float32. The probabilities alone are rounded
  * to the 16-bit type, in this kernel and the two for many rows: the matrix units take both factors in
@@ -85,9 +91,9 @@ struct Few {
                 for (int i = 0; i < SW; i++) k.s[u][i] = ((const unsigned_any *)q)[i];
         }
     }
-    /* K by way of LDS: 64 lanes bring in 1 KiB of whole rows an instruction, where 16 lanes that read 16 bytes of 16 rows
-     * each touch 16 cache lines. The 16-byte pieces of a row are exchanged by row, so that those 16 lanes meet 16 different
-     * columns of the 256 bytes of banks. */
+    /* K by way of LDS: 64 lanes bring in 1 KiB of whole rows an instruction, where 16 lanes that read 16 bytes
+     * of 16 rows each touch 16 cache lines. The 16-byte pieces of a row are exchanged by row, so that those 16
+     * lanes meet 16 different columns of the 256 bytes of banks. */
     static constexpr int P = RB / 16, RI = 1024 / RB, N = STEP * RB / 1024;   /* pieces of a row, rows an instruction, instructions */
     static __device__ __forceinline__ int swz(int r) { return P >= 16 ? r & 15 : r / (16 / P) & (P - 1); }
     /* z: instruction; rows: the first of its rows */
@@ -150,8 +156,8 @@ struct Few {
                     s[u] = T::mfma16(__builtin_bit_cast(v8, w), q[SL * i + h], s[u]);
                 }
     }
-    /* The softmax of a lane's scores x in base 2, against the running maximum m: x become the probabilities, packed into
-     * pf, l their sum; sums and l are rescaled where a maximum has grown by more than GROWTH. */
+    /* The softmax of a lane's scores x in base 2, against the running maximum m: x become the probabilities,
+     * packed into pf, l their sum; sums and l are rescaled where a maximum has grown by more than GROWTH. */
     template <int GROWTH>
     static __device__ __forceinline__ void weights(float (&x)[4 * NT], v8 (&pf)[NT / 2], f4 (&acc)[NB * PL], float &m, float &l) {
         float mx = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
@@ -178,8 +184,8 @@ struct Few {
             pf[k] = __builtin_bit_cast(v8, (u4){T::pack(p[0], p[1]), T::pack(p[2], p[3]), T::pack(p[4], p[5]), T::pack(p[6], p[7])});
         }
     }
-    /* acc += V^T P^T. ALL: every row counts as it is; otherwise rows for which there(tile, row of the tile) is false are taken
-     * as zeros, and so are infinities and NaN, which `odd` tells of */
+    /* acc += V^T P^T. ALL: every row counts as it is; otherwise rows for which there(tile, row of the tile) is
+     * false are taken as zeros, and so are infinities and NaN, which `odd` tells of */
     template <bool ALL, class THERE>
     static __device__ __forceinline__ void add(f4 (&acc)[NB * PL], const V &v, const v8 (&pf)[NT / 2], int lc, bool &odd, THERE there) {
 #pragma unroll
@@ -661,17 +667,20 @@ void join_t(const AttendArgs &a, hipStream_t st) {
  * sequences of 4096 rows, width 128, few against many: 8-bit rows 42 and 51 us at 32 columns, 82
  * and 51 at 40; 16-bit ones 47 and 44 at 32, 111 and 46 at 48; of width 256 108 and 132 at 24. */
 static bool takes_many(int64_t cols) { return cols > 32; }
+/* of 4-bit rows, whose bytes are few: passes over the cache cost less than rows made 16 bits in LDS (27 and 46 us
+ * at 32 columns, 35 and 49 at 64, 53 and 53 at 96; of width 256 118 and 149 at 96) */
+static bool takes_many4(int64_t cols) { return cols > 96; }
 
-/* Rows a split takes: enough workgroups for the 256 units, two each (one of the latent form, which
- * fills a unit; with four of few rows a unit 32 tokens over 2048 to 8192 8-bit rows took 51 us, not
- * 45, and one over 131071 16-bit rows 59, not 55: more partial sums to write and join). Few query
- * rows are not split below 512 rows: one launch of 500 rows takes 10 us where a split one and its
- * join take 12.5; at 1000 rows two splits take 16 us and eight 15. Many are split down to 192 rows (85 tokens over 2132 rows:
- * 26 us, at 128 rows 31; 64 over 500: 17 us, at 256 rows 20), the latent form down to 128 (1 token
- * over 500 rows: 21 us, at 256 rows 26; 1 over 8192: 30 us, at 64 rows 35). */
-Split attend_split(int n_seqs, int max_q, int kv_cap, int heads, int kv_heads, bool latent) {
+/* Rows a split takes: enough workgroups for the 256 units, two each (one of the latent form, which fills a
+ * unit; with four of few rows a unit 32 tokens over 2048 to 8192 8-bit rows took 51 us, not 45, and one over
+ * 131071 16-bit rows 59, not 55: more partial sums to write and join). Few query rows are not split below 512
+ * rows: one launch of 500 rows takes 10 us where a split one and its join take 12.5; at 1000 rows two splits
+ * take 16 us and eight 15. Many are split down to 192 rows (85 tokens over 2132 rows: 26 us, at 128 rows 31; 64
+ * over 500: 17 us, at 256 rows 20), the latent form down to 128 (1 token over 500 rows: 21 us, at 256 rows 26;
+ * 1 over 8192: 30 us, at 64 rows 35). */
+Split attend_split(int n_seqs, int max_q, int kv_cap, int heads, int kv_heads, bool latent, bool four) {
     const int64_t cols = (int64_t)max_q * (heads / kv_heads);
-    const bool many = !latent && takes_many(cols);
+    const bool many = !latent && (four ? takes_many4(cols) : takes_many(cols));
     const int tile = latent ? 64 : many ? 128 : 16, step = latent ? 64 : 128, at_once = latent ? 256 : 512;
     const int64_t wgs = std::max<int64_t>((int64_t)n_seqs * kv_heads * ((cols + tile - 1) / tile), 1);
     const int64_t want = std::max<int64_t>(1, at_once / wgs);

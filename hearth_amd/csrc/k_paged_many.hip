@@ -134,8 +134,8 @@ __global__ __launch_bounds__(64 * MANY_WAVES, D <= 128 ? 2 : 1) void k_attend_ma
     constexpr int RW = M::ROWS / 4, LANES = M::PIECES / PL, RI = 64 / LANES, N = RW / RI;   /* lanes of a row, rows an instruction, instructions */
     constexpr int RB = D * BITS / 8;                                                          /* bytes of a row */
     static_assert(N >= 1 && N * RI == RW);
-    /* 4-bit: 16 lanes write one piece of 16 rows, which lie in different banks; lanes by rows met four to a column (1000
-     * tokens over 5000 rows: 128 us, so 118; 8-bit rows are faster by rows) */
+    /* 4-bit: 16 lanes write one piece of 16 rows, which lie in different banks; lanes by rows met four to a
+     * column (1000 tokens over 5000 rows: 128 us, so 118; 8-bit rows are faster by rows) */
     const int my = wave * RW, lr = BITS == 4 ? lane % RI : lane / LANES, lp = BITS == 4 ? lane / RI : lane % LANES;
     /* 16-bit: byte of a lane's pieces in memory (the z-th instruction's 1 KiB further, there and in LDS) */
     int off[N];

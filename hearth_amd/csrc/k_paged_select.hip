@@ -61,7 +61,9 @@ __device__ __forceinline__ void load8(const uint8_t *data, const uint8_t *sc, in
  *
  * A workgroup takes one block and head: D / 8 threads a row, eight elements each, 2048 / D rows at
  * once; the rows' minima and maxima meet across lanes and then through LDS. The blocks are those that
- * hold rows of the call's tokens, taken over all of their rows that exist. */
+ * hold rows of the call's tokens, taken over all of their rows that exist. One block of 64 rows (16 KiB of
+ * 16-bit ones) is a chain of latencies: length, page, rows, LDS, 4.3 us and a launch's own 2; the blocks of a
+ * prompt run side by side. */
 constexpr int BOUND_THREADS = 256;
 
 template <int DT, int D>
@@ -140,14 +142,14 @@ __global__ __launch_bounds__(BOUND_THREADS) void k_key_bounds(BoundsArgs a) {
  * LDS. Columns are blocks, 16 a matrix instruction: a lane ends with four rows of one block, whose maximum over a
  * token's heads is taken in its registers and with the lanes 16 and 32 further. A wave's instructions bound
  * it (rows and columns the other way round, with the maximum between neighbouring lanes, took 21 us for 600 tokens
- * over 313 blocks). */
+ * over 313 blocks, k_block_scores_many takes 12.7); one token over 2048 blocks, 4.9 us, waits for latencies. */
 constexpr int SCORE_WAVES = 4, MAX_CHUNKS = 8;
 
 /* heads of a token in a tile of 16 rows */
 __host__ __device__ inline int padded(int group) { return group > 8 ? 16 : group > 4 ? 8 : group > 2 ? 4 : group; }
 
-/* Sixteen rows of queries as whole numbers: a lane's row lc, 16 elements of each 64 (from 16 g on), positive and negative
- * parts, and the step */
+/* Sixteen rows of queries as whole numbers: a lane's row lc, 16 elements of each 64 (from 16 g on), positive
+ * and negative parts, and the step */
 template <int KS> struct Rows16 { i4 up[KS], down[KS]; int byte; };
 
 /* p: a lane's row. v * r + 3 * 2^22 rounds v / step to nearest even into the low byte of the float's bits (two's
@@ -203,8 +205,9 @@ __device__ __forceinline__ Rows16<KS> quantise(const uint8_t *p, int g, bool on)
     return c;
 }
 
-/* What becomes of a lane's four rows (rows 4 g .. of tokens of `pad` heads each) of one block: the token's maxima into `out`,
- * the first token's place of this block. -infinity tells a block whose page is not there; an overflow stays above it. */
+/* What becomes of a lane's four rows (rows 4 g .. of tokens of `pad` heads each) of one block: the token's
+ * maxima into `out`, the first token's place of this block. -infinity tells a block whose page is not there; an
+ * overflow stays above it. */
 struct Put {
     float *out;
     int64_t ld_tok;
@@ -341,7 +344,7 @@ __global__ __launch_bounds__(64 * SCORE_WAVES) void k_block_scores(SelectArgs a)
 
 /* Many tokens: four waves with 16 rows each share the bounds of 64 blocks a step, which come in by whole rows of
  * codes (16 lanes a row of width 128) and through LDS: read by each wave for itself, 16 bytes of a row a lane, they
- * were bound by the cache lines that a load touches (600 tokens over 313 blocks: 20 us). Pieces of 16 bytes are
+ * were bound by the cache lines that a load touches (600 tokens over 313 blocks: 20 us, so 12.7). Pieces of 16 bytes are
  * exchanged by row, so that 16 lanes that read one piece of 16 rows meet no bank conflict. The next step's
  * are in flight meanwhile (two buffers). */
 template <class T, int D>
@@ -461,7 +464,7 @@ __device__ __forceinline__ unsigned sum_upto(unsigned x) {
 /* ---------------------------------------------------------------- the best of a token
  *
  * W waves take one token and kv head, each its share of the blocks, in order: four waves, or one where the keys of all
- * blocks fit its registers, which then waits for no other (2400 rows of 313 blocks: four waves 9.4 us). Keys are the
+ * blocks fit its registers, which then waits for no other (2400 rows of 313 blocks: 7.4 us, four waves 9.4). Keys are the
  * scores' bits in an order of unsigned numbers, the greatest for blocks that are kept in any case, 0 for those that
  * cannot be taken. Keys of one row lie close together, so the top-th greatest is looked for within their range: 256
  * bins over it, then over the bin that holds it, until the bin is taken whole or holds one value (two rounds in most rows).
@@ -627,9 +630,9 @@ void key_bounds(const BoundsArgs &a, int cache_dtype, int width, hipStream_t st)
 
 int select_group_limit() { return 16 * MAX_CHUNKS; }
 
-/* Blocks are shared out among workgroups until four are there for each unit, 64 at least each (16 a wave; 600 tokens over
- * 313 blocks: 13.2 us, with two 15).
- * Tokens that fill the rows of four waves share their blocks' bounds. */
+/* Blocks are shared out among workgroups until four are there for each unit, 64 at least each (16 a wave; 600
+ * tokens over 313 blocks: 12.7 us, with two 15). Tokens that fill the rows of four waves share their blocks'
+ * bounds. */
 void select_blocks(SelectArgs a, int q_dtype, int width, int n_blocks, hipStream_t st) {
     int tpt = a.group <= 16 ? 16 / padded(a.group) : 1;
     const bool many = a.group <= 16 && a.b.max_q >= SCORE_WAVES * tpt;

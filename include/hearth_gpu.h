@@ -308,9 +308,9 @@ typedef struct hearth_gpu_rows {
     int64_t scale_page_stride, scale_head_stride;
 } hearth_gpu_rows;
 
-/* A cache: k and v of the same shape, or k alone (v.data NULL: latent rows, which hold a
- * token's latent vector and then its rotated part). page: a power of two from 16 to 4096;
- * width: a multiple of 32 up to 1024; dtype: HEARTH_F16, HEARTH_BF16, HEARTH_GPU_MX8 or HEARTH_GPU_MX4. */
+/* A cache: k and v of the same shape, or k alone (v.data NULL: latent rows, which hold a token's
+ * latent vector and then its rotated part). page: a power of two from 16 to 4096; width: a multiple
+ * of 32 up to 1024; dtype: HEARTH_F16, HEARTH_BF16, HEARTH_GPU_MX8 or HEARTH_GPU_MX4. */
 typedef struct hearth_gpu_cache {
     hearth_gpu_rows k, v;
     int32_t dtype, n_pages, n_heads, page, width;
@@ -353,29 +353,31 @@ HEARTH_API int hearth_gpu_rope(const hearth_gpu_array *x, const hearth_gpu_array
                                const double *freqs, int n_freqs, int offset, int interleaved, int inverse,
                                double factor, int dev, void *stream);
 
-/* Writes the call's tokens' rows into the cache, converted (16-bit) or quantised (MX8, MX4). With
- * k and v in the cache, the arrays have its heads and width; a latent cache takes the latent
- * as k and the rotated part as v (NULL: none), one head each, widths multiples of 32 that add
- * up to the cache's. MX8: a block's scale is the least power of two with max |x| / scale <=
- * 448 over the block's finite values (scale byte 1 at least), codes round to nearest even; a
- * NaN or infinity is stored as NaN; a value whose rounding would leave the range of x's type
- * is stored as the largest code within it. MX4 alike: max |x| / scale <= 7 (6, the largest code, and
- * half the step above it: no element is off by more than half a step), and a block that holds a NaN or
- * an infinity gets scale byte 255 and reads as NaN throughout. Tokens at negative positions (more tokens than
- * rows) and rows past the bounds are not stored; min(max_q, n_tokens) is at most 2^26 - 4 (more
- * where a token's rows, k and v together, have at most 1024 elements; reads alike); two sequences that share a page in which
- * they write the same row leave one or a mixture of the two. */
+/* Writes the call's tokens' rows into the cache, converted (16-bit) or quantised (MX8, MX4). With k
+ * and v in the cache, the arrays have its heads and width; a latent cache takes the latent as k and
+ * the rotated part as v (NULL: none), one head each, widths multiples of 32 that add up to the
+ * cache's. MX8: a block's scale is the least power of two with max |x| / scale <= 448 over the
+ * block's finite values (scale byte 1 at least), codes round to nearest even; a NaN or infinity is
+ * stored as NaN; a value whose rounding would leave the range of x's type is stored as the largest
+ * code within it. MX4 alike: max |x| / scale <= 7 (6, the largest code, and half the step above it:
+ * no element is off by more than half a step), and a block that holds a NaN or an infinity gets
+ * scale byte 255 and reads as NaN throughout. Tokens at negative positions (more tokens than rows)
+ * and rows past the bounds are not stored; min(max_q, n_tokens) is at most 2^26 - 4 (more where a
+ * token's rows, k and v together, have at most 1024 elements; reads alike); two sequences that
+ * share a page in which they write the same row leave one or a mixture of the two. */
 HEARTH_API int hearth_gpu_kv_append(const hearth_gpu_cache *c, const hearth_gpu_batch *b, const hearth_gpu_array *k,
                                     const hearth_gpu_array *v, int dev, void *stream);
 
-/* hearth_gpu_rope of queries and keys and hearth_gpu_kv_append of the rotated keys and the values in one
- * launch, to the same bits (float16 arrays off 16 bytes or rotated parts off 8 elements: to one rounding):
- * q [n_tokens][H][width] rotated into q_out (q itself, or an array that shares no element with q, k and v;
- * both NULL: none), k rotated on its way into the cache (its array is left as it is), v as it is. A latent cache takes the latent as k and rotates v, its second part, whose width q has.
- * pos: a position for each of the n_tokens tokens (int32, or int64 when pos64 is 1), NULL: a token's row
- * number in its sequence, q_start and kv_len telling. freqs, n_freqs, offset, interleaved, factor: as in
- * hearth_gpu_rope. All arrays have one dtype; n_heads * width of the cache up to 2^23, min(max_q, n_tokens)
- * up to 2^24 - 1. Queries of tokens whose rows are not stored are rotated all the same. */
+/* hearth_gpu_rope of queries and keys and hearth_gpu_kv_append of the rotated keys and the values
+ * in one launch, to the same bits (float16 arrays off 16 bytes or rotated parts off 8 elements: to
+ * one rounding): q [n_tokens][H][width] rotated into q_out (q itself, or an array that shares no
+ * element with q, k and v; both NULL: none), k rotated on its way into the cache (its array is left
+ * as it is), v as it is. A latent cache takes the latent as k and rotates v, its second part, whose
+ * width q has. pos: a position for each of the n_tokens tokens (int32, or int64 when pos64 is 1),
+ * NULL: a token's row number in its sequence, q_start and kv_len telling. freqs, n_freqs, offset,
+ * interleaved, factor: as in hearth_gpu_rope. All arrays have one dtype; n_heads * width of the
+ * cache up to 2^23, min(max_q, n_tokens) up to 2^24 - 1. Queries of tokens whose rows are not
+ * stored are rotated all the same. */
 HEARTH_API int hearth_gpu_kv_append_rotated(const hearth_gpu_cache *c, const hearth_gpu_batch *b, const hearth_gpu_array *q,
                                             const hearth_gpu_array *q_out, const hearth_gpu_array *k, const hearth_gpu_array *v,
                                             const void *pos, int pos64, const double *freqs, int n_freqs, int offset,
@@ -387,16 +389,16 @@ HEARTH_API int hearth_gpu_kv_read(const hearth_gpu_cache *c, const hearth_gpu_ba
                                   const hearth_gpu_array *v, int dev, void *stream);
 
 /* Attention of the call's tokens over the cache: q [n_tokens][H][width], out alike, of dtype
- * HEARTH_F16 or HEARTH_BF16; H a multiple of the cache's heads, head h reads kv head
- * h / (H / n_heads); width 64, 128 or 256. out = softmax(scale * q . k) v over the rows a
- * token attends; a token that attends nothing gets zeros, one all of whose scores are -infinity
- * NaN (0 / 0). 16-bit caches have q's dtype; MX8 and MX4
- * rows are taken as their values in q's dtype, in whose range they must lie. min(max_q,
- * n_tokens) * H up to 2^26; min(max_kv, pages_per_seq * page) below 2^30 - 65536. Scores, softmax statistics and sums are
- * float32; the probabilities are rounded to q's dtype for the product with v. lse: NULL or
- * [n_tokens][H] float32, the natural logarithm of the sum of exponentials (-infinity where
- * that is 0). work: device memory of hearth_gpu_attend_workspace bytes, 16-byte
- * aligned; calls that may run at the same time must not share it. */
+ * HEARTH_F16 or HEARTH_BF16; H a multiple of the cache's heads, head h reads kv head h / (H /
+ * n_heads); width 64, 128 or 256. out = softmax(scale * q . k) v over the rows a token attends; a
+ * token that attends nothing gets zeros, one all of whose scores are -infinity NaN (0 / 0). 16-bit
+ * caches have q's dtype; MX8 and MX4 rows are taken as their values in q's dtype, in whose range
+ * they must lie. min(max_q, n_tokens) * H up to 2^26; min(max_kv, pages_per_seq * page) below 2^30
+ * - 65536. Scores, softmax statistics and sums are float32; the probabilities are rounded to q's
+ * dtype for the product with v. lse: NULL or [n_tokens][H] float32, the natural logarithm of the
+ * sum of exponentials (-infinity where that is 0). work: device memory of
+ * hearth_gpu_attend_workspace bytes, 16-byte aligned; calls that may run at the same time must not
+ * share it. */
 HEARTH_API int hearth_gpu_attend(const hearth_gpu_cache *c, const hearth_gpu_batch *b, const hearth_gpu_array *q,
                                  const hearth_gpu_array *out, float *lse, float scale, void *work, size_t work_bytes,
                                  int dev, void *stream);
@@ -425,11 +427,11 @@ HEARTH_API int64_t hearth_gpu_attend_workspace(const hearth_gpu_cache *c, const 
  * bounds of their keys selects. Blocks are `block` consecutive rows of a sequence (block n: rows n *
  * block ..), a power of two from 16 up to a page's rows, so none crosses a page. */
 
-/* Bounds of the keys of every block: codes int8 [n_pages][n_heads][blocks][2][width], the least and then the
- * greatest value of each element over the block's rows in whole steps (up to 127), the step of a block
- * 2^(scale - 127), scales [n_pages][n_heads][blocks]; blocks: of a page (block * blocks rows of it). The last three
- * dimensions of codes and the last one of scales are dense; strides in elements, those of codes and its address multiples
- * of 16. width: 64, 128 or 256. */
+/* Bounds of the keys of every block: codes int8 [n_pages][n_heads][blocks][2][width], the least and
+ * then the greatest value of each element over the block's rows in whole steps (up to 127), the
+ * step of a block 2^(scale - 127), scales [n_pages][n_heads][blocks]; blocks: of a page (block *
+ * blocks rows of it). The last three dimensions of codes and the last one of scales are dense;
+ * strides in elements, those of codes and its address multiples of 16. width: 64, 128 or 256. */
 typedef struct hearth_gpu_bounds {
     int8_t *codes;
     uint8_t *scales;
@@ -446,42 +448,49 @@ typedef struct hearth_gpu_blocks {
     int32_t top, block;
 } hearth_gpu_blocks;
 
-/* Brings the bounds of the blocks that hold rows of the call's tokens up to date, from all of their rows that exist (kv_len,
- * max_kv): call it after the rows are written. Not for latent caches. A row's element that is NaN or infinite
- * counts as 0. The step is the least power of two with which 127 steps reach the block's largest magnitude (scale
- * 1 at least), codes round to nearest even. Blocks on pages that are not in the cache are left alone. */
+/* Brings the bounds of the blocks that hold rows of the call's tokens up to date, from all of their
+ * rows that exist (kv_len, max_kv): call it after the rows are written. Not for latent caches. A
+ * row's element that is NaN or infinite counts as 0. The step is the least power of two with which
+ * 127 steps reach the block's largest magnitude (scale 1 at least), codes round to nearest even.
+ * Blocks on pages that are not in the cache are left alone. */
 HEARTH_API int hearth_gpu_key_bounds(const hearth_gpu_cache *c, const hearth_gpu_batch *b, const hearth_gpu_bounds *s, int dev,
                                      void *stream);
 
-/* The `top` best blocks of each of the call's tokens and cache heads, in ascending order, -1 behind the last
- * where fewer can be taken. q [n_tokens][H][width] of dtype HEARTH_F16 or HEARTH_BF16; H a multiple of the bounds' heads,
- * up to 128 of them each. A token may take the blocks up to the one of its own row (or of its sequence's last row
- * within max_kv, whichever comes first) whose pages are in the cache. It keeps the `first` first of them and the
- * `last` last (at least 1: its own block, whose bounds look at later rows too); with a mask also those from the block
- * of the call's first token on. The others come by their score, the greatest over the head's queries of
- * sum_d max(q_d low_d, q_d high_d), with q in whole numbers of up to 127 steps of the least power of two that reaches its
- * largest magnitude (NaN and infinities count as 0): whole numbers throughout, so the choice does not depend
- * on any order of sums, and of equal scores the lower block is taken. first + last <= top; with a mask first + the blocks
- * that max_q rows may touch as well. out's block is the bounds'. work: hearth_gpu_select_workspace bytes, 16-byte
- * aligned. n_heads * min(max_q, n_tokens) up to 2^23; tokens of no sequence are left alone. */
+/* The `top` best blocks of each of the call's tokens and cache heads, in ascending order, -1 behind
+ * the last where fewer can be taken. q [n_tokens][H][width] of dtype HEARTH_F16 or HEARTH_BF16; H a
+ * multiple of the bounds' heads, up to 128 of them each. A token may take the blocks up to the one
+ * of its own row (or of its sequence's last row within max_kv, whichever comes first) whose pages
+ * are in the cache. It keeps the `first` first of them and the `last` last (at least 1: its own
+ * block, whose bounds look at later rows too); with a mask also those from the block of the call's
+ * first token on. The others come by their score, the greatest over the head's queries of sum_d
+ * max(q_d low_d, q_d high_d), with q in whole numbers of up to 127 steps of the least power of two
+ * that reaches its largest magnitude (NaN and infinities count as 0): whole numbers throughout, so
+ * the choice does not depend on any order of sums, and of equal scores the lower block is taken.
+ * first + last <= top; with a mask first + the blocks that max_q rows may touch as well. out's
+ * block is the bounds'. work: hearth_gpu_select_workspace bytes, 16-byte aligned. n_heads *
+ * min(max_q, n_tokens) up to 2^23; tokens of no sequence are left alone. */
 HEARTH_API int hearth_gpu_select_blocks(const hearth_gpu_bounds *s, const hearth_gpu_batch *b, const hearth_gpu_array *q,
                                         const hearth_gpu_blocks *out, int first, int last, void *work, size_t work_bytes, int dev,
                                         void *stream);
 
-/* Workspace of hearth_gpu_select_blocks in bytes, from the host-side fields only; -1 for arguments it would refuse. */
+/* Workspace of hearth_gpu_select_blocks in bytes, from the host-side fields only; -1 for arguments
+ * it would refuse. */
 HEARTH_API int64_t hearth_gpu_select_workspace(const hearth_gpu_bounds *s, const hearth_gpu_batch *b);
 
-/* hearth_gpu_attend over the rows of each token's chosen blocks alone: of them a token attends those that it
- * would attend without a choice (up to its own row, or its mask). Blocks may stand in any order; one that stands
- * twice counts twice; negative numbers and blocks past the sequence count for nothing. A token whose blocks hold no row that it
- * attends gets zeros. Not for latent caches. block: a power of two from 16 up to a page, top * block below 2^30 -
- * 65536; n_heads * min(max_q, n_tokens) * (query heads of a cache head / 16, rounded up) up to 2^24 - 1; the rest
- * as hearth_gpu_attend. work: device memory of hearth_gpu_attend_blocks_workspace bytes, 16-byte aligned. */
+/* hearth_gpu_attend over the rows of each token's chosen blocks alone: of them a token attends
+ * those that it would attend without a choice (up to its own row, or its mask). Blocks may stand in
+ * any order; one that stands twice counts twice; negative numbers and blocks past the sequence
+ * count for nothing. A token whose blocks hold no row that it attends gets zeros. Not for latent
+ * caches. block: a power of two from 16 up to a page, top * block below 2^30 - 65536; n_heads *
+ * min(max_q, n_tokens) * (query heads of a cache head / 16, rounded up) up to 2^24 - 1; the rest as
+ * hearth_gpu_attend. work: device memory of hearth_gpu_attend_blocks_workspace bytes, 16-byte
+ * aligned. */
 HEARTH_API int hearth_gpu_attend_blocks(const hearth_gpu_cache *c, const hearth_gpu_batch *b, const hearth_gpu_array *q,
                                         const hearth_gpu_blocks *blocks, const hearth_gpu_array *out, float *lse, float scale,
                                         void *work, size_t work_bytes, int dev, void *stream);
 
-/* Its workspace in bytes (0: none needed), from the host-side fields only; -1 for arguments it would refuse. */
+/* Its workspace in bytes (0: none needed), from the host-side fields only; -1 for arguments it
+ * would refuse. */
 HEARTH_API int64_t hearth_gpu_attend_blocks_workspace(const hearth_gpu_cache *c, const hearth_gpu_batch *b, int n_heads, int top, int block);
 
 #ifdef __cplusplus

@@ -146,6 +146,15 @@ def test_trees(kind, heads, kv_heads, width):
     attend(width + 2, kind, heads, kv_heads, width, [9, 4], [4, 4], 16, [O.tree(4, 2), torch.zeros(4, 4, dtype=torch.bool)])
 
 
+@pytest.mark.parametrize("kind", [BF, HF])
+@pytest.mark.parametrize("heads,kv_heads,width,n", [(4, 4, 64, 96), (4, 4, 64, 97), (6, 2, 128, 32), (6, 2, 128, 33), (2, 2, 256, 70), (32, 4, 128, 12), (32, 4, 128, 13)])
+def test_columns_of_both_kernels(kind, heads, kv_heads, width, n):
+    """Up to 96 query rows of a kv head and above: causal, trees of more than a word, splits."""
+    lens, news = [n, 3000, n + 130, 5], [n, n, 40 if n > 40 else n, 2]
+    for trees in (None, [O.tree(k) for k in news]):
+        attend(heads + width + n, kind, heads, kv_heads, width, lens, news, 64, trees)
+
+
 def test_nothing_attended():
     attend(11, BF, 16, 1, 128, [0, 3, 40], [2, 10, 1], 16)
     attend(12, HF, 16, 1, 128, [4, 20], [4, 4], 16, [torch.zeros(4, 4, dtype=torch.bool), O.tree(4)])
