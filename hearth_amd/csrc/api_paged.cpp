@@ -413,10 +413,11 @@ HEARTH_API int hearth_gpu_select_blocks(const hearth_gpu_bounds *s, const hearth
     a.kv_heads = s->n_heads; a.group = group; a.top = out->top; a.first = first; a.last = last;
     a.score = (float *)work;
     a.ld_score = blocks_of(a.b.kv_cap, s->block);
+    score_split(a);
     if (hipPeekAtLastError() != hipSuccess) return E_IO;
     DeviceGuard g(dev);
     if (!g.ok) return no_device();
-    select_blocks(a, q->dtype, s->width, (int)a.ld_score, (hipStream_t)stream);
+    select_blocks(a, q->dtype, s->width, (hipStream_t)stream);
     return finish();
 }
 

@@ -124,7 +124,8 @@ struct SelectArgs {
     int kv_heads, group, top, first, last;
     float *score;                     /* [n_tokens][kv_heads][ld_score] */
     int64_t ld_score;
-    int chunk, n_chunks;              /* blocks a workgroup scores */
+    int tiles, chunk, n_chunks;       /* of the scores: workgroups of tokens, blocks a workgroup, its shares (0: no blocks) */
+    bool many;                        /* tokens share their blocks' bounds */
 };
 
 /* device of a call made current while the object lives */
@@ -159,7 +160,8 @@ void attend_latent(const AttendArgs &a, int q_dtype, int cache_dtype, hipStream_
 
 void key_bounds(const BoundsArgs &a, int cache_dtype, int width, hipStream_t st);   /* k_paged_select.hip */
 int select_group_limit();   /* query heads of a kv head */
-void select_blocks(SelectArgs a, int q_dtype, int width, int n_blocks, hipStream_t st);
+void score_split(SelectArgs &a);
+void select_blocks(const SelectArgs &a, int q_dtype, int width, hipStream_t st);
 
 /* ------------------------------------------------------------------ device helpers */
 

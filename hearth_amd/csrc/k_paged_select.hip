@@ -612,9 +612,9 @@ void bounds_t(const BoundsArgs &a, int width, hipStream_t st) {
 }
 
 template <class T, int D>
-void scores_t(const SelectArgs &a, int tiles, bool many, hipStream_t st) {
-    const dim3 grid((unsigned)((int64_t)tiles * a.n_chunks * a.kv_heads), 1, a.b.n_seqs), block(64 * SCORE_WAVES);
-    if (many) hipLaunchKernelGGL((k_block_scores_many<T, D>), grid, block, 0, st, a);
+void scores_t(const SelectArgs &a, hipStream_t st) {
+    const dim3 grid((unsigned)((int64_t)a.tiles * a.n_chunks * a.kv_heads), 1, a.b.n_seqs), block(64 * SCORE_WAVES);
+    if (a.many) hipLaunchKernelGGL((k_block_scores_many<T, D>), grid, block, 0, st, a);
     else if (a.group <= 16) hipLaunchKernelGGL((k_block_scores<T, D, true>), grid, block, 0, st, a);
     else hipLaunchKernelGGL((k_block_scores<T, D, false>), grid, block, 0, st, a);
 }
@@ -633,17 +633,23 @@ int select_group_limit() { return 16 * MAX_CHUNKS; }
 /* Blocks are shared out among workgroups until four are there for each unit, 64 at least each (16 a wave; 600
  * tokens over 313 blocks: 12.7 us, with two 15). Tokens that fill the rows of four waves share their blocks'
  * bounds. */
-void select_blocks(SelectArgs a, int q_dtype, int width, int n_blocks, hipStream_t st) {
+void score_split(SelectArgs &a) {
     int tpt = a.group <= 16 ? 16 / padded(a.group) : 1;
-    const bool many = a.group <= 16 && a.b.max_q >= SCORE_WAVES * tpt;
-    if (many) tpt *= SCORE_WAVES;
-    const int tiles = (a.b.max_q + tpt - 1) / tpt;
-    const int64_t wgs = (int64_t)a.b.n_seqs * a.kv_heads * tiles;
+    a.many = a.group <= 16 && a.b.max_q >= SCORE_WAVES * tpt;
+    if (a.many) tpt *= SCORE_WAVES;
+    a.tiles = (a.b.max_q + tpt - 1) / tpt;
+    const int64_t wgs = (int64_t)a.b.n_seqs * a.kv_heads * a.tiles;
     const int64_t want = std::max<int64_t>(1, 1024 / wgs);
-    a.chunk = (int)(((n_blocks + want - 1) / want + 63) / 64 * 64);
-    a.n_chunks = (n_blocks + a.chunk - 1) / a.chunk;
-    if (q_dtype == DT_BF16) width == 64 ? scores_t<Bf16, 64>(a, tiles, many, st) : width == 128 ? scores_t<Bf16, 128>(a, tiles, many, st) : scores_t<Bf16, 256>(a, tiles, many, st);
-    else width == 64 ? scores_t<F16, 64>(a, tiles, many, st) : width == 128 ? scores_t<F16, 128>(a, tiles, many, st) : scores_t<F16, 256>(a, tiles, many, st);
+    a.chunk = (int)std::max<int64_t>(((a.ld_score + want - 1) / want + 63) / 64 * 64, 64);   /* no blocks: no shares */
+    a.n_chunks = (int)((a.ld_score + a.chunk - 1) / a.chunk);
+}
+
+void select_blocks(const SelectArgs &a, int q_dtype, int width, hipStream_t st) {
+    if (a.n_chunks) {
+        if (q_dtype == DT_BF16) width == 64 ? scores_t<Bf16, 64>(a, st) : width == 128 ? scores_t<Bf16, 128>(a, st) : scores_t<Bf16, 256>(a, st);
+        else width == 64 ? scores_t<F16, 64>(a, st) : width == 128 ? scores_t<F16, 128>(a, st) : scores_t<F16, 256>(a, st);
+    }
+    const int64_t n_blocks = a.ld_score;
     const int64_t rows = (int64_t)a.b.max_q * a.kv_heads;
     const bool alone = n_blocks <= 64 * PICK_ALONE;
     const dim3 grid((unsigned)(alone ? (rows + 3) / 4 : rows), 1, a.b.n_seqs), threads(PICK_THREADS);

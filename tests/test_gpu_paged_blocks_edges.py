@@ -1,0 +1,34 @@
+"""The choice of blocks at the ends of what is allowed, on the GPU: calls without rows."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+import test_gpu_paged as base
+from hearth_amd import paged
+from test_gpu_paged_blocks import new_bounds
+
+pytestmark = pytest.mark.gpu
+
+BF, HF = torch.bfloat16, torch.float16
+
+
+def test_choice_without_rows():
+    """max_kv of 0, and page tables of no columns: nothing can be taken, and nothing is attended."""
+    bd = new_bounds(3, 2, 16, 16, 64)
+    cache = paged.Cache(*(torch.ones(3, 2, 16, 64, dtype=BF, device="cuda") for _ in range(2)))
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    for heads, news in ((4, [2, 1]), (4, [30, 40]), (64, [1, 1])):
+        n = sum(news)
+        starts, lens = i32(0, news[0], n), i32(50, 7)
+        for pages, max_kv in ((torch.zeros(2, 1, dtype=torch.int32, device="cuda"), 0), (torch.zeros(2, 0, dtype=torch.int32, device="cuda"), 60)):
+            b = paged.Batch(pages, lens, starts, max_q=max(news), max_kv=max_kv)
+            q, out = torch.ones(n + 1, heads, 64, dtype=BF, device="cuda"), torch.full((n + 1, heads, 64), 3, dtype=BF, device="cuda")
+            chosen = torch.full((n + 1, 2, 5), 9, dtype=torch.int32, device="cuda")
+            paged.update_bounds(cache, b, bd, stream=base._stream())
+            paged.select(bd, b, q, chosen, stream=base._stream())
+            paged.attend_blocks(cache, b, q, chosen, out, block=16, scale=0.1, stream=base._stream())
+            torch.cuda.synchronize()
+            assert (chosen[:n] == -1).all() and (chosen[n:] == 9).all()
+            assert (out[:n] == 0).all() and (out[n:] == 3).all()
+    assert (bd.low_high == 77).all()

@@ -1,0 +1,22 @@
+"""Calls of the choice of blocks and of attention over them at the ends of what is allowed, on the CPU: with a
+device that is not there (-4 where the arguments fit together, -1 where they are refused)."""
+from __future__ import annotations
+
+from ctypes import byref
+
+import pytest
+
+from hearth_amd import paged
+from test_paged_args import Fake, batch
+from test_paged_blocks import bounds
+from test_paged_bounds import NONE, but
+
+
+@pytest.mark.parametrize("tokens,max_q,heads", [(1, 1, 4), (5, 3, 4), (40, 40, 4), (3, 3, 64)])
+def test_choice_without_rows(tokens, max_q, heads):
+    """max_kv of 0, and page tables of no columns: no scores, no workspace, and a call that reaches the device."""
+    s, q, out = bounds(), Fake((tokens, heads, 64)), Fake((tokens, 2, 6), "int32")
+    for b in (batch(max_q=max_q, max_kv=0), batch(per=0, max_q=max_q), batch(per=0, max_q=max_q, max_kv=0)):
+        assert paged.select_workspace_bytes(s, b, tokens) == 0
+        assert paged._fn("hearth_gpu_select_blocks")(s._ref, b._of(tokens), byref(paged._array(q, "q", 0)), byref(paged._blocks(out, "c", 0, tokens, 2, 16)), 1, 1,
+                                                     None, 0, NONE, None) == -4
