@@ -542,7 +542,8 @@ __global__ __launch_bounds__(PICK_THREADS) void k_block_pick(SelectArgs a) {
     if (can > a.top) {
         if (left <= 0) limit = ~0u - 1;
         else
-            for (int round = 0;; round ^= 1) {
+            for (int z = 0; z < 4; z++) {   /* shifts of up to 24, 16, 8 and 0: the fourth round ends it */
+                const int round = z & 1;
                 const int shift = max(24 - __builtin_clz(hi - lo | 1u), 0);   /* (hi - lo) >> shift < 256 */
                 keys([&](int, unsigned k) {
                     if (k >= lo && k <= hi) atomicAdd(&bins[round][(k - lo) >> shift], 1u);
@@ -567,7 +568,7 @@ __global__ __launch_bounds__(PICK_THREADS) void k_block_pick(SelectArgs a) {
                 lo += bin << shift;
                 if (in == (unsigned)left) { limit = lo - 1; break; }
                 if (shift == 0) { limit = lo; ties = left; break; }
-                hi = min(hi, lo + (1u << shift) - 1);
+                hi = lo + min(hi - lo, (1u << shift) - 1);   /* lo + 2^24 may pass 32 bits */
                 /* the other set of bins is clear; this one is for the round after the next */
                 meet();
                 for (int i = id; i < 256; i += 64 * W) bins[round][i] = 0;

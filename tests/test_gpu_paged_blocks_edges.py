@@ -1,12 +1,14 @@
-"""The choice of blocks at the ends of what is allowed, on the GPU: calls without rows."""
+"""The choice of blocks at the ends of what is allowed, on the GPU: calls without rows, scores
+next to the ends of float32's range."""
 from __future__ import annotations
 
 import pytest
 import torch
 
+import block_oracle as B
 import test_gpu_paged as base
 from hearth_amd import paged
-from test_gpu_paged_blocks import new_bounds
+from test_gpu_paged_blocks import choice, new_bounds
 
 pytestmark = pytest.mark.gpu
 
@@ -32,3 +34,27 @@ def test_choice_without_rows():
             assert (chosen[:n] == -1).all() and (chosen[n:] == 9).all()
             assert (out[:n] == 0).all() and (out[n:] == 3).all()
     assert (bd.low_high == 77).all()
+
+
+def scaled(sizes):
+    """an edit of a cache's keys: block i (a page) keeps its random rows' directions times sizes[i % len(sizes)]"""
+    def edit(k, pages):
+        for i in range(k.shape[0]):
+            k[i] = (k[i].double().sign() * sizes[i % len(sizes)]).to(k.dtype)
+    return edit
+
+
+@pytest.mark.parametrize("rows", [40 * 16, 600 * 16, 2500 * 16, 9000 * 16])
+@pytest.mark.parametrize("sizes,size", [((1e20,), 1e20), ((1e20, -1e20, 1.0, 3e19), 1e20), ((2.0 ** 60,), 2.0 ** 64), ((2.0 ** 60, -1.5, 2.0 ** 59, 2.0 ** 56), 2.0 ** 64)])
+def test_choice_of_scores_near_infinity(rows, sizes, size):
+    """Scores of both signs up to the largest floats and past them (equal infinities: the lowest blocks). Each block's
+    rows are alike, so that a score is its rows' own, of either sign; a choice of fewer than there are infinities, and of more."""
+    def edit(k, pages):
+        scaled(sizes)(k, pages)
+        k[:] = k[:, :, :1]
+
+    n = rows // 16
+    order = torch.arange(n, dtype=torch.int32)[None]
+    for top, heads in ((2, 1), (5, 1), (25, 3), (n // 3, 1)):
+        choice(base._gen(top), BF, "bf16", heads, 1, 64, [rows], [1], 16, 16, top, 0, 1, pages=order, n_pages=n, edit=edit,
+               queries=lambda q: q.copy_((q.double().sign() * size).to(BF)))
