@@ -6,8 +6,9 @@
  * the score of all its rows: q . k <= sum_d max(q_d lo_d, q_d hi_d) = q+ . hi + q- . lo, with q's
  * positive and negative parts. Bounds and queries are rounded to whole numbers of up to 127 steps of
  * a power of two, one step for a block and one for a query head, which makes the sum two 8-bit matrix
- * products, exact in 32 bits (at most 127 * 127 * 256 < 2^24, so that its float32 is exact too): the
- * order of the blocks does not depend on how the sums are split, and ties go to the lowest block.
+ * products, exact in 32 bits (at most 127 * 127 * 256 < 2^24, so that its float32 is exact too, and
+ * the product with the steps but past float32's range at either end): the order of the blocks does
+ * not depend on how the sums are split, and ties go to the lowest block.
  */
 #include "hx_paged.h"
 
@@ -499,7 +500,7 @@ __global__ __launch_bounds__(PICK_THREADS) void k_block_pick(SelectArgs a) {
     auto fetch = [&](int i) __attribute__((always_inline)) -> unsigned {   /* of block from + i of the wave */
         if (from + i >= to) return 0u;
         const float s = score[from + i];
-        const unsigned u = __float_as_uint(s);
+        const unsigned u = s == 0.0f ? 0u : __float_as_uint(s);   /* a sum below 0 times steps whose product underflows is -0, which is no less than 0 */
         if (s == -__builtin_huge_valf()) return 0u;
         return from + i < a.first || from + i >= tail ? ~0u : u & 0x80000000u ? ~u : u | 0x80000000u;
     };

@@ -464,8 +464,10 @@ HEARTH_API int hearth_gpu_key_bounds(const hearth_gpu_cache *c, const hearth_gpu
  * block, whose bounds look at later rows too); with a mask also those from the block of the call's
  * first token on. The others come by their score, the greatest over the head's queries of sum_d
  * max(q_d low_d, q_d high_d), with q in whole numbers of up to 127 steps of the least power of two
- * that reaches its largest magnitude (NaN and infinities count as 0): whole numbers throughout, so
+ * that reaches its largest magnitude (NaN and infinities count as 0): sums of whole numbers, so
  * the choice does not depend on any order of sums, and of equal scores the lower block is taken.
+ * The sum times both steps is held as a float32: scores past its range are equal infinities, those
+ * next to 0 are rounded to its least numbers (steps whose product is below 2^-149).
  * first + last <= top; with a mask first + the blocks that max_q rows may touch as well. out's
  * block is the bounds'. work: hearth_gpu_select_workspace bytes, 16-byte aligned. n_heads *
  * min(max_q, n_tokens) up to 2^23; tokens of no sequence are left alone. */

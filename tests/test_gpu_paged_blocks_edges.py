@@ -58,3 +58,21 @@ def test_choice_of_scores_near_infinity(rows, sizes, size):
     for top, heads in ((2, 1), (5, 1), (25, 3), (n // 3, 1)):
         choice(base._gen(top), BF, "bf16", heads, 1, 64, [rows], [1], 16, 16, top, 0, 1, pages=order, n_pages=n, edit=edit,
                queries=lambda q: q.copy_((q.double().sign() * size).to(BF)))
+
+
+@pytest.mark.parametrize("rows", [40 * 16, 600 * 16, 9000 * 16])
+@pytest.mark.parametrize("heads", [1, 3, 20])
+def test_choice_of_scores_near_zero(rows, heads):
+    """Products of steps below float32's least: scores of 0 from sums of either sign are equal, and the lowest blocks
+    are taken; and least numbers of both signs, which are not."""
+    def edit(k, pages):
+        scaled((2.0 ** -120, -2.0 ** -122))(k, pages)
+        k[:] = k[:, :, :1]
+
+    n = rows // 16
+    order = torch.arange(n, dtype=torch.int32)[None]
+    for size, top in ((2.0 ** -110, 9), (2.0 ** -110, n // 2), (2.0 ** -30, 9), (2.0 ** -29, n // 2)):
+        got = choice(base._gen(n), BF, "bf16", heads, 1, 64, [rows], [1], 16, 16, top, 0, 1, pages=order, n_pages=n, edit=edit,
+                     queries=lambda q: q.copy_((q.double().sign() * size).to(BF)))
+        if size == 2.0 ** -110:
+            assert torch.equal(got[0, 0, :-1], torch.arange(top - 1, dtype=torch.int32))
