@@ -258,7 +258,9 @@ int64_t score_bytes(const hearth_gpu_bounds *s, const hearth_gpu_batch *b) {
     const Batch o = batch_of(*b, s->n_pages, s->block * s->blocks);
     if (o.kv_cap > MAX_ROWS || (int64_t)o.max_q * s->n_heads > MAX_PICKS) return E_ARG;
     if (!o.n_seqs || !o.max_q) return 0;
-    return (int64_t)o.n_tokens * s->n_heads * blocks_of(o.kv_cap, s->block) * (int64_t)sizeof(float);
+    int64_t bytes;   /* up to 2^71: few query rows a sequence say nothing of all tokens */
+    if (__builtin_mul_overflow((int64_t)o.n_tokens * s->n_heads, blocks_of(o.kv_cap, s->block) * (int64_t)sizeof(float), &bytes)) return E_ARG;
+    return bytes;
 }
 
 } // namespace

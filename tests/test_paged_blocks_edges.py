@@ -20,3 +20,13 @@ def test_choice_without_rows(tokens, max_q, heads):
         assert paged.select_workspace_bytes(s, b, tokens) == 0
         assert paged._fn("hearth_gpu_select_blocks")(s._ref, b._of(tokens), byref(paged._array(q, "q", 0)), byref(paged._blocks(out, "c", 0, tokens, 2, 16)), 1, 1,
                                                      None, 0, NONE, None) == -4
+
+
+@pytest.mark.parametrize("heads,max_q,tokens,per,S", [(1, 1, 0x7fffffff, 1 << 26, 65535), (16, 16, 0x7fffffff, 1 << 26, 65535), (64, 3, 1 << 30, 1 << 26, 9), (4096, 2048, 0x7fffffff, 1 << 26, 65535),
+                                                      (4096, 1, 1 << 27, 1 << 25, 1), (4096, 1, 1 << 26, 1 << 24, 1), (4, 1, 70, 4, 1)])
+def test_workspace_of_the_choice_past_64_bits(heads, max_q, tokens, per, S):
+    """Bytes that 64 bits do not hold are refused, not cut."""
+    s = but(bounds(heads=2, blocks=1)._s, n_heads=heads)
+    b = but(batch()._of(1)._obj, n_seqs=S, n_tokens=tokens, max_q=max_q, max_kv=0x3fff0000, pages_per_seq=per, ld_pages=per)
+    want = tokens * heads * min(0x3fff0000 // 16, per) * 4
+    assert paged._fn("hearth_gpu_select_workspace")(byref(s), byref(b)) == (want if want < 2 ** 63 else -1)
