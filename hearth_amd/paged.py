@@ -597,6 +597,8 @@ def attend_blocks(cache: Cache, batch: Batch, q, chosen, out, *, block: int, sca
     attend_blocks_workspace_bytes."""
     if cache.v is None:
         raise ValueError("attend_blocks: a latent cache has no keys of its own")
+    if chosen is None:
+        raise ValueError("attend_blocks: chosen is missing")
     _attend("attend_blocks", cache, batch, q, None, out, lse, scale, workspace, stream, chosen, block)
 
 

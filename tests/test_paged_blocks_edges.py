@@ -7,7 +7,7 @@ from ctypes import byref
 import pytest
 
 from hearth_amd import paged
-from test_paged_args import Fake, batch
+from test_paged_args import Fake, batch, cache
 from test_paged_blocks import bounds
 from test_paged_bounds import NONE, but
 
@@ -30,3 +30,10 @@ def test_workspace_of_the_choice_past_64_bits(heads, max_q, tokens, per, S):
     b = but(batch()._of(1)._obj, n_seqs=S, n_tokens=tokens, max_q=max_q, max_kv=0x3fff0000, pages_per_seq=per, ld_pages=per)
     want = tokens * heads * min(0x3fff0000 // 16, per) * 4
     assert paged._fn("hearth_gpu_select_workspace")(byref(s), byref(b)) == (want if want < 2 ** 63 else -1)
+
+
+def test_attention_over_no_lists():
+    """None in the place of the chosen blocks is no call of attend."""
+    q = Fake((5, 4, 64))
+    with pytest.raises(ValueError, match="chosen"):
+        paged.attend_blocks(cache(), batch(), q, None, q, block=16, scale=0.1)
