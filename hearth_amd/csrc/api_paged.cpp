@@ -22,6 +22,7 @@ constexpr int MAX_ROWS = 0x3fff0000;                /* rows of a sequence that a
 constexpr int64_t MAX_LATENT_TILES = 0x7ffff0;      /* workgroups of 512 threads in one dimension of a grid (below 2^32 threads) */
 constexpr int64_t MAX_COPY_GROUPS = 0xffffff;       /* workgroups of 256 likewise */
 constexpr int64_t MAX_PICKS = 1 << 23;              /* workgroups of 256 that choose blocks, likewise */
+constexpr int MAX_HEADS = 65536;                    /* of an array */
 constexpr int64_t MAX_ROPE_ROW = 1 << 24;           /* elements of a token: four of them count within 31 bits */
 
 bool pow2(int x) { return x > 0 && (x & (x - 1)) == 0; }
@@ -59,7 +60,7 @@ int elem(int dtype) { return dtype == HEARTH_F32 ? 4 : dtype == HEARTH_F16 || dt
 
 /* n: tokens; without any, data may be NULL */
 bool array_ok(const hearth_gpu_array *x, int n) {
-    if (!x || (n && !x->data) || !elem(x->dtype) || x->n_heads < 1 || x->n_heads > 65536 || x->width < 1 || x->width > 65536) return false;
+    if (!x || (n && !x->data) || !elem(x->dtype) || x->n_heads < 1 || x->n_heads > MAX_HEADS || x->width < 1 || x->width > 65536) return false;
     if ((uintptr_t)x->data % elem(x->dtype)) return false;
     return std::llabs(x->token_stride) <= MAX_STRIDE && std::llabs(x->head_stride) <= MAX_STRIDE;
 }
@@ -181,7 +182,7 @@ int copy_call(bool write, const hearth_gpu_cache *c, const hearth_gpu_batch *b, 
 /* arguments that both attentions share */
 bool attend_shape_ok(const hearth_gpu_cache *c, const hearth_gpu_batch *b, int heads) {
     if (!cache_ok(c) || !batch_ok(b)) return false;
-    if (heads < 1 || heads % c->n_heads) return false;
+    if (heads < 1 || heads > MAX_HEADS || heads % c->n_heads) return false;
     const Batch o = batch_of(*b, *c);
     if ((int64_t)o.max_q * heads > (1 << 26) || o.kv_cap > MAX_ROWS) return false;
     if (!c->v.data && ((int64_t)o.max_q * heads + 63) / 64 * o.n_seqs > MAX_LATENT_TILES) return false;

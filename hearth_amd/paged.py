@@ -396,12 +396,20 @@ def read(cache: Cache, batch: Batch, k, v=None, *, stream=0) -> None:
         _check(rc, "read")
 
 
+def _for_tokens(batch, tokens) -> _BatchS:
+    """The struct of a call of `tokens` tokens (None: as many as sequences times max_q)."""
+    s = _BatchS.from_buffer_copy(batch._s)
+    s.n_tokens = n = min(s.n_seqs * s.max_q, 0x7fffffff) if tokens is None else tokens
+    if s.n_tokens != n:
+        raise ValueError(f"{n} tokens (at most 2147483647)")
+    return s
+
+
 def workspace_bytes(cache: Cache, batch: Batch, heads: int, tokens: int | None = None) -> int:
     """Bytes of device workspace that attend / attend_latent need for `tokens` query tokens
     (None: as many as sequences times max_q) of `heads` heads: 0 when none is."""
-    s = _BatchS.from_buffer_copy(batch._s)
-    s.n_tokens = min(s.n_seqs * s.max_q, 0x7fffffff) if tokens is None else tokens
-    n = _fn("hearth_gpu_attend_workspace")(cache._ref, byref(s), heads)
+    s = _for_tokens(batch, tokens)
+    n = _fn("hearth_gpu_attend_workspace")(cache._ref, byref(s), heads) if 1 <= heads <= 65536 else -1
     if n < 0:
         raise ValueError(f"no attention over this cache (heads {cache._s.n_heads}, width {cache._s.width}) "
                          f"with {heads} query heads")
@@ -538,8 +546,7 @@ def update_bounds(cache: Cache, batch: Batch, bounds: Bounds, *, stream=0) -> No
 def select_workspace_bytes(bounds: Bounds, batch: Batch, tokens: int | None = None) -> int:
     """Bytes of device workspace that select needs for `tokens` query tokens (None: as many as sequences
     times max_q)."""
-    s = _BatchS.from_buffer_copy(batch._s)
-    s.n_tokens = min(s.n_seqs * s.max_q, 0x7fffffff) if tokens is None else tokens
+    s = _for_tokens(batch, tokens)
     n = _fn("hearth_gpu_select_workspace")(bounds._ref, byref(s))
     if n < 0:
         raise ValueError(f"select: {s.max_q} tokens of {s.max_kv} rows are beyond its limits (see include/hearth_gpu.h)")
@@ -578,10 +585,9 @@ def select(bounds: Bounds, batch: Batch, q, chosen, *, first: int = 1, last: int
 def attend_blocks_workspace_bytes(cache: Cache, batch: Batch, heads: int, top: int, block: int, tokens: int | None = None) -> int:
     """Bytes of device workspace that attend_blocks needs for `tokens` query tokens (None: as many as
     sequences times max_q) of `heads` heads and `top` chosen blocks of `block` rows: 0 when none is."""
-    s = _BatchS.from_buffer_copy(batch._s)
-    s.n_tokens = min(s.n_seqs * s.max_q, 0x7fffffff) if tokens is None else tokens
+    s = _for_tokens(batch, tokens)
     n = -1
-    if 1 <= heads <= 1 << 26 and 1 <= top <= 1 << 20 and 16 <= block <= 4096:
+    if 1 <= heads <= 65536 and 1 <= top <= 1 << 20 and 16 <= block <= 4096:
         n = _fn("hearth_gpu_attend_blocks_workspace")(cache._ref, byref(s), heads, top, block)
     if n < 0:
         raise ValueError(f"no attention over {top} blocks of {block} rows of this cache (pages of {cache._s.page} rows, heads {cache._s.n_heads}, "

@@ -37,3 +37,23 @@ def test_attention_over_no_lists():
     q = Fake((5, 4, 64))
     with pytest.raises(ValueError, match="chosen"):
         paged.attend_blocks(cache(), batch(), q, None, q, block=16, scale=0.1)
+
+
+def test_workspaces_of_heads_that_no_array_has():
+    """Bytes are told for the calls that the attentions take: up to 65536 heads an array."""
+    one = batch(S=4, per=1 << 26, max_q=0x7fffffff, max_kv=0x3fff0000)
+    for c in (cache(), cache(heads=1, width=576, latent=True)):
+        for heads in (65536, 65538, 1 << 25, (1 << 32) + 4):
+            if heads == 65536:
+                assert paged.workspace_bytes(c, one, heads, 1) >= 0
+            else:
+                with pytest.raises(ValueError):
+                    paged.workspace_bytes(c, one, heads, 1)
+    assert paged.attend_blocks_workspace_bytes(cache(), one, 65536, 6, 16, 1) >= 0
+    with pytest.raises(ValueError):
+        paged.attend_blocks_workspace_bytes(cache(), one, 65538, 6, 16, 1)
+    for tokens in (-1, 1 << 31, (1 << 32) + 5):          # no cut to 32 bits
+        for call in (lambda: paged.workspace_bytes(cache(), one, 4, tokens), lambda: paged.select_workspace_bytes(bounds(), one, tokens),
+                     lambda: paged.attend_blocks_workspace_bytes(cache(), one, 4, 6, 16, tokens)):
+            with pytest.raises(ValueError):
+                call()
