@@ -346,6 +346,7 @@ def append_rotated(cache: Cache, batch: Batch, q, k, v, freqs, *, pos=None, fact
     [tokens, heads, width] in place or into q_out (None: keys alone), k on its way into the cache (the
     tensor stays as it is). A latent cache takes the latents as k and rotates v, their second part,
     whose width q has. pos [tokens] (int32 or int64), None: each token's row number in its sequence.
+    Queries of tokens of no sequence (padding) and of those past max_q are left as they are, in q_out too.
     freqs, factor, layout, offset: as in rope; q_out is q or shares nothing with q, k and v."""
     if layout not in ("half", "interleaved"):
         raise ValueError(f"layout {layout!r} is neither 'half' nor 'interleaved'")

@@ -376,8 +376,9 @@ HEARTH_API int hearth_gpu_kv_append(const hearth_gpu_cache *c, const hearth_gpu_
  * width q has. pos: a position for each of the n_tokens tokens (int32, or int64 when pos64 is 1),
  * NULL: a token's row number in its sequence, q_start and kv_len telling. freqs, n_freqs, offset,
  * interleaved, factor: as in hearth_gpu_rope. All arrays have one dtype; n_heads * width of the
- * cache up to 2^23, min(max_q, n_tokens) up to 2^24 - 1. Queries of tokens whose rows are not
- * stored are rotated all the same. */
+ * cache up to 2^23, min(max_q, n_tokens) up to 2^24 - 1. Queries are rotated of the tokens that
+ * belong to a sequence and lie below max_q in it, also where their rows have no page or do not
+ * exist (hearth_gpu_rope rotates all n_tokens); q_out is left as it is for the others. */
 HEARTH_API int hearth_gpu_kv_append_rotated(const hearth_gpu_cache *c, const hearth_gpu_batch *b, const hearth_gpu_array *q,
                                             const hearth_gpu_array *q_out, const hearth_gpu_array *k, const hearth_gpu_array *v,
                                             const void *pos, int pos64, const double *freqs, int n_freqs, int offset,

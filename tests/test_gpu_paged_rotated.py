@@ -161,3 +161,33 @@ def test_no_tokens():
         paged.append_rotated(c, b, e(4), e(2), e(2), f, pos=i32(), stream=base._stream())
     torch.cuda.synchronize()
     assert (d["k"] == 0).all()
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+def test_queries_without_rows_and_of_no_sequence(in_place):
+    """Queries of tokens whose rows have no page, lie past max_kv or before the first row are rotated; those of tokens past
+    max_q and of no sequence (before and behind the sequences') are left alone."""
+    g = base._gen(21)
+    H, Hkv, W, T = 4, 2, 64, 40
+    pages = torch.tensor([[0, 77, -1], [1, 2, 3], [4, 5, 6]], dtype=torch.int32).cuda()
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    b = paged.Batch(pages, i32(48, 4, 40), i32(3, 15, 25, 36), max_q=10, max_kv=35)
+    d, c = make_cache(7, Hkv, 16, W, "bf16")
+    q, k, v = (torch.randn(T, h, W, generator=g).to(BF).cuda() for h in (H, Hkv, Hkv))
+    f = torch.from_numpy(paged.rope_frequencies(W)[0]).cuda()
+    rows = torch.zeros(T, dtype=torch.int64)
+    done = torch.zeros(T, dtype=torch.bool)
+    for lo, n, L in ((3, 12, 48), (15, 10, 4), (25, 11, 40)):
+        rows[lo:lo + n] = torch.arange(L - n, L)
+        done[lo:lo + min(n, 10)] = True
+    want = torch.empty_like(q)
+    paged.rope(q, rows.cuda(), f, out=want, stream=base._stream())
+    old = q.clone() if in_place else torch.full_like(q, 5)
+    out = q if in_place else old.clone()
+    paged.append_rotated(c, b, q, k, v, f, q_out=None if in_place else out, stream=base._stream())
+    torch.cuda.synchronize()
+    assert torch.equal(out[done], want[done]) and torch.equal(out[~done], old[~done])
+    # sequence 0 has no pages for rows 36 .. 45; of sequence 1 the last 4 of 10 tokens' rows exist; of sequence 2 rows 29 .. 34
+    stored = torch.zeros(7, 16, dtype=torch.bool)
+    stored[1, :4] = stored[5, 13:] = stored[6, :3] = True
+    assert torch.equal(d["v"].cpu().ne(0).any(-1).any(1), stored) and torch.equal(d["k"].cpu().ne(0).any(-1).any(1), stored)
