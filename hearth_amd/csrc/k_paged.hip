@@ -178,9 +178,10 @@ __global__ __launch_bounds__(ROPE_THREADS) void k_rope(RopeArgs a, int tok) {
  * with amax * 2^-e <= 448 = 1.75 * 2^8, read off the bits of amax = m * 2^x: x - 8 where
  * m <= 1.75, else x - 7. Dividing by 2^e is exact; the hardware conversion rounds to nearest
  * even. Where rounding up would leave the range of the source type (its largest exponent, m
- * above 1.9375) the code is cut to 240, which is within half a step (2^-4) of the value. MX4
+ * above 1.9375) the code is cut to 240: off by up to the step below it, 2^-4 of the value. MX4
  * alike, with amax * 2^-e <= 7 = 1.75 * 2^2: a value between 6, the largest code, and 7 rounds to 6 and
- * is off by no more than half the step of the codes above 4. e2m1 has no NaN, so a block that holds one, or an
+ * is off by no more than half the step of the codes above 4; at the range's end (m above 1.75) the
+ * code is cut to 3, off by up to the step to 4, 2^-2 of the value. e2m1 has no NaN, so a block that holds one, or an
  * infinity, gets the scale byte 255, which the conversions back turn into NaN. Looking at every element for these took
  * 12 us for 3 x 4093 rows of 4 heads of 128 into 4 bits, a look at the block's largest bits 9.1 (floor 6.3). */
 __device__ __forceinline__ bool fin(float x) { return __builtin_fabsf(x) < __builtin_huge_valf(); }
@@ -261,7 +262,7 @@ __device__ __forceinline__ void put8(const Piece &p, const Spot &at, int h, int 
                 }
                 byte = byte_of(max_of4(f));
             }
-            /* the code above these would leave the source type's range: they are within half a step of the value */
+            /* the code above these would leave the source type's range: they are off by up to the step to it */
             const float top = byte == FULL ? (DST == DT_MX4 ? 3.0f : 240.0f) * mx_scale(byte) : __builtin_huge_valf();
 #pragma unroll
             for (int j = 0; j < 8; j++) x[j] = (DST == DT_MX4 ? whole : fin(v[j])) ? fminf(fmaxf(v[j], -top), top) : 0.0f;

@@ -360,8 +360,10 @@ HEARTH_API int hearth_gpu_rope(const hearth_gpu_array *x, const hearth_gpu_array
  * block's finite values (scale byte 1 at least), codes round to nearest even; a NaN or infinity is
  * stored as NaN; a value whose rounding would leave the range of x's type is stored as the largest
  * code within it. MX4 alike: max |x| / scale <= 7 (6, the largest code, and half the step above it:
- * no element is off by more than half a step), and a block that holds a NaN or an infinity gets
- * scale byte 255 and reads as NaN throughout. Tokens at negative positions (more tokens than rows)
+ * no element is off by more than half a step, but for those whose nearest code, 4 of the largest
+ * scale, is out of x's type's range: they are stored as 3 and off by up to that step, 2^-2 of the
+ * value; magnitudes above 57344 of float16, 3.5 * 2^126 of the others), and a block that holds a
+ * NaN or an infinity gets scale byte 255 and reads as NaN throughout. Tokens at negative positions (more tokens than rows)
  * and rows past the bounds are not stored; min(max_q, n_tokens) is at most 2^26 - 4 (more where a
  * token's rows, k and v together, have at most 1024 elements; reads alike); two sequences that
  * share a page in which they write the same row leave one or a mixture of the two. */

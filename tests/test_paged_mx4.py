@@ -49,6 +49,26 @@ def test_codes_are_the_nearest(dtype):
     assert torch.equal(P.values(codes, sc), torch.where(c >= 8, -1.0, 1.0) * P.GRID[c & 7] * step)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_how_far_off_at_the_end_of_the_range(dtype):
+    """Half a step of the codes up to 3.5 times the largest scale; above, where 4 would leave the type, up to the
+    step from 3 to 4 and a quarter of the value."""
+    big = torch.finfo(dtype).max
+    top = 2.0 ** (15 if dtype == torch.float16 else 127)
+    g = torch.Generator().manual_seed(4)
+    x = (torch.rand(400, 32, generator=g, dtype=torch.float64) * 2 - 1) * big
+    x[0, :6] = torch.tensor([big, -big, 1.75 * top, 1.5 * top, 1.25 * top, 1.75 * top * (1 + 2.0 ** -6)])
+    x = x.to(dtype)
+    codes, sc = P.mx4(x)
+    v, a = P.values(codes, sc), x.double().abs()
+    step = torch.exp2(sc.double() - 127).repeat_interleave(32, -1)
+    gap = torch.where(a / step >= 4, 2.0, torch.where(a / step >= 2, 1.0, 0.5)) * step
+    off, end = (v - x.double()).abs(), a > 1.75 * top
+    assert (off[~end] <= gap[~end] / 2).all() and (off[end] <= gap[end]).all() and (off[end] <= a[end] / 4).all()
+    assert end.sum() > 100 and (off[end] > gap[end] / 2).all() and torch.isfinite(v.to(dtype)).all()
+    assert dtype != torch.float16 or (1.75 * top == 57344 and off[0, 0] == 65504 - 49152)
+
+
 def test_ends_of_the_range():
     for dtype, big in ((torch.bfloat16, 3.3895e38), (torch.float16, 65504.0), (torch.float32, 3.4028e38)):
         x = torch.zeros(4, 32).to(dtype)
