@@ -2,9 +2,11 @@
  * k_paged.hip — rotary positions and the writes and reads of a paged cache. All three move
  * each element once and are bound by HBM for prompts and by launch latency for single tokens:
  * rotating 64 of 192 elements of 2001 tokens of 128 heads (66 MB) takes 13.9 us (4.8 TB/s, near a
- * large copy's 4.9), quantising 3 x 4093 rows into 8 bits (31 MB) 10 us, reading 8 x 4095 back (71 MB) 15 us
- * (4.7 TB/s), the rows of 32 single tokens 3.2 us, rotating 3 x 4093 tokens of 32 + 4 heads of 128 into
- * 16-bit pages (205 MB) 40 us (5.1 TB/s).
+ * large copy's 4.9). Rows of 4 heads of 128, keys and values: quantising three prompts of up to 4093 rows,
+ * 10012 in all, into 8 bits (31 MB) 10 us, reading eight sequences of up to 4095, 22927 in all, back (71 MB)
+ * 15 us (4.7 TB/s), the rows of 32 single tokens 3.2 us; with their rotation and 32 query heads' the three
+ * prompts into 16-bit pages (205 MB) 40 us (5.1 TB/s), into 8 and 4 bits (195 and 190 MB) 41 and 40; three latent
+ * prompts of 9819 rows and 16 query heads 15 us (63 MB), into 8 and 4 bits 17.
  */
 #include "hx_paged.h"
 
@@ -183,7 +185,8 @@ __global__ __launch_bounds__(ROPE_THREADS) void k_rope(RopeArgs a, int tok) {
  * is off by no more than half the step of the codes above 4; at the range's end (m above 1.75) the
  * code is cut to 3, off by up to the step to 4, 2^-2 of the value. e2m1 has no NaN, so a block that holds one, or an
  * infinity, gets the scale byte 255, which the conversions back turn into NaN. Looking at every element for these took
- * 12 us for 3 x 4093 rows of 4 heads of 128 into 4 bits, a look at the block's largest bits 9.1 (floor 6.3). */
+ * 12 us for the 10012 rows of three prompts, 4 heads of 128, into 4 bits (26 MB, 5.1 us at a large copy's rate), a look at
+ * the block's largest bits 9.1. */
 __device__ __forceinline__ bool fin(float x) { return __builtin_fabsf(x) < __builtin_huge_valf(); }
 
 /* over four neighbouring lanes */
@@ -194,9 +197,9 @@ __device__ __forceinline__ unsigned max_of4(unsigned m) {
 
 /* The eight elements that a thread of either kernel takes of each of its tokens: octs threads a
  * token (grid.z of them where that is more than a workgroup), several tokens a workgroup where it is
- * less; which piece, head and element they are is worked out once for COPY_TOKENS tokens (16 x 4093
- * rows of 4 heads of 128 into 8 bits: 37 us, one by one 44, eight at once 15% more than four on 3 x
- * 4093). The four tokens' page ids, then their rows, are under way together. */
+ * less; which piece, head and element they are is worked out once for COPY_TOKENS tokens (16 prompts of
+ * up to 4093 rows, 42348 in all, of 4 heads of 128 into 8 bits: 37 us, one by one 44; eight at once 15% more
+ * than four on three such prompts). The four tokens' page ids, then their rows, are under way together. */
 constexpr int COPY_TOKENS = 4;
 struct Place {
     const Piece *p;
