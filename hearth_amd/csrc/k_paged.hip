@@ -5,8 +5,8 @@
  * large copy's 4.9). Rows of 4 heads of 128, keys and values: quantising three prompts of up to 4093 rows,
  * 10012 in all, into 8 bits (31 MB) 10 us, reading eight sequences of up to 4095, 22927 in all, back (71 MB)
  * 15 us (4.7 TB/s), the rows of 32 single tokens 3.2 us; with their rotation and 32 query heads' the three
- * prompts into 16-bit pages (205 MB) 40 us (5.1 TB/s), into 8 and 4 bits (195 and 190 MB) 41 and 40; three latent
- * prompts of 9819 rows and 16 query heads 15 us (63 MB), into 8 and 4 bits 17.
+ * prompts into 16-bit pages (205 MB) 40 us (5.1 TB/s), three of 9819 rows into 8 and 4 bits (191 and 186 MB) 41
+ * and 40, 9819 latent rows with 16 query heads 15 us (63 MB), into 8 and 4 bits 17.
  */
 #include "hx_paged.h"
 

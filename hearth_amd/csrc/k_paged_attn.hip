@@ -10,14 +10,18 @@
  * a byte permutation a pair of elements.
  * It is bound by the cache's bytes: 268 MB of one token over 131071 rows in 49.7 us (5.4 TB/s), 178
  * MB of 32 tokens over 8-bit rows in 44 us (4.1 TB/s), the joins 5 us each. Nothing of the cache
- * goes through LDS (no row is read by two waves), V is under way before the scores and the next K
- * before the sums (32 tokens over 8-bit rows with each load where it is used: 114 us, not 48). Rows
- * of 4 bits (32 tokens, 92 MB: 24.7 us, 3.7 TB/s) are bound by their conversions and the exchanges
- * between lanes as much as by bytes: an instruction converts two codes a lane in 4.5 cycles, 72 for
- * 16 rows of 128, whose matrix products take 64.
+ * goes through LDS (no row is read by two waves) but the keys of blocks that many tokens choose (BY_LDS),
+ * V is under way before the scores and the next K before the sums (32 tokens over 8-bit rows with each
+ * load where it is used: 114 us, not 48). Rows of 4 bits: one token over 131071 rows, 71 MB in 17.3 us (4.1
+ * TB/s); 32 tokens up to 8192 rows, 92 MB in 25 us (3.7 TB/s), wait for the longest sequences: the split goes by
+ * the longest, so that 388 of 512 workgroups have rows, up to 2048 where an equal share is 1314. A wave takes 478
+ * vector instructions for 64 rows (138 of them conversions), 4 to 5 cycles each: 8 us of either if
+ * they were spread evenly.
  * Chosen blocks: 32 tokens over 32 blocks of 64 16-bit rows each 27.7 us (134 MB, 4.8 TB/s), 600
- * tokens over 16 blocks of 8-bit rows each 66.6 (from the chip's caches, 8 of a
- * tile's 16 columns in use for 8 heads a kv head; bound by the conversions, 24 M vector instructions).
+ * tokens over 16 blocks of 8-bit rows each 60 (from the chip's caches). The latter is bound by vector
+ * instructions, 22.5 M: 22000 a SIMD are 37 us at 4 cycles each. 5.2 M of them are conversions; the others
+ * are the softmax, for 16 columns of which 8 are in use with 8 heads a kv head, scale bytes taken out
+ * row by row, V's byte permutations, masks and addresses.
  *
  * Scores, maxima, sums of probabilities and of rows are float32. The probabilities alone are rounded
  * to the 16-bit type, in this kernel and the two for many rows: the matrix units take both factors in
@@ -255,8 +259,8 @@ struct Few {
  * lines that K's loads touch bound the kernel (a row of 16 lanes' loads at a time from as many rows;
  * by LDS whole rows): 600 tokens over 16 blocks of 64 rows each, by LDS and straight, 16-bit rows 66 and
  * 95 us, 8-bit 62 and 77; 4-bit, whose rows are a quarter of a line's, 61 and 57. Single tokens'
- * blocks come from memory, and straight is faster (32 of them over 32 blocks each, 16-bit rows: 29.5 and
- * 27.7 us). */
+ * blocks come from memory, where neither way is faster in general (32 of them over 32 blocks each, 16-bit
+ * rows: 29.5 and 27.7 us once, 31.3 and 31.2 in other calls; of width 256 61 and 60). */
 template <class T, int BITS, int D, bool BLOCKS, bool ONE, bool BY_LDS>
 __global__ __launch_bounds__(64 * FEW_WAVES, D <= 128 ? 2 : 1) void k_attend_few(AttendArgs a) {
     using F = Few<T, BITS, D>;
@@ -629,8 +633,11 @@ __global__ __launch_bounds__(JOIN_THREADS) void k_attend_join(AttendArgs a) {
     if (a.lse && e == 0) a.lse[row] = L == 0.0f ? NINF : (M + __log2f(L)) * 0.69314718055994531f;
 }
 
-/* Tokens of a sequence from which on K goes by LDS (see BY_LDS; one sequence, 16 blocks a token, by LDS
- * and straight: 1 to 8 tokens level, 16 10.3 and 11.4, 128 17.4 and 24.4 us) */
+/* Tokens of a sequence from which on K goes by LDS (see BY_LDS). By LDS and straight, us, 8 heads a kv head:
+ * one sequence, 16 blocks a token of width 128: 16 tokens 10.3 and 11.4, 128 17.4 and 24.4; 32 sequences, 32 blocks
+ * a token, 4, 8, 16 tokens each: 16-bit rows of width 64 28 / 29, 40 / 53, 67 / 93, of 128 55 / 56, 75 / 90, 119 /
+ * 164, of 256 107 / 111, 167 / 181, 299 / 337; 8-bit rows of 128 37 / 36, 63 / 65, 96 / 121. 8-bit rows of widths 64
+ * and 256 lose by it (24 / 23, 33 / 32, 56 / 55; 88 / 87, 159 / 157, 294 / 291), one sequence of them up to 6%. */
 constexpr int SHARING = 16;
 
 template <class T, int BITS, int D, bool BLOCKS>
@@ -667,8 +674,10 @@ void join_t(const AttendArgs &a, hipStream_t st) {
  * sequences of 4096 rows, width 128, few against many: 8-bit rows 42 and 51 us at 32 columns, 82
  * and 51 at 40; 16-bit ones 47 and 44 at 32, 111 and 46 at 48; of width 256 108 and 132 at 24. */
 static bool takes_many(int64_t cols) { return cols > 32; }
-/* of 4-bit rows, whose bytes are few: passes over the cache cost less than rows made 16 bits in LDS (27 and 46 us
- * at 32 columns, 35 and 49 at 64, 53 and 53 at 96; of width 256 118 and 149 at 96) */
+/* of 4-bit rows, whose bytes are few: passes over the cache cost less than rows made 16 bits in LDS. 32 sequences of
+ * 4096 rows, few and many, us at 32, 64, 96 and 128 columns: width 64 22 / 37, 31 / 39, 38 / 40, 48 / 41; 128 28 / 48,
+ * 38 / 50, 54 / 54, 70 / 59; 256 62 / 134, 92 / 141, 128 / 148, 168 / 154. One sequence of 32768 (128: 16 / 22, 20 / 25,
+ * 24 / 28, 28 / 30) and four of 2048 are faster by few at 128 columns too. */
 static bool takes_many4(int64_t cols) { return cols > 96; }
 
 /* Rows a split takes: enough workgroups for the 256 units, two each (one of the latent form, which fills a
