@@ -455,7 +455,9 @@ typedef struct hearth_gpu_blocks {
  * rows that exist (kv_len, max_kv): call it after the rows are written. Not for latent caches. A
  * row's element that is NaN or infinite counts as 0. The step is the least power of two with which
  * 127 steps reach the block's largest magnitude (scale 1 at least), codes round to nearest even.
- * Blocks on pages that are not in the cache are left alone. */
+ * Blocks on pages that are not in the cache are left alone. Two sequences of the call that share
+ * a page and both have tokens of theirs in a block of it have to have the same rows of it: one
+ * with fewer may leave bounds of those alone. */
 HEARTH_API int hearth_gpu_key_bounds(const hearth_gpu_cache *c, const hearth_gpu_batch *b, const hearth_gpu_bounds *s, int dev,
                                      void *stream);
 
