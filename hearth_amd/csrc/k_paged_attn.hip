@@ -14,9 +14,9 @@
  * V is under way before the scores and the next K before the sums (32 tokens over 8-bit rows with each
  * load where it is used: 114 us, not 48). Rows of 4 bits: one token over 131071 rows, 71 MB in 17.3 us (4.1
  * TB/s); 32 tokens up to 8192 rows, 92 MB in 25 us (3.7 TB/s), wait for the longest sequences: the split goes by
- * the longest, so that 388 of 512 workgroups have rows, up to 2048 where an equal share is 1314. A wave takes 478
- * vector instructions for 64 rows (138 of them conversions), 4 to 5 cycles each: 8 us of either if
- * they were spread evenly.
+ * the longest, so that 388 of 512 workgroups have rows, up to 2048 where an equal share is 1314. A wave takes
+ * about 500 vector instructions for 64 rows (139 of them conversions), four cycles each: 7 and 8 us of
+ * the two, spread evenly.
  * Chosen blocks: 32 tokens over 32 blocks of 64 16-bit rows each 27.7 us (134 MB, 4.8 TB/s), 600
  * tokens over 16 blocks of 8-bit rows each 60 (from the chip's caches). The latter is bound by vector
  * instructions, 22.5 M: 22000 a SIMD are 37 us at 4 cycles each. 5.2 M of them are conversions; the others
